@@ -1,0 +1,1007 @@
+// Softmax cross entropy of a language model's head on MI355X (gfx950), with its gradients, without the logits in
+// memory.
+//
+//   z[n, v] = h[n] . W[v] + b[v]        l[n] = log sum_v exp z[n, v] - z[n, t_n]
+//   dz[n, v] = g_n (exp(z[n, v]) / sum_u exp(z[n, u]) - [v = t_n])
+//   dh = dz W        dW = dz^T h        db[v] = sum_n dz[n, v]
+//
+// Rows whose target is the ignored index are taken out first (k_rows), so nothing they hold is read and they cost
+// nothing; their loss and their row of dh are zero. A target outside the vocabulary makes its row's loss NaN.
+//
+// The head's three products are 2 N V H operations each and run on the matrix cores (ews_tiles.h); they bound the
+// call for all but the smallest N. What is between them:
+//
+//   k_logits  a tile of z in registers; every wavefront takes the maximum m and the sum of exp(z - m) of its slab of
+//             the vocabulary for each of its rows. A training call also writes exp(z - m), for bfloat16 inputs as 16
+//             bits of (m - z) log2 e in steps of 2^-9: off by less than 2^-10.5 of exp(z - m) whatever its size, a
+//             fifth of what dz loses in bfloat16 afterwards (bfloat16 itself would lose as much again, and a logit
+//             rounded to it more than its probability).
+//   k_join    joins a row's slabs: the row's maximum M and sum, its loss.
+//   k_dz      dz = exp(z - m) exp(m - M) g / sum, in place and transposed; the target's entry from its own float32
+//             logit, so a target of probability near one loses nothing. The mean's factor stays out of it: most
+//             targets' entries are near -1, which bfloat16 holds, while their common factor's rounding would scale
+//             the whole gradient.
+//   k_grad    dh and dW, sums in float32. Few tiles are split over k and joined in order by k_reduce.
+//
+// It is kept for kChunkBytes of rows at a time; dW is summed over the chunks in float32. Nothing is added with
+// atomics: the same inputs give the same bits.
+//
+// Float32 inputs are multiplied as three bfloat16 planes (ews_tiles.h): float32's accuracy at the bfloat16 rate over
+// six, against one sixteenth for the float32 matrix instructions.
+#include <hip/hip_runtime.h>
+
+#include "ews_hip.h"
+#include "ews_tiles.h"
+#include "ews_vec.h"
+
+namespace ews {
+namespace loss {
+
+using namespace ews::vec;
+using namespace ews::tiles;
+
+typedef Tile<2, 4, 4, 2> Large;   // 256 x 256, eight wavefronts
+typedef Tile<2, 2, 2, 2> Medium;  // 128 x 128, four wavefronts
+typedef Tile<4, 1, 2, 1> Flat;    // 256 x 32, four wavefronts: few rows
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kSteps = 512.0f;    // 16-bit logarithms: steps to a factor of two; 65535 stands for a probability of 0
+
+struct Rows {
+  int* map;       // (N) the kept rows' places, in order
+  int* target;    // (N) their targets; -1 outside the vocabulary
+  int* kept;      // [0]: how many
+  float* scale;   // [0]: 1 / max(kept, 1) for the mean, 1 for the sum
+};
+
+struct Stats {
+  float2* slab;   // (slabs, chunk rows) maximum and sum of one wavefront's slab
+  float* zt;      // (N) the target's logit
+  float* top;     // (N) the row's maximum
+  float* inv;     // (N) one over its sum
+  float* loss;    // (N) the kept rows' losses
+};
+
+// ------------------------------------------------------------------------------------------------- rows and planes
+// One workgroup. A thread counts the kept ones of a stretch of rows, the counts are summed, the stretch is written.
+__global__ __launch_bounds__(1024) void k_rows(const int64_t* targets, int n, int vocab, int64_t ignore, int mean,
+                                               Rows r, float* loss_rows) {
+  __shared__ int wsum[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (n + 1023) / 1024;
+  const int lo = tid * each < n ? tid * each : n;
+  const int hi = lo + each < n ? lo + each : n;
+  int m = 0;
+  for (int i = lo; i < hi; ++i) m += targets[i] != ignore;
+  int at = m;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int up = __shfl_up(at, s);
+    if (lane >= s) at += up;
+  }
+  if (lane == 63) wsum[wave] = at;
+  at -= m;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) at += wsum[w];
+    total += wsum[w];
+  }
+  for (int i = lo; i < hi; ++i) {
+    const int64_t t = targets[i];
+    if (t != ignore) {
+      r.map[at] = i;
+      r.target[at++] = t >= 0 && t < vocab ? (int)t : -1;
+    } else if (loss_rows) {
+      loss_rows[i] = 0.0f;
+    }
+  }
+  if (tid == 0) {
+    r.kept[0] = total;
+    r.scale[0] = mean ? 1.0f / (float)(total > 0 ? total : 1) : 1.0f;
+  }
+}
+
+// The three bfloat16 planes of a float32 number, x = p0 + p1 + p2 exactly: each plane is the rest rounded to eight bits
+// (cut where rounding would reach infinity), so the second is at most 2^-8 and the third 2^-16 of x. An infinity or
+// NaN has nothing after its first plane.
+__device__ __forceinline__ float plane_value(uint16_t p) { return __uint_as_float((uint32_t)p << 16); }
+__device__ __forceinline__ void planes(float x, uint16_t (&p)[3]) {
+  const uint32_t u = __float_as_uint(x);
+  const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+  p[0] = round_bf16(x);
+  if (finite && (p[0] & 0x7f80u) == 0x7f80u) p[0] = (uint16_t)(u >> 16);
+  const float b = finite ? x - plane_value(p[0]) : 0.0f;
+  p[1] = round_bf16(b);
+  p[2] = round_bf16(b - plane_value(p[1]));
+}
+__device__ __forceinline__ void planes(bf16 x, uint16_t (&p)[1]) { p[0] = x.bits; }
+
+struct PackArgs {
+  const void* src;
+  int64_t stride;
+  int rows, cols;          // of the source (rows: kept[0] where there is a map)
+  const int* map;          // gathers the rows; null: all of them
+  const int* kept;
+  uint16_t* dst;           // planes (rows, ld), zero in further columns and in rows up to a multiple of 64; may be null
+  int64_t ld, plane;
+  int dst_rows;
+  uint16_t* turned;        // planes (cols, ldt), likewise; may be null
+  int64_t ldt, plane_t;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack(PackArgs a) {
+  constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+  __shared__ T tile[64][sizeof(T) == 4 ? 65 : 66];
+  const int rows = a.map ? a.kept[0] : a.rows;
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  if (r0 >= rows) return;
+  const int col = threadIdx.x & 63;
+  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
+    const int row = r0 + i;
+    T x = narrow<T>(0.0f);
+    if (row < rows && c0 + col < a.cols)
+      x = ((const T*)a.src)[(int64_t)(a.map ? a.map[row] : row) * a.stride + c0 + col];
+    tile[i][col] = x;
+    if (a.dst && row < a.dst_rows) {
+      uint16_t p[NP];
+      planes(x, p);
+#pragma unroll
+      for (int q = 0; q < NP; ++q) a.dst[q * a.plane + (int64_t)row * a.ld + c0 + col] = p[q];
+    }
+  }
+  if (!a.turned) return;
+  __syncthreads();
+  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
+    uint16_t p[NP];
+    planes(tile[col][i], p);
+#pragma unroll
+    for (int q = 0; q < NP; ++q) a.turned[q * a.plane_t + (int64_t)(c0 + i) * a.ldt + r0 + col] = p[q];
+  }
+}
+
+// The bias in float32, -inf past the vocabulary: those columns of a tile then have no weight in any row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_bias(const T* bias, int vocab, int padded, float* out) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v < padded) out[v] = v >= vocab ? -__builtin_inff() : (bias ? widen(bias[v]) : 0.0f);
+}
+
+// ------------------------------------------------------------------------------------------------------ the logits
+struct LogitArgs {
+  Operand W, X;
+  int ti, tj;             // tiles along the vocabulary and along the chunk's rows
+  int kblocks, pairs;
+  int c0, chunk;          // the chunk's first row, its rows
+  const float* bias;
+  Rows rows;
+  Stats st;
+  void* prob;             // exp(z - m) (chunk, ldp): a 16-bit logarithm, or float32 where there are three planes
+  int64_t ldp;
+};
+
+// KEEP: 0 the loss alone, 1 also 16-bit logarithms, 2 also float32 probabilities.
+template <class T, int KEEP>
+__global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
+  extern __shared__ char lds[];
+  int it, jt;
+  tile_of(blockIdx.x, a.ti, a.tj, it, jt);
+  const int i0 = it * T::I, j0 = jt * T::J;
+  const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
+  if (j0 >= live) return;
+  f32x16 acc[T::TI][T::TJ];
+  product<T>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, a.pairs, lds, acc);
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = wave % T::WI, wj = wave / T::WI;
+  const int r32 = lane & 31, half = lane >> 5;
+  const int ibase = i0 + wi * T::kSlab;
+  const float* bias = a.bias + ibase + half * 4;
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b) {
+    const int j = j0 + (wj * T::TJ + b) * 32 + r32;
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < T::TI; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 add = *reinterpret_cast<const f32x4*>(bias + t * 32 + g * 8);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float z = acc[t][b][4 * g + q] + add[q];
+          acc[t][b][4 * g + q] = z;
+          m = fmaxf(m, z);
+        }
+      }
+    m = fmaxf(m, __shfl_xor(m, 32));
+    // the target's logit, from the one lane that holds it
+    const int want = (j < live ? a.rows.target[a.c0 + j] : -1) - ibase;
+    const bool mine = want >= 0 && want < T::kSlab && ((want >> 2) & 1) == half;
+    if (__any(mine)) {
+      float zt = 0.0f;
+#pragma unroll
+      for (int t = 0; t < T::TI; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (t * 32 + 8 * (r / 4) + 4 * half + r % 4 == want) zt = acc[t][b][r];
+      if (mine) a.st.zt[a.c0 + j] = zt;
+    }
+    // z - m before the factor log2 e: neither a row of the type's lowest values nor one of -inf alone overflows
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int t = 0; t < T::TI; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float y = (acc[t][b][r] - ref) * kLog2e;
+        const float e = __builtin_amdgcn_exp2f(y);
+        acc[t][b][r] = KEEP == 1 ? fminf(y * -kSteps, 65535.0f) : e;
+        s += e;
+      }
+    s += __shfl_xor(s, 32);
+    if (half == 0 && j < live) a.st.slab[(int64_t)(it * T::WI + wi) * a.chunk + j] = make_float2(m, s);
+  }
+  if (KEEP) {
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < T::TJ; ++b)
+      rows_of<T>(lds, acc, b, [&](int jrow, int i, const float(&x)[8]) {
+        const int j = j0 + jrow;
+        if (j >= live || i0 + i >= a.ldp) return;
+        if (KEEP == 1) {
+          u32x4 w;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            w[q] = (uint32_t)(x[2 * q] + 0.5f) | ((uint32_t)(x[2 * q + 1] + 0.5f) << 16);
+          *reinterpret_cast<u32x4*>((uint16_t*)a.prob + j * a.ldp + i0 + i) = w;
+        } else {
+          float* p = (float*)a.prob + j * a.ldp + i0 + i;
+          Pack<float, 4> lo, hi;
+          lo.set(x);
+          hi.set(x + 4);
+          lo.store(p);
+          hi.store(p + 4);
+        }
+      });
+  }
+}
+
+// Maximum and sum of two parts of a row.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  const float ref = top == -__builtin_inff() ? 0.0f : top;
+  s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * kLog2e);
+  m = top;
+}
+
+// 64 rows a workgroup, sixteen wavefronts along the slabs.
+__global__ __launch_bounds__(1024) void k_join(Stats st, Rows rows, int slabs, int c0, int chunk, float* loss_rows) {
+  __shared__ float ms[16][64], ss[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int live = rows.kept[0] - c0 < chunk ? rows.kept[0] - c0 : chunk;
+  const int j = blockIdx.x * 64 + lane;
+  if (blockIdx.x * 64 >= live) return;
+  float m = -__builtin_inff(), s = 0.0f;
+  if (j < live) {
+#pragma unroll 4
+    for (int k = wave; k < slabs; k += 16) {
+      const float2 x = st.slab[(int64_t)k * chunk + j];
+      join(m, s, x.x, x.y);
+    }
+  }
+  ms[wave][lane] = m;
+  ss[wave][lane] = s;
+  __syncthreads();
+  if (wave || j >= live) return;
+  for (int w = 1; w < 16; ++w) join(m, s, ms[w][lane], ss[w][lane]);
+  const int row = c0 + j;
+  st.top[row] = m;
+  st.inv[row] = 1.0f / s;
+  const float l = rows.target[row] < 0 ? __builtin_nanf("") : logf(s) + (m - st.zt[row]);
+  st.loss[row] = l;
+  if (loss_rows) loss_rows[rows.map[row]] = l;
+}
+
+// The sum or mean of the kept rows' losses.
+__global__ __launch_bounds__(1024) void k_total(Stats st, Rows rows, float* out) {
+  __shared__ double part[16];
+  double s = 0.0;
+  const int n = rows.kept[0];
+  for (int i = threadIdx.x; i < n; i += 1024) s += (double)st.loss[i];
+#pragma unroll
+  for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0.0;
+  for (int w = 0; w < 16; ++w) s += part[w];
+  out[0] = (float)(s * (double)rows.scale[0]);
+}
+
+// ---------------------------------------------------------------------------------------------------------- dz
+struct DzArgs {
+  Rows rows;
+  Stats st;
+  const float* upstream;  // (N) or null: 1 (k_grad applies the reduction's factor)
+  int c0, chunk, slab, slabs;
+  void* prob;
+  int64_t ld;             // the vocabulary padded to a multiple of 64
+  uint16_t* dz;           // planes (chunk, ld): prob itself in bfloat16
+  int64_t plane;
+  uint16_t* turned;       // planes (ld, chunk)
+  int64_t plane_t;
+  float* bias;            // (ceil(chunk / 256), ld) sums over the rows; may be null
+};
+
+template <int NP>
+__global__ __launch_bounds__(256) void k_dz(DzArgs a) {
+  __shared__ float tile[64][65];
+  const int v0 = blockIdx.x * 64;
+  const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
+  const int padded = (live + 63) / 64 * 64;
+  const int slab = v0 / a.slab;
+  float sums[2] = {0.0f, 0.0f};
+  for (int r0 = blockIdx.y * 256; r0 < blockIdx.y * 256 + 256 && r0 < padded; r0 += 64) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int idx = threadIdx.x + 256 * c;
+      const int i = idx >> 3, v = v0 + (idx & 7) * 8, j = r0 + i;
+      float x[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = 0.0f;
+      if (j < live) {
+        const int row = a.c0 + j;
+        const int t = a.rows.target[row];
+        const float top = a.st.top[row], inv = a.st.inv[row];
+        const float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
+        const float m = a.st.slab[(int64_t)slab * a.chunk + j].x;
+        const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f((m - top) * kLog2e) * inv * g;
+        if (NP == 1) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)a.prob + j * a.ld + v);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t y = (w[q >> 1] >> (16 * (q & 1))) & 0xffffu;
+            x[q] = y == 65535u ? 0.0f * f : __builtin_amdgcn_exp2f((float)y * (-1.0f / kSteps)) * f;
+          }
+        } else {
+          Pack<float, 4> lo, hi;
+          lo.load((const float*)a.prob + j * a.ld + v);
+          hi.load((const float*)a.prob + j * a.ld + v + 4);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? lo.get(q) : hi.get(q - 4)) * f;
+        }
+        if (t >= v && t < v + 8) {
+          const float own = (__builtin_amdgcn_exp2f((a.st.zt[row] - top) * kLog2e) * inv - 1.0f) * g;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[q] = t == v + q ? own : x[q];
+        }
+      }
+      if (NP == 1) {
+        Pack<bf16, 8> p;
+        p.set(x);
+        if (j < live) p.store((bf16*)a.dz + j * a.ld + v);
+      } else if (j < live) {
+        uint16_t p[8][3];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) planes(x[q], p[q]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          u32x4 w;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[q] = (uint32_t)p[2 * q][k] | ((uint32_t)p[2 * q + 1][k] << 16);
+          *reinterpret_cast<u32x4*>(a.dz + k * a.plane + j * a.ld + v) = w;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) tile[i][(idx & 7) * 8 + q] = x[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int idx = threadIdx.x + 256 * c;
+      const int v = idx >> 3, i = (idx & 7) * 8;
+      float x[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        x[q] = tile[i + q][v];
+        sums[c] += x[q];
+      }
+      uint16_t* dst = a.turned + (int64_t)(v0 + v) * a.chunk + r0 + i;
+      if (NP == 1) {
+        Pack<bf16, 8> p;
+        p.set(x);
+        p.store((bf16*)dst);
+      } else {
+        uint16_t p[8][3];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) planes(x[q], p[q]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          u32x4 w;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[q] = (uint32_t)p[2 * q][k] | ((uint32_t)p[2 * q + 1][k] << 16);
+          *reinterpret_cast<u32x4*>(dst + k * a.plane_t) = w;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (!a.bias) return;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float s = sums[c];
+    s += __shfl_xor(s, 1);
+    s += __shfl_xor(s, 2);
+    s += __shfl_xor(s, 4);
+    const int idx = threadIdx.x + 256 * c;
+    if ((idx & 7) == 0) a.bias[(int64_t)blockIdx.y * a.ld + v0 + (idx >> 3)] = s;
+  }
+}
+
+// The bias's gradient: k_dz's sums over rows, added to those of the chunks before; the last chunk writes it.
+template <typename T>
+__global__ __launch_bounds__(256) void k_dbias(const float* part, int parts, int64_t ld, int vocab, float* sum,
+                                               int add, const float* factor, T* out) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= vocab) return;
+  float s = 0.0f;
+  for (int p = 0; p < parts; ++p) s += part[p * ld + v];
+  s = (factor ? s * factor[0] : s) + (add ? sum[v] : 0.0f);
+  if (out)
+    out[v] = narrow<T>(s);
+  else
+    sum[v] = s;
+}
+
+// ------------------------------------------------------------------------------------------------------ the gradients
+struct GradArgs {
+  Operand P, Q;
+  int ti, tj, splits;
+  int kblocks, per;       // k blocks, and those of one split
+  int pairs;
+  int by_rows;            // 1: k is the chunk's kept rows (dW); 0: the result's rows are (dh)
+  int c0, chunk;
+  Rows rows;
+  int I, J;               // the result's columns and (where by_rows) rows
+  float* part;            // (splits, J or chunk, I) where splits > 1
+  float* sum;             // float32 sums over the chunks, or null
+  int add;                // sum holds those of earlier chunks
+  void* out;              // the result, or null before the last chunk
+  int wide;               // the result's rows start at multiples of 16 bytes
+  const float* factor;    // of every result; null: 1
+};
+
+// Eight consecutive results of result row `row`, from column i on.
+template <typename T>
+__device__ __forceinline__ void finish(const GradArgs& a, int64_t row, int i, const float (&x)[8]) {
+  const int64_t at = row * a.I + i;
+  const int n = a.I - i < 8 ? a.I - i : 8;
+  const float f = a.factor ? a.factor[0] : 1.0f;
+  float y[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) y[q] = x[q] * f + (a.add && q < n ? a.sum[at + q] : 0.0f);
+  if (!a.out) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) a.sum[at + q] = y[q];
+  } else if (a.wide && n == 8) {
+#pragma unroll
+    for (int q = 0; q < 8; q += kWide<T>) {
+      Pack<T, kWide<T>> p;
+      p.set(y + q);
+      p.store((T*)a.out + at + q);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) ((T*)a.out)[at + q] = narrow<T>(y[q]);
+  }
+}
+
+template <class T, typename O>
+__global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
+  extern __shared__ char lds[];
+  const int split = blockIdx.y;
+  int it, jt;
+  tile_of(blockIdx.x, a.ti, a.tj, it, jt);
+  const int i0 = it * T::I, j0 = jt * T::J;
+  int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
+  live = live > 0 ? live : 0;
+  const int nj = a.by_rows ? a.J : live;
+  if (j0 >= nj) return;
+  int kb0 = split * a.per, kb1 = kb0 + a.per < a.kblocks ? kb0 + a.per : a.kblocks;
+  if (a.by_rows && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
+  f32x16 acc[T::TI][T::TJ];
+  product<T>(a.P, a.Q, i0, j0, kb0, kb1, a.pairs, lds, acc);
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b)
+    rows_of<T>(lds, acc, b, [&](int jrow, int icol, const float(&x)[8]) {
+      const int j = j0 + jrow, i = i0 + icol;
+      if (j >= nj || i >= a.I) return;
+      if (a.splits > 1) {
+        float* p = a.part + ((int64_t)split * (a.by_rows ? a.J : a.chunk) + j) * a.I + i;
+        const int n = a.I - i < 8 ? a.I - i : 8;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < n) p[q] = x[q];
+      } else {
+        finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], i, x);
+      }
+    });
+}
+
+template <typename O>
+__global__ __launch_bounds__(256) void k_reduce(GradArgs a) {
+  const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
+  const int nj = a.by_rows ? a.J : live;
+  const int rows = a.by_rows ? a.J : a.chunk;
+  const int packs = (a.I + 7) / 8;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t j = at / packs;
+  if (j >= nj) return;
+  const int i = (int)(at % packs) * 8;
+  const int n = a.I - i < 8 ? a.I - i : 8;
+  float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = a.part + ((int64_t)s * rows + j) * a.I + i;
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) x[q] += p[q];
+  }
+  finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], i, x);
+}
+
+// Zero rows of dh where the target is ignored.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ignored(const int64_t* targets, int n, int64_t ignore, T* grad, int H) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= n || targets[row] != ignore) return;
+  for (int c = threadIdx.x & 63; c < H; c += 64) grad[(int64_t)row * H + c] = narrow<T>(0.0f);
+}
+
+}  // namespace loss
+}  // namespace ews
+
+namespace {
+
+using namespace ews::loss;
+
+// Rows kept at a time: exp(z - m) and the transposed dz (float32: with their three planes) of as many as fit in this.
+constexpr int64_t kChunkBytes = (int64_t)2 << 30;
+constexpr int64_t kScoreRows = 65536;  // rows of a call without gradients whose slabs' sums are kept at a time
+constexpr int kFill = 512;  // workgroups that a product is split into along k where it has fewer tiles than CUs
+
+enum Kind { kLarge, kMedium, kFlat };
+
+struct Product {
+  Kind kind;
+  int ti, tj, slab, splits, per, kblocks;
+};
+
+struct LPlan {
+  int N, H, V, np, pairs;
+  int64_t Hp, Vp, Np, chunk;
+  int chunks, slabs, bias_pad;
+  bool train, packed;
+  Product logits, dh, dw;
+  size_t map, target, meta, zt, top, inv, loss, xp, xt, wp, wt, bias, slab, prob, dz, turned, dbias, dbsum, part, acc;
+  size_t total;
+};
+
+size_t al256x(size_t x) { return (x + 255) & ~(size_t)255; }
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// A product of I x J results: 256 x 32 tiles where J fits one; 256 x 256 ones where they fill the 256 CUs; else
+// 128 x 128 ones, of which a CU holds two.
+Product pick(int64_t I, int64_t J, int kblocks, bool split) {
+  Product p;
+  p.kblocks = kblocks;
+  if (J <= 32)
+    p.kind = kFlat;
+  else
+    p.kind = (int64_t)ceil_div(I, 256) * ceil_div(J, 256) >= 192 ? kLarge : kMedium;
+  const int ti = p.kind == kMedium ? 128 : 256;
+  const int tj = p.kind == kLarge ? 256 : p.kind == kMedium ? 128 : 32;
+  p.slab = p.kind == kLarge ? Large::kSlab : p.kind == kMedium ? Medium::kSlab : Flat::kSlab;
+  p.ti = ceil_div(I, ti);
+  p.tj = ceil_div(J, tj);
+  p.splits = 1;
+  p.per = kblocks;
+  const int64_t n = (int64_t)p.ti * p.tj;
+  if (split && n < 256 && kblocks >= 8) {
+    int z = (int)(kFill / n);
+    if (z > kblocks / 4) z = kblocks / 4;
+    if (z > 1) {
+      p.per = ceil_div(kblocks, z);
+      p.splits = ceil_div(kblocks, p.per);
+    }
+  }
+  return p;
+}
+
+int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
+  if (!s) return EWS_ERR_NULL;
+  if (s->dtype != EWS_DTYPE_F32 && s->dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
+  if (s->bias_dtype != EWS_DTYPE_F32 && s->bias_dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
+  if (s->reduction < 0 || s->reduction > 2) return EWS_ERR_OPTION;
+  if (s->rows < 1 || s->hidden < 1 || s->vocab < 1 || s->rows > 1 << 23 || s->hidden > 1 << 16 || s->vocab > 1 << 22)
+    return EWS_ERR_SHAPE;
+  if (s->hidden_stride < s->hidden || s->weight_stride < s->hidden) return EWS_ERR_SHAPE;
+  p.N = s->rows;
+  p.H = s->hidden;
+  p.V = s->vocab;
+  p.np = s->dtype == EWS_DTYPE_F32 ? 3 : 1;
+  p.pairs = p.np == 3 ? kPairs : 1;
+  p.train = train;
+  p.packed = !direct;
+  p.Hp = (int64_t)ceil_div(p.H, 64) * 64;
+  p.Vp = (int64_t)ceil_div(p.V, 64) * 64;
+  p.Np = (int64_t)ceil_div(p.N, 64) * 64;
+  const int64_t each = p.Vp * (p.np == 3 ? 16 : 4);
+  int64_t fit = train ? kChunkBytes / each / 256 * 256 : kScoreRows;
+  if (fit < 256) fit = 256;
+  p.chunk = p.Np < fit ? p.Np : fit;
+  p.chunks = ceil_div(p.Np, p.chunk);
+  p.logits = pick(p.V, p.chunk, (int)(p.Hp / 64), false);
+  p.dh = pick(p.H, p.chunk, (int)(p.Vp / 64), true);
+  p.dw = pick(p.H, p.V, (int)(p.chunk / 64), true);
+  const int tile_i = p.logits.kind == kMedium ? 128 : 256;
+  p.bias_pad = p.logits.ti * tile_i;
+  p.slabs = p.bias_pad / p.logits.slab;
+  size_t off = 0;
+  auto take = [&off](size_t bytes) {
+    const size_t at = off;
+    off += al256x(bytes);
+    return at;
+  };
+  p.map = take((size_t)p.N * 4);
+  p.target = take((size_t)p.N * 4);
+  p.meta = take(8);
+  p.zt = take((size_t)p.N * 4);
+  p.top = take((size_t)p.N * 4);
+  p.inv = take((size_t)p.N * 4);
+  p.loss = take((size_t)p.N * 4);
+  p.xp = take((size_t)(p.Np * p.Hp * p.np * 2));
+  p.wp = take(p.packed ? (size_t)(p.V * p.Hp * p.np * 2) : 0);
+  p.bias = take((size_t)p.bias_pad * 4);
+  p.slab = take((size_t)p.slabs * p.chunk * 8);
+  if (train) {
+    p.xt = take((size_t)(p.Np * p.Hp * p.np * 2));
+    p.wt = take((size_t)(p.Vp * p.Hp * p.np * 2));
+    p.prob = take((size_t)(p.chunk * p.Vp) * (p.np == 3 ? 4 : 2));
+    p.dz = p.np == 3 ? take((size_t)(p.chunk * p.Vp) * 6) : p.prob;
+    p.turned = take((size_t)(p.chunk * p.Vp) * p.np * 2);
+    p.dbias = take((size_t)(ceil_div(p.chunk, 256) * p.Vp) * 4);
+    p.dbsum = take((size_t)p.V * 4);
+    size_t part = 0;
+    if (p.dh.splits > 1) part = (size_t)p.dh.splits * p.chunk * p.H * 4;
+    if (p.dw.splits > 1 && (size_t)p.dw.splits * p.V * p.H * 4 > part) part = (size_t)p.dw.splits * p.V * p.H * 4;
+    p.part = take(part);
+    p.acc = take(p.chunks > 1 && s->dtype == EWS_DTYPE_BF16 ? (size_t)p.V * p.H * 4 : 0);
+  }
+  p.total = off;
+  return EWS_OK;
+}
+
+// bfloat16 weights whose rows start at multiples of 16 bytes and fill whole k blocks are read where they are.
+bool reads_direct(const ews_loss_desc* s, const void* weight) {
+  return s->dtype == EWS_DTYPE_BF16 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0 && (uintptr_t)weight % 16 == 0;
+}
+
+struct Call {
+  const ews_loss_desc* s;
+  LPlan p;
+  char* w;
+  hipStream_t st;
+  Rows rows;
+  Stats stats;
+};
+
+#define LOSS_CHECK()                                             \
+  do {                                                           \
+    if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH; \
+  } while (0)
+
+template <class K>
+int allow_lds(K kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                             bytes) == hipSuccess
+             ? EWS_OK
+             : EWS_ERR_LAUNCH;
+}
+
+template <class T, int KEEP>
+int launch_logits_as(const LogitArgs& a, hipStream_t st) {
+  const int rc = allow_lds(k_logits<T, KEEP>, T::kLdsBytes);
+  if (rc != EWS_OK) return rc;
+  hipLaunchKernelGGL((k_logits<T, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), T::kLdsBytes, st, a);
+  LOSS_CHECK();
+  return EWS_OK;
+}
+
+template <int KEEP>
+int launch_logits(Kind kind, const LogitArgs& a, hipStream_t st) {
+  if (kind == kLarge) return launch_logits_as<Large, KEEP>(a, st);
+  return kind == kMedium ? launch_logits_as<Medium, KEEP>(a, st) : launch_logits_as<Flat, KEEP>(a, st);
+}
+
+template <class T, typename O>
+int launch_grad_as(const GradArgs& a, hipStream_t st) {
+  const int rc = allow_lds(k_grad<T, O>, T::kLdsBytes);
+  if (rc != EWS_OK) return rc;
+  hipLaunchKernelGGL((k_grad<T, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
+  LOSS_CHECK();
+  if (a.splits > 1) {
+    const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * ((a.I + 7) / 8);
+    hipLaunchKernelGGL((k_reduce<O>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
+    LOSS_CHECK();
+  }
+  return EWS_OK;
+}
+
+template <typename O>
+int launch_grad(Kind kind, const GradArgs& a, hipStream_t st) {
+  if (kind == kLarge) return launch_grad_as<Large, O>(a, st);
+  return kind == kMedium ? launch_grad_as<Medium, O>(a, st) : launch_grad_as<Flat, O>(a, st);
+}
+
+template <typename T>
+int pack(const PackArgs& a, int64_t rows, int64_t cols, hipStream_t st) {
+  hipLaunchKernelGGL((k_pack<T>), dim3(ceil_div(rows, 64), ceil_div(cols, 64)), dim3(256), 0, st, a);
+  LOSS_CHECK();
+  return EWS_OK;
+}
+
+// What every call begins with: the kept rows, the operands' planes, the bias.
+int begin(Call& c, const void* hidden, const void* weight, const void* bias, const int64_t* targets, float* loss_rows,
+          bool turn_hidden, bool turn_weight) {
+  const LPlan& p = c.p;
+  const bool f32 = p.np == 3;
+  hipLaunchKernelGGL(k_rows, dim3(1), dim3(1024), 0, c.st, targets, p.N, p.V, c.s->ignore_index,
+                     c.s->reduction == EWS_LOSS_MEAN ? 1 : 0, c.rows, loss_rows);
+  LOSS_CHECK();
+  PackArgs x{};
+  x.src = hidden;
+  x.stride = c.s->hidden_stride;
+  x.rows = p.N;
+  x.cols = p.H;
+  x.map = c.rows.map;
+  x.kept = c.rows.kept;
+  x.dst = (uint16_t*)(c.w + p.xp);
+  x.ld = p.Hp;
+  x.plane = p.Np * p.Hp;
+  x.dst_rows = (int)p.Np;
+  if (turn_hidden) {
+    x.turned = (uint16_t*)(c.w + p.xt);
+    x.ldt = p.Np;
+    x.plane_t = p.Np * p.Hp;
+  }
+  int rc = f32 ? pack<float>(x, p.Np, p.Hp, c.st) : pack<bf16>(x, p.Np, p.Hp, c.st);
+  if (rc != EWS_OK) return rc;
+  if (p.packed || turn_weight) {
+    PackArgs w{};
+    w.src = weight;
+    w.stride = c.s->weight_stride;
+    w.rows = p.V;
+    w.cols = p.H;
+    if (p.packed) {
+      w.dst = (uint16_t*)(c.w + p.wp);
+      w.ld = p.Hp;
+      w.plane = p.V * p.Hp;
+      w.dst_rows = p.V;
+    }
+    if (turn_weight) {
+      w.turned = (uint16_t*)(c.w + p.wt);
+      w.ldt = p.Vp;
+      w.plane_t = p.Vp * p.Hp;
+    }
+    rc = f32 ? pack<float>(w, p.Vp, p.Hp, c.st) : pack<bf16>(w, p.Vp, p.Hp, c.st);
+    if (rc != EWS_OK) return rc;
+  }
+  float* b32 = (float*)(c.w + p.bias);
+  const int blocks = ceil_div(p.bias_pad, 256);
+  if (c.s->bias_dtype == EWS_DTYPE_BF16)
+    hipLaunchKernelGGL((k_bias<bf16>), dim3(blocks), dim3(256), 0, c.st, (const bf16*)bias, p.V, p.bias_pad, b32);
+  else
+    hipLaunchKernelGGL((k_bias<float>), dim3(blocks), dim3(256), 0, c.st, (const float*)bias, p.V, p.bias_pad, b32);
+  LOSS_CHECK();
+  return EWS_OK;
+}
+
+int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
+  const LPlan& p = c.p;
+  LogitArgs a{};
+  a.W.p = p.packed ? (const uint16_t*)(c.w + p.wp) : (const uint16_t*)weight;
+  a.W.ld = p.packed ? p.Hp : c.s->weight_stride;
+  a.W.plane = p.V * p.Hp;
+  a.W.rows = p.V;
+  a.X.p = (const uint16_t*)(c.w + p.xp);
+  a.X.ld = p.Hp;
+  a.X.plane = p.Np * p.Hp;
+  a.X.rows = (int)p.Np;
+  a.ti = p.logits.ti;
+  a.tj = p.logits.tj;
+  a.kblocks = p.logits.kblocks;
+  a.pairs = p.pairs;
+  a.c0 = (int)(chunk * p.chunk);
+  a.chunk = (int)p.chunk;
+  a.bias = (const float*)(c.w + p.bias);
+  a.rows = c.rows;
+  a.st = c.stats;
+  int rc;
+  if (p.train) {
+    a.prob = c.w + p.prob;
+    a.ldp = p.Vp;
+    rc = p.np == 3 ? launch_logits<2>(p.logits.kind, a, c.st) : launch_logits<1>(p.logits.kind, a, c.st);
+  } else {
+    rc = launch_logits<0>(p.logits.kind, a, c.st);
+  }
+  if (rc != EWS_OK) return rc;
+  hipLaunchKernelGGL(k_join, dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, a.c0, a.chunk,
+                     loss_rows);
+  LOSS_CHECK();
+  return EWS_OK;
+}
+
+Call make_call(const ews_loss_desc* s, const LPlan& p, void* workspace, ews_stream_t stream) {
+  Call c{};
+  c.s = s;
+  c.p = p;
+  c.w = (char*)workspace;
+  c.st = (hipStream_t)stream;
+  c.rows.map = (int*)(c.w + p.map);
+  c.rows.target = (int*)(c.w + p.target);
+  c.rows.kept = (int*)(c.w + p.meta);
+  c.rows.scale = (float*)(c.w + p.meta + 4);
+  c.stats.slab = (float2*)(c.w + p.slab);
+  c.stats.zt = (float*)(c.w + p.zt);
+  c.stats.top = (float*)(c.w + p.top);
+  c.stats.inv = (float*)(c.w + p.inv);
+  c.stats.loss = (float*)(c.w + p.loss);
+  return c;
+}
+
+int total_loss(const Call& c, float* loss) {
+  hipLaunchKernelGGL(k_total, dim3(1), dim3(1024), 0, c.st, c.stats, c.rows, loss);
+  LOSS_CHECK();
+  return EWS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train) {
+  LPlan p;
+  return loss_plan(desc, train != 0, false, p) == EWS_OK ? p.total : 0;
+}
+
+int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
+                     const int64_t* targets, float* loss, void* workspace, ews_stream_t stream) {
+  LPlan p;
+  int rc = loss_plan(desc, false, desc && reads_direct(desc, weight), p);
+  if (rc != EWS_OK) return rc;
+  if (!hidden || !weight || !targets || !loss || !workspace) return EWS_ERR_NULL;
+  Call c = make_call(desc, p, workspace, stream);
+  float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
+  rc = begin(c, hidden, weight, bias, targets, rows, false, false);
+  if (rc != EWS_OK) return rc;
+  for (int k = 0; k < p.chunks; ++k) {
+    rc = logits(c, weight, k, rows);
+    if (rc != EWS_OK) return rc;
+  }
+  return rows ? EWS_OK : total_loss(c, loss);
+}
+
+int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
+                   const int64_t* targets, const float* upstream, float* loss, void* grad_hidden, void* grad_weight,
+                   void* grad_bias, void* workspace, ews_stream_t stream) {
+  LPlan p;
+  int rc = loss_plan(desc, true, desc && reads_direct(desc, weight), p);
+  if (rc != EWS_OK) return rc;
+  if (!hidden || !weight || !targets || !workspace || (grad_bias && !bias)) return EWS_ERR_NULL;
+  Call c = make_call(desc, p, workspace, stream);
+  const bool f32 = p.np == 3;
+  float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
+  rc = begin(c, hidden, weight, bias, targets, rows, grad_weight != nullptr, grad_hidden != nullptr);
+  if (rc != EWS_OK) return rc;
+  if (grad_hidden) {
+    const int blocks = ceil_div(p.N, 4);
+    if (f32)
+      hipLaunchKernelGGL((k_ignored<float>), dim3(blocks), dim3(256), 0, c.st, targets, p.N, desc->ignore_index,
+                         (float*)grad_hidden, p.H);
+    else
+      hipLaunchKernelGGL((k_ignored<bf16>), dim3(blocks), dim3(256), 0, c.st, targets, p.N, desc->ignore_index,
+                         (bf16*)grad_hidden, p.H);
+    LOSS_CHECK();
+  }
+  const int wide = (p.H * (f32 ? 4 : 2)) % 16 == 0 && (uintptr_t)grad_hidden % 16 == 0 && (uintptr_t)grad_weight % 16 == 0;
+  const float* factor = upstream ? nullptr : c.rows.scale;
+  for (int k = 0; k < p.chunks; ++k) {
+    const bool last = k + 1 == p.chunks;
+    rc = logits(c, weight, k, rows);
+    if (rc != EWS_OK) return rc;
+    DzArgs z{};
+    z.rows = c.rows;
+    z.st = c.stats;
+    z.upstream = upstream;
+    z.c0 = (int)(k * p.chunk);
+    z.chunk = (int)p.chunk;
+    z.slab = p.logits.slab;
+    z.slabs = p.slabs;
+    z.prob = c.w + p.prob;
+    z.ld = p.Vp;
+    z.dz = (uint16_t*)(c.w + p.dz);
+    z.plane = p.chunk * p.Vp;
+    z.turned = (uint16_t*)(c.w + p.turned);
+    z.plane_t = p.chunk * p.Vp;
+    z.bias = grad_bias ? (float*)(c.w + p.dbias) : nullptr;
+    const dim3 grid((uint32_t)(p.Vp / 64), ceil_div(p.chunk, 256));
+    if (f32)
+      hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
+    else
+      hipLaunchKernelGGL((k_dz<1>), grid, dim3(256), 0, c.st, z);
+    LOSS_CHECK();
+    if (grad_bias) {
+      float* sum = (float*)(c.w + p.dbsum);
+      const dim3 g(ceil_div(p.V, 256));
+      if (desc->bias_dtype == EWS_DTYPE_BF16)
+        hipLaunchKernelGGL((k_dbias<bf16>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0, factor,
+                           last ? (bf16*)grad_bias : nullptr);
+      else
+        hipLaunchKernelGGL((k_dbias<float>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0, factor,
+                           last ? (float*)grad_bias : nullptr);
+      LOSS_CHECK();
+    }
+    GradArgs g{};
+    g.pairs = p.pairs;
+    g.c0 = z.c0;
+    g.chunk = z.chunk;
+    g.rows = c.rows;
+    g.wide = wide;
+    g.factor = factor;
+    g.part = (float*)(c.w + p.part);
+    if (grad_hidden) {
+      g.P = Operand{(const uint16_t*)(c.w + p.wt), p.Vp, p.Vp * p.Hp, (int)p.Hp};
+      g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk};
+      g.ti = p.dh.ti;
+      g.tj = p.dh.tj;
+      g.splits = p.dh.splits;
+      g.kblocks = p.dh.kblocks;
+      g.per = p.dh.per;
+      g.by_rows = 0;
+      g.I = p.H;
+      g.J = (int)p.chunk;
+      g.sum = nullptr;
+      g.add = 0;
+      g.out = grad_hidden;
+      rc = f32 ? launch_grad<float>(p.dh.kind, g, c.st) : launch_grad<bf16>(p.dh.kind, g, c.st);
+      if (rc != EWS_OK) return rc;
+    }
+    if (grad_weight) {
+      g.P = Operand{(const uint16_t*)(c.w + p.xt) + z.c0, p.Np, p.Np * p.Hp, (int)p.Hp};
+      g.Q = Operand{z.turned, p.chunk, z.plane_t, (int)p.Vp};
+      g.ti = p.dw.ti;
+      g.tj = p.dw.tj;
+      g.splits = p.dw.splits;
+      g.kblocks = p.dw.kblocks;
+      g.per = p.dw.per;
+      g.by_rows = 1;
+      g.I = p.H;
+      g.J = p.V;
+      g.sum = f32 ? (float*)grad_weight : (float*)(c.w + p.acc);
+      g.add = k > 0 ? 1 : 0;
+      g.out = last || f32 ? grad_weight : nullptr;
+      rc = f32 ? launch_grad<float>(p.dw.kind, g, c.st) : launch_grad<bf16>(p.dw.kind, g, c.st);
+      if (rc != EWS_OK) return rc;
+    }
+  }
+  if (!loss || rows) return EWS_OK;
+  return total_loss(c, loss);
+}
+
+}  // extern "C"

@@ -25,6 +25,9 @@ from .front import (  # noqa: F401
 )
 from .mixer import GradedRMSNorm, MixerEpilogue, graded_level_slices  # noqa: F401
 from .block import EWSBlock, RMSNorm, StackedEWS  # noqa: F401
+from .embed import embedding_lookup  # noqa: F401
+from .loss import linear_cross_entropy  # noqa: F401
+from .clip import clip_grad_norm_, clip_grads, global_grad_norm  # noqa: F401
 from .ops import diag_scan, mixer_epilogue  # noqa: F401
 from .token_scan import build_token_cache, token_cached_prefix_scan  # noqa: F401
 from .params import (  # noqa: F401

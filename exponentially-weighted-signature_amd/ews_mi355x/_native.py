@@ -90,6 +90,15 @@ EXPORTED = (
     "ews_diag_mixer_forward",
     "ews_diag_suited_chunk",
     "ews_diag_uses_chunk_kernels",
+    "ews_embed_forward",
+    "ews_embed_workspace_bytes",
+    "ews_embed_backward",
+    "ews_loss_workspace_bytes",
+    "ews_loss_forward",
+    "ews_loss_train",
+    "ews_clip_workspace_bytes",
+    "ews_clip",
+    "ews_scale",
 )
 
 JORDAN_KINDS = {"real": 0, "complex": 1}
@@ -100,6 +109,8 @@ CLOCK_SCALINGS = {"none": 0, "[0,1]": 1, "[-1,1]": 2, "steps": 3}
 LIFT_NONE = 0
 LIFT_FULL = 1
 LIFT_PRESERVE = 2
+
+LOSS_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 GRADED_VARIANTS = {"live_rms": 0, "static_gain": 1, "dilation": 2}
 
@@ -236,6 +247,33 @@ class LiftDesc(ctypes.Structure):
         ("increment", ctypes.c_int32),
         ("has_mask", ctypes.c_int32),
         ("basepoint", ctypes.c_int32),
+    ]
+
+
+class EmbedDesc(ctypes.Structure):
+    _fields_ = [
+        ("count", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("padding", ctypes.c_int64),
+        ("width", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("token_bytes", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class LossDesc(ctypes.Structure):
+    _fields_ = [
+        ("hidden_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
     ]
 
 
@@ -387,6 +425,26 @@ def load():
     lib.ews_token1_scan.restype = i32
     lib.ews_token1_scan_backward.argtypes = [t1p, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.ews_token1_scan_backward.restype = i32
+    edp = ctypes.POINTER(EmbedDesc)
+    lib.ews_embed_forward.argtypes = [edp, vp, vp, vp, vp]
+    lib.ews_embed_forward.restype = i32
+    lib.ews_embed_workspace_bytes.argtypes = [edp]
+    lib.ews_embed_workspace_bytes.restype = sz
+    lib.ews_embed_backward.argtypes = [edp, vp, vp, vp, vp, vp]
+    lib.ews_embed_backward.restype = i32
+    lsp = ctypes.POINTER(LossDesc)
+    lib.ews_loss_workspace_bytes.argtypes = [lsp, i32]
+    lib.ews_loss_workspace_bytes.restype = sz
+    lib.ews_loss_forward.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_loss_forward.restype = i32
+    lib.ews_loss_train.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_loss_train.restype = i32
+    lib.ews_clip_workspace_bytes.argtypes = [i32, vp]
+    lib.ews_clip_workspace_bytes.restype = sz
+    lib.ews_clip.argtypes = [i32, vp, vp, vp, vp, ctypes.c_float, i32, vp, vp, vp]
+    lib.ews_clip.restype = i32
+    lib.ews_scale.argtypes = [i32, vp, vp, vp, vp, vp, vp]
+    lib.ews_scale.restype = i32
     _lib = lib
     return lib
 

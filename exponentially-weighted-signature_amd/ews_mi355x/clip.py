@@ -1,0 +1,128 @@
+"""Gradient clipping by the global norm over many tensors (csrc/ews_clip.hip): the end of a training step (the
+reference's optax.clip_by_global_norm in its trainers' optimisers)."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native as nat
+from .embed import DTYPES, check_tensor, on_device
+
+
+def _dense(t):
+    """Whether t's elements fill one stretch of memory, each once, in whatever order."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _tables(tensors, outs):
+    n = len(tensors)
+    ptrs = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in tensors])
+    out = ptrs if outs is tensors else (ctypes.c_uint64 * n)(*[t.data_ptr() for t in outs])
+    counts = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
+    types = (ctypes.c_int32 * n)(*[DTYPES[t.dtype] for t in tensors])
+    return n, ptrs, out, counts, types
+
+
+def _check(tensors):
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise TypeError(f"gradients must be dense tensors, got layout {t.layout}")
+        check_tensor("every gradient", t)
+        if t.device != tensors[0].device:
+            raise ValueError(f"gradients are on {tensors[0].device} and {t.device}")
+
+
+def _norm_and_scale(tensors, outs, max_norm):
+    """The norm of tensors; where outs is not None, outs = the clipped tensors (outs is tensors: in place)."""
+    lib = nat.load()
+    dev = tensors[0].device
+    src = [t if _dense(t) else t.contiguous() for t in tensors]
+    dst = src
+    if outs is not None and outs is not tensors:
+        dst = [o if _dense(o) and o.stride() == s.stride() else torch.empty_like(s) for o, s in zip(outs, src)]
+    n, ptrs, out, counts, types = _tables(src, dst)
+    result = torch.empty(2, device=dev, dtype=torch.float32)
+    ws = torch.empty(int(lib.ews_clip_workspace_bytes(n, counts)), device=dev, dtype=torch.uint8)
+    with on_device(dev):
+        nat.check(lib.ews_clip(n, ptrs, out, counts, types, max_norm, 0 if outs is None else 1, result.data_ptr(),
+                               ws.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "ews_clip")
+    for o, d in zip(outs if outs is not None else (), dst):
+        if o is not d:
+            o.copy_(d)
+    return result[0]
+
+
+def scale_tensors(tensors, factor):
+    """tensors *= factor in place, factor a float32 number on the device; contiguous tensors, nothing for a 1."""
+    if not tensors:
+        return
+    dev = tensors[0].device
+    n, ptrs, out, counts, types = _tables(tensors, tensors)
+    with on_device(dev):
+        nat.check(nat.load().ews_scale(n, ptrs, out, counts, types, factor.data_ptr(),
+                                       torch.cuda.current_stream(dev).cuda_stream), "ews_scale")
+
+
+def _max_norm(max_norm):
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    return max_norm
+
+
+@torch.no_grad()
+def global_grad_norm(tensors):
+    """The square root of the sum of all squares over float32 and bfloat16 tensors of any shapes and strides on one HIP
+    device, a float32 number there; squares are added in float64. No tensors: 0 on the CPU."""
+    tensors = list(tensors)
+    if not tensors:
+        return torch.zeros(())
+    _check(tensors)
+    return _norm_and_scale(tensors, None, 0.0)
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, out=None):
+    """(norm, clipped): ``grads`` times ``min(1, max_norm / (norm + 1e-6))``, written to the tensors of ``out`` (same
+    shapes and types; a tensor of grads itself: in place; otherwise without overlap) or to new ones."""
+    grads = list(grads)
+    max_norm = _max_norm(max_norm)
+    if not grads:
+        return torch.zeros(()), []
+    _check(grads)
+    if out is None:
+        out = [torch.empty_like(t) for t in grads]
+    else:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"out has {len(out)} tensors for {len(grads)} gradients")
+        _check(out)
+        for g, o in zip(grads, out):
+            if g.shape != o.shape or g.dtype != o.dtype or g.device != o.device:
+                raise ValueError(f"out has {o.dtype} {tuple(o.shape)} on {o.device} for {g.dtype} {tuple(g.shape)} on "
+                                 f"{g.device}")
+    return _norm_and_scale(grads, out, max_norm), out
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """Scales the gradients of ``parameters`` (an iterable, or one) in place by ``min(1, max_norm / (norm + 1e-6))`` and
+    returns their norm, a float32 number on the device; the host does not wait. Parameters without a gradient are left
+    out. A norm that is not finite scales by 0 (infinite) or NaN, as the formula does."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [p.grad for p in parameters if p.grad is not None]
+    max_norm = _max_norm(max_norm)
+    if not grads:
+        return torch.zeros(())
+    _check(grads)
+    return _norm_and_scale(grads, grads, max_norm)

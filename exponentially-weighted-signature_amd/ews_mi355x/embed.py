@@ -1,0 +1,105 @@
+"""Embedding lookup with scaling, and its gradient by sorted tokens (csrc/ews_embed.hip): the token end of a
+``StackedEWS`` (the reference's eqx.nn.Embedding, ews/block.py:473-756)."""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as nat
+
+DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16}
+_NO_PADDING = -1
+
+
+def on_device(dev):
+    """A context in which launches go to dev (nothing where it is the current device)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def check_tensor(name, t):
+    if not t.is_cuda:
+        raise RuntimeError(f"ews_mi355x runs on a HIP device only: move {name} to the GPU (no CPU path)")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+
+
+def row_major(t):
+    """A 2-D tensor whose rows are contiguous and do not overlap (a copy only where they do), and its row stride."""
+    n, w = t.shape
+    if (t.stride(1) != 1 and w > 1) or (t.stride(0) < w and n > 1):
+        t = t.contiguous()
+    return t, (t.stride(0) if n > 1 else w)
+
+
+def _desc(tokens, weight, stride, scale, padding):
+    return nat.EmbedDesc(tokens.numel(), stride, padding, weight.shape[1], weight.shape[0], DTYPES[weight.dtype],
+                         tokens.element_size(), scale)
+
+
+def _stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _lookup(tokens, weight, scale, padding):
+    out = torch.empty((*tokens.shape, weight.shape[1]), device=weight.device, dtype=weight.dtype)
+    if tokens.numel() == 0:
+        return out
+    weight, stride = row_major(weight)
+    with on_device(weight.device):
+        nat.check(nat.load().ews_embed_forward(_desc(tokens, weight, stride, scale, padding), tokens.data_ptr(),
+                                               weight.data_ptr(), out.data_ptr(), _stream(weight.device)),
+                  "ews_embed_forward")
+    return out
+
+
+class _Lookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, tokens, scale, padding):
+        ctx.save_for_backward(tokens)
+        ctx.args = (weight.shape, weight.dtype, scale, padding)
+        return _lookup(tokens, weight, scale, padding)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        (tokens,) = ctx.saved_tensors
+        shape, dtype, scale, padding = ctx.args
+        grad = torch.empty(shape, device=gout.device, dtype=dtype)
+        if tokens.numel() == 0:
+            return grad.zero_(), None, None, None
+        lib = nat.load()
+        gout = gout.contiguous()
+        desc = _desc(tokens, grad, shape[1], scale, padding)
+        ws = torch.empty(int(lib.ews_embed_workspace_bytes(desc)), device=gout.device, dtype=torch.uint8)
+        with on_device(gout.device):
+            nat.check(lib.ews_embed_backward(desc, tokens.data_ptr(), gout.data_ptr(), grad.data_ptr(), ws.data_ptr(),
+                                             _stream(gout.device)), "ews_embed_backward")
+        return grad, None, None, None
+
+
+def embedding_lookup(tokens, weight, scale=1.0, padding_idx=None):
+    """``scale * weight[tokens]``: tokens of any shape (int64 or int32), weight (V, H) float32 or bfloat16 on the HIP
+    device -> (*tokens.shape, H) in weight's type. Differentiable in weight: a token's gradient rows are added in the
+    order of the tokens, in float32 and without atomics, so the same inputs give the same gradient bits; the rows of
+    ``padding_idx`` get none. A token outside [0, V) gives a row of NaN and has no gradient (the host does not wait to
+    look at the tokens)."""
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError(f"weight must be (V, H) with V, H >= 1, got {tuple(weight.shape)}")
+    check_tensor("weight", weight)
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"tokens must be int64 or int32, got {tokens.dtype}")
+    if tokens.device != weight.device:
+        raise ValueError(f"tokens are on {tokens.device}, weight on {weight.device}")
+    padding = _NO_PADDING
+    if padding_idx is not None:
+        padding = int(padding_idx) + (weight.shape[0] if padding_idx < 0 else 0)
+        if not 0 <= padding < weight.shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} is outside a vocabulary of {weight.shape[0]}")
+    tokens = tokens.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _Lookup.apply(weight, tokens, float(scale), padding)
+    return _lookup(tokens, weight, float(scale), padding)

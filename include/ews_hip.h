@@ -590,6 +590,76 @@ int ews_lift_backward(const ews_lift_desc* desc, const float* branch, const floa
                       const float* matrix, const void* residual, const float* grad_path, float* grad_branch,
                       float* grad_theta_app, float* grad_matrix, void* workspace, ews_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Around the blocks of a token model (the reference's StackedEWS, ews/block.py:473-756, with a training step's
+ * eqx.nn.Embedding, head with softmax cross entropy, and global-norm clipping): the operators at the two ends of a
+ * step. Their sums are float32 (norms float64) in a fixed order: the same inputs give the same bits.
+ * --------------------------------------------------------------------------------------------------------- */
+typedef struct ews_embed_desc {
+  int64_t count;         /* n: tokens, 1..2^25 */
+  int64_t weight_stride; /* elements between the table's rows, at least width */
+  int64_t padding;       /* a token whose rows have no gradient; outside [0, vocab): none */
+  int32_t width;         /* H: 1..2^20 */
+  int32_t vocab;         /* V: 1..2^25 */
+  int32_t dtype;         /* EWS_DTYPE_*: of weight, out and their gradients */
+  int32_t token_bytes;   /* 8 (int64) or 4 (int32) */
+  float scale;           /* s */
+} ews_embed_desc;
+
+/* out (n, H) = s weight[tokens]; a token outside [0, vocab) gives a row of NaN. */
+int ews_embed_forward(const ews_embed_desc* desc, const void* tokens, const void* weight, void* out,
+                      ews_stream_t stream);
+
+size_t ews_embed_workspace_bytes(const ews_embed_desc* desc);
+
+/* grad_weight (V, H), contiguous: s times the sum of grad_out's rows (contiguous) of every token, added in the
+ * tokens' order; zero where there are none. Tokens outside [0, vocab) are left out. */
+int ews_embed_backward(const ews_embed_desc* desc, const void* tokens, const void* grad_out, void* grad_weight,
+                       void* workspace, ews_stream_t stream);
+
+#define EWS_LOSS_NONE 0 /* loss (N): every row's own */
+#define EWS_LOSS_MEAN 1 /* loss (1): their sum over the number of rows that are not ignored (0 where all are) */
+#define EWS_LOSS_SUM 2  /* loss (1) */
+
+typedef struct ews_loss_desc {
+  int64_t hidden_stride; /* elements between rows of hidden, at least H */
+  int64_t weight_stride; /* elements between rows of weight, at least H */
+  int64_t ignore_index;  /* rows with this target have no loss and are not read */
+  int32_t rows;          /* N: 1..2^23 */
+  int32_t hidden;        /* H: 1..2^16 */
+  int32_t vocab;         /* V: 1..2^22 */
+  int32_t dtype;         /* EWS_DTYPE_*: of hidden, weight and their gradients */
+  int32_t bias_dtype;    /* EWS_DTYPE_*: of bias and its gradient */
+  int32_t reduction;     /* EWS_LOSS_* */
+} ews_loss_desc;
+
+/* Scratch of one call (train != 0: of ews_loss_train). It does not grow with N V: a training call keeps 2 GiB of
+ * probabilities and their transpose at most. */
+size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train);
+
+/* z = hidden weight^T + bias (bias may be NULL; entries of -inf take a token out of the vocabulary),
+ * loss_n = log sum_v exp z_nv - z_n,target. A target outside [0, vocab) that is not ignore_index: NaN. */
+int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
+                     const int64_t* targets, float* loss, void* workspace, ews_stream_t stream);
+
+/* The loss (may be NULL) and the gradients (contiguous; each may be NULL) of sum_n g_n loss_n in one pass: g_n is
+ * upstream[n], or where upstream is NULL the reduction's own factor (mean: 1 / kept rows; else 1). */
+int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
+                   const int64_t* targets, const float* upstream, float* loss, void* grad_hidden, void* grad_weight,
+                   void* grad_bias, void* workspace, ews_stream_t stream);
+
+/* Gradient clipping over n tensors, given by host arrays of device addresses, element counts (0 allowed) and
+ * EWS_DTYPE_*: result[0] = norm = sqrt(sum of all squares), result[1] = c = min(1, max_norm / (norm + 1e-6)) (NaN for
+ * a NaN norm). scale != 0: also out = c in for every tensor (out[i] == in[i]: in place; otherwise they may not
+ * overlap). The host arrays are read before the call returns. */
+size_t ews_clip_workspace_bytes(int n, const int64_t* counts);
+int ews_clip(int n, const uint64_t* in, const uint64_t* out, const int64_t* counts, const int32_t* dtypes,
+             float max_norm, int32_t scale, float* result, void* workspace, ews_stream_t stream);
+
+/* out = factor[0] in for every tensor, factor on the device; in place with a factor of 1 nothing is touched. */
+int ews_scale(int n, const uint64_t* in, const uint64_t* out, const int64_t* counts, const int32_t* dtypes,
+              const float* factor, ews_stream_t stream);
+
 /* Human-readable text of a return code. */
 const char* ews_error_string(int code);
 
