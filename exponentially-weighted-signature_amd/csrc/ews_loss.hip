@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void k_bias(const T* bias, int vocab, int padd
 struct LogitArgs {
   Operand W, X;
   int ti, tj;             // tiles along the vocabulary and along the chunk's rows
-  int kblocks, pairs;
+  int kblocks;
   int c0, chunk;          // the chunk's first row, its rows
   const float* bias;
   Rows rows;
@@ -183,7 +183,7 @@ struct LogitArgs {
 };
 
 // KEEP: 0 the loss alone, 1 also 16-bit logarithms, 2 also float32 probabilities.
-template <class T, int KEEP>
+template <class T, int PAIRS, int KEEP>
 __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
   extern __shared__ char lds[];
   int it, jt;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   if (j0 >= live) return;
   f32x16 acc[T::TI][T::TJ];
-  product<T>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, a.pairs, lds, acc);
+  product<T, PAIRS>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, lds, acc);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave % T::WI, wj = wave / T::WI;
@@ -244,7 +244,6 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
     if (half == 0 && j < live) a.st.slab[(int64_t)(it * T::WI + wi) * a.chunk + j] = make_float2(m, s);
   }
   if (KEEP) {
-    __syncthreads();
 #pragma unroll
     for (int b = 0; b < T::TJ; ++b)
       rows_of<T>(lds, acc, b, [&](int jrow, int i, const float(&x)[8]) {
@@ -460,7 +459,6 @@ struct GradArgs {
   Operand P, Q;
   int ti, tj, splits;
   int kblocks, per;       // k blocks, and those of one split
-  int pairs;
   int by_rows;            // 1: k is the chunk's kept rows (dW); 0: the result's rows are (dh)
   int c0, chunk;
   Rows rows;
@@ -500,7 +498,7 @@ __device__ __forceinline__ void finish(const GradArgs& a, int64_t row, int i, co
   }
 }
 
-template <class T, typename O>
+template <class T, int PAIRS, typename O>
 __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
   extern __shared__ char lds[];
   const int split = blockIdx.y;
@@ -514,8 +512,7 @@ __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
   int kb0 = split * a.per, kb1 = kb0 + a.per < a.kblocks ? kb0 + a.per : a.kblocks;
   if (a.by_rows && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
   f32x16 acc[T::TI][T::TJ];
-  product<T>(a.P, a.Q, i0, j0, kb0, kb1, a.pairs, lds, acc);
-  __syncthreads();
+  product<T, PAIRS>(a.P, a.Q, i0, j0, kb0, kb1, lds, acc);
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b)
     rows_of<T>(lds, acc, b, [&](int jrow, int icol, const float(&x)[8]) {
@@ -582,7 +579,7 @@ struct Product {
 };
 
 struct LPlan {
-  int N, H, V, np, pairs;
+  int N, H, V, np;
   int64_t Hp, Vp, Np, chunk;
   int chunks, slabs, bias_pad;
   bool train, packed;
@@ -628,14 +625,13 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   if (s->dtype != EWS_DTYPE_F32 && s->dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
   if (s->bias_dtype != EWS_DTYPE_F32 && s->bias_dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
   if (s->reduction < 0 || s->reduction > 2) return EWS_ERR_OPTION;
-  if (s->rows < 1 || s->hidden < 1 || s->vocab < 1 || s->rows > 1 << 23 || s->hidden > 1 << 16 || s->vocab > 1 << 22)
+  if (s->rows < 1 || s->hidden < 1 || s->vocab < 1 || s->rows > 1 << 22 || s->hidden > 1 << 16 || s->vocab > 1 << 22)
     return EWS_ERR_SHAPE;
   if (s->hidden_stride < s->hidden || s->weight_stride < s->hidden) return EWS_ERR_SHAPE;
   p.N = s->rows;
   p.H = s->hidden;
   p.V = s->vocab;
   p.np = s->dtype == EWS_DTYPE_F32 ? 3 : 1;
-  p.pairs = p.np == 3 ? kPairs : 1;
   p.train = train;
   p.packed = !direct;
   p.Hp = (int64_t)ceil_div(p.H, 64) * 64;
@@ -646,8 +642,9 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   if (fit < 256) fit = 256;
   p.chunk = p.Np < fit ? p.Np : fit;
   p.chunks = ceil_div(p.Np, p.chunk);
-  p.logits = pick(p.V, p.chunk, (int)(p.Hp / 64), false);
-  p.dh = pick(p.H, p.chunk, (int)(p.Vp / 64), true);
+  const int64_t most = p.chunk < p.N ? p.chunk : p.N;  // rows of a chunk
+  p.logits = pick(p.V, most, (int)(p.Hp / 64), false);
+  p.dh = pick(p.H, most, (int)(p.Vp / 64), true);
   p.dw = pick(p.H, p.V, (int)(p.chunk / 64), true);
   const int tile_i = p.logits.kind == kMedium ? 128 : 256;
   p.bias_pad = p.logits.ti * tile_i;
@@ -714,26 +711,27 @@ int allow_lds(K kernel, int bytes) {
              : EWS_ERR_LAUNCH;
 }
 
-template <class T, int KEEP>
+template <class T, int PAIRS, int KEEP>
 int launch_logits_as(const LogitArgs& a, hipStream_t st) {
-  const int rc = allow_lds(k_logits<T, KEEP>, T::kLdsBytes);
+  const int rc = allow_lds(k_logits<T, PAIRS, KEEP>, T::kLdsBytes);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_logits<T, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), T::kLdsBytes, st, a);
+  hipLaunchKernelGGL((k_logits<T, PAIRS, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), T::kLdsBytes, st, a);
   LOSS_CHECK();
   return EWS_OK;
 }
 
-template <int KEEP>
+template <int PAIRS, int KEEP>
 int launch_logits(Kind kind, const LogitArgs& a, hipStream_t st) {
-  if (kind == kLarge) return launch_logits_as<Large, KEEP>(a, st);
-  return kind == kMedium ? launch_logits_as<Medium, KEEP>(a, st) : launch_logits_as<Flat, KEEP>(a, st);
+  if (kind == kLarge) return launch_logits_as<Large, PAIRS, KEEP>(a, st);
+  return kind == kMedium ? launch_logits_as<Medium, PAIRS, KEEP>(a, st) : launch_logits_as<Flat, PAIRS, KEEP>(a, st);
 }
 
 template <class T, typename O>
 int launch_grad_as(const GradArgs& a, hipStream_t st) {
-  const int rc = allow_lds(k_grad<T, O>, T::kLdsBytes);
+  constexpr int kP = sizeof(O) == 4 ? kPairs : 1;  // float32 gradients are those of float32 operands
+  const int rc = allow_lds(k_grad<T, kP, O>, T::kLdsBytes);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_grad<T, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
+  hipLaunchKernelGGL((k_grad<T, kP, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
   LOSS_CHECK();
   if (a.splits > 1) {
     const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * ((a.I + 7) / 8);
@@ -826,7 +824,6 @@ int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
   a.ti = p.logits.ti;
   a.tj = p.logits.tj;
   a.kblocks = p.logits.kblocks;
-  a.pairs = p.pairs;
   a.c0 = (int)(chunk * p.chunk);
   a.chunk = (int)p.chunk;
   a.bias = (const float*)(c.w + p.bias);
@@ -836,9 +833,9 @@ int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
   if (p.train) {
     a.prob = c.w + p.prob;
     a.ldp = p.Vp;
-    rc = p.np == 3 ? launch_logits<2>(p.logits.kind, a, c.st) : launch_logits<1>(p.logits.kind, a, c.st);
+    rc = p.np == 3 ? launch_logits<kPairs, 2>(p.logits.kind, a, c.st) : launch_logits<1, 1>(p.logits.kind, a, c.st);
   } else {
-    rc = launch_logits<0>(p.logits.kind, a, c.st);
+    rc = p.np == 3 ? launch_logits<kPairs, 0>(p.logits.kind, a, c.st) : launch_logits<1, 0>(p.logits.kind, a, c.st);
   }
   if (rc != EWS_OK) return rc;
   hipLaunchKernelGGL(k_join, dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, a.c0, a.chunk,
@@ -958,7 +955,6 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
       LOSS_CHECK();
     }
     GradArgs g{};
-    g.pairs = p.pairs;
     g.c0 = z.c0;
     g.chunk = z.chunk;
     g.rows = c.rows;

@@ -8,8 +8,13 @@
 // j = l % 32, i = 8 (r / 4) + 4 (l / 32) + r % 4 of register r). P is the instruction's first operand so that a lane
 // holds four consecutive i of one j: the contiguous direction of every result written here.
 //
-// k runs in blocks of 64. A block's rows lie in LDS as eight 16-byte pieces, piece c of row r at c ^ (r % 8): rows are
-// 128 bytes apart, so eight rows that read the same k read eight different groups of banks.
+// k runs in blocks of 64, two stages of 32. A stage's rows (64 bytes each) are copied straight from global memory to LDS
+// (buffer loads to LDS: no registers, no instructions to store them) into a ring of four, three stages ahead of the
+// products, so a copy has the time of three stages' products to arrive. One barrier a stage: a wavefront waits until
+// its own copies of the stage have arrived (the eight or so younger ones go on), the barrier says that everyone's have
+// and that nobody reads the stage before any more, whose place the next copies take.
+// The 16-byte piece c of row r lies at c ^ (r / 2 ^ r / 8) % 4, so that the sixteen rows that read the same k at a time
+// spread over all banks.
 //
 // Float32 operands come as three bfloat16 planes (x = x0 + x1 + x2 exactly, |x1| <= 2^-8 |x|, |x2| <= 2^-16 |x|) and are
 // multiplied as six products, the smallest first: the three left out are at most 2^-23 of x w, 2^-26 or so at random.
@@ -42,39 +47,64 @@ struct Tile {
   static constexpr int kSlab = 32 * TI;                    // consecutive i of one wavefront
   static constexpr int kRowWords = kSlab + 4;              // a staged result row, padded off the banks
   static constexpr int kStageBytes = WI * WJ * 32 * kRowWords * 4;
-  static constexpr int kLoadBytes = (I + J) * 128;
-  static constexpr int kLdsBytes = kStageBytes > kLoadBytes ? kStageBytes : kLoadBytes;
+  static constexpr int kCopiesP = I * 4 / kThreads;        // 16-byte pieces a thread copies in a stage
+  static constexpr int kCopiesQ = J * 4 > kThreads ? J * 4 / kThreads : 1;
+  static constexpr int kBytesP = kCopiesP * kThreads * 16;
+  static constexpr int kStage = (kCopiesP + kCopiesQ) * kThreads * 16;
+  static constexpr int kLdsBytes = kStageBytes > 4 * kStage ? kStageBytes : 4 * kStage;
 };
 
 constexpr int kPairs = 6;
 __device__ __forceinline__ int piece_p(int pair) { return (0x001102 >> (4 * pair)) & 15; }  // 2 0 1 1 0 0
 __device__ __forceinline__ int piece_q(int pair) { return (0x010120 >> (4 * pair)) & 15; }  // 0 2 1 0 1 0
 
-// One operand's rows of a k block, global memory to registers and on to LDS.
-template <int ROWS, int THREADS>
-struct Loader {
-  static constexpr int kEach = ROWS * 8 / THREADS;
-  u32x4 r[kEach];
-  __device__ __forceinline__ void fetch(const Operand& o, int piece, int row0, int64_t k) {
+__device__ __forceinline__ int place(int row, int piece) { return piece ^ (((row >> 1) ^ (row >> 3)) & 3); }
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+// One operand's rows of a tile: what each thread copies, and the copies of a stage.
+template <int COPIES, int THREADS>
+struct Copier {
+  const uint16_t* base;
+  int64_t plane;
+  int offset[COPIES];   // bytes from the tile's first row; at most 256 rows of 2^22 numbers apart
+  __device__ __forceinline__ Copier(const Operand& o, int row0) {
+    row0 = row0 < o.rows ? row0 : o.rows - 1;
+    base = o.p + row0 * o.ld;
+    plane = o.plane;
 #pragma unroll
-    for (int c = 0; c < kEach; ++c) {
+    for (int c = 0; c < COPIES; ++c) {
       const int idx = threadIdx.x + c * THREADS;
-      const int row = idx >> 3, pos = idx & 7;
-      const int src = row0 + row < o.rows ? row0 + row : o.rows - 1;
-      r[c] = *reinterpret_cast<const u32x4*>(o.p + piece * o.plane + src * o.ld + k + 8 * (pos ^ (row & 7)));
+      const int row = idx >> 2;
+      const int src = row0 + row < o.rows ? row : o.rows - 1 - row0;
+      offset[c] = (int)((uint32_t)src * (uint32_t)(o.ld * 2) + 16 * place(row, idx & 3));
     }
   }
-  __device__ __forceinline__ void put(char* lds) const {
+  // k32: the stage's first k in units of 32
+  __device__ __forceinline__ void copy(char* lds, int piece, int k32) const {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass does not know the buffer builtins
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + piece * plane + (int64_t)k32 * 32), 0, -1,
+                                                        0x00020000);
+    char* to = lds + (threadIdx.x >> 6) * 1024;
 #pragma unroll
-    for (int c = 0; c < kEach; ++c) *reinterpret_cast<u32x4*>(lds + (threadIdx.x + c * THREADS) * 16) = r[c];
+    for (int c = 0; c < COPIES; ++c)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + c * THREADS * 16), 16, offset[c], 0, 0, 0);
+#endif
   }
 };
 
-// The results of the workgroup's tile at (i0, j0) over k blocks [kb0, kb1); pairs: 1, or kPairs for three planes.
-template <class T>
+// Waits until no more than N of this wavefront's loads are on their way and its LDS reads are done, then for everyone.
+template <int N>
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// The results of the workgroup's tile at (i0, j0) over k blocks [kb0, kb1); PAIRS: 1, or kPairs for three planes. On
+// return LDS is free.
+template <class T, int PAIRS>
 __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
-                                        int pairs, char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+                                        char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave % T::WI, wj = wave / T::WI;
 #pragma unroll
   for (int a = 0; a < T::TI; ++a)
@@ -83,47 +113,48 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
   if (kb0 >= kb1) return;
-  char* ldsP = lds;
-  char* ldsQ = lds + T::I * 128;
-  Loader<T::I, T::kThreads> lp;
-  Loader<T::J, T::kThreads> lq;
-  const int steps = (kb1 - kb0) * pairs;
-  auto fetch = [&](int s) {
-    const int pair = pairs == 1 ? kPairs - 1 : s % pairs;
-    const int64_t k = (int64_t)(kb0 + s / pairs) * 64;
-    lp.fetch(P, piece_p(pair), i0, k);
-    lq.fetch(Q, piece_q(pair), j0, k);
+  const Copier<T::kCopiesP, T::kThreads> cp(P, i0);
+  const Copier<T::kCopiesQ, T::kThreads> cq(Q, j0);
+  const int stages = (kb1 - kb0) * PAIRS * 2;
+  // past the last stage the copies repeat it, into places that nobody reads again: every wait counts the same
+  auto copy = [&](int s) {
+    char* to = lds + (s & 3) * T::kStage;
+    const int t = s < stages ? s : stages - 1;
+    const int pair = PAIRS == 1 ? kPairs - 1 : (t >> 1) % PAIRS;
+    const int k32 = (kb0 + (t >> 1) / PAIRS) * 2 + (t & 1);
+    cp.copy(to, piece_p(pair), k32);
+    cq.copy(to + T::kBytesP, piece_q(pair), k32);
   };
-  fetch(0);
-  lp.put(ldsP);
-  lq.put(ldsQ);
-  __syncthreads();
+  copy(0);
+  copy(1);
+  copy(2);
   const int r32 = lane & 31, half = lane >> 5;
-  const char* rowP = ldsP + (wi * T::TI * 32 + r32) * 128;
-  const char* rowQ = ldsQ + (wj * T::TJ * 32 + r32) * 128;
-  for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) fetch(s + 1);
+  const int atP = (wi * T::TI * 32 + r32) * 64, atQ = T::kBytesP + (wj * T::TJ * 32 + r32) * 64;
+  const int at0 = place(r32, half) * 16, at1 = place(r32, 2 + half) * 16;
+  for (int s = 0; s < stages; s += 2) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const int off = ((ks * 2 + half) ^ (r32 & 7)) * 16;
-      bf16x8 fp[T::TI], fq[T::TJ];
+    for (int u = 0; u < 2; ++u) {
+      arrive<2 * (T::kCopiesP + T::kCopiesQ)>();
+      copy(s + u + 3);
+      const char* stage = lds + ((s & 2) + u) * T::kStage;
 #pragma unroll
-      for (int a = 0; a < T::TI; ++a) fp[a] = *reinterpret_cast<const bf16x8*>(rowP + a * 32 * 128 + off);
+      for (int ks = 0; ks < 2; ++ks) {
+        bf16x8 fp[T::TI], fq[T::TJ];
 #pragma unroll
-      for (int b = 0; b < T::TJ; ++b) fq[b] = *reinterpret_cast<const bf16x8*>(rowQ + b * 32 * 128 + off);
-#pragma unroll
-      for (int a = 0; a < T::TI; ++a)
+        for (int a = 0; a < T::TI; ++a)
+          fp[a] = *reinterpret_cast<const bf16x8*>(stage + atP + a * 2048 + (ks ? at1 : at0));
 #pragma unroll
         for (int b = 0; b < T::TJ; ++b)
-          acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp[a], fq[b], acc[a][b], 0, 0, 0);
-    }
-    __syncthreads();
-    if (s + 1 < steps) {
-      lp.put(ldsP);
-      lq.put(ldsQ);
-      __syncthreads();
+          fq[b] = *reinterpret_cast<const bf16x8*>(stage + atQ + b * 2048 + (ks ? at1 : at0));
+#pragma unroll
+        for (int a = 0; a < T::TI; ++a)
+#pragma unroll
+          for (int b = 0; b < T::TJ; ++b)
+            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp[a], fq[b], acc[a][b], 0, 0, 0);
+      }
     }
   }
+  arrive<0>();
 }
 
 // Tile coordinates of a workgroup. Consecutive workgroups go to the eight XCDs in turn; each XCD gets a contiguous

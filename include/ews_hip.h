@@ -625,7 +625,7 @@ typedef struct ews_loss_desc {
   int64_t hidden_stride; /* elements between rows of hidden, at least H */
   int64_t weight_stride; /* elements between rows of weight, at least H */
   int64_t ignore_index;  /* rows with this target have no loss and are not read */
-  int32_t rows;          /* N: 1..2^23 */
+  int32_t rows;          /* N: 1..2^22 */
   int32_t hidden;        /* H: 1..2^16 */
   int32_t vocab;         /* V: 1..2^22 */
   int32_t dtype;         /* EWS_DTYPE_*: of hidden, weight and their gradients */

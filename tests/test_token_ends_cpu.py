@@ -63,7 +63,7 @@ def test_loss_error_codes():
     assert lib.ews_loss_forward(_loss(), *nulls) == -1
     assert lib.ews_loss_train(_loss(), *nulls, *[NULL] * 4) == -1
     for bad, code in ((dict(rows=0), -2), (dict(hidden=0), -2), (dict(vocab=0), -2), (dict(hidden_stride=63), -2),
-                      (dict(weight_stride=63), -2), (dict(vocab=2**22 + 1), -2), (dict(rows=2**23 + 1), -2),
+                      (dict(weight_stride=63), -2), (dict(vocab=2**22 + 1), -2), (dict(rows=2**22 + 1), -2),
                       (dict(hidden=2**16 + 1, hidden_stride=2**17, weight_stride=2**17), -2), (dict(dtype=3), -4),
                       (dict(bias_dtype=-1), -4), (dict(reduction=3), -4)):
         assert lib.ews_loss_forward(_loss(**bad), *nulls) == code, bad
