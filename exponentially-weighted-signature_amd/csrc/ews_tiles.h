@@ -10,11 +10,12 @@
 //
 // k runs in blocks of 64, two stages of 32. A stage's rows (64 bytes each) are copied straight from global memory to LDS
 // (buffer loads to LDS: no registers, no instructions to store them) into a ring of four, three stages ahead of the
-// products, so a copy has the time of three stages' products to arrive. One barrier a stage: a wavefront waits until
-// its own copies of the stage have arrived (the eight or so younger ones go on), the barrier says that everyone's have
-// and that nobody reads the stage before any more, whose place the next copies take.
-// The 16-byte piece c of row r lies at c ^ (r / 2 ^ r / 8) % 4, so that the sixteen rows that read the same k at a time
-// spread over all banks.
+// products. One barrier a stage: a wavefront waits until its own copies of the next stage have arrived (the younger ones
+// go on); the barrier says that everyone's have, and that nobody reads the stage before any more, whose place the next
+// copies take. Operands are read sixteen k ahead of their products, across the barrier, so the products go on after it
+// at once; reads and copies go out one by one between products that do not wait for them.
+// The 16-byte piece c of row r lies at c ^ (r / 4) % 4. A 16-byte read serves lanes {0-3, 12-15, 20-27}, then {4-11,
+// 16-19, 28-31}, and so the other half: the rows of each such sixteen lie in sixteen different groups of four banks.
 //
 // Float32 operands come as three bfloat16 planes (x = x0 + x1 + x2 exactly, |x1| <= 2^-8 |x|, |x2| <= 2^-16 |x|) and are
 // multiplied as six products, the smallest first: the three left out are at most 2^-23 of x w, 2^-26 or so at random.
@@ -58,7 +59,7 @@ constexpr int kPairs = 6;
 __device__ __forceinline__ int piece_p(int pair) { return (0x001102 >> (4 * pair)) & 15; }  // 2 0 1 1 0 0
 __device__ __forceinline__ int piece_q(int pair) { return (0x010120 >> (4 * pair)) & 15; }  // 0 2 1 0 1 0
 
-__device__ __forceinline__ int place(int row, int piece) { return piece ^ (((row >> 1) ^ (row >> 3)) & 3); }
+__device__ __forceinline__ int place(int row, int piece) { return piece ^ ((row >> 2) & 3); }
 
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -80,15 +81,15 @@ struct Copier {
       offset[c] = (int)((uint32_t)src * (uint32_t)(o.ld * 2) + 16 * place(row, idx & 3));
     }
   }
-  // k32: the stage's first k in units of 32
-  __device__ __forceinline__ void copy(char* lds, int piece, int k32) const {
+  // The address of a stage's rows; k32: its first k in units of 32.
+  __device__ __forceinline__ const uint16_t* at(int piece, int k32) const {
+    return base + piece * plane + (int64_t)k32 * 32;
+  }
+  // One of the copies; `to`: this wavefront's kilobyte of the stage.
+  __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host's pass does not know the buffer builtins
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + piece * plane + (int64_t)k32 * 32), 0, -1,
-                                                        0x00020000);
-    char* to = lds + (threadIdx.x >> 6) * 1024;
-#pragma unroll
-    for (int c = 0; c < COPIES; ++c)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + c * THREADS * 16), 16, offset[c], 0, 0, 0);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, -1, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + c * THREADS * 16), 16, offset[c], 0, 0, 0);
 #endif
   }
 };
@@ -96,7 +97,9 @@ struct Copier {
 // Waits until no more than N of this wavefront's loads are on their way and its LDS reads are done, then for everyone.
 template <int N>
 __device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // The results of the workgroup's tile at (i0, j0) over k blocks [kb0, kb1); PAIRS: 1, or kPairs for three planes. On
@@ -116,42 +119,68 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
   const Copier<T::kCopiesP, T::kThreads> cp(P, i0);
   const Copier<T::kCopiesQ, T::kThreads> cq(Q, j0);
   const int stages = (kb1 - kb0) * PAIRS * 2;
+  constexpr int kCopies = T::kCopiesP + T::kCopiesQ, kReads = T::TI + T::TJ, kProducts = T::TI * T::TJ;
   // past the last stage the copies repeat it, into places that nobody reads again: every wait counts the same
-  auto copy = [&](int s) {
-    char* to = lds + (s & 3) * T::kStage;
+  const uint16_t *fromP, *fromQ;
+  char* to;
+  auto aim = [&](int s) {
     const int t = s < stages ? s : stages - 1;
     const int pair = PAIRS == 1 ? kPairs - 1 : (t >> 1) % PAIRS;
     const int k32 = (kb0 + (t >> 1) / PAIRS) * 2 + (t & 1);
-    cp.copy(to, piece_p(pair), k32);
-    cq.copy(to + T::kBytesP, piece_q(pair), k32);
+    fromP = cp.at(piece_p(pair), k32);
+    fromQ = cq.at(piece_q(pair), k32);
+    to = lds + (s & 3) * T::kStage + wave * 1024;
   };
-  copy(0);
-  copy(1);
-  copy(2);
+  auto copy = [&](int c) {
+    if (c < T::kCopiesP)
+      cp.copy(c, fromP, to);
+    else
+      cq.copy(c - T::kCopiesP, fromQ, to + T::kBytesP);
+  };
   const int r32 = lane & 31, half = lane >> 5;
   const int atP = (wi * T::TI * 32 + r32) * 64, atQ = T::kBytesP + (wj * T::TJ * 32 + r32) * 64;
-  const int at0 = place(r32, half) * 16, at1 = place(r32, 2 + half) * 16;
+  const int at[2] = {place(r32, half) * 16, place(r32, 2 + half) * 16};
+  struct Rows32 {
+    bf16x8 p[T::TI], q[T::TJ];
+  } even, odd;  // the first and the second sixteen k of a stage
+  // the n-th of a sixteen's reads: the first product's two rows of blocks first
+  auto read = [&](Rows32& f, int s, int ks, int n) {
+    const char* stage = lds + (s & 3) * T::kStage + at[ks];
+    if (n >= 1 && n <= T::TJ)
+      f.q[n - 1] = *reinterpret_cast<const bf16x8*>(stage + atQ + (n - 1) * 2048);
+    else
+      f.p[n ? n - T::TJ : 0] = *reinterpret_cast<const bf16x8*>(stage + atP + (n ? n - T::TJ : 0) * 2048);
+  };
+  constexpr int kSlots = kReads > kProducts ? (kReads > kCopies ? kReads : kCopies) : (kProducts > kCopies ? kProducts : kCopies);
+  // the products of one sixteen k, and between them the reads of the next and this stage's copies
+  auto multiply = [&](const Rows32& f, Rows32& next, int s, int ks, bool copies) {
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      if (i < kReads) read(next, s, ks, i);
+      if (copies && i < kCopies) copy(i);
+      if (i < kProducts) {
+        const int a = i / T::TJ, b = i % T::TJ;
+        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.p[a], f.q[b], acc[a][b], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0x6);  // scalar and vector arithmetic may move past
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < 3; ++s) {
+    aim(s);
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) copy(c);
+  }
+  arrive<2 * kCopies>();
+#pragma unroll
+  for (int n = 0; n < kReads; ++n) read(even, 0, 0, n);
   for (int s = 0; s < stages; s += 2) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      arrive<2 * (T::kCopiesP + T::kCopiesQ)>();
-      copy(s + u + 3);
-      const char* stage = lds + ((s & 2) + u) * T::kStage;
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        bf16x8 fp[T::TI], fq[T::TJ];
-#pragma unroll
-        for (int a = 0; a < T::TI; ++a)
-          fp[a] = *reinterpret_cast<const bf16x8*>(stage + atP + a * 2048 + (ks ? at1 : at0));
-#pragma unroll
-        for (int b = 0; b < T::TJ; ++b)
-          fq[b] = *reinterpret_cast<const bf16x8*>(stage + atQ + b * 2048 + (ks ? at1 : at0));
-#pragma unroll
-        for (int a = 0; a < T::TI; ++a)
-#pragma unroll
-          for (int b = 0; b < T::TJ; ++b)
-            acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp[a], fq[b], acc[a][b], 0, 0, 0);
-      }
+      arrive<kCopies>();
+      aim(s + u + 3);
+      multiply(even, odd, s + u, 1, true);
+      multiply(odd, even, s + u + 1, 0, false);
     }
   }
   arrive<0>();
