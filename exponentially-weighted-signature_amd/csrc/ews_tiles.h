@@ -8,13 +8,13 @@
 // j = l % 32, i = 8 (r / 4) + 4 (l / 32) + r % 4 of register r). P is the instruction's first operand so that a lane
 // holds four consecutive i of one j: the contiguous direction of every result written here.
 //
-// k runs in blocks of 64, two stages of 32. A stage's rows (64 bytes each) are copied straight from global memory to LDS
-// (buffer loads to LDS: no registers, no instructions to store them) into a ring of four, three stages ahead of the
-// products. One barrier a stage: a wavefront waits until its own copies of the next stage have arrived (the younger ones
-// go on); the barrier says that everyone's have, and that nobody reads the stage before any more, whose place the next
-// copies take. Operands are read sixteen k ahead of their products, across the barrier, so the products go on after it
-// at once; reads and copies go out one by one between products that do not wait for them.
-// The 16-byte piece c of row r lies at c ^ (r / 4) % 4. A 16-byte read serves lanes {0-3, 12-15, 20-27}, then {4-11,
+// k runs in stages of 64. A stage's rows (128 bytes each: whole cache lines) are copied straight from global memory to
+// LDS (buffer loads to LDS: no registers, no instructions to store them) into one half of the tile's LDS while the other
+// half is multiplied. Operands are read sixteen k ahead of their products, so when a stage's last sixteen are in
+// registers its half is free: there is the stage's one barrier. Before it a wavefront waits until its own copies of the
+// next stage have arrived; after it the products go on at once, and the copies of the stage after the next begin.
+// Reads and copies go out one by one between products that do not wait for them.
+// The 16-byte piece c of row r lies at c ^ (r / 2) % 8. A 16-byte read serves lanes {0-3, 12-15, 20-27}, then {4-11,
 // 16-19, 28-31}, and so the other half: the rows of each such sixteen lie in sixteen different groups of four banks.
 //
 // Float32 operands come as three bfloat16 planes (x = x0 + x1 + x2 exactly, |x1| <= 2^-8 |x|, |x2| <= 2^-16 |x|) and are
@@ -48,18 +48,18 @@ struct Tile {
   static constexpr int kSlab = 32 * TI;                    // consecutive i of one wavefront
   static constexpr int kRowWords = kSlab + 4;              // a staged result row, padded off the banks
   static constexpr int kStageBytes = WI * WJ * 32 * kRowWords * 4;
-  static constexpr int kCopiesP = I * 4 / kThreads;        // 16-byte pieces a thread copies in a stage
-  static constexpr int kCopiesQ = J * 4 > kThreads ? J * 4 / kThreads : 1;
+  static constexpr int kCopiesP = I * 8 / kThreads;        // 16-byte pieces a thread copies in a stage
+  static constexpr int kCopiesQ = J * 8 / kThreads;
   static constexpr int kBytesP = kCopiesP * kThreads * 16;
   static constexpr int kStage = (kCopiesP + kCopiesQ) * kThreads * 16;
-  static constexpr int kLdsBytes = kStageBytes > 4 * kStage ? kStageBytes : 4 * kStage;
+  static constexpr int kLdsBytes = kStageBytes > 2 * kStage ? kStageBytes : 2 * kStage;
 };
 
 constexpr int kPairs = 6;
 __device__ __forceinline__ int piece_p(int pair) { return (0x001102 >> (4 * pair)) & 15; }  // 2 0 1 1 0 0
 __device__ __forceinline__ int piece_q(int pair) { return (0x010120 >> (4 * pair)) & 15; }  // 0 2 1 0 1 0
 
-__device__ __forceinline__ int place(int row, int piece) { return piece ^ ((row >> 2) & 3); }
+__device__ __forceinline__ int place(int row, int piece) { return piece ^ ((row >> 1) & 7); }
 
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -76,14 +76,14 @@ struct Copier {
 #pragma unroll
     for (int c = 0; c < COPIES; ++c) {
       const int idx = threadIdx.x + c * THREADS;
-      const int row = idx >> 2;
+      const int row = idx >> 3;
       const int src = row0 + row < o.rows ? row : o.rows - 1 - row0;
-      offset[c] = (int)((uint32_t)src * (uint32_t)(o.ld * 2) + 16 * place(row, idx & 3));
+      offset[c] = (int)((uint32_t)src * (uint32_t)(o.ld * 2) + 16 * place(row, idx & 7));
     }
   }
-  // The address of a stage's rows; k32: its first k in units of 32.
-  __device__ __forceinline__ const uint16_t* at(int piece, int k32) const {
-    return base + piece * plane + (int64_t)k32 * 32;
+  // The address of the rows of k block kb.
+  __device__ __forceinline__ const uint16_t* at(int piece, int kb) const {
+    return base + piece * plane + (int64_t)kb * 64;
   }
   // One of the copies; `to`: this wavefront's kilobyte of the stage.
   __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const {
@@ -118,18 +118,18 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
   if (kb0 >= kb1) return;
   const Copier<T::kCopiesP, T::kThreads> cp(P, i0);
   const Copier<T::kCopiesQ, T::kThreads> cq(Q, j0);
-  const int stages = (kb1 - kb0) * PAIRS * 2;
+  const int stages = (kb1 - kb0) * PAIRS;
   constexpr int kCopies = T::kCopiesP + T::kCopiesQ, kReads = T::TI + T::TJ, kProducts = T::TI * T::TJ;
-  // past the last stage the copies repeat it, into places that nobody reads again: every wait counts the same
+  constexpr int kMost = kReads > kProducts ? kReads : kProducts, kSlots = kMost > kCopies ? kMost : kCopies;
+  // past the last stage the copies repeat it, into a half that nobody reads again
   const uint16_t *fromP, *fromQ;
   char* to;
   auto aim = [&](int s) {
     const int t = s < stages ? s : stages - 1;
-    const int pair = PAIRS == 1 ? kPairs - 1 : (t >> 1) % PAIRS;
-    const int k32 = (kb0 + (t >> 1) / PAIRS) * 2 + (t & 1);
-    fromP = cp.at(piece_p(pair), k32);
-    fromQ = cq.at(piece_q(pair), k32);
-    to = lds + (s & 3) * T::kStage + wave * 1024;
+    const int pair = PAIRS == 1 ? kPairs - 1 : t % PAIRS;
+    fromP = cp.at(piece_p(pair), kb0 + t / PAIRS);
+    fromQ = cq.at(piece_q(pair), kb0 + t / PAIRS);
+    to = lds + (s & 1) * T::kStage + wave * 1024;
   };
   auto copy = [&](int c) {
     if (c < T::kCopiesP)
@@ -138,25 +138,26 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
       cq.copy(c - T::kCopiesP, fromQ, to + T::kBytesP);
   };
   const int r32 = lane & 31, half = lane >> 5;
-  const int atP = (wi * T::TI * 32 + r32) * 64, atQ = T::kBytesP + (wj * T::TJ * 32 + r32) * 64;
-  const int at[2] = {place(r32, half) * 16, place(r32, 2 + half) * 16};
-  struct Rows32 {
+  const int atP = (wi * T::TI * 32 + r32) * 128, atQ = T::kBytesP + (wj * T::TJ * 32 + r32) * 128;
+  int at[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) at[k] = place(r32, 2 * k + half) * 16;
+  struct Sixteen {
     bf16x8 p[T::TI], q[T::TJ];
-  } even, odd;  // the first and the second sixteen k of a stage
-  // the n-th of a sixteen's reads: the first product's two rows of blocks first
-  auto read = [&](Rows32& f, int s, int ks, int n) {
-    const char* stage = lds + (s & 3) * T::kStage + at[ks];
+  } even, odd;
+  // the n-th of a sixteen's reads: the first product's two first
+  auto read = [&](Sixteen& f, int s, int k, int n) {
+    const char* stage = lds + (s & 1) * T::kStage + at[k];
     if (n >= 1 && n <= T::TJ)
-      f.q[n - 1] = *reinterpret_cast<const bf16x8*>(stage + atQ + (n - 1) * 2048);
+      f.q[n - 1] = *reinterpret_cast<const bf16x8*>(stage + atQ + (n - 1) * 4096);
     else
-      f.p[n ? n - T::TJ : 0] = *reinterpret_cast<const bf16x8*>(stage + atP + (n ? n - T::TJ : 0) * 2048);
+      f.p[n ? n - T::TJ : 0] = *reinterpret_cast<const bf16x8*>(stage + atP + (n ? n - T::TJ : 0) * 4096);
   };
-  constexpr int kSlots = kReads > kProducts ? (kReads > kCopies ? kReads : kCopies) : (kProducts > kCopies ? kProducts : kCopies);
-  // the products of one sixteen k, and between them the reads of the next and this stage's copies
-  auto multiply = [&](const Rows32& f, Rows32& next, int s, int ks, bool copies) {
+  // the products of one sixteen, and between them the reads of sixteen k of stage s and where asked its successor's copies
+  auto multiply = [&](const Sixteen& f, Sixteen& next, int s, int k, bool copies) {
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      if (i < kReads) read(next, s, ks, i);
+      if (i < kReads) read(next, s, k, i);
       if (copies && i < kCopies) copy(i);
       if (i < kProducts) {
         const int a = i / T::TJ, b = i % T::TJ;
@@ -165,24 +166,27 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
       __builtin_amdgcn_sched_barrier(0x6);  // scalar and vector arithmetic may move past
     }
   };
+  aim(0);
 #pragma unroll
-  for (int s = 0; s < 3; ++s) {
-    aim(s);
+  for (int c = 0; c < kCopies; ++c) copy(c);
+  const bf16x8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c) copy(c);
+  for (int a = 0; a < T::TI; ++a) odd.p[a] = zero;
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b) odd.q[b] = zero;
+  for (int s = 0; s < stages; ++s) {
+    arrive<0>();
+    aim(s + 1);
+    multiply(odd, even, s, 0, true);  // the stage before's last sixteen (at first nothing)
+    multiply(even, odd, s, 1, false);
+    multiply(odd, even, s, 2, false);
+    multiply(even, odd, s, 3, false);
   }
-  arrive<2 * kCopies>();
 #pragma unroll
-  for (int n = 0; n < kReads; ++n) read(even, 0, 0, n);
-  for (int s = 0; s < stages; s += 2) {
+  for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      arrive<kCopies>();
-      aim(s + u + 3);
-      multiply(even, odd, s + u, 1, true);
-      multiply(odd, even, s + u + 1, 0, false);
-    }
-  }
+    for (int b = 0; b < T::TJ; ++b)
+      acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(odd.p[a], odd.q[b], acc[a][b], 0, 0, 0);
   arrive<0>();
 }
 
