@@ -45,6 +45,7 @@ typedef Tile<2, 2, 2, 2> Medium;  // 128 x 128, four wavefronts
 typedef Tile<4, 1, 2, 1> Flat;    // 256 x 32, four wavefronts: few rows
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
 constexpr float kSteps = 512.0f;    // 16-bit logarithms: steps to a factor of two; 65535 stands for a probability of 0
 
 struct Rows {
@@ -54,8 +55,9 @@ struct Rows {
   float* scale;   // [0]: 1 / max(kept, 1) for the mean, 1 for the sum
 };
 
+// Logits are kept in units of a factor of two: z log2 e.
 struct Stats {
-  float2* slab;   // (slabs, chunk rows) maximum and sum of one wavefront's slab
+  float2* slab;   // (slabs, chunk rows) maximum and sum of 2^(z - maximum) of one wavefront's slab
   float* zt;      // (N) the target's logit
   float* top;     // (N) the row's maximum
   float* inv;     // (N) one over its sum
@@ -162,11 +164,19 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   }
 }
 
-// The bias in float32, -inf past the vocabulary: those columns of a tile then have no weight in any row.
+// The bias in float32 times log2 e, -inf past the vocabulary: those columns of a tile then have no weight in any row. A
+// finite bias stays finite (a mask of the type's lowest value is not -inf: a row of nothing else is uniform).
 template <typename T>
 __global__ __launch_bounds__(256) void k_bias(const T* bias, int vocab, int padded, float* out) {
   const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v < padded) out[v] = v >= vocab ? -__builtin_inff() : (bias ? widen(bias[v]) : 0.0f);
+  if (v >= padded) return;
+  float b = -__builtin_inff();
+  if (v < vocab) {
+    const float x = bias ? widen(bias[v]) : 0.0f;
+    b = x * kLog2e;
+    if (__builtin_isinf(b) && !__builtin_isinf(x)) b = copysignf(3.402823466e+38f, x);
+  }
+  out[v] = b;
 }
 
 // ------------------------------------------------------------------------------------------------------ the logits
@@ -210,7 +220,7 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
         const f32x4 add = *reinterpret_cast<const f32x4*>(bias + t * 32 + g * 8);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float z = acc[t][b][4 * g + q] + add[q];
+          const float z = fmaf(acc[t][b][4 * g + q], kLog2e, add[q]);
           acc[t][b][4 * g + q] = z;
           m = fmaxf(m, z);
         }
@@ -228,42 +238,32 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
           if (t * 32 + 8 * (r / 4) + 4 * half + r % 4 == want) zt = acc[t][b][r];
       if (mine) a.st.zt[a.c0 + j] = zt;
     }
-    // z - m before the factor log2 e: neither a row of the type's lowest values nor one of -inf alone overflows
-    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    const float ref = m == -__builtin_inff() ? 0.0f : m;  // a slab of -inf alone has the sum 0
+    const float shift = ref * kSteps + 0.5f;
     float s = 0.0f;
 #pragma unroll
     for (int t = 0; t < T::TI; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float y = (acc[t][b][r] - ref) * kLog2e;
-        const float e = __builtin_amdgcn_exp2f(y);
-        acc[t][b][r] = KEEP == 1 ? fminf(y * -kSteps, 65535.0f) : e;
+        const float z = acc[t][b][r];
+        const float e = __builtin_amdgcn_exp2f(z - ref);
         s += e;
+        if (KEEP == 1) acc[t][b][r] = fminf(fmaf(z, -kSteps, shift), 65535.0f);
+        if (KEEP == 2) acc[t][b][r] = e;
       }
     s += __shfl_xor(s, 32);
     if (half == 0 && j < live) a.st.slab[(int64_t)(it * T::WI + wi) * a.chunk + j] = make_float2(m, s);
-  }
-  if (KEEP) {
-#pragma unroll
-    for (int b = 0; b < T::TJ; ++b)
-      rows_of<T>(lds, acc, b, [&](int jrow, int i, const float(&x)[8]) {
+    if (KEEP == 1) {
+      rows_of<T, uint16_t>(lds, acc, b, [&](int jrow, int i, const u32x4& w) {
         const int j = j0 + jrow;
-        if (j >= live || i0 + i >= a.ldp) return;
-        if (KEEP == 1) {
-          u32x4 w;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            w[q] = (uint32_t)(x[2 * q] + 0.5f) | ((uint32_t)(x[2 * q + 1] + 0.5f) << 16);
-          *reinterpret_cast<u32x4*>((uint16_t*)a.prob + j * a.ldp + i0 + i) = w;
-        } else {
-          float* p = (float*)a.prob + j * a.ldp + i0 + i;
-          Pack<float, 4> lo, hi;
-          lo.set(x);
-          hi.set(x + 4);
-          lo.store(p);
-          hi.store(p + 4);
-        }
+        if (j < live && i0 + i < a.ldp) *reinterpret_cast<u32x4*>((uint16_t*)a.prob + j * a.ldp + i0 + i) = w;
       });
+    } else if (KEEP == 2) {
+      rows_of<T, float>(lds, acc, b, [&](int jrow, int i, const u32x4& w) {
+        const int j = j0 + jrow;
+        if (j < live && i0 + i < a.ldp) *reinterpret_cast<u32x4*>((float*)a.prob + j * a.ldp + i0 + i) = w;
+      });
+    }
   }
 }
 
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
   const float ref = top == -__builtin_inff() ? 0.0f : top;
-  s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * kLog2e);
+  s = s * __builtin_amdgcn_exp2f(m - ref) + s2 * __builtin_amdgcn_exp2f(m2 - ref);
   m = top;
 }
 
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(1024) void k_join(Stats st, Rows rows, int slabs, i
   const int row = c0 + j;
   st.top[row] = m;
   st.inv[row] = 1.0f / s;
-  const float l = rows.target[row] < 0 ? __builtin_nanf("") : logf(s) + (m - st.zt[row]);
+  const float l = rows.target[row] < 0 ? __builtin_nanf("") : logf(s) + (m - st.zt[row]) * kLn2;
   st.loss[row] = l;
   if (loss_rows) loss_rows[rows.map[row]] = l;
 }
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
         const float top = a.st.top[row], inv = a.st.inv[row];
         const float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
         const float m = a.st.slab[(int64_t)slab * a.chunk + j].x;
-        const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f((m - top) * kLog2e) * inv * g;
+        const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f(m - top) * inv * g;
         if (NP == 1) {
           const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)a.prob + j * a.ld + v);
 #pragma unroll
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
           for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? lo.get(q) : hi.get(q - 4)) * f;
         }
         if (t >= v && t < v + 8) {
-          const float own = (__builtin_amdgcn_exp2f((a.st.zt[row] - top) * kLog2e) * inv - 1.0f) * g;
+          const float own = (__builtin_amdgcn_exp2f(a.st.zt[row] - top) * inv - 1.0f) * g;
 #pragma unroll
           for (int q = 0; q < 8; ++q) x[q] = t == v + q ? own : x[q];
         }
@@ -515,8 +515,9 @@ __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
   product<T, PAIRS>(a.P, a.Q, i0, j0, kb0, kb1, lds, acc);
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b)
-    rows_of<T>(lds, acc, b, [&](int jrow, int icol, const float(&x)[8]) {
+    rows_of<T, Eight>(lds, acc, b, [&](int jrow, int icol, const Eight& e) {
       const int j = j0 + jrow, i = i0 + icol;
+      const auto& x = e.x;
       if (j >= nj || i >= a.I) return;
       if (a.splits > 1) {
         float* p = a.part + ((int64_t)split * (a.by_rows ? a.J : a.chunk) + j) * a.I + i;

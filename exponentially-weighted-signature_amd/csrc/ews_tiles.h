@@ -203,32 +203,50 @@ __device__ __forceinline__ void tile_of(int id, int ti, int tj, int& i, int& j) 
   j = group * 8 + rest % width;
 }
 
-// A wavefront's block column b of its results, staged through its own part of LDS and handed on as rows: f(jrow, i, x)
-// gets eight consecutive results x of tile row jrow from tile column i on. Every lane of a row's lanes calls it.
-template <class T, class F>
+struct Eight {
+  float x[8];
+};
+
+// A wavefront's block column b of its results, staged through its own part of LDS and handed on as rows of numbers of
+// type W: f(jrow, i, x) gets the results of tile row jrow from tile column i on; float and uint16_t (whole numbers, cut
+// from floats in range) 16 bytes of them, Eight eight floats.
+template <class T, typename W, class F>
 __device__ __forceinline__ void rows_of(char* lds, const f32x16 (&acc)[T::TI][T::TJ], int b, F f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave % T::WI, wj = wave / T::WI;
-  float* stage = reinterpret_cast<float*>(lds) + wave * 32 * T::kRowWords;
+  char* stage = lds + wave * 32 * T::kRowWords * 4;
   const int r32 = lane & 31, half = lane >> 5;
+  constexpr bool kHalf = sizeof(W) == 2;
+  constexpr int kRow = kHalf ? T::kSlab * 2 + 16 : T::kRowWords * 4;  // bytes between rows
 #pragma unroll
   for (int a = 0; a < T::TI; ++a)
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<vec::f32x4*>(stage + r32 * T::kRowWords + a * 32 + g * 8 + half * 4) =
-          vec::f32x4{acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
+    for (int g = 0; g < 4; ++g) {
+      const vec::f32x4 x = {acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
+      const int at = r32 * kRow + (a * 32 + g * 8 + half * 4) * (kHalf ? 2 : 4);
+      if (kHalf)
+        *reinterpret_cast<vec::u32x2*>(stage + at) =
+            vec::u32x2{(uint32_t)x[0] | ((uint32_t)x[1] << 16), (uint32_t)x[2] | ((uint32_t)x[3] << 16)};
+      else
+        *reinterpret_cast<vec::f32x4*>(stage + at) = x;
+    }
   asm volatile("" ::: "memory");
   __builtin_amdgcn_wave_barrier();
-  constexpr int kLanes = T::kSlab / 8;   // lanes of one row
+  constexpr int kEach = sizeof(W) == sizeof(Eight) ? 8 : 16 / (int)sizeof(W);  // numbers handed on at a time
+  constexpr int kLanes = T::kSlab / kEach;                                     // lanes of one row
+  constexpr int kBytes = kHalf ? 16 : 4 * kEach;
 #pragma unroll
   for (int it = 0; it < 32 * kLanes / 64; ++it) {
     const int row = it * (64 / kLanes) + lane / kLanes;
-    const int col = (lane % kLanes) * 8;
-    const float* s = stage + row * T::kRowWords + col;
-    const vec::f32x4 lo = *reinterpret_cast<const vec::f32x4*>(s);
-    const vec::f32x4 hi = *reinterpret_cast<const vec::f32x4*>(s + 4);
-    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    f((wj * T::TJ + b) * 32 + row, wi * T::kSlab + col, x);
+    const char* s = stage + row * kRow + (lane % kLanes) * kBytes;
+    const int j = (wj * T::TJ + b) * 32 + row, i = wi * T::kSlab + (lane % kLanes) * kEach;
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(s);
+    if constexpr (kEach == 8 && !kHalf) {
+      const vec::f32x4 x = __builtin_bit_cast(vec::f32x4, lo), y = *reinterpret_cast<const vec::f32x4*>(s + 16);
+      f(j, i, Eight{{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}});
+    } else {
+      f(j, i, lo);
+    }
   }
   asm volatile("" ::: "memory");
   __builtin_amdgcn_wave_barrier();
