@@ -17,11 +17,11 @@
 //             fifth of what dz loses in bfloat16 afterwards (bfloat16 itself would lose as much again, and a logit
 //             rounded to it more than its probability).
 //   k_join    joins a row's slabs: the row's maximum M and sum, its loss.
-//   k_dz      dz = exp(z - m) exp(m - M) g / sum, in place and transposed; the target's entry from its own float32
+//   k_dz      dz = exp(z - m) exp(m - M) g / sum, in place; the target's entry from its own float32
 //             logit, so a target of probability near one loses nothing. The mean's factor stays out of it: most
 //             targets' entries are near -1, which bfloat16 holds, while their common factor's rounding would scale
 //             the whole gradient.
-//   k_grad    dh and dW, sums in float32. Few tiles are split over k and joined in order by k_reduce.
+//   k_grad    dh and dW, sums in float32, reading W, h and dz as they are, with k along their rows. Few tiles are split over k and joined in order by k_reduce.
 //
 // It is kept for kChunkBytes of rows at a time; dW is summed over the chunks in float32. Nothing is added with
 // atomics: the same inputs give the same bits.
@@ -126,41 +126,28 @@ struct PackArgs {
   int rows, cols;          // of the source (rows: kept[0] where there is a map)
   const int* map;          // gathers the rows; null: all of them
   const int* kept;
-  uint16_t* dst;           // planes (rows, ld), zero in further columns and in rows up to a multiple of 64; may be null
+  uint16_t* dst;           // planes (rows, ld), zero in further columns and in rows up to a multiple of 64
   int64_t ld, plane;
   int dst_rows;
-  uint16_t* turned;        // planes (cols, ldt), likewise; may be null
-  int64_t ldt, plane_t;
 };
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;
-  __shared__ T tile[64][sizeof(T) == 4 ? 65 : 66];
   const int rows = a.map ? a.kept[0] : a.rows;
   const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
   if (r0 >= rows) return;
   const int col = threadIdx.x & 63;
   for (int i = threadIdx.x >> 6; i < 64; i += 4) {
     const int row = r0 + i;
+    if (row >= a.dst_rows) break;
     T x = narrow<T>(0.0f);
     if (row < rows && c0 + col < a.cols)
       x = ((const T*)a.src)[(int64_t)(a.map ? a.map[row] : row) * a.stride + c0 + col];
-    tile[i][col] = x;
-    if (a.dst && row < a.dst_rows) {
-      uint16_t p[NP];
-      planes(x, p);
-#pragma unroll
-      for (int q = 0; q < NP; ++q) a.dst[q * a.plane + (int64_t)row * a.ld + c0 + col] = p[q];
-    }
-  }
-  if (!a.turned) return;
-  __syncthreads();
-  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
     uint16_t p[NP];
-    planes(tile[col][i], p);
+    planes(x, p);
 #pragma unroll
-    for (int q = 0; q < NP; ++q) a.turned[q * a.plane_t + (int64_t)(c0 + i) * a.ldt + r0 + col] = p[q];
+    for (int q = 0; q < NP; ++q) a.dst[q * a.plane + (int64_t)row * a.ld + c0 + col] = p[q];
   }
 }
 
@@ -202,7 +189,7 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   if (j0 >= live) return;
   f32x16 acc[T::TI][T::TJ];
-  product<T, PAIRS>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, lds, acc);
+  product<T, PAIRS, false, false>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, lds, acc);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave % T::WI, wj = wave / T::WI;
@@ -327,115 +314,88 @@ struct DzArgs {
   int c0, chunk, slab, slabs;
   void* prob;
   int64_t ld;             // the vocabulary padded to a multiple of 64
-  uint16_t* dz;           // planes (chunk, ld): prob itself in bfloat16
+  uint16_t* dz;           // planes (chunk, ld): in bfloat16 prob itself; zero rows up to a multiple of 64
   int64_t plane;
-  uint16_t* turned;       // planes (ld, chunk)
-  int64_t plane_t;
-  float* bias;            // (ceil(chunk / 256), ld) sums over the rows; may be null
+  float* bias;            // (ceil(chunk / kDzRows), ld) sums over the rows; may be null
 };
+
+constexpr int kDzRows = 128;  // rows a workgroup of k_dz goes over, one wavefront a row, 512 columns wide
 
 template <int NP>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
-  __shared__ float tile[64][65];
-  const int v0 = blockIdx.x * 64;
+  __shared__ float part[4][64][9];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int v = (blockIdx.x * 64 + lane) * 8;
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   const int padded = (live + 63) / 64 * 64;
-  const int slab = v0 / a.slab;
-  float sums[2] = {0.0f, 0.0f};
-  for (int r0 = blockIdx.y * 256; r0 < blockIdx.y * 256 + 256 && r0 < padded; r0 += 64) {
+  const bool in = v < a.ld;
+  const int slab = in ? v / a.slab : 0;
+  const int r0 = blockIdx.y * kDzRows, r1 = r0 + kDzRows < padded ? r0 + kDzRows : padded;
+  float sums[8];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int idx = threadIdx.x + 256 * c;
-      const int i = idx >> 3, v = v0 + (idx & 7) * 8, j = r0 + i;
-      float x[8];
+  for (int q = 0; q < 8; ++q) sums[q] = 0.0f;
+  for (int j = r0 + wave; j < r1; j += 4) {
+    float x[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) x[q] = 0.0f;
-      if (j < live) {
-        const int row = a.c0 + j;
-        const int t = a.rows.target[row];
-        const float top = a.st.top[row], inv = a.st.inv[row];
-        const float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
-        const float m = a.st.slab[(int64_t)slab * a.chunk + j].x;
-        const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f(m - top) * inv * g;
-        if (NP == 1) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)a.prob + j * a.ld + v);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint32_t y = (w[q >> 1] >> (16 * (q & 1))) & 0xffffu;
-            x[q] = y == 65535u ? 0.0f * f : __builtin_amdgcn_exp2f((float)y * (-1.0f / kSteps)) * f;
-          }
-        } else {
-          Pack<float, 4> lo, hi;
-          lo.load((const float*)a.prob + j * a.ld + v);
-          hi.load((const float*)a.prob + j * a.ld + v + 4);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? lo.get(q) : hi.get(q - 4)) * f;
-        }
-        if (t >= v && t < v + 8) {
-          const float own = (__builtin_amdgcn_exp2f(a.st.zt[row] - top) * inv - 1.0f) * g;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] = t == v + q ? own : x[q];
-        }
-      }
+    for (int q = 0; q < 8; ++q) x[q] = 0.0f;
+    if (j < live && in) {
+      const int row = a.c0 + j;
+      const int t = a.rows.target[row];
+      const float top = a.st.top[row], inv = a.st.inv[row];
+      const float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
+      const float m = a.st.slab[(int64_t)slab * a.chunk + j].x;
+      const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f(m - top) * inv * g;
       if (NP == 1) {
-        Pack<bf16, 8> p;
-        p.set(x);
-        if (j < live) p.store((bf16*)a.dz + j * a.ld + v);
-      } else if (j < live) {
-        uint16_t p[8][3];
+        const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)a.prob + j * a.ld + v);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) planes(x[q], p[q]);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          u32x4 w;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) w[q] = (uint32_t)p[2 * q][k] | ((uint32_t)p[2 * q + 1][k] << 16);
-          *reinterpret_cast<u32x4*>(a.dz + k * a.plane + j * a.ld + v) = w;
+        for (int q = 0; q < 8; ++q) {
+          const uint32_t y = (w[q >> 1] >> (16 * (q & 1))) & 0xffffu;
+          x[q] = y == 65535u ? 0.0f * f : __builtin_amdgcn_exp2f((float)y * (-1.0f / kSteps)) * f;
         }
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) tile[i][(idx & 7) * 8 + q] = x[q];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int idx = threadIdx.x + 256 * c;
-      const int v = idx >> 3, i = (idx & 7) * 8;
-      float x[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        x[q] = tile[i + q][v];
-        sums[c] += x[q];
-      }
-      uint16_t* dst = a.turned + (int64_t)(v0 + v) * a.chunk + r0 + i;
-      if (NP == 1) {
-        Pack<bf16, 8> p;
-        p.set(x);
-        p.store((bf16*)dst);
       } else {
-        uint16_t p[8][3];
+        Pack<float, 4> lo, hi;
+        lo.load((const float*)a.prob + j * a.ld + v);
+        hi.load((const float*)a.prob + j * a.ld + v + 4);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) planes(x[q], p[q]);
+        for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? lo.get(q) : hi.get(q - 4)) * f;
+      }
+      if (t >= v && t < v + 8) {
+        const float own = (__builtin_amdgcn_exp2f(a.st.zt[row] - top) * inv - 1.0f) * g;
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-          u32x4 w;
+        for (int q = 0; q < 8; ++q) x[q] = t == v + q ? own : x[q];
+      }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) w[q] = (uint32_t)p[2 * q][k] | ((uint32_t)p[2 * q + 1][k] << 16);
-          *reinterpret_cast<u32x4*>(dst + k * a.plane_t) = w;
-        }
+      for (int q = 0; q < 8; ++q) sums[q] += x[q];
+    }
+    if (!in) continue;
+    if (NP == 1) {
+      Pack<bf16, 8> p;
+      p.set(x);
+      p.store((bf16*)a.dz + j * a.ld + v);
+    } else {
+      uint16_t p[8][3];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) planes(x[q], p[q]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        u32x4 w;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = (uint32_t)p[2 * q][k] | ((uint32_t)p[2 * q + 1][k] << 16);
+        *reinterpret_cast<u32x4*>(a.dz + k * a.plane + j * a.ld + v) = w;
       }
     }
-    __syncthreads();
   }
   if (!a.bias) return;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    float s = sums[c];
-    s += __shfl_xor(s, 1);
-    s += __shfl_xor(s, 2);
-    s += __shfl_xor(s, 4);
-    const int idx = threadIdx.x + 256 * c;
-    if ((idx & 7) == 0) a.bias[(int64_t)blockIdx.y * a.ld + v0 + (idx >> 3)] = s;
+  for (int q = 0; q < 8; ++q) part[wave][lane][q] = sums[q];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 512; c += 256) {
+    const int col = blockIdx.x * 512 + c;
+    if (col >= a.ld) break;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) s += part[w][c >> 3][c & 7];
+    a.bias[(int64_t)blockIdx.y * a.ld + col] = s;
   }
 }
 
@@ -498,7 +458,8 @@ __device__ __forceinline__ void finish(const GradArgs& a, int64_t row, int i, co
   }
 }
 
-template <class T, int PAIRS, typename O>
+// ROWS: dW, whose k is the chunk's kept rows and whose operands are both turned; else dh, whose rows they are.
+template <class T, int PAIRS, bool ROWS, typename O>
 __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
   extern __shared__ char lds[];
   const int split = blockIdx.y;
@@ -507,12 +468,12 @@ __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
   const int i0 = it * T::I, j0 = jt * T::J;
   int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   live = live > 0 ? live : 0;
-  const int nj = a.by_rows ? a.J : live;
+  const int nj = ROWS ? a.J : live;
   if (j0 >= nj) return;
   int kb0 = split * a.per, kb1 = kb0 + a.per < a.kblocks ? kb0 + a.per : a.kblocks;
-  if (a.by_rows && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
+  if (ROWS && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
   f32x16 acc[T::TI][T::TJ];
-  product<T, PAIRS>(a.P, a.Q, i0, j0, kb0, kb1, lds, acc);
+  product<T, PAIRS, true, ROWS>(a.P, a.Q, i0, j0, kb0, kb1, lds, acc);
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b)
     rows_of<T, Eight>(lds, acc, b, [&](int jrow, int icol, const Eight& e) {
@@ -520,13 +481,13 @@ __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
       const auto& x = e.x;
       if (j >= nj || i >= a.I) return;
       if (a.splits > 1) {
-        float* p = a.part + ((int64_t)split * (a.by_rows ? a.J : a.chunk) + j) * a.I + i;
+        float* p = a.part + ((int64_t)split * (ROWS ? a.J : a.chunk) + j) * a.I + i;
         const int n = a.I - i < 8 ? a.I - i : 8;
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           if (q < n) p[q] = x[q];
       } else {
-        finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], i, x);
+        finish<O>(a, ROWS ? j : a.rows.map[a.c0 + j], i, x);
       }
     });
 }
@@ -567,7 +528,7 @@ namespace {
 
 using namespace ews::loss;
 
-// Rows kept at a time: exp(z - m) and the transposed dz (float32: with their three planes) of as many as fit in this.
+// Rows kept at a time: exp(z - m), and dz in its place (float32: dz in three planes beside it), of as many as fit here.
 constexpr int64_t kChunkBytes = (int64_t)2 << 30;
 constexpr int64_t kScoreRows = 65536;  // rows of a call without gradients whose slabs' sums are kept at a time
 constexpr int kFill = 512;  // workgroups that a product is split into along k where it has fewer tiles than CUs
@@ -585,7 +546,7 @@ struct LPlan {
   int chunks, slabs, bias_pad;
   bool train, packed;
   Product logits, dh, dw;
-  size_t map, target, meta, zt, top, inv, loss, xp, xt, wp, wt, bias, slab, prob, dz, turned, dbias, dbsum, part, acc;
+  size_t map, target, meta, zt, top, inv, loss, xp, wp, bias, slab, prob, dz, dbias, dbsum, part, acc;
   size_t total;
 };
 
@@ -638,7 +599,7 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.Hp = (int64_t)ceil_div(p.H, 64) * 64;
   p.Vp = (int64_t)ceil_div(p.V, 64) * 64;
   p.Np = (int64_t)ceil_div(p.N, 64) * 64;
-  const int64_t each = p.Vp * (p.np == 3 ? 16 : 4);
+  const int64_t each = p.Vp * (p.np == 3 ? 10 : 2);
   int64_t fit = train ? kChunkBytes / each / 256 * 256 : kScoreRows;
   if (fit < 256) fit = 256;
   p.chunk = p.Np < fit ? p.Np : fit;
@@ -668,12 +629,9 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.bias = take((size_t)p.bias_pad * 4);
   p.slab = take((size_t)p.slabs * p.chunk * 8);
   if (train) {
-    p.xt = take((size_t)(p.Np * p.Hp * p.np * 2));
-    p.wt = take((size_t)(p.Vp * p.Hp * p.np * 2));
     p.prob = take((size_t)(p.chunk * p.Vp) * (p.np == 3 ? 4 : 2));
     p.dz = p.np == 3 ? take((size_t)(p.chunk * p.Vp) * 6) : p.prob;
-    p.turned = take((size_t)(p.chunk * p.Vp) * p.np * 2);
-    p.dbias = take((size_t)(ceil_div(p.chunk, 256) * p.Vp) * 4);
+    p.dbias = take((size_t)(ceil_div(p.chunk, kDzRows) * p.Vp) * 4);
     p.dbsum = take((size_t)p.V * 4);
     size_t part = 0;
     if (p.dh.splits > 1) part = (size_t)p.dh.splits * p.chunk * p.H * 4;
@@ -687,7 +645,8 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
 
 // bfloat16 weights whose rows start at multiples of 16 bytes and fill whole k blocks are read where they are.
 bool reads_direct(const ews_loss_desc* s, const void* weight) {
-  return s->dtype == EWS_DTYPE_BF16 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0 && (uintptr_t)weight % 16 == 0;
+  return s->dtype == EWS_DTYPE_BF16 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0 &&
+         s->weight_stride <= 1 << 22 && (uintptr_t)weight % 16 == 0;
 }
 
 struct Call {
@@ -727,12 +686,12 @@ int launch_logits(Kind kind, const LogitArgs& a, hipStream_t st) {
   return kind == kMedium ? launch_logits_as<Medium, PAIRS, KEEP>(a, st) : launch_logits_as<Flat, PAIRS, KEEP>(a, st);
 }
 
-template <class T, typename O>
+template <class T, bool ROWS, typename O>
 int launch_grad_as(const GradArgs& a, hipStream_t st) {
   constexpr int kP = sizeof(O) == 4 ? kPairs : 1;  // float32 gradients are those of float32 operands
-  const int rc = allow_lds(k_grad<T, kP, O>, T::kLdsBytes);
+  const int rc = allow_lds(k_grad<T, kP, ROWS, O>, T::kLdsBytes);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_grad<T, kP, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
+  hipLaunchKernelGGL((k_grad<T, kP, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
   LOSS_CHECK();
   if (a.splits > 1) {
     const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * ((a.I + 7) / 8);
@@ -742,10 +701,10 @@ int launch_grad_as(const GradArgs& a, hipStream_t st) {
   return EWS_OK;
 }
 
-template <typename O>
+template <bool ROWS, typename O>
 int launch_grad(Kind kind, const GradArgs& a, hipStream_t st) {
-  if (kind == kLarge) return launch_grad_as<Large, O>(a, st);
-  return kind == kMedium ? launch_grad_as<Medium, O>(a, st) : launch_grad_as<Flat, O>(a, st);
+  if (kind == kLarge) return launch_grad_as<Large, ROWS, O>(a, st);
+  return kind == kMedium ? launch_grad_as<Medium, ROWS, O>(a, st) : launch_grad_as<Flat, ROWS, O>(a, st);
 }
 
 template <typename T>
@@ -756,8 +715,7 @@ int pack(const PackArgs& a, int64_t rows, int64_t cols, hipStream_t st) {
 }
 
 // What every call begins with: the kept rows, the operands' planes, the bias.
-int begin(Call& c, const void* hidden, const void* weight, const void* bias, const int64_t* targets, float* loss_rows,
-          bool turn_hidden, bool turn_weight) {
+int begin(Call& c, const void* hidden, const void* weight, const void* bias, const int64_t* targets, float* loss_rows) {
   const LPlan& p = c.p;
   const bool f32 = p.np == 3;
   hipLaunchKernelGGL(k_rows, dim3(1), dim3(1024), 0, c.st, targets, p.N, p.V, c.s->ignore_index,
@@ -774,31 +732,19 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   x.ld = p.Hp;
   x.plane = p.Np * p.Hp;
   x.dst_rows = (int)p.Np;
-  if (turn_hidden) {
-    x.turned = (uint16_t*)(c.w + p.xt);
-    x.ldt = p.Np;
-    x.plane_t = p.Np * p.Hp;
-  }
   int rc = f32 ? pack<float>(x, p.Np, p.Hp, c.st) : pack<bf16>(x, p.Np, p.Hp, c.st);
   if (rc != EWS_OK) return rc;
-  if (p.packed || turn_weight) {
+  if (p.packed) {
     PackArgs w{};
     w.src = weight;
     w.stride = c.s->weight_stride;
     w.rows = p.V;
     w.cols = p.H;
-    if (p.packed) {
-      w.dst = (uint16_t*)(c.w + p.wp);
-      w.ld = p.Hp;
-      w.plane = p.V * p.Hp;
-      w.dst_rows = p.V;
-    }
-    if (turn_weight) {
-      w.turned = (uint16_t*)(c.w + p.wt);
-      w.ldt = p.Vp;
-      w.plane_t = p.Vp * p.Hp;
-    }
-    rc = f32 ? pack<float>(w, p.Vp, p.Hp, c.st) : pack<bf16>(w, p.Vp, p.Hp, c.st);
+    w.dst = (uint16_t*)(c.w + p.wp);
+    w.ld = p.Hp;
+    w.plane = p.V * p.Hp;
+    w.dst_rows = p.V;
+    rc = f32 ? pack<float>(w, p.V, p.Hp, c.st) : pack<bf16>(w, p.V, p.Hp, c.st);
     if (rc != EWS_OK) return rc;
   }
   float* b32 = (float*)(c.w + p.bias);
@@ -811,17 +757,22 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   return EWS_OK;
 }
 
+Operand weight_operand(const Call& c, const void* weight) {
+  const LPlan& p = c.p;
+  if (p.packed) return Operand{(const uint16_t*)(c.w + p.wp), p.Hp, p.V * p.Hp, p.V, (int)p.Hp};
+  return Operand{(const uint16_t*)weight, c.s->weight_stride, 0, p.V, (int)p.Hp};
+}
+
+Operand hidden_operand(const Call& c) {
+  const LPlan& p = c.p;
+  return Operand{(const uint16_t*)(c.w + p.xp), p.Hp, p.Np * p.Hp, (int)p.Np, (int)p.Hp};
+}
+
 int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
   const LPlan& p = c.p;
   LogitArgs a{};
-  a.W.p = p.packed ? (const uint16_t*)(c.w + p.wp) : (const uint16_t*)weight;
-  a.W.ld = p.packed ? p.Hp : c.s->weight_stride;
-  a.W.plane = p.V * p.Hp;
-  a.W.rows = p.V;
-  a.X.p = (const uint16_t*)(c.w + p.xp);
-  a.X.ld = p.Hp;
-  a.X.plane = p.Np * p.Hp;
-  a.X.rows = (int)p.Np;
+  a.W = weight_operand(c, weight);
+  a.X = hidden_operand(c);
   a.ti = p.logits.ti;
   a.tj = p.logits.tj;
   a.kblocks = p.logits.kblocks;
@@ -886,7 +837,7 @@ int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* 
   if (!hidden || !weight || !targets || !loss || !workspace) return EWS_ERR_NULL;
   Call c = make_call(desc, p, workspace, stream);
   float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
-  rc = begin(c, hidden, weight, bias, targets, rows, false, false);
+  rc = begin(c, hidden, weight, bias, targets, rows);
   if (rc != EWS_OK) return rc;
   for (int k = 0; k < p.chunks; ++k) {
     rc = logits(c, weight, k, rows);
@@ -905,7 +856,7 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
   Call c = make_call(desc, p, workspace, stream);
   const bool f32 = p.np == 3;
   float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
-  rc = begin(c, hidden, weight, bias, targets, rows, grad_weight != nullptr, grad_hidden != nullptr);
+  rc = begin(c, hidden, weight, bias, targets, rows);
   if (rc != EWS_OK) return rc;
   if (grad_hidden) {
     const int blocks = ceil_div(p.N, 4);
@@ -935,10 +886,8 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
     z.ld = p.Vp;
     z.dz = (uint16_t*)(c.w + p.dz);
     z.plane = p.chunk * p.Vp;
-    z.turned = (uint16_t*)(c.w + p.turned);
-    z.plane_t = p.chunk * p.Vp;
     z.bias = grad_bias ? (float*)(c.w + p.dbias) : nullptr;
-    const dim3 grid((uint32_t)(p.Vp / 64), ceil_div(p.chunk, 256));
+    const dim3 grid(ceil_div(p.Vp, 512), ceil_div(p.chunk, kDzRows));
     if (f32)
       hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
     else
@@ -963,8 +912,8 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
     g.factor = factor;
     g.part = (float*)(c.w + p.part);
     if (grad_hidden) {
-      g.P = Operand{(const uint16_t*)(c.w + p.wt), p.Vp, p.Vp * p.Hp, (int)p.Hp};
-      g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk};
+      g.P = weight_operand(c, weight);
+      g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, 0};
       g.ti = p.dh.ti;
       g.tj = p.dh.tj;
       g.splits = p.dh.splits;
@@ -976,12 +925,14 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
       g.sum = nullptr;
       g.add = 0;
       g.out = grad_hidden;
-      rc = f32 ? launch_grad<float>(p.dh.kind, g, c.st) : launch_grad<bf16>(p.dh.kind, g, c.st);
+      rc = f32 ? launch_grad<false, float>(p.dh.kind, g, c.st) : launch_grad<false, bf16>(p.dh.kind, g, c.st);
       if (rc != EWS_OK) return rc;
     }
     if (grad_weight) {
-      g.P = Operand{(const uint16_t*)(c.w + p.xt) + z.c0, p.Np, p.Np * p.Hp, (int)p.Hp};
-      g.Q = Operand{z.turned, p.chunk, z.plane_t, (int)p.Vp};
+      g.P = hidden_operand(c);
+      g.P.p += z.c0 * p.Hp;
+      g.P.rows -= z.c0;
+      g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, (int)p.Vp};
       g.ti = p.dw.ti;
       g.tj = p.dw.tj;
       g.splits = p.dw.splits;
@@ -993,7 +944,7 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
       g.sum = f32 ? (float*)grad_weight : (float*)(c.w + p.acc);
       g.add = k > 0 ? 1 : 0;
       g.out = last || f32 ? grad_weight : nullptr;
-      rc = f32 ? launch_grad<float>(p.dw.kind, g, c.st) : launch_grad<bf16>(p.dw.kind, g, c.st);
+      rc = f32 ? launch_grad<true, float>(p.dw.kind, g, c.st) : launch_grad<true, bf16>(p.dw.kind, g, c.st);
       if (rc != EWS_OK) return rc;
     }
   }

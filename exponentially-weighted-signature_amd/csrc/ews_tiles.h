@@ -1,7 +1,7 @@
 // Matrix products of bfloat16 operands on the matrix cores of MI355X (gfx950), as tiles for kernels with epilogues of
 // their own (ews_loss.hip).
 //
-//   D[j, i] = sum_k Q[j, k] P[i, k]      both operands with k contiguous, float32 sums
+//   D[j, i] = sum_k Q[j, k] P[i, k]      float32 sums; each operand with k contiguous, or stored turned, k its rows
 //
 // A workgroup of WI x WJ wavefronts owns I = 32 TI WI by J = 32 TJ WJ results, each wavefront TI x TJ blocks of 32 x 32
 // (v_mfma_f32_32x32x16_bf16: lane l holds row l % 32 of either operand at k = 8 (l / 32) + 0..7, and results
@@ -16,6 +16,9 @@
 // Reads and copies go out one by one between products that do not wait for them.
 // The 16-byte piece c of row r lies at c ^ (r / 2) % 8. A 16-byte read serves lanes {0-3, 12-15, 20-27}, then {4-11,
 // 16-19, 28-31}, and so the other half: the rows of each such sixteen lie in sixteen different groups of four banks.
+// A turned operand's stage is 64 rows of k, each as wide as the tile. It is read by the LDS's transposing reads (sixteen
+// lanes name four rows of k by sixteen columns, each gets four k of its column), two to a fragment, so nothing is turned
+// in memory. Piece c of row k lies at c ^ 4 (k % 4): the four rows that 32 lanes read at a time are in different banks.
 //
 // Float32 operands come as three bfloat16 planes (x = x0 + x1 + x2 exactly, |x1| <= 2^-8 |x|, |x2| <= 2^-16 |x|) and are
 // multiplied as six products, the smallest first: the three left out are at most 2^-23 of x w, 2^-26 or so at random.
@@ -35,9 +38,10 @@ using vec::u32x4;
 
 struct Operand {
   const uint16_t* p;
-  int64_t ld;      // elements between rows, a multiple of 8
+  int64_t ld;      // elements between rows, a multiple of 8, 2^22 at most
   int64_t plane;   // elements between planes
-  int rows;        // rows that may be read (a tile's further rows read the last one)
+  int rows;        // rows that may be read; what a tile has beyond them reads the last one
+  int cols;        // turned: columns that may be read, a multiple of 8, likewise
 };
 
 template <int WI_, int WJ_, int TI_, int TJ_>
@@ -60,36 +64,96 @@ __device__ __forceinline__ int piece_p(int pair) { return (0x001102 >> (4 * pair
 __device__ __forceinline__ int piece_q(int pair) { return (0x010120 >> (4 * pair)) & 15; }  // 0 2 1 0 1 0
 
 __device__ __forceinline__ int place(int row, int piece) { return piece ^ ((row >> 1) & 7); }
+template <int WIDTH>
+__device__ __forceinline__ int place_turned(int k, int piece) {
+  return WIDTH >= 128 ? piece ^ ((k & 3) << 2) : piece;
+}
 
 typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// One operand's rows of a tile: what each thread copies, and the copies of a stage.
-template <int COPIES, int THREADS>
+// One operand of a tile, WIDTH results wide: what each thread copies of a stage.
+template <bool TURNED, int WIDTH, int THREADS>
 struct Copier {
+  static constexpr int kCopies = WIDTH * 8 / THREADS;
+  static constexpr int kPieces = TURNED ? WIDTH / 8 : 8;  // pieces of a stage's row
   const uint16_t* base;
   int64_t plane;
-  int offset[COPIES];   // bytes from the tile's first row; at most 256 rows of 2^22 numbers apart
-  __device__ __forceinline__ Copier(const Operand& o, int row0) {
-    row0 = row0 < o.rows ? row0 : o.rows - 1;
-    base = o.p + row0 * o.ld;
-    plane = o.plane;
+  uint32_t stride;           // bytes between rows
+  int rows, first, cols;
+  uint32_t offset[kCopies];  // bytes from the stage's first row
+  __device__ __forceinline__ Copier(const Operand& o, int tile)
+      : plane(o.plane), stride((uint32_t)o.ld * 2), rows(o.rows), first(tile), cols(o.cols) {
+    if (TURNED) {
+      base = o.p;
+      aim_turned(63);
+    } else {
+      first = first < rows ? first : rows - 1;
+      base = o.p + first * o.ld;
 #pragma unroll
-    for (int c = 0; c < COPIES; ++c) {
-      const int idx = threadIdx.x + c * THREADS;
-      const int row = idx >> 3;
-      const int src = row0 + row < o.rows ? row : o.rows - 1 - row0;
-      offset[c] = (int)((uint32_t)src * (uint32_t)(o.ld * 2) + 16 * place(row, idx & 7));
+      for (int c = 0; c < kCopies; ++c) {
+        const int idx = threadIdx.x + c * THREADS;
+        const int row = idx / kPieces;
+        offset[c] = (uint32_t)(first + row < rows ? row : rows - 1 - first) * stride + 16 * place(row, idx % kPieces);
+      }
     }
   }
-  // The address of the rows of k block kb.
-  __device__ __forceinline__ const uint16_t* at(int piece, int kb) const {
-    return base + piece * plane + (int64_t)kb * 64;
+  // Turned: a stage's rows of k, those past `last` read it again.
+  __device__ __forceinline__ void aim_turned(int last) {
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const int idx = threadIdx.x + c * THREADS;
+      const int k = idx / kPieces;
+      const int col = first + 8 * place_turned<WIDTH>(k, idx % kPieces);
+      offset[c] = (uint32_t)(k < last ? k : last) * stride + 2 * (col < cols ? col : cols - 8);
+    }
   }
-  // One of the copies; `to`: this wavefront's kilobyte of the stage.
+  // The address of k block kb; blocks are asked for in order, so one that is not whole is the last.
+  __device__ __forceinline__ const uint16_t* at(int piece, int kb) {
+    if (!TURNED) return base + piece * plane + (int64_t)kb * 64;
+    if (rows - kb * 64 < 64) aim_turned(rows - 1 - kb * 64);
+    return base + piece * plane + (int64_t)kb * 64 * (stride / 2);
+  }
+  // One of the copies; `to`: this wavefront's kilobyte of the stage. Written out, not a builtin: before every
+  // transposing read the compiler would wait for all the copies that it knows of. It has no result in a register; what
+  // is read of it waits in arrive().
   __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const {
-#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass does not know the buffer builtins
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, -1, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + c * THREADS * 16), 16, offset[c], 0, 0, 0);
+    const uint64_t at = (uint64_t)from;
+    const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)(to + c * THREADS * 16);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset[c]), "s"(rsrc)
+                 : "memory", "m0");
+  }
+};
+
+// A wavefront's fragments of one operand: BLOCKS blocks of 32 from block `first` of the tile on.
+template <bool TURNED, int WIDTH, int BLOCKS>
+struct Reader {
+  int at[TURNED ? BLOCKS : 4];
+  __device__ __forceinline__ Reader(int first, int lane) {
+    const int r32 = lane & 31, half = lane >> 5;
+    if (TURNED) {
+      const int k = (lane >> 2) & 3;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+        at[b] = (8 * half + k) * WIDTH * 2 +
+                place_turned<WIDTH>(k, (first + b) * 4 + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + (lane & 1) * 8;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) at[k] = (first * 32 + r32) * 128 + place(r32, 2 * k + half) * 16;
+    }
+  }
+  // Block b at the stage's k-th sixteen.
+  __device__ __forceinline__ bf16x8 get(char* stage, int k, int b) const {
+    if (!TURNED) return *reinterpret_cast<const bf16x8*>(stage + at[k] + b * 4096);
+#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass does not know the builtin
+    char* from = stage + at[b] + k * 16 * WIDTH * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)from);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(from + 4 * WIDTH * 2));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#else
+    return bf16x8{};
 #endif
   }
 };
@@ -104,7 +168,7 @@ __device__ __forceinline__ void arrive() {
 
 // The results of the workgroup's tile at (i0, j0) over k blocks [kb0, kb1); PAIRS: 1, or kPairs for three planes. On
 // return LDS is free.
-template <class T, int PAIRS>
+template <class T, int PAIRS, bool TURNED_P, bool TURNED_Q>
 __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
                                         char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -116,8 +180,8 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
   if (kb0 >= kb1) return;
-  const Copier<T::kCopiesP, T::kThreads> cp(P, i0);
-  const Copier<T::kCopiesQ, T::kThreads> cq(Q, j0);
+  Copier<TURNED_P, T::I, T::kThreads> cp(P, i0);
+  Copier<TURNED_Q, T::J, T::kThreads> cq(Q, j0);
   const int stages = (kb1 - kb0) * PAIRS;
   constexpr int kCopies = T::kCopiesP + T::kCopiesQ, kReads = T::TI + T::TJ, kProducts = T::TI * T::TJ;
   constexpr int kMost = kReads > kProducts ? kReads : kProducts, kSlots = kMost > kCopies ? kMost : kCopies;
@@ -137,21 +201,18 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
     else
       cq.copy(c - T::kCopiesP, fromQ, to + T::kBytesP);
   };
-  const int r32 = lane & 31, half = lane >> 5;
-  const int atP = (wi * T::TI * 32 + r32) * 128, atQ = T::kBytesP + (wj * T::TJ * 32 + r32) * 128;
-  int at[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) at[k] = place(r32, 2 * k + half) * 16;
+  const Reader<TURNED_P, T::I, T::TI> rp(wi * T::TI, lane);
+  const Reader<TURNED_Q, T::J, T::TJ> rq(wj * T::TJ, lane);
   struct Sixteen {
     bf16x8 p[T::TI], q[T::TJ];
   } even, odd;
   // the n-th of a sixteen's reads: the first product's two first
   auto read = [&](Sixteen& f, int s, int k, int n) {
-    const char* stage = lds + (s & 1) * T::kStage + at[k];
+    char* stage = lds + (s & 1) * T::kStage;
     if (n >= 1 && n <= T::TJ)
-      f.q[n - 1] = *reinterpret_cast<const bf16x8*>(stage + atQ + (n - 1) * 4096);
+      f.q[n - 1] = rq.get(stage + T::kBytesP, k, n - 1);
     else
-      f.p[n ? n - T::TJ : 0] = *reinterpret_cast<const bf16x8*>(stage + atP + (n ? n - T::TJ : 0) * 4096);
+      f.p[n ? n - T::TJ : 0] = rp.get(stage, k, n ? n - T::TJ : 0);
   };
   // the products of one sixteen, and between them the reads of sixteen k of stage s and where asked its successor's copies
   auto multiply = [&](const Sixteen& f, Sixteen& next, int s, int k, bool copies) {
