@@ -5,7 +5,7 @@
 //   dz[n, v] = g_n (exp(z[n, v]) / sum_u exp(z[n, u]) - [v = t_n])
 //   dh = dz W        dW = dz^T h        db[v] = sum_n dz[n, v]
 //
-// Rows whose target is the ignored index are taken out first (k_rows), so nothing they hold is read and they cost
+// Rows whose target is the ignored index are taken out first (k_prepare), so nothing they hold is read and they cost
 // nothing; their loss and their row of dh are zero. A target outside the vocabulary makes its row's loss NaN.
 //
 // The head's three products are 2 N V H operations each and run on the matrix cores (ews_tiles.h); they bound the
@@ -65,46 +65,6 @@ struct Stats {
 };
 
 // ------------------------------------------------------------------------------------------------- rows and planes
-// One workgroup. A thread counts the kept ones of a stretch of rows, the counts are summed, the stretch is written.
-__global__ __launch_bounds__(1024) void k_rows(const int64_t* targets, int n, int vocab, int64_t ignore, int mean,
-                                               Rows r, float* loss_rows) {
-  __shared__ int wsum[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int each = (n + 1023) / 1024;
-  const int lo = tid * each < n ? tid * each : n;
-  const int hi = lo + each < n ? lo + each : n;
-  int m = 0;
-  for (int i = lo; i < hi; ++i) m += targets[i] != ignore;
-  int at = m;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int up = __shfl_up(at, s);
-    if (lane >= s) at += up;
-  }
-  if (lane == 63) wsum[wave] = at;
-  at -= m;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    if (w < wave) at += wsum[w];
-    total += wsum[w];
-  }
-  for (int i = lo; i < hi; ++i) {
-    const int64_t t = targets[i];
-    if (t != ignore) {
-      r.map[at] = i;
-      r.target[at++] = t >= 0 && t < vocab ? (int)t : -1;
-    } else if (loss_rows) {
-      loss_rows[i] = 0.0f;
-    }
-  }
-  if (tid == 0) {
-    r.kept[0] = total;
-    r.scale[0] = mean ? 1.0f / (float)(total > 0 ? total : 1) : 1.0f;
-  }
-}
-
 // The three bfloat16 planes of a float32 number, x = p0 + p1 + p2 exactly: each plane is the rest rounded to eight bits
 // (cut where rounding would reach infinity), so the second is at most 2^-8 and the third 2^-16 of x. An infinity or
 // NaN has nothing after its first plane.
@@ -151,19 +111,83 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------------ preparation
+struct PrepareArgs {
+  const int64_t* targets;
+  int n, vocab, padded, mean, H;
+  int64_t ignore;
+  Rows rows;
+  float* loss_rows;        // (N) or null: the ignored rows' zeros
+  const void* bias;        // or null
+  int bias_bf16;
+  float* bias_out;         // (padded)
+  void* grad_hidden;       // or null: the ignored rows' zeros
+  int bias_blocks;
+};
+
+// One workgroup. A thread counts the kept ones of a stretch of rows, the counts are summed, the stretch is written.
+__device__ __forceinline__ void keep_rows(const PrepareArgs& a) {
+  __shared__ int wsum[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (a.n + 1023) / 1024;
+  const int lo = tid * each < a.n ? tid * each : a.n;
+  const int hi = lo + each < a.n ? lo + each : a.n;
+  int m = 0;
+#pragma unroll 4
+  for (int i = lo; i < hi; ++i) m += a.targets[i] != a.ignore;
+  int at = m;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int up = __shfl_up(at, s);
+    if (lane >= s) at += up;
+  }
+  if (lane == 63) wsum[wave] = at;
+  at -= m;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) at += wsum[w];
+    total += wsum[w];
+  }
+  for (int i = lo; i < hi; ++i) {
+    const int64_t t = a.targets[i];
+    if (t != a.ignore) {
+      a.rows.map[at] = i;
+      a.rows.target[at++] = t >= 0 && t < a.vocab ? (int)t : -1;
+    } else if (a.loss_rows) {
+      a.loss_rows[i] = 0.0f;
+    }
+  }
+  if (tid == 0) {
+    a.rows.kept[0] = total;
+    a.rows.scale[0] = a.mean ? 1.0f / (float)(total > 0 ? total : 1) : 1.0f;
+  }
+}
+
 // The bias in float32 times log2 e, -inf past the vocabulary: those columns of a tile then have no weight in any row. A
 // finite bias stays finite (a mask of the type's lowest value is not -inf: a row of nothing else is uniform).
-template <typename T>
-__global__ __launch_bounds__(256) void k_bias(const T* bias, int vocab, int padded, float* out) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= padded) return;
+__device__ __forceinline__ void scale_bias(const PrepareArgs& a, int v) {
+  if (v >= a.padded) return;
   float b = -__builtin_inff();
-  if (v < vocab) {
-    const float x = bias ? widen(bias[v]) : 0.0f;
+  if (v < a.vocab) {
+    const float x = !a.bias ? 0.0f : a.bias_bf16 ? widen(((const bf16*)a.bias)[v]) : ((const float*)a.bias)[v];
     b = x * kLog2e;
     if (__builtin_isinf(b) && !__builtin_isinf(x)) b = copysignf(3.402823466e+38f, x);
   }
-  out[v] = b;
+  a.bias_out[v] = b;
+}
+
+// What needs nothing of the others, in one launch: the first workgroup lists the kept rows, some write the bias, the
+// others (16 rows each) zero the ignored rows of dh.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_prepare(PrepareArgs a) {
+  if (blockIdx.x == 0) return keep_rows(a);
+  const int b = blockIdx.x - 1;
+  if (b < a.bias_blocks) return scale_bias(a, b * 1024 + threadIdx.x);
+  const int row = (b - a.bias_blocks) * 16 + (threadIdx.x >> 6);
+  if (row >= a.n || a.targets[row] != a.ignore) return;
+  for (int c = threadIdx.x & 63; c < a.H; c += 64) ((T*)a.grad_hidden)[(int64_t)row * a.H + c] = narrow<T>(0.0f);
 }
 
 // ------------------------------------------------------------------------------------------------------ the logits
@@ -262,26 +286,32 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-// 64 rows a workgroup, sixteen wavefronts along the slabs.
+// ROWS rows a workgroup, the other threads along the slabs; joined as a tree.
+template <int ROWS>
 __global__ __launch_bounds__(1024) void k_join(Stats st, Rows rows, int slabs, int c0, int chunk, float* loss_rows) {
-  __shared__ float ms[16][64], ss[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kGroups = 1024 / ROWS;
+  __shared__ float ms[1024], ss[1024];
+  const int tid = threadIdx.x, group = tid / ROWS;
   const int live = rows.kept[0] - c0 < chunk ? rows.kept[0] - c0 : chunk;
-  const int j = blockIdx.x * 64 + lane;
-  if (blockIdx.x * 64 >= live) return;
+  const int j = blockIdx.x * ROWS + tid % ROWS;
+  if (blockIdx.x * ROWS >= live) return;
   float m = -__builtin_inff(), s = 0.0f;
   if (j < live) {
 #pragma unroll 4
-    for (int k = wave; k < slabs; k += 16) {
+    for (int k = group; k < slabs; k += kGroups) {
       const float2 x = st.slab[(int64_t)k * chunk + j];
       join(m, s, x.x, x.y);
     }
   }
-  ms[wave][lane] = m;
-  ss[wave][lane] = s;
-  __syncthreads();
-  if (wave || j >= live) return;
-  for (int w = 1; w < 16; ++w) join(m, s, ms[w][lane], ss[w][lane]);
+#pragma unroll
+  for (int g = kGroups / 2; g; g >>= 1) {
+    ms[tid] = m;
+    ss[tid] = s;
+    __syncthreads();
+    if (group < g) join(m, s, ms[tid + g * ROWS], ss[tid + g * ROWS]);
+    __syncthreads();
+  }
+  if (group || j >= live) return;
   const int row = c0 + j;
   st.top[row] = m;
   st.inv[row] = 1.0f / s;
@@ -316,10 +346,10 @@ struct DzArgs {
   int64_t ld;             // the vocabulary padded to a multiple of 64
   uint16_t* dz;           // planes (chunk, ld): in bfloat16 prob itself; zero rows up to a multiple of 64
   int64_t plane;
-  float* bias;            // (ceil(chunk / kDzRows), ld) sums over the rows; may be null
+  float* bias;            // (ceil(chunk / each), ld) sums over the rows; may be null
+  int each;               // rows a workgroup goes over, one wavefront a row, 512 columns wide
 };
 
-constexpr int kDzRows = 128;  // rows a workgroup of k_dz goes over, one wavefront a row, 512 columns wide
 
 template <int NP>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
@@ -330,7 +360,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   const int padded = (live + 63) / 64 * 64;
   const bool in = v < a.ld;
   const int slab = in ? v / a.slab : 0;
-  const int r0 = blockIdx.y * kDzRows, r1 = r0 + kDzRows < padded ? r0 + kDzRows : padded;
+  const int r0 = blockIdx.y * a.each, r1 = r0 + a.each < padded ? r0 + a.each : padded;
   float sums[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) sums[q] = 0.0f;
@@ -513,14 +543,6 @@ __global__ __launch_bounds__(256) void k_reduce(GradArgs a) {
   finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], i, x);
 }
 
-// Zero rows of dh where the target is ignored.
-template <typename T>
-__global__ __launch_bounds__(256) void k_ignored(const int64_t* targets, int n, int64_t ignore, T* grad, int H) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= n || targets[row] != ignore) return;
-  for (int c = threadIdx.x & 63; c < H; c += 64) grad[(int64_t)row * H + c] = narrow<T>(0.0f);
-}
-
 }  // namespace loss
 }  // namespace ews
 
@@ -542,7 +564,7 @@ struct Product {
 struct LPlan {
   int N, H, V, np;
   int64_t Hp, Vp, Np, chunk;
-  int chunks, slabs, bias_pad;
+  int chunks, slabs, bias_pad, dz_rows;
   bool train, packed;
   Product logits, dh, dw;
   size_t map, target, meta, zt, top, inv, loss, xp, wp, bias, slab, prob, dz, dbias, dbsum, part, acc;
@@ -556,7 +578,7 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // A product of I x J results over kblocks of k: 256 x 32 tiles where J fits one; 256 x 256 ones where they give (split
 // over k, where that is allowed, into parts of 16 blocks at least) half the CUs work; else 128 x 128 ones, of which a CU
 // holds two. Measured at float32 N=4095 H=512 V=32000, dh (30 large tiles, split by 8): 0.55 ms, 0.80 ms with the small.
-Product pick(int64_t I, int64_t J, int kblocks, bool split) {
+Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split) {
   Product p;
   p.kblocks = kblocks;
   const int64_t large = (int64_t)ceil_div(I, 256) * ceil_div(J, 256);
@@ -574,9 +596,9 @@ Product pick(int64_t I, int64_t J, int kblocks, bool split) {
   p.per = kblocks;
   // one round of workgroups: a CU holds one of the large tiles, two of the others
   const int64_t n = (int64_t)p.ti * p.tj, room = p.kind == kLarge ? 256 : 512;
-  if (split && 2 * n <= room && kblocks >= 8) {
+  if (split && 2 * n <= room) {
     int64_t z = room / n;
-    const int64_t most = p.kind == kLarge ? parts : kblocks / 4;
+    const int64_t most = p.kind == kLarge ? parts : kblocks * pairs / 4 < kblocks ? kblocks * pairs / 4 : kblocks;
     if (z > most) z = most;
     if (z > 1) {
       p.per = ceil_div(kblocks, z);
@@ -609,9 +631,10 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.chunk = p.Np < fit ? p.Np : fit;
   p.chunks = ceil_div(p.Np, p.chunk);
   const int64_t most = p.chunk < p.N ? p.chunk : p.N;  // rows of a chunk
-  p.logits = pick(p.V, most, (int)(p.Hp / 64), false);
-  p.dh = pick(p.H, most, (int)(p.Vp / 64), true);
-  p.dw = pick(p.H, p.V, (int)(p.chunk / 64), true);
+  const int pairs = p.np == 3 ? kPairs : 1;
+  p.logits = pick(p.V, most, (int)(p.Hp / 64), pairs, false);
+  p.dh = pick(p.H, most, (int)(p.Vp / 64), pairs, true);
+  p.dw = pick(p.H, p.V, (int)(p.chunk / 64), pairs, true);
   const int tile_i = p.logits.kind == kMedium ? 128 : 256;
   p.bias_pad = p.logits.ti * tile_i;
   p.slabs = p.bias_pad / p.logits.slab;
@@ -635,7 +658,10 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   if (train) {
     p.prob = take((size_t)(p.chunk * p.Vp) * (p.np == 3 ? 4 : 2));
     p.dz = p.np == 3 ? take((size_t)(p.chunk * p.Vp) * 6) : p.prob;
-    p.dbias = take((size_t)(ceil_div(p.chunk, kDzRows) * p.Vp) * 4);
+    // 128 rows a workgroup (the bias's partial sums stay small), fewer where that leaves CUs without one
+    p.dz_rows = 128;
+    while (p.dz_rows > 4 && (int64_t)ceil_div(p.chunk, p.dz_rows) * ceil_div(p.Vp, 512) < 1024) p.dz_rows /= 2;
+    p.dbias = take((size_t)(ceil_div(p.chunk, p.dz_rows) * p.Vp) * 4);
     p.dbsum = take((size_t)p.V * 4);
     size_t part = 0;
     if (p.dh.splits > 1) part = (size_t)p.dh.splits * p.chunk * p.H * 4;
@@ -669,6 +695,7 @@ struct Call {
 
 template <class K>
 int allow_lds(K kernel, int bytes) {
+  if (bytes <= 64 << 10) return EWS_OK;  // allowed as it is
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                              bytes) == hipSuccess
              ? EWS_OK
@@ -719,11 +746,30 @@ int pack(const PackArgs& a, int64_t rows, int64_t cols, hipStream_t st) {
 }
 
 // What every call begins with: the kept rows, the operands' planes, the bias.
-int begin(Call& c, const void* hidden, const void* weight, const void* bias, const int64_t* targets, float* loss_rows) {
+int begin(Call& c, const void* hidden, const void* weight, const void* bias, const int64_t* targets, float* loss_rows,
+          void* grad_hidden) {
   const LPlan& p = c.p;
   const bool f32 = p.np == 3;
-  hipLaunchKernelGGL(k_rows, dim3(1), dim3(1024), 0, c.st, targets, p.N, p.V, c.s->ignore_index,
-                     c.s->reduction == EWS_LOSS_MEAN ? 1 : 0, c.rows, loss_rows);
+  PrepareArgs r{};
+  r.targets = targets;
+  r.n = p.N;
+  r.vocab = p.V;
+  r.padded = p.bias_pad;
+  r.mean = c.s->reduction == EWS_LOSS_MEAN ? 1 : 0;
+  r.H = p.H;
+  r.ignore = c.s->ignore_index;
+  r.rows = c.rows;
+  r.loss_rows = loss_rows;
+  r.bias = bias;
+  r.bias_bf16 = c.s->bias_dtype == EWS_DTYPE_BF16;
+  r.bias_out = (float*)(c.w + p.bias);
+  r.grad_hidden = grad_hidden;
+  r.bias_blocks = ceil_div(p.bias_pad, 1024);
+  const dim3 blocks(1 + r.bias_blocks + (grad_hidden ? ceil_div(p.N, 16) : 0));
+  if (f32)
+    hipLaunchKernelGGL((k_prepare<float>), blocks, dim3(1024), 0, c.st, r);
+  else
+    hipLaunchKernelGGL((k_prepare<bf16>), blocks, dim3(1024), 0, c.st, r);
   LOSS_CHECK();
   PackArgs x{};
   x.src = hidden;
@@ -751,13 +797,6 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
     rc = f32 ? pack<float>(w, p.V, p.Hp, c.st) : pack<bf16>(w, p.V, p.Hp, c.st);
     if (rc != EWS_OK) return rc;
   }
-  float* b32 = (float*)(c.w + p.bias);
-  const int blocks = ceil_div(p.bias_pad, 256);
-  if (c.s->bias_dtype == EWS_DTYPE_BF16)
-    hipLaunchKernelGGL((k_bias<bf16>), dim3(blocks), dim3(256), 0, c.st, (const bf16*)bias, p.V, p.bias_pad, b32);
-  else
-    hipLaunchKernelGGL((k_bias<float>), dim3(blocks), dim3(256), 0, c.st, (const float*)bias, p.V, p.bias_pad, b32);
-  LOSS_CHECK();
   return EWS_OK;
 }
 
@@ -794,8 +833,13 @@ int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
     rc = p.np == 3 ? launch_logits<kPairs, 0>(p.logits.kind, a, c.st) : launch_logits<1, 0>(p.logits.kind, a, c.st);
   }
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL(k_join, dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, a.c0, a.chunk,
-                     loss_rows);
+  // one row's slabs by a workgroup's threads where there are few rows: N=1, V=100003: 23 us with 16 threads a row
+  if (p.N <= 256)
+    hipLaunchKernelGGL((k_join<4>), dim3(ceil_div(p.chunk, 4)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, a.c0,
+                       a.chunk, loss_rows);
+  else
+    hipLaunchKernelGGL((k_join<64>), dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, a.c0,
+                       a.chunk, loss_rows);
   LOSS_CHECK();
   return EWS_OK;
 }
@@ -841,7 +885,7 @@ int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* 
   if (!hidden || !weight || !targets || !loss || !workspace) return EWS_ERR_NULL;
   Call c = make_call(desc, p, workspace, stream);
   float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
-  rc = begin(c, hidden, weight, bias, targets, rows);
+  rc = begin(c, hidden, weight, bias, targets, rows, nullptr);
   if (rc != EWS_OK) return rc;
   for (int k = 0; k < p.chunks; ++k) {
     rc = logits(c, weight, k, rows);
@@ -860,18 +904,8 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
   Call c = make_call(desc, p, workspace, stream);
   const bool f32 = p.np == 3;
   float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
-  rc = begin(c, hidden, weight, bias, targets, rows);
+  rc = begin(c, hidden, weight, bias, targets, rows, grad_hidden);
   if (rc != EWS_OK) return rc;
-  if (grad_hidden) {
-    const int blocks = ceil_div(p.N, 4);
-    if (f32)
-      hipLaunchKernelGGL((k_ignored<float>), dim3(blocks), dim3(256), 0, c.st, targets, p.N, desc->ignore_index,
-                         (float*)grad_hidden, p.H);
-    else
-      hipLaunchKernelGGL((k_ignored<bf16>), dim3(blocks), dim3(256), 0, c.st, targets, p.N, desc->ignore_index,
-                         (bf16*)grad_hidden, p.H);
-    LOSS_CHECK();
-  }
   const int wide = (p.H * (f32 ? 4 : 2)) % 16 == 0 && (uintptr_t)grad_hidden % 16 == 0 && (uintptr_t)grad_weight % 16 == 0;
   const float* factor = upstream ? nullptr : c.rows.scale;
   for (int k = 0; k < p.chunks; ++k) {
@@ -891,7 +925,8 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
     z.dz = (uint16_t*)(c.w + p.dz);
     z.plane = p.chunk * p.Vp;
     z.bias = grad_bias ? (float*)(c.w + p.dbias) : nullptr;
-    const dim3 grid(ceil_div(p.Vp, 512), ceil_div(p.chunk, kDzRows));
+    z.each = p.dz_rows;
+    const dim3 grid(ceil_div(p.Vp, 512), ceil_div(p.chunk, p.dz_rows));
     if (f32)
       hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
     else
