@@ -13,7 +13,7 @@
 //
 //   k_logits  a tile of z in registers; every wavefront takes the maximum m and the sum of exp(z - m) of its slab of
 //             the vocabulary for each of its rows. A training call also writes exp(z - m), for bfloat16 inputs as 16
-//             bits of (m - z) log2 e in steps of 2^-9: off by less than 2^-10.5 of exp(z - m) whatever its size, a
+//             bits of (m - z) log2 e in steps of 1/512: off by less than 2^-10.5 of exp(z - m) whatever its size, a
 //             fifth of what dz loses in bfloat16 afterwards (bfloat16 itself would lose as much again, and a logit
 //             rounded to it more than its probability).
 //   k_join    joins a row's slabs: the row's maximum M and sum, its loss.
@@ -46,7 +46,7 @@ typedef Tile<4, 1, 2, 1> Flat;    // 256 x 32, four wavefronts: few rows
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
-constexpr float kSteps = 512.0f;    // 16-bit logarithms: steps to a factor of two; 65535 stands for a probability of 0
+constexpr float kOctaves = 128.0f;  // 16-bit logarithms: 65535 is 2^-128 and stands for a probability of 0
 
 struct Rows {
   int* map;       // (N) the kept rows' places, in order
@@ -212,6 +212,15 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
   const int i0 = it * T::I, j0 = jt * T::J;
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   if (j0 >= live) return;
+  // the epilogue's operands, where it need not wait for them
+  float* tile_bias = reinterpret_cast<float*>(lds + T::kLdsBytes);
+  int* tile_target = reinterpret_cast<int*>(tile_bias + T::I);
+  for (int t = threadIdx.x; t < T::I + T::J; t += T::kThreads) {
+    if (t < T::I)
+      tile_bias[t] = a.bias[i0 + t];
+    else
+      tile_target[t - T::I] = j0 + t - T::I < live ? a.rows.target[a.c0 + j0 + t - T::I] : -1;
+  }
   f32x16 acc[T::TI][T::TJ];
   product<T, PAIRS, false, false>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, lds, acc);
 
@@ -219,7 +228,7 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
   const int wi = wave % T::WI, wj = wave / T::WI;
   const int r32 = lane & 31, half = lane >> 5;
   const int ibase = i0 + wi * T::kSlab;
-  const float* bias = a.bias + ibase + half * 4;
+  const float* bias = tile_bias + wi * T::kSlab + half * 4;
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) {
     const int j = j0 + (wj * T::TJ + b) * 32 + r32;
@@ -238,7 +247,7 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
       }
     m = fmaxf(m, __shfl_xor(m, 32));
     // the target's logit, from the one lane that holds it
-    const int want = (j < live ? a.rows.target[a.c0 + j] : -1) - ibase;
+    const int want = tile_target[(wj * T::TJ + b) * 32 + r32] - ibase;
     const bool mine = want >= 0 && want < T::kSlab && ((want >> 2) & 1) == half;
     if (__any(mine)) {
       float zt = 0.0f;
@@ -250,16 +259,15 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
       if (mine) a.st.zt[a.c0 + j] = zt;
     }
     const float ref = m == -__builtin_inff() ? 0.0f : m;  // a slab of -inf alone has the sum 0
-    const float shift = ref * kSteps + 0.5f;
     float s = 0.0f;
 #pragma unroll
     for (int t = 0; t < T::TI; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float z = acc[t][b][r];
-        const float e = __builtin_amdgcn_exp2f(z - ref);
+        const float y = acc[t][b][r] - ref;
+        const float e = __builtin_amdgcn_exp2f(y);
         s += e;
-        if (KEEP == 1) acc[t][b][r] = fminf(fmaf(z, -kSteps, shift), 65535.0f);
+        if (KEEP == 1) acc[t][b][r] = y * (-1.0f / kOctaves);
         if (KEEP == 2) acc[t][b][r] = e;
       }
     s += __shfl_xor(s, 32);
@@ -380,7 +388,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           const uint32_t y = (w[q >> 1] >> (16 * (q & 1))) & 0xffffu;
-          x[q] = y == 65535u ? 0.0f * f : __builtin_amdgcn_exp2f((float)y * (-1.0f / kSteps)) * f;
+          x[q] = y == 65535u ? 0.0f * f : __builtin_amdgcn_exp2f((float)y * (-kOctaves / 65535.0f)) * f;
         }
       } else {
         Pack<float, 4> lo, hi;
@@ -629,6 +637,9 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   int64_t fit = train ? kChunkBytes / each / 256 * 256 : kScoreRows;
   if (fit < 256) fit = 256;
   p.chunk = p.Np < fit ? p.Np : fit;
+  // equal chunks: the last one's tiles fill the CUs as the others' do
+  p.chunks = ceil_div(p.Np, p.chunk);
+  if (p.chunks > 1) p.chunk = (int64_t)ceil_div(ceil_div(p.Np, p.chunks), 256) * 256;
   p.chunks = ceil_div(p.Np, p.chunk);
   const int64_t most = p.chunk < p.N ? p.chunk : p.N;  // rows of a chunk
   const int pairs = p.np == 3 ? kPairs : 1;
@@ -704,9 +715,10 @@ int allow_lds(K kernel, int bytes) {
 
 template <class T, int PAIRS, int KEEP>
 int launch_logits_as(const LogitArgs& a, hipStream_t st) {
-  const int rc = allow_lds(k_logits<T, PAIRS, KEEP>, T::kLdsBytes);
+  constexpr int kLds = T::kLdsBytes + (T::I + T::J) * 4;
+  const int rc = allow_lds(k_logits<T, PAIRS, KEEP>, kLds);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_logits<T, PAIRS, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), T::kLdsBytes, st, a);
+  hipLaunchKernelGGL((k_logits<T, PAIRS, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), kLds, st, a);
   LOSS_CHECK();
   return EWS_OK;
 }

@@ -269,8 +269,8 @@ struct Eight {
 };
 
 // A wavefront's block column b of its results, staged through its own part of LDS and handed on as rows of numbers of
-// type W: f(jrow, i, x) gets the results of tile row jrow from tile column i on; float and uint16_t (whole numbers, cut
-// from floats in range) 16 bytes of them, Eight eight floats.
+// type W: f(jrow, i, x) gets the results of tile row jrow from tile column i on; float and uint16_t (65535ths of results
+// held to [0, 1]) 16 bytes of them, Eight eight floats.
 template <class T, typename W, class F>
 __device__ __forceinline__ void rows_of(char* lds, const f32x16 (&acc)[T::TI][T::TJ], int b, F f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -287,7 +287,8 @@ __device__ __forceinline__ void rows_of(char* lds, const f32x16 (&acc)[T::TI][T:
       const int at = r32 * kRow + (a * 32 + g * 8 + half * 4) * (kHalf ? 2 : 4);
       if (kHalf)
         *reinterpret_cast<vec::u32x2*>(stage + at) =
-            vec::u32x2{(uint32_t)x[0] | ((uint32_t)x[1] << 16), (uint32_t)x[2] | ((uint32_t)x[3] << 16)};
+            vec::u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(x[0], x[1])),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(x[2], x[3]))};
       else
         *reinterpret_cast<vec::f32x4*>(stage + at) = x;
     }
