@@ -89,25 +89,39 @@ struct PackArgs {
   uint16_t* dst;           // planes (rows, ld), zero in further columns and in rows up to a multiple of 64
   int64_t ld, plane;
   int dst_rows;
+  int wide;
 };
 
+// A thread takes eight columns of a row; wide: rows of the source start at multiples of 16 bytes.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;
   const int rows = a.map ? a.kept[0] : a.rows;
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-  if (r0 >= rows) return;
-  const int col = threadIdx.x & 63;
-  for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-    const int row = r0 + i;
-    if (row >= a.dst_rows) break;
-    T x = narrow<T>(0.0f);
-    if (row < rows && c0 + col < a.cols)
-      x = ((const T*)a.src)[(int64_t)(a.map ? a.map[row] : row) * a.stride + c0 + col];
-    uint16_t p[NP];
-    planes(x, p);
+  const int padded = (rows + 63) / 64 * 64 < a.dst_rows ? (rows + 63) / 64 * 64 : a.dst_rows;
+  const int packs = (int)(a.ld / 8);
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = at / packs;
+  if (row >= padded) return;
+  const int c0 = (int)(at % packs) * 8;
+  const int n = row >= rows ? 0 : a.cols - c0 < 8 ? a.cols - c0 : 8;
+  T x[8];
+  const T* src = (const T*)a.src + (n > 0 ? (int64_t)(a.map ? a.map[row] : row) * a.stride + c0 : 0);
+  if (a.wide && n == 8) {
 #pragma unroll
-    for (int q = 0; q < NP; ++q) a.dst[q * a.plane + (int64_t)row * a.ld + c0 + col] = p[q];
+    for (int k = 0; k < 8; k += kWide<T>) *reinterpret_cast<u32x4*>(x + k) = *reinterpret_cast<const u32x4*>(src + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = k < n ? src[k] : narrow<T>(0.0f);
+  }
+  uint16_t p[8][NP];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) planes(x[k], p[k]);
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)p[2 * k][q] | ((uint32_t)p[2 * k + 1][q] << 16);
+    *reinterpret_cast<u32x4*>(a.dst + q * a.plane + row * a.ld + c0) = w;
   }
 }
 
@@ -125,39 +139,40 @@ struct PrepareArgs {
   int bias_blocks;
 };
 
-// One workgroup. A thread counts the kept ones of a stretch of rows, the counts are summed, the stretch is written.
+// One workgroup. A wavefront counts the kept ones of a stretch of rows, the counts are summed, the stretch is written.
 __device__ __forceinline__ void keep_rows(const PrepareArgs& a) {
-  __shared__ int wsum[16];
+  __shared__ int counts[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int each = (a.n + 1023) / 1024;
-  const int lo = tid * each < a.n ? tid * each : a.n;
+  const int each = (a.n + 1023) / 1024 * 64;
+  const int lo = wave * each < a.n ? wave * each : a.n;
   const int hi = lo + each < a.n ? lo + each : a.n;
   int m = 0;
-#pragma unroll 4
-  for (int i = lo; i < hi; ++i) m += a.targets[i] != a.ignore;
-  int at = m;
+#pragma unroll 8
+  for (int i = lo + lane; i < hi; i += 64) m += a.targets[i] != a.ignore;
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int up = __shfl_up(at, s);
-    if (lane >= s) at += up;
-  }
-  if (lane == 63) wsum[wave] = at;
-  at -= m;
+  for (int s = 32; s; s >>= 1) m += __shfl_xor(m, s);
+  if (lane == 0) counts[wave] = m;
   __syncthreads();
-  int total = 0;
+  int total = 0, at = 0;
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
-    if (w < wave) at += wsum[w];
-    total += wsum[w];
+    if (w < wave) at += counts[w];
+    total += counts[w];
   }
-  for (int i = lo; i < hi; ++i) {
-    const int64_t t = a.targets[i];
-    if (t != a.ignore) {
-      a.rows.map[at] = i;
-      a.rows.target[at++] = t >= 0 && t < a.vocab ? (int)t : -1;
-    } else if (a.loss_rows) {
+#pragma unroll 4
+  for (int i0 = lo; i0 < hi; i0 += 64) {
+    const int i = i0 + lane;
+    const int64_t t = i < hi ? a.targets[i] : a.ignore;
+    const bool keep = t != a.ignore;
+    const uint64_t kept = __ballot(keep);
+    if (keep) {
+      const int to = at + __popcll(kept & ((1ull << lane) - 1ull));
+      a.rows.map[to] = i;
+      a.rows.target[to] = t >= 0 && t < a.vocab ? (int)t : -1;
+    } else if (i < hi && a.loss_rows) {
       a.loss_rows[i] = 0.0f;
     }
+    at += __popcll(kept);
   }
   if (tid == 0) {
     a.rows.kept[0] = total;
@@ -624,6 +639,9 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   if (s->rows < 1 || s->hidden < 1 || s->vocab < 1 || s->rows > 1 << 22 || s->hidden > 1 << 16 || s->vocab > 1 << 22)
     return EWS_ERR_SHAPE;
   if (s->hidden_stride < s->hidden || s->weight_stride < s->hidden) return EWS_ERR_SHAPE;
+  // a launch has fewer than 2^32 threads, one for eight numbers of either operand
+  const int64_t wide = (s->hidden + 63) / 64 * 64;
+  if (s->rows * wide > (int64_t)1 << 34 || s->vocab * wide > (int64_t)1 << 34) return EWS_ERR_SHAPE;
   p.N = s->rows;
   p.H = s->hidden;
   p.V = s->vocab;
@@ -751,8 +769,10 @@ int launch_grad(Kind kind, const GradArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-int pack(const PackArgs& a, int64_t rows, int64_t cols, hipStream_t st) {
-  hipLaunchKernelGGL((k_pack<T>), dim3(ceil_div(rows, 64), ceil_div(cols, 64)), dim3(256), 0, st, a);
+int pack(PackArgs a, int64_t rows, hipStream_t st) {
+  a.wide = (uintptr_t)a.src % 16 == 0 && a.stride * (int64_t)sizeof(T) % 16 == 0;
+  const int64_t n = rows * (a.ld / 8);  // threads
+  hipLaunchKernelGGL((k_pack<T>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
   LOSS_CHECK();
   return EWS_OK;
 }
@@ -794,7 +814,7 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   x.ld = p.Hp;
   x.plane = p.Np * p.Hp;
   x.dst_rows = (int)p.Np;
-  int rc = f32 ? pack<float>(x, p.Np, p.Hp, c.st) : pack<bf16>(x, p.Np, p.Hp, c.st);
+  int rc = f32 ? pack<float>(x, p.Np, c.st) : pack<bf16>(x, p.Np, c.st);
   if (rc != EWS_OK) return rc;
   if (p.packed) {
     PackArgs w{};
@@ -806,7 +826,7 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
     w.ld = p.Hp;
     w.plane = p.V * p.Hp;
     w.dst_rows = p.V;
-    rc = f32 ? pack<float>(w, p.V, p.Hp, c.st) : pack<bf16>(w, p.V, p.Hp, c.st);
+    rc = f32 ? pack<float>(w, p.V, c.st) : pack<bf16>(w, p.V, c.st);
     if (rc != EWS_OK) return rc;
   }
   return EWS_OK;

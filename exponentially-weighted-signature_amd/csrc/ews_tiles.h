@@ -252,16 +252,29 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
 }
 
 // Tile coordinates of a workgroup. Consecutive workgroups go to the eight XCDs in turn; each XCD gets a contiguous
-// stretch of tiles, walked in groups of eight j so that the tiles in flight on one XCD share rows in its L2.
+// stretch of tiles, walked in groups of up to eight j, as equal as can be, so that the tiles in flight on one XCD share
+// rows in its L2 (41 j in five groups of eight and one of one: 0.83 PFLOP/s where 32 in four reach 1.06).
 __device__ __forceinline__ void tile_of(int id, int ti, int tj, int& i, int& j) {
   const int n = ti * tj, xcd = id & 7, at = id >> 3;
   const int each = n >> 3, more = n & 7;
   id = xcd * each + (xcd < more ? xcd : more) + at;
-  const int group = id / (8 * ti);
-  const int rest = id - group * 8 * ti;
-  const int width = tj - group * 8 < 8 ? tj - group * 8 : 8;
+  const int groups = (tj + 7) >> 3;
+  const int wide = tj / groups, wider = tj % groups;  // the first `wider` groups have one j more
+  const int split = wider * (wide + 1) * ti;
+  int group, rest, width;
+  if (id < split) {
+    width = wide + 1;
+    group = id / (width * ti);
+    rest = id - group * width * ti;
+    j = group * width;
+  } else {
+    width = wide;
+    group = (id - split) / (width * ti);
+    rest = id - split - group * width * ti;
+    j = wider * (wide + 1) + group * width;
+  }
   i = rest / width;
-  j = group * 8 + rest % width;
+  j += rest % width;
 }
 
 struct Eight {
