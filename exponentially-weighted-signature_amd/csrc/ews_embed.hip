@@ -7,13 +7,15 @@
 // token (stable, so a token's rows are added in the order of the text) and sums runs of equal tokens, in float32,
 // rounding each row of dW once. The same inputs give the same bits.
 //
-//   k_sort   a workgroup owns a range of the vocabulary, reads every token twice (the ids stay in L2) and writes the
-//            sorted positions of its own ones: counts first, then the places. No workgroup waits for another.
-//   k_runs   a wavefront takes kRun sorted positions and one column tile, whatever tokens they are, so a frequent
-//            token costs no more than rare ones: rows of runs that lie inside are written, the ends of runs that go on
-//            in a neighbour's positions are kept as float32 partial rows.
-//   k_join   adds the partial rows of the runs that were cut, in order.
-//   k_absent zeroes the rows of dW without a token.
+//   k_sort   the vocabulary is dealt to the workgroups one token at a time (frequent tokens are often neighbours). Each
+//            looks through all the tokens (the ids stay in L2): its wavefronts count their own stretch's own tokens and
+//            list them in LDS; from the counts every wavefront knows where its first one of each token goes. No
+//            workgroup waits for another.
+//   k_runs   a wavefront takes a run of sorted positions and one column tile, whatever tokens they are, so a frequent
+//            token costs no more than rare ones: rows of tokens that lie inside are written, the ends of tokens that go
+//            on in a neighbour's positions are kept as float32 partial rows. Further workgroups of the same launch zero
+//            the rows of dW without a token.
+//   k_join   adds the partial rows of the tokens that were cut, in order.
 //
 // An id outside [0, vocab) reads nothing: its output row is NaN and it has no gradient.
 #include <hip/hip_runtime.h>
@@ -28,16 +30,18 @@ using namespace ews::vec;
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kPerThread = 4;                        // consecutive tokens a thread reads at a time
-constexpr int kPiece = kSortThreads * kPerThread;    // tokens a workgroup looks through at a time
-constexpr int kMaxRange = 1024;                      // vocabulary entries a workgroup of k_sort may own
-constexpr int kRun = 32;                             // sorted positions a wavefront of k_runs adds up
+constexpr int kListed = 640;      // own tokens a wavefront lists: of 131071, 32 where all are alike rare
+constexpr int kMaxRange = 512;    // vocabulary entries a workgroup of k_sort may own
 constexpr int kJoinWaves = 4;
+constexpr int kFewRows = 16;
 
 struct Args {
   int64_t n, stride, pad;
-  int H, V, R;     // R: vocabulary entries per workgroup of k_sort
+  int H, V;
+  int deal, range; // token t is entry t >> deal of workgroup t % 2^deal of k_sort, which owns 2^range: slot (group, entry)
   int lanes;       // lanes a row of the lookup is spread over
+  int run;         // sorted positions a wavefront of k_runs adds up
+  int runs, tiles; // how many there are, and column tiles of a row
   float scale;
   const void* tokens;
   const void* weight;
@@ -45,8 +49,8 @@ struct Args {
   const void* gout;
   void* gweight;
   int* order;      // (n) positions, sorted by token
-  int* sorted;     // (n) their tokens
-  int* start;      // (V + 1) first sorted position of every token; start[V]: positions that count
+  int* sorted;     // (n) their tokens' slots
+  int* start;      // (slots + 1) first sorted position of every slot; the last: positions that count
   float* part;     // (runs, 2, H) sums of the runs cut at a wavefront's first and last position
 };
 
@@ -72,39 +76,80 @@ __global__ __launch_bounds__(256) void k_lookup(Args a) {
   }
 }
 
-template <typename Tok>
-__device__ __forceinline__ int local_id(const Tok* tokens, int64_t i, int64_t n, int64_t lo, int64_t hi, int64_t pad,
-                                        int64_t vocab, int& below) {
-  if (i >= n) return -1;
-  const int64_t t = (int64_t)tokens[i];
-  if (t < 0 || t >= vocab || t == pad) return -1;
-  if (t < lo) ++below;
-  return (t >= lo && t < hi) ? (int)(t - lo) : -1;
+// A token that counts, or kNone.
+constexpr uint32_t kNone = ~0u;
+__device__ __forceinline__ uint32_t counted(int64_t t, const Args& a) {
+  return (uint64_t)t < (uint64_t)a.V && t != a.pad ? (uint32_t)t : kNone;
+}
+
+__device__ __forceinline__ int token_of(const Args& a, int slot) {
+  return (slot & ((1 << a.range) - 1)) << a.deal | slot >> a.range;
+}
+
+// Places 64 positions of own tokens (entry < 0: none); equal tokens keep their order.
+__device__ __forceinline__ void place(const Args& a, int entry, int position, int* next) {
+  const int lane = threadIdx.x & 63;
+  uint64_t left = __ballot(entry >= 0);
+  while (left) {
+    const int leader = __ffsll((unsigned long long)left) - 1;
+    const int one = __builtin_amdgcn_readlane(entry, leader);
+    const uint64_t same = __ballot(entry == one);
+    const int first = next[one];
+    if (entry == one) {
+      const int to = first + __popcll(same & ((1ull << lane) - 1ull));
+      a.order[to] = position;
+      a.sorted[to] = ((int)blockIdx.x << a.range) + entry;
+    }
+    if (lane == leader) next[one] = first + __popcll(same);
+    left &= ~same;
+  }
 }
 
 template <typename Tok>
 __global__ __launch_bounds__(kSortThreads) void k_sort(Args a) {
-  __shared__ int cnt[kMaxRange];             // occurrences, then the next free place, of every own token
+  __shared__ int next[kSortWaves][kMaxRange];    // a wavefront's occurrences, then its next place, of every own token
+  __shared__ int pos[kSortWaves][kListed];       // own positions, in the order of the text
+  __shared__ uint16_t ids[kSortWaves][kListed];
   __shared__ int wsum[kSortWaves];
-  __shared__ int lpos[kPiece];               // own positions of a piece, in the order of the text
-  __shared__ uint16_t lid[kPiece];
   __shared__ int base;
   const Tok* tokens = (const Tok*)a.tokens;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t lo = (int64_t)blockIdx.x * a.R;
-  const int64_t hi = lo + a.R < a.V ? lo + a.R : a.V;
-  const int range = (int)(hi - lo);
-  for (int i = tid; i < range; i += kSortThreads) cnt[i] = 0;
+  const uint32_t group = blockIdx.x, mask = (1u << a.deal) - 1u;
+  const int range = 1 << a.range;
+  for (int i = tid; i < kSortWaves * range; i += kSortThreads) next[i >> a.range][i & (range - 1)] = 0;
   if (tid == 0) base = 0;
   __syncthreads();
 
-  // how often each own token occurs, and how many positions the smaller tokens take
-  int below = 0;
-  for (int64_t p0 = 0; p0 < a.n; p0 += kPiece) {
+  // a wavefront looks through a stretch of the text: how often each own token occurs, how many tokens go to smaller
+  // groups, and where its own ones are, as far as its list goes
+  const int64_t each = (a.n + kSortThreads - 1) / kSortThreads * 64;
+  const int64_t from = wave * each, to = from + each < a.n ? from + each : a.n;
+  int below = 0, m = 0;
+  constexpr int kAhead = 8;
+  for (int64_t i0 = from; i0 < to; i0 += 64 * kAhead) {
+    Tok t[kAhead];
 #pragma unroll
-    for (int q = 0; q < kPerThread; ++q) {
-      const int id = local_id(tokens, p0 + (int64_t)q * kSortThreads + tid, a.n, lo, hi, a.pad, a.V, below);
-      if (id >= 0) atomicAdd(&cnt[id], 1);
+    for (int q = 0; q < kAhead; ++q) {
+      const int64_t i = i0 + 64 * q + lane;
+      t[q] = i < to ? tokens[i] : (Tok)-1;
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const uint32_t x = counted(t[q], a);
+      below += (x & mask) < group && x != kNone;
+      const bool own = (x & mask) == group && x != kNone;
+      const uint64_t mine = __ballot(own);
+      if (!mine) continue;
+      const int at = m + __popcll(mine & ((1ull << lane) - 1ull));
+      if (own) {
+        const int entry = (int)(x >> a.deal);
+        atomicAdd(&next[wave][entry], 1);
+        if (at < kListed) {
+          pos[wave][at] = (int)(i0 + 64 * q + lane);
+          ids[wave][at] = (uint16_t)entry;
+        }
+      }
+      m += __popcll(mine);
     }
   }
 #pragma unroll
@@ -112,9 +157,11 @@ __global__ __launch_bounds__(kSortThreads) void k_sort(Args a) {
   if (lane == 0) atomicAdd(&base, below);
   __syncthreads();
 
-  // the first place of every own token (exclusive sums of the counts; range <= kMaxRange = one per thread)
-  const int mine = tid < range ? cnt[tid] : 0;
-  int incl = mine;
+  // every wavefront's first place of every own token: by token, then by wavefront (one thread a token)
+  int count = 0;
+  if (tid < range)
+    for (int w = 0; w < kSortWaves; ++w) count += next[w][tid];
+  int incl = count;
 #pragma unroll
   for (int s = 1; s < 64; s <<= 1) {
     const int up = __shfl_up(incl, s);
@@ -122,100 +169,94 @@ __global__ __launch_bounds__(kSortThreads) void k_sort(Args a) {
   }
   if (lane == 63) wsum[wave] = incl;
   __syncthreads();
-  int first = base + incl - mine;
-  for (int w = 0; w < wave; ++w) first += wsum[w];
   if (tid < range) {
-    cnt[tid] = first;
-    a.start[lo + tid] = first;
-    if (lo + tid == a.V - 1) a.start[a.V] = first + mine;
+    int first = base + incl - count;
+    for (int w = 0; w < wave; ++w) first += wsum[w];
+    a.start[group * range + tid] = first;
+    if (group == mask && tid == range - 1) a.start[(group + 1) * range] = first + count;
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int k = next[w][tid];
+      next[w][tid] = first;
+      first += k;
+    }
   }
   __syncthreads();
 
-  for (int64_t p0 = 0; p0 < a.n; p0 += kPiece) {
-    int ids[kPerThread], m = 0, unused = 0;
-    const int64_t i0 = p0 + (int64_t)tid * kPerThread;
+  if (m <= kListed) {
+    for (int l = lane; l - lane < m; l += 64)
+      place(a, l < m ? (int)ids[wave][l] : -1, l < m ? pos[wave][l] : 0, next[wave]);
+    return;
+  }
+  for (int64_t i0 = from; i0 < to; i0 += 64 * kAhead) {  // more than its list holds: the stretch again
+    Tok t[kAhead];
 #pragma unroll
-    for (int q = 0; q < kPerThread; ++q) {
-      ids[q] = local_id(tokens, i0 + q, a.n, lo, hi, a.pad, a.V, unused);
-      m += ids[q] >= 0;
-    }
-    int at = m;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int up = __shfl_up(at, s);
-      if (lane >= s) at += up;
-    }
-    if (lane == 63) wsum[wave] = at;
-    at -= m;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      if (w < wave) at += wsum[w];
-      total += wsum[w];
+    for (int q = 0; q < kAhead; ++q) {
+      const int64_t i = i0 + 64 * q + lane;
+      t[q] = i < to ? tokens[i] : (Tok)-1;
     }
 #pragma unroll
-    for (int q = 0; q < kPerThread; ++q)
-      if (ids[q] >= 0) {
-        lpos[at] = (int)(i0 + q);
-        lid[at] = (uint16_t)ids[q];
-        ++at;
-      }
-    __syncthreads();
-    // tokens are dealt to the wavefronts, so a token's next place has one owner; equal tokens of 64 keep their order
-    for (int l0 = 0; l0 < total; l0 += 64) {
-      const int l = l0 + lane;
-      const int id = l < total ? (int)lid[l] : -1;
-      uint64_t left = __ballot(id >= 0 && id % kSortWaves == wave);
-      while (left) {
-        const int leader = __ffsll((unsigned long long)left) - 1;
-        const int same_id = __shfl(id, leader);
-        const uint64_t same = __ballot(id == same_id);
-        const int place = cnt[same_id];
-        if (id == same_id) {
-          const int rank = __popcll(same & ((1ull << lane) - 1ull));
-          a.order[place + rank] = lpos[l];
-          a.sorted[place + rank] = (int)lo + id;
-        }
-        if (lane == leader) cnt[same_id] = place + __popcll(same);
-        left &= ~same;
-      }
+    for (int q = 0; q < kAhead; ++q) {
+      const uint32_t x = counted(t[q], a);
+      const bool own = (x & mask) == group && x != kNone;
+      place(a, own ? (int)(x >> a.deal) : -1, (int)(i0 + 64 * q + lane), next[wave]);
     }
-    __syncthreads();
   }
 }
 
 template <typename T, int V>
+__device__ __forceinline__ void zero_absent(const Args& a, int v, int col) {
+  if (v >= a.V || col >= a.H) return;
+  const int slot = ((v & ((1 << a.deal) - 1)) << a.range) + (v >> a.deal);
+  if (a.start[slot] != a.start[slot + 1]) return;
+  float x[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = 0.0f;
+  Pack<T, V> z;
+  z.set(x);
+  z.store((T*)a.gweight + (int64_t)v * a.H + col);
+}
+
+template <typename T, int V>
 __global__ __launch_bounds__(256) void k_runs(Args a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t run = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int col = ((int)blockIdx.y * 64 + lane) * V;
-  const int total = a.start[a.V];
-  const int64_t b = run * kRun;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // a row's column tiles are neighbours; run and tile are scalar, so positions and tokens are scalar loads
+  const int unit = (int)blockIdx.x * 4 + wave, run = unit / a.tiles;
+  const int col = ((unit - run * a.tiles) * 64 + lane) * V;
+  if (run >= a.runs) return zero_absent<T, V>(a, run - a.runs, col);
+  const int total = a.start[1 << (a.deal + a.range)];
+  const int64_t b = (int64_t)run * a.run;
   if (b >= total) return;
-  const int j0 = (int)b, j1 = j0 + kRun < total ? j0 + kRun : total;
+  const int j0 = (int)b, j1 = j0 + a.run < total ? j0 + a.run : total;
   const bool in = col < a.H;
   const T* g = (const T*)a.gout + (in ? col : 0);
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.0f;
   constexpr int kAhead = 8;
-  for (int j = j0; j < j1; j += kAhead) {
-    Pack<T, V> p[kAhead];
+  Pack<T, V> p[kAhead];
+  auto fetch = [&](int j) {
+    if (j + kAhead <= j1) {
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
-      const int jj = j + q < j1 ? j + q : j1 - 1;
-      p[q].load(g + (int64_t)a.order[jj] * a.H);
+      for (int q = 0; q < kAhead; ++q) p[q].load(g + (int64_t)a.order[j + q] * a.H);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) p[q].load(g + (int64_t)a.order[j + q < j1 ? j + q : j1 - 1] * a.H);
     }
+  };
+  int t = a.sorted[j0];
+  for (int j = j0; j < j1; j += kAhead) {
+    fetch(j);
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       if (j + q >= j1) break;
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] += p[q].get(i);
-      const int t = a.sorted[j + q];
-      const bool last = j + q + 1 == j1;
-      if (!last && a.sorted[j + q + 1] == t) continue;
-      const int s0 = a.start[t], s1 = a.start[t + 1];
+      const int now = t;
+      if (j + q + 1 < j1) {
+        t = a.sorted[j + q + 1];
+        if (t == now) continue;
+      }
+      const int s0 = a.start[now], s1 = a.start[now + 1];
       if (in) {
         if (s0 >= j0 && s1 <= j1) {
           Pack<T, V> o;
@@ -223,9 +264,9 @@ __global__ __launch_bounds__(256) void k_runs(Args a) {
 #pragma unroll
           for (int i = 0; i < V; ++i) x[i] = acc[i] * a.scale;
           o.set(x);
-          o.store((T*)a.gweight + (int64_t)t * a.H + col);
+          o.store((T*)a.gweight + (int64_t)token_of(a, now) * a.H + col);
         } else {
-          float* part = a.part + (run * 2 + (s0 < j0 ? 0 : 1)) * a.H + col;
+          float* part = a.part + ((int64_t)run * 2 + (s0 < j0 ? 0 : 1)) * a.H + col;
 #pragma unroll
           for (int i = 0; i < V; ++i) part[i] = acc[i];
         }
@@ -236,53 +277,77 @@ __global__ __launch_bounds__(256) void k_runs(Args a) {
   }
 }
 
-// One workgroup per run of kRun positions and 64 columns; only those whose last token starts in them and goes on work.
-// The wavefronts add contiguous quarters of the partial rows, the first one joins them.
-template <typename T>
+// One workgroup per run; only those whose last token starts in them and goes on work. A token of few partial rows: the
+// wavefronts take a column tile each. One of many: they add a contiguous part of its rows each, one tile after another,
+// and the first one joins them.
+template <typename T, int V>
 __global__ __launch_bounds__(64 * kJoinWaves) void k_join(Args a) {
-  __shared__ float sums[kJoinWaves][64];
-  const int total = a.start[a.V];
+  __shared__ float sums[kJoinWaves][64][V];
+  const int total = a.start[1 << (a.deal + a.range)];
   const int64_t run = blockIdx.x;
-  const int64_t b = run * kRun;
+  const int64_t b = run * a.run;
   if (b >= total) return;
-  const int j0 = (int)b, j1 = j0 + kRun < total ? j0 + kRun : total;
+  const int j0 = (int)b, j1 = j0 + a.run < total ? j0 + a.run : total;
   const int t = a.sorted[j1 - 1];
   const int s0 = a.start[t], s1 = a.start[t + 1];
   if (s0 < j0 || s1 <= j1) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t last = (int64_t)(s1 - 1) / kRun;  // the last run that holds the token
-  const int64_t per = (last - run + kJoinWaves - 1) / kJoinWaves;
-  const int64_t c0 = run + 1 + wave * per;
-  const int64_t c1 = c0 + per < last + 1 ? c0 + per : last + 1;
-  for (int col0 = blockIdx.y * 64; col0 < a.H; col0 += gridDim.y * 64) {
-    const int col = col0 + lane;
-    float s = 0.0f;
-    if (col < a.H) {
-      if (wave == 0) s = a.part[(run * 2 + 1) * a.H + col];
-#pragma unroll 8
-      for (int64_t c = c0; c < c1; ++c) s += a.part[c * 2 * a.H + col];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, token = token_of(a, t);
+  const int rows = (int)((s1 - 1) / a.run - run);  // partial rows of the runs after this one
+  const float* own = a.part + (run * 2 + 1) * a.H;
+  const float* next = a.part + (run + 1) * 2 * a.H;
+  auto add = [&](float (&s)[V], int c0, int c1, int col) {
+#pragma unroll 16
+    for (int c = c0; c < c1; ++c) {
+      Pack<float, V> x;
+      x.load(next + (int64_t)c * 2 * a.H + col);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += x.get(i);
     }
-    sums[wave][lane] = s;
+  };
+  auto finish = [&](const float (&s)[V], int col) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) ((T*)a.gweight)[(int64_t)token * a.H + col + i] = narrow<T>(s[i] * a.scale);
+  };
+  if (rows <= kFewRows) {
+    const int col = ((blockIdx.y * kJoinWaves + wave) * 64 + lane) * V;
+    if (col >= a.H) return;
+    float s[V];
+    Pack<float, V> x;
+    x.load(own + col);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = x.get(i);
+    add(s, 0, rows, col);
+    finish(s, col);
+    return;
+  }
+  const int per = (rows + kJoinWaves - 1) / kJoinWaves;
+  const int c0 = wave * per, c1 = c0 + per < rows ? c0 + per : rows;
+  for (int tile = 0; tile < kJoinWaves; ++tile) {
+    const int col = ((blockIdx.y * kJoinWaves + tile) * 64 + lane) * V;
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = 0.0f;
+    if (col < a.H) {
+      if (wave == 0) {
+        Pack<float, V> x;
+        x.load(own + col);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] = x.get(i);
+      }
+      add(s, c0, c1, col);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[wave][lane][i] = s[i];
     __syncthreads();
     if (wave == 0 && col < a.H) {
-      for (int w = 1; w < kJoinWaves; ++w) s += sums[w][lane];
-      ((T*)a.gweight)[(int64_t)t * a.H + col] = narrow<T>(s * a.scale);
+#pragma unroll
+      for (int w = 1; w < kJoinWaves; ++w)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += sums[w][lane][i];
+      finish(s, col);
     }
     __syncthreads();
   }
-}
-
-template <typename T, int V>
-__global__ __launch_bounds__(256) void k_absent(Args a) {
-  const int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (v >= a.V || a.start[v] != a.start[v + 1]) return;
-  float x[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) x[i] = 0.0f;
-  Pack<T, V> z;
-  z.set(x);
-  T* row = (T*)a.gweight + v * a.H;
-  for (int c = (threadIdx.x & 63) * V; c < a.H; c += 64 * V) z.store(row + c);
 }
 
 }  // namespace embed
@@ -294,7 +359,7 @@ using namespace ews::embed;
 
 struct EPlan {
   int64_t runs;
-  int groups, R;
+  int deal, range, run;
   size_t order, sorted, start, part, total;
 };
 
@@ -308,16 +373,20 @@ int embed_plan(const ews_embed_desc* s, EPlan& p) {
   if (s->count < 1 || s->count > 1 << 25 || s->width < 1 || s->vocab < 1) return EWS_ERR_SHAPE;
   if (s->width > 1 << 20 || s->vocab > 1 << 25 || s->weight_stride < s->width) return EWS_ERR_SHAPE;
   // one workgroup of k_sort per CU where the vocabulary allows it; each reads all the ids
-  int groups = s->vocab < 256 ? s->vocab : 256;
-  const int least = (s->vocab + kMaxRange - 1) / kMaxRange;
-  if (groups < least) groups = least;
-  p.R = (s->vocab + groups - 1) / groups;
-  p.groups = (s->vocab + p.R - 1) / p.R;
-  p.runs = (s->count + kRun - 1) / kRun;
+  p.deal = 0;
+  while (p.deal < 8 && (1 << p.deal) < s->vocab) ++p.deal;
+  while (s->vocab > (int64_t)kMaxRange << p.deal) ++p.deal;
+  p.range = 0;
+  while (s->vocab > (int64_t)1 << (p.deal + p.range)) ++p.range;
+  // long runs cut few tokens, but two thousand wavefronts keep the memory busy
+  const int64_t tiles = (s->width + (s->dtype == EWS_DTYPE_F32 ? 255 : 511)) / (s->dtype == EWS_DTYPE_F32 ? 256 : 512);
+  p.run = 32;
+  while (p.run > 8 && s->count / p.run * tiles < 2048) p.run /= 2;
+  p.runs = (s->count + p.run - 1) / p.run;
   size_t off = 0;
   p.order = off; off += al256e((size_t)s->count * 4);
   p.sorted = off; off += al256e((size_t)s->count * 4);
-  p.start = off; off += al256e(((size_t)s->vocab + 1) * 4);
+  p.start = off; off += al256e((((size_t)1 << (p.deal + p.range)) + 1) * 4);
   p.part = off; off += al256e((size_t)p.runs * 2 * s->width * 4);
   p.total = off;
   return EWS_OK;
@@ -354,14 +423,18 @@ int launch_lookup(const ews_embed_desc* s, Args a, hipStream_t st) {
 }
 
 template <typename T, int V>
-int launch_sums(const EPlan& p, const Args& a, hipStream_t st) {
-  const int tiles = (a.H + 64 * V - 1) / (64 * V);
-  hipLaunchKernelGGL((k_runs<T, V>), dim3((uint32_t)((p.runs + 3) / 4), tiles), dim3(256), 0, st, a);
+int launch_sums(const EPlan& p, Args a, hipStream_t st) {
+  a.tiles = (a.H + 64 * V - 1) / (64 * V);
+  const int64_t units = (p.runs + a.V) * a.tiles;
+  if (units > ((int64_t)1 << 26) - 4) return EWS_ERR_SHAPE;  // a launch has fewer than 2^32 threads
+  hipLaunchKernelGGL((k_runs<T, V>), dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, st, a);
   if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH;
-  const int ctiles = (a.H + 63) / 64;
-  hipLaunchKernelGGL((k_join<T>), dim3((uint32_t)p.runs, ctiles < 64 ? ctiles : 64), dim3(64 * kJoinWaves), 0, st, a);
-  if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH;
-  hipLaunchKernelGGL((k_absent<T, V>), dim3((uint32_t)((a.V + 3) / 4)), dim3(256), 0, st, a);
+  const int v = a.H % 4 == 0 ? 4 : 1;  // partial rows that start at multiples of 16 bytes
+  const dim3 grid((uint32_t)p.runs, (a.H + 64 * v * kJoinWaves - 1) / (64 * v * kJoinWaves));
+  if (v == 4)
+    hipLaunchKernelGGL((k_join<T, 4>), grid, dim3(64 * kJoinWaves), 0, st, a);
+  else
+    hipLaunchKernelGGL((k_join<T, 1>), grid, dim3(64 * kJoinWaves), 0, st, a);
   return hipGetLastError() == hipSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
@@ -402,16 +475,19 @@ int ews_embed_backward(const ews_embed_desc* desc, const void* tokens, const voi
   a.tokens = tokens;
   a.gout = grad_out;
   a.gweight = grad_weight;
-  a.R = p.R;
+  a.deal = p.deal;
+  a.range = p.range;
+  a.run = p.run;
+  a.runs = (int)p.runs;
   a.order = (int*)(w + p.order);
   a.sorted = (int*)(w + p.sorted);
   a.start = (int*)(w + p.start);
   a.part = (float*)(w + p.part);
   hipStream_t st = (hipStream_t)stream;
   if (desc->token_bytes == 8)
-    hipLaunchKernelGGL((k_sort<int64_t>), dim3(p.groups), dim3(kSortThreads), 0, st, a);
+    hipLaunchKernelGGL((k_sort<int64_t>), dim3(1u << p.deal), dim3(kSortThreads), 0, st, a);
   else
-    hipLaunchKernelGGL((k_sort<int32_t>), dim3(p.groups), dim3(kSortThreads), 0, st, a);
+    hipLaunchKernelGGL((k_sort<int32_t>), dim3(1u << p.deal), dim3(kSortThreads), 0, st, a);
   if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH;
   const bool wide = rows_aligned(desc, grad_out, grad_weight, desc->width);
   if (desc->dtype == EWS_DTYPE_F32)

@@ -459,6 +459,7 @@ __global__ __launch_bounds__(256) void k_dbias(const float* part, int parts, int
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= vocab) return;
   float s = 0.0f;
+#pragma unroll 8
   for (int p = 0; p < parts; ++p) s += part[p * ld + v];
   s = (factor ? s * factor[0] : s) + (add ? sum[v] : 0.0f);
   if (out)
@@ -557,6 +558,7 @@ __global__ __launch_bounds__(256) void k_reduce(GradArgs a) {
   const int i = (int)(at % packs) * 8;
   const int n = a.I - i < 8 ? a.I - i : 8;
   float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
     const float* p = a.part + ((int64_t)s * rows + j) * a.I + i;
 #pragma unroll

@@ -9,7 +9,7 @@ import math
 import torch
 
 from . import _native as nat
-from .embed import DTYPES, check_tensor, on_device
+from .embed import DTYPES, check_tensor, launch
 
 
 def _dense(t):
@@ -34,12 +34,13 @@ def _tables(tensors, outs):
 
 
 def _check(tensors):
+    dev = tensors[0].device
     for t in tensors:
-        if t.layout != torch.strided:
-            raise TypeError(f"gradients must be dense tensors, got layout {t.layout}")
-        check_tensor("every gradient", t)
-        if t.device != tensors[0].device:
-            raise ValueError(f"gradients are on {tensors[0].device} and {t.device}")
+        if t.dtype not in DTYPES or not t.is_cuda or t.layout is not torch.strided or t.device != dev:
+            if t.layout is not torch.strided:
+                raise TypeError(f"gradients must be dense tensors, got layout {t.layout}")
+            check_tensor("every gradient", t)
+            raise ValueError(f"gradients are on {dev} and {t.device}")
 
 
 def _norm_and_scale(tensors, outs, max_norm):
@@ -53,9 +54,8 @@ def _norm_and_scale(tensors, outs, max_norm):
     n, ptrs, out, counts, types = _tables(src, dst)
     result = torch.empty(2, device=dev, dtype=torch.float32)
     ws = torch.empty(int(lib.ews_clip_workspace_bytes(n, counts)), device=dev, dtype=torch.uint8)
-    with on_device(dev):
-        nat.check(lib.ews_clip(n, ptrs, out, counts, types, max_norm, 0 if outs is None else 1, result.data_ptr(),
-                               ws.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "ews_clip")
+    nat.check(launch(dev, lib.ews_clip, n, ptrs, out, counts, types, max_norm, 0 if outs is None else 1,
+                     result.data_ptr(), ws.data_ptr()), "ews_clip")
     for o, d in zip(outs if outs is not None else (), dst):
         if o is not d:
             o.copy_(d)
@@ -68,9 +68,7 @@ def scale_tensors(tensors, factor):
         return
     dev = tensors[0].device
     n, ptrs, out, counts, types = _tables(tensors, tensors)
-    with on_device(dev):
-        nat.check(nat.load().ews_scale(n, ptrs, out, counts, types, factor.data_ptr(),
-                                       torch.cuda.current_stream(dev).cuda_stream), "ews_scale")
+    nat.check(launch(dev, nat.load().ews_scale, n, ptrs, out, counts, types, factor.data_ptr()), "ews_scale")
 
 
 def _max_norm(max_norm):

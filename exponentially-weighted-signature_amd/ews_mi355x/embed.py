@@ -3,9 +3,6 @@
 
 from __future__ import annotations
 
-import contextlib
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -15,9 +12,12 @@ DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16}
 _NO_PADDING = -1
 
 
-def on_device(dev):
-    """A context in which launches go to dev (nothing where it is the current device)."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def launch(dev, fn, *args):
+    """fn(*args, stream) on dev's current stream, with dev the current device."""
+    if dev.index == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
 
 
 def check_tensor(name, t):
@@ -40,19 +40,13 @@ def _desc(tokens, weight, stride, scale, padding):
                          tokens.element_size(), scale)
 
 
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
 def _lookup(tokens, weight, scale, padding):
     out = torch.empty((*tokens.shape, weight.shape[1]), device=weight.device, dtype=weight.dtype)
     if tokens.numel() == 0:
         return out
     weight, stride = row_major(weight)
-    with on_device(weight.device):
-        nat.check(nat.load().ews_embed_forward(_desc(tokens, weight, stride, scale, padding), tokens.data_ptr(),
-                                               weight.data_ptr(), out.data_ptr(), _stream(weight.device)),
-                  "ews_embed_forward")
+    nat.check(launch(weight.device, nat.load().ews_embed_forward, _desc(tokens, weight, stride, scale, padding),
+                     tokens.data_ptr(), weight.data_ptr(), out.data_ptr()), "ews_embed_forward")
     return out
 
 
@@ -75,9 +69,8 @@ class _Lookup(torch.autograd.Function):
         gout = gout.contiguous()
         desc = _desc(tokens, grad, shape[1], scale, padding)
         ws = torch.empty(int(lib.ews_embed_workspace_bytes(desc)), device=gout.device, dtype=torch.uint8)
-        with on_device(gout.device):
-            nat.check(lib.ews_embed_backward(desc, tokens.data_ptr(), gout.data_ptr(), grad.data_ptr(), ws.data_ptr(),
-                                             _stream(gout.device)), "ews_embed_backward")
+        nat.check(launch(gout.device, lib.ews_embed_backward, desc, tokens.data_ptr(), gout.data_ptr(),
+                         grad.data_ptr(), ws.data_ptr()), "ews_embed_backward")
         return grad, None, None, None
 
 

@@ -8,7 +8,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from .clip import scale_tensors
-from .embed import DTYPES, check_tensor, on_device, row_major
+from .embed import DTYPES, check_tensor, launch, row_major
 
 
 def _desc(hidden, hs, weight, wst, bias, ignore_index, reduction):
@@ -38,15 +38,13 @@ def _run(hidden, weight, bias, targets, ignore_index, reduction, needs, upstream
     desc = _desc(hidden, hs, weight, wst, bias, ignore_index, reduction)
     train = any(needs)
     ws = torch.empty(int(lib.ews_loss_workspace_bytes(desc, int(train))), device=dev, dtype=torch.uint8)
-    with on_device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if train:
-            nat.check(lib.ews_loss_train(desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias), targets.data_ptr(),
-                                         _ptr(upstream), _ptr(loss), *(_ptr(g) for g in grads), ws.data_ptr(), stream),
-                      "ews_loss_train")
-        else:
-            nat.check(lib.ews_loss_forward(desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias), targets.data_ptr(),
-                                           loss.data_ptr(), ws.data_ptr(), stream), "ews_loss_forward")
+    if train:
+        nat.check(launch(dev, lib.ews_loss_train, desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias),
+                         targets.data_ptr(), _ptr(upstream), _ptr(loss), *(_ptr(g) for g in grads), ws.data_ptr()),
+                  "ews_loss_train")
+    else:
+        nat.check(launch(dev, lib.ews_loss_forward, desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias),
+                         targets.data_ptr(), loss.data_ptr(), ws.data_ptr()), "ews_loss_forward")
     return loss, grads
 
 
