@@ -94,12 +94,11 @@ struct PackArgs {
 
 // A thread takes eight columns of a row; wide: rows of the source start at multiples of 16 bytes.
 template <typename T>
-__global__ __launch_bounds__(256) void k_pack(PackArgs a) {
+__device__ __forceinline__ void pack_eight(const PackArgs& a, int64_t at) {
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;
   const int rows = a.map ? a.kept[0] : a.rows;
   const int padded = (rows + 63) / 64 * 64 < a.dst_rows ? (rows + 63) / 64 * 64 : a.dst_rows;
   const int packs = (int)(a.ld / 8);
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = at / packs;
   if (row >= padded) return;
   const int c0 = (int)(at % packs) * 8;
@@ -125,6 +124,11 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs a) {
   }
 }
 
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack(PackArgs a) {
+  pack_eight<T>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
+}
+
 // ------------------------------------------------------------------------------------------------------ preparation
 struct PrepareArgs {
   const int64_t* targets;
@@ -136,7 +140,9 @@ struct PrepareArgs {
   int bias_bf16;
   float* bias_out;         // (padded)
   void* grad_hidden;       // or null: the ignored rows' zeros
-  int bias_blocks;
+  int bias_blocks, ignored_blocks;
+  PackArgs weight;         // packed by the further workgroups
+  PackArgs few;            // the hidden rows, where the first workgroup packs them too; dst null: k_pack does
 };
 
 // One workgroup. A wavefront counts the kept ones of a stretch of rows, the counts are summed, the stretch is written.
@@ -193,13 +199,23 @@ __device__ __forceinline__ void scale_bias(const PrepareArgs& a, int v) {
   a.bias_out[v] = b;
 }
 
-// What needs nothing of the others, in one launch: the first workgroup lists the kept rows, some write the bias, the
-// others (16 rows each) zero the ignored rows of dh.
+// What needs nothing of the others, in one launch: the first workgroup lists the kept rows (and packs a few), some write
+// the bias, some (16 rows each) zero the ignored rows of dh, the others pack W where it is not read as it is.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_prepare(PrepareArgs a) {
-  if (blockIdx.x == 0) return keep_rows(a);
+  if (blockIdx.x == 0) {
+    keep_rows(a);
+    if (!a.few.dst) return;
+    __threadfence_block();
+    __syncthreads();  // the list is this workgroup's own
+    const int64_t packs = (int64_t)a.few.dst_rows * (a.few.ld / 8);
+    for (int64_t at = threadIdx.x; at < packs; at += 1024) pack_eight<T>(a.few, at);
+    return;
+  }
   const int b = blockIdx.x - 1;
   if (b < a.bias_blocks) return scale_bias(a, b * 1024 + threadIdx.x);
+  if (b >= a.bias_blocks + a.ignored_blocks)
+    return pack_eight<T>(a.weight, (int64_t)(b - a.bias_blocks - a.ignored_blocks) * 1024 + threadIdx.x);
   const int row = (b - a.bias_blocks) * 16 + (threadIdx.x >> 6);
   if (row >= a.n || a.targets[row] != a.ignore) return;
   for (int c = threadIdx.x & 63; c < a.H; c += 64) ((T*)a.grad_hidden)[(int64_t)row * a.H + c] = narrow<T>(0.0f);
@@ -343,21 +359,24 @@ __global__ __launch_bounds__(1024) void k_join(Stats st, Rows rows, int slabs, i
   if (loss_rows) loss_rows[rows.map[row]] = l;
 }
 
-// The sum or mean of the kept rows' losses.
-__global__ __launch_bounds__(1024) void k_total(Stats st, Rows rows, float* out) {
+// The sum or mean of the kept rows' losses, by one workgroup of up to 1024 threads.
+__device__ __forceinline__ void total_loss(const Stats& st, const Rows& rows, float* out) {
   __shared__ double part[16];
   double s = 0.0;
-  const int n = rows.kept[0];
-  for (int i = threadIdx.x; i < n; i += 1024) s += (double)st.loss[i];
+  const int n = rows.kept[0], threads = blockDim.x;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += threads) s += (double)st.loss[i];
 #pragma unroll
   for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x) return;
   s = 0.0;
-  for (int w = 0; w < 16; ++w) s += part[w];
+  for (int w = 0; w < threads / 64; ++w) s += part[w];
   out[0] = (float)(s * (double)rows.scale[0]);
 }
+
+__global__ __launch_bounds__(1024) void k_total(Stats st, Rows rows, float* out) { total_loss(st, rows, out); }
 
 // ---------------------------------------------------------------------------------------------------------- dz
 struct DzArgs {
@@ -371,11 +390,16 @@ struct DzArgs {
   int64_t plane;
   float* bias;            // (ceil(chunk / each), ld) sums over the rows; may be null
   int each;               // rows a workgroup goes over, one wavefront a row, 512 columns wide
+  float* loss;            // or null: the call's loss, by one further workgroup
 };
 
 
 template <int NP>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
+  if (blockIdx.x * 512 >= a.ld) {
+    if (blockIdx.y == 0) total_loss(a.st, a.rows, a.loss);
+    return;
+  }
   __shared__ float part[4][64][9];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int v = (blockIdx.x * 64 + lane) * 8;
@@ -770,13 +794,8 @@ int launch_grad(Kind kind, const GradArgs& a, hipStream_t st) {
   return kind == kMedium ? launch_grad_as<Medium, ROWS, O>(a, st) : launch_grad_as<Flat, ROWS, O>(a, st);
 }
 
-template <typename T>
-int pack(PackArgs a, int64_t rows, hipStream_t st) {
-  a.wide = (uintptr_t)a.src % 16 == 0 && a.stride * (int64_t)sizeof(T) % 16 == 0;
-  const int64_t n = rows * (a.ld / 8);  // threads
-  hipLaunchKernelGGL((k_pack<T>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
-  LOSS_CHECK();
-  return EWS_OK;
+int rows_wide(const void* p, int64_t stride, bool f32) {
+  return (uintptr_t)p % 16 == 0 && stride * (f32 ? 4 : 2) % 16 == 0;
 }
 
 // What every call begins with: the kept rows, the operands' planes, the bias.
@@ -784,6 +803,18 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
           void* grad_hidden) {
   const LPlan& p = c.p;
   const bool f32 = p.np == 3;
+  PackArgs x{};
+  x.src = hidden;
+  x.stride = c.s->hidden_stride;
+  x.rows = p.N;
+  x.cols = p.H;
+  x.map = c.rows.map;
+  x.kept = c.rows.kept;
+  x.dst = (uint16_t*)(c.w + p.xp);
+  x.ld = p.Hp;
+  x.plane = p.Np * p.Hp;
+  x.dst_rows = (int)p.Np;
+  x.wide = rows_wide(x.src, x.stride, f32);
   PrepareArgs r{};
   r.targets = targets;
   r.n = p.N;
@@ -799,27 +830,10 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   r.bias_out = (float*)(c.w + p.bias);
   r.grad_hidden = grad_hidden;
   r.bias_blocks = ceil_div(p.bias_pad, 1024);
-  const dim3 blocks(1 + r.bias_blocks + (grad_hidden ? ceil_div(p.N, 16) : 0));
-  if (f32)
-    hipLaunchKernelGGL((k_prepare<float>), blocks, dim3(1024), 0, c.st, r);
-  else
-    hipLaunchKernelGGL((k_prepare<bf16>), blocks, dim3(1024), 0, c.st, r);
-  LOSS_CHECK();
-  PackArgs x{};
-  x.src = hidden;
-  x.stride = c.s->hidden_stride;
-  x.rows = p.N;
-  x.cols = p.H;
-  x.map = c.rows.map;
-  x.kept = c.rows.kept;
-  x.dst = (uint16_t*)(c.w + p.xp);
-  x.ld = p.Hp;
-  x.plane = p.Np * p.Hp;
-  x.dst_rows = (int)p.Np;
-  int rc = f32 ? pack<float>(x, p.Np, c.st) : pack<bf16>(x, p.Np, c.st);
-  if (rc != EWS_OK) return rc;
+  r.ignored_blocks = grad_hidden ? ceil_div(p.N, 16) : 0;
+  int64_t blocks = 1 + r.bias_blocks + r.ignored_blocks;
   if (p.packed) {
-    PackArgs w{};
+    PackArgs& w = r.weight;
     w.src = weight;
     w.stride = c.s->weight_stride;
     w.rows = p.V;
@@ -828,9 +842,24 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
     w.ld = p.Hp;
     w.plane = p.V * p.Hp;
     w.dst_rows = p.V;
-    rc = f32 ? pack<float>(w, p.V, c.st) : pack<bf16>(w, p.V, c.st);
-    if (rc != EWS_OK) return rc;
+    w.wide = rows_wide(w.src, w.stride, f32);
+    blocks += ceil_div(p.V * (p.Hp / 8), 1024);
   }
+  // up to eight sixteen-byte packs a thread cost less there than a launch does
+  const bool few = p.Np * (p.Hp / 8) <= 8192;
+  if (few) r.few = x;
+  if (f32)
+    hipLaunchKernelGGL((k_prepare<float>), dim3((uint32_t)blocks), dim3(1024), 0, c.st, r);
+  else
+    hipLaunchKernelGGL((k_prepare<bf16>), dim3((uint32_t)blocks), dim3(1024), 0, c.st, r);
+  LOSS_CHECK();
+  if (few) return EWS_OK;
+  const uint32_t packs = (uint32_t)((p.Np * (p.Hp / 8) + 255) / 256);
+  if (f32)
+    hipLaunchKernelGGL((k_pack<float>), dim3(packs), dim3(256), 0, c.st, x);
+  else
+    hipLaunchKernelGGL((k_pack<bf16>), dim3(packs), dim3(256), 0, c.st, x);
+  LOSS_CHECK();
   return EWS_OK;
 }
 
@@ -896,7 +925,7 @@ Call make_call(const ews_loss_desc* s, const LPlan& p, void* workspace, ews_stre
   return c;
 }
 
-int total_loss(const Call& c, float* loss) {
+int launch_total(const Call& c, float* loss) {
   hipLaunchKernelGGL(k_total, dim3(1), dim3(1024), 0, c.st, c.stats, c.rows, loss);
   LOSS_CHECK();
   return EWS_OK;
@@ -925,7 +954,7 @@ int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* 
     rc = logits(c, weight, k, rows);
     if (rc != EWS_OK) return rc;
   }
-  return rows ? EWS_OK : total_loss(c, loss);
+  return rows ? EWS_OK : launch_total(c, loss);
 }
 
 int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
@@ -960,7 +989,8 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
     z.plane = p.chunk * p.Vp;
     z.bias = grad_bias ? (float*)(c.w + p.dbias) : nullptr;
     z.each = p.dz_rows;
-    const dim3 grid(ceil_div(p.Vp, 512), ceil_div(p.chunk, p.dz_rows));
+    z.loss = last && !rows ? loss : nullptr;
+    const dim3 grid(ceil_div(p.Vp, 512) + (z.loss ? 1 : 0), ceil_div(p.chunk, p.dz_rows));
     if (f32)
       hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
     else
@@ -1021,8 +1051,7 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
       if (rc != EWS_OK) return rc;
     }
   }
-  if (!loss || rows) return EWS_OK;
-  return total_loss(c, loss);
+  return EWS_OK;
 }
 
 }  // extern "C"

@@ -36,29 +36,34 @@ def _tables(tensors, outs):
 def _check(tensors):
     dev = tensors[0].device
     for t in tensors:
-        if t.dtype not in DTYPES or not t.is_cuda or t.layout is not torch.strided or t.device != dev:
-            if t.layout is not torch.strided:
-                raise TypeError(f"gradients must be dense tensors, got layout {t.layout}")
-            check_tensor("every gradient", t)
-            raise ValueError(f"gradients are on {dev} and {t.device}")
+        if t.dtype in DTYPES and t.device == dev and t.layout is torch.strided and t.is_cuda:
+            continue
+        if t.layout is not torch.strided:
+            raise TypeError(f"gradients must be dense tensors, got layout {t.layout}")
+        check_tensor("every gradient", t)
+        raise ValueError(f"gradients are on {dev} and {t.device}")
 
 
 def _norm_and_scale(tensors, outs, max_norm):
     """The norm of tensors; where outs is not None, outs = the clipped tensors (outs is tensors: in place)."""
     lib = nat.load()
     dev = tensors[0].device
-    src = [t if _dense(t) else t.contiguous() for t in tensors]
-    dst = src
+    src = dst = tensors
+    if not all([t.is_contiguous() for t in tensors]):
+        src = dst = [t if _dense(t) else t.contiguous() for t in tensors]
     if outs is not None and outs is not tensors:
-        dst = [o if _dense(o) and o.stride() == s.stride() else torch.empty_like(s) for o, s in zip(outs, src)]
+        dst = outs
+        if src is not tensors or not all([o.is_contiguous() for o in outs]):
+            dst = [o if _dense(o) and o.stride() == s.stride() else torch.empty_like(s) for o, s in zip(outs, src)]
     n, ptrs, out, counts, types = _tables(src, dst)
     result = torch.empty(2, device=dev, dtype=torch.float32)
     ws = torch.empty(int(lib.ews_clip_workspace_bytes(n, counts)), device=dev, dtype=torch.uint8)
     nat.check(launch(dev, lib.ews_clip, n, ptrs, out, counts, types, max_norm, 0 if outs is None else 1,
                      result.data_ptr(), ws.data_ptr()), "ews_clip")
-    for o, d in zip(outs if outs is not None else (), dst):
-        if o is not d:
-            o.copy_(d)
+    if outs is not None and dst is not outs:
+        for o, d in zip(outs, dst):
+            if o is not d:
+                o.copy_(d)
     return result[0]
 
 
@@ -106,7 +111,7 @@ def clip_grads(grads, max_norm, out=None):
             raise ValueError(f"out has {len(out)} tensors for {len(grads)} gradients")
         _check(out)
         for g, o in zip(grads, out):
-            if g.shape != o.shape or g.dtype != o.dtype or g.device != o.device:
+            if g.shape != o.shape or g.dtype is not o.dtype or g.device != o.device:
                 raise ValueError(f"out has {o.dtype} {tuple(o.shape)} on {o.device} for {g.dtype} {tuple(g.shape)} on "
                                  f"{g.device}")
     return _norm_and_scale(grads, out, max_norm), out
