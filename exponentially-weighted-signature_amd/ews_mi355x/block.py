@@ -27,8 +27,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .embed import embedding_lookup
 from .front import B, BlockFront, ClockSpec, make_clock
 from .layer import EWS
+from .loss import linear_cross_entropy
 from .mixer import MixerEpilogue
 from .params import AParamBoundedRotation, AParamDampedRotation, AParamDefinitePlusSkew, is_rotation_planes
 
@@ -347,6 +349,9 @@ class StackedEWS(nn.Module):
     def hidden(self, X, *, t=None, mask=None, raw_driver=None, inference: bool = False):
         """ews/block.py:581-624 for a batch: encoder and blocks, no head -> (B, L, hidden_dim)."""
         h = self.embedding(X.long()) if self.tokens else self.embedding(X)
+        return self._blocks(h, t, mask, raw_driver, inference)
+
+    def _blocks(self, h, t, mask, raw_driver, inference):
         enc = h
         for i, block in enumerate(self.blocks):
             driver = None
@@ -359,22 +364,65 @@ class StackedEWS(nn.Module):
             h = self.final_norm(h)
         return h
 
-    def _cosine_logits(self, head, h):
+    def _unit(self, head, h):
+        """The cosine head's two sides, rows of length one (ews/block.py:689-693)."""
         W = head.weight
-        W_hat = W / (torch.linalg.norm(W, dim=1, keepdim=True) + 1e-8)
-        h_hat = h / (torch.linalg.norm(h, dim=-1, keepdim=True) + 1e-8)
+        return (h / (torch.linalg.norm(h, dim=-1, keepdim=True) + 1e-8),
+                W / (torch.linalg.norm(W, dim=1, keepdim=True) + 1e-8))
+
+    def _cosine_logits(self, head, h):
+        h_hat, W_hat = self._unit(head, h)
         return (h_hat @ W_hat.t()) / self.cosine_head_tau
+
+    def _pool(self, h, mask):
+        if mask is not None:
+            w = mask.to(h.dtype)[..., None]
+            return (h * w).sum(-2) / torch.clamp(w.sum(-2), min=1.0)
+        return h.mean(-2)
 
     def _apply_head(self, head, h, mask):
         """ews/block.py:695-707."""
+        if self.head_mode != "seq2seq":
+            h = self._pool(h, mask)
+        return self._cosine_logits(head, h) if self.cosine_head_tau is not None else head(h)
+
+    def _head_loss(self, head, h, targets, ignore_index, reduction):
+        if self.cosine_head_tau is None:
+            return linear_cross_entropy(h, head.weight, targets, bias=head.bias, ignore_index=ignore_index,
+                                        reduction=reduction)
+        h_hat, W_hat = self._unit(head, h)
+        return linear_cross_entropy(h_hat / self.cosine_head_tau, W_hat, targets, ignore_index=ignore_index,
+                                    reduction=reduction)
+
+    def loss(self, X, targets, *, t=None, mask=None, raw_driver=None, inference: bool = False,
+             ignore_index: int = -100, reduction: str = "mean"):
+        """The softmax cross entropy of the heads' logits against whole-number targets (the reference's trainers'
+        objective, e.g. experiments/fl/train.py:754-761), without the logits in memory (``linear_cross_entropy``) and
+        with the embedding's gradient by sorted tokens (``embedding_lookup``): the forward's values are those of
+        ``forward`` and a cross entropy of its result. X, t, mask and raw_driver as ``forward``'s, with a batch;
+        targets (B, L) for "seq2seq" (positions off the mask count as ignored), (B,) for "mean_pool"; for several heads a
+        tuple of them, whose losses are added."""
+        if X.dim() != (2 if self.tokens else 3):
+            raise ValueError(f"X must carry a batch, got shape {tuple(X.shape)}")
+        if mask is not None and mask.dim() == 1:
+            mask = mask[None].expand(X.shape[0], -1)
+        heads = list(self.head) if isinstance(self.head, nn.ModuleList) else [self.head]
+        all_targets = list(targets) if isinstance(targets, (tuple, list)) else [targets]
+        if len(all_targets) != len(heads):
+            raise ValueError(f"{len(heads)} head(s), {len(all_targets)} tensor(s) of targets")
+        h = embedding_lookup(X.long(), self.embedding.weight) if self.tokens else self.embedding(X)
+        h = self._blocks(h, t, mask, raw_driver, inference)
         if self.head_mode == "seq2seq":
-            return self._cosine_logits(head, h) if self.cosine_head_tau is not None else head(h)
-        if mask is not None:
-            w = mask.to(h.dtype)[..., None]
-            pooled = (h * w).sum(-2) / torch.clamp(w.sum(-2), min=1.0)
+            if mask is not None:
+                off = ~mask.to(torch.bool)
+                all_targets = [y.masked_fill(off, ignore_index) for y in all_targets]
         else:
-            pooled = h.mean(-2)
-        return self._cosine_logits(head, pooled) if self.cosine_head_tau is not None else head(pooled)
+            h = self._pool(h, mask)
+        total = None
+        for head, y in zip(heads, all_targets):
+            one = self._head_loss(head, h, y, ignore_index, reduction)
+            total = one if total is None else total + one
+        return total
 
     def forward(self, X, *, t=None, mask=None, raw_driver=None, inference: bool = False):
         """ews/block.py:709-756: tokens (L,) / (B, L) or series (L, c) / (B, L, c)."""
