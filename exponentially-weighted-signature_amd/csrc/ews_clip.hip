@@ -268,12 +268,26 @@ int ews_clip(int n, const uint64_t* in, const uint64_t* out, const int64_t* coun
   return scale ? scale_all(n, in, out, counts, dtypes, result + 1, st) : EWS_OK;
 }
 
-int ews_scale(int n, const uint64_t* in, const uint64_t* out, const int64_t* counts, const int32_t* dtypes,
-              const float* factor, ews_stream_t stream) {
-  const int rc = check(n, in, out, counts, dtypes);
-  if (rc != EWS_OK) return rc;
-  if (!factor || (n > 0 && !out)) return EWS_ERR_NULL;
-  return scale_all(n, in, out, counts, dtypes, factor, (hipStream_t)stream);
+// The gradients of ews_loss_train, scaled in place as a clipped set is.
+int ews_loss_scale(const ews_loss_desc* desc, void* grad_hidden, void* grad_weight, void* grad_bias, const float* factor,
+                   ews_stream_t stream) {
+  if (!desc || !factor) return EWS_ERR_NULL;
+  if (ews_loss_workspace_bytes(desc, 0) == 0) return EWS_ERR_SHAPE;
+  uint64_t at[3];
+  int64_t counts[3];
+  int32_t dtypes[3];
+  int n = 0;
+  auto take = [&](void* p, int64_t count, int32_t dtype) {
+    if (!p) return;
+    at[n] = (uint64_t)p;
+    counts[n] = count;
+    dtypes[n++] = dtype;
+  };
+  take(grad_hidden, (int64_t)desc->rows * desc->hidden, desc->dtype);
+  take(grad_weight, (int64_t)desc->vocab * desc->hidden, desc->dtype);
+  take(grad_bias, desc->vocab, desc->bias_dtype);
+  const int rc = check(n, at, at, counts, dtypes);
+  return rc != EWS_OK ? rc : scale_all(n, at, at, counts, dtypes, factor, (hipStream_t)stream);
 }
 
 }  // extern "C"

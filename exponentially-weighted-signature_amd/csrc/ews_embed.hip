@@ -17,6 +17,9 @@
 //            the rows of dW without a token.
 //   k_join   adds the partial rows of the tokens that were cut, in order.
 //
+// Up to kFewTokens tokens need no order: k_few gives a wavefront a row of dW and a column tile, which looks through all the
+// tokens and adds its own ones' rows. One launch for three and no scratch (n=64, V=100, H=64: 7 us on the host for 15).
+//
 // An id outside [0, vocab) reads nothing: its output row is NaN and it has no gradient.
 #include <hip/hip_runtime.h>
 
@@ -33,6 +36,7 @@ constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kListed = 640;      // own tokens a wavefront lists: of 131071, 32 where all are alike rare
 constexpr int kMaxRange = 512;    // vocabulary entries a workgroup of k_sort may own
 constexpr int kJoinWaves = 4;
+constexpr int kFewTokens = 256;   // one wavefront would add them all in about 30 us
 constexpr int kFewRows = 16;
 
 struct Args {
@@ -277,6 +281,52 @@ __global__ __launch_bounds__(256) void k_runs(Args a) {
   }
 }
 
+template <typename T, int V, typename Tok>
+__global__ __launch_bounds__(256) void k_few(Args a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = (int)blockIdx.x * 4 + wave, v = unit / a.tiles;
+  const int col = ((unit - v * a.tiles) * 64 + lane) * V;
+  if (v >= a.V) return;
+  const bool in = col < a.H;
+  const T* g = (const T*)a.gout + (in ? col : 0);
+  const Tok* tokens = (const Tok*)a.tokens;
+  Tok t[kFewTokens / 64];
+#pragma unroll
+  for (int q = 0; q < kFewTokens / 64; ++q) t[q] = 64 * q + lane < (int)a.n ? tokens[64 * q + lane] : (Tok)-1;
+  float x[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = 0.0f;
+#pragma unroll
+  for (int q = 0; q < kFewTokens / 64; ++q) {
+    uint64_t left = __ballot((int64_t)t[q] == v && v != a.pad);
+    while (left) {
+      constexpr int kAhead = 8;
+      Pack<T, V> p[kAhead];
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {  // the next eight, or the last one again
+        const int j = __ffsll((unsigned long long)left) - 1;
+        if (k == 0 || left) {
+          p[k].load(g + (int64_t)(64 * q + j) * a.H);
+          left &= left - 1;
+          ++n;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (k < n)
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[i] += p[k].get(i);
+    }
+  }
+  if (!in) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] *= a.scale;
+  Pack<T, V> o;
+  o.set(x);
+  o.store((T*)a.gweight + (int64_t)v * a.H + col);
+}
+
 // One workgroup per run; only those whose last token starts in them and goes on work. A token of few partial rows: the
 // wavefronts take a column tile each. One of many: they add a contiguous part of its rows each, one tile after another,
 // and the first one joins them.
@@ -384,6 +434,10 @@ int embed_plan(const ews_embed_desc* s, EPlan& p) {
   while (p.run > 8 && s->count / p.run * tiles < 2048) p.run /= 2;
   p.runs = (s->count + p.run - 1) / p.run;
   size_t off = 0;
+  if (s->count <= kFewTokens) {
+    p.total = 0;
+    return EWS_OK;
+  }
   p.order = off; off += al256e((size_t)s->count * 4);
   p.sorted = off; off += al256e((size_t)s->count * 4);
   p.start = off; off += al256e((((size_t)1 << (p.deal + p.range)) + 1) * 4);
@@ -419,6 +473,19 @@ int launch_lookup(const ews_embed_desc* s, Args a, hipStream_t st) {
     hipLaunchKernelGGL((k_lookup<T, V, int64_t>), dim3((uint32_t)blocks), dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL((k_lookup<T, V, int32_t>), dim3((uint32_t)blocks), dim3(256), 0, st, a);
+  return hipGetLastError() == hipSuccess ? EWS_OK : EWS_ERR_LAUNCH;
+}
+
+template <typename T, int V>
+int launch_few(const ews_embed_desc* s, Args a, hipStream_t st) {
+  a.tiles = (a.H + 64 * V - 1) / (64 * V);
+  const int64_t units = (int64_t)a.V * a.tiles;
+  if (units > ((int64_t)1 << 26) - 4) return EWS_ERR_SHAPE;  // a launch has fewer than 2^32 threads
+  const dim3 grid((uint32_t)((units + 3) / 4));
+  if (s->token_bytes == 8)
+    hipLaunchKernelGGL((k_few<T, V, int64_t>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((k_few<T, V, int32_t>), grid, dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
@@ -469,7 +536,7 @@ int ews_embed_backward(const ews_embed_desc* desc, const void* tokens, const voi
   EPlan p;
   const int rc = embed_plan(desc, p);
   if (rc != EWS_OK) return rc;
-  if (!tokens || !grad_out || !grad_weight || !workspace) return EWS_ERR_NULL;
+  if (!tokens || !grad_out || !grad_weight || (!workspace && desc->count > kFewTokens)) return EWS_ERR_NULL;
   Args a = embed_args(desc);
   char* w = (char*)workspace;
   a.tokens = tokens;
@@ -484,12 +551,16 @@ int ews_embed_backward(const ews_embed_desc* desc, const void* tokens, const voi
   a.start = (int*)(w + p.start);
   a.part = (float*)(w + p.part);
   hipStream_t st = (hipStream_t)stream;
+  const bool wide = rows_aligned(desc, grad_out, grad_weight, desc->width);
+  if (desc->count <= kFewTokens) {
+    if (desc->dtype == EWS_DTYPE_F32) return wide ? launch_few<float, 4>(desc, a, st) : launch_few<float, 1>(desc, a, st);
+    return wide ? launch_few<bf16, 8>(desc, a, st) : launch_few<bf16, 1>(desc, a, st);
+  }
   if (desc->token_bytes == 8)
     hipLaunchKernelGGL((k_sort<int64_t>), dim3(1u << p.deal), dim3(kSortThreads), 0, st, a);
   else
     hipLaunchKernelGGL((k_sort<int32_t>), dim3(1u << p.deal), dim3(kSortThreads), 0, st, a);
   if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH;
-  const bool wide = rows_aligned(desc, grad_out, grad_weight, desc->width);
   if (desc->dtype == EWS_DTYPE_F32)
     return wide ? launch_sums<float, 4>(p, a, st) : launch_sums<float, 1>(p, a, st);
   return wide ? launch_sums<bf16, 8>(p, a, st) : launch_sums<bf16, 1>(p, a, st);

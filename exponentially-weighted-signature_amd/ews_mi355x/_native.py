@@ -98,7 +98,7 @@ EXPORTED = (
     "ews_loss_train",
     "ews_clip_workspace_bytes",
     "ews_clip",
-    "ews_scale",
+    "ews_loss_scale",
 )
 
 JORDAN_KINDS = {"real": 0, "complex": 1}
@@ -443,8 +443,8 @@ def load():
     lib.ews_clip_workspace_bytes.restype = sz
     lib.ews_clip.argtypes = [i32, vp, vp, vp, vp, ctypes.c_float, i32, vp, vp, vp]
     lib.ews_clip.restype = i32
-    lib.ews_scale.argtypes = [i32, vp, vp, vp, vp, vp, vp]
-    lib.ews_scale.restype = i32
+    lib.ews_loss_scale.argtypes = [lsp, vp, vp, vp, vp, vp]
+    lib.ews_loss_scale.restype = i32
     _lib = lib
     return lib
 

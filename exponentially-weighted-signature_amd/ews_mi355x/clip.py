@@ -67,15 +67,6 @@ def _norm_and_scale(tensors, outs, max_norm):
     return result[0]
 
 
-def scale_tensors(tensors, factor):
-    """tensors *= factor in place, factor a float32 number on the device; contiguous tensors, nothing for a 1."""
-    if not tensors:
-        return
-    dev = tensors[0].device
-    n, ptrs, out, counts, types = _tables(tensors, tensors)
-    nat.check(launch(dev, nat.load().ews_scale, n, ptrs, out, counts, types, factor.data_ptr()), "ews_scale")
-
-
 def _max_norm(max_norm):
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:

@@ -68,9 +68,10 @@ class _Lookup(torch.autograd.Function):
         lib = nat.load()
         gout = gout.contiguous()
         desc = _desc(tokens, grad, shape[1], scale, padding)
-        ws = torch.empty(int(lib.ews_embed_workspace_bytes(desc)), device=gout.device, dtype=torch.uint8)
+        size = lib.ews_embed_workspace_bytes(desc)
+        ws = torch.empty(size, device=gout.device, dtype=torch.uint8) if size else None
         nat.check(launch(gout.device, lib.ews_embed_backward, desc, tokens.data_ptr(), gout.data_ptr(),
-                         grad.data_ptr(), ws.data_ptr()), "ews_embed_backward")
+                         grad.data_ptr(), ws.data_ptr() if size else None), "ews_embed_backward")
         return grad, None, None, None
 
 

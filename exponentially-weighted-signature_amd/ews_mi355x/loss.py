@@ -7,7 +7,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .clip import scale_tensors
 from .embed import DTYPES, check_tensor, launch, row_major
 
 
@@ -21,7 +20,8 @@ def _ptr(t):
 
 
 def _run(hidden, weight, bias, targets, ignore_index, reduction, needs, upstream=None, want_loss=True):
-    """(loss, [grad_hidden, grad_weight, grad_bias]); the gradients that ``needs`` asks for, None for the others."""
+    """(loss, [grad_hidden, grad_weight, grad_bias], descriptor); the gradients that ``needs`` asks for, None for the
+    others, and no descriptor where there are no rows."""
     lib = nat.load()
     dev = weight.device
     n = hidden.shape[0]
@@ -31,13 +31,13 @@ def _run(hidden, weight, bias, targets, ignore_index, reduction, needs, upstream
     if n == 0:  # no rows: the sum and the mean of nothing are 0
         if loss is not None:
             loss.zero_()
-        return loss, [None if g is None else g.zero_() for g in grads]
+        return loss, [None if g is None else g.zero_() for g in grads], None
     hidden, hs = row_major(hidden)
     weight, wst = row_major(weight)
     bias = None if bias is None else bias.contiguous()
     desc = _desc(hidden, hs, weight, wst, bias, ignore_index, reduction)
     train = any(needs)
-    ws = torch.empty(int(lib.ews_loss_workspace_bytes(desc, int(train))), device=dev, dtype=torch.uint8)
+    ws = torch.empty(lib.ews_loss_workspace_bytes(desc, int(train)), device=dev, dtype=torch.uint8)
     if train:
         nat.check(launch(dev, lib.ews_loss_train, desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias),
                          targets.data_ptr(), _ptr(upstream), _ptr(loss), *(_ptr(g) for g in grads), ws.data_ptr()),
@@ -45,7 +45,7 @@ def _run(hidden, weight, bias, targets, ignore_index, reduction, needs, upstream
     else:
         nat.check(launch(dev, lib.ews_loss_forward, desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias),
                          targets.data_ptr(), loss.data_ptr(), ws.data_ptr()), "ews_loss_forward")
-    return loss, grads
+    return loss, grads, desc
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -58,7 +58,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.save_for_backward(hidden, weight, bias, targets)
         ctx.args = (ignore_index, reduction)
         needs = ctx.needs_input_grad[:3] if reduction != "none" else (False, False, False)
-        loss, grads = _run(hidden, weight, bias, targets, ignore_index, reduction, needs)
+        loss, grads, ctx.desc = _run(hidden, weight, bias, targets, ignore_index, reduction, needs)
         ctx.grads = grads if any(needs) else None
         return loss
 
@@ -66,14 +66,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         ignore_index, reduction = ctx.args
-        gout = gout.to(torch.float32).contiguous()
+        if gout.dtype is not torch.float32 or not gout.is_contiguous():
+            gout = gout.to(torch.float32).contiguous()
         grads, ctx.grads = ctx.grads, None
         if grads is None:
             hidden, weight, bias, targets = ctx.saved_tensors
-            _, grads = _run(hidden, weight, bias, targets, ignore_index, reduction, ctx.needs_input_grad[:3],
-                            upstream=gout if reduction == "none" else None, want_loss=False)
-        if reduction != "none":
-            scale_tensors([g for g in grads if g is not None], gout)
+            _, grads, ctx.desc = _run(hidden, weight, bias, targets, ignore_index, reduction, ctx.needs_input_grad[:3],
+                                      upstream=gout if reduction == "none" else None, want_loss=False)
+        if reduction != "none" and ctx.desc is not None:
+            nat.check(launch(gout.device, nat.load().ews_loss_scale, ctx.desc, *(_ptr(g) for g in grads),
+                             gout.data_ptr()), "ews_loss_scale")
         return (*grads, None, None, None)
 
 
@@ -91,29 +93,33 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
         raise ValueError(f"reduction must be one of {tuple(nat.LOSS_REDUCTIONS)}, got {reduction!r}")
     if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError(f"weight must be (V, H) with V, H >= 1, got {tuple(weight.shape)}")
-    if hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
-        raise ValueError(f"hidden must be (..., {weight.shape[1]}), got {tuple(hidden.shape)}")
-    if tuple(targets.shape) != tuple(hidden.shape[:-1]):
-        raise ValueError(f"targets must be {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
-    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
-        raise ValueError(f"bias must be {(weight.shape[0],)}, got {tuple(bias.shape)}")
+    V, H = weight.shape
+    shape = hidden.shape[:-1]
+    if hidden.dim() < 1 or hidden.shape[-1] != H:
+        raise ValueError(f"hidden must be (..., {H}), got {tuple(hidden.shape)}")
+    if targets.shape != shape:
+        raise ValueError(f"targets must be {tuple(shape)}, got {tuple(targets.shape)}")
+    if bias is not None and bias.shape != (V,):
+        raise ValueError(f"bias must be {(V,)}, got {tuple(bias.shape)}")
     check_tensor("weight", weight)
     check_tensor("hidden", hidden)
-    if hidden.dtype != weight.dtype:
+    if hidden.dtype is not weight.dtype:
         raise TypeError(f"hidden is {hidden.dtype}, weight {weight.dtype}")
     if bias is not None:
         check_tensor("bias", bias)
     if targets.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"targets must be int64 or int32, got {targets.dtype}")
+    dev = weight.device
     for name, t in (("hidden", hidden), ("targets", targets), ("bias", bias)):
-        if t is not None and t.device != weight.device:
-            raise ValueError(f"{name} is on {t.device}, weight on {weight.device}")
-    shape = hidden.shape[:-1]
-    rows = hidden.reshape(-1, hidden.shape[-1])
-    t = targets.reshape(-1).to(torch.int64).contiguous()
-    inputs = (rows, weight, bias)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, weight on {dev}")
+    rows = hidden if hidden.dim() == 2 else hidden.reshape(-1, H)
+    t = targets if targets.dim() == 1 else targets.reshape(-1)
+    if t.dtype is not torch.int64 or not t.is_contiguous():
+        t = t.to(torch.int64).contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
         loss = _LinearCrossEntropy.apply(rows, weight, bias, t, int(ignore_index), reduction)
     else:
-        loss, _ = _run(rows, weight, bias, t, int(ignore_index), reduction, (False, False, False))
-    return loss.reshape(shape) if reduction == "none" else loss
+        loss = _run(rows, weight, bias, t, int(ignore_index), reduction, (False, False, False))[0]
+    return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss

@@ -610,6 +610,7 @@ typedef struct ews_embed_desc {
 int ews_embed_forward(const ews_embed_desc* desc, const void* tokens, const void* weight, void* out,
                       ews_stream_t stream);
 
+/* 0 for up to 256 tokens: workspace may then be NULL. */
 size_t ews_embed_workspace_bytes(const ews_embed_desc* desc);
 
 /* grad_weight (V, H), contiguous: s times the sum of grad_out's rows (contiguous) of every token, added in the
@@ -648,6 +649,11 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
                    const int64_t* targets, const float* upstream, float* loss, void* grad_hidden, void* grad_weight,
                    void* grad_bias, void* workspace, ews_stream_t stream);
 
+/* grad_* = factor[0] grad_* in place (each may be NULL), factor on the device: the gradients of factor[0] times the loss.
+ * With a factor of 1 nothing is touched. */
+int ews_loss_scale(const ews_loss_desc* desc, void* grad_hidden, void* grad_weight, void* grad_bias, const float* factor,
+                   ews_stream_t stream);
+
 /* Gradient clipping over n tensors, given by host arrays of device addresses, element counts (0 allowed) and
  * EWS_DTYPE_*: result[0] = norm = sqrt(sum of all squares), result[1] = c = min(1, max_norm / (norm + 1e-6)) (NaN for
  * a NaN norm). scale != 0: also out = c in for every tensor (out[i] == in[i]: in place; otherwise they may not
@@ -655,10 +661,6 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
 size_t ews_clip_workspace_bytes(int n, const int64_t* counts);
 int ews_clip(int n, const uint64_t* in, const uint64_t* out, const int64_t* counts, const int32_t* dtypes,
              float max_norm, int32_t scale, float* result, void* workspace, ews_stream_t stream);
-
-/* out = factor[0] in for every tensor, factor on the device; in place with a factor of 1 nothing is touched. */
-int ews_scale(int n, const uint64_t* in, const uint64_t* out, const int64_t* counts, const int32_t* dtypes,
-              const float* factor, ews_stream_t stream);
 
 /* Human-readable text of a return code. */
 const char* ews_error_string(int code);

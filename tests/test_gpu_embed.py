@@ -141,6 +141,15 @@ def test_no_tokens_and_other_streams():
     assert torch.equal(g[:, 0], torch.bincount(t, minlength=6).float())
 
 
+def test_second_derivatives_are_refused():
+    w = torch.randn(6, 16, device=DEV, requires_grad=True)
+    out = E.embedding_lookup(torch.arange(6, device=DEV), w)
+    gout = torch.ones_like(out, requires_grad=True)
+    (g,) = torch.autograd.grad(out, w, gout, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), gout)
+
+
 def test_refusals_on_the_device():
     w = torch.randn(6, 16, device=DEV)
     t = torch.zeros(3, dtype=torch.int64, device=DEV)

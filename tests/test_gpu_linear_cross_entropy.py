@@ -283,6 +283,14 @@ def test_another_stream_and_the_same_bits():
         assert torch.equal(a, r)
 
 
+def test_second_derivatives_are_refused():
+    h, w, b, t = _inputs(6, 16, 20, torch.float32, bias=torch.float32)
+    h.requires_grad_()
+    (g,) = torch.autograd.grad(E.linear_cross_entropy(h, w, t), h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), h)
+
+
 def test_no_rows():
     w = torch.randn(9, 16, device=DEV, requires_grad=True)
     h = torch.empty(0, 16, device=DEV, requires_grad=True)

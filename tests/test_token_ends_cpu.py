@@ -42,7 +42,8 @@ def _embed(**kw):
 def test_embed_error_codes():
     lib = nat.load()
     assert lib.ews_embed_forward(_embed(), NULL, NULL, NULL, NULL) == -1
-    assert lib.ews_embed_workspace_bytes(_embed()) > 0
+    assert lib.ews_embed_workspace_bytes(_embed(count=1000)) > 0
+    assert lib.ews_embed_workspace_bytes(_embed(count=256)) == 0
     for bad, code in ((dict(count=0), -2), (dict(count=2**25 + 1), -2), (dict(width=0), -2), (dict(vocab=0), -2),
                       (dict(weight_stride=15), -2), (dict(vocab=2**25 + 1), -2), (dict(dtype=2), -4),
                       (dict(token_bytes=2), -4)):
@@ -93,4 +94,5 @@ def test_clip_error_codes():
     assert lib.ews_clip(-1, one, one, count, dtype, 1.0, 1, NULL, NULL, NULL) == -2
     assert lib.ews_clip(1, one, one, (ctypes.c_int64 * 1)(-1), dtype, 1.0, 1, NULL, NULL, NULL) == -2
     assert lib.ews_clip(1, one, one, count, (ctypes.c_int32 * 1)(5), 1.0, 1, NULL, NULL, NULL) == -4
-    assert lib.ews_scale(1, one, (ctypes.c_uint64 * 1)(0), count, dtype, NULL, NULL) == -1
+    assert lib.ews_loss_scale(_loss(), NULL, NULL, NULL, NULL, NULL) == -1
+    assert lib.ews_loss_scale(_loss(rows=0), NULL, NULL, NULL, one, NULL) == -2
