@@ -505,36 +505,51 @@ struct GradArgs {
   float* sum;             // float32 sums over the chunks, or null
   int add;                // sum holds those of earlier chunks
   void* out;              // the result, or null before the last chunk
-  int wide;               // the result's rows start at multiples of 16 bytes
+  int wide;               // the result's rows start at multiples of 16 bytes and hold whole eights
   const float* factor;    // of every result; null: 1
 };
 
-// Eight consecutive results of result row `row`, from column i on.
+// Eight consecutive results of result row `row`, from column i on; all in the row, at a multiple of 16 bytes.
 template <typename T>
-__device__ __forceinline__ void finish(const GradArgs& a, int64_t row, int i, const float (&x)[8]) {
+__device__ __forceinline__ void finish(const GradArgs& a, int64_t row, int i, const Eight& e) {
   const int64_t at = row * a.I + i;
-  const int n = a.I - i < 8 ? a.I - i : 8;
   const float f = a.factor ? a.factor[0] : 1.0f;
   float y[8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) y[q] = x[q] * f + (a.add && q < n ? a.sum[at + q] : 0.0f);
+  for (int q = 0; q < 8; ++q) y[q] = e.x[q] * f + (a.add ? a.sum[at + q] : 0.0f);
   if (!a.out) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (q < n) a.sum[at + q] = y[q];
-  } else if (a.wide && n == 8) {
+    for (int q = 0; q < 8; ++q) a.sum[at + q] = y[q];
+    return;
+  }
 #pragma unroll
-    for (int q = 0; q < 8; q += kWide<T>) {
-      Pack<T, kWide<T>> p;
-      p.set(y + q);
-      p.store((T*)a.out + at + q);
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (q < n) ((T*)a.out)[at + q] = narrow<T>(y[q]);
+  for (int q = 0; q < 8; q += kWide<T>) {
+    Pack<T, kWide<T>> p;
+    p.set(y + q);
+    p.store((T*)a.out + at + q);
   }
 }
+
+// One result.
+template <typename T>
+__device__ __forceinline__ void finish(const GradArgs& a, int64_t row, int i, const One& e) {
+  const int64_t at = row * a.I + i;
+  const float y = e.x * (a.factor ? a.factor[0] : 1.0f) + (a.add ? a.sum[at] : 0.0f);
+  if (a.out)
+    ((T*)a.out)[at] = narrow<T>(y);
+  else
+    a.sum[at] = y;
+}
+
+// Results of a split, kept for k_reduce.
+__device__ __forceinline__ void keep(float* to, const Eight& e) {
+  Pack<float, 4> lo, hi;
+  lo.set(e.x);
+  hi.set(e.x + 4);
+  lo.store(to);
+  hi.store(to + 4);
+}
+__device__ __forceinline__ void keep(float* to, const One& e) { *to = e.x; }
 
 // ROWS: dW, whose k is the chunk's kept rows and whose operands are both turned; else dh, whose rows they are.
 template <class T, int PAIRS, bool ROWS, typename O>
@@ -552,44 +567,51 @@ __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
   if (ROWS && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
   f32x16 acc[T::TI][T::TJ];
   product<T, PAIRS, true, ROWS>(a.P, a.Q, i0, j0, kb0, kb1, lds, acc);
+  auto rows = [&](auto each) {
+    using W = decltype(each);
 #pragma unroll
-  for (int b = 0; b < T::TJ; ++b)
-    rows_of<T, Eight>(lds, acc, b, [&](int jrow, int icol, const Eight& e) {
-      const int j = j0 + jrow, i = i0 + icol;
-      const auto& x = e.x;
-      if (j >= nj || i >= a.I) return;
-      if (a.splits > 1) {
-        float* p = a.part + ((int64_t)split * (ROWS ? a.J : a.chunk) + j) * a.I + i;
-        const int n = a.I - i < 8 ? a.I - i : 8;
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (q < n) p[q] = x[q];
-      } else {
-        finish<O>(a, ROWS ? j : a.rows.map[a.c0 + j], i, x);
-      }
-    });
+    for (int b = 0; b < T::TJ; ++b)
+      rows_of<T, W>(lds, acc, b, [&](int jrow, int icol, const W& e) {
+        const int j = j0 + jrow, i = i0 + icol;
+        if (j >= nj || i >= a.I) return;
+        if (a.splits > 1)
+          keep(a.part + ((int64_t)split * (ROWS ? a.J : a.chunk) + j) * a.I + i, e);
+        else
+          finish<O>(a, ROWS ? j : a.rows.map[a.c0 + j], i, e);
+      });
+  };
+  // rows of other lengths are written one number a lane: 64 neighbours at a time, not eight apart
+  if (a.wide)
+    rows(Eight{});
+  else
+    rows(One{});
 }
 
+// The splits' results added in order: 32 results a workgroup, its eight groups of lanes a contiguous part of the splits
+// each, joined in LDS.
 template <typename O>
 __global__ __launch_bounds__(256) void k_reduce(GradArgs a) {
+  __shared__ float parts[8][32];
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   const int nj = a.by_rows ? a.J : live;
-  const int rows = a.by_rows ? a.J : a.chunk;
-  const int packs = (a.I + 7) / 8;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t j = at / packs;
-  if (j >= nj) return;
-  const int i = (int)(at % packs) * 8;
-  const int n = a.I - i < 8 ? a.I - i : 8;
-  float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const float* p = a.part + ((int64_t)s * rows + j) * a.I + i;
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (q < n) x[q] += p[q];
+  const int64_t stride = (int64_t)(a.by_rows ? a.J : a.chunk) * a.I;
+  const int64_t at = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+  const int group = threadIdx.x >> 5;
+  const bool in = at < (int64_t)nj * a.I;
+  const int per = (a.splits + 7) / 8;
+  const int s0 = group * per, s1 = s0 + per < a.splits ? s0 + per : a.splits;
+  float x = 0.0f;
+  if (in) {
+#pragma unroll 8
+    for (int s = s0; s < s1; ++s) x += a.part[s * stride + at];
   }
-  finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], i, x);
+  parts[group][threadIdx.x & 31] = x;
+  __syncthreads();
+  if (group || !in) return;
+#pragma unroll
+  for (int g = 1; g < 8; ++g) x += parts[g][threadIdx.x];
+  const int64_t j = at / a.I;
+  finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], (int)(at - j * a.I), One{x});
 }
 
 }  // namespace loss
@@ -602,6 +624,8 @@ using namespace ews::loss;
 // Rows kept at a time: exp(z - m), and dz in its place (float32: dz in three planes beside it), of as many as fit here.
 constexpr int64_t kChunkBytes = (int64_t)2 << 30;
 constexpr int64_t kScoreRows = 65536;  // rows of a call without gradients whose slabs' sums are kept at a time
+
+constexpr int kLongProduct = 8;  // stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared
 
 enum Kind { kLarge, kMedium, kFlat };
 
@@ -635,7 +659,7 @@ Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split) {
   if (J <= 32)
     p.kind = kFlat;
   else
-    p.kind = I > 128 && J > 128 && large * parts >= 128 ? kLarge : kMedium;
+    p.kind = I > 128 && J > 128 && large * parts >= 128 && kblocks * pairs >= kLongProduct ? kLarge : kMedium;
   const int ti = p.kind == kMedium ? 128 : 256;
   const int tj = p.kind == kLarge ? 256 : p.kind == kMedium ? 128 : 32;
   p.slab = p.kind == kLarge ? Large::kSlab : p.kind == kMedium ? Medium::kSlab : Flat::kSlab;
@@ -649,6 +673,7 @@ Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split) {
     int64_t z = room / n;
     const int64_t most = p.kind == kLarge ? parts : kblocks * pairs / 4 < kblocks ? kblocks * pairs / 4 : kblocks;
     if (z > most) z = most;
+    if (z > 128) z = 128;  // each split's results are written and read once more
     if (z > 1) {
       p.per = ceil_div(kblocks, z);
       p.splits = ceil_div(kblocks, p.per);
@@ -781,8 +806,8 @@ int launch_grad_as(const GradArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((k_grad<T, kP, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
   LOSS_CHECK();
   if (a.splits > 1) {
-    const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * ((a.I + 7) / 8);
-    hipLaunchKernelGGL((k_reduce<O>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
+    const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * a.I;
+    hipLaunchKernelGGL((k_reduce<O>), dim3((uint32_t)((n + 31) / 32)), dim3(256), 0, st, a);
     LOSS_CHECK();
   }
   return EWS_OK;
@@ -969,7 +994,7 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
   float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
   rc = begin(c, hidden, weight, bias, targets, rows, grad_hidden);
   if (rc != EWS_OK) return rc;
-  const int wide = (p.H * (f32 ? 4 : 2)) % 16 == 0 && (uintptr_t)grad_hidden % 16 == 0 && (uintptr_t)grad_weight % 16 == 0;
+  const int wide = p.H % 8 == 0 && (uintptr_t)grad_hidden % 16 == 0 && (uintptr_t)grad_weight % 16 == 0;
   const float* factor = upstream ? nullptr : c.rows.scale;
   for (int k = 0; k < p.chunks; ++k) {
     const bool last = k + 1 == p.chunks;

@@ -27,6 +27,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ews_vec.h"
 
 namespace ews {
@@ -280,10 +282,13 @@ __device__ __forceinline__ void tile_of(int id, int ti, int tj, int& i, int& j) 
 struct Eight {
   float x[8];
 };
+struct One {
+  float x;
+};
 
 // A wavefront's block column b of its results, staged through its own part of LDS and handed on as rows of numbers of
 // type W: f(jrow, i, x) gets the results of tile row jrow from tile column i on; float and uint16_t (65535ths of results
-// held to [0, 1]) 16 bytes of them, Eight eight floats.
+// held to [0, 1]) 16 bytes of them, Eight eight floats, One one, neighbouring lanes neighbouring results.
 template <class T, typename W, class F>
 __device__ __forceinline__ void rows_of(char* lds, const f32x16 (&acc)[T::TI][T::TJ], int b, F f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -307,16 +312,29 @@ __device__ __forceinline__ void rows_of(char* lds, const f32x16 (&acc)[T::TI][T:
     }
   asm volatile("" ::: "memory");
   __builtin_amdgcn_wave_barrier();
-  constexpr int kEach = sizeof(W) == sizeof(Eight) ? 8 : 16 / (int)sizeof(W);  // numbers handed on at a time
-  constexpr int kLanes = T::kSlab / kEach;                                     // lanes of one row
+  constexpr bool kOne = std::is_same<W, One>::value;
+  constexpr int kEach = kOne ? 1 : sizeof(W) == sizeof(Eight) ? 8 : 16 / (int)sizeof(W);  // numbers handed on at a time
+  constexpr int kLanes = T::kSlab / kEach < 64 ? T::kSlab / kEach : 64;                   // lanes of one row
+  if constexpr (kOne) {
+    for (int row = 0; row < 32; ++row)
+#pragma unroll
+      for (int c = 0; c < T::kSlab; c += 64)
+        if (T::kSlab >= 64 || lane < T::kSlab)
+          f((wj * T::TJ + b) * 32 + row, wi * T::kSlab + c + lane,
+            One{*reinterpret_cast<const float*>(stage + row * kRow + (c + lane) * 4)});
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    return;
+  }
   constexpr int kBytes = kHalf ? 16 : 4 * kEach;
 #pragma unroll
-  for (int it = 0; it < 32 * kLanes / 64; ++it) {
+  for (int it = 0; it < (kOne ? 0 : 32 * kLanes / 64); ++it) {
     const int row = it * (64 / kLanes) + lane / kLanes;
     const char* s = stage + row * kRow + (lane % kLanes) * kBytes;
     const int j = (wj * T::TJ + b) * 32 + row, i = wi * T::kSlab + (lane % kLanes) * kEach;
     const u32x4 lo = *reinterpret_cast<const u32x4*>(s);
-    if constexpr (kEach == 8 && !kHalf) {
+    if constexpr (kOne) {
+    } else if constexpr (kEach == 8 && !kHalf) {
       const vec::f32x4 x = __builtin_bit_cast(vec::f32x4, lo), y = *reinterpret_cast<const vec::f32x4*>(s + 16);
       f(j, i, Eight{{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}});
     } else {
