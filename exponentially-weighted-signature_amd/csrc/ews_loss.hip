@@ -32,6 +32,7 @@
 
 #include "ews_hip.h"
 #include "ews_tiles.h"
+#include "ews_tiles32.h"
 #include "ews_vec.h"
 
 namespace ews {
@@ -43,6 +44,10 @@ using namespace ews::tiles;
 typedef Tile<2, 4, 4, 2> Large;   // 256 x 256, eight wavefronts
 typedef Tile<2, 2, 2, 2> Medium;  // 128 x 128, four wavefronts
 typedef Tile<4, 1, 2, 1> Flat;    // 256 x 32, four wavefronts: few rows
+template <int BYTES>
+using Few32 = Tile32<1, BYTES>;   // 128 x 32 and 128 x 64, float32 W read as it is: few rows
+template <int BYTES>
+using More32 = Tile32<2, BYTES>;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
@@ -224,6 +229,7 @@ __global__ __launch_bounds__(1024) void k_prepare(PrepareArgs a) {
 // ------------------------------------------------------------------------------------------------------ the logits
 struct LogitArgs {
   Operand W, X;
+  Operand32 W32;          // float32 W where it is read as it is
   int ti, tj;             // tiles along the vocabulary and along the chunk's rows
   int kblocks;
   int c0, chunk;          // the chunk's first row, its rows
@@ -234,7 +240,8 @@ struct LogitArgs {
   int64_t ldp;
 };
 
-// KEEP: 0 the loss alone, 1 also 16-bit logarithms, 2 also float32 probabilities.
+// PAIRS: 1, kPairs for planes, or 0 for float32 W. KEEP: 0 the loss alone, 1 also 16-bit logarithms, 2 also float32
+// probabilities.
 template <class T, int PAIRS, int KEEP>
 __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
   extern __shared__ char lds[];
@@ -253,7 +260,10 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
       tile_target[t - T::I] = j0 + t - T::I < live ? a.rows.target[a.c0 + j0 + t - T::I] : -1;
   }
   f32x16 acc[T::TI][T::TJ];
-  product<T, PAIRS, false, false>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, lds, acc);
+  if constexpr (PAIRS == 0)
+    product32<T, false>(a.W32, a.X, i0, j0 + a.c0, 0, a.kblocks, lds, acc);
+  else
+    product<T, PAIRS, false, false>(a.W, a.X, i0, j0 + a.c0, 0, a.kblocks, lds, acc);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wi = wave % T::WI, wj = wave / T::WI;
@@ -495,6 +505,7 @@ __global__ __launch_bounds__(256) void k_dbias(const float* part, int parts, int
 // ------------------------------------------------------------------------------------------------------ the gradients
 struct GradArgs {
   Operand P, Q;
+  Operand32 P32;          // float32 W where it is read as it is
   int ti, tj, splits;
   int kblocks, per;       // k blocks, and those of one split
   int by_rows;            // 1: k is the chunk's kept rows (dW); 0: the result's rows are (dh)
@@ -566,7 +577,10 @@ __global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
   int kb0 = split * a.per, kb1 = kb0 + a.per < a.kblocks ? kb0 + a.per : a.kblocks;
   if (ROWS && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
   f32x16 acc[T::TI][T::TJ];
-  product<T, PAIRS, true, ROWS>(a.P, a.Q, i0, j0, kb0, kb1, lds, acc);
+  if constexpr (PAIRS == 0)
+    product32<T, true>(a.P32, a.Q, i0, j0, kb0, kb1, lds, acc);
+  else
+    product<T, PAIRS, true, ROWS>(a.P, a.Q, i0, j0, kb0, kb1, lds, acc);
   auto rows = [&](auto each) {
     using W = decltype(each);
 #pragma unroll
@@ -623,22 +637,25 @@ using namespace ews::loss;
 
 // Rows kept at a time: exp(z - m), and dz in its place (float32: dz in three planes beside it), of as many as fit here.
 constexpr int64_t kChunkBytes = (int64_t)2 << 30;
+// float32 W is read as it is for up to so many rows, else packed into planes first. H=2048 V=30000, packing, logits and dh:
+// N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54.
+constexpr int kFewRows32 = 256;
 constexpr int64_t kScoreRows = 65536;  // rows of a call without gradients whose slabs' sums are kept at a time
 
 constexpr int kLongProduct = 8;  // stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared
 
-enum Kind { kLarge, kMedium, kFlat };
+enum Kind { kLarge, kMedium, kFlat, kFew32, kMore32 };
 
 struct Product {
   Kind kind;
-  int ti, tj, slab, splits, per, kblocks;
+  int ti, tj, tile_i, slab, splits, per, kblocks;
 };
 
 struct LPlan {
   int N, H, V, np;
   int64_t Hp, Vp, Np, chunk;
   int chunks, slabs, bias_pad, dz_rows;
-  bool train, packed;
+  bool train, packed, as_is;
   Product logits, dh, dw;
   size_t map, target, meta, zt, top, inv, loss, xp, wp, bias, slab, prob, dz, dbias, dbsum, part, acc;
   size_t total;
@@ -651,24 +668,29 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // A product of I x J results over kblocks of k: 256 x 32 tiles where J fits one; 256 x 256 ones where they give (split
 // over k, where that is allowed, into parts of 16 blocks at least) half the CUs work; else 128 x 128 ones, of which a CU
 // holds two. Measured at float32 N=4095 H=512 V=32000, dh (30 large tiles, split by 8): 0.55 ms, 0.80 ms with the small.
-Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split) {
+// as_is: float32 W is read as it is, in k blocks of 32.
+Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split, bool as_is) {
   Product p;
   p.kblocks = kblocks;
   const int64_t large = (int64_t)ceil_div(I, 256) * ceil_div(J, 256);
   const int parts = split ? (kblocks >= 32 ? kblocks / 16 : 1) : 1;
-  if (J <= 32)
+  if (as_is)
+    p.kind = J <= 32 ? kFew32 : kMore32;
+  else if (J <= 32)
     p.kind = kFlat;
   else
     p.kind = I > 128 && J > 128 && large * parts >= 128 && kblocks * pairs >= kLongProduct ? kLarge : kMedium;
-  const int ti = p.kind == kMedium ? 128 : 256;
-  const int tj = p.kind == kLarge ? 256 : p.kind == kMedium ? 128 : 32;
-  p.slab = p.kind == kLarge ? Large::kSlab : p.kind == kMedium ? Medium::kSlab : Flat::kSlab;
-  p.ti = ceil_div(I, ti);
-  p.tj = ceil_div(J, tj);
+  const int tile_i[] = {Large::I, Medium::I, Flat::I, Few32<16>::I, More32<16>::I};
+  const int tile_j[] = {Large::J, Medium::J, Flat::J, Few32<16>::J, More32<16>::J};
+  const int slab[] = {Large::kSlab, Medium::kSlab, Flat::kSlab, Few32<16>::kSlab, More32<16>::kSlab};
+  p.slab = slab[p.kind];
+  p.tile_i = tile_i[p.kind];
+  p.ti = ceil_div(I, p.tile_i);
+  p.tj = ceil_div(J, tile_j[p.kind]);
   p.splits = 1;
   p.per = kblocks;
   // one round of workgroups: a CU holds one of the large tiles, two of the others
-  const int64_t n = (int64_t)p.ti * p.tj, room = p.kind == kLarge ? 256 : 512;
+  const int64_t n = (int64_t)p.ti * p.tj, room = p.kind == kLarge ? 256 : as_is ? 1024 : 512;
   if (split && 2 * n <= room) {
     int64_t z = room / n;
     const int64_t most = p.kind == kLarge ? parts : kblocks * pairs / 4 < kblocks ? kblocks * pairs / 4 : kblocks;
@@ -712,11 +734,11 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.chunks = ceil_div(p.Np, p.chunk);
   const int64_t most = p.chunk < p.N ? p.chunk : p.N;  // rows of a chunk
   const int pairs = p.np == 3 ? kPairs : 1;
-  p.logits = pick(p.V, most, (int)(p.Hp / 64), pairs, false);
-  p.dh = pick(p.H, most, (int)(p.Vp / 64), pairs, true);
-  p.dw = pick(p.H, p.V, (int)(p.chunk / 64), pairs, true);
-  const int tile_i = p.logits.kind == kMedium ? 128 : 256;
-  p.bias_pad = p.logits.ti * tile_i;
+  p.as_is = p.np == 3 && direct;
+  p.logits = pick(p.V, most, p.as_is ? ceil_div(p.H, 32) : (int)(p.Hp / 64), pairs, false, p.as_is);
+  p.dh = pick(p.H, most, p.as_is ? ceil_div(p.V, 32) : (int)(p.Vp / 64), pairs, true, p.as_is);
+  p.dw = pick(p.H, p.V, (int)(p.chunk / 64), pairs, true, false);
+  p.bias_pad = p.logits.ti * p.logits.tile_i;
   p.slabs = p.bias_pad / p.logits.slab;
   size_t off = 0;
   auto take = [&off](size_t bytes) {
@@ -753,10 +775,12 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   return EWS_OK;
 }
 
-// bfloat16 weights whose rows start at multiples of 16 bytes and fill whole k blocks are read where they are.
+// bfloat16 weights whose rows start at multiples of 16 bytes and fill whole k blocks are read where they are, and float32
+// weights for few rows (of a stride that the tiles' offsets hold).
 bool reads_direct(const ews_loss_desc* s, const void* weight) {
-  return s->dtype == EWS_DTYPE_BF16 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0 &&
-         s->weight_stride <= 1 << 22 && (uintptr_t)weight % 16 == 0;
+  if (s->weight_stride > 1 << 22) return false;
+  if (s->dtype == EWS_DTYPE_F32) return s->rows <= kFewRows32;
+  return (uintptr_t)weight % 16 == 0 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0;
 }
 
 struct Call {
@@ -782,6 +806,9 @@ int allow_lds(K kernel, int bytes) {
              : EWS_ERR_LAUNCH;
 }
 
+// Whether a float32 operand can be copied 16 bytes a lane.
+bool pieces(const Operand32& o) { return (uintptr_t)o.p % 16 == 0 && o.ld % 4 == 0 && o.cols % 4 == 0; }
+
 template <class T, int PAIRS, int KEEP>
 int launch_logits_as(const LogitArgs& a, hipStream_t st) {
   constexpr int kLds = T::kLdsBytes + (T::I + T::J) * 4;
@@ -794,13 +821,19 @@ int launch_logits_as(const LogitArgs& a, hipStream_t st) {
 
 template <int PAIRS, int KEEP>
 int launch_logits(Kind kind, const LogitArgs& a, hipStream_t st) {
+  if constexpr (KEEP != 1 && PAIRS != 1) {
+    if (kind == kFew32)
+      return pieces(a.W32) ? launch_logits_as<Few32<16>, 0, KEEP>(a, st) : launch_logits_as<Few32<4>, 0, KEEP>(a, st);
+    if (kind == kMore32)
+      return pieces(a.W32) ? launch_logits_as<More32<16>, 0, KEEP>(a, st) : launch_logits_as<More32<4>, 0, KEEP>(a, st);
+  }
   if (kind == kLarge) return launch_logits_as<Large, PAIRS, KEEP>(a, st);
   return kind == kMedium ? launch_logits_as<Medium, PAIRS, KEEP>(a, st) : launch_logits_as<Flat, PAIRS, KEEP>(a, st);
 }
 
-template <class T, bool ROWS, typename O>
+// kP: float32 gradients are those of float32 operands
+template <class T, bool ROWS, typename O, int kP = sizeof(O) == 4 ? kPairs : 1>
 int launch_grad_as(const GradArgs& a, hipStream_t st) {
-  constexpr int kP = sizeof(O) == 4 ? kPairs : 1;  // float32 gradients are those of float32 operands
   const int rc = allow_lds(k_grad<T, kP, ROWS, O>, T::kLdsBytes);
   if (rc != EWS_OK) return rc;
   hipLaunchKernelGGL((k_grad<T, kP, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
@@ -815,6 +848,12 @@ int launch_grad_as(const GradArgs& a, hipStream_t st) {
 
 template <bool ROWS, typename O>
 int launch_grad(Kind kind, const GradArgs& a, hipStream_t st) {
+  if constexpr (!ROWS && sizeof(O) == 4) {
+    if (kind == kFew32)
+      return pieces(a.P32) ? launch_grad_as<Few32<16>, ROWS, O, 0>(a, st) : launch_grad_as<Few32<4>, ROWS, O, 0>(a, st);
+    if (kind == kMore32)
+      return pieces(a.P32) ? launch_grad_as<More32<16>, ROWS, O, 0>(a, st) : launch_grad_as<More32<4>, ROWS, O, 0>(a, st);
+  }
   if (kind == kLarge) return launch_grad_as<Large, ROWS, O>(a, st);
   return kind == kMedium ? launch_grad_as<Medium, ROWS, O>(a, st) : launch_grad_as<Flat, ROWS, O>(a, st);
 }
@@ -888,6 +927,11 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   return EWS_OK;
 }
 
+Operand32 weight_operand32(const Call& c, const void* weight) {
+  const LPlan& p = c.p;
+  return Operand32{(const float*)weight, c.s->weight_stride, p.V, p.H};
+}
+
 Operand weight_operand(const Call& c, const void* weight) {
   const LPlan& p = c.p;
   if (p.packed) return Operand{(const uint16_t*)(c.w + p.wp), p.Hp, p.V * p.Hp, p.V, (int)p.Hp};
@@ -902,7 +946,10 @@ Operand hidden_operand(const Call& c) {
 int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
   const LPlan& p = c.p;
   LogitArgs a{};
-  a.W = weight_operand(c, weight);
+  if (p.as_is)
+    a.W32 = weight_operand32(c, weight);
+  else
+    a.W = weight_operand(c, weight);
   a.X = hidden_operand(c);
   a.ti = p.logits.ti;
   a.tj = p.logits.tj;
@@ -1040,7 +1087,10 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
     g.factor = factor;
     g.part = (float*)(c.w + p.part);
     if (grad_hidden) {
-      g.P = weight_operand(c, weight);
+      if (p.as_is)
+        g.P32 = weight_operand32(c, weight);
+      else
+        g.P = weight_operand(c, weight);
       g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, 0};
       g.ti = p.dh.ti;
       g.tj = p.dh.tj;

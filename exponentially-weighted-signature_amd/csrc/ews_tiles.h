@@ -62,8 +62,8 @@ struct Tile {
 };
 
 constexpr int kPairs = 6;
-__device__ __forceinline__ int piece_p(int pair) { return (0x001102 >> (4 * pair)) & 15; }  // 2 0 1 1 0 0
-__device__ __forceinline__ int piece_q(int pair) { return (0x010120 >> (4 * pair)) & 15; }  // 0 2 1 0 1 0
+__device__ __forceinline__ constexpr int piece_p(int pair) { return (0x001102 >> (4 * pair)) & 15; }  // 2 0 1 1 0 0
+__device__ __forceinline__ constexpr int piece_q(int pair) { return (0x010120 >> (4 * pair)) & 15; }  // 0 2 1 0 1 0
 
 __device__ __forceinline__ int place(int row, int piece) { return piece ^ ((row >> 1) & 7); }
 template <int WIDTH>
@@ -74,6 +74,22 @@ __device__ __forceinline__ int place_turned(int k, int piece) {
 typedef __attribute__((address_space(3))) void lds_void;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// BYTES (16 or 4) a lane from `from` + offset to `to` on. Written out, not a builtin: before every transposing read the compiler
+// would wait for all the copies that it knows of. It has no result in a register; who reads what it wrote waits in
+// arrive().
+template <int BYTES = 16>
+__device__ __forceinline__ void copy_piece(const void* from, uint32_t offset, char* to) {
+  const uint64_t at = (uint64_t)from;
+  const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)to;
+  if (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc)
+                 : "memory", "m0");
+}
 
 // One operand of a tile, WIDTH results wide: what each thread copies of a stage.
 template <bool TURNED, int WIDTH, int THREADS>
@@ -117,15 +133,9 @@ struct Copier {
     if (rows - kb * 64 < 64) aim_turned(rows - 1 - kb * 64);
     return base + piece * plane + (int64_t)kb * 64 * (stride / 2);
   }
-  // One of the copies; `to`: this wavefront's kilobyte of the stage. Written out, not a builtin: before every
-  // transposing read the compiler would wait for all the copies that it knows of. It has no result in a register; what
-  // is read of it waits in arrive().
+  // One of the copies; `to`: this wavefront's kilobyte of the stage.
   __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const {
-    const uint64_t at = (uint64_t)from;
-    const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, 0xffffffffu, 0x00020000u};
-    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)(to + c * THREADS * 16);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset[c]), "s"(rsrc)
-                 : "memory", "m0");
+    copy_piece(from, offset[c], to + c * THREADS * 16);
   }
 };
 
