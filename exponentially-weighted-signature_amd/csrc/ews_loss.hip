@@ -21,7 +21,8 @@
 //             logit, so a target of probability near one loses nothing. The mean's factor stays out of it: most
 //             targets' entries are near -1, which bfloat16 holds, while their common factor's rounding would scale
 //             the whole gradient.
-//   k_grad    dh and dW, sums in float32, reading W, h and dz as they are, with k along their rows. Few tiles are split over k and joined in order by k_reduce.
+//   k_grad    dh and dW, sums in float32, reading W, h and dz as they are, with k along their rows. Few tiles are
+//             split over k and joined in order by k_reduce.
 //
 // It is kept for kChunkBytes of rows at a time; dW is summed over the chunks in float32. Nothing is added with
 // atomics: the same inputs give the same bits.
@@ -393,7 +394,7 @@ struct DzArgs {
   Rows rows;
   Stats st;
   const float* upstream;  // (N) or null: 1 (k_grad applies the reduction's factor)
-  int c0, chunk, slab, slabs;
+  int c0, chunk, slab;
   void* prob;
   int64_t ld;             // the vocabulary padded to a multiple of 64
   uint16_t* dz;           // planes (chunk, ld): in bfloat16 prob itself; zero rows up to a multiple of 64
@@ -402,7 +403,6 @@ struct DzArgs {
   int each;               // rows a workgroup goes over, one wavefront a row, 512 columns wide
   float* loss;            // or null: the call's loss, by one further workgroup
 };
-
 
 template <int NP>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
@@ -637,12 +637,13 @@ using namespace ews::loss;
 
 // Rows kept at a time: exp(z - m), and dz in its place (float32: dz in three planes beside it), of as many as fit here.
 constexpr int64_t kChunkBytes = (int64_t)2 << 30;
-// float32 W is read as it is for up to so many rows, else packed into planes first. H=2048 V=30000, packing, logits and dh:
-// N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54.
+// float32 W is read as it is for up to so many rows, else packed into planes first. H=2048 V=30000, packing, logits and
+// dh: N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54.
 constexpr int kFewRows32 = 256;
 constexpr int64_t kScoreRows = 65536;  // rows of a call without gradients whose slabs' sums are kept at a time
 
-constexpr int kLongProduct = 8;  // stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared
+// Stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared.
+constexpr int kLongProduct = 8;
 
 enum Kind { kLarge, kMedium, kFlat, kFew32, kMore32 };
 
@@ -836,7 +837,8 @@ template <class T, bool ROWS, typename O, int kP = sizeof(O) == 4 ? kPairs : 1>
 int launch_grad_as(const GradArgs& a, hipStream_t st) {
   const int rc = allow_lds(k_grad<T, kP, ROWS, O>, T::kLdsBytes);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_grad<T, kP, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), T::kLdsBytes, st, a);
+  hipLaunchKernelGGL((k_grad<T, kP, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads),
+                     T::kLdsBytes, st, a);
   LOSS_CHECK();
   if (a.splits > 1) {
     const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * a.I;
@@ -1003,6 +1005,94 @@ int launch_total(const Call& c, float* loss) {
   return EWS_OK;
 }
 
+// Chunk k's gradients from what logits() kept of it; the last chunk writes the call's loss too, where asked.
+int gradients(const Call& c, const void* weight, int k, const float* upstream, float* loss, void* grad_hidden,
+              void* grad_weight, void* grad_bias) {
+  const LPlan& p = c.p;
+  const bool f32 = p.np == 3, last = k + 1 == p.chunks;
+  const int wide = p.H % 8 == 0 && (uintptr_t)grad_hidden % 16 == 0 && (uintptr_t)grad_weight % 16 == 0;
+  const float* factor = upstream ? nullptr : c.rows.scale;
+  int rc;
+  DzArgs z{};
+  z.rows = c.rows;
+  z.st = c.stats;
+  z.upstream = upstream;
+  z.c0 = (int)(k * p.chunk);
+  z.chunk = (int)p.chunk;
+  z.slab = p.logits.slab;
+  z.prob = c.w + p.prob;
+  z.ld = p.Vp;
+  z.dz = (uint16_t*)(c.w + p.dz);
+  z.plane = p.chunk * p.Vp;
+  z.bias = grad_bias ? (float*)(c.w + p.dbias) : nullptr;
+  z.each = p.dz_rows;
+  z.loss = last ? loss : nullptr;
+  const dim3 grid(ceil_div(p.Vp, 512) + (z.loss ? 1 : 0), ceil_div(p.chunk, p.dz_rows));
+  if (f32)
+    hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
+  else
+    hipLaunchKernelGGL((k_dz<1>), grid, dim3(256), 0, c.st, z);
+  LOSS_CHECK();
+  if (grad_bias) {
+    float* sum = (float*)(c.w + p.dbsum);
+    const dim3 g(ceil_div(p.V, 256));
+    if (c.s->bias_dtype == EWS_DTYPE_BF16)
+      hipLaunchKernelGGL((k_dbias<bf16>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0,
+                         factor, last ? (bf16*)grad_bias : nullptr);
+    else
+      hipLaunchKernelGGL((k_dbias<float>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0,
+                         factor, last ? (float*)grad_bias : nullptr);
+    LOSS_CHECK();
+  }
+  GradArgs g{};
+  g.c0 = z.c0;
+  g.chunk = z.chunk;
+  g.rows = c.rows;
+  g.wide = wide;
+  g.factor = factor;
+  g.part = (float*)(c.w + p.part);
+  if (grad_hidden) {
+    if (p.as_is)
+      g.P32 = weight_operand32(c, weight);
+    else
+      g.P = weight_operand(c, weight);
+    g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, 0};
+    g.ti = p.dh.ti;
+    g.tj = p.dh.tj;
+    g.splits = p.dh.splits;
+    g.kblocks = p.dh.kblocks;
+    g.per = p.dh.per;
+    g.by_rows = 0;
+    g.I = p.H;
+    g.J = (int)p.chunk;
+    g.sum = nullptr;
+    g.add = 0;
+    g.out = grad_hidden;
+    rc = f32 ? launch_grad<false, float>(p.dh.kind, g, c.st) : launch_grad<false, bf16>(p.dh.kind, g, c.st);
+    if (rc != EWS_OK) return rc;
+  }
+  if (grad_weight) {
+    g.P = hidden_operand(c);
+    g.P.p += z.c0 * p.Hp;
+    g.P.rows -= z.c0;
+    g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, (int)p.Vp};
+    g.ti = p.dw.ti;
+    g.tj = p.dw.tj;
+    g.splits = p.dw.splits;
+    g.kblocks = p.dw.kblocks;
+    g.per = p.dw.per;
+    g.by_rows = 1;
+    g.I = p.H;
+    g.J = p.V;
+    g.sum = f32 ? (float*)grad_weight : (float*)(c.w + p.acc);
+    g.add = k > 0 ? 1 : 0;
+    g.out = last || f32 ? grad_weight : nullptr;
+    rc = f32 ? launch_grad<true, float>(p.dw.kind, g, c.st) : launch_grad<true, bf16>(p.dw.kind, g, c.st);
+    if (rc != EWS_OK) return rc;
+  }
+  return EWS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1037,96 +1127,44 @@ int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* we
   if (rc != EWS_OK) return rc;
   if (!hidden || !weight || !targets || !workspace || (grad_bias && !bias)) return EWS_ERR_NULL;
   Call c = make_call(desc, p, workspace, stream);
-  const bool f32 = p.np == 3;
   float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
   rc = begin(c, hidden, weight, bias, targets, rows, grad_hidden);
-  if (rc != EWS_OK) return rc;
-  const int wide = p.H % 8 == 0 && (uintptr_t)grad_hidden % 16 == 0 && (uintptr_t)grad_weight % 16 == 0;
-  const float* factor = upstream ? nullptr : c.rows.scale;
-  for (int k = 0; k < p.chunks; ++k) {
-    const bool last = k + 1 == p.chunks;
+  for (int k = 0; k < p.chunks && rc == EWS_OK; ++k) {
     rc = logits(c, weight, k, rows);
-    if (rc != EWS_OK) return rc;
-    DzArgs z{};
-    z.rows = c.rows;
-    z.st = c.stats;
-    z.upstream = upstream;
-    z.c0 = (int)(k * p.chunk);
-    z.chunk = (int)p.chunk;
-    z.slab = p.logits.slab;
-    z.slabs = p.slabs;
-    z.prob = c.w + p.prob;
-    z.ld = p.Vp;
-    z.dz = (uint16_t*)(c.w + p.dz);
-    z.plane = p.chunk * p.Vp;
-    z.bias = grad_bias ? (float*)(c.w + p.dbias) : nullptr;
-    z.each = p.dz_rows;
-    z.loss = last && !rows ? loss : nullptr;
-    const dim3 grid(ceil_div(p.Vp, 512) + (z.loss ? 1 : 0), ceil_div(p.chunk, p.dz_rows));
-    if (f32)
-      hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
-    else
-      hipLaunchKernelGGL((k_dz<1>), grid, dim3(256), 0, c.st, z);
-    LOSS_CHECK();
-    if (grad_bias) {
-      float* sum = (float*)(c.w + p.dbsum);
-      const dim3 g(ceil_div(p.V, 256));
-      if (desc->bias_dtype == EWS_DTYPE_BF16)
-        hipLaunchKernelGGL((k_dbias<bf16>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0, factor,
-                           last ? (bf16*)grad_bias : nullptr);
-      else
-        hipLaunchKernelGGL((k_dbias<float>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0, factor,
-                           last ? (float*)grad_bias : nullptr);
-      LOSS_CHECK();
-    }
-    GradArgs g{};
-    g.c0 = z.c0;
-    g.chunk = z.chunk;
-    g.rows = c.rows;
-    g.wide = wide;
-    g.factor = factor;
-    g.part = (float*)(c.w + p.part);
-    if (grad_hidden) {
-      if (p.as_is)
-        g.P32 = weight_operand32(c, weight);
-      else
-        g.P = weight_operand(c, weight);
-      g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, 0};
-      g.ti = p.dh.ti;
-      g.tj = p.dh.tj;
-      g.splits = p.dh.splits;
-      g.kblocks = p.dh.kblocks;
-      g.per = p.dh.per;
-      g.by_rows = 0;
-      g.I = p.H;
-      g.J = (int)p.chunk;
-      g.sum = nullptr;
-      g.add = 0;
-      g.out = grad_hidden;
-      rc = f32 ? launch_grad<false, float>(p.dh.kind, g, c.st) : launch_grad<false, bf16>(p.dh.kind, g, c.st);
-      if (rc != EWS_OK) return rc;
-    }
-    if (grad_weight) {
-      g.P = hidden_operand(c);
-      g.P.p += z.c0 * p.Hp;
-      g.P.rows -= z.c0;
-      g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, (int)p.Vp};
-      g.ti = p.dw.ti;
-      g.tj = p.dw.tj;
-      g.splits = p.dw.splits;
-      g.kblocks = p.dw.kblocks;
-      g.per = p.dw.per;
-      g.by_rows = 1;
-      g.I = p.H;
-      g.J = p.V;
-      g.sum = f32 ? (float*)grad_weight : (float*)(c.w + p.acc);
-      g.add = k > 0 ? 1 : 0;
-      g.out = last || f32 ? grad_weight : nullptr;
-      rc = f32 ? launch_grad<true, float>(p.dw.kind, g, c.st) : launch_grad<true, bf16>(p.dw.kind, g, c.st);
-      if (rc != EWS_OK) return rc;
-    }
+    if (rc == EWS_OK)
+      rc = gradients(c, weight, k, upstream, rows ? nullptr : loss, grad_hidden, grad_weight, grad_bias);
   }
-  return EWS_OK;
+  return rc;
+}
+
+int ews_loss_keeps(const ews_loss_desc* desc) {
+  LPlan p;
+  return loss_plan(desc, true, false, p) == EWS_OK && p.chunks == 1;
+}
+
+int ews_loss_keep(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
+                  const int64_t* targets, float* loss, void* grad_hidden, void* workspace, ews_stream_t stream) {
+  LPlan p;
+  int rc = loss_plan(desc, true, desc && reads_direct(desc, weight), p);
+  if (rc != EWS_OK) return rc;
+  if (p.chunks > 1) return EWS_ERR_SHAPE;
+  if (!hidden || !weight || !targets || !loss || !workspace) return EWS_ERR_NULL;
+  Call c = make_call(desc, p, workspace, stream);
+  float* rows = desc->reduction == EWS_LOSS_NONE ? loss : nullptr;
+  rc = begin(c, hidden, weight, bias, targets, rows, grad_hidden);
+  if (rc == EWS_OK) rc = logits(c, weight, 0, rows);
+  return rc != EWS_OK || rows ? rc : launch_total(c, loss);
+}
+
+int ews_loss_kept(const ews_loss_desc* desc, const void* weight, const float* upstream, void* grad_hidden,
+                  void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream) {
+  LPlan p;
+  const int rc = loss_plan(desc, true, desc && reads_direct(desc, weight), p);
+  if (rc != EWS_OK) return rc;
+  if (p.chunks > 1) return EWS_ERR_SHAPE;
+  if (!weight || !workspace) return EWS_ERR_NULL;
+  return gradients(make_call(desc, p, workspace, stream), weight, 0, upstream, nullptr, grad_hidden, grad_weight,
+                   grad_bias);
 }
 
 }  // extern "C"

@@ -96,6 +96,9 @@ EXPORTED = (
     "ews_loss_workspace_bytes",
     "ews_loss_forward",
     "ews_loss_train",
+    "ews_loss_keeps",
+    "ews_loss_keep",
+    "ews_loss_kept",
     "ews_clip_workspace_bytes",
     "ews_clip",
     "ews_loss_scale",
@@ -439,6 +442,12 @@ def load():
     lib.ews_loss_forward.restype = i32
     lib.ews_loss_train.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.ews_loss_train.restype = i32
+    lib.ews_loss_keeps.argtypes = [lsp]
+    lib.ews_loss_keeps.restype = i32
+    lib.ews_loss_keep.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_loss_keep.restype = i32
+    lib.ews_loss_kept.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_loss_kept.restype = i32
     lib.ews_clip_workspace_bytes.argtypes = [i32, vp]
     lib.ews_clip_workspace_bytes.restype = sz
     lib.ews_clip.argtypes = [i32, vp, vp, vp, vp, ctypes.c_float, i32, vp, vp, vp]

@@ -10,72 +10,105 @@ from . import _native as nat
 from .embed import DTYPES, check_tensor, launch, row_major
 
 
-def _desc(hidden, hs, weight, wst, bias, ignore_index, reduction):
-    return nat.LossDesc(hs, wst, ignore_index, hidden.shape[0], weight.shape[1], weight.shape[0], DTYPES[weight.dtype],
-                        nat.DTYPE_F32 if bias is None else DTYPES[bias.dtype], nat.LOSS_REDUCTIONS[reduction])
-
-
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _run(hidden, weight, bias, targets, ignore_index, reduction, needs, upstream=None, want_loss=True):
-    """(loss, [grad_hidden, grad_weight, grad_bias], descriptor); the gradients that ``needs`` asks for, None for the
-    others, and no descriptor where there are no rows."""
-    lib = nat.load()
-    dev = weight.device
-    n = hidden.shape[0]
-    loss = torch.empty((n,) if reduction == "none" else (), device=dev, dtype=torch.float32) if want_loss else None
-    grads = [torch.empty(t.shape, device=dev, dtype=t.dtype) if need else None
-             for t, need in zip((hidden, weight, bias), needs)]
-    if n == 0:  # no rows: the sum and the mean of nothing are 0
-        if loss is not None:
-            loss.zero_()
-        return loss, [None if g is None else g.zero_() for g in grads], None
-    hidden, hs = row_major(hidden)
-    weight, wst = row_major(weight)
-    bias = None if bias is None else bias.contiguous()
-    desc = _desc(hidden, hs, weight, wst, bias, ignore_index, reduction)
-    train = any(needs)
-    ws = torch.empty(lib.ews_loss_workspace_bytes(desc, int(train)), device=dev, dtype=torch.uint8)
-    if train:
-        nat.check(launch(dev, lib.ews_loss_train, desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias),
-                         targets.data_ptr(), _ptr(upstream), _ptr(loss), *(_ptr(g) for g in grads), ws.data_ptr()),
-                  "ews_loss_train")
-    else:
-        nat.check(launch(dev, lib.ews_loss_forward, desc, hidden.data_ptr(), weight.data_ptr(), _ptr(bias),
-                         targets.data_ptr(), loss.data_ptr(), ws.data_ptr()), "ews_loss_forward")
-    return loss, grads, desc
+class _Call:
+    """One call's operands as the library takes them."""
+
+    def __init__(self, hidden, weight, bias, targets, ignore_index, reduction):
+        self.hidden, hs = row_major(hidden)
+        self.weight, wst = row_major(weight)
+        self.bias = None if bias is None else bias.contiguous()
+        self.targets, self.reduction, self.dev = targets, reduction, weight.device
+        self.desc = nat.LossDesc(hs, wst, ignore_index, hidden.shape[0], weight.shape[1], weight.shape[0],
+                                 DTYPES[weight.dtype], nat.DTYPE_F32 if bias is None else DTYPES[bias.dtype],
+                                 nat.LOSS_REDUCTIONS[reduction])
+
+    def workspace(self, train):
+        return torch.empty(nat.load().ews_loss_workspace_bytes(self.desc, train), device=self.dev, dtype=torch.uint8)
+
+    def inputs(self):
+        return self.desc, self.hidden.data_ptr(), self.weight.data_ptr(), _ptr(self.bias), self.targets.data_ptr()
+
+    def loss(self):
+        return torch.empty((self.desc.rows,) if self.reduction == "none" else (), device=self.dev, dtype=torch.float32)
+
+    def grads(self, needs):
+        return [torch.empty(t.shape, device=self.dev, dtype=t.dtype) if need else None
+                for t, need in zip((self.hidden, self.weight, self.bias), needs)]
+
+    def forward(self):
+        loss, ws = self.loss(), self.workspace(0)
+        nat.check(launch(self.dev, nat.load().ews_loss_forward, *self.inputs(), loss.data_ptr(), ws.data_ptr()),
+                  "ews_loss_forward")
+        return loss
+
+    def train(self, needs, upstream=None, want_loss=True):
+        """(loss or None, the gradients that ``needs`` asks for) of one pass over the rows."""
+        loss, grads, ws = self.loss() if want_loss else None, self.grads(needs), self.workspace(1)
+        nat.check(launch(self.dev, nat.load().ews_loss_train, *self.inputs(), _ptr(upstream), _ptr(loss),
+                         *map(_ptr, grads), ws.data_ptr()), "ews_loss_train")
+        return loss, grads
+
+    def keep(self, need_hidden):
+        """The rows' losses, and what ``kept`` forms the gradients from: hidden's and the workspace."""
+        loss, (gh, _, _), ws = self.loss(), self.grads((need_hidden, False, False)), self.workspace(1)
+        nat.check(launch(self.dev, nat.load().ews_loss_keep, *self.inputs(), loss.data_ptr(), _ptr(gh), ws.data_ptr()),
+                  "ews_loss_keep")
+        return loss, (gh, ws)
+
+    def kept(self, needs, upstream, state):
+        gh, ws = state
+        grads = [gh, *self.grads((False, *needs[1:]))[1:]]
+        nat.check(launch(self.dev, nat.load().ews_loss_kept, self.desc, self.weight.data_ptr(), upstream.data_ptr(),
+                         *map(_ptr, grads), ws.data_ptr()), "ews_loss_kept")
+        return grads
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     """The mean and the sum have one upstream number, so their forward computes the gradients with the loss in one pass
-    over the rows (ews_loss_train) and the first backward scales them; a second backward of the same graph, and the
-    rows' own losses, compute them in the backward."""
+    over the rows and the first backward scales them. The rows' own losses keep the probabilities for the first
+    backward, where they fit the scratch (2 GiB). A second backward of the same graph, and the rows' own losses of
+    more, compute the probabilities once more."""
 
     @staticmethod
     def forward(ctx, hidden, weight, bias, targets, ignore_index, reduction):
         ctx.save_for_backward(hidden, weight, bias, targets)
         ctx.args = (ignore_index, reduction)
-        needs = ctx.needs_input_grad[:3] if reduction != "none" else (False, False, False)
-        loss, grads, ctx.desc = _run(hidden, weight, bias, targets, ignore_index, reduction, needs)
-        ctx.grads = grads if any(needs) else None
+        ctx.first = None
+        needs = ctx.needs_input_grad[:3]
+        call = _Call(hidden, weight, bias, targets, ignore_index, reduction)
+        if reduction != "none":
+            loss, grads = call.train(needs)
+            ctx.first = call.desc, grads
+        elif nat.load().ews_loss_keeps(call.desc):
+            loss, state = call.keep(needs[0])
+            ctx.first = call, state
+        else:
+            loss = call.forward()
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        ignore_index, reduction = ctx.args
+        inputs = ctx.saved_tensors  # refused where one has been changed since
+        needs, none = ctx.needs_input_grad[:3], ctx.args[1] == "none"
         if gout.dtype is not torch.float32 or not gout.is_contiguous():
             gout = gout.to(torch.float32).contiguous()
-        grads, ctx.grads = ctx.grads, None
-        if grads is None:
-            hidden, weight, bias, targets = ctx.saved_tensors
-            _, grads, ctx.desc = _run(hidden, weight, bias, targets, ignore_index, reduction, ctx.needs_input_grad[:3],
-                                      upstream=gout if reduction == "none" else None, want_loss=False)
-        if reduction != "none" and ctx.desc is not None:
-            nat.check(launch(gout.device, nat.load().ews_loss_scale, ctx.desc, *(_ptr(g) for g in grads),
-                             gout.data_ptr()), "ews_loss_scale")
+        first, ctx.first = ctx.first, None
+        if first is None:
+            call = _Call(*inputs, *ctx.args)
+            desc, grads = call.desc, call.train(needs, upstream=gout if none else None, want_loss=False)[1]
+        elif none:
+            call, state = first
+            grads = call.kept(needs, gout, state)
+        else:
+            desc, grads = first
+        if not none:
+            nat.check(launch(gout.device, nat.load().ews_loss_scale, desc, *map(_ptr, grads), gout.data_ptr()),
+                      "ews_loss_scale")
         return (*grads, None, None, None)
 
 
@@ -117,9 +150,12 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     t = targets if targets.dim() == 1 else targets.reshape(-1)
     if t.dtype is not torch.int64 or not t.is_contiguous():
         t = t.to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
+    if rows.shape[0] == 0:  # the sum and the mean of nothing are 0, and so are their gradients
+        zero = sum(x[:0].sum(dtype=torch.float32) for x in (rows, weight, bias) if x is not None)
+        loss = zero.expand(0) if reduction == "none" else zero
+    elif torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or
+                                      (bias is not None and bias.requires_grad)):
         loss = _LinearCrossEntropy.apply(rows, weight, bias, t, int(ignore_index), reduction)
     else:
-        loss = _run(rows, weight, bias, t, int(ignore_index), reduction, (False, False, False))[0]
+        loss = _Call(rows, weight, bias, t, int(ignore_index), reduction).forward()
     return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss

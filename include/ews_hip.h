@@ -634,8 +634,8 @@ typedef struct ews_loss_desc {
   int32_t reduction;     /* EWS_LOSS_* */
 } ews_loss_desc;
 
-/* Scratch of one call (train != 0: of ews_loss_train). It does not grow with N V: a training call keeps 2 GiB of
- * probabilities and their transpose at most. */
+/* Scratch of one call (train != 0: of ews_loss_train and ews_loss_keep). It does not grow with N V: a training call
+ * keeps 2 GiB of probabilities at most (of 256 rows where those need more). */
 size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train);
 
 /* z = hidden weight^T + bias (bias may be NULL; entries of -inf take a token out of the vocabulary),
@@ -648,6 +648,16 @@ int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* 
 int ews_loss_train(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
                    const int64_t* targets, const float* upstream, float* loss, void* grad_hidden, void* grad_weight,
                    void* grad_bias, void* workspace, ews_stream_t stream);
+
+/* ews_loss_train in two calls, for a caller that has upstream only after the loss: ews_loss_keep writes the loss and
+ * leaves in workspace what ews_loss_kept, once, forms the gradients from. Both take the same desc, weight, grad_hidden
+ * (the first zeroes its ignored rows) and workspace. Only where ews_loss_keeps(desc) is 1, that is, where all rows'
+ * probabilities fit the scratch; else EWS_ERR_SHAPE. */
+int ews_loss_keeps(const ews_loss_desc* desc);
+int ews_loss_keep(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
+                  const int64_t* targets, float* loss, void* grad_hidden, void* workspace, ews_stream_t stream);
+int ews_loss_kept(const ews_loss_desc* desc, const void* weight, const float* upstream, void* grad_hidden,
+                  void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream);
 
 /* grad_* = factor[0] grad_* in place (each may be NULL), factor on the device: the gradients of factor[0] times the loss.
  * With a factor of 1 nothing is touched. */

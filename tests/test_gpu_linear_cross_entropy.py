@@ -283,6 +283,27 @@ def test_another_stream_and_the_same_bits():
         assert torch.equal(a, r)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N", [1, 70, 301])
+def test_kept_probabilities_and_new_ones_give_the_same_bits(N, dtype):
+    """The first backward of the rows' own losses forms the gradients from what the forward kept, a second one (whose
+    upstream may differ) computes it again."""
+    h, w, b, t = _inputs(N, 136, 500, dtype, bias=torch.float32, ignored=0.2 if N > 1 else 0.0)
+    wrt = [x.requires_grad_() for x in (h, w, b)]
+    up = torch.rand(N, device=DEV) + 0.5
+    rows = E.linear_cross_entropy(h, w, t, bias=b, reduction="none")
+    first = torch.autograd.grad(rows, wrt, up, retain_graph=True)
+    other = torch.autograd.grad(rows, wrt, up * 2.0, retain_graph=True)
+    again = torch.autograd.grad(rows, wrt, up)
+    for a, c, d in zip(first, other, again):
+        assert torch.equal(a, d) and torch.equal(c, a * 2.0)
+    rows = E.linear_cross_entropy(h, w, t, bias=b, reduction="none")
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(rows, wrt, up)
+
+
 def test_second_derivatives_are_refused():
     h, w, b, t = _inputs(6, 16, 20, torch.float32, bias=torch.float32)
     h.requires_grad_()
