@@ -112,9 +112,9 @@ def clip_grads(grads, max_norm, out=None):
 def clip_grad_norm_(parameters, max_norm):
     """Scales the gradients of ``parameters`` (an iterable, or one) in place by ``min(1, max_norm / (norm + 1e-6))`` and
     returns their norm, a float32 number on the device; the host does not wait. Parameters without a gradient are left
-    out. A norm that is not finite scales by 0 (infinite) or NaN, as the formula does."""
+    out, and one that is named twice counts once. A norm that is not finite scales by 0 (infinite) or NaN, as the formula does."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = list(dict.fromkeys(p.grad for p in parameters if p.grad is not None))
     max_norm = _max_norm(max_norm)
     if not grads:
         return torch.zeros(())

@@ -138,3 +138,11 @@ def test_refusals_on_the_device():
                        (lambda: E.global_grad_norm([g.to_sparse()]), TypeError)):
         with pytest.raises(kind):
             call()
+
+
+def test_a_parameter_named_twice_counts_once():
+    (g,) = _tensors([(70, 33)], [torch.float32])
+    p = torch.zeros_like(g).requires_grad_()
+    p.grad = g.clone()
+    norm = E.clip_grad_norm_([p, p], 0.5)
+    _check([g], 0.5, norm, [p.grad])
