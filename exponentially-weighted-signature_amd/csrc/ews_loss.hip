@@ -241,10 +241,19 @@ struct LogitArgs {
   int64_t ldp;
 };
 
+// A product of one stage needs no second half: more workgroups share a CU.
+template <class T, int PAIRS>
+__host__ __device__ constexpr int lds_bytes(int kblocks) {
+  if constexpr (PAIRS == 1) {
+    if (kblocks == 1) return T::kLdsBytesOne;
+  }
+  return T::kLdsBytes;
+}
+
 // PAIRS: 1, kPairs for planes, or 0 for float32 W. KEEP: 0 the loss alone, 1 also 16-bit logarithms, 2 also float32
 // probabilities.
 template <class T, int PAIRS, int KEEP>
-__global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
+__global__ __launch_bounds__(T::kThreads, T::kWaves) void k_logits(LogitArgs a) {
   extern __shared__ char lds[];
   int it, jt;
   tile_of(blockIdx.x, a.ti, a.tj, it, jt);
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(T::kThreads) void k_logits(LogitArgs a) {
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   if (j0 >= live) return;
   // the epilogue's operands, where it need not wait for them
-  float* tile_bias = reinterpret_cast<float*>(lds + T::kLdsBytes);
+  float* tile_bias = reinterpret_cast<float*>(lds + lds_bytes<T, PAIRS>(a.kblocks));
   int* tile_target = reinterpret_cast<int*>(tile_bias + T::I);
   for (int t = threadIdx.x; t < T::I + T::J; t += T::kThreads) {
     if (t < T::I)
@@ -537,7 +546,7 @@ __device__ __forceinline__ void finish(const GradArgs& a, int64_t row, int i, co
   for (int q = 0; q < 8; q += kWide<T>) {
     Pack<T, kWide<T>> p;
     p.set(y + q);
-    p.store((T*)a.out + at + q);
+    p.store_past((T*)a.out + at + q);
   }
 }
 
@@ -564,7 +573,7 @@ __device__ __forceinline__ void keep(float* to, const One& e) { *to = e.x; }
 
 // ROWS: dW, whose k is the chunk's kept rows and whose operands are both turned; else dh, whose rows they are.
 template <class T, int PAIRS, bool ROWS, typename O>
-__global__ __launch_bounds__(T::kThreads) void k_grad(GradArgs a) {
+__global__ __launch_bounds__(T::kThreads, T::kWaves) void k_grad(GradArgs a) {
   extern __shared__ char lds[];
   const int split = blockIdx.y;
   int it, jt;
@@ -812,10 +821,10 @@ bool pieces(const Operand32& o) { return (uintptr_t)o.p % 16 == 0 && o.ld % 4 ==
 
 template <class T, int PAIRS, int KEEP>
 int launch_logits_as(const LogitArgs& a, hipStream_t st) {
-  constexpr int kLds = T::kLdsBytes + (T::I + T::J) * 4;
-  const int rc = allow_lds(k_logits<T, PAIRS, KEEP>, kLds);
+  const int lds = lds_bytes<T, PAIRS>(a.kblocks) + (T::I + T::J) * 4;
+  const int rc = allow_lds(k_logits<T, PAIRS, KEEP>, lds);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_logits<T, PAIRS, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), kLds, st, a);
+  hipLaunchKernelGGL((k_logits<T, PAIRS, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), lds, st, a);
   LOSS_CHECK();
   return EWS_OK;
 }
@@ -835,10 +844,10 @@ int launch_logits(Kind kind, const LogitArgs& a, hipStream_t st) {
 // kP: float32 gradients are those of float32 operands
 template <class T, bool ROWS, typename O, int kP = sizeof(O) == 4 ? kPairs : 1>
 int launch_grad_as(const GradArgs& a, hipStream_t st) {
-  const int rc = allow_lds(k_grad<T, kP, ROWS, O>, T::kLdsBytes);
+  const int lds = lds_bytes<T, kP>(a.per);
+  const int rc = allow_lds(k_grad<T, kP, ROWS, O>, lds);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_grad<T, kP, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads),
-                     T::kLdsBytes, st, a);
+  hipLaunchKernelGGL((k_grad<T, kP, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), lds, st, a);
   LOSS_CHECK();
   if (a.splits > 1) {
     const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * a.I;

@@ -51,6 +51,7 @@ struct Tile {
   static constexpr int WI = WI_, WJ = WJ_, TI = TI_, TJ = TJ_;
   static constexpr int I = 32 * TI * WI, J = 32 * TJ * WJ;
   static constexpr int kThreads = 64 * WI * WJ;
+  static constexpr int kWaves = TI * TJ > 4 ? 2 : 4;       // on a SIMD, as far as registers go
   static constexpr int kSlab = 32 * TI;                    // consecutive i of one wavefront
   static constexpr int kRowWords = kSlab + 4;              // a staged result row, padded off the banks
   static constexpr int kStageBytes = WI * WJ * 32 * kRowWords * 4;
@@ -59,6 +60,7 @@ struct Tile {
   static constexpr int kBytesP = kCopiesP * kThreads * 16;
   static constexpr int kStage = (kCopiesP + kCopiesQ) * kThreads * 16;
   static constexpr int kLdsBytes = kStageBytes > 2 * kStage ? kStageBytes : 2 * kStage;
+  static constexpr int kLdsBytesOne = kStageBytes > kStage ? kStageBytes : kStage;  // for products of one stage
 };
 
 constexpr int kPairs = 6;
@@ -197,14 +199,12 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
   const int stages = (kb1 - kb0) * PAIRS;
   constexpr int kCopies = T::kCopiesP + T::kCopiesQ, kReads = T::TI + T::TJ, kProducts = T::TI * T::TJ;
   constexpr int kMost = kReads > kProducts ? kReads : kProducts, kSlots = kMost > kCopies ? kMost : kCopies;
-  // past the last stage the copies repeat it, into a half that nobody reads again
   const uint16_t *fromP, *fromQ;
   char* to;
   auto aim = [&](int s) {
-    const int t = s < stages ? s : stages - 1;
-    const int pair = PAIRS == 1 ? kPairs - 1 : t % PAIRS;
-    fromP = cp.at(piece_p(pair), kb0 + t / PAIRS);
-    fromQ = cq.at(piece_q(pair), kb0 + t / PAIRS);
+    const int pair = PAIRS == 1 ? kPairs - 1 : s % PAIRS;
+    fromP = cp.at(piece_p(pair), kb0 + s / PAIRS);
+    fromQ = cq.at(piece_q(pair), kb0 + s / PAIRS);
     to = lds + (s & 1) * T::kStage + wave * 1024;
   };
   auto copy = [&](int c) {
@@ -247,14 +247,16 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
   for (int a = 0; a < T::TI; ++a) odd.p[a] = zero;
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) odd.q[b] = zero;
-  for (int s = 0; s < stages; ++s) {
+  auto stage = [&](int s, bool copies) {
     arrive<0>();
-    aim(s + 1);
-    multiply(odd, even, s, 0, true);  // the stage before's last sixteen (at first nothing)
+    if (copies) aim(s + 1);
+    multiply(odd, even, s, 0, copies);  // the stage before's last sixteen (at first nothing)
     multiply(even, odd, s, 1, false);
     multiply(odd, even, s, 2, false);
     multiply(even, odd, s, 3, false);
-  }
+  };
+  for (int s = 0; s + 1 < stages; ++s) stage(s, true);
+  stage(stages - 1, false);
 #pragma unroll
   for (int a = 0; a < T::TI; ++a)
 #pragma unroll

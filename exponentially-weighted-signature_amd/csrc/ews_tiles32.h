@@ -18,6 +18,7 @@ struct Tile32 {
   static constexpr int WI = 4, WJ = 1, TI = 1, TJ = TJ_;
   static constexpr int I = 128, J = 32 * TJ;
   static constexpr int kThreads = 256;
+  static constexpr int kWaves = 4;
   static constexpr int kSlab = 32;
   static constexpr int kRowWords = kSlab + 4;
   static constexpr int kStageBytes = WI * 32 * kRowWords * 4;

@@ -48,6 +48,9 @@ struct Pack<float, 4> {
   __device__ __forceinline__ float get(int i) const { return w[i]; }
   __device__ __forceinline__ void set(const float* x) { w = f32x4{x[0], x[1], x[2], x[3]}; }
   __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<f32x4*>(p) = w; }
+  __device__ __forceinline__ void store_past(float* p) const {
+    __builtin_nontemporal_store(w, reinterpret_cast<f32x4*>(p));
+  }
 };
 
 template <>
@@ -62,6 +65,9 @@ struct Pack<bf16, 8> {
     w = u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
   }
   __device__ __forceinline__ void store(bf16* p) const { *reinterpret_cast<u32x4*>(p) = w; }
+  __device__ __forceinline__ void store_past(bf16* p) const {
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+  }
 };
 
 template <typename T>
