@@ -610,8 +610,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_grad(GradArgs a) {
     rows(One{});
 }
 
-// The splits' results added in order: 32 results a workgroup, its eight groups of lanes a contiguous part of the splits
-// each, joined in LDS.
+// The splits' results added in order. Many splits: 32 results a workgroup, its eight groups of lanes a contiguous part of
+// the splits each, joined in LDS.
 template <typename O>
 __global__ __launch_bounds__(256) void k_reduce(GradArgs a) {
   __shared__ float parts[8][32];
@@ -637,6 +637,38 @@ __global__ __launch_bounds__(256) void k_reduce(GradArgs a) {
   finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], (int)(at - j * a.I), One{x});
 }
 
+// Few splits: a thread adds one result's (W: One) or, where rows are wide, eight results'.
+template <typename O, typename W>
+__global__ __launch_bounds__(256) void k_reduce_few(GradArgs a) {
+  constexpr int kEach = sizeof(W) / 4;
+  const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
+  const int nj = a.by_rows ? a.J : live;
+  const int64_t stride = (int64_t)(a.by_rows ? a.J : a.chunk) * a.I;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * kEach;
+  if (at >= (int64_t)nj * a.I) return;
+  float x[kEach];
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) x[q] = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float* from = a.part + s * stride + at;
+    if constexpr (kEach == 1) {
+      x[0] += from[0];
+    } else {
+#pragma unroll
+      for (int q = 0; q < kEach; q += 4) {
+        const f32x4 w = *reinterpret_cast<const f32x4*>(from + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[q + e] += w[e];
+      }
+    }
+  }
+  W w;
+  __builtin_memcpy(&w, x, sizeof(w));
+  const int64_t j = at / a.I;
+  finish<O>(a, a.by_rows ? j : a.rows.map[a.c0 + j], (int)(at - j * a.I), w);
+}
+
 }  // namespace loss
 }  // namespace ews
 
@@ -653,6 +685,9 @@ constexpr int64_t kScoreRows = 65536;  // rows of a call without gradients whose
 
 // Stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared.
 constexpr int kLongProduct = 8;
+
+// Splits that one thread adds: two of 2000 x 256 by 32000 13 us (eight groups of lanes: 60), eight of 4095 x 512 13 (36).
+constexpr int kFewSplits = 8;
 
 enum Kind { kLarge, kMedium, kFlat, kFew32, kMore32 };
 
@@ -851,7 +886,12 @@ int launch_grad_as(const GradArgs& a, hipStream_t st) {
   LOSS_CHECK();
   if (a.splits > 1) {
     const int64_t n = (int64_t)(a.by_rows ? a.J : a.chunk) * a.I;
-    hipLaunchKernelGGL((k_reduce<O>), dim3((uint32_t)((n + 31) / 32)), dim3(256), 0, st, a);
+    if (a.splits > kFewSplits)
+      hipLaunchKernelGGL((k_reduce<O>), dim3((uint32_t)((n + 31) / 32)), dim3(256), 0, st, a);
+    else if (a.wide)
+      hipLaunchKernelGGL((k_reduce_few<O, Eight>), dim3((uint32_t)((n / 8 + 255) / 256)), dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((k_reduce_few<O, One>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
     LOSS_CHECK();
   }
   return EWS_OK;
