@@ -14,10 +14,21 @@ _NO_PADDING = -1
 
 def launch(dev, fn, *args):
     """fn(*args, stream) on dev's current stream, with dev the current device."""
-    if dev.index == torch.cuda.current_device():
+    if dev.index == torch._C._cuda_getDevice():
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     with torch.cuda.device(dev):
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+
+
+def once(backward):
+    """``once_differentiable``, which costs a small call 5 us, where a graph of the backward is asked for; else backward
+    itself."""
+    refusing = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def check_tensor(name, t):
@@ -30,47 +41,49 @@ def check_tensor(name, t):
 def row_major(t):
     """A 2-D tensor whose rows are contiguous and do not overlap (a copy only where they do), and its row stride."""
     n, w = t.shape
+    if t.is_contiguous():
+        return t, w
     if (t.stride(1) != 1 and w > 1) or (t.stride(0) < w and n > 1):
         t = t.contiguous()
     return t, (t.stride(0) if n > 1 else w)
 
 
-def _desc(tokens, weight, stride, scale, padding):
-    return nat.EmbedDesc(tokens.numel(), stride, padding, weight.shape[1], weight.shape[0], DTYPES[weight.dtype],
-                         tokens.element_size(), scale)
-
-
 def _lookup(tokens, weight, scale, padding):
-    out = torch.empty((*tokens.shape, weight.shape[1]), device=weight.device, dtype=weight.dtype)
-    if tokens.numel() == 0:
-        return out
+    """The rows, and the descriptor of the call and of its gradient."""
+    shape = weight.shape
+    out = weight.new_empty((*tokens.shape, shape[1]))
+    n = tokens.numel()
+    if n == 0:
+        return out, None
     weight, stride = row_major(weight)
-    nat.check(launch(weight.device, nat.load().ews_embed_forward, _desc(tokens, weight, stride, scale, padding),
-                     tokens.data_ptr(), weight.data_ptr(), out.data_ptr()), "ews_embed_forward")
-    return out
+    desc = nat.EmbedDesc(n, stride, padding, shape[1], shape[0], DTYPES[weight.dtype], tokens.element_size(), scale)
+    nat.check(launch(weight.device, nat.load().ews_embed_forward, desc, tokens.data_ptr(), weight.data_ptr(),
+                     out.data_ptr()), "ews_embed_forward")
+    return out, desc
 
 
 class _Lookup(torch.autograd.Function):
+    # A small training call costs its host time, and the backward's thread runs Python two to three times slower than
+    # the caller's (each finds the interpreter's memory in the other core's cache): what the backward needs is prepared
+    # in the forward, and every attribute or call spared counts.
     @staticmethod
     def forward(ctx, weight, tokens, scale, padding):
         ctx.save_for_backward(tokens)
-        ctx.args = (weight.shape, weight.dtype, scale, padding)
-        return _lookup(tokens, weight, scale, padding)
+        out, desc = _lookup(tokens, weight, scale, padding)
+        ctx.args = desc, weight.shape, desc and nat.load().ews_embed_workspace_bytes(desc)
+        return out
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, gout):
-        (tokens,) = ctx.saved_tensors
-        shape, dtype, scale, padding = ctx.args
-        grad = torch.empty(shape, device=gout.device, dtype=dtype)
-        if tokens.numel() == 0:
+        desc, shape, size = ctx.args
+        grad = gout.new_empty(shape)
+        if desc is None:
             return grad.zero_(), None, None, None
-        lib = nat.load()
+        (tokens,) = ctx.saved_tensors
         gout = gout.contiguous()
-        desc = _desc(tokens, grad, shape[1], scale, padding)
-        size = lib.ews_embed_workspace_bytes(desc)
-        ws = torch.empty(size, device=gout.device, dtype=torch.uint8) if size else None
-        nat.check(launch(gout.device, lib.ews_embed_backward, desc, tokens.data_ptr(), gout.data_ptr(),
+        ws = gout.new_empty(size, dtype=torch.uint8) if size else None
+        nat.check(launch(gout.device, nat.load().ews_embed_backward, desc, tokens.data_ptr(), gout.data_ptr(),
                          grad.data_ptr(), ws.data_ptr() if size else None), "ews_embed_backward")
         return grad, None, None, None
 
@@ -96,4 +109,4 @@ def embedding_lookup(tokens, weight, scale=1.0, padding_idx=None):
     tokens = tokens.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
         return _Lookup.apply(weight, tokens, float(scale), padding)
-    return _lookup(tokens, weight, float(scale), padding)
+    return _lookup(tokens, weight, float(scale), padding)[0]

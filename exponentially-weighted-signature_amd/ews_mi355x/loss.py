@@ -4,10 +4,9 @@
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .embed import DTYPES, check_tensor, launch, row_major
+from .embed import DTYPES, check_tensor, launch, once, row_major
 
 
 def _ptr(t):
@@ -21,23 +20,24 @@ class _Call:
         self.hidden, hs = row_major(hidden)
         self.weight, wst = row_major(weight)
         self.bias = None if bias is None else bias.contiguous()
-        self.targets, self.reduction, self.dev = targets, reduction, weight.device
-        self.desc = nat.LossDesc(hs, wst, ignore_index, hidden.shape[0], weight.shape[1], weight.shape[0],
-                                 DTYPES[weight.dtype], nat.DTYPE_F32 if bias is None else DTYPES[bias.dtype],
-                                 nat.LOSS_REDUCTIONS[reduction])
+        self.targets, self.dev = targets, weight.device
+        V, H = weight.shape
+        self.desc = nat.LossDesc(hs, wst, ignore_index, hidden.shape[0], H, V, DTYPES[weight.dtype],
+                                 nat.DTYPE_F32 if bias is None else DTYPES[bias.dtype], nat.LOSS_REDUCTIONS[reduction])
 
     def workspace(self, train):
-        return torch.empty(nat.load().ews_loss_workspace_bytes(self.desc, train), device=self.dev, dtype=torch.uint8)
+        return self.hidden.new_empty(nat.load().ews_loss_workspace_bytes(self.desc, train), dtype=torch.uint8)
 
     def inputs(self):
         return self.desc, self.hidden.data_ptr(), self.weight.data_ptr(), _ptr(self.bias), self.targets.data_ptr()
 
     def loss(self):
-        return torch.empty((self.desc.rows,) if self.reduction == "none" else (), device=self.dev, dtype=torch.float32)
+        return self.hidden.new_empty((self.desc.rows,) if self.desc.reduction == 0 else (), dtype=torch.float32)
 
-    def grads(self, needs):
-        return [torch.empty(t.shape, device=self.dev, dtype=t.dtype) if need else None
-                for t, need in zip((self.hidden, self.weight, self.bias), needs)]
+    def grads(self, hidden, weight, bias):
+        return (self.hidden.new_empty(self.hidden.shape) if hidden else None,
+                self.weight.new_empty(self.weight.shape) if weight else None,
+                self.bias.new_empty(self.bias.shape) if bias else None)
 
     def forward(self):
         loss, ws = self.loss(), self.workspace(0)
@@ -47,24 +47,23 @@ class _Call:
 
     def train(self, needs, upstream=None, want_loss=True):
         """(loss or None, the gradients that ``needs`` asks for) of one pass over the rows."""
-        loss, grads, ws = self.loss() if want_loss else None, self.grads(needs), self.workspace(1)
-        nat.check(launch(self.dev, nat.load().ews_loss_train, *self.inputs(), _ptr(upstream), _ptr(loss),
-                         *map(_ptr, grads), ws.data_ptr()), "ews_loss_train")
-        return loss, grads
+        loss, (gh, gw, gb), ws = self.loss() if want_loss else None, self.grads(*needs), self.workspace(1)
+        nat.check(launch(self.dev, nat.load().ews_loss_train, *self.inputs(), _ptr(upstream), _ptr(loss), _ptr(gh),
+                         _ptr(gw), _ptr(gb), ws.data_ptr()), "ews_loss_train")
+        return loss, (gh, gw, gb)
 
     def keep(self, need_hidden):
         """The rows' losses, and what ``kept`` forms the gradients from: hidden's and the workspace."""
-        loss, (gh, _, _), ws = self.loss(), self.grads((need_hidden, False, False)), self.workspace(1)
+        loss, gh, ws = self.loss(), self.grads(need_hidden, False, False)[0], self.workspace(1)
         nat.check(launch(self.dev, nat.load().ews_loss_keep, *self.inputs(), loss.data_ptr(), _ptr(gh), ws.data_ptr()),
                   "ews_loss_keep")
-        return loss, (gh, ws)
+        return loss, gh, ws
 
-    def kept(self, needs, upstream, state):
-        gh, ws = state
-        grads = [gh, *self.grads((False, *needs[1:]))[1:]]
+    def kept(self, needs, upstream, gh, ws):
+        _, gw, gb = self.grads(False, needs[1], needs[2])
         nat.check(launch(self.dev, nat.load().ews_loss_kept, self.desc, self.weight.data_ptr(), upstream.data_ptr(),
-                         *map(_ptr, grads), ws.data_ptr()), "ews_loss_kept")
-        return grads
+                         _ptr(gh), _ptr(gw), _ptr(gb), ws.data_ptr()), "ews_loss_kept")
+        return gh, gw, gb
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -76,40 +75,44 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, targets, ignore_index, reduction):
         ctx.save_for_backward(hidden, weight, bias, targets)
-        ctx.args = (ignore_index, reduction)
-        ctx.first = None
-        needs = ctx.needs_input_grad[:3]
+        needs = ctx.needs_input_grad
         call = _Call(hidden, weight, bias, targets, ignore_index, reduction)
+        first = None
         if reduction != "none":
-            loss, grads = call.train(needs)
-            ctx.first = call.desc, grads
+            loss, grads = call.train(needs[:3])
+            first = call.desc, grads
         elif nat.load().ews_loss_keeps(call.desc):
-            loss, state = call.keep(needs[0])
-            ctx.first = call, state
+            loss, *state = call.keep(needs[0])
+            first = call, state
         else:
             loss = call.forward()
+        ctx.args = first, ignore_index, reduction
         return loss
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, gout):
-        inputs = ctx.saved_tensors  # refused where one has been changed since
-        needs, none = ctx.needs_input_grad[:3], ctx.args[1] == "none"
+        first, ignore_index, reduction = ctx.args
+        ctx.args = None, ignore_index, reduction
+        none = reduction == "none"
         if gout.dtype is not torch.float32 or not gout.is_contiguous():
             gout = gout.to(torch.float32).contiguous()
-        first, ctx.first = ctx.first, None
-        if first is None:
-            call = _Call(*inputs, *ctx.args)
-            desc, grads = call.desc, call.train(needs, upstream=gout if none else None, want_loss=False)[1]
-        elif none:
-            call, state = first
-            grads = call.kept(needs, gout, state)
+        if first is None or none:
+            inputs = ctx.saved_tensors  # refused where one has been changed since
+            needs = ctx.needs_input_grad[:3]
+            call, state = first or (_Call(*inputs, ignore_index, reduction), None)
+            desc = call.desc
+            if state:
+                grads = call.kept(needs, gout, *state)
+            else:
+                grads = call.train(needs, upstream=gout if none else None, want_loss=False)[1]
         else:
             desc, grads = first
+        gh, gw, gb = grads
         if not none:
-            nat.check(launch(gout.device, nat.load().ews_loss_scale, desc, *map(_ptr, grads), gout.data_ptr()),
-                      "ews_loss_scale")
-        return (*grads, None, None, None)
+            nat.check(launch(gout.device, nat.load().ews_loss_scale, desc, _ptr(gh), _ptr(gw), _ptr(gb),
+                             gout.data_ptr()), "ews_loss_scale")
+        return gh, gw, gb, None, None, None
 
 
 def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, reduction="mean"):
