@@ -92,7 +92,7 @@ struct PackArgs {
   int rows, cols;          // of the source (rows: kept[0] where there is a map)
   const int* map;          // gathers the rows; null: all of them
   const int* kept;
-  uint16_t* dst;           // planes (rows, ld), zero in further columns and in rows up to a multiple of 64
+  uint16_t* dst;           // planes (dst_rows, ld), zero in further columns and, if any, in rows up to a multiple of 64
   int64_t ld, plane;
   int dst_rows;
   int wide;
@@ -768,7 +768,7 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.packed = !direct;
   p.Hp = (int64_t)ceil_div(p.H, 64) * 64;
   p.Vp = (int64_t)ceil_div(p.V, 64) * 64;
-  p.Np = (int64_t)ceil_div(p.N, 64) * 64;
+  p.Np = train ? (int64_t)ceil_div(p.N, 64) * 64 : p.N;  // dW's k goes in blocks of 64 rows
   const int64_t each = p.Vp * (p.np == 3 ? 10 : 2);
   int64_t fit = train ? kChunkBytes / each / 256 * 256 : kScoreRows;
   if (fit < 256) fit = 256;

@@ -38,6 +38,7 @@ __device__ __forceinline__ bf16 narrow<bf16>(float x) {
 }
 
 // V consecutive numbers: V = 16 / sizeof(T) as one 16-byte access (the address a multiple of 16), V = 1 as one number.
+// store_past: for results that nobody reads soon, past the caches where whole pieces are written.
 template <typename T, int V>
 struct Pack;
 
@@ -77,6 +78,7 @@ struct Pack<T, 1> {
   __device__ __forceinline__ float get(int) const { return widen(w); }
   __device__ __forceinline__ void set(const float* x) { w = narrow<T>(x[0]); }
   __device__ __forceinline__ void store(T* p) const { *p = w; }
+  __device__ __forceinline__ void store_past(T* p) const { *p = w; }
 };
 
 template <typename T>
