@@ -3,9 +3,9 @@
 //   forward   out[n, :] = s W[t_n, :]
 //   backward  dW[v, :] = s sum_{n : t_n = v} g[n, :], zero for a token that does not occur and for the padding token
 //
-// Both only move rows, so memory bounds them: 131071 tokens of width 2048 in bfloat16 are looked up in 132 us, summed in
-// 230 (k_runs, the bulk of it, moves 5.2 TB/s). Rows are stored past the caches, which hold what is read again (k_lookup
-// 159 -> 148 us, k_runs 190 -> 158). The backward adds no number with an atomic: it sorts the positions by
+// Both only move rows, so memory bounds them: 131071 tokens of width 2048 in bfloat16 are looked up in 132 us, summed
+// in 230 (k_runs, the bulk of it, moves 5.2 TB/s). Rows are stored past the caches, which hold what is read again
+// (k_lookup 159 -> 148 us, k_runs 190 -> 158). The backward adds no number with an atomic: it sorts the positions by
 // token (stable, so a token's rows are added in the order of the text) and sums runs of equal tokens, in float32,
 // rounding each row of dW once. The same inputs give the same bits.
 //
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void k_few(Args a) {
       Pack<T, V> p[kAhead];
       int n = 0;
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {  // the next eight, or the last one again
+      for (int k = 0; k < kAhead; ++k) {  // the next eight, as far as there are
         const int j = __ffsll((unsigned long long)left) - 1;
         if (k == 0 || left) {
           p[k].load(g + (int64_t)(64 * q + j) * a.H);

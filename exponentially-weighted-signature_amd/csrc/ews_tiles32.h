@@ -1,11 +1,12 @@
 // The products of ews_tiles.h with a float32 first operand read as it is: for products that its bytes bound, where
-// packing it into planes first (read 4 bytes, write 6, read 12 in six products' stages) costs more than the products do.
+// packing it into planes first (read 4 bytes, write 6, read 12 in six products' stages) costs more than the
+// products do. 128 rows by 30000 x 2048, logits and dh: 0.25 ms, 2.0 TB/s of W; 0.51 ms packed.
 //
-// k runs in stages of 32. The first operand's stage is copied to LDS in float32 (rows of 128 bytes, or turned: 32 rows of
-// k, as wide as the tile) and cut into three bfloat16 planes in registers, on the way from LDS to the matrix cores; the
-// second comes as three planes. A stage does all six products at once, so either is read once. Several workgroups share a
-// CU and hide each other's waits: nothing is read ahead across the barrier. Rows that do not start at multiples of 16 bytes
-// are copied four bytes a lane.
+// k runs in stages of 32. The first operand's stage is copied to LDS in float32 (rows of 128 bytes, or turned: 32 rows
+// of k, as wide as the tile) and cut into three bfloat16 planes in registers, on the way from LDS to the matrix cores;
+// the second comes as three planes. A stage does all six products at once, so either is read once. Several workgroups
+// share a CU and hide each other's waits: nothing is read ahead across the barrier. Rows that do not start at multiples
+// of 16 bytes are copied four bytes a lane.
 #pragma once
 
 #include "ews_tiles.h"
@@ -66,7 +67,8 @@ struct Copier32 {
         offset[c] = (uint32_t)(row < left ? row : left - 1) * stride + 4 * (col < cols ? col : cols - kEach);
       } else {
         const int col = 4 * place(row, pos) + in;
-        offset[c] = (uint32_t)(first + row < rows ? row : rows - 1 - first) * stride + 4 * (col < left ? col : left - kEach);
+        offset[c] = (uint32_t)(first + row < rows ? row : rows - 1 - first) * stride +
+                    4 * (col < left ? col : left - kEach);
       }
     }
   }
@@ -132,7 +134,8 @@ __device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int k = 16 * ks + 8 * half + e, col = wave * 32 + r32;
-          x[e] = *reinterpret_cast<const float*>(stage + k * T::I * 4 + ((col >> 2) ^ (half << 3)) * 16 + (col & 3) * 4);
+          x[e] =
+              *reinterpret_cast<const float*>(stage + k * T::I * 4 + ((col >> 2) ^ (half << 3)) * 16 + (col & 3) * 4);
         }
       } else {
 #pragma unroll
@@ -155,7 +158,8 @@ __device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, 
       for (int pair = 0; pair < kPairs; ++pair)
 #pragma unroll
         for (int b = 0; b < T::TJ; ++b)
-          acc[0][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[piece_p(pair)], q[piece_q(pair)][b], acc[0][b], 0, 0, 0);
+          acc[0][b] =
+              __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[piece_p(pair)], q[piece_q(pair)][b], acc[0][b], 0, 0, 0);
     }
   }
   arrive<0>();

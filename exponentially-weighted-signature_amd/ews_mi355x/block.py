@@ -400,8 +400,8 @@ class StackedEWS(nn.Module):
         objective, e.g. experiments/fl/train.py:754-761), without the logits in memory (``linear_cross_entropy``) and
         with the embedding's gradient by sorted tokens (``embedding_lookup``): the forward's values are those of
         ``forward`` and a cross entropy of its result. X, t, mask and raw_driver as ``forward``'s, with a batch;
-        targets (B, L) for "seq2seq" (positions off the mask count as ignored), (B,) for "mean_pool"; for several heads a
-        tuple of them, whose losses are added."""
+        targets (B, L) for "seq2seq" (positions off the mask count as ignored), (B,) for "mean_pool"; for several heads
+        a tuple of them, whose losses are added."""
         if X.dim() != (2 if self.tokens else 3):
             raise ValueError(f"X must carry a batch, got shape {tuple(X.shape)}")
         if mask is not None and mask.dim() == 1:

@@ -659,10 +659,10 @@ int ews_loss_keep(const ews_loss_desc* desc, const void* hidden, const void* wei
 int ews_loss_kept(const ews_loss_desc* desc, const void* weight, const float* upstream, void* grad_hidden,
                   void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream);
 
-/* grad_* = factor[0] grad_* in place (each may be NULL), factor on the device: the gradients of factor[0] times the loss.
- * With a factor of 1 nothing is touched. */
-int ews_loss_scale(const ews_loss_desc* desc, void* grad_hidden, void* grad_weight, void* grad_bias, const float* factor,
-                   ews_stream_t stream);
+/* grad_* = factor[0] grad_* in place (each may be NULL), factor on the device: the gradients of factor[0] times the
+ * loss. With a factor of 1 nothing is touched. */
+int ews_loss_scale(const ews_loss_desc* desc, void* grad_hidden, void* grad_weight, void* grad_bias,
+                   const float* factor, ews_stream_t stream);
 
 /* Gradient clipping over n tensors, given by host arrays of device addresses, element counts (0 allowed) and
  * EWS_DTYPE_*: result[0] = norm = sqrt(sum of all squares), result[1] = c = min(1, max_norm / (norm + 1e-6)) (NaN for

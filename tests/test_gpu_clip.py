@@ -62,7 +62,8 @@ def test_clip(shapes, dtypes):
         assert torch.equal(norm, norm2) and all(torch.equal(a, b) for a, b in zip(out, kept))
         if max_norm > want:
             assert all(torch.equal(a, b) for a, b in zip(out, grads))
-        params = [torch.zeros_like(g).requires_grad_() for g in grads] + [torch.zeros(3, device=DEV, requires_grad=True)]
+        params = [torch.zeros_like(g).requires_grad_() for g in grads]
+        params.append(torch.zeros(3, device=DEV, requires_grad=True))
         for p, g in zip(params, grads):
             p.grad = g.clone()
         norm3 = E.clip_grad_norm_(params, max_norm)
@@ -98,7 +99,8 @@ def test_not_finite():
 def test_strides_and_alignment(dtype):
     base = torch.randn(70, 90, device=DEV).to(dtype)
     flat = torch.randn(40001, device=DEV).to(dtype)
-    views = [base.t(), base[::2, 1:50], base[3], base[:, 7], flat[1:20000], flat[20001:40000], base[:3, :1].expand(3, 4)]
+    views = [base.t(), base[::2, 1:50], base[3], base[:, 7], flat[1:20000], flat[20001:40000],
+             base[:3, :1].expand(3, 4)]
     norm, out = E.clip_grads(views, 1.0)
     _check([v.clone() for v in views], 1.0, norm, out)
     # in place through every view of which no two elements share memory
