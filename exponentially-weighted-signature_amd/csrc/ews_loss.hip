@@ -1153,7 +1153,12 @@ extern "C" {
 
 size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train) {
   LPlan p;
-  return loss_plan(desc, train != 0, false, p) == EWS_OK ? p.total : 0;
+  if (loss_plan(desc, train != 0, false, p) != EWS_OK) return 0;
+  // the weight's address decides how it is read; read as it is it needs no packed copy, but float32's tiles are smaller
+  // (more slabs and splits)
+  const size_t packed = p.total;
+  loss_plan(desc, train != 0, true, p);
+  return p.total > packed ? p.total : packed;
 }
 
 int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,

@@ -304,6 +304,41 @@ def test_kept_probabilities_and_new_ones_give_the_same_bits(N, dtype):
         torch.autograd.grad(rows, wrt, up)
 
 
+SCRATCH = [(141, 396, 1980), (256, 64, 1000), (200, 1000, 333), (33, 257, 4001), (7, 4096, 700), (300, 130, 900)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,H,V", SCRATCH)
+def test_scratch_holds_what_a_call_writes(N, H, V, dtype, monkeypatch):
+    """Beyond the bytes that the library asks for, a workspace stays as it was, whatever the address of the weight makes
+    of the plan."""
+    from ews_mi355x import loss as module
+
+    spaces = []
+
+    def workspace(self, train):
+        size = module.nat.load().ews_loss_workspace_bytes(self.desc, train)
+        whole = torch.full((size + (64 << 20),), 91, dtype=torch.uint8, device=DEV)
+        spaces.append((whole, size))
+        return whole[:size]
+
+    monkeypatch.setattr(module._Call, "workspace", workspace)
+    h, w, b, t = _inputs(N, H, V, dtype, bias=torch.float32, ignored=0.3)
+    odd = torch.empty(V * H + 1, device=DEV, dtype=dtype)[1:].view(V, H)
+    for weight in (w, odd.copy_(w)):
+        weight = weight.detach().requires_grad_()
+        for reduction in ("none", "mean"):
+            hidden = h.detach().requires_grad_()
+            rows = E.linear_cross_entropy(hidden, weight, t, bias=b, reduction=reduction)
+            torch.autograd.grad(rows, [hidden, weight], torch.ones_like(rows))
+        with torch.no_grad():
+            E.linear_cross_entropy(h, weight, t, bias=b)
+    torch.cuda.synchronize()
+    assert len(spaces) == 6
+    for whole, size in spaces:
+        assert bool((whole[size:] == 91).all())
+
+
 def test_second_derivatives_are_refused():
     h, w, b, t = _inputs(6, 16, 20, torch.float32, bias=torch.float32)
     h.requires_grad_()
