@@ -684,7 +684,9 @@ constexpr int64_t kChunkBytes = (int64_t)2 << 30;
 // float32 W is read as it is for up to so many rows, else packed into planes first. H=2048 V=30000, packing, logits and
 // dh: N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54.
 constexpr int kFewRows32 = 256;
-constexpr int64_t kScoreRows = 65536;  // rows of a call without gradients whose slabs' sums are kept at a time
+// A call without gradients keeps eight bytes for every row's slabs (64 of the vocabulary at least) of as many rows as
+// fit here.
+constexpr int64_t kScoreBytes = (int64_t)256 << 20;
 
 // Stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared.
 constexpr int kLongProduct = 8;
@@ -774,7 +776,7 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.Vp = (int64_t)ceil_div(p.V, 64) * 64;
   p.Np = train ? (int64_t)ceil_div(p.N, 64) * 64 : p.N;  // dW's k goes in blocks of 64 rows
   const int64_t each = p.Vp * (p.np == 3 ? 10 : 2);
-  int64_t fit = train ? kChunkBytes / each / 256 * 256 : kScoreRows;
+  int64_t fit = train ? kChunkBytes / each / 256 * 256 : kScoreBytes / (p.Vp / 8) / 256 * 256;
   if (fit < 256) fit = 256;
   p.chunk = p.Np < fit ? p.Np : fit;
   // equal chunks: the last one's tiles fill the CUs as the others' do
@@ -828,7 +830,8 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
 // float32 weights for few rows (of a stride that the tiles' offsets hold).
 bool reads_direct(const ews_loss_desc* s, const void* weight) {
   if (s->weight_stride > 1 << 22) return false;
-  if (s->dtype == EWS_DTYPE_F32) return s->rows <= kFewRows32;
+  // three planes of dz, kFewRows32 rows each, lie within 32-bit offsets
+  if (s->dtype == EWS_DTYPE_F32) return s->rows <= kFewRows32 && s->vocab <= 1 << 21;
   return (uintptr_t)weight % 16 == 0 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0;
 }
 

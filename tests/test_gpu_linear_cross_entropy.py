@@ -143,6 +143,31 @@ def test_rows_in_chunks(dtype, N):
     _check(h, w, b, t)
 
 
+def test_scores_in_chunks():
+    """Rows of a call without gradients beyond those whose slabs are kept at a time; a row's loss is its own, so some
+    rows are looked at. A row's sum goes through up to 200 additions one after another."""
+    h, w, b, t = _inputs(22000, 16, 100003, torch.bfloat16, bias=torch.float32, ignored=0.05)
+    with torch.no_grad():
+        got = E.linear_cross_entropy(h, w, t, bias=b, reduction="none")
+    for lo in (0, 10980, 11240, 21230, 21950):
+        rows = slice(lo, lo + 50)
+        want, bound = _reference(h[rows], w, b, t[rows], "none", None, grads=False)
+        _close(got[rows], want, bound + 200 * U, f"rows from {lo}")
+
+
+def test_few_rows_of_a_huge_vocabulary():
+    """The probabilities' planes of 250 rows and 2^22 tokens are wider than 32-bit offsets reach. A row's sum goes
+    through up to 600 additions one after another."""
+    h, w, b, t = _inputs(250, 8, 1 << 22, torch.float32)
+    h.requires_grad_()
+    loss = E.linear_cross_entropy(h, w, t, reduction="none")
+    (got,) = torch.autograd.grad(loss, h, torch.ones_like(loss))
+    rows = slice(246, 250)
+    want, bound = _reference(h[rows].detach(), w, b, t[rows], "none", torch.ones(4, device=DEV))
+    _close(loss[rows].detach(), want[0], bound[0] + 600 * U, "loss")
+    _close(got[rows], want[1], bound[1], "grad_hidden")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_ignored_rows_are_not_read(dtype, reduction):
