@@ -98,6 +98,7 @@ struct PackArgs {
   uint16_t* dst;           // planes (dst_rows, ld), zero in further columns and, if any, in rows up to a multiple of 64
   int64_t ld, plane;
   int dst_rows;
+  int again;               // the rows are written once more from this one on; 0: once
   int wide;
 };
 
@@ -106,14 +107,15 @@ template <typename T>
 __device__ __forceinline__ void pack_eight(const PackArgs& a, int64_t at) {
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;
   const int rows = a.map ? a.kept[0] : a.rows;
-  const int padded = (rows + 63) / 64 * 64 < a.dst_rows ? (rows + 63) / 64 * 64 : a.dst_rows;
+  const int padded = a.again || (rows + 63) / 64 * 64 > a.dst_rows ? a.dst_rows : (rows + 63) / 64 * 64;
   const int packs = (int)(a.ld / 8);
   const int64_t row = at / packs;
   if (row >= padded) return;
   const int c0 = (int)(at % packs) * 8;
-  const int n = row >= rows ? 0 : a.cols - c0 < 8 ? a.cols - c0 : 8;
+  const int64_t own = a.again && row >= a.again ? row - a.again : row;
+  const int n = own >= rows ? 0 : a.cols - c0 < 8 ? a.cols - c0 : 8;
   T x[8];
-  const T* src = (const T*)a.src + (n > 0 ? (int64_t)(a.map ? a.map[row] : row) * a.stride + c0 : 0);
+  const T* src = (const T*)a.src + (n > 0 ? (int64_t)(a.map ? a.map[own] : own) * a.stride + c0 : 0);
   if (a.wide && n == 8) {
 #pragma unroll
     for (int k = 0; k < 8; k += kWide<T>) *reinterpret_cast<u32x4*>(x + k) = *reinterpret_cast<const u32x4*>(src + k);
@@ -409,13 +411,14 @@ struct DzArgs {
   int c0, chunk, slab;
   void* prob;
   int64_t ld;             // the vocabulary padded to a multiple of 64
-  uint16_t* dz;           // planes (chunk, ld): in bfloat16 prob itself; zero rows up to a multiple of 64
+  uint16_t* dz;           // planes (chunk, ld): in bfloat16 the first is prob itself; zero rows up to a multiple of 64
   int64_t plane;
   float* bias;            // (ceil(chunk / each), ld) sums over the rows; may be null
   int each;               // rows a workgroup goes over, one wavefront a row, 512 columns wide
   float* loss;            // or null: the call's loss, by one further workgroup
 };
 
+// NP planes: 3 of float32 inputs, 1 or (few rows) 2 of bfloat16 ones.
 template <int NP>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   if (blockIdx.x * 512 >= a.ld) {
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int v = (blockIdx.x * 64 + lane) * 8;
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
-  const int padded = (live + 63) / 64 * 64;
+  const int padded = NP == 2 ? a.chunk : (live + 63) / 64 * 64;
   const bool in = v < a.ld;
   const int slab = in ? v / a.slab : 0;
   const int r0 = blockIdx.y * a.each, r1 = r0 + a.each < padded ? r0 + a.each : padded;
@@ -444,7 +447,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
       const float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
       const float m = a.st.slab[(int64_t)slab * a.chunk + j].x;
       const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f(m - top) * inv * g;
-      if (NP == 1) {
+      if (NP != 3) {
         const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)a.prob + j * a.ld + v);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
@@ -467,10 +470,16 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
       for (int q = 0; q < 8; ++q) sums[q] += x[q];
     }
     if (!in) continue;
-    if (NP == 1) {
+    if (NP != 3) {
       Pack<bf16, 8> p;
       p.set(x);
       p.store((bf16*)a.dz + j * a.ld + v);
+      if (NP == 2) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = __builtin_isfinite(p.get(q)) ? x[q] - p.get(q) : 0.0f;
+        p.set(x);
+        p.store((bf16*)a.dz + a.plane + j * a.ld + v);
+      }
     } else {
       uint16_t p[8][3];
 #pragma unroll
@@ -521,6 +530,7 @@ struct GradArgs {
   int ti, tj, splits;
   int kblocks, per;       // k blocks, and those of one split
   int by_rows;            // 1: k is the chunk's kept rows (dW); 0: the result's rows are (dh)
+  int twice;              // dW of few rows: k is the rows of both planes of dz, all of them
   int c0, chunk;
   Rows rows;
   int I, J;               // the result's columns and (where by_rows) rows
@@ -587,7 +597,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_grad(GradArgs a) {
   const int nj = ROWS ? a.J : live;
   if (j0 >= nj) return;
   int kb0 = split * a.per, kb1 = kb0 + a.per < a.kblocks ? kb0 + a.per : a.kblocks;
-  if (ROWS && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
+  if (ROWS && !a.twice && kb1 > (live + 63) / 64) kb1 = (live + 63) / 64;
   f32x16 acc[T::TI][T::TJ];
   if constexpr (PAIRS == 0)
     product32<T, true>(a.P32, a.Q, i0, j0, kb0, kb1, lds, acc);
@@ -695,18 +705,26 @@ constexpr int kLongProduct = 8;
 // (36).
 constexpr int kFewSplits = 8;
 
+// Up to so many rows of bfloat16, dz is kept in two planes: where few rows add up, the rounding of dz to eight bits
+// (most of it that of the targets' entries, g (p - 1)) does not average out. Against the results' own rounding alone,
+// dh and dW are up to 2.5 times as far off at 2 rows and 1.8 at 16 with one plane, 1.0 with two; from 256 rows on 1.4 to
+// 1.5. Where g stays out of dz (the mean and the sum) the targets' entries are near -1 and lose less: up to 2.2 times at
+// 2 rows, 1.4 at 16. The planes lie one behind the other, and so do two copies of h: dW's k is twice the rows, and dh
+// takes two products a stage.
+constexpr int kFewRowsNone = 256, kFewRowsMean = 16;
+
 enum Kind { kLarge, kMedium, kFlat, kFew32, kMore32 };
 
 struct Product {
   Kind kind;
-  int ti, tj, tile_i, slab, splits, per, kblocks;
+  int ti, tj, tile_i, slab, splits, per, kblocks, pairs;
 };
 
 struct LPlan {
   int N, H, V, np;
   int64_t Hp, Vp, Np, chunk;
   int chunks, slabs, bias_pad, dz_rows;
-  bool train, packed, as_is;
+  bool train, packed, as_is, twice;
   Product logits, dh, dw;
   size_t map, target, meta, zt, top, inv, loss, xp, wp, bias, slab, prob, dz, dbias, dbsum, part, acc;
   size_t total;
@@ -723,6 +741,7 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split, bool as_is) {
   Product p;
   p.kblocks = kblocks;
+  p.pairs = pairs;
   const int64_t large = (int64_t)ceil_div(I, 256) * ceil_div(J, 256);
   const int parts = split ? (kblocks >= 32 ? kblocks / 16 : 1) : 1;
   if (as_is)
@@ -783,12 +802,17 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.chunks = ceil_div(p.Np, p.chunk);
   if (p.chunks > 1) p.chunk = (int64_t)ceil_div(ceil_div(p.Np, p.chunks), 256) * 256;
   p.chunks = ceil_div(p.Np, p.chunk);
+  p.twice = train && p.np == 1 && p.N <= (s->reduction == EWS_LOSS_NONE ? kFewRowsNone : kFewRowsMean);
+  if (p.twice) {
+    p.chunk = (int64_t)ceil_div(p.N, 32) * 32;
+    p.Np = 2 * p.chunk;
+  }
   const int64_t most = p.chunk < p.N ? p.chunk : p.N;  // rows of a chunk
   const int pairs = p.np == 3 ? kPairs : 1;
   p.as_is = p.np == 3 && direct;
   p.logits = pick(p.V, most, p.as_is ? ceil_div(p.H, 32) : (int)(p.Hp / 64), pairs, false, p.as_is);
-  p.dh = pick(p.H, most, p.as_is ? ceil_div(p.V, 32) : (int)(p.Vp / 64), pairs, true, p.as_is);
-  p.dw = pick(p.H, p.V, (int)(p.chunk / 64), pairs, true, false);
+  p.dh = pick(p.H, most, p.as_is ? ceil_div(p.V, 32) : (int)(p.Vp / 64), p.twice ? 2 : pairs, true, p.as_is);
+  p.dw = pick(p.H, p.V, (int)((p.twice ? p.Np : p.chunk) / 64), pairs, true, false);
   p.bias_pad = p.logits.ti * p.logits.tile_i;
   p.slabs = p.bias_pad / p.logits.slab;
   size_t off = 0;
@@ -809,7 +833,7 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.bias = take((size_t)p.bias_pad * 4);
   p.slab = take((size_t)p.slabs * p.chunk * 8);
   if (train) {
-    p.prob = take((size_t)(p.chunk * p.Vp) * (p.np == 3 ? 4 : 2));
+    p.prob = take((size_t)(p.chunk * p.Vp) * (p.np == 3 || p.twice ? 4 : 2));
     p.dz = p.np == 3 ? take((size_t)(p.chunk * p.Vp) * 6) : p.prob;
     // 128 rows a workgroup (the bias's partial sums stay small), fewer where that leaves CUs without one
     p.dz_rows = 128;
@@ -884,7 +908,7 @@ int launch_logits(Kind kind, const LogitArgs& a, hipStream_t st) {
 }
 
 // kP: float32 gradients are those of float32 operands
-template <class T, bool ROWS, typename O, int kP = sizeof(O) == 4 ? kPairs : 1>
+template <class T, bool ROWS, typename O, int kP>
 int launch_grad_as(const GradArgs& a, hipStream_t st) {
   const int lds = lds_bytes<T, kP>(a.per);
   const int rc = allow_lds(k_grad<T, kP, ROWS, O>, lds);
@@ -905,16 +929,23 @@ int launch_grad_as(const GradArgs& a, hipStream_t st) {
 }
 
 template <bool ROWS, typename O>
-int launch_grad(Kind kind, const GradArgs& a, hipStream_t st) {
-  if constexpr (!ROWS && sizeof(O) == 4) {
-    if (kind == kFew32)
+int launch_grad(const Product& p, const GradArgs& a, hipStream_t st) {
+  constexpr int kP = sizeof(O) == 4 ? kPairs : 1;
+  if constexpr (!ROWS && kP == kPairs) {
+    if (p.kind == kFew32)
       return pieces(a.P32) ? launch_grad_as<Few32<16>, ROWS, O, 0>(a, st) : launch_grad_as<Few32<4>, ROWS, O, 0>(a, st);
-    if (kind == kMore32)
+    if (p.kind == kMore32)
       return pieces(a.P32) ? launch_grad_as<More32<16>, ROWS, O, 0>(a, st)
                            : launch_grad_as<More32<4>, ROWS, O, 0>(a, st);
   }
-  if (kind == kLarge) return launch_grad_as<Large, ROWS, O>(a, st);
-  return kind == kMedium ? launch_grad_as<Medium, ROWS, O>(a, st) : launch_grad_as<Flat, ROWS, O>(a, st);
+  if constexpr (!ROWS && kP == 1) {
+    if (p.pairs == 2) {
+      if (p.kind == kLarge) return launch_grad_as<Large, ROWS, O, 2>(a, st);
+      return p.kind == kMedium ? launch_grad_as<Medium, ROWS, O, 2>(a, st) : launch_grad_as<Flat, ROWS, O, 2>(a, st);
+    }
+  }
+  if (p.kind == kLarge) return launch_grad_as<Large, ROWS, O, kP>(a, st);
+  return p.kind == kMedium ? launch_grad_as<Medium, ROWS, O, kP>(a, st) : launch_grad_as<Flat, ROWS, O, kP>(a, st);
 }
 
 int rows_wide(const void* p, int64_t stride, bool f32) {
@@ -937,6 +968,7 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   x.ld = p.Hp;
   x.plane = p.Np * p.Hp;
   x.dst_rows = (int)p.Np;
+  x.again = p.twice ? (int)p.chunk : 0;
   x.wide = rows_wide(x.src, x.stride, f32);
   PrepareArgs r{};
   r.targets = targets;
@@ -1087,6 +1119,8 @@ int gradients(const Call& c, const void* weight, int k, const float* upstream, f
   const dim3 grid(ceil_div(p.Vp, 512) + (z.loss ? 1 : 0), ceil_div(p.chunk, p.dz_rows));
   if (f32)
     hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
+  else if (p.twice)
+    hipLaunchKernelGGL((k_dz<2>), grid, dim3(256), 0, c.st, z);
   else
     hipLaunchKernelGGL((k_dz<1>), grid, dim3(256), 0, c.st, z);
   LOSS_CHECK();
@@ -1125,14 +1159,15 @@ int gradients(const Call& c, const void* weight, int k, const float* upstream, f
     g.sum = nullptr;
     g.add = 0;
     g.out = grad_hidden;
-    rc = f32 ? launch_grad<false, float>(p.dh.kind, g, c.st) : launch_grad<false, bf16>(p.dh.kind, g, c.st);
+    rc = f32 ? launch_grad<false, float>(p.dh, g, c.st) : launch_grad<false, bf16>(p.dh, g, c.st);
     if (rc != EWS_OK) return rc;
   }
   if (grad_weight) {
     g.P = hidden_operand(c);
     g.P.p += z.c0 * p.Hp;
     g.P.rows -= z.c0;
-    g.Q = Operand{z.dz, p.Vp, z.plane, (int)p.chunk, (int)p.Vp};
+    g.Q = Operand{z.dz, p.Vp, z.plane, (int)(p.twice ? 2 * p.chunk : p.chunk), (int)p.Vp};
+    g.twice = p.twice;
     g.ti = p.dw.ti;
     g.tj = p.dw.tj;
     g.splits = p.dw.splits;
@@ -1144,7 +1179,7 @@ int gradients(const Call& c, const void* weight, int k, const float* upstream, f
     g.sum = f32 ? (float*)grad_weight : (float*)(c.w + p.acc);
     g.add = k > 0 ? 1 : 0;
     g.out = last || f32 ? grad_weight : nullptr;
-    rc = f32 ? launch_grad<true, float>(p.dw.kind, g, c.st) : launch_grad<true, bf16>(p.dw.kind, g, c.st);
+    rc = f32 ? launch_grad<true, float>(p.dw, g, c.st) : launch_grad<true, bf16>(p.dw, g, c.st);
     if (rc != EWS_OK) return rc;
   }
   return EWS_OK;

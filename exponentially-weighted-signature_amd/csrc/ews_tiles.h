@@ -191,8 +191,8 @@ __device__ __forceinline__ void arrive() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The results of the workgroup's tile at (i0, j0) over k blocks [kb0, kb1); PAIRS: 1, or kPairs for three planes. On
-// return LDS is free.
+// The results of the workgroup's tile at (i0, j0) over k blocks [kb0, kb1); PAIRS: 1, 2 for two planes of Q alone, or
+// kPairs for three of either. On return LDS is free.
 template <class T, int PAIRS, bool TURNED_P, bool TURNED_Q>
 __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
                                         char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
@@ -214,8 +214,8 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
   char* to;
   auto aim = [&](int s) {
     const int pair = PAIRS == 1 ? kPairs - 1 : s % PAIRS;
-    fromP = cp.at(piece_p(pair), kb0 + s / PAIRS);
-    fromQ = cq.at(piece_q(pair), kb0 + s / PAIRS);
+    fromP = cp.at(PAIRS == 2 ? 0 : piece_p(pair), kb0 + s / PAIRS);
+    fromQ = cq.at(PAIRS == 2 ? 1 - pair : piece_q(pair), kb0 + s / PAIRS);
     to = lds + (s & 1) * T::kStage + wave * 1024;
   };
   auto copy = [&](int c) {

@@ -31,7 +31,7 @@ def _inputs(N, H, V, dtype, bias=None, ignored=0.0, seed=0, spread=1.5):
     return h, w, b, t
 
 
-def _reference(h, w, b, t, reduction, upstream=None, grads=True):
+def _reference(h, w, b, t, reduction, upstream=None, grads=True, planes=1):
     """(loss, gh, gw, gb), their bounds; kept rows only are looked at."""
     V = w.shape[0]
     keep = t != -100
@@ -69,8 +69,10 @@ def _reference(h, w, b, t, reduction, upstream=None, grads=True):
     d *= g[:, None]
     e = 2 * zerr + 16 * U + 2 * U * zmag
     derr = p * (e * g.abs())[:, None] + 4 * U * d.abs()
-    if h.dtype == torch.bfloat16:
+    if h.dtype == torch.bfloat16 and planes == 1:
         derr = derr + 2 * 2.0**-8 * 1.01 * d.abs()
+    elif h.dtype == torch.bfloat16:  # probabilities as 16-bit logarithms, then 16 bits of dz
+        derr = derr + 1.1 * 2.0**-10.5 * p * g.abs()[:, None] + 2.0**-16 * d.abs()
     gh = torch.zeros_like(h, dtype=torch.float64)
     gh[keep] = d @ wd
     herr = torch.zeros_like(gh)
@@ -141,6 +143,21 @@ def test_rows_in_chunks(dtype, N):
     _check(h, w, b, t)
     t[N // 4:] = -100
     _check(h, w, b, t)
+
+
+@pytest.mark.parametrize("N,H,V,reduction", [(1, 72, 67, "none"), (8, 128, 67, "none"), (33, 64, 500, "none"),
+                                             (200, 136, 1003, "none"), (256, 64, 300, "none"), (2, 128, 67, "mean"),
+                                             (16, 200, 1000, "sum")])
+def test_few_rows_of_bfloat16_are_rounded_once(N, H, V, reduction):
+    """Where few rows add up, dz has sixteen bits: the gradients are off by little more than their own rounding."""
+    h, w, b, t = _inputs(N, H, V, torch.bfloat16, bias=torch.float32, ignored=0.1 if N > 4 else 0.0)
+    wrt = [x.requires_grad_() for x in (h, w, b)]
+    loss = E.linear_cross_entropy(h, w, t, bias=b, reduction=reduction)
+    up = torch.rand(N, device=DEV) + 0.5 if reduction == "none" else None
+    got = torch.autograd.grad(loss, wrt, up)
+    want, bound = _reference(*(x.detach() for x in wrt), t, reduction, up, planes=2)
+    for a, r, e, name in zip(got, want[1:], bound[1:], ("hidden", "weight", "bias")):
+        _close(a, r, e, f"grad_{name}")
 
 
 def test_scores_in_chunks():
