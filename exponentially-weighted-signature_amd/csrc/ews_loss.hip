@@ -692,8 +692,9 @@ using namespace ews::loss;
 // Rows kept at a time: exp(z - m), and dz in its place (float32: dz in three planes beside it), of as many as fit here.
 constexpr int64_t kChunkBytes = (int64_t)2 << 30;
 // float32 W is read as it is for up to so many rows, else packed into planes first. H=2048 V=30000, packing, logits and
-// dh: N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54.
-constexpr int kFewRows32 = 256;
+// dh: N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54. Packing and logits alone, H=1772 V=45646: N=260 0.34 and
+// 0.61, N=400 0.50 and 0.67; H=1024 V=32000: N=520 0.26 and 0.32, N=800 0.38 and 0.35.
+constexpr int kFewRows32 = 512;
 // A call without gradients keeps eight bytes for every row's slabs (64 of the vocabulary at least) of as many rows as
 // fit here.
 constexpr int64_t kScoreBytes = (int64_t)256 << 20;
@@ -855,7 +856,7 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
 bool reads_direct(const ews_loss_desc* s, const void* weight) {
   if (s->weight_stride > 1 << 22) return false;
   // three planes of dz, kFewRows32 rows each, lie within 32-bit offsets
-  if (s->dtype == EWS_DTYPE_F32) return s->rows <= kFewRows32 && s->vocab <= 1 << 21;
+  if (s->dtype == EWS_DTYPE_F32) return s->rows <= kFewRows32 && s->vocab <= 1 << 20;
   return (uintptr_t)weight % 16 == 0 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0;
 }
 

@@ -172,17 +172,19 @@ def test_scores_in_chunks():
         _close(got[rows], want, bound + 200 * U, f"rows from {lo}")
 
 
-def test_few_rows_of_a_huge_vocabulary():
-    """The probabilities' planes of 250 rows and 2^22 tokens are wider than 32-bit offsets reach. A row's sum goes
-    through up to 600 additions one after another."""
-    h, w, b, t = _inputs(250, 8, 1 << 22, torch.float32)
+@pytest.mark.parametrize("N,V", [(250, 1 << 22), (500, 1 << 20)])
+def test_few_rows_of_a_huge_vocabulary(N, V):
+    """The probabilities' planes of 250 rows and 2^22 tokens are wider than 32-bit offsets reach; 500 rows of 2^20 are
+    done in chunks with W read as it is. A row's sum goes through up to 600 additions one after another."""
+    h, w, b, t = _inputs(N, 8, V, torch.float32)
     h.requires_grad_()
     loss = E.linear_cross_entropy(h, w, t, reduction="none")
     (got,) = torch.autograd.grad(loss, h, torch.ones_like(loss))
-    rows = slice(246, 250)
-    want, bound = _reference(h[rows].detach(), w, b, t[rows], "none", torch.ones(4, device=DEV))
-    _close(loss[rows].detach(), want[0], bound[0] + 600 * U, "loss")
-    _close(got[rows], want[1], bound[1], "grad_hidden")
+    for lo in (0, N // 2 + 10, N - 4):
+        rows = slice(lo, lo + 4)
+        want, bound = _reference(h[rows].detach(), w, b, t[rows], "none", torch.ones(4, device=DEV))
+        _close(loss[rows].detach(), want[0], bound[0] + 600 * U, f"loss from {lo}")
+        _close(got[rows], want[1], bound[1], f"grad_hidden from {lo}")
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
