@@ -691,10 +691,13 @@ using namespace ews::loss;
 
 // Rows kept at a time: exp(z - m), and dz in its place (float32: dz in three planes beside it), of as many as fit here.
 constexpr int64_t kChunkBytes = (int64_t)2 << 30;
-// float32 W is read as it is for up to so many rows, else packed into planes first. H=2048 V=30000, packing, logits and
-// dh: N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54. Packing and logits alone, H=1772 V=45646: N=260 0.34 and
-// 0.61, N=400 0.50 and 0.67; H=1024 V=32000: N=520 0.26 and 0.32, N=800 0.38 and 0.35.
+// float32 W is read as it is for up to so many rows or logits, else packed into planes first. H=2048 V=30000, packing,
+// logits and dh: N=128 0.25 ms as it is, 0.51 packed; N=256 0.50 and 0.54. Packing and logits alone, H=1772 V=45646:
+// N=260 0.34 and 0.61, N=400 0.50 and 0.67; H=1024 V=32000: N=520 0.26 and 0.32, N=800 0.38 and 0.35. Few logits give
+// few tiles, which six products a stage serve better: packing, logits, dh and dW of N=645 H=3904 V=1037 0.22 and 0.31
+// ms, of N=2000 H=1024 V=1000 0.11 and 0.12, of N=3000 H=333 V=2000 0.13 and 0.13.
 constexpr int kFewRows32 = 512;
+constexpr int64_t kFewLogits32 = 1 << 22;
 // A call without gradients keeps eight bytes for every row's slabs (64 of the vocabulary at least) of as many rows as
 // fit here.
 constexpr int64_t kScoreBytes = (int64_t)256 << 20;
@@ -708,10 +711,10 @@ constexpr int kFewSplits = 8;
 
 // Up to so many rows of bfloat16, dz is kept in two planes: where few rows add up, the rounding of dz to eight bits
 // (most of it that of the targets' entries, g (p - 1)) does not average out. Against the results' own rounding alone,
-// dh and dW are up to 2.5 times as far off at 2 rows and 1.8 at 16 with one plane, 1.0 with two; from 256 rows on 1.4 to
-// 1.5. Where g stays out of dz (the mean and the sum) the targets' entries are near -1 and lose less: up to 2.2 times at
-// 2 rows, 1.4 at 16. The planes lie one behind the other, and so do two copies of h: dW's k is twice the rows, and dh
-// takes two products a stage.
+// dh and dW are up to 2.5 times as far off at 2 rows and 1.8 at 16 with one plane, 1.0 with two; from 256 rows on 1.4
+// to 1.5. Where g stays out of dz (the mean and the sum) the targets' entries are near -1 and lose less: up to 2.2
+// times at 2 rows, 1.4 at 16. The planes lie one behind the other, and so do two copies of h: dW's k is twice the rows,
+// and dh takes two products a stage.
 constexpr int kFewRowsNone = 256, kFewRowsMean = 16;
 
 enum Kind { kLarge, kMedium, kFlat, kFew32, kMore32 };
@@ -855,8 +858,11 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
 // float32 weights for few rows (of a stride that the tiles' offsets hold).
 bool reads_direct(const ews_loss_desc* s, const void* weight) {
   if (s->weight_stride > 1 << 22) return false;
-  // three planes of dz, kFewRows32 rows each, lie within 32-bit offsets
-  if (s->dtype == EWS_DTYPE_F32) return s->rows <= kFewRows32 && s->vocab <= 1 << 20;
+  if (s->dtype == EWS_DTYPE_F32) {
+    // the three planes of h, and of a chunk's dz, lie within 32-bit offsets
+    if ((s->rows + 63) * (int64_t)(s->hidden + 63) > 1 << 29 || s->vocab > 1 << 20) return false;
+    return s->rows <= kFewRows32 || s->rows * (int64_t)s->vocab <= kFewLogits32;
+  }
   return (uintptr_t)weight % 16 == 0 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0;
 }
 
