@@ -151,30 +151,48 @@ struct PrepareArgs {
   int bias_bf16;
   float* bias_out;         // (padded)
   void* grad_hidden;       // or null: the ignored rows' zeros
+  int each, kept_blocks;   // rows that a workgroup lists, and those workgroups
   int bias_blocks, ignored_blocks;
   PackArgs weight;         // packed by the further workgroups
   PackArgs few;            // the hidden rows, where the first workgroup packs them too; dst null: k_pack does
 };
 
-// One workgroup. A wavefront counts the kept ones of a stretch of rows, the counts are summed, the stretch is written.
+// Lists the kept ones of `each` rows. A workgroup counts those of all rows before its own by itself (the targets stay
+// in L2), its wavefronts those of their own stretches, and so every one knows where its first goes. 131072 rows by 16
+// workgroups: 21 us; 100000 by one: 43.
 __device__ __forceinline__ void keep_rows(const PrepareArgs& a) {
-  __shared__ int counts[16];
+  __shared__ int counts[16], earlier[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int each = (a.n + 1023) / 1024 * 64;
-  const int lo = wave * each < a.n ? wave * each : a.n;
-  const int hi = lo + each < a.n ? lo + each : a.n;
-  int m = 0;
+  const int start = (int)blockIdx.x * a.each, end = start + a.each < a.n ? start + a.each : a.n;
+  const int part = (end - start + 1023) / 1024 * 64;
+  const int lo = start + wave * part < end ? start + wave * part : end;
+  const int hi = lo + part < end ? lo + part : end;
+  int before = 0, m = 0;
+  for (int i = tid; i < start; i += 8 * 1024) {  // `each` is a multiple of that where there is more than one workgroup
+    int64_t t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = a.targets[i + k * 1024];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) before += t[k] != a.ignore;
+  }
 #pragma unroll 8
   for (int i = lo + lane; i < hi; i += 64) m += a.targets[i] != a.ignore;
 #pragma unroll
-  for (int s = 32; s; s >>= 1) m += __shfl_xor(m, s);
-  if (lane == 0) counts[wave] = m;
+  for (int s = 32; s; s >>= 1) {
+    m += __shfl_xor(m, s);
+    before += __shfl_xor(before, s);
+  }
+  if (lane == 0) {
+    counts[wave] = m;
+    earlier[wave] = before;
+  }
   __syncthreads();
   int total = 0, at = 0;
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
     if (w < wave) at += counts[w];
-    total += counts[w];
+    at += earlier[w];
+    total += counts[w] + earlier[w];
   }
 #pragma unroll 4
   for (int i0 = lo; i0 < hi; i0 += 64) {
@@ -191,7 +209,7 @@ __device__ __forceinline__ void keep_rows(const PrepareArgs& a) {
     }
     at += __popcll(kept);
   }
-  if (tid == 0) {
+  if (tid == 0 && end == a.n) {
     a.rows.kept[0] = total;
     a.rows.scale[0] = a.mean ? 1.0f / (float)(total > 0 ? total : 1) : 1.0f;
   }
@@ -210,20 +228,20 @@ __device__ __forceinline__ void scale_bias(const PrepareArgs& a, int v) {
   a.bias_out[v] = b;
 }
 
-// What needs nothing of the others, in one launch: the first workgroup lists the kept rows (and packs a few), some
+// What needs nothing of the others, in one launch: the first workgroups list the kept rows (one packs a few), some
 // write the bias, some (16 rows each) zero the ignored rows of dh, the others pack W where it is not read as it is.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_prepare(PrepareArgs a) {
-  if (blockIdx.x == 0) {
+  if ((int)blockIdx.x < a.kept_blocks) {
     keep_rows(a);
-    if (!a.few.dst) return;
+    if (!a.few.dst) return;  // else there is one such workgroup
     __threadfence_block();
     __syncthreads();  // the list is this workgroup's own
     const int64_t packs = (int64_t)a.few.dst_rows * (a.few.ld / 8);
     for (int64_t at = threadIdx.x; at < packs; at += 1024) pack_eight<T>(a.few, at);
     return;
   }
-  const int b = blockIdx.x - 1;
+  const int b = blockIdx.x - a.kept_blocks;
   if (b < a.bias_blocks) return scale_bias(a, b * 1024 + threadIdx.x);
   if (b >= a.bias_blocks + a.ignored_blocks)
     return pack_eight<T>(a.weight, (int64_t)(b - a.bias_blocks - a.ignored_blocks) * 1024 + threadIdx.x);
@@ -415,11 +433,13 @@ struct DzArgs {
   int64_t plane;
   float* bias;            // (ceil(chunk / each), ld) sums over the rows; may be null
   int each;               // rows a workgroup goes over, one wavefront a row, 512 columns wide
+  int lanes;              // narrow: so many lanes a row, 64 / lanes rows a wavefront; a power of two
   float* loss;            // or null: the call's loss, by one further workgroup
 };
 
-// NP planes: 3 of float32 inputs, 1 or (few rows) 2 of bfloat16 ones.
-template <int NP>
+// NP planes: 3 of float32 inputs, 1 or (few rows) 2 of bfloat16 ones. NARROW: a row fills half a wavefront at most, so
+// several rows share one (131072 rows by V=8: 94 -> 38 us).
+template <int NP, bool NARROW>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   if (blockIdx.x * 512 >= a.ld) {
     if (blockIdx.y == 0) total_loss(a.st, a.rows, a.loss);
@@ -427,7 +447,8 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   }
   __shared__ float part[4][64][9];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int v = (blockIdx.x * 64 + lane) * 8;
+  const int lanes = NARROW ? a.lanes : 64, abreast = NARROW ? 64 / lanes : 1;
+  const int v = NARROW ? (lane & (lanes - 1)) * 8 : (blockIdx.x * 64 + lane) * 8;
   const int live = a.rows.kept[0] - a.c0 < a.chunk ? a.rows.kept[0] - a.c0 : a.chunk;
   const int padded = NP == 2 ? a.chunk : (live + 63) / 64 * 64;
   const bool in = v < a.ld;
@@ -436,7 +457,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   float sums[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) sums[q] = 0.0f;
-  for (int j = r0 + wave; j < r1; j += 4) {
+  for (int j = NARROW ? r0 + wave * abreast + lane / lanes : r0 + wave; j < r1; j += 4 * abreast) {
     float x[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) x[q] = 0.0f;
@@ -497,25 +518,36 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) part[wave][lane][q] = sums[q];
   __syncthreads();
-  for (int c = threadIdx.x; c < 512; c += 256) {
+  for (int c = threadIdx.x; c < 8 * lanes; c += 256) {
     const int col = blockIdx.x * 512 + c;
     if (col >= a.ld) break;
     float s = 0.0f;
+    for (int r = 0; r < 64; r += lanes)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) s += part[w][c >> 3][c & 7];
+      for (int w = 0; w < 4; ++w) s += part[w][r + (c >> 3)][c & 7];
     a.bias[(int64_t)blockIdx.y * a.ld + col] = s;
   }
 }
 
-// The bias's gradient: k_dz's sums over rows, added to those of the chunks before; the last chunk writes it.
+// The bias's gradient: k_dz's sums over rows, added to those of the chunks before; the last chunk writes it. 64 columns
+// a workgroup, its sixteen wavefronts a contiguous part of the sums each (4096 of them by V=200: 6 us, by one thread a
+// column 44).
 template <typename T>
-__global__ __launch_bounds__(256) void k_dbias(const float* part, int parts, int64_t ld, int vocab, float* sum,
-                                               int add, const float* factor, T* out) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= vocab) return;
+__global__ __launch_bounds__(1024) void k_dbias(const float* part, int parts, int64_t ld, int vocab, float* sum,
+                                                int add, const float* factor, T* out) {
+  __shared__ float joined[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v = blockIdx.x * 64 + lane;
+  const int each = (parts + 15) / 16, p1 = (wave + 1) * each < parts ? (wave + 1) * each : parts;
   float s = 0.0f;
+  if (v < vocab) {
 #pragma unroll 8
-  for (int p = 0; p < parts; ++p) s += part[p * ld + v];
+    for (int p = wave * each; p < p1; ++p) s += part[p * ld + v];
+  }
+  joined[wave][lane] = s;
+  __syncthreads();
+  if (wave || v >= vocab) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) s += joined[w][lane];
   s = (factor ? s * factor[0] : s) + (add ? sum[v] : 0.0f);
   if (out)
     out[v] = narrow<T>(s);
@@ -991,9 +1023,12 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   r.bias_bf16 = c.s->bias_dtype == EWS_DTYPE_BF16;
   r.bias_out = (float*)(c.w + p.bias);
   r.grad_hidden = grad_hidden;
+  // 64 workgroups at most list rows, 8192 or a multiple each
+  r.each = ceil_div(ceil_div(p.N, 64), 8192) * 8192;
+  r.kept_blocks = ceil_div(p.N, r.each);
   r.bias_blocks = ceil_div(p.bias_pad, 1024);
   r.ignored_blocks = grad_hidden ? ceil_div(p.N, 16) : 0;
-  int64_t blocks = 1 + r.bias_blocks + r.ignored_blocks;
+  int64_t blocks = r.kept_blocks + r.bias_blocks + r.ignored_blocks;
   if (p.packed) {
     PackArgs& w = r.weight;
     w.src = weight;
@@ -1124,21 +1159,30 @@ int gradients(const Call& c, const void* weight, int k, const float* upstream, f
   z.each = p.dz_rows;
   z.loss = last ? loss : nullptr;
   const dim3 grid(ceil_div(p.Vp, 512) + (z.loss ? 1 : 0), ceil_div(p.chunk, p.dz_rows));
-  if (f32)
-    hipLaunchKernelGGL((k_dz<3>), grid, dim3(256), 0, c.st, z);
-  else if (p.twice)
-    hipLaunchKernelGGL((k_dz<2>), grid, dim3(256), 0, c.st, z);
-  else
-    hipLaunchKernelGGL((k_dz<1>), grid, dim3(256), 0, c.st, z);
+  if (p.Vp <= 256) {
+    z.lanes = p.Vp <= 64 ? 8 : p.Vp <= 128 ? 16 : 32;
+    if (f32)
+      hipLaunchKernelGGL((k_dz<3, true>), grid, dim3(256), 0, c.st, z);
+    else if (p.twice)
+      hipLaunchKernelGGL((k_dz<2, true>), grid, dim3(256), 0, c.st, z);
+    else
+      hipLaunchKernelGGL((k_dz<1, true>), grid, dim3(256), 0, c.st, z);
+  } else if (f32) {
+    hipLaunchKernelGGL((k_dz<3, false>), grid, dim3(256), 0, c.st, z);
+  } else if (p.twice) {
+    hipLaunchKernelGGL((k_dz<2, false>), grid, dim3(256), 0, c.st, z);
+  } else {
+    hipLaunchKernelGGL((k_dz<1, false>), grid, dim3(256), 0, c.st, z);
+  }
   LOSS_CHECK();
   if (grad_bias) {
     float* sum = (float*)(c.w + p.dbsum);
-    const dim3 g(ceil_div(p.V, 256));
+    const dim3 g(ceil_div(p.V, 64));
     if (c.s->bias_dtype == EWS_DTYPE_BF16)
-      hipLaunchKernelGGL((k_dbias<bf16>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0,
+      hipLaunchKernelGGL((k_dbias<bf16>), g, dim3(1024), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0,
                          factor, last ? (bf16*)grad_bias : nullptr);
     else
-      hipLaunchKernelGGL((k_dbias<float>), g, dim3(256), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0,
+      hipLaunchKernelGGL((k_dbias<float>), g, dim3(1024), 0, c.st, z.bias, (int)grid.y, p.Vp, p.V, sum, k > 0 ? 1 : 0,
                          factor, last ? (float*)grad_bias : nullptr);
     LOSS_CHECK();
   }
