@@ -9,7 +9,7 @@ import math
 import torch
 
 from . import _native as nat
-from .embed import DTYPES, check_tensor, launch
+from .embed import DTYPES, check_tensor, launch, refuse_tangents
 
 
 def _dense(t):
@@ -42,6 +42,7 @@ def _check(tensors):
             raise TypeError(f"gradients must be dense tensors, got layout {t.layout}")
         check_tensor("every gradient", t)
         raise ValueError(f"gradients are on {dev} and {t.device}")
+    refuse_tangents(tensors)
 
 
 def _norm_and_scale(tensors, outs, max_norm):

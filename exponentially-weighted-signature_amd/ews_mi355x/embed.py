@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -29,6 +30,16 @@ def once(backward):
         return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
+
+
+def refuse_tangents(tensors):
+    """Forward-mode derivatives are not formed: a tensor (or None) that carries one is refused, as an autograd function
+    without a jvp refuses it, not answered without a tangent, which would read as a derivative of zero."""
+    if forward_ad._current_level < 0:  # no forward-mode differentiation is going on
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("ews_mi355x has no forward-mode derivatives (jvp) of this operator")
 
 
 def check_tensor(name, t):
@@ -90,13 +101,14 @@ class _Lookup(torch.autograd.Function):
 
 def embedding_lookup(tokens, weight, scale=1.0, padding_idx=None):
     """``scale * weight[tokens]``: tokens of any shape (int64 or int32), weight (V, H) float32 or bfloat16 on the HIP
-    device -> (*tokens.shape, H) in weight's type. Differentiable in weight: a token's gradient rows are added in the
-    order of the tokens, in float32 and without atomics, so the same inputs give the same gradient bits; the rows of
-    ``padding_idx`` get none. A token outside [0, V) gives a row of NaN and has no gradient (the host does not wait to
-    look at the tokens)."""
+    device -> (*tokens.shape, H) in weight's type. Differentiable in weight (reverse mode): a token's gradient rows are
+    added in the order of the tokens, in float32 and without atomics, so the same inputs give the same gradient bits;
+    the rows of ``padding_idx`` get none. A token outside [0, V) gives a row of NaN and has no gradient (the host does
+    not wait to look at the tokens)."""
     if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError(f"weight must be (V, H) with V, H >= 1, got {tuple(weight.shape)}")
     check_tensor("weight", weight)
+    refuse_tangents((weight,))
     if tokens.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"tokens must be int64 or int32, got {tokens.dtype}")
     if tokens.device != weight.device:

@@ -6,7 +6,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
-from .embed import DTYPES, check_tensor, launch, once, row_major
+from .embed import DTYPES, check_tensor, launch, once, refuse_tangents, row_major
 
 
 def _ptr(t):
@@ -121,7 +121,7 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
 
     hidden (..., H) and weight (V, H), both float32 or both bfloat16, bias (V,) of either type or None, targets (...)
     int64 or int32, all on the HIP device. ``reduction``: "mean" over the rows that are not ignored (0 where all are),
-    "sum", or "none" for every row's own loss, (...). Differentiable in hidden, weight and bias.
+    "sum", or "none" for every row's own loss, (...). Differentiable in hidden, weight and bias (reverse mode).
 
     Rows whose target is ``ignore_index`` have loss and gradient zero, whatever they hold, and cost nothing. A target
     outside [0, V) that is not ``ignore_index`` gives NaN. A bias of -inf takes a token out of the vocabulary."""
@@ -149,6 +149,7 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     for name, t in (("hidden", hidden), ("targets", targets), ("bias", bias)):
         if t is not None and t.device != dev:
             raise ValueError(f"{name} is on {t.device}, weight on {dev}")
+    refuse_tangents((hidden, weight, bias))
     rows = hidden if hidden.dim() == 2 else hidden.reshape(-1, H)
     t = targets if targets.dim() == 1 else targets.reshape(-1)
     if t.dtype is not torch.int64 or not t.is_contiguous():
