@@ -26,11 +26,12 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules import module as nn_module
 
 from .embed import embedding_lookup
 from .front import B, BlockFront, ClockSpec, make_clock
 from .layer import EWS
-from .loss import linear_cross_entropy
+from .loss import linear_cross_entropy, logits_cross_entropy
 from .mixer import MixerEpilogue
 from .params import AParamBoundedRotation, AParamDampedRotation, AParamDefinitePlusSkew, is_rotation_planes
 
@@ -261,6 +262,16 @@ def _needs_grad(path, theta, module):
     return path.requires_grad or theta.requires_grad or any(p.requires_grad for p in module.parameters())
 
 
+def _is_plain(module, cls):
+    """Whether calling the module is cls.forward on its weights and nothing else: no hooks (they may set the weights, as
+    pruning does, or change the result) and no forward of its own."""
+    return (isinstance(module, cls) and type(module).forward is cls.forward and "forward" not in module.__dict__
+            and not (module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks
+                     or module._backward_hooks or nn_module._global_forward_pre_hooks
+                     or nn_module._global_forward_hooks or nn_module._global_backward_pre_hooks
+                     or nn_module._global_backward_hooks))
+
+
 class StackedEWS(nn.Module):
     """An encoder, ``num_blocks`` EWSBlocks and a head (ews/block.py:473-756). The encoder is an Embedding for
     tokens (``tokens=True``) or a Linear map for series; the head acts per position ("seq2seq") or on a masked mean
@@ -386,8 +397,19 @@ class StackedEWS(nn.Module):
             h = self._pool(h, mask)
         return self._cosine_logits(head, h) if self.cosine_head_tau is not None else head(h)
 
+    def _encode(self, X):
+        """The encoder's rows. A plain Embedding's by ``embedding_lookup``; anything else is called as the module it is."""
+        e = self.embedding
+        if not self.tokens:
+            return e(X)
+        if not _is_plain(e, nn.Embedding) or e.max_norm is not None or e.scale_grad_by_freq or e.sparse:
+            return e(X.long())
+        return embedding_lookup(X.long(), e.weight, padding_idx=e.padding_idx)
+
     def _head_loss(self, head, h, targets, ignore_index, reduction):
         if self.cosine_head_tau is None:
+            if not _is_plain(head, nn.Linear):
+                return logits_cross_entropy(head(h), targets, ignore_index, reduction)
             return linear_cross_entropy(h, head.weight, targets, bias=head.bias, ignore_index=ignore_index,
                                         reduction=reduction)
         h_hat, W_hat = self._unit(head, h)
@@ -399,7 +421,8 @@ class StackedEWS(nn.Module):
         """The softmax cross entropy of the heads' logits against whole-number targets (the reference's trainers'
         objective, e.g. experiments/fl/train.py:754-761), without the logits in memory (``linear_cross_entropy``) and
         with the embedding's gradient by sorted tokens (``embedding_lookup``): the forward's values are those of
-        ``forward`` and a cross entropy of its result. X, t, mask and raw_driver as ``forward``'s, with a batch;
+        ``forward`` and a cross entropy of its result. An embedding or a head that has hooks or a forward of its own is
+        called as a module, and its rows or logits are then in memory as ``forward``'s are. X, t, mask and raw_driver as ``forward``'s, with a batch;
         targets (B, L) for "seq2seq" (positions off the mask count as ignored), (B,) for "mean_pool"; for several heads
         a tuple of them, whose losses are added."""
         if X.dim() != (2 if self.tokens else 3):
@@ -410,8 +433,7 @@ class StackedEWS(nn.Module):
         all_targets = list(targets) if isinstance(targets, (tuple, list)) else [targets]
         if len(all_targets) != len(heads):
             raise ValueError(f"{len(heads)} head(s), {len(all_targets)} tensor(s) of targets")
-        h = embedding_lookup(X.long(), self.embedding.weight) if self.tokens else self.embedding(X)
-        h = self._blocks(h, t, mask, raw_driver, inference)
+        h = self._blocks(self._encode(X), t, mask, raw_driver, inference)
         if self.head_mode == "seq2seq":
             if mask is not None:
                 off = ~mask.to(torch.bool)

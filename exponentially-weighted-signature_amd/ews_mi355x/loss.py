@@ -115,6 +115,26 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return gh, gw, gb, None, None, None
 
 
+def logits_cross_entropy(logits, targets, ignore_index, reduction):
+    """``linear_cross_entropy`` of logits (..., V) that are in memory, in torch operations: for a head that is more than a
+    linear map. Ignored rows and targets outside the vocabulary are answered alike."""
+    if reduction not in nat.LOSS_REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(nat.LOSS_REDUCTIONS)}, got {reduction!r}")
+    if targets.shape != logits.shape[:-1]:
+        raise ValueError(f"targets must be {tuple(logits.shape[:-1])}, got {tuple(targets.shape)}")
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"targets must be int64 or int32, got {targets.dtype}")
+    kept = targets != ignore_index
+    known = (targets >= 0) & (targets < logits.shape[-1])
+    z = torch.where(kept[..., None], logits.float(), 0.0)
+    at = torch.where(known, targets, 0).long()
+    rows = -torch.log_softmax(z, -1).gather(-1, at[..., None])[..., 0]
+    rows = torch.where(kept, rows * torch.where(known | ~kept, 1.0, float("nan")), 0.0)
+    if reduction == "none":
+        return rows
+    return rows.sum() / kept.sum().clamp(min=1) if reduction == "mean" else rows.sum()
+
+
 def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, reduction="mean"):
     """Cross entropy of the logits ``hidden @ weight.T + bias`` with whole-number targets, in float32, without the
     logits in memory.
