@@ -75,8 +75,10 @@ struct Stats {
 
 // ------------------------------------------------------------------------------------------------- rows and planes
 // The three bfloat16 planes of a float32 number, x = p0 + p1 + p2 exactly: each plane is the rest rounded to eight bits
-// (cut where rounding would reach infinity), so the second is at most 2^-8 and the third 2^-16 of x. An infinity or
-// NaN has nothing after its first plane.
+// (cut where rounding would reach infinity), so the second is at most 2^-8 and the third 2^-16 of x. A NaN has nothing
+// after its first plane. An infinity is (1, 0, infinity) with its sign: the third plane meets the other side's first
+// alone, which has the sign of the whole (and is 0 where it is), while the 1 meets the third plane of an infinity on
+// the other side. So infinity times w is the infinity of its sign for w other than 0, and NaN for 0, as it has to be.
 __device__ __forceinline__ float plane_value(uint16_t p) { return __uint_as_float((uint32_t)p << 16); }
 __device__ __forceinline__ void planes(float x, uint16_t (&p)[3]) {
   const uint32_t u = __float_as_uint(x);
@@ -86,6 +88,10 @@ __device__ __forceinline__ void planes(float x, uint16_t (&p)[3]) {
   const float b = finite ? x - plane_value(p[0]) : 0.0f;
   p[1] = round_bf16(b);
   p[2] = round_bf16(b - plane_value(p[1]));
+  if ((u & 0x7fffffffu) == 0x7f800000u) {
+    p[2] = p[0];
+    p[0] = (uint16_t)((u >> 16 & 0x8000u) | 0x3f80u);
+  }
 }
 __device__ __forceinline__ void planes(bf16 x, uint16_t (&p)[1]) { p[0] = x.bits; }
 

@@ -54,7 +54,7 @@ struct Copier32 {
     }
     aim(32);
   }
-  // What each thread copies of a stage of `left` k; further ones read the last again (the other operand is zero there).
+  // What each thread copies of a stage of `left` k; further ones read the last again (product32 takes them out).
   __device__ __forceinline__ void aim(int left) {
     const uint32_t stride = (uint32_t)ld * 4;
 #pragma unroll
@@ -79,22 +79,25 @@ struct Copier32 {
   }
 };
 
-// Three planes of eight numbers. Finite numbers stay finite (the first plane is held to bfloat16's range).
+// Three planes of eight numbers. CAREFUL: finite numbers stay finite (the first plane is held to bfloat16's range), and
+// an infinity is (1, 0, infinity) with its sign, as in planes() of ews_loss.hip. Otherwise infinities and numbers that
+// round to one in bfloat16 have a plane of NaN, so that every result they are in is NaN.
+template <bool CAREFUL>
 __device__ __forceinline__ void cut(const float (&x)[8], bf16x8 (&p)[3]) {
   constexpr float kMost = 3.3895313892515355e+38f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    p[0][e] = (__bf16)fminf(fmaxf(x[e], -kMost), kMost);
+    const bool infinite = CAREFUL && __builtin_isinf(x[e]);
+    p[0][e] = (__bf16)(infinite ? copysignf(1.0f, x[e]) : CAREFUL ? fminf(fmaxf(x[e], -kMost), kMost) : x[e]);
     const float b = x[e] - (float)p[0][e];
-    p[1][e] = (__bf16)b;
+    p[1][e] = (__bf16)(infinite ? 0.0f : b);
     p[2][e] = (__bf16)(b - (float)p[1][e]);
   }
 }
 
-// As product() of ews_tiles.h; k blocks are of 32.
-template <class T, bool TURNED>
-__device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
-                                          char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
+template <class T, bool TURNED, bool CAREFUL>
+__device__ __forceinline__ void product32_once(const Operand32& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
+                                               char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b)
@@ -127,7 +130,7 @@ __device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, 
     arrive<0>();
     if (kb + 1 < kb1) copy(kb + 1, s ^ 1);
     const char* stage = lds + s * T::kStage;
-#pragma unroll
+#pragma unroll(CAREFUL ? 1 : 2)
     for (int ks = 0; ks < 2; ++ks) {
       float x[8];
       if (TURNED) {
@@ -146,6 +149,11 @@ __device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, 
           for (int e = 0; e < 4; ++e) x[4 * h + e] = w[e];
         }
       }
+      if (CAREFUL) {  // k past the end: the other operand is zero there, but zero times an infinity is not
+        const int left = (TURNED ? P.rows : P.cols) - kb * 32;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 16 * ks + 8 * half + e < left ? x[e] : 0.0f;
+      }
       bf16x8 p[3], q[3][T::TJ];
 #pragma unroll
       for (int n = 0; n < 3; ++n)
@@ -153,7 +161,7 @@ __device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, 
         for (int b = 0; b < T::TJ; ++b)
           q[n][b] = *reinterpret_cast<const bf16x8*>(stage + T::kBytesP + (n * T::J + b * 32 + r32) * 64 +
                                                      ((2 * ks + half) ^ ((r32 >> 2) & 3)) * 16);
-      cut(x, p);
+      cut<CAREFUL>(x, p);
 #pragma unroll
       for (int pair = 0; pair < kPairs; ++pair)
 #pragma unroll
@@ -163,6 +171,27 @@ __device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, 
     }
   }
   arrive<0>();
+}
+
+// As product() of ews_tiles.h; k blocks are of 32. A tile with a NaN is formed once more, with care: infinities cost such
+// tiles twice the time and the others nothing (told apart number by number they cost all calls 3 to 10%).
+template <class T, bool TURNED>
+__device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
+                                          char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
+  product32_once<T, TURNED, false>(P, Q, i0, j0, kb0, kb1, lds, acc);
+  bool bad = false;
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bad |= __builtin_isnan(acc[0][b][r]);
+  int* flags = reinterpret_cast<int*>(lds);  // nobody reads a stage any more
+  bad = __any(bad);
+  if ((threadIdx.x & 63) == 0) flags[threadIdx.x >> 6] = bad;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < T::WI * T::WJ; ++w) bad |= flags[w] != 0;
+  __syncthreads();
+  if (bad) product32_once<T, TURNED, true>(P, Q, i0, j0, kb0, kb1, lds, acc);
 }
 
 }  // namespace tiles

@@ -144,7 +144,9 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     "sum", or "none" for every row's own loss, (...). Differentiable in hidden, weight and bias (reverse mode).
 
     Rows whose target is ``ignore_index`` have loss and gradient zero, whatever they hold, and cost nothing. A target
-    outside [0, V) that is not ``ignore_index`` gives NaN. A bias of -inf takes a token out of the vocabulary."""
+    outside [0, V) that is not ``ignore_index`` gives NaN. A bias of -inf takes a token out of the vocabulary, and so
+    does a logit of -inf from an infinite weight; a row with a logit of +inf or NaN has a loss of NaN. A row whose target
+    has been taken out has an infinite loss, and its gradients may be NaN."""
     if reduction not in nat.LOSS_REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(nat.LOSS_REDUCTIONS)}, got {reduction!r}")
     if weight.dim() != 2 or weight.numel() == 0:
