@@ -7,6 +7,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from .embed import DTYPES, check_tensor, launch, refuse_tangents
@@ -61,10 +62,12 @@ def _norm_and_scale(tensors, outs, max_norm):
     ws = torch.empty(int(lib.ews_clip_workspace_bytes(n, counts)), device=dev, dtype=torch.uint8)
     nat.check(launch(dev, lib.ews_clip, n, ptrs, out, counts, types, max_norm, 0 if outs is None else 1,
                      result.data_ptr(), ws.data_ptr()), "ews_clip")
-    if outs is not None and dst is not outs:
-        for o, d in zip(outs, dst):
-            if o is not d:
-                o.copy_(d)
+    if outs is not None:
+        increment_version(outs)  # a graph that has saved one of them refuses its backward, as after torch's own writes
+        if dst is not outs:
+            for o, d in zip(outs, dst):
+                if o is not d:
+                    o.copy_(d)
     return result[0]
 
 

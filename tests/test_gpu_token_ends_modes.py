@@ -43,3 +43,44 @@ def test_jvp_is_refused():
         torch.func.jvp(lambda x: E.embedding_lookup(t, x), (w,), (w,))
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.jvp(lambda x: E.linear_cross_entropy(x, w, t), (h,), (h,))
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_clipping_in_place_is_seen_by_graphs_that_saved_the_gradient(strided):
+    """A product has saved the gradient; once it is clipped the product's backward would be another number's."""
+
+    def tensor():
+        return torch.randn(8, 6, device=DEV)[:, ::2] if strided else torch.randn(8, 3, device=DEV)
+
+    def saved(g):
+        w = torch.ones(g.shape, device=DEV, requires_grad=True)
+        return (w * g).sum()
+
+    g = tensor()
+    for call in (lambda: E.clip_grads([g], 1e-3, out=[g]), lambda: E.clip_grads([tensor()], 1e-3, out=[g]),
+                 lambda: E.clip_grads([g], 1e6, out=[g])):
+        y, before = saved(g), g._version
+        call()
+        assert g._version > before
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    p = torch.zeros(8, 3, device=DEV, requires_grad=True)
+    p.grad = tensor()
+    y = saved(p.grad)
+    E.clip_grad_norm_([p], 1e-3)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    # what is only read stays as it was
+    y = saved(g)
+    E.global_grad_norm([g])
+    E.clip_grads([g], 1e-3)
+    y.backward()
+
+
+def test_clipping_under_inference_mode():
+    with torch.inference_mode():
+        g = torch.randn(8, 3, device=DEV)
+        want = g.clone()
+        norm, out = E.clip_grads([g], 1e-3)
+        E.clip_grads([g], 1e-3, out=[g])
+        assert torch.equal(g, out[0]) and not torch.equal(g, want)
