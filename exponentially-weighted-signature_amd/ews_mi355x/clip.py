@@ -25,13 +25,14 @@ def _dense(t):
     return True
 
 
-def _tables(tensors, outs):
-    n = len(tensors)
-    ptrs = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in tensors])
-    out = ptrs if outs is tensors else (ctypes.c_uint64 * n)(*[t.data_ptr() for t in outs])
-    counts = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    types = (ctypes.c_int32 * n)(*[DTYPES[t.dtype] for t in tensors])
-    return n, ptrs, out, counts, types
+def _by_place(tensors):
+    """The tensors by the memory that they name; several of the same (one named twice, two views alike) give one. Empty
+    ones name none."""
+    places = {}
+    for t in tensors:
+        n = t.numel()
+        places[(t.data_ptr(), n, None if t.is_contiguous() else (t.shape, t.stride())) if n else id(t)] = t
+    return places
 
 
 def _check(tensors):
@@ -47,7 +48,8 @@ def _check(tensors):
 
 
 def _norm_and_scale(tensors, outs, max_norm):
-    """The norm of tensors; where outs is not None, outs = the clipped tensors (outs is tensors: in place)."""
+    """The norm of tensors; where outs is not None, outs = the clipped tensors (outs is tensors: in place, memory that is
+    named twice counting once)."""
     lib = nat.load()
     dev = tensors[0].device
     src = dst = tensors
@@ -57,7 +59,18 @@ def _norm_and_scale(tensors, outs, max_norm):
         dst = outs
         if src is not tensors or not all([o.is_contiguous() for o in outs]):
             dst = [o if _dense(o) and o.stride() == s.stride() else torch.empty_like(s) for o, s in zip(outs, src)]
-    n, ptrs, out, counts, types = _tables(src, dst)
+    n, at = len(src), [t.data_ptr() for t in src]
+    to = at if outs is None or dst is src else [t.data_ptr() for t in dst]
+    if outs is not None and len(set(to if dst is outs else [t.data_ptr() for t in outs])) < n:
+        places = _by_place(outs)
+        if len(places) < n:  # in place, two workgroups would scale it once or twice, as it happens
+            if outs is not tensors:
+                raise ValueError("out names the same memory twice")
+            once = list(places.values())
+            return _norm_and_scale(once, once, max_norm)
+    ptrs, counts = (ctypes.c_uint64 * n)(*at), (ctypes.c_int64 * n)(*[t.numel() for t in src])
+    out = ptrs if to is at else (ctypes.c_uint64 * n)(*to)
+    types = (ctypes.c_int32 * n)(*[DTYPES[t.dtype] for t in src])
     result = torch.empty(2, device=dev, dtype=torch.float32)
     ws = torch.empty(int(lib.ews_clip_workspace_bytes(n, counts)), device=dev, dtype=torch.uint8)
     nat.check(launch(dev, lib.ews_clip, n, ptrs, out, counts, types, max_norm, 0 if outs is None else 1,
@@ -92,7 +105,8 @@ def global_grad_norm(tensors):
 @torch.no_grad()
 def clip_grads(grads, max_norm, out=None):
     """(norm, clipped): ``grads`` times ``min(1, max_norm / (norm + 1e-6))``, written to the tensors of ``out`` (same
-    shapes and types; a tensor of grads itself: in place; otherwise without overlap) or to new ones."""
+    shapes and types; a tensor of grads itself: in place; otherwise without overlap, and no two of the same memory) or to
+    new ones."""
     grads = list(grads)
     max_norm = _max_norm(max_norm)
     if not grads:
@@ -116,7 +130,8 @@ def clip_grads(grads, max_norm, out=None):
 def clip_grad_norm_(parameters, max_norm):
     """Scales the gradients of ``parameters`` (an iterable, or one) in place by ``min(1, max_norm / (norm + 1e-6))`` and
     returns their norm, a float32 number on the device; the host does not wait. Parameters without a gradient are left
-    out, and one that is named twice counts once. A norm that is not finite scales by 0 (infinite) or NaN, as the formula does."""
+    out; one that is named twice, or whose gradient is another's memory, counts once. A norm that is not finite scales by
+    0 (infinite) or NaN, as the formula does."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     grads = list(dict.fromkeys(p.grad for p in parameters if p.grad is not None))
     max_norm = _max_norm(max_norm)

@@ -84,3 +84,32 @@ def test_clipping_under_inference_mode():
         norm, out = E.clip_grads([g], 1e-3)
         E.clip_grads([g], 1e-3, out=[g])
         assert torch.equal(g, out[0]) and not torch.equal(g, want)
+
+
+def test_memory_named_twice_is_scaled_once():
+    """Two workgroups that scale one tensor in place would scale it once or twice, as it happens."""
+    g = torch.randn(70, 33, device=DEV)
+    p, q, r = (torch.zeros(70, 33, device=DEV, requires_grad=True) for _ in range(3))
+    p.grad, q.grad = g.clone(), torch.randn(70, 33, device=DEV)
+    r.grad = p.grad.view(70, 33)
+    e = torch.zeros(0, device=DEV, requires_grad=True)
+    e.grad = torch.zeros(0, device=DEV)
+    want_norm, want = E.clip_grads([g, q.grad.clone()], 0.5)
+    norm = E.clip_grad_norm_([p, q, e, r, e, p], 0.5)
+    assert torch.equal(norm, want_norm)
+    assert torch.equal(p.grad, want[0]) and torch.equal(q.grad, want[1])
+    for out in ([g, g], [g, g.view(70, 33)]):
+        with pytest.raises(ValueError, match="twice"):
+            E.clip_grads([g, g], 0.5, out=out)
+    none = [torch.zeros(0, device=DEV) for _ in range(2)]
+    E.clip_grads(none, 0.5, out=none)
+    # a row and a column that begin alike are not the same memory
+    base = torch.randn(33, 40, device=DEV)
+    rows = [base[:, :20], base[:, 20:]]
+    assert len(E.clip_grads(rows, 0.5, out=rows)[1]) == 2
+    s, t = (torch.zeros(40, device=DEV, requires_grad=True) for _ in range(2))
+    line = torch.randn(80, device=DEV)
+    line[0] = 0.0
+    s.grad, t.grad = line[:40], line[::2]
+    assert float(E.clip_grad_norm_([s, t], 1e9)) == pytest.approx(
+        float((line[:40].square().sum() + line[::2].square().sum()).sqrt()), rel=1e-6)
