@@ -48,7 +48,8 @@ struct Args {
   int deal, range; // token t is entry t >> deal of workgroup t % 2^deal of k_sort, which owns 2^range (its slot)
   int lanes;       // lanes a row of the lookup is spread over
   int run;         // sorted positions a wavefront of k_runs adds up
-  int runs, tiles; // how many there are, and column tiles of a row
+  int runs;        // how many there are
+  uint32_t tiles;  // column tiles of a row
   float scale;
   const void* tokens;
   const void* weight;
@@ -231,12 +232,15 @@ __device__ __forceinline__ void zero_absent(const Args& a, int v, int col) {
   z.store_past((T*)a.gweight + (int64_t)v * a.H + col);
 }
 
+// The unit of a wavefront of workgroups of four, in the grid of unit_grid().
+__device__ __forceinline__ uint32_t unit_of(int wave) { return (blockIdx.y * gridDim.x + blockIdx.x) * 4 + wave; }
+
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_runs(Args a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // a row's column tiles are neighbours; run and tile are scalar, so positions and tokens are scalar loads
-  const int unit = (int)blockIdx.x * 4 + wave, run = unit / a.tiles;
-  const int col = ((unit - run * a.tiles) * 64 + lane) * V;
+  const uint32_t unit = unit_of(wave);
+  const int run = (int)(unit / a.tiles), col = ((int)(unit % a.tiles) * 64 + lane) * V;
   if (run >= a.runs) return zero_absent<T, V>(a, run - a.runs, col);
   const int total = a.start[1 << (a.deal + a.range)];
   const int64_t b = (int64_t)run * a.run;
@@ -295,8 +299,8 @@ __global__ __launch_bounds__(256) void k_runs(Args a) {
 template <typename T, int V, typename Tok>
 __global__ __launch_bounds__(256) void k_few(Args a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int unit = (int)blockIdx.x * 4 + wave, v = unit / a.tiles;
-  const int col = ((unit - v * a.tiles) * 64 + lane) * V;
+  const uint32_t unit = unit_of(wave);
+  const int v = (int)(unit / a.tiles), col = ((int)(unit % a.tiles) * 64 + lane) * V;
   if (v >= a.V) return;
   const bool in = col < a.H;
   const T* g = (const T*)a.gout + (in ? col : 0);
@@ -424,6 +428,15 @@ struct EPlan {
   size_t order, sorted, start, part, total;
 };
 
+// Units of one wavefront each (a row or run by one column tile) that a launch has. A grid's x holds fewer than 2^32
+// threads, so workgroups past 2^23 go to y; their number stays below 2^32 with the last y's that are over.
+constexpr int64_t kMostUnits = ((int64_t)1 << 32) - (1 << 26);
+
+dim3 unit_grid(int64_t units) {
+  const int64_t blocks = (units + 3) / 4, x = blocks < 1 << 23 ? blocks : 1 << 23;
+  return dim3((uint32_t)x, (uint32_t)((blocks + x - 1) / x));
+}
+
 size_t al256e(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int embed_plan(const ews_embed_desc* s, EPlan& p) {
@@ -444,6 +457,8 @@ int embed_plan(const ews_embed_desc* s, EPlan& p) {
   p.run = 32;
   while (p.run > 8 && s->count / p.run * tiles < 2048) p.run /= 2;
   p.runs = (s->count + p.run - 1) / p.run;
+  // with the narrowest tiles, so that what is refused does not depend on addresses, nor on the direction
+  if ((p.runs + s->vocab) * ((s->width + 63) / 64) > kMostUnits) return EWS_ERR_SHAPE;
   size_t off = 0;
   if (s->count <= kFewTokens) {
     p.total = 0;
@@ -490,9 +505,7 @@ int launch_lookup(const ews_embed_desc* s, Args a, hipStream_t st) {
 template <typename T, int V>
 int launch_few(const ews_embed_desc* s, Args a, hipStream_t st) {
   a.tiles = (a.H + 64 * V - 1) / (64 * V);
-  const int64_t units = (int64_t)a.V * a.tiles;
-  if (units > ((int64_t)1 << 26) - 4) return EWS_ERR_SHAPE;  // a launch has fewer than 2^32 threads
-  const dim3 grid((uint32_t)((units + 3) / 4));
+  const dim3 grid = unit_grid((int64_t)a.V * a.tiles);
   if (s->token_bytes == 8)
     hipLaunchKernelGGL((k_few<T, V, int64_t>), grid, dim3(256), 0, st, a);
   else
@@ -503,9 +516,7 @@ int launch_few(const ews_embed_desc* s, Args a, hipStream_t st) {
 template <typename T, int V>
 int launch_sums(const EPlan& p, Args a, hipStream_t st) {
   a.tiles = (a.H + 64 * V - 1) / (64 * V);
-  const int64_t units = (p.runs + a.V) * a.tiles;
-  if (units > ((int64_t)1 << 26) - 4) return EWS_ERR_SHAPE;  // a launch has fewer than 2^32 threads
-  hipLaunchKernelGGL((k_runs<T, V>), dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_runs<T, V>), unit_grid((p.runs + a.V) * a.tiles), dim3(256), 0, st, a);
   if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH;
   const int v = a.H % 4 == 0 ? 4 : 1;  // partial rows that start at multiples of 16 bytes
   const dim3 grid((uint32_t)p.runs, (a.H + 64 * v * kJoinWaves - 1) / (64 * v * kJoinWaves));

@@ -595,6 +595,7 @@ int ews_lift_backward(const ews_lift_desc* desc, const float* branch, const floa
  * eqx.nn.Embedding, head with softmax cross entropy, and global-norm clipping): the operators at the two ends of a
  * step. Their sums are float32 (norms float64) in a fixed order: the same inputs give the same bits.
  * --------------------------------------------------------------------------------------------------------- */
+/* Also (V + n / 8) ceil(H / 64) up to 2^32 - 2^26, which a table of 288 GB does not reach. */
 typedef struct ews_embed_desc {
   int64_t count;         /* n: tokens, 1..2^25 */
   int64_t weight_stride; /* elements between the table's rows, at least width */
