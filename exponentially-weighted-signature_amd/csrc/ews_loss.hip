@@ -737,7 +737,7 @@ constexpr int64_t kChunkBytes = (int64_t)2 << 30;
 constexpr int kFewRows32 = 512;
 constexpr int64_t kFewLogits32 = 1 << 22;
 // A call without gradients keeps eight bytes for every row's slabs (64 of the vocabulary at least) of as many rows as
-// fit here.
+// fit here. Float32 W read as it is has slabs of 32, but few rows or logits: half as much at most.
 constexpr int64_t kScoreBytes = (int64_t)256 << 20;
 
 // Stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared.
@@ -893,15 +893,20 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
 }
 
 // bfloat16 weights whose rows start at multiples of 16 bytes and fill whole k blocks are read where they are, and
-// float32 weights for few rows (of a stride that the tiles' offsets hold).
-bool reads_direct(const ews_loss_desc* s, const void* weight) {
+// float32 weights for few rows (of a stride that the tiles' offsets hold). Here what the sizes allow; bfloat16's address
+// has to fit too.
+bool may_read_direct(const ews_loss_desc* s) {
   if (s->weight_stride > 1 << 22) return false;
   if (s->dtype == EWS_DTYPE_F32) {
     // the three planes of h, and of a chunk's dz, lie within 32-bit offsets
     if ((s->rows + 63) * (int64_t)(s->hidden + 63) > 1 << 29 || s->vocab > 1 << 20) return false;
     return s->rows <= kFewRows32 || s->rows * (int64_t)s->vocab <= kFewLogits32;
   }
-  return (uintptr_t)weight % 16 == 0 && s->hidden % 64 == 0 && s->weight_stride % 8 == 0;
+  return s->hidden % 64 == 0 && s->weight_stride % 8 == 0;
+}
+
+bool reads_direct(const ews_loss_desc* s, const void* weight) {
+  return may_read_direct(s) && (s->dtype == EWS_DTYPE_F32 || (uintptr_t)weight % 16 == 0);
 }
 
 struct Call {
@@ -1249,9 +1254,9 @@ extern "C" {
 size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train) {
   LPlan p;
   if (loss_plan(desc, train != 0, false, p) != EWS_OK) return 0;
-  // the weight's address decides how it is read; read as it is it needs no packed copy, but float32's tiles are smaller
-  // (more slabs and splits)
-  const size_t packed = p.total;
+  if (!may_read_direct(desc)) return p.total;
+  // read as it is W needs no packed copy; bfloat16's address, which is not known here, may ask for one all the same
+  const size_t packed = desc->dtype == EWS_DTYPE_F32 ? 0 : p.total;
   loss_plan(desc, train != 0, true, p);
   return p.total > packed ? p.total : packed;
 }

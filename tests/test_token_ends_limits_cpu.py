@@ -26,3 +26,24 @@ def test_lookup_and_gradient_take_the_same_sizes(vocab, width, taken, dtype, cou
     assert lib.ews_embed_forward(d, NULL, NULL, NULL, NULL) == code
     assert lib.ews_embed_backward(d, NULL, NULL, NULL, NULL, NULL) == code
     assert (lib.ews_embed_workspace_bytes(d) > 0) == (taken and count > 256)
+
+
+def _scratch(rows, train, hidden=512, vocab=100003, dtype=0, reduction=1):
+    d = nat.LossDesc(hidden_stride=hidden, weight_stride=hidden, ignore_index=-100, rows=rows, hidden=hidden, vocab=vocab,
+                     dtype=dtype, bias_dtype=0, reduction=reduction)
+    return nat.load().ews_loss_workspace_bytes(d, train)
+
+
+@pytest.mark.parametrize("rows,hidden", [(65536, 64), (1 << 20, 64), (8192, 512), (600, 64), (600, 4096)])
+def test_float32_scores_keep_256_mib_of_slabs(rows, hidden):
+    """Beside the planes of rows and weight and eight numbers a row or token at most."""
+    planes = (rows + 100003) * ((hidden + 63) // 64 * 64) * 6
+    assert _scratch(rows, 0, hidden) <= planes + (256 << 20) + 32 * (rows + 100003 + 1024)
+
+
+@pytest.mark.parametrize("rows,train,most", [(1, 0, 2 << 20), (512, 0, 140 << 20), (64, 1, 180 << 20)])
+def test_float32_weight_read_as_it_is_has_no_copy(rows, train, most):
+    """Few rows: W (1.6 GB here, its planes 2.5) is not copied. A row has a slab's eight bytes for 32 tokens, in training
+    ten bytes a token, and the results of up to 128 splits of dh."""
+    splits = 128 * rows * 4096 * 4 if train else 0
+    assert _scratch(rows, train, 4096) <= most + splits
