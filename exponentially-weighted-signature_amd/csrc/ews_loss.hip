@@ -1261,6 +1261,11 @@ size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train) {
   return p.total > packed ? p.total : packed;
 }
 
+size_t ews_loss_workspace_bytes_for(const ews_loss_desc* desc, const void* weight, int train) {
+  LPlan p;
+  return loss_plan(desc, train != 0, desc && reads_direct(desc, weight), p) == EWS_OK ? p.total : 0;
+}
+
 int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,
                      const int64_t* targets, float* loss, void* workspace, ews_stream_t stream) {
   LPlan p;

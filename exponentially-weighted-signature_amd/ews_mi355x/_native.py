@@ -94,6 +94,7 @@ EXPORTED = (
     "ews_embed_workspace_bytes",
     "ews_embed_backward",
     "ews_loss_workspace_bytes",
+    "ews_loss_workspace_bytes_for",
     "ews_loss_forward",
     "ews_loss_train",
     "ews_loss_keeps",
@@ -438,6 +439,8 @@ def load():
     lsp = ctypes.POINTER(LossDesc)
     lib.ews_loss_workspace_bytes.argtypes = [lsp, i32]
     lib.ews_loss_workspace_bytes.restype = sz
+    lib.ews_loss_workspace_bytes_for.argtypes = [lsp, vp, i32]
+    lib.ews_loss_workspace_bytes_for.restype = sz
     lib.ews_loss_forward.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp]
     lib.ews_loss_forward.restype = i32
     lib.ews_loss_train.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]

@@ -26,7 +26,8 @@ class _Call:
                                  nat.DTYPE_F32 if bias is None else DTYPES[bias.dtype], nat.LOSS_REDUCTIONS[reduction])
 
     def workspace(self, train):
-        return self.hidden.new_empty(nat.load().ews_loss_workspace_bytes(self.desc, train), dtype=torch.uint8)
+        size = nat.load().ews_loss_workspace_bytes_for(self.desc, self.weight.data_ptr(), train)
+        return self.hidden.new_empty(size, dtype=torch.uint8)
 
     def inputs(self):
         return self.desc, self.hidden.data_ptr(), self.weight.data_ptr(), _ptr(self.bias), self.targets.data_ptr()

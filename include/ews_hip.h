@@ -639,6 +639,10 @@ typedef struct ews_loss_desc {
  * keeps 2 GiB of probabilities at most (of 256 rows where those need more). */
 size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train);
 
+/* The same for calls with this weight (its address alone matters: nothing is read). A bfloat16 weight whose rows can be
+ * read where they are needs no packed copy, which the query above has to allow for. */
+size_t ews_loss_workspace_bytes_for(const ews_loss_desc* desc, const void* weight, int train);
+
 /* z = hidden weight^T + bias (bias may be NULL; entries of -inf take a token out of the vocabulary),
  * loss_n = log sum_v exp z_nv - z_n,target. A target outside [0, vocab) that is not ignore_index: NaN. */
 int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,

@@ -47,3 +47,22 @@ def test_float32_weight_read_as_it_is_has_no_copy(rows, train, most):
     ten bytes a token, and the results of up to 128 splits of dh."""
     splits = 128 * rows * 4096 * 4 if train else 0
     assert _scratch(rows, train, 4096) <= most + splits
+
+
+@pytest.mark.parametrize("train", [0, 1])
+@pytest.mark.parametrize("rows,hidden,dtype", [(1, 4096, 1), (1000, 4096, 1), (1, 4000, 1), (3, 4096, 0), (7000, 512, 0)])
+def test_scratch_of_a_weight_at_an_address(rows, hidden, dtype, train):
+    """The query without the address holds any weight's; with it, a bfloat16 weight that is read where it is has no copy."""
+    lib = nat.load()
+    d = nat.LossDesc(hidden_stride=hidden, weight_stride=hidden, ignore_index=-100, rows=rows, hidden=hidden,
+                     vocab=100003, dtype=dtype, bias_dtype=0, reduction=0)
+    any_weight = lib.ews_loss_workspace_bytes(d, train)
+    aligned, odd = (lib.ews_loss_workspace_bytes_for(d, ctypes.c_void_p(a), train) for a in (4096, 4098))
+    copy = 100003 * ((hidden + 63) // 64 * 64) * 2
+    assert max(aligned, odd) == any_weight
+    assert aligned == any_weight - (copy + 255) // 256 * 256 if dtype == 1 and hidden % 64 == 0 else aligned == odd
+    if rows == 1 and hidden == 4096 and not train:
+        assert aligned < 1 << 20
+    assert lib.ews_loss_workspace_bytes_for(None, None, train) == 0
+    d.rows = 0
+    assert lib.ews_loss_workspace_bytes_for(d, ctypes.c_void_p(4096), train) == 0
