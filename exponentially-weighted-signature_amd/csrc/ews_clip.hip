@@ -6,7 +6,9 @@
 // writes once. The tensors go by value in a launch's arguments (kMany to a launch): no table is copied to the device
 // and the host waits for nothing. A workgroup takes one chunk of one tensor; squares are added in float64, so no
 // gradient that float32 holds overflows or vanishes, and the chunks' sums are added in a fixed order.
-// The scaling walks the chunks backwards: the data read last by the norm is read first, while it is in the caches.
+// A scaling launch walks its chunks backwards: of a set in one launch the data read last by the norm is read first, while
+// it is in the caches. The launches of a larger set go in the norm's order: backwards too they measured the same (196
+// tensors, 1.2 GB: 656 us for 659; 132 tensors, 6.4 GB: 3480 for 3475).
 // In place with c = 1 nothing is read or written again.
 //
 // 3.2 G bfloat16 numbers in 132 tensors: read for the norm in 1.07 ms (6.1 TB/s), scaled in 2.35 (5.5 TB/s).
