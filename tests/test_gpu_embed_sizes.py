@@ -44,3 +44,24 @@ def test_more_rows_than_a_grid_holds(n):
     gout = torch.randn(n, H, generator=g, device=DEV).bfloat16()
     (grad,) = torch.autograd.grad(out, w, gout)
     _check(grad, t, gout, 0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,H,half", [(9000, 60000, 24, False), (30001, 131072, 16, True), (5000, 131073, 40, False),
+                                        (40003, 200003, 20, True), (3000, 1000003, 8, True)])
+def test_vocabularies_of_many_sorting_workgroups(n, V, H, half, dtype):
+    """A workgroup that owns 256 and 512 tokens; 512 to 2048 workgroups. half: half the text is one token, more than a
+    wavefront lists."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    t = torch.randint(0, V, (n,), generator=g, device=DEV)
+    t[:6] = torch.tensor([0, V - 1, V // 2, 511, 512, 255], device=DEV)
+    if half:
+        t[torch.rand(n, generator=g, device=DEV) < 0.5] = V - 3
+    w = torch.randn(V, H, generator=g, device=DEV).to(dtype).requires_grad_()
+    gout = torch.randn(n, H, generator=g, device=DEV).to(dtype)
+    for tokens in (t, t.int()):
+        out = E.embedding_lookup(tokens, w, scale=2.5)
+        (grad,) = torch.autograd.grad(out, w, gout)
+        _check(grad, t, gout, 2.5)
+    (again,) = torch.autograd.grad(E.embedding_lookup(t, w, scale=2.5), w, gout)
+    assert torch.equal(grad, again)
