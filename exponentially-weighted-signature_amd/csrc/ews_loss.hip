@@ -759,7 +759,7 @@ enum Kind { kLarge, kMedium, kFlat, kFew32, kMore32 };
 
 struct Product {
   Kind kind;
-  int ti, tj, tile_i, slab, splits, per, kblocks, pairs;
+  int ti, tj, tile_i, tile_j, slab, splits, per, kblocks, pairs;
 };
 
 struct LPlan {
@@ -797,8 +797,9 @@ Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split, bool as_i
   const int slab[] = {Large::kSlab, Medium::kSlab, Flat::kSlab, Few32<16>::kSlab, More32<16>::kSlab};
   p.slab = slab[p.kind];
   p.tile_i = tile_i[p.kind];
+  p.tile_j = tile_j[p.kind];
   p.ti = ceil_div(I, p.tile_i);
-  p.tj = ceil_div(J, tile_j[p.kind]);
+  p.tj = ceil_div(J, p.tile_j);
   p.splits = 1;
   p.per = kblocks;
   // one round of workgroups: a CU holds one of the large tiles, two of the others
@@ -1264,6 +1265,20 @@ size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train) {
 size_t ews_loss_workspace_bytes_for(const ews_loss_desc* desc, const void* weight, int train) {
   LPlan p;
   return loss_plan(desc, train != 0, desc && reads_direct(desc, weight), p) == EWS_OK ? p.total : 0;
+}
+
+int ews_loss_tile(const ews_loss_desc* desc, const void* weight, int train, int product, int32_t* tile) {
+  LPlan p;
+  const int rc = loss_plan(desc, train != 0, desc && reads_direct(desc, weight), p);
+  if (rc != EWS_OK) return rc;
+  if (!tile) return EWS_ERR_NULL;
+  if (product < 0 || product > (train ? 2 : 0)) return EWS_ERR_OPTION;
+  const Product& q = product == 0 ? p.logits : product == 1 ? p.dh : p.dw;
+  tile[0] = q.tile_i;
+  tile[1] = q.tile_j;
+  tile[2] = q.splits;
+  tile[3] = p.chunks;
+  return EWS_OK;
 }
 
 int ews_loss_forward(const ews_loss_desc* desc, const void* hidden, const void* weight, const void* bias,

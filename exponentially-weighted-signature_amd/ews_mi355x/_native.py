@@ -95,6 +95,7 @@ EXPORTED = (
     "ews_embed_backward",
     "ews_loss_workspace_bytes",
     "ews_loss_workspace_bytes_for",
+    "ews_loss_tile",
     "ews_loss_forward",
     "ews_loss_train",
     "ews_loss_keeps",
@@ -441,6 +442,8 @@ def load():
     lib.ews_loss_workspace_bytes.restype = sz
     lib.ews_loss_workspace_bytes_for.argtypes = [lsp, vp, i32]
     lib.ews_loss_workspace_bytes_for.restype = sz
+    lib.ews_loss_tile.argtypes = [lsp, vp, i32, i32, ctypes.POINTER(i32)]
+    lib.ews_loss_tile.restype = i32
     lib.ews_loss_forward.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp]
     lib.ews_loss_forward.restype = i32
     lib.ews_loss_train.argtypes = [lsp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
