@@ -179,3 +179,31 @@ def test_the_two_halves_give_the_whole(reduction, N, dtype):
     want = _reference(h, w, b, t, up, reduction)
     for name, a, (r, e) in zip(("loss", "grad_hidden", "grad_weight", "grad_bias"), one, want):
         _close(a.reshape(r.shape), r, e, name)
+
+
+@pytest.mark.parametrize("reduction,N,V", [("mean", 300, 1003), ("none", 300, 1003), ("sum", 1030, 9001)])
+def test_dz_number_by_number(reduction, N, V):
+    """Row n of h is 3 in column n alone, so a number of dW is 3 dz of one row: dz's errors do not average out. One
+    rounding of dz to bfloat16, one of the result and the logarithm's steps are allowed; probabilities held in bfloat16
+    would add a rounding."""
+    H = N
+    _, w, b, t, up = _inputs(N, H, V, torch.bfloat16)
+    w = (w.float() * math.sqrt(H)).bfloat16()  # logits of a few units
+    h = torch.zeros(N, H, device=DEV, dtype=torch.bfloat16).fill_diagonal_(3.0).requires_grad_()
+    w.requires_grad_()
+    loss = E.linear_cross_entropy(h, w, t, bias=b, reduction=reduction)
+    (gw,) = torch.autograd.grad(loss, [w], up if reduction == "none" else None)
+    z = 3.0 * w.detach().double().t() + b.double()
+    d = torch.softmax(z, 1)
+    kept = (t != -100).nonzero()[:, 0]
+    d[kept, t[kept]] -= 1.0
+    d *= (t != -100)[:, None]
+    d *= (up.double() if reduction == "none" else torch.full_like(z[:, 0], 1.0 / len(kept)) if reduction == "mean"
+          else torch.ones_like(z[:, 0]))[:, None]
+    want = 3.0 * d.t()
+    half = 2.0**-8
+    f32 = 16 * U + 8 * U * (1 + float(z.abs().max()))  # the logits', the sums' and the factors' roundings
+    bound = (1.01 * half + half + 1.1 * 2.0**-10.5 + f32) * want.abs()
+    own = torch.zeros_like(bound)
+    own[t[kept], kept] = 3.0 * f32  # the targets' entries: p - 1 of a p that is off by f32
+    _close(gw, want, bound + own, "dW")
