@@ -69,7 +69,9 @@ class _Call:
 
 class _LinearCrossEntropy(torch.autograd.Function):
     """The mean and the sum have one upstream number, so their forward computes the gradients with the loss in one pass
-    over the rows and the first backward scales them. The rows' own losses keep the probabilities for the first
+    over the rows and the first backward scales them: for an upstream that is no power of two a bfloat16 gradient is
+    rounded a second time (float32 until then would be twice the memory, and a pass over it in every step, also in the
+    ordinary one whose upstream is 1 and for which nothing is read). The rows' own losses keep the probabilities for the first
     backward, where they fit the scratch (2 GiB). A second backward of the same graph, and the rows' own losses of
     more, compute the probabilities once more."""
 
@@ -143,6 +145,10 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     hidden (..., H) and weight (V, H), both float32 or both bfloat16, bias (V,) of either type or None, targets (...)
     int64 or int32, all on the HIP device. ``reduction``: "mean" over the rows that are not ignored (0 where all are),
     "sum", or "none" for every row's own loss, (...). Differentiable in hidden, weight and bias (reverse mode).
+
+    Where a gradient is required the mean and the sum form it with the loss, three products for one: a validation loss is
+    best taken under ``torch.no_grad``. bfloat16 gradients are rounded once where the upstream number of the mean or the
+    sum is a power of two (1 as a rule), else a second time after the multiplication by it.
 
     Rows whose target is ``ignore_index`` have loss and gradient zero, whatever they hold, and cost nothing. A target
     outside [0, V) that is not ``ignore_index`` gives NaN. A bias of -inf takes a token out of the vocabulary, and so

@@ -671,7 +671,7 @@ int ews_loss_kept(const ews_loss_desc* desc, const void* weight, const float* up
                   void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream);
 
 /* grad_* = factor[0] grad_* in place (each may be NULL), factor on the device: the gradients of factor[0] times the
- * loss. With a factor of 1 nothing is touched. */
+ * loss. With a factor of 1 nothing is touched; one that is no power of two rounds them to their type a second time. */
 int ews_loss_scale(const ews_loss_desc* desc, void* grad_hidden, void* grad_weight, void* grad_bias,
                    const float* factor, ews_stream_t stream);
 

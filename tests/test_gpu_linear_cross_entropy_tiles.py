@@ -207,3 +207,26 @@ def test_dz_number_by_number(reduction, N, V):
     own = torch.zeros_like(bound)
     own[t[kept], kept] = 3.0 * f32  # the targets' entries: p - 1 of a p that is off by f32
     _close(gw, want, bound + own, "dW")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_an_upstream_number_multiplies_the_rounded_gradients(reduction, dtype):
+    """Of the mean and the sum: a power of two rounds nothing, another number once more, and the upstream numbers of a sum
+    of losses are each their own."""
+    h, w, b, t, _ = _inputs(300, 72, 515, dtype)
+    wrt = [x.requires_grad_() for x in (h, w, b.to(dtype))]
+
+    def grads(factor):
+        loss = E.linear_cross_entropy(wrt[0], wrt[1], t, bias=wrt[2], reduction=reduction)
+        return torch.autograd.grad(loss * factor, wrt)
+
+    one = grads(1.0)
+    for factor in (0.25, -2.0, 3.0, 0.3, 0.0):
+        scale = torch.tensor(factor, device=DEV)
+        for a, c in zip(grads(factor), one):
+            assert torch.equal(a, (c.float() * scale).to(dtype))
+    two = [E.linear_cross_entropy(wrt[0], wrt[1], t, bias=wrt[2], reduction=reduction) for _ in range(2)]
+    got = torch.autograd.grad(two[0] * 3.0 + two[1] * 0.3, wrt)
+    for a, x, y in zip(got, grads(3.0), grads(0.3)):
+        assert torch.equal(a, x + y)
