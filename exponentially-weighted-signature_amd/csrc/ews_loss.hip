@@ -24,8 +24,9 @@
 //   k_grad    dh and dW, sums in float32, reading W, h and dz as they are, with k along their rows. Few tiles are
 //             split over k and joined in order by k_reduce.
 //
-// 8192 rows (a tenth of them ignored), H=2048, V=32000, bfloat16: k_logits 0.96 ms (1.0 PFLOP/s), k_dz 0.20 (4.6 TB/s),
-// dh and dW 0.84 and 0.83 (1.15), all else 0.03. One row by V=100003, H=4096: k_logits 0.15 ms, 5.6 TB/s of W.
+// 8192 rows (a tenth of them ignored), H=2048, V=32000, bfloat16, in a trace of ten calls: k_logits 0.94 ms (1.0
+// PFLOP/s), k_dz 0.20 (4.6 TB/s), dh and dW 0.83 each (1.16), all else 0.035; calls in a row, untraced, take 2.69 ms in
+// all. One row by V=100003, H=4096: k_logits 0.15 ms, 5.6 TB/s of W.
 //
 // The probabilities are kept for kChunkBytes of rows at a time; dW is summed over the chunks in float32. Nothing is
 // added with atomics: the same inputs give the same bits.

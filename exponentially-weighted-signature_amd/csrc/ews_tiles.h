@@ -23,9 +23,9 @@
 // is turned in memory. Piece c of row k lies at c ^ 4 (k % 4): the four rows that 32 lanes read at a time are in
 // different banks.
 //
-// 256 x 256 tiles of eight wavefronts (two a SIMD, 128 KB of LDS) run at 1.15 PFLOP/s in products of 7400 x 2048 x
-// 32000, at 1.1 to 1.2 in ten times larger ones, where the card's power holds its clock down: the library's product of
-// the same sizes, calls in a row, 1.2.
+// 256 x 256 tiles of eight wavefronts (two a SIMD, 128 KB of LDS) run at 1.16 PFLOP/s in products of 7400 x 2048 x
+// 32000 and at 1.10 to 1.22 in ten times larger ones; the library's products of the same sizes, calls in a row, at 0.89
+// (32000 summed) and 1.17 (2048 summed), and at 1.16.
 //
 // Float32 operands come as three bfloat16 planes (x = x0 + x1 + x2 exactly, |x1| <= 2^-8 |x|, |x2| <= 2^-16 |x|) and
 // are multiplied as six products, the smallest first: the three left out are at most 2^-23 of x w, 2^-26 or so at
