@@ -6,10 +6,10 @@
 // writes once. The tensors go by value in a launch's arguments (kMany to a launch): no table is copied to the device
 // and the host waits for nothing. A workgroup takes one chunk of one tensor; squares are added in float64, so no
 // gradient that float32 holds overflows or vanishes, and the chunks' sums are added in a fixed order.
-// A scaling launch walks its chunks backwards: of a set in one launch the data read last by the norm is read first, while
-// it is in the caches. The launches of a larger set go in the norm's order: backwards too they measured the same (196
-// tensors, 1.2 GB: 656 us for 659; 132 tensors, 6.4 GB: 3480 for 3475).
-// In place with c = 1 nothing is read or written again.
+// A scaling launch walks its chunks backwards: of a set in one launch the data read last by the norm is read first,
+// while it is in the caches. The launches of a larger set go in the norm's order: backwards too they measured the same
+// (196 tensors, 1.2 GB: 656 us for 659; 132 tensors, 6.4 GB: 3480 for 3475). In place with c = 1 nothing is read or
+// written again.
 //
 // 3.2 G bfloat16 numbers in 132 tensors: read for the norm in 1.07 ms (6.1 TB/s), scaled in 2.35 (5.5 TB/s).
 #include <hip/hip_runtime.h>
@@ -273,8 +273,8 @@ int ews_clip(int n, const uint64_t* in, const uint64_t* out, const int64_t* coun
 }
 
 // The gradients of ews_loss_train, scaled in place as a clipped set is. They have been rounded to their type already: a
-// factor that is no power of two rounds bfloat16 ones again (half a unit each time). Kept in float32 for this they would
-// take twice the memory and be read and written once more in every step, where a factor of 1 now reads nothing.
+// factor that is no power of two rounds bfloat16 ones again (half a unit each time). Kept in float32 for this they
+// would take twice the memory and be read and written once more in every step, where a factor of 1 now reads nothing.
 int ews_loss_scale(const ews_loss_desc* desc, void* grad_hidden, void* grad_weight, void* grad_bias,
                    const float* factor, ews_stream_t stream) {
   if (!desc || !factor) return EWS_ERR_NULL;

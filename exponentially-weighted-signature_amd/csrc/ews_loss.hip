@@ -895,8 +895,8 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
 }
 
 // bfloat16 weights whose rows start at multiples of 16 bytes and fill whole k blocks are read where they are, and
-// float32 weights for few rows (of a stride that the tiles' offsets hold). Here what the sizes allow; bfloat16's address
-// has to fit too.
+// float32 weights for few rows (of a stride that the tiles' offsets hold). Here what the sizes allow; bfloat16's
+// address has to fit too.
 bool may_read_direct(const ews_loss_desc* s) {
   if (s->weight_stride > 1 << 22) return false;
   if (s->dtype == EWS_DTYPE_F32) {

@@ -173,8 +173,8 @@ __device__ __forceinline__ void product32_once(const Operand32& P, const Operand
   arrive<0>();
 }
 
-// As product() of ews_tiles.h; k blocks are of 32. A tile with a NaN is formed once more, with care: infinities cost such
-// tiles twice the time and the others nothing (told apart number by number they cost all calls 3 to 10%).
+// As product() of ews_tiles.h; k blocks are of 32. A tile with a NaN is formed once more, with care: infinities cost
+// such tiles twice the time and the others nothing (told apart number by number they cost all calls 3 to 10%).
 template <class T, bool TURNED>
 __device__ __forceinline__ void product32(const Operand32& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
                                           char* lds, f32x16 (&acc)[T::TI][T::TJ]) {

@@ -398,7 +398,8 @@ class StackedEWS(nn.Module):
         return self._cosine_logits(head, h) if self.cosine_head_tau is not None else head(h)
 
     def _encode(self, X):
-        """The encoder's rows. A plain Embedding's by ``embedding_lookup``; anything else is called as the module it is."""
+        """The encoder's rows. A plain Embedding's by ``embedding_lookup``; anything else is called as the module it
+        is."""
         e = self.embedding
         if not self.tokens:
             return e(X)
@@ -422,9 +423,9 @@ class StackedEWS(nn.Module):
         objective, e.g. experiments/fl/train.py:754-761), without the logits in memory (``linear_cross_entropy``) and
         with the embedding's gradient by sorted tokens (``embedding_lookup``): the forward's values are those of
         ``forward`` and a cross entropy of its result. An embedding or a head that has hooks or a forward of its own is
-        called as a module, and its rows or logits are then in memory as ``forward``'s are. X, t, mask and raw_driver as ``forward``'s, with a batch;
-        targets (B, L) for "seq2seq" (positions off the mask count as ignored), (B,) for "mean_pool"; for several heads
-        a tuple of them, whose losses are added."""
+        called as a module, and its rows or logits are then in memory as ``forward``'s are. X, t, mask and raw_driver as
+        ``forward``'s, with a batch; targets (B, L) for "seq2seq" (positions off the mask count as ignored), (B,) for
+        "mean_pool"; for several heads a tuple of them, whose losses are added."""
         if X.dim() != (2 if self.tokens else 3):
             raise ValueError(f"X must carry a batch, got shape {tuple(X.shape)}")
         if mask is not None and mask.dim() == 1:

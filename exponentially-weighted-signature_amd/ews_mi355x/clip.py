@@ -48,8 +48,8 @@ def _check(tensors):
 
 
 def _norm_and_scale(tensors, outs, max_norm):
-    """The norm of tensors; where outs is not None, outs = the clipped tensors (outs is tensors: in place, memory that is
-    named twice counting once)."""
+    """The norm of tensors; where outs is not None, outs = the clipped tensors (outs is tensors: in place, memory that
+    is named twice counting once)."""
     lib = nat.load()
     dev = tensors[0].device
     src = dst = tensors
@@ -105,8 +105,8 @@ def global_grad_norm(tensors):
 @torch.no_grad()
 def clip_grads(grads, max_norm, out=None):
     """(norm, clipped): ``grads`` times ``min(1, max_norm / (norm + 1e-6))``, written to the tensors of ``out`` (same
-    shapes and types; a tensor of grads itself: in place; otherwise without overlap, and no two of the same memory) or to
-    new ones."""
+    shapes and types; a tensor of grads itself: in place; otherwise without overlap, and no two of the same memory) or
+    to new ones."""
     grads = list(grads)
     max_norm = _max_norm(max_norm)
     if not grads:
@@ -130,8 +130,8 @@ def clip_grads(grads, max_norm, out=None):
 def clip_grad_norm_(parameters, max_norm):
     """Scales the gradients of ``parameters`` (an iterable, or one) in place by ``min(1, max_norm / (norm + 1e-6))`` and
     returns their norm, a float32 number on the device; the host does not wait. Parameters without a gradient are left
-    out; one that is named twice, or whose gradient is another's memory, counts once. A norm that is not finite scales by
-    0 (infinite) or NaN, as the formula does."""
+    out; one that is named twice, or whose gradient is another's memory, counts once. A norm that is not finite scales
+    by 0 (infinite) or NaN, as the formula does."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     grads = list(dict.fromkeys(p.grad for p in parameters if p.grad is not None))
     max_norm = _max_norm(max_norm)

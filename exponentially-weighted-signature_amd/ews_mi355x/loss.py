@@ -71,8 +71,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
     """The mean and the sum have one upstream number, so their forward computes the gradients with the loss in one pass
     over the rows and the first backward scales them: for an upstream that is no power of two a bfloat16 gradient is
     rounded a second time (float32 until then would be twice the memory, and a pass over it in every step, also in the
-    ordinary one whose upstream is 1 and for which nothing is read). The rows' own losses keep the probabilities for the first
-    backward, where they fit the scratch (2 GiB). A second backward of the same graph, and the rows' own losses of
+    ordinary one whose upstream is 1 and for which nothing is read). The rows' own losses keep the probabilities for the
+    first backward, where they fit the scratch (2 GiB). A second backward of the same graph, and the rows' own losses of
     more, compute the probabilities once more."""
 
     @staticmethod
@@ -119,8 +119,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
 
 def logits_cross_entropy(logits, targets, ignore_index, reduction):
-    """``linear_cross_entropy`` of logits (..., V) that are in memory, in torch operations: for a head that is more than a
-    linear map. Ignored rows and targets outside the vocabulary are answered alike."""
+    """``linear_cross_entropy`` of logits (..., V) that are in memory, in torch operations: for a head that is more than
+    a linear map. Ignored rows and targets outside the vocabulary are answered alike."""
     if reduction not in nat.LOSS_REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(nat.LOSS_REDUCTIONS)}, got {reduction!r}")
     if targets.shape != logits.shape[:-1]:
@@ -146,14 +146,14 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     int64 or int32, all on the HIP device. ``reduction``: "mean" over the rows that are not ignored (0 where all are),
     "sum", or "none" for every row's own loss, (...). Differentiable in hidden, weight and bias (reverse mode).
 
-    Where a gradient is required the mean and the sum form it with the loss, three products for one: a validation loss is
-    best taken under ``torch.no_grad``. bfloat16 gradients are rounded once where the upstream number of the mean or the
-    sum is a power of two (1 as a rule), else a second time after the multiplication by it.
+    Where a gradient is required the mean and the sum form it with the loss, three products for one: a validation loss
+    is best taken under ``torch.no_grad``. bfloat16 gradients are rounded once where the upstream number of the mean or
+    the sum is a power of two (1 as a rule), else a second time after the multiplication by it.
 
     Rows whose target is ``ignore_index`` have loss and gradient zero, whatever they hold, and cost nothing. A target
     outside [0, V) that is not ``ignore_index`` gives NaN. A bias of -inf takes a token out of the vocabulary, and so
-    does a logit of -inf from an infinite weight; a row with a logit of +inf or NaN has a loss of NaN. A row whose target
-    has been taken out has an infinite loss, and its gradients may be NaN."""
+    does a logit of -inf from an infinite weight; a row with a logit of +inf or NaN has a loss of NaN. A row whose
+    target has been taken out has an infinite loss, and its gradients may be NaN."""
     if reduction not in nat.LOSS_REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(nat.LOSS_REDUCTIONS)}, got {reduction!r}")
     if weight.dim() != 2 or weight.numel() == 0:

@@ -644,9 +644,9 @@ size_t ews_loss_workspace_bytes(const ews_loss_desc* desc, int train);
 size_t ews_loss_workspace_bytes_for(const ews_loss_desc* desc, const void* weight, int train);
 
 /* What a call with these sizes and this weight's address runs, for tests and profiles: of product 0 (the logits), 1
- * (grad_hidden) or 2 (grad_weight; the last two of training calls) tile[0] x tile[1] = the results of one workgroup (along
- * the vocabulary or the hidden width, and along the rows or, for 2, the vocabulary), tile[2] = the splits of its sum,
- * tile[3] = the parts that the call's rows are done in. */
+ * (grad_hidden) or 2 (grad_weight; the last two of training calls) tile[0] x tile[1] = the results of one workgroup
+ * (along the vocabulary or the hidden width, and along the rows or, for 2, the vocabulary), tile[2] = the splits of its
+ * sum, tile[3] = the parts that the call's rows are done in. */
 int ews_loss_tile(const ews_loss_desc* desc, const void* weight, int train, int product, int32_t* tile);
 
 /* z = hidden weight^T + bias (bias may be NULL; entries of -inf take a token out of the vocabulary),

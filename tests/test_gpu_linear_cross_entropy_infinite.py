@@ -3,8 +3,8 @@ infinite factor gives an infinity of the products' sign, or NaN beside a zero or
 of -inf takes its token out of the row's softmax; one of +inf, or NaN, makes the row's loss NaN.
 
 The oracle is the formula in float64 on the CPU. Where its value is finite the bounds are those of finite inputs, with S
-the sum of the finite products' magnitudes: a logit (H + 8) 2^-24 S (plus bfloat16's half unit where a gradient is rounded
-to it), a loss twice that and 8 * 2^-24 (1 + |z|)."""
+the sum of the finite products' magnitudes: a logit (H + 8) 2^-24 S (plus bfloat16's half unit where a gradient is
+rounded to it), a loss twice that and 8 * 2^-24 (1 + |z|)."""
 
 import math
 
@@ -57,10 +57,10 @@ def _run(h, w, t, reduction="none"):
         return E.linear_cross_entropy(h.to(DEV), w.to(DEV), t.to(DEV), reduction=reduction)
 
 
-# float32 W as it is (one, few and more rows; rows of W at multiples of 16 bytes or not; stages that H does not fill) and
-# in planes (128 x 128 and 256 x 256 tiles); bfloat16 as it is and packed
-SHAPES = [(1, 64, 300), (20, 72, 300), (20, 77, 301), (100, 96, 1000), (100, 61, 1001), (700, 64, 6500), (520, 333, 16500),
-          (300, 77, 500)]
+# float32 W as it is (one, few and more rows; rows of W at multiples of 16 bytes or not; stages that H does not fill)
+# and in planes (128 x 128 and 256 x 256 tiles); bfloat16 as it is and packed
+SHAPES = [(1, 64, 300), (20, 72, 300), (20, 77, 301), (100, 96, 1000), (100, 61, 1001), (700, 64, 6500),
+          (520, 333, 16500), (300, 77, 500)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

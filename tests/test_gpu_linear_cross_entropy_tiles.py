@@ -1,12 +1,12 @@
 """Linear cross entropy (csrc/ews_loss.hip) on each of its tiles, in chunks, and through its entry points' two halves,
 against the formula in float64.
 
-Bounds, number by number, with u = 2^-24, half(T) = 2^-24 or 2^-8 (the relative error of one rounding to T) and S = sum_k
-|h_k w_k|: a logit is off by at most (H + 8) u S, a loss by twice that and 8 u (1 + |z|) and, for the slabs joined one
-after another, 200 u. A probability is off by the factor e = 2 max (H + 8) u S + 16 u + 2 u max |z|, and where it is kept
-as a 16-bit logarithm in steps of 1/512 octave by 2^-10.5 more. dz carries that and its own rounding: half(bfloat16) |dz|
-in one bfloat16, half(bfloat16)^2 in two. A gradient is off by dz's error times the other operand's magnitude, its float32
-sum's (K + 8) u of the summed magnitudes, half of its own type and 2 u of the mean's factor."""
+Bounds, number by number, with u = 2^-24, half(T) = 2^-24 or 2^-8 (the relative error of one rounding to T) and S =
+sum_k |h_k w_k|: a logit is off by at most (H + 8) u S, a loss by twice that and 8 u (1 + |z|) and, for the slabs joined
+one after another, 200 u. A probability is off by the factor e = 2 max (H + 8) u S + 16 u + 2 u max |z|, and where it is
+kept as a 16-bit logarithm in steps of 1/512 octave by 2^-10.5 more. dz carries that and its own rounding:
+half(bfloat16) |dz| in one bfloat16, half(bfloat16)^2 in two. A gradient is off by dz's error times the other operand's
+magnitude, its float32 sum's (K + 8) u of the summed magnitudes, half of its own type and 2 u of the mean's factor."""
 
 import ctypes
 import math
@@ -133,7 +133,8 @@ def test_chunks(dtype, N, reduction):
     print(f"chunks {dtype} N={N} {reduction}", flush=True)
     h, w, b, t, up = _inputs(N, H, V, dtype)
     desc = nat.LossDesc(hidden_stride=H, weight_stride=H, ignore_index=-100, rows=N, hidden=H, vocab=V,
-                        dtype=0 if dtype == torch.float32 else 1, bias_dtype=0, reduction=nat.LOSS_REDUCTIONS[reduction])
+                        dtype=0 if dtype == torch.float32 else 1, bias_dtype=0,
+                        reduction=nat.LOSS_REDUCTIONS[reduction])
     tile = (ctypes.c_int32 * 4)()
     assert nat.load().ews_loss_tile(desc, w.data_ptr(), 1, 0, tile) == 0 and tile[3] > 1
     assert not nat.load().ews_loss_keeps(desc)
@@ -156,7 +157,8 @@ def test_the_two_halves_give_the_whole(reduction, N, dtype):
     h, w, b, t, up = _inputs(N, H, V, dtype)
     lib = nat.load()
     desc = nat.LossDesc(hidden_stride=H, weight_stride=H, ignore_index=-100, rows=N, hidden=H, vocab=V,
-                        dtype=0 if dtype == torch.float32 else 1, bias_dtype=0, reduction=nat.LOSS_REDUCTIONS[reduction])
+                        dtype=0 if dtype == torch.float32 else 1, bias_dtype=0,
+                        reduction=nat.LOSS_REDUCTIONS[reduction])
     assert lib.ews_loss_keeps(desc) == 1
     size = lib.ews_loss_workspace_bytes_for(desc, w.data_ptr(), 1)
     st = torch.cuda.current_stream().cuda_stream
@@ -212,8 +214,8 @@ def test_dz_number_by_number(reduction, N, V):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("reduction", ["mean", "sum"])
 def test_an_upstream_number_multiplies_the_rounded_gradients(reduction, dtype):
-    """Of the mean and the sum: a power of two rounds nothing, another number once more, and the upstream numbers of a sum
-    of losses are each their own."""
+    """Of the mean and the sum: a power of two rounds nothing, another number once more, and the upstream numbers of a
+    sum of losses are each their own."""
     h, w, b, t, _ = _inputs(300, 72, 515, dtype)
     wrt = [x.requires_grad_() for x in (h, w, b.to(dtype))]
 

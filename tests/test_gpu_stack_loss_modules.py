@@ -2,9 +2,9 @@
 normalisation), hooks that change or watch the result, modules with options of their own. The loss has to be a cross
 entropy of what ``forward`` returns.
 
-Both sides run the same float32 blocks; the head's two forms differ by a few 2^-24 of a logit of a few units (1e-5 of the
-loss allowed), and the blocks' backward may amplify a cotangent's last bits a thousandfold: 8 * 2^-24 * 1000 = 5e-4 of a
-gradient's largest number, 1e-3 allowed."""
+Both sides run the same float32 blocks; the head's two forms differ by a few 2^-24 of a logit of a few units (1e-5 of
+the loss allowed), and the blocks' backward may amplify a cotangent's last bits a thousandfold: 8 * 2^-24 * 1000 = 5e-4
+of a gradient's largest number, 1e-3 allowed."""
 
 import pytest
 import torch

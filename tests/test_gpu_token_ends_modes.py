@@ -1,5 +1,5 @@
-"""How the token model's ends stand with torch's other ways to differentiate: a derivative that is not formed is refused,
-never dropped."""
+"""How the token model's ends stand with torch's other ways to differentiate: a derivative that is not formed is
+refused, never dropped."""
 
 import pytest
 import torch

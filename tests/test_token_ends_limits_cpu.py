@@ -29,8 +29,8 @@ def test_lookup_and_gradient_take_the_same_sizes(vocab, width, taken, dtype, cou
 
 
 def _scratch(rows, train, hidden=512, vocab=100003, dtype=0, reduction=1):
-    d = nat.LossDesc(hidden_stride=hidden, weight_stride=hidden, ignore_index=-100, rows=rows, hidden=hidden, vocab=vocab,
-                     dtype=dtype, bias_dtype=0, reduction=reduction)
+    d = nat.LossDesc(hidden_stride=hidden, weight_stride=hidden, ignore_index=-100, rows=rows, hidden=hidden,
+                     vocab=vocab, dtype=dtype, bias_dtype=0, reduction=reduction)
     return nat.load().ews_loss_workspace_bytes(d, train)
 
 
@@ -43,16 +43,18 @@ def test_float32_scores_keep_256_mib_of_slabs(rows, hidden):
 
 @pytest.mark.parametrize("rows,train,most", [(1, 0, 2 << 20), (512, 0, 140 << 20), (64, 1, 180 << 20)])
 def test_float32_weight_read_as_it_is_has_no_copy(rows, train, most):
-    """Few rows: W (1.6 GB here, its planes 2.5) is not copied. A row has a slab's eight bytes for 32 tokens, in training
-    ten bytes a token, and the results of up to 128 splits of dh."""
+    """Few rows: W (1.6 GB here, its planes 2.5) is not copied. A row has a slab's eight bytes for 32 tokens, in
+    training ten bytes a token, and the results of up to 128 splits of dh."""
     splits = 128 * rows * 4096 * 4 if train else 0
     assert _scratch(rows, train, 4096) <= most + splits
 
 
 @pytest.mark.parametrize("train", [0, 1])
-@pytest.mark.parametrize("rows,hidden,dtype", [(1, 4096, 1), (1000, 4096, 1), (1, 4000, 1), (3, 4096, 0), (7000, 512, 0)])
+@pytest.mark.parametrize("rows,hidden,dtype", [(1, 4096, 1), (1000, 4096, 1), (1, 4000, 1), (3, 4096, 0),
+                                               (7000, 512, 0)])
 def test_scratch_of_a_weight_at_an_address(rows, hidden, dtype, train):
-    """The query without the address holds any weight's; with it, a bfloat16 weight that is read where it is has no copy."""
+    """The query without the address holds any weight's; with it, a bfloat16 weight that is read where it is has no
+    copy."""
     lib = nat.load()
     d = nat.LossDesc(hidden_stride=hidden, weight_stride=hidden, ignore_index=-100, rows=rows, hidden=hidden,
                      vocab=100003, dtype=dtype, bias_dtype=0, reduction=0)
