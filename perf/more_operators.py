@@ -328,7 +328,7 @@ def _plain_scan(s):
     del total, b
     if not s["train"]:
         return h.to(dt), h[:, -1].clone()
-    up = s["upstream"].float()
+    up = s["upstream"].float().clone()  # float32 too: the state keeps its own
     up[:, -1] += s["upstream_last"]
     after = torch.cat([a[:, 1:], torch.zeros_like(a[:, :1])], 1)
     _, lam = _doubling(after.flip(1), up.flip(1))
