@@ -104,6 +104,10 @@ EXPORTED = (
     "ews_clip_workspace_bytes",
     "ews_clip",
     "ews_loss_scale",
+    "ews_gated_scan_residual_bytes",
+    "ews_gated_scan_workspace_bytes",
+    "ews_gated_scan_forward",
+    "ews_gated_scan_backward",
 )
 
 JORDAN_KINDS = {"real": 0, "complex": 1}
@@ -116,6 +120,8 @@ LIFT_FULL = 1
 LIFT_PRESERVE = 2
 
 LOSS_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+GATED_SCAN_FORMS = {"convex": 0, "linear": 1}
 
 GRADED_VARIANTS = {"live_rms": 0, "static_gain": 1, "dilation": 2}
 
@@ -265,6 +271,21 @@ class EmbedDesc(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("token_bytes", ctypes.c_int32),
         ("scale", ctypes.c_float),
+    ]
+
+
+class GatedScanDesc(ctypes.Structure):
+    _fields_ = [
+        ("x_batch", ctypes.c_int64),
+        ("x_step", ctypes.c_int64),
+        ("gate_batch", ctypes.c_int64),
+        ("gate_step", ctypes.c_int64),
+        ("mask_batch", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("length", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("form", ctypes.c_int32),
     ]
 
 
@@ -460,6 +481,15 @@ def load():
     lib.ews_clip.restype = i32
     lib.ews_loss_scale.argtypes = [lsp, vp, vp, vp, vp, vp]
     lib.ews_loss_scale.restype = i32
+    gsp = ctypes.POINTER(GatedScanDesc)
+    lib.ews_gated_scan_residual_bytes.argtypes = [gsp]
+    lib.ews_gated_scan_residual_bytes.restype = sz
+    lib.ews_gated_scan_workspace_bytes.argtypes = [gsp]
+    lib.ews_gated_scan_workspace_bytes.restype = sz
+    lib.ews_gated_scan_forward.argtypes = [gsp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_gated_scan_forward.restype = i32
+    lib.ews_gated_scan_backward.argtypes = [gsp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_gated_scan_backward.restype = i32
     _lib = lib
     return lib
 

@@ -683,6 +683,40 @@ size_t ews_clip_workspace_bytes(int n, const int64_t* counts);
 int ews_clip(int n, const uint64_t* in, const uint64_t* out, const int64_t* counts, const int32_t* dtypes,
              float max_norm, int32_t scale, float* result, void* workspace, ews_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Inside a token model's blocks.
+ * --------------------------------------------------------------------------------------------------------- */
+#define EWS_GATED_SCAN_CONVEX 0 /* a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t */
+#define EWS_GATED_SCAN_LINEAR 1 /* a = gate,          h_t = a_t h_{t-1} + x_t */
+
+typedef struct ews_gated_scan_desc {
+  int64_t x_batch, x_step;       /* elements between sequences and between steps of x; channels are neighbours */
+  int64_t gate_batch, gate_step; /* of gate */
+  int64_t mask_batch;            /* between sequences of mask, whose steps are neighbours */
+  int32_t batch;                 /* B: 1..2^20 */
+  int32_t length;                /* L: 1..2^28 */
+  int32_t dim;                   /* D: 1..2^20 */
+  int32_t dtype;                 /* EWS_DTYPE_*: of x, gate, out and their gradients */
+  int32_t form;                  /* EWS_GATED_SCAN_* */
+} ews_gated_scan_desc;
+
+/* The residual that a forward leaves for its backward, and the scratch of either (0: may be NULL). */
+size_t ews_gated_scan_residual_bytes(const ews_gated_scan_desc* desc);
+size_t ews_gated_scan_workspace_bytes(const ews_gated_scan_desc* desc);
+
+/* out (B, L, D) contiguous and last (B, D) float32, the state after the last step. state (B, D) float32 may be NULL
+ * (zero) or last itself; mask (B, L), one byte a step, may be NULL: a step whose byte is 0 leaves the state as it is.
+ * residual may be NULL where no backward follows. */
+int ews_gated_scan_forward(const ews_gated_scan_desc* desc, const void* x, const void* gate, const uint8_t* mask,
+                           const float* state, void* out, float* last, void* residual, void* workspace,
+                           ews_stream_t stream);
+
+/* The gradients (contiguous; grad_state may be NULL) for those of out (contiguous) and last, either of which may be
+ * NULL (zero). grad_x and grad_gate are zero off the mask. */
+int ews_gated_scan_backward(const ews_gated_scan_desc* desc, const void* x, const void* gate, const uint8_t* mask,
+                            const void* residual, const void* grad_out, const float* grad_last, void* grad_x,
+                            void* grad_gate, float* grad_state, void* workspace, ews_stream_t stream);
+
 /* Human-readable text of a return code. */
 const char* ews_error_string(int code);
 
