@@ -65,6 +65,29 @@ struct Rows {
   float* scale;   // [0]: 1 / max(kept, 1) for the mean, 1 for the sum
 };
 
+// Distillation: a row's target is the distribution of a teacher's K entries (token v_k, probability p_k), at a
+// temperature T.
+//
+//   q[n, v] = softmax_v (z[n, v] / T)        l[n] = T^2 sum_k p_k (log p_k - log q[n, v_k])
+//   dz[n, v] = T g_n (q[n, v] - sum of the p_k with v_k = v)
+//
+// Everything above stays as it is but for what the targets need. k_teacher sorts a row's entries by token and says where
+// those of every 128 tokens begin, so that a tile finds its own at once (16384 rows of 64 entries each: one entry in four
+// tiles' rows). k_logits puts its block of z through LDS where one of its rows has an entry there, and hands out the
+// entries' own float32 logits; k_dz takes them in place of the kept probabilities, as it does a target's.
+constexpr int kBucket = 128;
+struct Top {
+  int count;              // K
+  const int* token;       // (N, K) sorted; INT_MAX where there is none
+  const float* p;         // (N, K) their probabilities
+  const float* entropy;   // (N) sum_k p_k log p_k
+  const uint16_t* first;  // (N, buckets + 1) the first entry at or past every 128th token
+  int buckets;
+  float* z;               // (N, K) their logits
+  float scale;            // log2(e) / T: of logits
+  float temperature;
+};
+
 // Logits are kept in units of a factor of two: z log2 e.
 struct Stats {
   float2* slab;   // (slabs, chunk rows) maximum and sum of 2^(z - maximum) of one wavefront's slab
@@ -157,6 +180,7 @@ struct PrepareArgs {
   const void* bias;        // or null
   int bias_bf16;
   float* bias_out;         // (padded)
+  float scale;             // of logits: log2(e), over the temperature
   void* grad_hidden;       // or null: the ignored rows' zeros
   int each, kept_blocks;   // rows that a workgroup lists, and those workgroups
   int bias_blocks, ignored_blocks;
@@ -229,7 +253,7 @@ __device__ __forceinline__ void scale_bias(const PrepareArgs& a, int v) {
   float b = -__builtin_inff();
   if (v < a.vocab) {
     const float x = !a.bias ? 0.0f : a.bias_bf16 ? widen(((const bf16*)a.bias)[v]) : ((const float*)a.bias)[v];
-    b = x * kLog2e;
+    b = x * a.scale;
     if (__builtin_isinf(b) && !__builtin_isinf(x)) b = copysignf(3.402823466e+38f, x);
   }
   a.bias_out[v] = b;
@@ -269,6 +293,7 @@ struct LogitArgs {
   Stats st;
   void* prob;             // exp(z - m) (chunk, ldp): a 16-bit logarithm, or float32 where there are three planes
   int64_t ldp;
+  Top top;
 };
 
 // A product of one stage needs no second half: more workgroups share a CU.
@@ -281,8 +306,8 @@ __host__ __device__ constexpr int lds_bytes(int kblocks) {
 }
 
 // PAIRS: 1, kPairs for planes, or 0 for float32 W. KEEP: 0 the loss alone, 1 also 16-bit logarithms, 2 also float32
-// probabilities.
-template <class T, int PAIRS, int KEEP>
+// probabilities. TOP: distillation.
+template <class T, int PAIRS, int KEEP, bool TOP>
 __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_logits(LogitArgs a) {
   extern __shared__ char lds[];
   int it, jt;
@@ -293,11 +318,22 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_logits(LogitArgs a) 
   // the epilogue's operands, where it need not wait for them
   float* tile_bias = reinterpret_cast<float*>(lds + lds_bytes<T, PAIRS>(a.kblocks));
   int* tile_target = reinterpret_cast<int*>(tile_bias + T::I);
+  // TOP: a row's place, and its entries of the tile's buckets
+  constexpr int kBuckets = T::I / kBucket;
+  int* tile_first = tile_target + T::J;
   for (int t = threadIdx.x; t < T::I + T::J; t += T::kThreads) {
-    if (t < T::I)
+    const int j = t - T::I;
+    if (t < T::I) {
       tile_bias[t] = a.bias[i0 + t];
-    else
-      tile_target[t - T::I] = j0 + t - T::I < live ? a.rows.target[a.c0 + j0 + t - T::I] : -1;
+    } else if (!TOP) {
+      tile_target[j] = j0 + j < live ? a.rows.target[a.c0 + j0 + j] : -1;
+    } else {
+      const int row = j0 + j < live ? a.rows.map[a.c0 + j0 + j] : -1;
+      tile_target[j] = row;
+      const uint16_t* first = a.top.first + (int64_t)row * (a.top.buckets + 1) + i0 / kBucket;
+#pragma unroll
+      for (int k = 0; k <= kBuckets; ++k) tile_first[k * T::J + j] = row < 0 ? 0 : first[k];
+    }
   }
   f32x16 acc[T::TI][T::TJ];
   if constexpr (PAIRS == 0)
@@ -321,16 +357,39 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_logits(LogitArgs a) 
         const f32x4 add = *reinterpret_cast<const f32x4*>(bias + t * 32 + g * 8);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float z = fmaf(acc[t][b][4 * g + q], kLog2e, add[q]);
+          const float z = fmaf(acc[t][b][4 * g + q], TOP ? a.top.scale : kLog2e, add[q]);
           acc[t][b][4 * g + q] = z;
           m = fmaxf(m, z);
         }
       }
     m = fmaxf(m, __shfl_xor(m, 32));
+    const int own = tile_target[(wj * T::TJ + b) * 32 + r32];
+    if (TOP) {
+      const int jt = (wj * T::TJ + b) * 32 + r32;
+      const int e0 = tile_first[wi * T::kSlab / kBucket * T::J + jt];
+      const int e1 = tile_first[((wi + 1) * T::kSlab - 1 + kBucket) / kBucket * T::J + jt];
+      if (__any(e0 < e1)) {
+        float* stage = reinterpret_cast<float*>(lds) + wave * 32 * T::kRowWords;
+#pragma unroll
+        for (int t = 0; t < T::TI; ++t)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(stage + r32 * T::kRowWords + t * 32 + g * 8 + half * 4) =
+                f32x4{acc[t][b][4 * g], acc[t][b][4 * g + 1], acc[t][b][4 * g + 2], acc[t][b][4 * g + 3]};
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        for (int e = e0 + half; e < e1; e += 2) {
+          const int i = a.top.token[(int64_t)own * a.top.count + e] - ibase;
+          if (i >= 0 && i < T::kSlab) a.top.z[(int64_t)own * a.top.count + e] = stage[r32 * T::kRowWords + i];
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
     // the target's logit, from the one lane that holds it
-    const int want = tile_target[(wj * T::TJ + b) * 32 + r32] - ibase;
+    const int want = TOP ? -1 : own - ibase;
     const bool mine = want >= 0 && want < T::kSlab && ((want >> 2) & 1) == half;
-    if (__any(mine)) {
+    if (!TOP && __any(mine)) {
       float zt = 0.0f;
 #pragma unroll
       for (int t = 0; t < T::TI; ++t)
@@ -375,8 +434,9 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   m = top;
 }
 
-// ROWS rows a workgroup, the other threads along the slabs; joined as a tree.
-template <int ROWS>
+// ROWS rows a workgroup, the other threads along the slabs; joined as a tree. TOP: what a row's entries have in common,
+// log sum exp (z - M), in the place of its loss; k_top_loss does the rest.
+template <int ROWS, bool TOP>
 __global__ __launch_bounds__(1024) void k_join(Stats st, Rows rows, int slabs, int c0, int chunk, float* loss_rows) {
   constexpr int kGroups = 1024 / ROWS;
   __shared__ float ms[1024], ss[1024];
@@ -404,7 +464,34 @@ __global__ __launch_bounds__(1024) void k_join(Stats st, Rows rows, int slabs, i
   const int row = c0 + j;
   st.top[row] = m;
   st.inv[row] = 1.0f / s;
+  if (TOP) {
+    st.loss[row] = logf(s);
+    return;
+  }
   const float l = rows.target[row] < 0 ? __builtin_nanf("") : logf(s) + (m - st.zt[row]) * kLn2;
+  st.loss[row] = l;
+  if (loss_rows) loss_rows[rows.map[row]] = l;
+}
+
+// A wavefront a row: l = T^2 (sum_k p_k log p_k + sum_k p_k (log sum exp (z - M) + M - z_k)). Entries of probability 0
+// count nothing, also where z_k is -inf.
+__global__ __launch_bounds__(256) void k_top_loss(Stats st, Rows rows, Top top, int c0, int chunk, float* loss_rows) {
+  const int live = rows.kept[0] - c0 < chunk ? rows.kept[0] - c0 : chunk;
+  const int j = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (j >= live) return;
+  const int row = c0 + j;
+  const int64_t from = (int64_t)rows.map[row] * top.count;
+  const float m = st.top[row], lse = st.loss[row];
+  float s = 0.0f;
+  for (int e = threadIdx.x & 63; e < top.count; e += 64) {
+    const float p = top.p[from + e];
+    if (p != 0.0f) s += p * (lse + (m - top.z[from + e]) * kLn2);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  if (threadIdx.x & 63) return;
+  const float t2 = top.temperature * top.temperature;
+  const float l = rows.target[row] < 0 ? __builtin_nanf("") : t2 * (top.entropy[rows.map[row]] + s);
   st.loss[row] = l;
   if (loss_rows) loss_rows[rows.map[row]] = l;
 }
@@ -442,11 +529,12 @@ struct DzArgs {
   int each;               // rows a workgroup goes over, one wavefront a row, 512 columns wide
   int lanes;              // narrow: so many lanes a row, 64 / lanes rows a wavefront; a power of two
   float* loss;            // or null: the call's loss, by one further workgroup
+  Top top;
 };
 
 // NP planes: 3 of float32 inputs, 1 or (few rows) 2 of bfloat16 ones. NARROW: a row fills half a wavefront at most, so
-// several rows share one (131072 rows by V=8: 94 -> 38 us).
-template <int NP, bool NARROW>
+// several rows share one (131072 rows by V=8: 94 -> 38 us). TOP: distillation.
+template <int NP, bool NARROW, bool TOP>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   if (blockIdx.x * 512 >= a.ld) {
     if (blockIdx.y == 0) total_loss(a.st, a.rows, a.loss);
@@ -472,7 +560,8 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
       const int row = a.c0 + j;
       const int t = a.rows.target[row];
       const float top = a.st.top[row], inv = a.st.inv[row];
-      const float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
+      float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
+      if (TOP) g *= a.top.temperature;
       const float m = a.st.slab[(int64_t)slab * a.chunk + j].x;
       const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f(m - top) * inv * g;
       if (NP != 3) {
@@ -489,7 +578,23 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? lo.get(q) : hi.get(q - 4)) * f;
       }
-      if (t >= v && t < v + 8) {
+      if (TOP && t >= 0) {
+        const int64_t at = a.rows.map[row];
+        const uint16_t* first = a.top.first + at * (a.top.buckets + 1) + v / kBucket;
+        int before = -1;
+        for (int e = first[0]; e < first[1]; ++e) {
+          const int token = a.top.token[at * a.top.count + e];
+          if (token >= v && token < v + 8) {
+            // the first entry of a token takes its probability's place, a further one adds to it
+            const float p = a.top.p[at * a.top.count + e];
+            const float own = (__builtin_amdgcn_exp2f(a.top.z[at * a.top.count + e] - top) * inv - p) * g;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] = token == v + q ? (token == before ? x[q] - p * g : own) : x[q];
+          }
+          before = token;
+        }
+      }
+      if (!TOP && t >= v && t < v + 8) {
         const float own = (__builtin_amdgcn_exp2f(a.st.zt[row] - top) * inv - 1.0f) * g;
 #pragma unroll
         for (int q = 0; q < 8; ++q) x[q] = t == v + q ? own : x[q];
@@ -560,6 +665,117 @@ __global__ __launch_bounds__(1024) void k_dbias(const float* part, int parts, in
     out[v] = narrow<T>(s);
   else
     sum[v] = s;
+}
+
+// ------------------------------------------------------------------------------------------------------- the teacher
+struct TeacherArgs {
+  const void* index;
+  const void* logit;
+  int64_t index_stride, logit_stride;
+  int n, count, vocab, buckets;
+  int ordered;             // count rounded up to a power of two
+  int index_bytes, logit_bf16;
+  float scale;             // log2(e) / T
+  int64_t* target;         // (n) 0; -1 where a token is outside the vocabulary, kNone where there is no entry
+  int* token;
+  float* p;
+  float* entropy;
+  uint16_t* first;
+};
+constexpr int64_t kNone = -100;
+constexpr int kMostTop = 1024;
+
+// A wavefront a row: its entries that count (a token that is not negative, a logit that is not -inf) sorted by token, by
+// a bitonic network in LDS, ties in the order given, with the teacher's softmax over them.
+__global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
+  extern __shared__ char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.x * 4 + wave;
+  if (row >= a.n) return;  // a wavefront uses no other's part of LDS
+  uint64_t* key = reinterpret_cast<uint64_t*>(lds) + wave * a.ordered;
+  auto logit = [&](int k) {
+    const int64_t at = row * a.logit_stride + k;
+    return a.logit_bf16 ? widen(((const bf16*)a.logit)[at]) : ((const float*)a.logit)[at];
+  };
+  float top = -__builtin_inff();
+  bool any = false, bad = false;
+  for (int k = lane; k < a.ordered; k += 64) {
+    uint32_t token = 0x7fffffffu;
+    if (k < a.count) {
+      const int64_t at = row * a.index_stride + k;
+      const int64_t i = a.index_bytes == 8 ? ((const int64_t*)a.index)[at] : ((const int32_t*)a.index)[at];
+      const float t = logit(k);
+      if (i >= 0 && t != -__builtin_inff()) {
+        any = true;
+        bad |= i >= a.vocab;
+        token = i < a.vocab ? (uint32_t)i : 0x7ffffffeu;
+        top = t > top || __builtin_isnan(t) ? t : top;  // once NaN, NaN
+      }
+    }
+    key[k] = (uint64_t)token << 32 | (uint32_t)k;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const float t = __shfl_xor(top, d);
+    top = t > top || __builtin_isnan(t) ? t : top;
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  for (int size = 2; size <= a.ordered; size <<= 1)
+    for (int d = size >> 1; d; d >>= 1) {
+      for (int k = lane; k < a.ordered; k += 64) {
+        const int other = k ^ d;
+        if (other > k) {
+          const uint64_t x = key[k], y = key[other];
+          if ((x > y) == ((k & size) == 0)) {
+            key[k] = y;
+            key[other] = x;
+          }
+        }
+      }
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+    }
+  float sum = 0.0f;
+  for (int e = lane; e < a.count; e += 64) {
+    const uint64_t k = key[e];
+    if ((uint32_t)(k >> 32) != 0x7fffffffu) sum += __builtin_amdgcn_exp2f((logit((uint32_t)k) - top) * a.scale);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  const float log_sum = __builtin_amdgcn_logf(sum);  // base 2
+  float entropy = 0.0f;
+  for (int e = lane; e < a.count; e += 64) {
+    const uint64_t k = key[e];
+    const int token = (int)(k >> 32);
+    float p = 0.0f;
+    if (token != 0x7fffffff) {
+      const float y = (logit((uint32_t)k) - top) * a.scale;
+      p = __builtin_amdgcn_exp2f(y) / sum;
+      if (p != 0.0f) entropy += p * (y - log_sum);
+    }
+    a.token[(int64_t)row * a.count + e] = token;
+    a.p[(int64_t)row * a.count + e] = p;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) entropy += __shfl_xor(entropy, d);
+  for (int b = lane; b <= a.buckets; b += 64) {
+    const uint64_t want = (uint64_t)b * kBucket << 32;
+    int lo = 0, hi = a.count;  // the first entry at or past it
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (key[mid] < want)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    a.first[(int64_t)row * (a.buckets + 1) + b] = (uint16_t)lo;
+  }
+  any = __any(any);
+  bad = __any(bad);
+  if (lane) return;
+  a.entropy[row] = entropy * kLn2;
+  a.target[row] = !any ? kNone : bad ? -1 : 0;
 }
 
 // ------------------------------------------------------------------------------------------------------ the gradients
@@ -770,6 +986,8 @@ struct LPlan {
   bool train, packed, as_is, twice;
   Product logits, dh, dw;
   size_t map, target, meta, zt, top, inv, loss, xp, wp, bias, slab, prob, dz, dbias, dbsum, part, acc;
+  int entries, buckets;    // distillation: K; the vocabulary's buckets
+  size_t flags, token, share, entropy, first;
   size_t total;
 };
 
@@ -818,7 +1036,8 @@ Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split, bool as_i
   return p;
 }
 
-int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
+// entries: the teacher's of a row; 0 where the targets are tokens.
+int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p, int entries = 0) {
   if (!s) return EWS_ERR_NULL;
   if (s->dtype != EWS_DTYPE_F32 && s->dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
   if (s->bias_dtype != EWS_DTYPE_F32 && s->bias_dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
@@ -868,7 +1087,8 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.map = take((size_t)p.N * 4);
   p.target = take((size_t)p.N * 4);
   p.meta = take(8);
-  p.zt = take((size_t)p.N * 4);
+  p.entries = entries;
+  p.zt = take((size_t)p.N * (entries ? entries : 1) * 4);
   p.top = take((size_t)p.N * 4);
   p.inv = take((size_t)p.N * 4);
   p.loss = take((size_t)p.N * 4);
@@ -876,6 +1096,14 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p) {
   p.wp = take(p.packed ? (size_t)(p.V * p.Hp * p.np * 2) : 0);
   p.bias = take((size_t)p.bias_pad * 4);
   p.slab = take((size_t)p.slabs * p.chunk * 8);
+  if (entries) {
+    p.buckets = p.bias_pad / kBucket;
+    p.flags = take((size_t)p.N * 8);
+    p.token = take((size_t)p.N * entries * 4);
+    p.share = take((size_t)p.N * entries * 4);
+    p.entropy = take((size_t)p.N * 4);
+    p.first = take((size_t)p.N * (p.buckets + 1) * 2);
+  }
   if (train) {
     p.prob = take((size_t)(p.chunk * p.Vp) * (p.np == 3 || p.twice ? 4 : 2));
     p.dz = p.np == 3 ? take((size_t)(p.chunk * p.Vp) * 6) : p.prob;
@@ -918,6 +1146,7 @@ struct Call {
   hipStream_t st;
   Rows rows;
   Stats stats;
+  Top top;
 };
 
 #define LOSS_CHECK()                                             \
@@ -937,14 +1166,19 @@ int allow_lds(K kernel, int bytes) {
 // Whether a float32 operand can be copied 16 bytes a lane.
 bool pieces(const Operand32& o) { return (uintptr_t)o.p % 16 == 0 && o.ld % 4 == 0 && o.cols % 4 == 0; }
 
-template <class T, int PAIRS, int KEEP>
-int launch_logits_as(const LogitArgs& a, hipStream_t st) {
-  const int lds = lds_bytes<T, PAIRS>(a.kblocks) + (T::I + T::J) * 4;
-  const int rc = allow_lds(k_logits<T, PAIRS, KEEP>, lds);
+template <class T, int PAIRS, int KEEP, bool TOP>
+int launch_logits_of(const LogitArgs& a, hipStream_t st) {
+  const int lds = lds_bytes<T, PAIRS>(a.kblocks) + (T::I + T::J + (TOP ? (T::I / kBucket + 1) * T::J : 0)) * 4;
+  const int rc = allow_lds(k_logits<T, PAIRS, KEEP, TOP>, lds);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_logits<T, PAIRS, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), lds, st, a);
+  hipLaunchKernelGGL((k_logits<T, PAIRS, KEEP, TOP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), lds, st, a);
   LOSS_CHECK();
   return EWS_OK;
+}
+
+template <class T, int PAIRS, int KEEP>
+int launch_logits_as(const LogitArgs& a, hipStream_t st) {
+  return a.top.count ? launch_logits_of<T, PAIRS, KEEP, true>(a, st) : launch_logits_of<T, PAIRS, KEEP, false>(a, st);
 }
 
 template <int PAIRS, int KEEP>
@@ -1035,6 +1269,7 @@ int begin(Call& c, const void* hidden, const void* weight, const void* bias, con
   r.bias = bias;
   r.bias_bf16 = c.s->bias_dtype == EWS_DTYPE_BF16;
   r.bias_out = (float*)(c.w + p.bias);
+  r.scale = p.entries ? c.top.scale : kLog2e;
   r.grad_hidden = grad_hidden;
   // 64 workgroups at most list rows, 8192 or a multiple each
   r.each = ceil_div(ceil_div(p.N, 64), 8192) * 8192;
@@ -1089,6 +1324,26 @@ Operand hidden_operand(const Call& c) {
   return Operand{(const uint16_t*)(c.w + p.xp), p.Hp, p.Np * p.Hp, (int)p.Np, (int)p.Hp};
 }
 
+template <bool TOP>
+int launch_join(const Call& c, int c0, float* loss_rows) {
+  const LPlan& p = c.p;
+  const int chunk = (int)p.chunk;
+  // one row's slabs by a workgroup's threads where there are few rows: N=1, V=100003: 23 us with 16 threads a row
+  if (p.N <= 256)
+    hipLaunchKernelGGL((k_join<4, TOP>), dim3(ceil_div(p.chunk, 4)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, c0,
+                       chunk, loss_rows);
+  else
+    hipLaunchKernelGGL((k_join<64, TOP>), dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, c0,
+                       chunk, loss_rows);
+  LOSS_CHECK();
+  if (TOP) {
+    hipLaunchKernelGGL(k_top_loss, dim3(ceil_div(p.chunk, 4)), dim3(256), 0, c.st, c.stats, c.rows, c.top, c0, chunk,
+                       loss_rows);
+    LOSS_CHECK();
+  }
+  return EWS_OK;
+}
+
 int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
   const LPlan& p = c.p;
   LogitArgs a{};
@@ -1105,6 +1360,7 @@ int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
   a.bias = (const float*)(c.w + p.bias);
   a.rows = c.rows;
   a.st = c.stats;
+  a.top = c.top;
   int rc;
   if (p.train) {
     a.prob = c.w + p.prob;
@@ -1114,18 +1370,10 @@ int logits(const Call& c, const void* weight, int chunk, float* loss_rows) {
     rc = p.np == 3 ? launch_logits<kPairs, 0>(p.logits.kind, a, c.st) : launch_logits<1, 0>(p.logits.kind, a, c.st);
   }
   if (rc != EWS_OK) return rc;
-  // one row's slabs by a workgroup's threads where there are few rows: N=1, V=100003: 23 us with 16 threads a row
-  if (p.N <= 256)
-    hipLaunchKernelGGL((k_join<4>), dim3(ceil_div(p.chunk, 4)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, a.c0,
-                       a.chunk, loss_rows);
-  else
-    hipLaunchKernelGGL((k_join<64>), dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, a.c0,
-                       a.chunk, loss_rows);
-  LOSS_CHECK();
-  return EWS_OK;
+  return p.entries ? launch_join<true>(c, a.c0, loss_rows) : launch_join<false>(c, a.c0, loss_rows);
 }
 
-Call make_call(const ews_loss_desc* s, const LPlan& p, void* workspace, ews_stream_t stream) {
+Call make_call(const ews_loss_desc* s, const LPlan& p, void* workspace, ews_stream_t stream, float temperature = 1.0f) {
   Call c{};
   c.s = s;
   c.p = p;
@@ -1140,6 +1388,17 @@ Call make_call(const ews_loss_desc* s, const LPlan& p, void* workspace, ews_stre
   c.stats.top = (float*)(c.w + p.top);
   c.stats.inv = (float*)(c.w + p.inv);
   c.stats.loss = (float*)(c.w + p.loss);
+  if (p.entries) {
+    c.top.count = p.entries;
+    c.top.token = (const int*)(c.w + p.token);
+    c.top.p = (const float*)(c.w + p.share);
+    c.top.entropy = (const float*)(c.w + p.entropy);
+    c.top.first = (const uint16_t*)(c.w + p.first);
+    c.top.buckets = p.buckets;
+    c.top.z = c.stats.zt;
+    c.top.temperature = temperature;
+    c.top.scale = kLog2e / temperature;
+  }
   return c;
 }
 
@@ -1147,6 +1406,19 @@ int launch_total(const Call& c, float* loss) {
   hipLaunchKernelGGL(k_total, dim3(1), dim3(1024), 0, c.st, c.stats, c.rows, loss);
   LOSS_CHECK();
   return EWS_OK;
+}
+
+template <int NP>
+void launch_dz(const DzArgs& z, dim3 grid, const LPlan& p, hipStream_t st) {
+  const bool narrow = p.Vp <= 256;
+  if (p.entries && narrow)
+    hipLaunchKernelGGL((k_dz<NP, true, true>), grid, dim3(256), 0, st, z);
+  else if (p.entries)
+    hipLaunchKernelGGL((k_dz<NP, false, true>), grid, dim3(256), 0, st, z);
+  else if (narrow)
+    hipLaunchKernelGGL((k_dz<NP, true, false>), grid, dim3(256), 0, st, z);
+  else
+    hipLaunchKernelGGL((k_dz<NP, false, false>), grid, dim3(256), 0, st, z);
 }
 
 // Chunk k's gradients from what logits() kept of it; the last chunk writes the call's loss too, where asked.
@@ -1171,22 +1443,15 @@ int gradients(const Call& c, const void* weight, int k, const float* upstream, f
   z.bias = grad_bias ? (float*)(c.w + p.dbias) : nullptr;
   z.each = p.dz_rows;
   z.loss = last ? loss : nullptr;
+  z.top = c.top;
   const dim3 grid(ceil_div(p.Vp, 512) + (z.loss ? 1 : 0), ceil_div(p.chunk, p.dz_rows));
-  if (p.Vp <= 256) {
-    z.lanes = p.Vp <= 64 ? 8 : p.Vp <= 128 ? 16 : 32;
-    if (f32)
-      hipLaunchKernelGGL((k_dz<3, true>), grid, dim3(256), 0, c.st, z);
-    else if (p.twice)
-      hipLaunchKernelGGL((k_dz<2, true>), grid, dim3(256), 0, c.st, z);
-    else
-      hipLaunchKernelGGL((k_dz<1, true>), grid, dim3(256), 0, c.st, z);
-  } else if (f32) {
-    hipLaunchKernelGGL((k_dz<3, false>), grid, dim3(256), 0, c.st, z);
-  } else if (p.twice) {
-    hipLaunchKernelGGL((k_dz<2, false>), grid, dim3(256), 0, c.st, z);
-  } else {
-    hipLaunchKernelGGL((k_dz<1, false>), grid, dim3(256), 0, c.st, z);
-  }
+  z.lanes = p.Vp <= 64 ? 8 : p.Vp <= 128 ? 16 : 32;
+  if (f32)
+    launch_dz<3>(z, grid, p, c.st);
+  else if (p.twice)
+    launch_dz<2>(z, grid, p, c.st);
+  else
+    launch_dz<1>(z, grid, p, c.st);
   LOSS_CHECK();
   if (grad_bias) {
     float* sum = (float*)(c.w + p.dbsum);
@@ -1345,6 +1610,127 @@ int ews_loss_kept(const ews_loss_desc* desc, const void* weight, const float* up
   if (!weight || !workspace) return EWS_ERR_NULL;
   return gradients(make_call(desc, p, workspace, stream), weight, 0, upstream, nullptr, grad_hidden, grad_weight,
                    grad_bias);
+}
+
+}  // extern "C"
+
+namespace {
+
+int distill_plan(const ews_distill_desc* d, bool train, bool direct, LPlan& p) {
+  if (!d) return EWS_ERR_NULL;
+  if (d->index_bytes != 4 && d->index_bytes != 8) return EWS_ERR_OPTION;
+  if (d->logit_dtype != EWS_DTYPE_F32 && d->logit_dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
+  if (!(d->temperature >= 1e-6f) || d->temperature > 1e6f) return EWS_ERR_OPTION;
+  if (d->entries < 1 || d->entries > kMostTop || d->index_stride < 0 || d->logit_stride < 0) return EWS_ERR_SHAPE;
+  return loss_plan(&d->head, train, direct, p, d->entries);
+}
+
+// A call whose targets are a teacher's entries: k_teacher lists them as it lists the rows that have any.
+struct Distill {
+  Call c;
+  ews_loss_desc head;
+  int rc;
+  Distill(const ews_distill_desc* d, bool train, const void* weight, void* workspace, ews_stream_t stream) {
+    LPlan p;
+    rc = distill_plan(d, train, d && reads_direct(&d->head, weight), p);
+    if (rc != EWS_OK) return;
+    if (!weight || !workspace) {
+      rc = EWS_ERR_NULL;
+      return;
+    }
+    head = d->head;
+    head.ignore_index = kNone;
+    c = make_call(&head, p, workspace, stream, d->temperature);
+  }
+  int begin(const ews_distill_desc* d, const void* hidden, const void* weight, const void* bias, const void* indices,
+            const void* teacher, float* loss_rows, void* grad_hidden) {
+    if (!hidden || !indices || !teacher) return EWS_ERR_NULL;
+    const LPlan& p = c.p;
+    TeacherArgs t{};
+    t.index = indices;
+    t.logit = teacher;
+    t.index_stride = d->index_stride;
+    t.logit_stride = d->logit_stride;
+    t.n = p.N;
+    t.count = p.entries;
+    t.vocab = p.V;
+    t.buckets = p.buckets;
+    t.ordered = 2;
+    while (t.ordered < t.count) t.ordered *= 2;
+    t.index_bytes = d->index_bytes;
+    t.logit_bf16 = d->logit_dtype == EWS_DTYPE_BF16;
+    t.scale = c.top.scale;
+    t.target = (int64_t*)(c.w + p.flags);
+    t.token = (int*)(c.w + p.token);
+    t.p = (float*)(c.w + p.share);
+    t.entropy = (float*)(c.w + p.entropy);
+    t.first = (uint16_t*)(c.w + p.first);
+    hipLaunchKernelGGL(k_teacher, dim3(ceil_div(p.N, 4)), dim3(256), 4 * t.ordered * 8, c.st, t);
+    LOSS_CHECK();
+    return ::begin(c, hidden, weight, bias, t.target, loss_rows, grad_hidden);
+  }
+};
+
+}  // namespace
+
+extern "C" {
+
+size_t ews_distill_workspace_bytes_for(const ews_distill_desc* desc, const void* weight, int train) {
+  LPlan p;
+  return distill_plan(desc, train != 0, desc && reads_direct(&desc->head, weight), p) == EWS_OK ? p.total : 0;
+}
+
+int ews_distill_forward(const ews_distill_desc* desc, const void* hidden, const void* weight, const void* bias,
+                        const void* indices, const void* teacher, float* loss, void* workspace, ews_stream_t stream) {
+  Distill d(desc, false, weight, workspace, stream);
+  if (d.rc != EWS_OK) return d.rc;
+  if (!loss) return EWS_ERR_NULL;
+  float* rows = desc->head.reduction == EWS_LOSS_NONE ? loss : nullptr;
+  int rc = d.begin(desc, hidden, weight, bias, indices, teacher, rows, nullptr);
+  for (int k = 0; k < d.c.p.chunks && rc == EWS_OK; ++k) rc = logits(d.c, weight, k, rows);
+  return rc != EWS_OK || rows ? rc : launch_total(d.c, loss);
+}
+
+int ews_distill_train(const ews_distill_desc* desc, const void* hidden, const void* weight, const void* bias,
+                      const void* indices, const void* teacher, const float* upstream, float* loss, void* grad_hidden,
+                      void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream) {
+  Distill d(desc, true, weight, workspace, stream);
+  if (d.rc != EWS_OK) return d.rc;
+  if (grad_bias && !bias) return EWS_ERR_NULL;
+  float* rows = desc->head.reduction == EWS_LOSS_NONE ? loss : nullptr;
+  int rc = d.begin(desc, hidden, weight, bias, indices, teacher, rows, grad_hidden);
+  for (int k = 0; k < d.c.p.chunks && rc == EWS_OK; ++k) {
+    rc = logits(d.c, weight, k, rows);
+    if (rc == EWS_OK)
+      rc = gradients(d.c, weight, k, upstream, rows ? nullptr : loss, grad_hidden, grad_weight, grad_bias);
+  }
+  return rc;
+}
+
+int ews_distill_keeps(const ews_distill_desc* desc) {
+  LPlan p;
+  return distill_plan(desc, true, false, p) == EWS_OK && p.chunks == 1;
+}
+
+int ews_distill_keep(const ews_distill_desc* desc, const void* hidden, const void* weight, const void* bias,
+                     const void* indices, const void* teacher, float* loss, void* grad_hidden, void* workspace,
+                     ews_stream_t stream) {
+  Distill d(desc, true, weight, workspace, stream);
+  if (d.rc != EWS_OK) return d.rc;
+  if (d.c.p.chunks > 1) return EWS_ERR_SHAPE;
+  if (!loss) return EWS_ERR_NULL;
+  float* rows = desc->head.reduction == EWS_LOSS_NONE ? loss : nullptr;
+  int rc = d.begin(desc, hidden, weight, bias, indices, teacher, rows, grad_hidden);
+  if (rc == EWS_OK) rc = logits(d.c, weight, 0, rows);
+  return rc != EWS_OK || rows ? rc : launch_total(d.c, loss);
+}
+
+int ews_distill_kept(const ews_distill_desc* desc, const void* weight, const float* upstream, void* grad_hidden,
+                     void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream) {
+  Distill d(desc, true, weight, workspace, stream);
+  if (d.rc != EWS_OK) return d.rc;
+  if (d.c.p.chunks > 1) return EWS_ERR_SHAPE;
+  return gradients(d.c, weight, 0, upstream, nullptr, grad_hidden, grad_weight, grad_bias);
 }
 
 }  // extern "C"

@@ -104,6 +104,12 @@ EXPORTED = (
     "ews_clip_workspace_bytes",
     "ews_clip",
     "ews_loss_scale",
+    "ews_distill_workspace_bytes_for",
+    "ews_distill_forward",
+    "ews_distill_train",
+    "ews_distill_keeps",
+    "ews_distill_keep",
+    "ews_distill_kept",
     "ews_gated_scan_residual_bytes",
     "ews_gated_scan_workspace_bytes",
     "ews_gated_scan_forward",
@@ -120,6 +126,7 @@ LIFT_FULL = 1
 LIFT_PRESERVE = 2
 
 LOSS_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+DISTILL_MOST_ENTRIES = 1024
 
 GATED_SCAN_FORMS = {"convex": 0, "linear": 1}
 
@@ -274,6 +281,32 @@ class EmbedDesc(ctypes.Structure):
     ]
 
 
+class LossDesc(ctypes.Structure):
+    _fields_ = [
+        ("hidden_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("hidden", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+    ]
+
+
+class DistillDesc(ctypes.Structure):
+    _fields_ = [
+        ("head", LossDesc),
+        ("index_stride", ctypes.c_int64),
+        ("logit_stride", ctypes.c_int64),
+        ("entries", ctypes.c_int32),
+        ("index_bytes", ctypes.c_int32),
+        ("logit_dtype", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+    ]
+
+
 class GatedScanDesc(ctypes.Structure):
     _fields_ = [
         ("x_batch", ctypes.c_int64),
@@ -286,20 +319,6 @@ class GatedScanDesc(ctypes.Structure):
         ("dim", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("form", ctypes.c_int32),
-    ]
-
-
-class LossDesc(ctypes.Structure):
-    _fields_ = [
-        ("hidden_stride", ctypes.c_int64),
-        ("weight_stride", ctypes.c_int64),
-        ("ignore_index", ctypes.c_int64),
-        ("rows", ctypes.c_int32),
-        ("hidden", ctypes.c_int32),
-        ("vocab", ctypes.c_int32),
-        ("dtype", ctypes.c_int32),
-        ("bias_dtype", ctypes.c_int32),
-        ("reduction", ctypes.c_int32),
     ]
 
 
@@ -481,6 +500,19 @@ def load():
     lib.ews_clip.restype = i32
     lib.ews_loss_scale.argtypes = [lsp, vp, vp, vp, vp, vp]
     lib.ews_loss_scale.restype = i32
+    dsp = ctypes.POINTER(DistillDesc)
+    lib.ews_distill_workspace_bytes_for.argtypes = [dsp, vp, i32]
+    lib.ews_distill_workspace_bytes_for.restype = sz
+    lib.ews_distill_forward.argtypes = [dsp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_distill_forward.restype = i32
+    lib.ews_distill_train.argtypes = [dsp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_distill_train.restype = i32
+    lib.ews_distill_keeps.argtypes = [dsp]
+    lib.ews_distill_keeps.restype = i32
+    lib.ews_distill_keep.argtypes = [dsp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_distill_keep.restype = i32
+    lib.ews_distill_kept.argtypes = [dsp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_distill_kept.restype = i32
     gsp = ctypes.POINTER(GatedScanDesc)
     lib.ews_gated_scan_residual_bytes.argtypes = [gsp]
     lib.ews_gated_scan_residual_bytes.restype = sz

@@ -31,7 +31,7 @@ from torch.nn.modules import module as nn_module
 from .embed import embedding_lookup
 from .front import B, BlockFront, ClockSpec, make_clock
 from .layer import EWS
-from .loss import linear_cross_entropy, logits_cross_entropy
+from .loss import linear_cross_entropy, linear_distillation, logits_cross_entropy, logits_distillation
 from .mixer import MixerEpilogue
 from .params import AParamBoundedRotation, AParamDampedRotation, AParamDefinitePlusSkew, is_rotation_planes
 
@@ -407,15 +407,34 @@ class StackedEWS(nn.Module):
             return e(X.long())
         return embedding_lookup(X.long(), e.weight, padding_idx=e.padding_idx)
 
-    def _head_loss(self, head, h, targets, ignore_index, reduction):
+    def _head_loss(self, head, h, fused, of_logits):
+        """The loss of one head's rows: ``fused`` of rows, weight and bias, or of a head that is more than a linear map
+        ``of_logits``."""
         if self.cosine_head_tau is None:
-            if not _is_plain(head, nn.Linear):
-                return logits_cross_entropy(head(h), targets, ignore_index, reduction)
-            return linear_cross_entropy(h, head.weight, targets, bias=head.bias, ignore_index=ignore_index,
-                                        reduction=reduction)
+            return fused(h, head.weight, head.bias) if _is_plain(head, nn.Linear) else of_logits(head(h))
         h_hat, W_hat = self._unit(head, h)
-        return linear_cross_entropy(h_hat / self.cosine_head_tau, W_hat, targets, ignore_index=ignore_index,
-                                    reduction=reduction)
+        return fused(h_hat / self.cosine_head_tau, W_hat, None)
+
+    def _heads(self, X, **given):
+        """The heads of a loss of X, and for each what is given of it."""
+        if X.dim() != (2 if self.tokens else 3):
+            raise ValueError(f"X must carry a batch, got shape {tuple(X.shape)}")
+        heads = list(self.head) if isinstance(self.head, nn.ModuleList) else [self.head]
+        of_each = []
+        for name, v in given.items():
+            of_each.append(list(v) if isinstance(v, (tuple, list)) else [v])
+            if len(of_each[-1]) != len(heads):
+                raise ValueError(f"{len(heads)} head(s), {len(of_each[-1])} tensor(s) of {name}")
+        return list(zip(heads, *of_each))
+
+    def _loss_rows(self, X, t, mask, raw_driver, inference):
+        """The rows that the heads read, and the positions off the mask (None where there are none)."""
+        if mask is not None and mask.dim() == 1:
+            mask = mask[None].expand(X.shape[0], -1)
+        h = self._blocks(self._encode(X), t, mask, raw_driver, inference)
+        if self.head_mode != "seq2seq":
+            return self._pool(h, mask), None
+        return h, None if mask is None else ~mask.to(torch.bool)
 
     def loss(self, X, targets, *, t=None, mask=None, raw_driver=None, inference: bool = False,
              ignore_index: int = -100, reduction: str = "mean"):
@@ -426,24 +445,36 @@ class StackedEWS(nn.Module):
         called as a module, and its rows or logits are then in memory as ``forward``'s are. X, t, mask and raw_driver as
         ``forward``'s, with a batch; targets (B, L) for "seq2seq" (positions off the mask count as ignored), (B,) for
         "mean_pool"; for several heads a tuple of them, whose losses are added."""
-        if X.dim() != (2 if self.tokens else 3):
-            raise ValueError(f"X must carry a batch, got shape {tuple(X.shape)}")
-        if mask is not None and mask.dim() == 1:
-            mask = mask[None].expand(X.shape[0], -1)
-        heads = list(self.head) if isinstance(self.head, nn.ModuleList) else [self.head]
-        all_targets = list(targets) if isinstance(targets, (tuple, list)) else [targets]
-        if len(all_targets) != len(heads):
-            raise ValueError(f"{len(heads)} head(s), {len(all_targets)} tensor(s) of targets")
-        h = self._blocks(self._encode(X), t, mask, raw_driver, inference)
-        if self.head_mode == "seq2seq":
-            if mask is not None:
-                off = ~mask.to(torch.bool)
-                all_targets = [y.masked_fill(off, ignore_index) for y in all_targets]
-        else:
-            h = self._pool(h, mask)
+        heads = self._heads(X, targets=targets)
+        h, off = self._loss_rows(X, t, mask, raw_driver, inference)
         total = None
-        for head, y in zip(heads, all_targets):
-            one = self._head_loss(head, h, y, ignore_index, reduction)
+        for head, y in heads:
+            if off is not None:
+                y = y.masked_fill(off, ignore_index)
+            one = self._head_loss(
+                head, h,
+                lambda x, w, b: linear_cross_entropy(x, w, y, bias=b, ignore_index=ignore_index, reduction=reduction),
+                lambda z: logits_cross_entropy(z, y, ignore_index, reduction))
+            total = one if total is None else total + one
+        return total
+
+    def distillation_loss(self, X, indices, logits, *, temperature: float = 1.0, t=None, mask=None, raw_driver=None,
+                          inference: bool = False, reduction: str = "mean"):
+        """The heads' distance from a teacher's largest logits (``linear_distillation``), in the place of ``loss``'s
+        cross entropy: for "seq2seq" heads indices and logits (B, L, K), the entries of positions off the mask counting
+        as none, for "mean_pool" (B, K); for several heads tuples of them, whose losses are added. Everything else is as
+        in ``loss``."""
+        heads = self._heads(X, indices=indices, logits=logits)
+        h, off = self._loss_rows(X, t, mask, raw_driver, inference)
+        total = None
+        for head, index, teacher in heads:
+            if off is not None:
+                index = index.masked_fill(off[..., None], -1)
+            one = self._head_loss(
+                head, h,
+                lambda x, w, b: linear_distillation(x, w, index, teacher, bias=b, temperature=temperature,
+                                                    reduction=reduction),
+                lambda z: logits_distillation(z, index, teacher, float(temperature), reduction))
             total = one if total is None else total + one
         return total
 

@@ -675,6 +675,35 @@ int ews_loss_kept(const ews_loss_desc* desc, const void* weight, const float* up
 int ews_loss_scale(const ews_loss_desc* desc, void* grad_hidden, void* grad_weight, void* grad_bias,
                    const float* factor, ews_stream_t stream);
 
+/* Distillation from a teacher's largest logits: of every row `entries` tokens with the teacher's logits t. With the
+ * temperature T, p = softmax(t / T) over a row's entries and q = softmax(z / T) over the vocabulary,
+ * loss_n = T^2 sum_k p_k (log p_k - log q_token(k)). An entry whose token is negative or whose logit is -inf is none; a
+ * row without any has loss and gradients zero and is not read. A token that is named twice is two entries. A row with a
+ * token of the vocabulary's size or more: NaN. */
+typedef struct ews_distill_desc {
+  ews_loss_desc head;    /* its ignore_index is not read */
+  int64_t index_stride;  /* elements between rows of indices */
+  int64_t logit_stride;  /* elements between rows of teacher */
+  int32_t entries;       /* K: 1..1024 */
+  int32_t index_bytes;   /* 8 (int64) or 4 (int32) */
+  int32_t logit_dtype;   /* EWS_DTYPE_* of teacher */
+  float temperature;     /* T: 1e-6..1e6 */
+} ews_distill_desc;
+
+/* As their namesakes of ews_loss; ews_loss_scale serves them too. */
+size_t ews_distill_workspace_bytes_for(const ews_distill_desc* desc, const void* weight, int train);
+int ews_distill_forward(const ews_distill_desc* desc, const void* hidden, const void* weight, const void* bias,
+                        const void* indices, const void* teacher, float* loss, void* workspace, ews_stream_t stream);
+int ews_distill_train(const ews_distill_desc* desc, const void* hidden, const void* weight, const void* bias,
+                      const void* indices, const void* teacher, const float* upstream, float* loss, void* grad_hidden,
+                      void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream);
+int ews_distill_keeps(const ews_distill_desc* desc);
+int ews_distill_keep(const ews_distill_desc* desc, const void* hidden, const void* weight, const void* bias,
+                     const void* indices, const void* teacher, float* loss, void* grad_hidden, void* workspace,
+                     ews_stream_t stream);
+int ews_distill_kept(const ews_distill_desc* desc, const void* weight, const float* upstream, void* grad_hidden,
+                     void* grad_weight, void* grad_bias, void* workspace, ews_stream_t stream);
+
 /* Gradient clipping over n tensors, given by host arrays of device addresses, element counts (0 allowed) and
  * EWS_DTYPE_*: result[0] = norm = sqrt(sum of all squares), result[1] = c = min(1, max_norm / (norm + 1e-6)) (NaN for
  * a NaN norm). scale != 0: also out = c in for every tensor (out[i] == in[i]: in place; otherwise they may not
