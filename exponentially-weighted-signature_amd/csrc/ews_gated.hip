@@ -1,0 +1,967 @@
+// Gated linear map of a channel stage on MI355X (gfx950), forward and backward.
+//
+//   v = x V^T + b      g = x G^T + c      y = v act(g)
+//   dv = dy act(g)     dg = dy v act'(g)
+//   dx = dv V + dg G   dV = dv^T x   dG = dg^T x   db = sum_n dv   dc = sum_n dg
+//
+// act: the logistic function s, g s(g), g s(2 sqrt(2/pi) (g + 0.044715 g^3)) (the tanh form of GELU), or max(g, 0).
+//
+// Three pairs of products of 2 N H F operations each bound all but the smallest calls; they run on the matrix cores
+// (ews_tiles.h). v and g of the same output meet in a wavefront's registers: a tile's first operand is interleaved, half
+// of every wavefront's rows from V and half from G, which costs nothing, as the copies to LDS can start anywhere. So y is
+// formed where the sums end, and v and g are never in memory. A training call writes act(g) and v act'(g) in x's type
+// beside y, what the backward multiplies dy with: each is rounded once, relative to itself (v and g rounded in their place
+// would be cheaper by nothing, and g's rounding would be multiplied by |g|). k_dz forms dv | dg from them, one after the
+// other along a row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows.
+//
+// Few rows (decoding) are bound by V and G's bytes: k_few reads them straight into the matrix instructions' registers,
+// many loads on their way at once, without LDS.
+//
+// Float32 numbers are multiplied as three bfloat16 planes and six products (ews_tiles.h), float32's accuracy. Sums are
+// float32, nothing is added with atomics: the same inputs give the same bits.
+#include <hip/hip_runtime.h>
+
+#include "ews_hip.h"
+#include "ews_pack.h"
+#include "ews_pick.h"
+#include "ews_tiles.h"
+#include "ews_vec.h"
+
+namespace ews {
+namespace gated {
+
+using namespace ews::tiles;
+using namespace ews::vec;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// s(g) and s(-g), either without the other's rounding.
+__device__ __forceinline__ void logistic(float g, float& p, float& q) {
+  const float y = g * -kLog2e;
+  const float e = __builtin_amdgcn_exp2f(y);
+  p = __builtin_amdgcn_rcpf(1.0f + e);
+  q = y > 126.0f ? 1.0f : e * p;  // e may be infinite
+}
+
+// act(g) and act'(g).
+__device__ __forceinline__ void activate(int kind, float g, float& act, float& slope) {
+  if (kind == EWS_GATED_RELU) {
+    act = g <= 0.0f ? 0.0f : g;  // a NaN stays one
+    slope = g > 0.0f ? 1.0f : 0.0f;
+    return;
+  }
+  float p, q;
+  if (kind == EWS_GATED_GELU) {
+    const float c = g > 30.0f ? 30.0f : g < -30.0f ? -30.0f : g;  // s is 0 or 1 long before; g^3 stays finite
+    const float c2 = c * c;
+    logistic(1.5957691216057308f * c * fmaf(0.044715f, c2, 1.0f), p, q);
+    act = g * p;
+    slope = fmaf(c * p * q, 1.5957691216057308f * fmaf(0.134145f, c2, 1.0f), p);
+    return;
+  }
+  logistic(g, p, q);
+  act = kind == EWS_GATED_SILU ? g * p : p;
+  slope = kind == EWS_GATED_SILU ? fmaf(g * p, q, p) : p * q;
+}
+
+// ------------------------------------------------------------------------------------------------------ the operands
+// V and G as a tile's first operand: of every wavefront's blocks of 32 rows the first half are V's, the others the same
+// rows of G. Rows start as far apart in both.
+struct Pair {
+  Operand v;
+  int64_t to_g;  // elements from V's numbers to G's
+};
+
+template <class T>
+struct CopierPair {
+  static constexpr int kCopies = T::kCopiesP, kHalf = T::TI / 2;
+  static_assert(T::TI % 2 == 0 && T::kThreads / 8 <= 32 * kHalf, "a copy's rows are of one side");
+  const uint16_t* base;
+  int64_t plane, to_g;
+  uint32_t offset[kCopies];
+  static constexpr __device__ __forceinline__ bool gate(int c) {
+    return c * (T::kThreads / 8) / 32 % T::TI >= kHalf;
+  }
+  __device__ __forceinline__ CopierPair(const Pair& o, int tile) : plane(o.v.plane), to_g(o.to_g) {
+    const int first = tile < o.v.rows ? tile : o.v.rows - 1;
+    base = o.v.p + first * o.v.ld;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const int idx = threadIdx.x + c * T::kThreads;
+      const int row = idx >> 3, block = row >> 5;
+      const int own = (block / T::TI * kHalf + block % kHalf) * 32 + (row & 31);
+      offset[c] = (uint32_t)(first + own < o.v.rows ? own : o.v.rows - 1 - first) * (uint32_t)o.v.ld * 2 +
+                  16 * place(row, idx & 7);
+    }
+  }
+  __device__ __forceinline__ const uint16_t* at(int piece, int kb) const { return base + piece * plane + (int64_t)kb * 64; }
+  __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const {
+    copy_piece(gate(c) ? from + to_g : from, offset[c], to + c * T::kThreads * 16);
+  }
+};
+
+// V and G one after the other along k: k blocks of V's rows (the last one's missing rows read its last row, which meets
+// zeros), then as many of G's.
+struct Chain {
+  Operand v;
+  int64_t to_g;
+  int blocks;  // of either
+};
+
+template <class T>
+struct CopierChain {
+  static constexpr int kCopies = T::kCopiesP;
+  Copier<true, T::I, T::kThreads> rows;
+  int64_t to_g;
+  int blocks;
+  __device__ __forceinline__ CopierChain(const Chain& o, int tile) : rows(o.v, tile), to_g(o.to_g), blocks(o.blocks) {}
+  __device__ __forceinline__ const uint16_t* at(int piece, int kb) {
+    const bool second = kb >= blocks;
+    const int own = second ? kb - blocks : kb;
+    if (second && own == 0) rows.aim_turned(63);  // V's last block may have had fewer
+    return rows.at(piece, own) + (second ? to_g : 0);
+  }
+  __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const { rows.copy(c, from, to); }
+};
+
+}  // namespace gated
+
+namespace tiles {
+template <class T>
+struct CopierOf<gated::Pair, T, false> {
+  typedef gated::CopierPair<T> type;
+};
+template <class T>
+struct CopierOf<gated::Chain, T, true> {
+  typedef gated::CopierChain<T> type;
+};
+}  // namespace tiles
+
+namespace gated {
+
+// ------------------------------------------------------------------------------------------------------- the forward
+struct ForwardArgs {
+  Pair W;
+  Operand X;
+  int ti, tj, kblocks;
+  int N, F;
+  const void* bias;        // or null
+  const void* gate_bias;
+  int act;
+  int wide;                // rows of out start at multiples of 16 bytes and hold whole eights
+  void* out;               // (N, F)
+  void* kept;              // (N, 2 ld): act(g) | v act'(g); or null
+  int64_t ld;              // F up to a multiple of 64
+};
+
+template <typename O>
+__device__ __forceinline__ void store(O* to, const Eight& e) {
+#pragma unroll
+  for (int q = 0; q < 8; q += kWide<O>) {
+    Pack<O, kWide<O>> p;
+    p.set(e.x + q);
+    p.store_past(to + q);
+  }
+}
+template <typename O>
+__device__ __forceinline__ void store(O* to, const One& e) {
+  *to = narrow<O>(e.x);
+}
+
+// A wavefront's 32 rows of 16 TI results each, z[a] its blocks, through its own part of LDS: f(row of the 32, column, W).
+template <class T, typename W, class F>
+__device__ __forceinline__ void rows_of_half(char* lds, const f32x16 (&z)[T::TI / 2], F f) {
+  constexpr int kCols = 16 * T::TI, kRow = kCols + 4, kEach = sizeof(W) / 4;
+  const int lane = threadIdx.x & 63, r32 = lane & 31, half = lane >> 5;
+  float* stage = reinterpret_cast<float*>(lds) + (threadIdx.x >> 6) * 32 * T::kRowWords;
+#pragma unroll
+  for (int a = 0; a < T::TI / 2; ++a)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(stage + r32 * kRow + a * 32 + g * 8 + half * 4) =
+          f32x4{z[a][4 * g], z[a][4 * g + 1], z[a][4 * g + 2], z[a][4 * g + 3]};
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  constexpr int kLanes = kCols / kEach < 64 ? kCols / kEach : 64;
+#pragma unroll
+  for (int it = 0; it < 32 * kCols / kEach / 64; ++it) {
+    const int row = it * (64 / kLanes) + lane / kLanes, col = lane % kLanes * kEach;
+    W w;
+    if constexpr (kEach == 8) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(stage + row * kRow + col);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(stage + row * kRow + col + 4);
+      w = Eight{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+    } else {
+      w = One{stage[row * kRow + col]};
+    }
+    f(row, col, w);
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <typename B>
+__device__ __forceinline__ float bias_at(const void* bias, int i) {
+  return bias ? widen(((const B*)bias)[i]) : 0.0f;
+}
+
+template <class T, int PAIRS, typename O>
+__global__ __launch_bounds__(T::kThreads, T::kWaves) void k_forward(ForwardArgs a) {
+  extern __shared__ char lds[];
+  int it, jt;
+  tile_of(blockIdx.x, a.ti, a.tj, it, jt);
+  const int i0 = it * (T::I / 2), j0 = jt * T::J;
+  float* bias = reinterpret_cast<float*>(lds + lds_bytes<T, PAIRS>(a.kblocks));  // V's, then G's
+  for (int t = threadIdx.x; t < T::I; t += T::kThreads) {
+    const int i = i0 + t % (T::I / 2), in = i < a.F ? i : a.F - 1;
+    bias[t] = bias_at<O>(t < T::I / 2 ? a.bias : a.gate_bias, in);
+  }
+  f32x16 acc[T::TI][T::TJ];
+  product<T, PAIRS, false, false>(a.W, a.X, i0, j0, 0, a.kblocks, lds, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wi = wave % T::WI, wj = wave / T::WI, half = lane >> 5;
+  constexpr int kHalf = T::TI / 2;
+#pragma unroll
+  for (int b = 0; b < T::TJ; ++b) {
+    f32x16 y[kHalf], p[kHalf], q[kHalf];
+#pragma unroll
+    for (int t = 0; t < kHalf; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = (wi * kHalf + t) * 32 + 8 * (r / 4) + 4 * half + r % 4;
+        const float v = acc[t][b][r] + bias[i];
+        float act, slope;
+        activate(a.act, acc[t + kHalf][b][r] + bias[T::I / 2 + i], act, slope);
+        y[t][r] = v * act;
+        p[t][r] = act;
+        q[t][r] = v * slope;
+      }
+    const int row0 = j0 + (wj * T::TJ + b) * 32, col0 = i0 + wi * kHalf * 32;
+    auto out = [&](auto each) {
+      using W = decltype(each);
+      rows_of_half<T, W>(lds, y, [&](int row, int col, const W& e) {
+        if (row0 + row < a.N && col0 + col < a.F)
+          store<O>((O*)a.out + (int64_t)(row0 + row) * a.F + col0 + col, e);
+      });
+    };
+    if (a.wide)
+      out(Eight{});
+    else
+      out(One{});
+    if (!a.kept) continue;
+    // whole eights up to ld: what lies past F is not read
+    rows_of_half<T, Eight>(lds, p, [&](int row, int col, const Eight& e) {
+      if (row0 + row < a.N && col0 + col < a.ld)
+        store<O>((O*)a.kept + (int64_t)(row0 + row) * 2 * a.ld + col0 + col, e);
+    });
+    rows_of_half<T, Eight>(lds, q, [&](int row, int col, const Eight& e) {
+      if (row0 + row < a.N && col0 + col < a.ld)
+        store<O>((O*)a.kept + (int64_t)(row0 + row) * 2 * a.ld + a.ld + col0 + col, e);
+    });
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------- few rows
+struct FewArgs {
+  const void* x;
+  const void* v;
+  const void* g;
+  int64_t xs, ws, gs;
+  int N, H, F;
+  const void* bias;
+  const void* gate_bias;
+  int act;
+  void* out;
+};
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
+// Eight neighbouring numbers of a row from column k on, zero past the row's end.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void eight(const T* row, int k, int H, T (&x)[8]) {
+  if (WIDE) {  // H is a multiple of 8 then
+    if (k < H) {
+#pragma unroll
+      for (int q = 0; q < 8; q += kWide<T>) *reinterpret_cast<u32x4*>(x + q) = *reinterpret_cast<const u32x4*>(row + k + q);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = narrow<T>(0.0f);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) x[q] = k + q < H ? row[k + q] : narrow<T>(0.0f);
+  }
+}
+
+template <typename T>
+constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+
+template <typename T>
+__device__ __forceinline__ void fragments(const T (&x)[8], bf16x8 (&f)[kPlanes<T>]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint16_t p[kPlanes<T>];
+    planes(x[q], p);
+#pragma unroll
+    for (int n = 0; n < kPlanes<T>; ++n) f[n][q] = __builtin_bit_cast(__bf16, p[n]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void multiply(const bf16x8 (&p)[kPlanes<T>], const bf16x8 (&q)[kPlanes<T>], f32x4v& acc) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int pair = 0; pair < kPairs; ++pair)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[piece_p(pair)], q[piece_q(pair)], acc, 0, 0, 0);
+  } else {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[0], q[0], acc, 0, 0, 0);
+  }
+}
+
+constexpr int kFewWaves = 4;
+
+// 16 outputs of up to 16 COLS rows a workgroup; its wavefronts take every fourth 32 AHEAD of k and are joined in LDS.
+// v_mfma_f32_16x16x32_bf16: lane l holds row l % 16 of either operand at k = 8 (l / 16) + 0..7, and results
+// column l % 16, rows 4 (l / 16) + 0..3.
+template <typename T, int COLS, bool WIDE>
+__global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
+  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
+  __shared__ f32x4v part[kFewWaves][2][COLS][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r16 = lane & 15, k8 = (lane >> 4) * 8;
+  const int f0 = blockIdx.x * 16;
+  const int row = f0 + r16 < a.F ? f0 + r16 : a.F - 1;
+  const T* v = (const T*)a.v + row * a.ws;
+  const T* g = (const T*)a.g + row * a.gs;
+  f32x4v accv[COLS], accg[COLS];
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) accv[c] = accg[c] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k0 = wave * 32 * kAhead; k0 < a.H; k0 += kFewWaves * 32 * kAhead) {
+    T wv[kAhead][8], wg[kAhead][8];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      eight<T, WIDE>(v, k0 + 32 * s + k8, a.H, wv[s]);
+      eight<T, WIDE>(g, k0 + 32 * s + k8, a.H, wg[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      bf16x8 fv[kPlanes<T>], fg[kPlanes<T>];
+      fragments<T>(wv[s], fv);
+      fragments<T>(wg[s], fg);
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) {
+        const int n = c * 16 + r16 < a.N ? c * 16 + r16 : a.N - 1;
+        T x[8];
+        bf16x8 fx[kPlanes<T>];
+        eight<T, WIDE>((const T*)a.x + n * a.xs, k0 + 32 * s + k8, a.H, x);
+        fragments<T>(x, fx);
+        multiply<T>(fv, fx, accv[c]);
+        multiply<T>(fg, fx, accg[c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    part[wave][0][c][lane] = accv[c];
+    part[wave][1][c][lane] = accg[c];
+  }
+  __syncthreads();
+  for (int c = wave; c < COLS; c += kFewWaves) {
+    f32x4v sv = part[0][0][c][lane], sg = part[0][1][c][lane];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) {
+      sv += part[w][0][c][lane];
+      sg += part[w][1][c][lane];
+    }
+    const int n = c * 16 + r16;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int f = f0 + (lane >> 4) * 4 + r;
+      if (n >= a.N || f >= a.F) continue;
+      float act, slope;
+      activate(a.act, sg[r] + bias_at<T>(a.gate_bias, f), act, slope);
+      ((T*)a.out)[(int64_t)n * a.F + f] = narrow<T>((sv[r] + bias_at<T>(a.bias, f)) * act);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ dv | dg
+struct DzArgs {
+  const void* dy;          // (N, F)
+  const void* kept;        // (N, 2 ld)
+  int N, F, padded;        // rows; and zeros up to this one
+  int64_t ld;
+  int wide;                // rows of dy start at multiples of 16 bytes and hold whole eights
+  uint16_t* dz;            // planes (padded, 2 ld), zero past F
+  int64_t plane;
+  float* sums;             // (workgroups along y, 2 ld) over the rows; or null
+  int each;                // rows of a workgroup
+};
+
+// A thread eight columns of every fourth of its workgroup's rows.
+template <typename T>
+__global__ __launch_bounds__(256) void k_dz(DzArgs a) {
+  constexpr int NP = kPlanes<T>;
+  __shared__ float part[4][2][64][9];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int f = (blockIdx.x * 64 + lane) * 8;
+  const int n = f >= a.F ? 0 : a.F - f < 8 ? a.F - f : 8;
+  const int r1 = (int)(blockIdx.y + 1) * a.each < a.padded ? (int)(blockIdx.y + 1) * a.each : a.padded;
+  float sums[2][8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) sums[0][q] = sums[1][q] = 0.0f;
+  for (int row = blockIdx.y * a.each + wave; row < r1 && f < a.ld; row += 4) {
+    float u[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) u[q] = 0.0f;
+    const int live = row < a.N ? n : 0;
+    const T* dy = (const T*)a.dy + (int64_t)row * a.F + f;
+    if (a.wide && live) {
+#pragma unroll
+      for (int q = 0; q < 8; q += kWide<T>) {
+        Pack<T, kWide<T>> p;
+        p.load(dy + q);
+#pragma unroll
+        for (int e = 0; e < kWide<T>; ++e) u[q + e] = p.get(e);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < live) u[q] = widen(dy[q]);
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      float z[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) z[q] = 0.0f;
+      if (live) {
+        const T* kept = (const T*)a.kept + ((int64_t)row * 2 + side) * a.ld + f;
+#pragma unroll
+        for (int q = 0; q < 8; q += kWide<T>) {
+          Pack<T, kWide<T>> p;
+          p.load(kept + q);
+#pragma unroll
+          for (int e = 0; e < kWide<T>; ++e) z[q + e] = q + e < live ? u[q + e] * p.get(e) : 0.0f;
+        }
+      }
+      uint16_t p[8][NP];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        sums[side][q] += z[q];
+        planes(narrow<T>(z[q]), p[q]);
+      }
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        u32x4 w;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = (uint32_t)p[2 * q][k] | ((uint32_t)p[2 * q + 1][k] << 16);
+        *reinterpret_cast<u32x4*>(a.dz + k * a.plane + ((int64_t)row * 2 + side) * a.ld + f) = w;
+      }
+    }
+  }
+  if (!a.sums) return;
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) part[wave][side][lane][q] = sums[side][q];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 1024; t += 256) {
+    const int side = t >> 9, c = t & 511, col = blockIdx.x * 512 + c;
+    if (col >= a.ld) continue;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) s += part[w][side][c >> 3][c & 7];
+    a.sums[((int64_t)blockIdx.y * 2 + side) * a.ld + col] = s;
+  }
+}
+
+// The biases' gradients: 64 columns a workgroup, its sixteen wavefronts a contiguous part of k_dz's sums each.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_dbias(const float* sums, int parts, int64_t ld, int F, T* dv, T* dg) {
+  __shared__ float joined[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, f = blockIdx.x * 64 + lane, side = blockIdx.y;
+  const int each = (parts + 15) / 16, p1 = (wave + 1) * each < parts ? (wave + 1) * each : parts;
+  T* out = side ? dg : dv;
+  float s = 0.0f;
+  if (f < F) {
+#pragma unroll 8
+    for (int p = wave * each; p < p1; ++p) s += sums[((int64_t)p * 2 + side) * ld + f];
+  }
+  joined[wave][lane] = s;
+  __syncthreads();
+  if (wave || f >= F || !out) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) s += joined[w][lane];
+  out[f] = narrow<T>(s);
+}
+
+// ------------------------------------------------------------------------------------------------------ the gradients
+struct GradArgs {
+  Chain W;                 // dx: k along 2 F
+  Operand X;               // dV | dG: k along the rows
+  Operand Z;               // dv | dg
+  int ti, tj, splits, kblocks, per;
+  int I, J;                // results along H; rows of dx, or 2 ld of dV | dG
+  int F, ld;               // dV | dG: those of the J that are V's and G's
+  float* part;             // (splits, J, I) where splits > 1
+  void* out;               // dx or dV
+  void* gate_out;          // dG
+  int wide;                // results' rows start at multiples of 16 bytes and hold whole eights
+};
+
+// Where result row j belongs; null: nowhere.
+template <bool ROWS, typename O>
+__device__ __forceinline__ O* result_row(const GradArgs& a, int j) {
+  if (!ROWS) return j < a.J ? (O*)a.out + (int64_t)j * a.I : nullptr;
+  const bool gate = j >= a.ld;
+  const int f = gate ? j - a.ld : j;
+  O* out = (O*)(gate ? a.gate_out : a.out);
+  return f < a.F && out ? out + (int64_t)f * a.I : nullptr;
+}
+
+__device__ __forceinline__ void keep(float* to, const Eight& e) {
+  *reinterpret_cast<f32x4*>(to) = f32x4{e.x[0], e.x[1], e.x[2], e.x[3]};
+  *reinterpret_cast<f32x4*>(to + 4) = f32x4{e.x[4], e.x[5], e.x[6], e.x[7]};
+}
+__device__ __forceinline__ void keep(float* to, const One& e) { *to = e.x; }
+
+// ROWS: dV | dG; else dx.
+template <class T, int PAIRS, bool ROWS, typename O>
+__global__ __launch_bounds__(T::kThreads, T::kWaves) void k_grad(GradArgs a) {
+  extern __shared__ char lds[];
+  int it, jt;
+  tile_of(blockIdx.x, a.ti, a.tj, it, jt);
+  const int i0 = it * T::I, j0 = jt * T::J, split = blockIdx.y;
+  const int kb0 = split * a.per, kb1 = kb0 + a.per < a.kblocks ? kb0 + a.per : a.kblocks;
+  f32x16 acc[T::TI][T::TJ];
+  if constexpr (ROWS)
+    product<T, PAIRS, true, true>(a.X, a.Z, i0, j0, kb0, kb1, lds, acc);
+  else
+    product<T, PAIRS, true, false>(a.W, a.Z, i0, j0, kb0, kb1, lds, acc);
+  auto rows = [&](auto each) {
+    using W = decltype(each);
+#pragma unroll
+    for (int b = 0; b < T::TJ; ++b)
+      rows_of<T, W>(lds, acc, b, [&](int jrow, int icol, const W& e) {
+        const int j = j0 + jrow, i = i0 + icol;
+        if (j >= a.J || i >= a.I) return;
+        if (a.splits > 1) return keep(a.part + ((int64_t)split * a.J + j) * a.I + i, e);
+        O* to = result_row<ROWS, O>(a, j);
+        if (to) store<O>(to + i, e);
+      });
+  };
+  if (a.wide)
+    rows(Eight{});
+  else
+    rows(One{});
+}
+
+// The splits' results added in order, by GROUPS groups of a workgroup's threads a contiguous part of them each; a thread
+// takes one result (W: One) or eight.
+template <bool ROWS, typename O, typename W, int GROUPS>
+__global__ __launch_bounds__(256) void k_join(GradArgs a) {
+  constexpr int kEach = sizeof(W) / 4, kThreads = 256 / GROUPS;
+  __shared__ float joined[GROUPS][kThreads][kEach];
+  const int group = threadIdx.x / kThreads, lane = threadIdx.x % kThreads;
+  const int64_t n = (int64_t)a.J * a.I, at = ((int64_t)blockIdx.x * kThreads + lane) * kEach;
+  const int per = (a.splits + GROUPS - 1) / GROUPS, s1 = (group + 1) * per < a.splits ? (group + 1) * per : a.splits;
+  float x[kEach];
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) x[q] = 0.0f;
+  if (at < n) {
+#pragma unroll 4
+    for (int s = group * per; s < s1; ++s) {
+      const float* from = a.part + s * n + at;
+      if constexpr (kEach == 1) {
+        x[0] += from[0];
+      } else {
+#pragma unroll
+        for (int q = 0; q < kEach; q += 4) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(from + q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[q + e] += w[e];
+        }
+      }
+    }
+  }
+  if (GROUPS > 1) {
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) joined[group][lane][q] = x[q];
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g)
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) x[q] += joined[g][lane][q];
+  }
+  if (at >= n) return;
+  const int j = (int)(at / a.I);
+  O* to = result_row<ROWS, O>(a, j);
+  W w;
+  __builtin_memcpy(&w, x, sizeof(w));
+  if (to) store<O>(to + (at - (int64_t)j * a.I), w);
+}
+
+}  // namespace gated
+}  // namespace ews
+
+namespace {
+
+using namespace ews::gated;
+namespace tiles = ews::tiles;
+using tiles::ceil_div;
+using tiles::Kind;
+using tiles::Operand;
+using tiles::Product;
+using ews::vec::bf16;
+
+// Rows up to which a forward alone reads V and G straight into registers.
+constexpr int kFewRows = 64;
+// Splits that one thread adds; more are added by eight groups of threads.
+constexpr int kFewSplits = 8;
+
+struct GPlan {
+  int N, H, F, np;
+  int64_t Hp, ld, Np;
+  bool pack_x, pack_w, few;
+  Product forward, dx, dw;
+  int dz_rows, dz_parts;
+  size_t xp, wp, dz, sums, part, total;
+};
+
+bool direct(const void* p, int64_t stride, int H) {
+  return H % 64 == 0 && stride % 8 == 0 && stride <= 1 << 22 && (uintptr_t)p % 16 == 0;
+}
+
+int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void* g, bool back, bool keep, GPlan& p) {
+  if (!s) return EWS_ERR_NULL;
+  if (s->dtype != EWS_DTYPE_F32 && s->dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
+  if (s->activation < 0 || s->activation > EWS_GATED_RELU) return EWS_ERR_OPTION;
+  if (s->rows < 1 || s->width < 1 || s->features < 1 || s->rows > 1 << 24 || s->width > 1 << 16 ||
+      s->features > 1 << 20)
+    return EWS_ERR_SHAPE;
+  if (s->x_stride < s->width || s->weight_stride < s->width || s->gate_stride < s->width) return EWS_ERR_SHAPE;
+  p.N = s->rows;
+  p.H = s->width;
+  p.F = s->features;
+  p.np = s->dtype == EWS_DTYPE_F32 ? 3 : 1;
+  p.Hp = (int64_t)ceil_div(p.H, 64) * 64;
+  p.ld = (int64_t)ceil_div(p.F, 64) * 64;
+  p.Np = (int64_t)ceil_div(p.N, 64) * 64;
+  // a launch has fewer than 2^32 threads, one for eight numbers; dv | dg's rows lie within the tiles' offsets
+  if (p.Np * p.Hp > (int64_t)1 << 34 || p.F * p.Hp > (int64_t)1 << 34 || p.Np * p.ld > (int64_t)1 << 34)
+    return EWS_ERR_SHAPE;
+  p.few = !back && !keep && p.N <= kFewRows;
+  p.pack_x = p.np == 3 || !direct(x, s->x_stride, p.H);
+  p.pack_w = p.np == 3 || !direct(v, s->weight_stride, p.H) || !direct(g, s->gate_stride, p.H) ||
+             s->weight_stride != s->gate_stride || ((uintptr_t)g - (uintptr_t)v) % 2;
+  const int pairs = p.np == 3 ? tiles::kPairs : 1;
+  p.forward = tiles::pick(2 * p.ld, p.N, (int)(p.Hp / 64), pairs, false, false);
+  p.dx = tiles::pick(p.H, p.N, (int)(2 * p.ld / 64), pairs, true, false);
+  p.dw = tiles::pick(p.H, 2 * p.ld, (int)(p.Np / 64), pairs, true, false);
+  size_t off = 0;
+  auto take = [&off](size_t bytes) {
+    const size_t at = off;
+    off += tiles::al256x(bytes);
+    return at;
+  };
+  if (!p.few) {
+    p.xp = take(p.pack_x ? (size_t)(p.N * p.Hp * p.np * 2) : 0);
+    p.wp = take(p.pack_w ? (size_t)(2 * p.F * p.Hp * p.np * 2) : 0);
+  }
+  if (back) {
+    p.dz = take((size_t)(p.Np * 2 * p.ld * p.np * 2));
+    // 64 rows a workgroup (the biases' partial sums stay small), fewer where that leaves CUs without one
+    p.dz_rows = 64;
+    while (p.dz_rows > 4 && (int64_t)ceil_div(p.Np, p.dz_rows) * ceil_div(p.ld, 512) < 1024) p.dz_rows /= 2;
+    while (ceil_div(p.Np, p.dz_rows) > 65535) p.dz_rows *= 2;  // a grid's second side
+    p.dz_parts = ceil_div(p.Np, p.dz_rows);
+    p.sums = take((size_t)p.dz_parts * 2 * p.ld * 4);
+    size_t part = 0;
+    if (p.dx.splits > 1) part = (size_t)p.dx.splits * p.N * p.H * 4;
+    const size_t other = p.dw.splits > 1 ? (size_t)p.dw.splits * 2 * p.ld * p.H * 4 : 0;
+    p.part = take(other > part ? other : part);
+  }
+  p.total = off;
+  return EWS_OK;
+}
+
+#define GATED_CHECK()                                            \
+  do {                                                           \
+    if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH; \
+  } while (0)
+
+struct GCall {
+  const ews_gated_desc* s;
+  GPlan p;
+  char* w;
+  hipStream_t st;
+  Operand x;
+  Operand v;
+  int64_t to_g;
+};
+
+int pack(const GCall& c, const void* src, int64_t stride, int rows, uint16_t* dst, int64_t plane) {
+  const GPlan& p = c.p;
+  tiles::PackArgs a{};
+  a.src = src;
+  a.stride = stride;
+  a.rows = rows;
+  a.cols = p.H;
+  a.dst = dst;
+  a.ld = p.Hp;
+  a.plane = plane;
+  a.dst_rows = rows;
+  a.wide = tiles::rows_wide(src, stride, p.np == 3);
+  const dim3 grid((uint32_t)((rows * (p.Hp / 8) + 255) / 256));
+  if (p.np == 3)
+    hipLaunchKernelGGL((tiles::k_pack<float>), grid, dim3(256), 0, c.st, a);
+  else
+    hipLaunchKernelGGL((tiles::k_pack<bf16>), grid, dim3(256), 0, c.st, a);
+  GATED_CHECK();
+  return EWS_OK;
+}
+
+// The operands, packed where they cannot be read as they are. want_x, want_w: those that the call reads.
+int operands(GCall& c, const void* x, const void* v, const void* g, bool want_x, bool want_w) {
+  const GPlan& p = c.p;
+  const ews_gated_desc* s = c.s;
+  c.x = Operand{(const uint16_t*)x, s->x_stride, 0, p.N, (int)p.Hp};
+  if (p.pack_x) {
+    uint16_t* to = (uint16_t*)(c.w + p.xp);
+    c.x = Operand{to, p.Hp, p.N * p.Hp, p.N, (int)p.Hp};
+    if (want_x) {
+      const int rc = pack(c, x, s->x_stride, p.N, to, c.x.plane);
+      if (rc != EWS_OK) return rc;
+    }
+  }
+  c.v = Operand{(const uint16_t*)v, s->weight_stride, 0, p.F, (int)p.Hp};
+  c.to_g = ((intptr_t)g - (intptr_t)v) / 2;
+  if (p.pack_w) {
+    uint16_t* to = (uint16_t*)(c.w + p.wp);
+    c.v = Operand{to, p.Hp, 2 * p.F * p.Hp, p.F, (int)p.Hp};
+    c.to_g = p.F * p.Hp;
+    if (want_w) {
+      int rc = pack(c, v, s->weight_stride, p.F, to, c.v.plane);
+      if (rc == EWS_OK) rc = pack(c, g, s->gate_stride, p.F, to + c.to_g, c.v.plane);
+      if (rc != EWS_OK) return rc;
+    }
+  }
+  return EWS_OK;
+}
+
+template <class T, int PAIRS, typename O>
+int launch_forward_as(const ForwardArgs& a, hipStream_t st) {
+  const int lds = tiles::lds_bytes<T, PAIRS>(a.kblocks) + T::I * 4;
+  const int rc = tiles::allow_lds(k_forward<T, PAIRS, O>, lds);
+  if (rc != EWS_OK) return rc;
+  hipLaunchKernelGGL((k_forward<T, PAIRS, O>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), lds, st, a);
+  GATED_CHECK();
+  return EWS_OK;
+}
+
+template <typename O>
+int launch_forward(Kind kind, const ForwardArgs& a, hipStream_t st) {
+  constexpr int kP = sizeof(O) == 4 ? tiles::kPairs : 1;
+  if (kind == tiles::kLarge) return launch_forward_as<tiles::Large, kP, O>(a, st);
+  return kind == tiles::kMedium ? launch_forward_as<tiles::Medium, kP, O>(a, st)
+                                : launch_forward_as<tiles::Flat, kP, O>(a, st);
+}
+
+template <typename T, bool WIDE>
+int launch_few(const FewArgs& a, hipStream_t st) {
+  const dim3 grid(ceil_div(a.F, 16)), block(64 * kFewWaves);
+  if (a.N <= 16)
+    hipLaunchKernelGGL((k_few<T, 1, WIDE>), grid, block, 0, st, a);
+  else if (a.N <= 32)
+    hipLaunchKernelGGL((k_few<T, 2, WIDE>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((k_few<T, 4, WIDE>), grid, block, 0, st, a);
+  GATED_CHECK();
+  return EWS_OK;
+}
+
+template <class T, int PAIRS, bool ROWS, typename O>
+int launch_grad_as(const GradArgs& a, hipStream_t st) {
+  const int lds = tiles::lds_bytes<T, PAIRS>(a.per);
+  const int rc = tiles::allow_lds(k_grad<T, PAIRS, ROWS, O>, lds);
+  if (rc != EWS_OK) return rc;
+  hipLaunchKernelGGL((k_grad<T, PAIRS, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), lds, st,
+                     a);
+  GATED_CHECK();
+  return EWS_OK;
+}
+
+template <bool ROWS, typename O>
+int launch_grad(const Product& p, GradArgs a, hipStream_t st) {
+  constexpr int kP = sizeof(O) == 4 ? tiles::kPairs : 1;
+  a.ti = p.ti;
+  a.tj = p.tj;
+  a.splits = p.splits;
+  a.kblocks = p.kblocks;
+  a.per = p.per;
+  int rc;
+  if (p.kind == tiles::kLarge)
+    rc = launch_grad_as<tiles::Large, kP, ROWS, O>(a, st);
+  else if (ROWS || p.kind == tiles::kMedium)  // the weights' gradients are 128 rows at least
+    rc = launch_grad_as<tiles::Medium, kP, ROWS, O>(a, st);
+  else
+    rc = launch_grad_as<tiles::Flat, kP, false, O>(a, st);
+  if (rc != EWS_OK || a.splits == 1) return rc;
+  const int64_t n = (int64_t)a.J * a.I;
+  if (a.splits > kFewSplits)
+    hipLaunchKernelGGL((k_join<ROWS, O, One, 8>), dim3((uint32_t)((n + 31) / 32)), dim3(256), 0, st, a);
+  else if (a.wide)
+    hipLaunchKernelGGL((k_join<ROWS, O, Eight, 1>), dim3((uint32_t)((n / 8 + 255) / 256)), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((k_join<ROWS, O, One, 1>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
+  GATED_CHECK();
+  return EWS_OK;
+}
+
+// Rows of results that are contiguous: whether they start at multiples of 16 bytes and hold whole eights.
+int results_wide(const void* p, int cols) { return cols % 8 == 0 && (uintptr_t)p % 16 == 0; }
+
+}  // namespace
+
+extern "C" {
+
+size_t ews_gated_kept_bytes(const ews_gated_desc* desc) {
+  GPlan p;
+  if (gated_plan(desc, nullptr, nullptr, nullptr, false, true, p) != EWS_OK) return 0;
+  return (size_t)(p.N * 2 * p.ld) * (p.np == 3 ? 4 : 2);
+}
+
+size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, const void* weight,
+                                 const void* gate_weight, int call) {
+  GPlan p;
+  if (gated_plan(desc, x, weight, gate_weight, call == EWS_GATED_BACKWARD, call == EWS_GATED_KEEP, p) != EWS_OK)
+    return 0;
+  return p.total;
+}
+
+int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile) {
+  GPlan p;
+  const int rc = gated_plan(desc, nullptr, nullptr, nullptr, true, true, p);
+  if (rc != EWS_OK) return rc;
+  if (!tile) return EWS_ERR_NULL;
+  if (product < 0 || product > 2) return EWS_ERR_OPTION;
+  const Product& q = product == 0 ? p.forward : product == 1 ? p.dx : p.dw;
+  tile[0] = q.tile_i;
+  tile[1] = q.tile_j;
+  tile[2] = q.splits;
+  return EWS_OK;
+}
+
+int ews_gated_forward(const ews_gated_desc* desc, const void* x, const void* weight, const void* bias,
+                      const void* gate_weight, const void* gate_bias, void* out, void* kept, void* workspace,
+                      ews_stream_t stream) {
+  GCall c{};
+  int rc = gated_plan(desc, x, weight, gate_weight, false, kept != nullptr, c.p);
+  if (rc != EWS_OK) return rc;
+  if (!x || !weight || !gate_weight || !out || (c.p.total && !workspace)) return EWS_ERR_NULL;
+  const bool f32 = c.p.np == 3;
+  c.s = desc;
+  c.w = (char*)workspace;
+  c.st = (hipStream_t)stream;
+  if (c.p.few) {
+    const FewArgs a{x,       weight,  gate_weight, desc->x_stride, desc->weight_stride, desc->gate_stride,
+                    c.p.N,   c.p.H,   c.p.F,       bias,           gate_bias,           desc->activation,
+                    out};
+    const bool wide = c.p.H % 8 == 0 && tiles::rows_wide(x, desc->x_stride, f32) &&
+                      tiles::rows_wide(weight, desc->weight_stride, f32) &&
+                      tiles::rows_wide(gate_weight, desc->gate_stride, f32);
+    if (f32) return wide ? launch_few<float, true>(a, c.st) : launch_few<float, false>(a, c.st);
+    return wide ? launch_few<bf16, true>(a, c.st) : launch_few<bf16, false>(a, c.st);
+  }
+  rc = operands(c, x, weight, gate_weight, true, true);
+  if (rc != EWS_OK) return rc;
+  ForwardArgs a{};
+  a.W = Pair{c.v, c.to_g};
+  a.X = c.x;
+  a.ti = c.p.forward.ti;
+  a.tj = c.p.forward.tj;
+  a.kblocks = c.p.forward.kblocks;
+  a.N = c.p.N;
+  a.F = c.p.F;
+  a.bias = bias;
+  a.gate_bias = gate_bias;
+  a.act = desc->activation;
+  a.wide = results_wide(out, c.p.F);
+  a.out = out;
+  a.kept = kept;
+  a.ld = c.p.ld;
+  return f32 ? launch_forward<float>(c.p.forward.kind, a, c.st) : launch_forward<bf16>(c.p.forward.kind, a, c.st);
+}
+
+int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* weight, const void* gate_weight,
+                       const void* kept, const void* grad_out, void* grad_x, void* grad_weight, void* grad_bias,
+                       void* grad_gate_weight, void* grad_gate_bias, void* workspace, ews_stream_t stream) {
+  GCall c{};
+  int rc = gated_plan(desc, x, weight, gate_weight, true, false, c.p);
+  if (rc != EWS_OK) return rc;
+  if (!x || !weight || !gate_weight || !kept || !grad_out || !workspace) return EWS_ERR_NULL;
+  const GPlan& p = c.p;
+  const bool f32 = p.np == 3;
+  c.s = desc;
+  c.w = (char*)workspace;
+  c.st = (hipStream_t)stream;
+  const bool weights = grad_weight || grad_gate_weight, biases = grad_bias || grad_gate_bias;
+  rc = operands(c, x, weight, gate_weight, weights, grad_x != nullptr);
+  if (rc != EWS_OK) return rc;
+  DzArgs z{};
+  z.dy = grad_out;
+  z.kept = kept;
+  z.N = p.N;
+  z.F = p.F;
+  z.padded = (int)p.Np;
+  z.ld = p.ld;
+  z.wide = results_wide(grad_out, p.F);
+  z.dz = (uint16_t*)(c.w + p.dz);
+  z.plane = p.Np * 2 * p.ld;
+  z.sums = biases ? (float*)(c.w + p.sums) : nullptr;
+  z.each = p.dz_rows;
+  const dim3 grid(ceil_div(p.ld, 512), p.dz_parts);
+  if (f32)
+    hipLaunchKernelGGL((k_dz<float>), grid, dim3(256), 0, c.st, z);
+  else
+    hipLaunchKernelGGL((k_dz<bf16>), grid, dim3(256), 0, c.st, z);
+  GATED_CHECK();
+  if (biases) {
+    const dim3 g(ceil_div(p.F, 64), 2);
+    if (f32)
+      hipLaunchKernelGGL((k_dbias<float>), g, dim3(1024), 0, c.st, z.sums, p.dz_parts, p.ld, p.F, (float*)grad_bias,
+                         (float*)grad_gate_bias);
+    else
+      hipLaunchKernelGGL((k_dbias<bf16>), g, dim3(1024), 0, c.st, z.sums, p.dz_parts, p.ld, p.F, (bf16*)grad_bias,
+                         (bf16*)grad_gate_bias);
+    GATED_CHECK();
+  }
+  GradArgs a{};
+  a.I = p.H;
+  a.F = p.F;
+  a.ld = (int)p.ld;
+  a.part = (float*)(c.w + p.part);
+  if (grad_x) {
+    a.W = Chain{c.v, c.to_g, (int)(p.ld / 64)};
+    a.Z = Operand{z.dz, 2 * p.ld, z.plane, (int)p.Np, 0};
+    a.J = p.N;
+    a.out = grad_x;
+    a.wide = results_wide(grad_x, p.H);
+    rc = f32 ? launch_grad<false, float>(p.dx, a, c.st) : launch_grad<false, bf16>(p.dx, a, c.st);
+    if (rc != EWS_OK) return rc;
+  }
+  if (weights) {
+    a.X = c.x;
+    a.Z = Operand{z.dz, 2 * p.ld, z.plane, (int)p.Np, (int)(2 * p.ld)};
+    a.J = (int)(2 * p.ld);
+    a.out = grad_weight;
+    a.gate_out = grad_gate_weight;
+    a.wide = p.H % 8 == 0 && (uintptr_t)grad_weight % 16 == 0 && (uintptr_t)grad_gate_weight % 16 == 0;
+    rc = f32 ? launch_grad<true, float>(p.dw, a, c.st) : launch_grad<true, bf16>(p.dw, a, c.st);
+    if (rc != EWS_OK) return rc;
+  }
+  return EWS_OK;
+}
+
+}  // extern "C"

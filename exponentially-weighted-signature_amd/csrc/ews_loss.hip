@@ -36,6 +36,8 @@
 #include <hip/hip_runtime.h>
 
 #include "ews_hip.h"
+#include "ews_pack.h"
+#include "ews_pick.h"
 #include "ews_tiles.h"
 #include "ews_tiles32.h"
 #include "ews_vec.h"
@@ -45,14 +47,6 @@ namespace loss {
 
 using namespace ews::vec;
 using namespace ews::tiles;
-
-typedef Tile<2, 4, 4, 2> Large;   // 256 x 256, eight wavefronts
-typedef Tile<2, 2, 2, 2> Medium;  // 128 x 128, four wavefronts
-typedef Tile<4, 1, 2, 1> Flat;    // 256 x 32, four wavefronts: few rows
-template <int BYTES>
-using Few32 = Tile32<1, BYTES>;   // 128 x 32 and 128 x 64, float32 W read as it is: few rows
-template <int BYTES>
-using More32 = Tile32<2, BYTES>;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
@@ -96,79 +90,6 @@ struct Stats {
   float* inv;     // (N) one over its sum
   float* loss;    // (N) the kept rows' losses
 };
-
-// ------------------------------------------------------------------------------------------------- rows and planes
-// The three bfloat16 planes of a float32 number, x = p0 + p1 + p2 exactly: each plane is the rest rounded to eight bits
-// (cut where rounding would reach infinity), so the second is at most 2^-8 and the third 2^-16 of x. A NaN has nothing
-// after its first plane. An infinity is (1, 0, infinity) with its sign: the third plane meets the other side's first
-// alone, which has the sign of the whole (and is 0 where it is), while the 1 meets the third plane of an infinity on
-// the other side. So infinity times w is the infinity of its sign for w other than 0, and NaN for 0, as it has to be.
-__device__ __forceinline__ float plane_value(uint16_t p) { return __uint_as_float((uint32_t)p << 16); }
-__device__ __forceinline__ void planes(float x, uint16_t (&p)[3]) {
-  const uint32_t u = __float_as_uint(x);
-  const bool finite = (u & 0x7f800000u) != 0x7f800000u;
-  p[0] = round_bf16(x);
-  if (finite && (p[0] & 0x7f80u) == 0x7f80u) p[0] = (uint16_t)(u >> 16);
-  const float b = finite ? x - plane_value(p[0]) : 0.0f;
-  p[1] = round_bf16(b);
-  p[2] = round_bf16(b - plane_value(p[1]));
-  if ((u & 0x7fffffffu) == 0x7f800000u) {
-    p[2] = p[0];
-    p[0] = (uint16_t)((u >> 16 & 0x8000u) | 0x3f80u);
-  }
-}
-__device__ __forceinline__ void planes(bf16 x, uint16_t (&p)[1]) { p[0] = x.bits; }
-
-struct PackArgs {
-  const void* src;
-  int64_t stride;
-  int rows, cols;          // of the source (rows: kept[0] where there is a map)
-  const int* map;          // gathers the rows; null: all of them
-  const int* kept;
-  uint16_t* dst;           // planes (dst_rows, ld), zero in further columns and, if any, in rows up to a multiple of 64
-  int64_t ld, plane;
-  int dst_rows;
-  int again;               // the rows are written once more from this one on; 0: once
-  int wide;
-};
-
-// A thread takes eight columns of a row; wide: rows of the source start at multiples of 16 bytes.
-template <typename T>
-__device__ __forceinline__ void pack_eight(const PackArgs& a, int64_t at) {
-  constexpr int NP = sizeof(T) == 4 ? 3 : 1;
-  const int rows = a.map ? a.kept[0] : a.rows;
-  const int padded = a.again || (rows + 63) / 64 * 64 > a.dst_rows ? a.dst_rows : (rows + 63) / 64 * 64;
-  const int packs = (int)(a.ld / 8);
-  const int64_t row = at / packs;
-  if (row >= padded) return;
-  const int c0 = (int)(at % packs) * 8;
-  const int64_t own = a.again && row >= a.again ? row - a.again : row;
-  const int n = own >= rows ? 0 : a.cols - c0 < 8 ? a.cols - c0 : 8;
-  T x[8];
-  const T* src = (const T*)a.src + (n > 0 ? (int64_t)(a.map ? a.map[own] : own) * a.stride + c0 : 0);
-  if (a.wide && n == 8) {
-#pragma unroll
-    for (int k = 0; k < 8; k += kWide<T>) *reinterpret_cast<u32x4*>(x + k) = *reinterpret_cast<const u32x4*>(src + k);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = k < n ? src[k] : narrow<T>(0.0f);
-  }
-  uint16_t p[8][NP];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) planes(x[k], p[k]);
-#pragma unroll
-  for (int q = 0; q < NP; ++q) {
-    u32x4 w;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)p[2 * k][q] | ((uint32_t)p[2 * k + 1][q] << 16);
-    *reinterpret_cast<u32x4*>(a.dst + q * a.plane + row * a.ld + c0) = w;
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_pack(PackArgs a) {
-  pack_eight<T>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
-}
 
 // ------------------------------------------------------------------------------------------------------ preparation
 struct PrepareArgs {
@@ -295,15 +216,6 @@ struct LogitArgs {
   int64_t ldp;
   Top top;
 };
-
-// A product of one stage needs no second half: more workgroups share a CU.
-template <class T, int PAIRS>
-__host__ __device__ constexpr int lds_bytes(int kblocks) {
-  if constexpr (PAIRS == 1) {
-    if (kblocks == 1) return T::kLdsBytesOne;
-  }
-  return T::kLdsBytes;
-}
 
 // PAIRS: 1, kPairs for planes, or 0 for float32 W. KEEP: 0 the loss alone, 1 also 16-bit logarithms, 2 also float32
 // probabilities. TOP: distillation.
@@ -957,9 +869,6 @@ constexpr int64_t kFewLogits32 = 1 << 22;
 // fit here. Float32 W read as it is has slabs of 32, but few rows or logits: half as much at most.
 constexpr int64_t kScoreBytes = (int64_t)256 << 20;
 
-// Stages below which a 128 x 128 tile is no slower (6 stages: 86 us for 94), its CUs better shared.
-constexpr int kLongProduct = 8;
-
 // Splits that one thread adds: two of 2000 x 256 by 32000 13 us (eight groups of lanes: 60), eight of 4095 x 512 13
 // (36).
 constexpr int kFewSplits = 8;
@@ -972,13 +881,6 @@ constexpr int kFewSplits = 8;
 // and dh takes two products a stage.
 constexpr int kFewRowsNone = 256, kFewRowsMean = 16;
 
-enum Kind { kLarge, kMedium, kFlat, kFew32, kMore32 };
-
-struct Product {
-  Kind kind;
-  int ti, tj, tile_i, tile_j, slab, splits, per, kblocks, pairs;
-};
-
 struct LPlan {
   int N, H, V, np;
   int64_t Hp, Vp, Np, chunk;
@@ -990,51 +892,6 @@ struct LPlan {
   size_t flags, token, share, entropy, first;
   size_t total;
 };
-
-size_t al256x(size_t x) { return (x + 255) & ~(size_t)255; }
-
-int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
-
-// A product of I x J results over kblocks of k: 256 x 32 tiles where J fits one; 256 x 256 ones where they give (split
-// over k, where that is allowed, into parts of 16 blocks at least) half the CUs work; else 128 x 128 ones, of which a
-// CU holds two. Measured at float32 N=4095 H=512 V=32000, dh (30 large tiles, split by 8): 0.55 ms, 0.80 ms with the
-// small. as_is: float32 W is read as it is, in k blocks of 32.
-Product pick(int64_t I, int64_t J, int kblocks, int pairs, bool split, bool as_is) {
-  Product p;
-  p.kblocks = kblocks;
-  p.pairs = pairs;
-  const int64_t large = (int64_t)ceil_div(I, 256) * ceil_div(J, 256);
-  const int parts = split ? (kblocks >= 32 ? kblocks / 16 : 1) : 1;
-  if (as_is)
-    p.kind = J <= 32 ? kFew32 : kMore32;
-  else if (J <= 32)
-    p.kind = kFlat;
-  else
-    p.kind = I > 128 && J > 128 && large * parts >= 128 && kblocks * pairs >= kLongProduct ? kLarge : kMedium;
-  const int tile_i[] = {Large::I, Medium::I, Flat::I, Few32<16>::I, More32<16>::I};
-  const int tile_j[] = {Large::J, Medium::J, Flat::J, Few32<16>::J, More32<16>::J};
-  const int slab[] = {Large::kSlab, Medium::kSlab, Flat::kSlab, Few32<16>::kSlab, More32<16>::kSlab};
-  p.slab = slab[p.kind];
-  p.tile_i = tile_i[p.kind];
-  p.tile_j = tile_j[p.kind];
-  p.ti = ceil_div(I, p.tile_i);
-  p.tj = ceil_div(J, p.tile_j);
-  p.splits = 1;
-  p.per = kblocks;
-  // one round of workgroups: a CU holds one of the large tiles, two of the others
-  const int64_t n = (int64_t)p.ti * p.tj, room = p.kind == kLarge ? 256 : as_is ? 1024 : 512;
-  if (split && 2 * n <= room) {
-    int64_t z = room / n;
-    const int64_t most = p.kind == kLarge ? parts : kblocks * pairs / 4 < kblocks ? kblocks * pairs / 4 : kblocks;
-    if (z > most) z = most;
-    if (z > 128) z = 128;  // each split's results are written and read once more
-    if (z > 1) {
-      p.per = ceil_div(kblocks, z);
-      p.splits = ceil_div(kblocks, p.per);
-    }
-  }
-  return p;
-}
 
 // entries: the teacher's of a row; 0 where the targets are tokens.
 int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p, int entries = 0) {
@@ -1154,15 +1011,6 @@ struct Call {
     if (hipGetLastError() != hipSuccess) return EWS_ERR_LAUNCH; \
   } while (0)
 
-template <class K>
-int allow_lds(K kernel, int bytes) {
-  if (bytes <= 64 << 10) return EWS_OK;  // allowed as it is
-  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                             bytes) == hipSuccess
-             ? EWS_OK
-             : EWS_ERR_LAUNCH;
-}
-
 // Whether a float32 operand can be copied 16 bytes a lane.
 bool pieces(const Operand32& o) { return (uintptr_t)o.p % 16 == 0 && o.ld % 4 == 0 && o.cols % 4 == 0; }
 
@@ -1232,10 +1080,6 @@ int launch_grad(const Product& p, const GradArgs& a, hipStream_t st) {
   }
   if (p.kind == kLarge) return launch_grad_as<Large, ROWS, O, kP>(a, st);
   return p.kind == kMedium ? launch_grad_as<Medium, ROWS, O, kP>(a, st) : launch_grad_as<Flat, ROWS, O, kP>(a, st);
-}
-
-int rows_wide(const void* p, int64_t stride, bool f32) {
-  return (uintptr_t)p % 16 == 0 && stride * (f32 ? 4 : 2) % 16 == 0;
 }
 
 // What every call begins with: the kept rows, the operands' planes, the bias.

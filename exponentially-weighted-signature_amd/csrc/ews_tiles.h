@@ -151,6 +151,12 @@ struct Copier {
   }
 };
 
+// The first operand's copier: a kernel may bring an operand of a type of its own.
+template <class O, class T, bool TURNED>
+struct CopierOf {
+  typedef Copier<TURNED, T::I, T::kThreads> type;
+};
+
 // A wavefront's fragments of one operand: BLOCKS blocks of 32 from block `first` of the tile on.
 template <bool TURNED, int WIDTH, int BLOCKS>
 struct Reader {
@@ -193,8 +199,8 @@ __device__ __forceinline__ void arrive() {
 
 // The results of the workgroup's tile at (i0, j0) over k blocks [kb0, kb1); PAIRS: 1, 2 for two planes of Q alone, or
 // kPairs for three of either. On return LDS is free.
-template <class T, int PAIRS, bool TURNED_P, bool TURNED_Q>
-__device__ __forceinline__ void product(const Operand& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
+template <class T, int PAIRS, bool TURNED_P, bool TURNED_Q, class O>
+__device__ __forceinline__ void product(const O& P, const Operand& Q, int i0, int j0, int kb0, int kb1,
                                         char* lds, f32x16 (&acc)[T::TI][T::TJ]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave % T::WI, wj = wave / T::WI;
@@ -205,7 +211,7 @@ __device__ __forceinline__ void product(const Operand& P, const Operand& Q, int 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.0f;
   if (kb0 >= kb1) return;
-  Copier<TURNED_P, T::I, T::kThreads> cp(P, i0);
+  typename CopierOf<O, T, TURNED_P>::type cp(P, i0);
   Copier<TURNED_Q, T::J, T::kThreads> cq(Q, j0);
   const int stages = (kb1 - kb0) * PAIRS;
   constexpr int kCopies = T::kCopiesP + T::kCopiesQ, kReads = T::TI + T::TJ, kProducts = T::TI * T::TJ;

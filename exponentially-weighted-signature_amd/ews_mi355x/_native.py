@@ -110,6 +110,11 @@ EXPORTED = (
     "ews_distill_keeps",
     "ews_distill_keep",
     "ews_distill_kept",
+    "ews_gated_kept_bytes",
+    "ews_gated_workspace_bytes",
+    "ews_gated_tile",
+    "ews_gated_forward",
+    "ews_gated_backward",
     "ews_gated_scan_residual_bytes",
     "ews_gated_scan_workspace_bytes",
     "ews_gated_scan_forward",
@@ -127,6 +132,11 @@ LIFT_PRESERVE = 2
 
 LOSS_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 DISTILL_MOST_ENTRIES = 1024
+
+GATED_ACTIVATIONS = {"sigmoid": 0, "silu": 1, "gelu": 2, "relu": 3}
+GATED_FORWARD = 0
+GATED_KEEP = 1
+GATED_BACKWARD = 2
 
 GATED_SCAN_FORMS = {"convex": 0, "linear": 1}
 
@@ -304,6 +314,19 @@ class DistillDesc(ctypes.Structure):
         ("index_bytes", ctypes.c_int32),
         ("logit_dtype", ctypes.c_int32),
         ("temperature", ctypes.c_float),
+    ]
+
+
+class GatedDesc(ctypes.Structure):
+    _fields_ = [
+        ("x_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("gate_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("features", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
     ]
 
 
@@ -513,6 +536,17 @@ def load():
     lib.ews_distill_keep.restype = i32
     lib.ews_distill_kept.argtypes = [dsp, vp, vp, vp, vp, vp, vp, vp]
     lib.ews_distill_kept.restype = i32
+    gdp = ctypes.POINTER(GatedDesc)
+    lib.ews_gated_kept_bytes.argtypes = [gdp]
+    lib.ews_gated_kept_bytes.restype = sz
+    lib.ews_gated_workspace_bytes.argtypes = [gdp, vp, vp, vp, i32]
+    lib.ews_gated_workspace_bytes.restype = sz
+    lib.ews_gated_tile.argtypes = [gdp, i32, ctypes.POINTER(i32)]
+    lib.ews_gated_tile.restype = i32
+    lib.ews_gated_forward.argtypes = [gdp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_gated_forward.restype = i32
+    lib.ews_gated_backward.argtypes = [gdp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_gated_backward.restype = i32
     gsp = ctypes.POINTER(GatedScanDesc)
     lib.ews_gated_scan_residual_bytes.argtypes = [gsp]
     lib.ews_gated_scan_residual_bytes.restype = sz

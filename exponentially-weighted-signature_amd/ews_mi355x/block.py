@@ -9,8 +9,8 @@ Per block (norm_placement "pre", ews/block.py:376-424):
     x        = x + Dropout(r [* sigmoid(gate(branch))])
     x        = x + Dropout(channel_stage(RMSNorm2(x)))
 
-The norms, the gate and the channel stage (plain linear maps and pointwise functions around the scan) are torch
-operations. Field names follow the reference (``norm1``, ``ewms``, ``graded``, ``c_down``, ``gate``, ``norm2``,
+The norms, the gate and the channel stages without a gate (plain linear maps and pointwise functions around the scan)
+are torch operations; gated channel stages run as ``gated_linear`` (csrc/ews_gated.hip). Field names follow the reference (``norm1``, ``ewms``, ``graded``, ``c_down``, ``gate``, ``norm2``,
 ``ff1``, ``ff2``, ``clock``, ``append_clock``, ``b_layer``), so a checkpoint converted key by key loads into the
 same places. Two differences from the reference's constructor: the generator is passed as a module (``a_param``,
 any parametrisation of ``ews_mi355x.params``; default the reference's definite_plus_skew with entries N(0, 0.005))
@@ -30,6 +30,7 @@ from torch.nn.modules import module as nn_module
 
 from .embed import embedding_lookup
 from .front import B, BlockFront, ClockSpec, make_clock
+from .gated import gated_linear, takes
 from .layer import EWS
 from .loss import linear_cross_entropy, linear_distillation, logits_cross_entropy, logits_distillation
 from .mixer import MixerEpilogue
@@ -154,6 +155,8 @@ class EWSBlock(nn.Module):
             self.mixer.c_down.weight.copy_(mixer_c.weight)
             self.mixer.c_down.bias.copy_(mixer_c.bias)
         self.gate = _linear(H, H, gen, dtype) if self.output_gate else None
+        # gated channel stages ("glu", "gelu_glu") run as gated_linear where their maps are plain; False calls the maps
+        self.fused_channel = True
         # calls that record no graph run the epilogue inside the scan's output pass where the scan allows it
         # (EWS.mixed_prefix); False keeps the scan -> epilogue composition for every call
         self.fused_epilogue = True
@@ -205,10 +208,17 @@ class EWSBlock(nn.Module):
         if self.channel_stage == "tanh":
             return torch.tanh(self.ff1(xhat))
         if self.channel_stage == "glu":
+            if self._fuses(xhat, self.ff1):
+                return gated_linear(xhat, self.ff1.weight, self.ff1.bias)
             a, b = self.ff1(xhat).chunk(2, dim=-1)
             return a * torch.sigmoid(b)
         h = F.gelu(xhat, approximate="tanh")
+        if self._fuses(h, self.ff1, self.ff2):
+            return gated_linear(h, self.ff1.weight, self.ff1.bias, self.ff2.weight, self.ff2.bias)
         return self.ff1(h) * torch.sigmoid(self.ff2(h))
+
+    def _fuses(self, x, *maps):
+        return (self.fused_channel and all(_is_plain(m, nn.Linear) and takes(x, m.weight, m.bias) for m in maps))
 
     def _drop(self, x, inference):
         if inference or self.dropout_rate == 0.0:

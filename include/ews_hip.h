@@ -746,6 +746,50 @@ int ews_gated_scan_backward(const ews_gated_scan_desc* desc, const void* x, cons
                             const void* residual, const void* grad_out, const float* grad_last, void* grad_x,
                             void* grad_gate, float* grad_state, void* workspace, ews_stream_t stream);
 
+#define EWS_GATED_SIGMOID 0
+#define EWS_GATED_SILU 1
+#define EWS_GATED_GELU 2 /* its tanh form */
+#define EWS_GATED_RELU 3
+
+#define EWS_GATED_FORWARD 0  /* a call of ews_gated_forward without kept */
+#define EWS_GATED_KEEP 1     /* one with it */
+#define EWS_GATED_BACKWARD 2
+
+typedef struct ews_gated_desc {
+  int64_t x_stride;      /* elements between rows of x, at least H */
+  int64_t weight_stride; /* of weight */
+  int64_t gate_stride;   /* of gate_weight */
+  int32_t rows;          /* N: 1..2^24 */
+  int32_t width;         /* H: 1..2^16 */
+  int32_t features;      /* F: 1..2^20 */
+  int32_t dtype;         /* EWS_DTYPE_*: of everything */
+  int32_t activation;    /* EWS_GATED_* */
+} ews_gated_desc;
+
+/* What a forward keeps for its backward: two numbers for each of out's, in its type. */
+size_t ews_gated_kept_bytes(const ews_gated_desc* desc);
+
+/* Scratch of one call (EWS_GATED_FORWARD, _KEEP or _BACKWARD) with these addresses, of which nothing is read; 0: may be
+ * NULL. Packed copies of x and the weights where they cannot be read as they are (float32; bfloat16 rows that do not
+ * start at multiples of 16 bytes or whose width is no multiple of 64), and for a backward 2 N F gradients. */
+size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, const void* weight,
+                                 const void* gate_weight, int call);
+
+/* For tests and profiles: of product 0 (v and g of a call that keeps or of many rows), 1 (grad_x) or 2 (the weights'
+ * gradients) tile[0] x tile[1] = the results of one workgroup, tile[2] = the splits of its sum. */
+int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile);
+
+/* out (N, F), contiguous, = (x weight^T + bias) act(x gate_weight^T + gate_bias); weight and gate_weight (F, H), either
+ * bias (F) may be NULL. */
+int ews_gated_forward(const ews_gated_desc* desc, const void* x, const void* weight, const void* bias,
+                      const void* gate_weight, const void* gate_bias, void* out, void* kept, void* workspace,
+                      ews_stream_t stream);
+
+/* The gradients (contiguous; each may be NULL) for out's (contiguous). */
+int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* weight, const void* gate_weight,
+                       const void* kept, const void* grad_out, void* grad_x, void* grad_weight, void* grad_bias,
+                       void* grad_gate_weight, void* grad_gate_bias, void* workspace, ews_stream_t stream);
+
 /* Human-readable text of a return code. */
 const char* ews_error_string(int code);
 
