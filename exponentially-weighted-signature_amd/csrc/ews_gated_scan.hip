@@ -33,6 +33,10 @@ namespace gscan {
 using namespace ews::vec;
 
 constexpr int kSteps = 8;           // of a thread in a tile
+#ifndef WF
+#define WF 8
+#endif
+constexpr int kWaves = WF;           // of a strip's workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Args {
@@ -133,20 +137,31 @@ __device__ __forceinline__ void fetch(Raw<T, V> (&r)[kSteps], const void* base, 
   }
 }
 
-// Bit i: step t0 + i is in the sequence (bit 8 + i: and on the mask).
-__device__ __forceinline__ uint32_t steps_on(const Args& a, int b, int t0) {
-  uint32_t on = 0;
-  const uint8_t* m = a.mask ? a.mask + b * a.mb : nullptr;
+// A thread's steps of the mask, a byte each; steps past the sequence's end are off.
+__device__ __forceinline__ uint64_t fetch_mask(const Args& a, int b, int t0) {
+  if (!a.mask) return ~0ull;
+  const uint8_t* m = a.mask + b * a.mb;
+  uint64_t w = 0;
+  if (t0 + kSteps <= a.L) {
+    __builtin_memcpy(&w, m + t0, 8);
+  } else {
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int t = t0 + i;
-    const bool in = t < a.L;
-    const bool kept = in && (!m || m[in ? t : 0] != 0);
-    on |= (in ? 1u << i : 0u) | (kept ? 256u << i : 0u);
+    for (int i = 0; i < kSteps; ++i) w |= (uint64_t)(t0 + i < a.L ? m[t0 + i] : 0) << (8 * i);
   }
-  return on;
+  return w;
 }
-static_assert(kSteps == 8, "two bits a step in one word");
+
+// Bit i: step t0 + i is in the sequence (bit 8 + i: and on the mask).
+constexpr uint32_t kWhole = 0xffffu;
+__device__ __forceinline__ uint32_t steps_on(const Args& a, uint64_t mask, int t0) {
+  const int left = a.L - t0;
+  const uint32_t in = left >= kSteps ? 0xffu : left > 0 ? (1u << left) - 1 : 0;
+  // bytes that are not 0 to their lowest bit, and those bits side by side
+  const uint64_t low = 0x7f7f7f7f7f7f7f7full;
+  const uint64_t one = (((mask & low) + low) | mask) >> 7 & 0x0101010101010101ull;
+  return in | ((uint32_t)(one * 0x0102040810204080ull >> 56) & in) << 8;
+}
+static_assert(kSteps == 8, "two bits a step in one word, a byte of the mask each in another");
 
 // (a, b) = (a2, b2) after (a, b).
 __device__ __forceinline__ void then(float& a, float& b, float a2, float b2) {
@@ -172,16 +187,18 @@ __global__ __launch_bounds__(64 * WAVES) void k_forward(Args a) {
       carry[v] = fmaf(a.ends[e], carry[v], a.ends[(int64_t)a.segs * a.B * a.D + e]);
     }
   Raw<T, V> rx[kSteps], rg[kSteps];
+  uint64_t mask;
   auto load = [&](int tile) {
     const int t0 = tile * a.tile + at.slot * kSteps;
     fetch(rx, a.x, a.xb, a.xs, at.b, at.c, t0, a.L);
     fetch(rg, a.g, a.gb, a.gs, at.b, at.c, t0, a.L);
+    mask = fetch_mask(a, at.b, t0);
   };
   load(at.first);
   for (int tile = at.first; tile < at.end; ++tile) {
     const int t0 = tile * a.tile + at.slot * kSteps;
-    const bool whole = !a.mask && (tile + 1) * a.tile <= a.L;
-    const uint32_t on = whole ? 0xffffu : steps_on(a, at.b, t0);
+    const uint32_t on = steps_on(a, mask, t0);
+    const bool whole = __all(on == kWhole);
     float ka[kSteps][V], kb[kSteps][V], A[V], H[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
@@ -276,32 +293,32 @@ __global__ __launch_bounds__(64 * WAVES) void k_backward(Args a) {
       const int64_t e = ((int64_t)s * a.B + at.b) * a.D + at.c + v;
       carry[v] = fmaf(a.ends[e], carry[v], a.ends[(int64_t)a.segs * a.B * a.D + e]);
     }
-  struct Tile {
-    Raw<T, V> x[kSteps], g[kSteps], u[kSteps];
-    float start[V];
-  } now, next;
-  auto load = [&](Tile& f, int tile) {
+  Raw<T, V> rx[kSteps], rg[kSteps], ru[kSteps];
+  uint64_t mask;
+  float start[V];
+  auto load = [&](int tile) {
     const int t0 = tile * a.tile + at.slot * kSteps;
-    fetch(f.x, a.x, a.xb, a.xs, at.b, at.c, t0, a.L);
-    fetch(f.g, a.g, a.gb, a.gs, at.b, at.c, t0, a.L);
-    if (a.dh) fetch(f.u, a.dh, (int64_t)a.L * a.D, a.D, at.b, at.c, t0, a.L);
+    fetch(rx, a.x, a.xb, a.xs, at.b, at.c, t0, a.L);
+    fetch(rg, a.g, a.gb, a.gs, at.b, at.c, t0, a.L);
+    if (a.dh) fetch(ru, a.dh, (int64_t)a.L * a.D, a.D, at.b, at.c, t0, a.L);
+    mask = fetch_mask(a, at.b, t0);
 #pragma unroll
-    for (int v = 0; v < V; ++v) f.start[v] = a.starts[((int64_t)at.b * a.tiles + tile) * a.D + at.c + v];
+    for (int v = 0; v < V; ++v) start[v] = a.starts[((int64_t)at.b * a.tiles + tile) * a.D + at.c + v];
   };
-  load(next, at.end - 1);
+  load(at.end - 1);
   for (int tile = at.end - 1; tile >= at.first; --tile) {
-    now = next;
-    if (tile > at.first) load(next, tile - 1);
     const int t0 = tile * a.tile + at.slot * kSteps;
-    const bool whole = !a.mask && (tile + 1) * a.tile <= a.L;
-    const uint32_t on = whole ? 0xffffu : steps_on(a, at.b, t0);
-    float ka[kSteps][V], take[kSteps][V], x[kSteps][V], u[kSteps][V];
+    const uint32_t on = steps_on(a, mask, t0);
+    const bool whole = __all(on == kWhole);
+    float ka[kSteps][V], take[kSteps][V], x[kSteps][V], u[kSteps][V], state[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) state[v] = start[v];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       float g[V];
-      widen_raw(now.x[i], x[i]);
-      widen_raw(now.g[i], g);
-      if (a.dh) widen_raw(now.u[i], u[i]);
+      widen_raw(rx[i], x[i]);
+      widen_raw(rg[i], g);
+      if (a.dh) widen_raw(ru[i], u[i]);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         open<CONVEX>(g[v], ka[i][v], take[i][v]);
@@ -315,10 +332,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_backward(Args a) {
         }
       }
     }
+    if (tile > at.first) load(tile - 1);
     float h[V], m[V];
     if (kAlone) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = now.start[v], m[v] = carry[v];
+      for (int v = 0; v < V; ++v) h[v] = state[v], m[v] = carry[v];
     } else {
       // A, H: the thread's steps composed; A, M: the same for m, from its last step to its first
       float A[V], H[V], M[V], B[V];
@@ -362,11 +380,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_backward(Args a) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int cell = (lane & (row - 1)) * V + v;
-        float state = now.start[v], back = carry[v];
+        float here = state[v], back = carry[v];
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-          if (w == wave) h[v] = state;
-          state = fmaf(ends[buf][w][0][cell], state, ends[buf][w][1][cell]);
+          if (w == wave) h[v] = here;
+          here = fmaf(ends[buf][w][0][cell], here, ends[buf][w][1][cell]);
         }
 #pragma unroll
         for (int w = WAVES - 1; w >= 0; --w) {
@@ -439,9 +457,9 @@ __global__ __launch_bounds__(512) void k_ends(Args a) {
     fetch(rg, a.g, a.gb, a.gs, at.b, at.c, t0, a.L);
     if (!BACK) fetch(r, a.x, a.xb, a.xs, at.b, at.c, t0, a.L);
     if (BACK && a.dh) fetch(r, a.dh, (int64_t)a.L * a.D, a.D, at.b, at.c, t0, a.L);
-    const bool whole = !a.mask && t0 + kSteps <= hi;
-    uint32_t on = whole ? 0xffffu : steps_on(a, at.b, t0);
+    uint32_t on = steps_on(a, fetch_mask(a, at.b, t0), t0);
     if (t0 + kSteps > hi) on &= ((1u << (hi - t0)) - 1) * 257u;  // steps of the next stretch
+    const bool whole = __all(on == kWhole);
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const int i = BACK ? kSteps - 1 - k : k;
@@ -518,7 +536,7 @@ int scan_plan(const ews_gated_scan_desc* s, SPlan& p) {
   } else {
     // else eight wavefronts a strip: 64 lanes wide, or 32 (a cache line of float32 or of bfloat16 pairs) where that
     // leaves CUs without one; narrower for few channels
-    p.waves = 8;
+    p.waves = kWaves;
     p.shift = (int64_t)s->batch * s_ceil(cells, 64) >= 512 ? 6 : 5;
     while (p.shift > 3 && cells <= 1 << (p.shift - 1)) --p.shift;
     p.lanes = 1 << p.shift;
@@ -581,11 +599,11 @@ int scan_launch(Args a, const SPlan& p, bool back, hipStream_t st) {
   if (back && p.waves == 1)
     hipLaunchKernelGGL((k_backward<T, V, CONVEX, 1>), grid, dim3(64), 0, st, a);
   else if (back)
-    hipLaunchKernelGGL((k_backward<T, V, CONVEX, 8>), grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((k_backward<T, V, CONVEX, kWaves>), grid, dim3(64 * kWaves), 0, st, a);
   else if (p.waves == 1)
     hipLaunchKernelGGL((k_forward<T, V, CONVEX, 1>), grid, dim3(64), 0, st, a);
   else
-    hipLaunchKernelGGL((k_forward<T, V, CONVEX, 8>), grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((k_forward<T, V, CONVEX, kWaves>), grid, dim3(64 * kWaves), 0, st, a);
   return hipGetLastError() == hipSuccess ? EWS_OK : EWS_ERR_LAUNCH;
 }
 
