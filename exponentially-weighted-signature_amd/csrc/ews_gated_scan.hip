@@ -33,10 +33,7 @@ namespace gscan {
 using namespace ews::vec;
 
 constexpr int kSteps = 8;           // of a thread in a tile
-#ifndef WF
-#define WF 8
-#endif
-constexpr int kWaves = WF;           // of a strip's workgroup
+constexpr int kWaves = 8;           // of a strip's workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Args {
@@ -511,6 +508,8 @@ namespace {
 using namespace ews::gscan;
 using ews::vec::bf16;
 
+constexpr int kFill = 192;  // workgroups that give most CUs work
+
 struct SPlan {
   int lanes, shift, waves, tile, tiles, seg_tiles, segs, pairs;  // pairs: two bfloat16 channels a thread
 };
@@ -528,16 +527,18 @@ int scan_plan(const ews_gated_scan_desc* s, SPlan& p) {
   p.pairs = s->dtype == EWS_DTYPE_BF16 && s->dim % 2 == 0 && s->x_step % 2 == 0 && s->gate_step % 2 == 0 &&
             s->x_batch % 2 == 0 && s->gate_batch % 2 == 0;
   const int cells = p.pairs ? s->dim / 2 : s->dim;  // threads that the channels need
-  // threads that walk alone: where eight wavefronts a CU can, or a sequence is but one or two of their tiles
-  if ((int64_t)s->batch * s_ceil(cells, 64) >= 2048 || s->length <= 2 * kSteps) {
+  // threads that walk alone: where sixteen wavefronts a CU can (bfloat16 64 x 512 x 4096 both ways: 437 us, by strips
+  // 455; half as many wavefronts: 510, by strips 456), or a sequence is but one or two of their tiles
+  if ((int64_t)s->batch * s_ceil(cells, 64) >= 4096 || s->length <= 2 * kSteps) {
     p.waves = 1;
     p.lanes = 64;
     p.shift = 6;
   } else {
-    // else eight wavefronts a strip: 64 lanes wide, or 32 (a cache line of float32 or of bfloat16 pairs) where that
-    // leaves CUs without one; narrower for few channels
+    // else eight wavefronts a strip: 64 lanes wide (8 x 2048 x 4096: 231 us, with 32 lanes 242), or 32, a cache line
+    // of float32 or of bfloat16 pairs, where those fill the CUs and the wider ones do not
     p.waves = kWaves;
-    p.shift = (int64_t)s->batch * s_ceil(cells, 64) >= 512 ? 6 : 5;
+    const int64_t wide = (int64_t)s->batch * s_ceil(cells, 64), narrow = (int64_t)s->batch * s_ceil(cells, 32);
+    p.shift = wide < kFill && narrow >= kFill ? 5 : 6;
     while (p.shift > 3 && cells <= 1 << (p.shift - 1)) --p.shift;
     p.lanes = 1 << p.shift;
   }
@@ -546,7 +547,7 @@ int scan_plan(const ews_gated_scan_desc* s, SPlan& p) {
   p.segs = 1;
   p.seg_tiles = p.tiles;
   const int64_t groups = (int64_t)s->batch * s_ceil(cells, p.lanes);
-  if (p.waves > 1 && groups < 192) {
+  if (p.waves > 1 && groups < kFill) {  // segments: two workgroups a CU
     int64_t z = 512 / groups;
     if (z > p.tiles / 2) z = p.tiles / 2;  // each reads x and g once more
     if (z > 1) {
@@ -555,7 +556,7 @@ int scan_plan(const ews_gated_scan_desc* s, SPlan& p) {
     }
   }
   const int64_t blocks = (int64_t)s->batch * s_ceil(s->dim, p.lanes) * p.segs;
-  if (blocks > 1 << 24) return EWS_ERR_SHAPE;
+  if (blocks > 1 << 25) return EWS_ERR_SHAPE;
   return EWS_OK;
 }
 

@@ -54,9 +54,11 @@ def _check(x, gate, state, mask, form, dh, dlast, forward_only=False):
 @pytest.mark.parametrize("B,L,D", [
     (1, 1, 1), (8, 1, 2048), (3, 2, 5), (2, 16, 70), (2, 17, 70), (1, 17, 1), (2, 129, 8), (3, 200, 9), (2, 257, 16),
     (1, 300, 24), (2, 127, 33), (2, 128, 64), (1, 513, 130),
-    (256, 33, 520),    # alone: 2304 wavefronts of float32
-    (256, 20, 1040),   # alone in bfloat16 pairs too
+    (600, 17, 450),    # alone: 4800 wavefronts of float32
+    (1100, 18, 500),   # alone in bfloat16 pairs too
     (128, 40, 516),    # 64 lanes
+    (12, 260, 516),    # 32 lanes of float32
+    (24, 260, 516),    # 32 lanes of bfloat16 pairs
     (1, 2100, 3),      # segments
     (2, 4099, 40),
 ])
@@ -71,7 +73,7 @@ def _args(inputs, form):
 
 @pytest.mark.parametrize("mask", ["tail", "holes", "none"])
 @pytest.mark.parametrize("form", ["convex", "linear"])
-@pytest.mark.parametrize("B,L,D", [(3, 9, 70), (2, 130, 24), (2, 2050, 12), (260, 20, 512)])
+@pytest.mark.parametrize("B,L,D", [(3, 9, 70), (2, 130, 24), (2, 2050, 12), (600, 20, 450)])
 def test_masks(B, L, D, form, mask):
     x, gate, state, m, dh, dlast = _inputs(B, L, D, torch.float32, form, mask=mask)
     _check(x, gate, state, m, form, dh, dlast)
