@@ -9,10 +9,11 @@
 // Three pairs of products of 2 N H F operations each bound all but the smallest calls; they run on the matrix cores
 // (ews_tiles.h). v and g of the same output meet in a wavefront's registers: a tile's first operand is interleaved, half
 // of every wavefront's rows from V and half from G, which costs nothing, as the copies to LDS can start anywhere. So y is
-// formed where the sums end, and v and g are never in memory. A training call writes act(g) and v act'(g) in x's type
-// beside y, what the backward multiplies dy with: each is rounded once, relative to itself (v and g rounded in their place
-// would be cheaper by nothing, and g's rounding would be multiplied by |g|). k_dz forms dv | dg from them, one after the
-// other along a row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows.
+// formed where the sums end, and v and g are never in memory. A training call also writes act(g) and v act'(g), what the
+// backward multiplies dy with: float32 as it is, for bfloat16 x its upper 24 bits (dv and dg are rounded to bfloat16
+// afterwards, and a second rounding of that size before it makes the gradients 1.7 times as far off as their own rounding
+// alone, where one makes 1.4; 16 bits would save 3% of a call). k_dz forms dv | dg from them, one after the other along a
+// row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows.
 //
 // Few rows (decoding) are bound by V and G's bytes: k_few reads them straight into the matrix instructions' registers,
 // many loads on their way at once, without LDS.
@@ -139,6 +140,73 @@ struct CopierOf<gated::Chain, T, true> {
 
 namespace gated {
 
+// x, V and G laid out in one launch, those of them that have to be.
+struct Packs {
+  PackArgs each[3];
+  uint32_t from[3];  // first workgroups
+  uint32_t blocks;
+  int count;
+  void add(const PackArgs& a) {
+    from[count] = blocks;
+    each[count++] = a;
+    blocks += (uint32_t)((a.rows * (a.ld / 8) + 255) / 256);
+  }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_packs(Packs a) {
+#pragma unroll
+  for (int k = 2; k >= 0; --k)
+    if (k < a.count && blockIdx.x >= a.from[k])
+      return pack_eight<T>(a.each[k], (int64_t)(blockIdx.x - a.from[k]) * 256 + threadIdx.x);
+}
+
+// ---------------------------------------------------------------------------------------------- what a forward keeps
+// Numbers that a forward keeps: float32, or for bfloat16 the upper 24 bits of float32, rounded, as 16 and 8 of them in
+// two arrays one after the other. (No NaN that bfloat16 inputs give has the low bits that rounding would carry out of.)
+template <typename O>
+struct Kept {
+  static __device__ __forceinline__ void store(void* kept, int64_t, int64_t at, const Eight& e) {
+    float* to = (float*)kept + at;
+    __builtin_nontemporal_store(f32x4{e.x[0], e.x[1], e.x[2], e.x[3]}, reinterpret_cast<f32x4*>(to));
+    __builtin_nontemporal_store(f32x4{e.x[4], e.x[5], e.x[6], e.x[7]}, reinterpret_cast<f32x4*>(to + 4));
+  }
+  static __device__ __forceinline__ void load(const void* kept, int64_t, int64_t at, float (&x)[8]) {
+    const float* from = (const float*)kept + at;
+#pragma unroll
+    for (int q = 0; q < 8; q += 4) {
+      const f32x4 w = *reinterpret_cast<const f32x4*>(from + q);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[q + k] = w[k];
+    }
+  }
+};
+template <>
+struct Kept<bf16> {
+  static __device__ __forceinline__ void store(void* kept, int64_t count, int64_t at, const Eight& e) {
+    u32x4 hi;
+    u32x2 lo;
+#pragma unroll
+    for (int q = 0; q < 8; q += 2) {
+      const uint32_t a = __float_as_uint(e.x[q]) + 0x80u, b = __float_as_uint(e.x[q + 1]) + 0x80u;
+      hi[q / 2] = (a >> 16) | (b & 0xffff0000u);
+      const uint32_t two = ((a >> 8) & 0xffu) | (b & 0xff00u);
+      lo[q / 4] = q % 4 ? lo[q / 4] | two << 16 : two;
+    }
+    __builtin_nontemporal_store(hi, reinterpret_cast<u32x4*>((uint16_t*)kept + at));
+    __builtin_nontemporal_store(lo, reinterpret_cast<u32x2*>((uint8_t*)kept + 2 * count + at));
+  }
+  static __device__ __forceinline__ void load(const void* kept, int64_t count, int64_t at, float (&x)[8]) {
+    const u32x4 hi = *reinterpret_cast<const u32x4*>((const uint16_t*)kept + at);
+    const u32x2 lo = *reinterpret_cast<const u32x2*>((const uint8_t*)kept + 2 * count + at);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t h = q % 2 ? hi[q / 2] & 0xffff0000u : hi[q / 2] << 16;
+      x[q] = __uint_as_float(h | ((lo[q / 4] >> (8 * (q % 4))) & 0xffu) << 8);
+    }
+  }
+};
+
 // ------------------------------------------------------------------------------------------------------- the forward
 struct ForwardArgs {
   Pair W;
@@ -150,7 +218,7 @@ struct ForwardArgs {
   int act;
   int wide;                // rows of out start at multiples of 16 bytes and hold whole eights
   void* out;               // (N, F)
-  void* kept;              // (N, 2 ld): act(g) | v act'(g); or null
+  void* kept;              // (N, 2 ld): act(g) | v act'(g); or null (Kept)
   int64_t ld;              // F up to a multiple of 64
 };
 
@@ -252,11 +320,11 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_forward(ForwardArgs 
     // whole eights up to ld: what lies past F is not read
     rows_of_half<T, Eight>(lds, p, [&](int row, int col, const Eight& e) {
       if (row0 + row < a.N && col0 + col < a.ld)
-        store<O>((O*)a.kept + (int64_t)(row0 + row) * 2 * a.ld + col0 + col, e);
+        Kept<O>::store(a.kept, 2 * a.ld * a.N, (int64_t)(row0 + row) * 2 * a.ld + col0 + col, e);
     });
     rows_of_half<T, Eight>(lds, q, [&](int row, int col, const Eight& e) {
       if (row0 + row < a.N && col0 + col < a.ld)
-        store<O>((O*)a.kept + (int64_t)(row0 + row) * 2 * a.ld + a.ld + col0 + col, e);
+        Kept<O>::store(a.kept, 2 * a.ld * a.N, (int64_t)(row0 + row) * 2 * a.ld + a.ld + col0 + col, e);
     });
   }
 }
@@ -435,14 +503,9 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) z[q] = 0.0f;
       if (live) {
-        const T* kept = (const T*)a.kept + ((int64_t)row * 2 + side) * a.ld + f;
+        Kept<T>::load(a.kept, 2 * a.ld * a.N, ((int64_t)row * 2 + side) * a.ld + f, z);
 #pragma unroll
-        for (int q = 0; q < 8; q += kWide<T>) {
-          Pack<T, kWide<T>> p;
-          p.load(kept + q);
-#pragma unroll
-          for (int e = 0; e < kWide<T>; ++e) z[q + e] = q + e < live ? u[q + e] * p.get(e) : 0.0f;
-        }
+        for (int q = 0; q < 8; ++q) z[q] = q < live ? u[q] * z[q] : 0.0f;
       }
       uint16_t p[8][NP];
 #pragma unroll
@@ -501,9 +564,10 @@ struct GradArgs {
   Operand X;               // dV | dG: k along the rows
   Operand Z;               // dv | dg
   int ti, tj, splits, kblocks, per;
+  int whole, pieces;       // tiles done by a workgroup each; workgroups that share each of the others
   int I, J;                // results along H; rows of dx, or 2 ld of dV | dG
   int F, ld;               // dV | dG: those of the J that are V's and G's
-  float* part;             // (splits, J, I) where splits > 1
+  float* part;             // (splits, J, I) where splits > 1; or the shared tiles' pieces, (tiles, pieces, tile)
   void* out;               // dx or dV
   void* gate_out;          // dG
   int wide;                // results' rows start at multiples of 16 bytes and hold whole eights
@@ -529,10 +593,14 @@ __device__ __forceinline__ void keep(float* to, const One& e) { *to = e.x; }
 template <class T, int PAIRS, bool ROWS, typename O>
 __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_grad(GradArgs a) {
   extern __shared__ char lds[];
+  const bool shared = (int)blockIdx.x >= a.whole;
+  const int other = blockIdx.x - a.whole;
+  const int split = shared ? other % a.pieces : blockIdx.y;
   int it, jt;
-  tile_of(blockIdx.x, a.ti, a.tj, it, jt);
-  const int i0 = it * T::I, j0 = jt * T::J, split = blockIdx.y;
-  const int kb0 = split * a.per, kb1 = kb0 + a.per < a.kblocks ? kb0 + a.per : a.kblocks;
+  tile_of(shared ? a.whole + other / a.pieces : blockIdx.x, a.ti, a.tj, it, jt);
+  const int i0 = it * T::I, j0 = jt * T::J;
+  const int per = shared ? (a.kblocks + a.pieces - 1) / a.pieces : a.per;
+  const int kb0 = split * per, kb1 = kb0 + per < a.kblocks ? kb0 + per : a.kblocks;
   f32x16 acc[T::TI][T::TJ];
   if constexpr (ROWS)
     product<T, PAIRS, true, true>(a.X, a.Z, i0, j0, kb0, kb1, lds, acc);
@@ -543,6 +611,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_grad(GradArgs a) {
 #pragma unroll
     for (int b = 0; b < T::TJ; ++b)
       rows_of<T, W>(lds, acc, b, [&](int jrow, int icol, const W& e) {
+        if (shared) return keep(a.part + (int64_t)other * T::I * T::J + jrow * T::I + icol, e);
         const int j = j0 + jrow, i = i0 + icol;
         if (j >= a.J || i >= a.I) return;
         if (a.splits > 1) return keep(a.part + ((int64_t)split * a.J + j) * a.I + i, e);
@@ -554,6 +623,30 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_grad(GradArgs a) {
     rows(Eight{});
   else
     rows(One{});
+}
+
+// The shared tiles' pieces added in order: 1024 results a workgroup.
+template <class T, bool ROWS, typename O, typename W>
+__global__ __launch_bounds__(1024 / (sizeof(W) / 4)) void k_shared(GradArgs a) {
+  constexpr int kEach = sizeof(W) / 4, kOf = T::I * T::J / 1024;
+  const int t = blockIdx.x / kOf, at = (blockIdx.x % kOf) * 1024 + threadIdx.x * kEach;
+  int it, jt;
+  tile_of(a.whole + t, a.ti, a.tj, it, jt);
+  const int j = jt * T::J + at / T::I, i = it * T::I + at % T::I;
+  if (j >= a.J || i >= a.I) return;
+  O* to = result_row<ROWS, O>(a, j);
+  if (!to) return;
+  float x[kEach];
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) x[q] = 0.0f;
+  for (int s = 0; s < a.pieces; ++s) {
+    const float* from = a.part + ((int64_t)t * a.pieces + s) * T::I * T::J + at;
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) x[q] += from[q];
+  }
+  W w;
+  __builtin_memcpy(&w, x, sizeof(w));
+  store<O>(to + i, w);
 }
 
 // The splits' results added in order, by GROUPS groups of a workgroup's threads a contiguous part of them each; a thread
@@ -620,11 +713,42 @@ constexpr int kFewRows = 64;
 // Splits that one thread adds; more are added by eight groups of threads.
 constexpr int kFewSplits = 8;
 
+// A product whose tiles of the last, mostly empty round of workgroups are shared out along k.
+struct GProduct : Product {
+  int whole, pieces;
+  size_t part_bytes(int64_t I, int64_t J) const {
+    const int64_t others = (int64_t)ti * tj - whole;
+    if (others) return (size_t)(others * pieces * tile_i * tile_j * 4);
+    return splits > 1 ? (size_t)(splits * I * J * 4) : 0;
+  }
+};
+
+// 256 large tiles are a round, one a CU. The last round's tiles are shared by two to four workgroups each where that
+// shortens it by a quarter at least: 11008 x 2048 results (344 tiles) over 8192 rows 415 us, shared 361.
+GProduct share(const Product& of) {
+  GProduct p;
+  static_cast<Product&>(p) = of;
+  const int n = p.ti * p.tj, others = n % 256;
+  p.whole = n;
+  p.pieces = 1;
+  if (p.kind != tiles::kLarge || p.splits > 1 || n < 256 || others == 0 || p.kblocks < 64) return p;
+  double best = 0.75;  // of a round
+  for (int z = 2; z <= 4; ++z) {
+    const double took = (double)ceil_div(others * z, 256) / z;
+    if (took >= best) continue;
+    best = took;
+    p.whole = n - others;
+    p.pieces = z;
+  }
+  return p;
+}
+
 struct GPlan {
   int N, H, F, np;
   int64_t Hp, ld, Np;
   bool pack_x, pack_w, few;
-  Product forward, dx, dw;
+  Product forward;
+  GProduct dx, dw;
   int dz_rows, dz_parts;
   size_t xp, wp, dz, sums, part, total;
 };
@@ -649,7 +773,7 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
   p.ld = (int64_t)ceil_div(p.F, 64) * 64;
   p.Np = (int64_t)ceil_div(p.N, 64) * 64;
   // a launch has fewer than 2^32 threads, one for eight numbers; dv | dg's rows lie within the tiles' offsets
-  if (p.Np * p.Hp > (int64_t)1 << 34 || p.F * p.Hp > (int64_t)1 << 34 || p.Np * p.ld > (int64_t)1 << 34)
+  if (p.Np * p.Hp > (int64_t)1 << 33 || p.F * p.Hp > (int64_t)1 << 33 || p.Np * p.ld > (int64_t)1 << 34)
     return EWS_ERR_SHAPE;
   p.few = !back && !keep && p.N <= kFewRows;
   p.pack_x = p.np == 3 || !direct(x, s->x_stride, p.H);
@@ -657,8 +781,8 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
              s->weight_stride != s->gate_stride || ((uintptr_t)g - (uintptr_t)v) % 2;
   const int pairs = p.np == 3 ? tiles::kPairs : 1;
   p.forward = tiles::pick(2 * p.ld, p.N, (int)(p.Hp / 64), pairs, false, false);
-  p.dx = tiles::pick(p.H, p.N, (int)(2 * p.ld / 64), pairs, true, false);
-  p.dw = tiles::pick(p.H, 2 * p.ld, (int)(p.Np / 64), pairs, true, false);
+  p.dx = share(tiles::pick(p.H, p.N, (int)(2 * p.ld / 64), pairs, true, false));
+  p.dw = share(tiles::pick(p.H, 2 * p.ld, (int)(p.Np / 64), pairs, true, false));
   size_t off = 0;
   auto take = [&off](size_t bytes) {
     const size_t at = off;
@@ -677,10 +801,8 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
     while (ceil_div(p.Np, p.dz_rows) > 65535) p.dz_rows *= 2;  // a grid's second side
     p.dz_parts = ceil_div(p.Np, p.dz_rows);
     p.sums = take((size_t)p.dz_parts * 2 * p.ld * 4);
-    size_t part = 0;
-    if (p.dx.splits > 1) part = (size_t)p.dx.splits * p.N * p.H * 4;
-    const size_t other = p.dw.splits > 1 ? (size_t)p.dw.splits * 2 * p.ld * p.H * 4 : 0;
-    p.part = take(other > part ? other : part);
+    const size_t dx = p.dx.part_bytes(p.H, p.N), dw = p.dw.part_bytes(p.H, 2 * p.ld);
+    p.part = take(dx > dw ? dx : dw);
   }
   p.total = off;
   return EWS_OK;
@@ -701,8 +823,7 @@ struct GCall {
   int64_t to_g;
 };
 
-int pack(const GCall& c, const void* src, int64_t stride, int rows, uint16_t* dst, int64_t plane) {
-  const GPlan& p = c.p;
+tiles::PackArgs pack_args(const GPlan& p, const void* src, int64_t stride, int rows, uint16_t* dst, int64_t plane) {
   tiles::PackArgs a{};
   a.src = src;
   a.stride = stride;
@@ -713,27 +834,19 @@ int pack(const GCall& c, const void* src, int64_t stride, int rows, uint16_t* ds
   a.plane = plane;
   a.dst_rows = rows;
   a.wide = tiles::rows_wide(src, stride, p.np == 3);
-  const dim3 grid((uint32_t)((rows * (p.Hp / 8) + 255) / 256));
-  if (p.np == 3)
-    hipLaunchKernelGGL((tiles::k_pack<float>), grid, dim3(256), 0, c.st, a);
-  else
-    hipLaunchKernelGGL((tiles::k_pack<bf16>), grid, dim3(256), 0, c.st, a);
-  GATED_CHECK();
-  return EWS_OK;
+  return a;
 }
 
 // The operands, packed where they cannot be read as they are. want_x, want_w: those that the call reads.
 int operands(GCall& c, const void* x, const void* v, const void* g, bool want_x, bool want_w) {
   const GPlan& p = c.p;
   const ews_gated_desc* s = c.s;
+  Packs a{};
   c.x = Operand{(const uint16_t*)x, s->x_stride, 0, p.N, (int)p.Hp};
   if (p.pack_x) {
     uint16_t* to = (uint16_t*)(c.w + p.xp);
     c.x = Operand{to, p.Hp, p.N * p.Hp, p.N, (int)p.Hp};
-    if (want_x) {
-      const int rc = pack(c, x, s->x_stride, p.N, to, c.x.plane);
-      if (rc != EWS_OK) return rc;
-    }
+    if (want_x) a.add(pack_args(p, x, s->x_stride, p.N, to, c.x.plane));
   }
   c.v = Operand{(const uint16_t*)v, s->weight_stride, 0, p.F, (int)p.Hp};
   c.to_g = ((intptr_t)g - (intptr_t)v) / 2;
@@ -742,11 +855,16 @@ int operands(GCall& c, const void* x, const void* v, const void* g, bool want_x,
     c.v = Operand{to, p.Hp, 2 * p.F * p.Hp, p.F, (int)p.Hp};
     c.to_g = p.F * p.Hp;
     if (want_w) {
-      int rc = pack(c, v, s->weight_stride, p.F, to, c.v.plane);
-      if (rc == EWS_OK) rc = pack(c, g, s->gate_stride, p.F, to + c.to_g, c.v.plane);
-      if (rc != EWS_OK) return rc;
+      a.add(pack_args(p, v, s->weight_stride, p.F, to, c.v.plane));
+      a.add(pack_args(p, g, s->gate_stride, p.F, to + c.to_g, c.v.plane));
     }
   }
+  if (!a.blocks) return EWS_OK;
+  if (p.np == 3)
+    hipLaunchKernelGGL((k_packs<float>), dim3(a.blocks), dim3(256), 0, c.st, a);
+  else
+    hipLaunchKernelGGL((k_packs<bf16>), dim3(a.blocks), dim3(256), 0, c.st, a);
+  GATED_CHECK();
   return EWS_OK;
 }
 
@@ -786,20 +904,32 @@ int launch_grad_as(const GradArgs& a, hipStream_t st) {
   const int lds = tiles::lds_bytes<T, PAIRS>(a.per);
   const int rc = tiles::allow_lds(k_grad<T, PAIRS, ROWS, O>, lds);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_grad<T, PAIRS, ROWS, O>), dim3((uint32_t)(a.ti * a.tj), a.splits), dim3(T::kThreads), lds, st,
-                     a);
+  const int others = a.ti * a.tj - a.whole;
+  hipLaunchKernelGGL((k_grad<T, PAIRS, ROWS, O>), dim3((uint32_t)(a.whole + others * a.pieces), a.splits),
+                     dim3(T::kThreads), lds, st, a);
   GATED_CHECK();
+  if constexpr (T::I == 256 && T::J == 256) {
+    if (!others) return EWS_OK;
+    const dim3 grid((uint32_t)(others * (T::I * T::J / 1024)));
+    if (a.wide)
+      hipLaunchKernelGGL((k_shared<T, ROWS, O, Eight>), grid, dim3(128), 0, st, a);
+    else
+      hipLaunchKernelGGL((k_shared<T, ROWS, O, One>), grid, dim3(1024), 0, st, a);
+    GATED_CHECK();
+  }
   return EWS_OK;
 }
 
 template <bool ROWS, typename O>
-int launch_grad(const Product& p, GradArgs a, hipStream_t st) {
+int launch_grad(const GProduct& p, GradArgs a, hipStream_t st) {
   constexpr int kP = sizeof(O) == 4 ? tiles::kPairs : 1;
   a.ti = p.ti;
   a.tj = p.tj;
   a.splits = p.splits;
   a.kblocks = p.kblocks;
   a.per = p.per;
+  a.whole = p.whole;
+  a.pieces = p.pieces;
   int rc;
   if (p.kind == tiles::kLarge)
     rc = launch_grad_as<tiles::Large, kP, ROWS, O>(a, st);
@@ -829,7 +959,7 @@ extern "C" {
 size_t ews_gated_kept_bytes(const ews_gated_desc* desc) {
   GPlan p;
   if (gated_plan(desc, nullptr, nullptr, nullptr, false, true, p) != EWS_OK) return 0;
-  return (size_t)(p.N * 2 * p.ld) * (p.np == 3 ? 4 : 2);
+  return (size_t)(p.N * 2 * p.ld) * (p.np == 3 ? 4 : 3);
 }
 
 size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, const void* weight,
@@ -846,10 +976,12 @@ int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile) {
   if (rc != EWS_OK) return rc;
   if (!tile) return EWS_ERR_NULL;
   if (product < 0 || product > 2) return EWS_ERR_OPTION;
-  const Product& q = product == 0 ? p.forward : product == 1 ? p.dx : p.dw;
+  const Product& q = product == 0 ? p.forward : product == 1 ? p.dx : static_cast<const Product&>(p.dw);
   tile[0] = q.tile_i;
   tile[1] = q.tile_j;
   tile[2] = q.splits;
+  tile[3] = product == 0 ? q.ti * q.tj : product == 1 ? p.dx.whole : p.dw.whole;
+  tile[4] = q.ti * q.tj;
   return EWS_OK;
 }
 

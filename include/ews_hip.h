@@ -766,7 +766,7 @@ typedef struct ews_gated_desc {
   int32_t activation;    /* EWS_GATED_* */
 } ews_gated_desc;
 
-/* What a forward keeps for its backward: two numbers for each of out's, in its type. */
+/* What a forward keeps for its backward: two numbers for each of out's, of 24 bits (float32: 32). */
 size_t ews_gated_kept_bytes(const ews_gated_desc* desc);
 
 /* Scratch of one call (EWS_GATED_FORWARD, _KEEP or _BACKWARD) with these addresses, of which nothing is read; 0: may be
@@ -776,7 +776,8 @@ size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, cons
                                  const void* gate_weight, int call);
 
 /* For tests and profiles: of product 0 (v and g of a call that keeps or of many rows), 1 (grad_x) or 2 (the weights'
- * gradients) tile[0] x tile[1] = the results of one workgroup, tile[2] = the splits of its sum. */
+ * gradients) tile[0] x tile[1] = the results of one workgroup, tile[2] = the splits of its sum, and tile[3] of the
+ * tile[4] tiles are done by a workgroup each, the others shared by several. */
 int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile);
 
 /* out (N, F), contiguous, = (x weight^T + bias) act(x gate_weight^T + gate_bias); weight and gate_weight (F, H), either

@@ -63,7 +63,7 @@ def test_tiles(case):
     name, N, H, F = case
     d = _desc(rows=N, width=H, features=F, x_stride=H, weight_stride=H, gate_stride=H,
               dtype=nat.DTYPE_F32 if name == "float32" else nat.DTYPE_BF16)
-    tile = (ctypes.c_int32 * 3)()
+    tile = (ctypes.c_int32 * 5)()
     for product, want in enumerate(TILES[case]):
         assert nat.load().ews_gated_tile(d, product, tile) == 0
         assert tuple(tile[:2]) == want, product
