@@ -15,6 +15,8 @@
 // alone, where one makes 1.4; 16 bits would save 3% of a call). k_dz forms dv | dg from them, one after the other along a
 // row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows.
 //
+// Narrow maps (both widths up to 64) have kernels of their own (ews_gated_narrow.h), and keep nothing.
+//
 // Few rows (decoding) are bound by V and G's bytes: k_few reads them straight into the matrix instructions' registers,
 // many loads on their way at once, without LDS.
 //
@@ -64,6 +66,14 @@ __device__ __forceinline__ void activate(int kind, float g, float& act, float& s
   act = kind == EWS_GATED_SILU ? g * p : p;
   slope = kind == EWS_GATED_SILU ? fmaf(g * p, q, p) : p * q;
 }
+
+}  // namespace gated
+}  // namespace ews
+
+#include "ews_gated_narrow.h"
+
+namespace ews {
+namespace gated {
 
 // ------------------------------------------------------------------------------------------------------ the operands
 // V and G as a tile's first operand: of every wavefront's blocks of 32 rows the first half are V's, the others the same
@@ -342,50 +352,6 @@ struct FewArgs {
   void* out;
 };
 
-typedef float f32x4v __attribute__((ext_vector_type(4)));
-
-// Eight neighbouring numbers of a row from column k on, zero past the row's end.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void eight(const T* row, int k, int H, T (&x)[8]) {
-  if (WIDE) {  // H is a multiple of 8 then
-    if (k < H) {
-#pragma unroll
-      for (int q = 0; q < 8; q += kWide<T>) *reinterpret_cast<u32x4*>(x + q) = *reinterpret_cast<const u32x4*>(row + k + q);
-    } else {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) x[q] = narrow<T>(0.0f);
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) x[q] = k + q < H ? row[k + q] : narrow<T>(0.0f);
-  }
-}
-
-template <typename T>
-constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
-
-template <typename T>
-__device__ __forceinline__ void fragments(const T (&x)[8], bf16x8 (&f)[kPlanes<T>]) {
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    uint16_t p[kPlanes<T>];
-    planes(x[q], p);
-#pragma unroll
-    for (int n = 0; n < kPlanes<T>; ++n) f[n][q] = __builtin_bit_cast(__bf16, p[n]);
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void multiply(const bf16x8 (&p)[kPlanes<T>], const bf16x8 (&q)[kPlanes<T>], f32x4v& acc) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int pair = 0; pair < kPairs; ++pair)
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[piece_p(pair)], q[piece_q(pair)], acc, 0, 0, 0);
-  } else {
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[0], q[0], acc, 0, 0, 0);
-  }
-}
-
 constexpr int kFewWaves = 4;
 
 // 16 outputs of up to 16 COLS rows a workgroup; its wavefronts take every fourth 32 AHEAD of k and are joined in LDS.
@@ -408,8 +374,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
     T wv[kAhead][8], wg[kAhead][8];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
-      eight<T, WIDE>(v, k0 + 32 * s + k8, a.H, wv[s]);
-      eight<T, WIDE>(g, k0 + 32 * s + k8, a.H, wg[s]);
+      eight_of<T>(v, k0 + 32 * s + k8, a.H, WIDE, wv[s]);
+      eight_of<T>(g, k0 + 32 * s + k8, a.H, WIDE, wg[s]);
     }
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
@@ -421,10 +387,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
         const int n = c * 16 + r16 < a.N ? c * 16 + r16 : a.N - 1;
         T x[8];
         bf16x8 fx[kPlanes<T>];
-        eight<T, WIDE>((const T*)a.x + n * a.xs, k0 + 32 * s + k8, a.H, x);
+        eight_of<T>((const T*)a.x + n * a.xs, k0 + 32 * s + k8, a.H, WIDE, x);
         fragments<T>(x, fx);
-        multiply<T>(fv, fx, accv[c]);
-        multiply<T>(fg, fx, accg[c]);
+        mac(fv, fx, accv[c]);
+        mac(fg, fx, accg[c]);
       }
     }
   }
@@ -746,12 +712,14 @@ GProduct share(const Product& of) {
 struct GPlan {
   int N, H, F, np;
   int64_t Hp, ld, Np;
-  bool pack_x, pack_w, few;
+  bool pack_x, pack_w, few, narrow;
   Product forward;
   GProduct dx, dw;
-  int dz_rows, dz_parts;
+  int dz_rows, dz_parts, narrow_groups;
   size_t xp, wp, dz, sums, part, total;
 };
+
+int narrow_pad(int n) { return n <= 32 ? 32 : 64; }
 
 bool direct(const void* p, int64_t stride, int H) {
   return H % 64 == 0 && stride % 8 == 0 && stride <= 1 << 22 && (uintptr_t)p % 16 == 0;
@@ -776,6 +744,15 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
   if (p.Np * p.Hp > (int64_t)1 << 33 || p.F * p.Hp > (int64_t)1 << 33 || p.Np * p.ld > (int64_t)1 << 34)
     return EWS_ERR_SHAPE;
   p.few = !back && !keep && p.N <= kFewRows;
+  p.narrow = p.H <= kNarrowWidth && p.F <= kNarrowWidth && !p.few;
+  if (p.narrow) {
+    // 32 rows a wavefront and turn; as many workgroups as are on the CUs at a time
+    const int groups = ceil_div(p.N, 32 * 4);
+    p.narrow_groups = groups < 512 ? groups : 512;
+    p.part = 0;
+    p.total = back ? (size_t)p.narrow_groups * 2 * narrow_pad(p.F) * (narrow_pad(p.H) + 1) * 4 : 0;
+    return EWS_OK;
+  }
   p.pack_x = p.np == 3 || !direct(x, s->x_stride, p.H);
   p.pack_w = p.np == 3 || !direct(v, s->weight_stride, p.H) || !direct(g, s->gate_stride, p.H) ||
              s->weight_stride != s->gate_stride || ((uintptr_t)g - (uintptr_t)v) % 2;
@@ -949,6 +926,52 @@ int launch_grad(const GProduct& p, GradArgs a, hipStream_t st) {
   return EWS_OK;
 }
 
+// Contiguous rows of whole fours, the first at a multiple of their size.
+int fours(const void* p, int cols, bool f32) { return cols % 4 == 0 && (uintptr_t)p % (f32 ? 16 : 8) == 0; }
+
+template <typename T, int HB, int FB>
+int launch_narrow_as(const NarrowArgs& a, int groups, bool back, hipStream_t st) {
+  typedef Narrow<T, HB, FB> S;
+  if (!back) {
+    // 16 rows a wavefront and turn
+    const int n = ceil_div(a.N, 16 * kNarrowWaves);
+    hipLaunchKernelGGL((k_narrow_forward<T, HB, FB>), dim3(n < 2048 ? n : 2048), dim3(64 * kNarrowWaves), 0, st, a);
+  } else {
+    static_assert(S::kLdsBytes <= 160 << 10 && 2 * S::FP * (S::HP + 1) * 4 <= S::kLdsBytes, "the sums fit too");
+    const int rc = tiles::allow_lds(k_narrow_backward<T, HB, FB>, S::kLdsBytes);
+    if (rc != EWS_OK) return rc;
+    hipLaunchKernelGGL((k_narrow_backward<T, HB, FB>), dim3(groups), dim3(64 * S::kWaves), S::kLdsBytes, st, a);
+  }
+  GATED_CHECK();
+  return EWS_OK;
+}
+
+template <typename T>
+int launch_narrow(const NarrowArgs& a, int groups, bool back, hipStream_t st) {
+  if (a.H <= 32)
+    return a.F <= 32 ? launch_narrow_as<T, 1, 1>(a, groups, back, st) : launch_narrow_as<T, 1, 2>(a, groups, back, st);
+  return a.F <= 32 ? launch_narrow_as<T, 2, 1>(a, groups, back, st) : launch_narrow_as<T, 2, 2>(a, groups, back, st);
+}
+
+NarrowArgs narrow_args(const ews_gated_desc* s, const void* x, const void* v, const void* g, const void* bias,
+                       const void* gate_bias) {
+  NarrowArgs a{};
+  a.x = x;
+  a.v = v;
+  a.g = g;
+  a.xs = s->x_stride;
+  a.vs = s->weight_stride;
+  a.gs = s->gate_stride;
+  a.N = s->rows;
+  a.H = s->width;
+  a.F = s->features;
+  a.bias = bias;
+  a.gate_bias = gate_bias;
+  a.act = s->activation;
+  a.wide_x = s->width % 8 == 0 && tiles::rows_wide(x, s->x_stride, s->dtype == EWS_DTYPE_F32);
+  return a;
+}
+
 // Rows of results that are contiguous: whether they start at multiples of 16 bytes and hold whole eights.
 int results_wide(const void* p, int cols) { return cols % 8 == 0 && (uintptr_t)p % 16 == 0; }
 
@@ -959,7 +982,7 @@ extern "C" {
 size_t ews_gated_kept_bytes(const ews_gated_desc* desc) {
   GPlan p;
   if (gated_plan(desc, nullptr, nullptr, nullptr, false, true, p) != EWS_OK) return 0;
-  return (size_t)(p.N * 2 * p.ld) * (p.np == 3 ? 4 : 3);
+  return p.narrow ? 0 : (size_t)(p.N * 2 * p.ld) * (p.np == 3 ? 4 : 3);
 }
 
 size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, const void* weight,
@@ -976,6 +999,10 @@ int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile) {
   if (rc != EWS_OK) return rc;
   if (!tile) return EWS_ERR_NULL;
   if (product < 0 || product > 2) return EWS_ERR_OPTION;
+  if (p.narrow) {
+    for (int k = 0; k < 5; ++k) tile[k] = 0;
+    return EWS_OK;
+  }
   const Product& q = product == 0 ? p.forward : product == 1 ? p.dx : static_cast<const Product&>(p.dw);
   tile[0] = q.tile_i;
   tile[1] = q.tile_j;
@@ -1006,6 +1033,12 @@ int ews_gated_forward(const ews_gated_desc* desc, const void* x, const void* wei
     if (f32) return wide ? launch_few<float, true>(a, c.st) : launch_few<float, false>(a, c.st);
     return wide ? launch_few<bf16, true>(a, c.st) : launch_few<bf16, false>(a, c.st);
   }
+  if (c.p.narrow) {
+    NarrowArgs a = narrow_args(desc, x, weight, gate_weight, bias, gate_bias);
+    a.out = out;
+    a.wide_f = fours(out, a.F, f32);
+    return f32 ? launch_narrow<float>(a, 0, false, c.st) : launch_narrow<bf16>(a, 0, false, c.st);
+  }
   rc = operands(c, x, weight, gate_weight, true, true);
   if (rc != EWS_OK) return rc;
   ForwardArgs a{};
@@ -1026,19 +1059,40 @@ int ews_gated_forward(const ews_gated_desc* desc, const void* x, const void* wei
   return f32 ? launch_forward<float>(c.p.forward.kind, a, c.st) : launch_forward<bf16>(c.p.forward.kind, a, c.st);
 }
 
-int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* weight, const void* gate_weight,
-                       const void* kept, const void* grad_out, void* grad_x, void* grad_weight, void* grad_bias,
-                       void* grad_gate_weight, void* grad_gate_bias, void* workspace, ews_stream_t stream) {
+int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* weight, const void* bias,
+                       const void* gate_weight, const void* gate_bias, const void* kept, const void* grad_out,
+                       void* grad_x, void* grad_weight, void* grad_bias, void* grad_gate_weight, void* grad_gate_bias,
+                       void* workspace, ews_stream_t stream) {
   GCall c{};
   int rc = gated_plan(desc, x, weight, gate_weight, true, false, c.p);
   if (rc != EWS_OK) return rc;
-  if (!x || !weight || !gate_weight || !kept || !grad_out || !workspace) return EWS_ERR_NULL;
+  if (!x || !weight || !gate_weight || (!kept && !c.p.narrow) || !grad_out || !workspace) return EWS_ERR_NULL;
   const GPlan& p = c.p;
   const bool f32 = p.np == 3;
   c.s = desc;
   c.w = (char*)workspace;
   c.st = (hipStream_t)stream;
   const bool weights = grad_weight || grad_gate_weight, biases = grad_bias || grad_gate_bias;
+  if (p.narrow) {
+    NarrowArgs n = narrow_args(desc, x, weight, gate_weight, bias, gate_bias);
+    n.dy = grad_out;
+    n.dx = grad_x;
+    n.wide_f = fours(grad_out, n.F, f32);
+    n.wide_h = fours(grad_x, n.H, f32);
+    n.part = weights || biases ? (float*)workspace : nullptr;
+    rc = f32 ? launch_narrow<float>(n, p.narrow_groups, true, c.st) : launch_narrow<bf16>(n, p.narrow_groups, true, c.st);
+    if (rc != EWS_OK || !n.part) return rc;
+    const int FP = narrow_pad(n.F), HP = narrow_pad(n.H);
+    const dim3 grid(ceil_div(2 * FP * (HP + 1), 64));
+    if (f32)
+      hipLaunchKernelGGL((k_join_narrow<float>), grid, dim3(1024), 0, c.st, n.part, p.narrow_groups, FP, HP, n.F, n.H,
+                         (float*)grad_weight, (float*)grad_bias, (float*)grad_gate_weight, (float*)grad_gate_bias);
+    else
+      hipLaunchKernelGGL((k_join_narrow<bf16>), grid, dim3(1024), 0, c.st, n.part, p.narrow_groups, FP, HP, n.F, n.H,
+                         (bf16*)grad_weight, (bf16*)grad_bias, (bf16*)grad_gate_weight, (bf16*)grad_gate_bias);
+    GATED_CHECK();
+    return EWS_OK;
+  }
   rc = operands(c, x, weight, gate_weight, weights, grad_x != nullptr);
   if (rc != EWS_OK) return rc;
   DzArgs z{};

@@ -453,6 +453,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
     return;
   }
   __shared__ float part[4][64][9];
+  __shared__ int places[TOP ? 128 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lanes = NARROW ? a.lanes : 64, abreast = NARROW ? 64 / lanes : 1;
   const int v = NARROW ? (lane & (lanes - 1)) * 8 : (blockIdx.x * 64 + lane) * 8;
@@ -464,7 +465,25 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   float sums[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) sums[q] = 0.0f;
-  for (int j = NARROW ? r0 + wave * abreast + lane / lanes : r0 + wave; j < r1; j += 4 * abreast) {
+  // TOP: the entries of a row's bucket are looked up a row ahead, and the rows' places before all of them: each would
+  // cost a row the memory's latency
+  int e0 = 0, e1 = 0;
+  auto look_up = [&](int j) {
+    e0 = e1 = 0;
+    if (j >= r1 || j >= live || !in) return;
+    const uint16_t* first = a.top.first + (int64_t)places[j - r0] * (a.top.buckets + 1) + v / kBucket;
+    e0 = first[0];
+    e1 = first[1];
+  };
+  const int start = NARROW ? r0 + wave * abreast + lane / lanes : r0 + wave;
+  if (TOP) {
+    for (int t = threadIdx.x; t < r1 - r0; t += 256) places[t] = r0 + t < live ? a.rows.map[a.c0 + r0 + t] : 0;
+    __syncthreads();
+    look_up(start);
+  }
+  for (int j = start; j < r1; j += 4 * abreast) {
+    const int e = e0, end = e1;
+    if (TOP) look_up(j + 4 * abreast);
     float x[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) x[q] = 0.0f;
@@ -490,16 +509,15 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? lo.get(q) : hi.get(q - 4)) * f;
       }
-      if (TOP && t >= 0) {
-        const int64_t at = a.rows.map[row];
-        const uint16_t* first = a.top.first + at * (a.top.buckets + 1) + v / kBucket;
+      if (TOP && t >= 0 && e < end) {
+        const int64_t at = (int64_t)places[j - r0] * a.top.count;
         int before = -1;
-        for (int e = first[0]; e < first[1]; ++e) {
-          const int token = a.top.token[at * a.top.count + e];
+        for (int k = e; k < end; ++k) {
+          const int token = a.top.token[at + k];
+          const float p = a.top.p[at + k], z = a.top.z[at + k];
           if (token >= v && token < v + 8) {
             // the first entry of a token takes its probability's place, a further one adds to it
-            const float p = a.top.p[at * a.top.count + e];
-            const float own = (__builtin_amdgcn_exp2f(a.top.z[at * a.top.count + e] - top) * inv - p) * g;
+            const float own = (__builtin_amdgcn_exp2f(z - top) * inv - p) * g;
 #pragma unroll
             for (int q = 0; q < 8; ++q) x[q] = token == v + q ? (token == before ? x[q] - p * g : own) : x[q];
           }

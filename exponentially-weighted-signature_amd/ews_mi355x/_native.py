@@ -545,7 +545,7 @@ def load():
     lib.ews_gated_tile.restype = i32
     lib.ews_gated_forward.argtypes = [gdp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.ews_gated_forward.restype = i32
-    lib.ews_gated_backward.argtypes = [gdp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ews_gated_backward.argtypes = [gdp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.ews_gated_backward.restype = i32
     gsp = ctypes.POINTER(GatedScanDesc)
     lib.ews_gated_scan_residual_bytes.argtypes = [gsp]

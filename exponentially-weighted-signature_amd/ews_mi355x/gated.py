@@ -49,7 +49,8 @@ class _Call:
         b, gb = self.biases
         lib = nat.load()
         out = self.x.new_empty((self.desc.rows, self.desc.features))
-        kept = self.x.new_empty(lib.ews_gated_kept_bytes(self.desc), dtype=torch.uint8) if keep else None
+        size = lib.ews_gated_kept_bytes(self.desc) if keep else 0
+        kept = self.x.new_empty(size, dtype=torch.uint8) if size else None
         ws = self.workspace(nat.GATED_KEEP if keep else nat.GATED_FORWARD)
         nat.check(launch(self.x.device, lib.ews_gated_forward, self.desc, x, v, b, g, gb, out.data_ptr(), _ptr(kept),
                          _ptr(ws)), "ews_gated_forward")
@@ -58,6 +59,7 @@ class _Call:
     def backward(self, kept, gout, needs):
         """The gradients of x, weight, bias, gate_weight and gate_bias that ``needs`` asks for."""
         x, v, g = self.at
+        bias, gate_bias = self.biases
         F, H, size = self.desc.features, self.desc.width, self.x.element_size()
         new = self.x.new_empty
         gx = new(self.x.shape) if needs[0] else None
@@ -69,7 +71,7 @@ class _Call:
             pg = None if gv is None else pv + F * H * size
             pgb = None if gb is None else pb + F * size
         ws = self.workspace(nat.GATED_BACKWARD)
-        nat.check(launch(gout.device, nat.load().ews_gated_backward, self.desc, x, v, g, kept.data_ptr(),
+        nat.check(launch(gout.device, nat.load().ews_gated_backward, self.desc, x, v, bias, g, gate_bias, _ptr(kept),
                          gout.data_ptr(), _ptr(gx), pv, pb, pg, pgb, ws.data_ptr()), "ews_gated_backward")
         return gx, gv, gb, gg, ggb
 
@@ -79,15 +81,15 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):
         call = _Call(x, weight, bias, gate_weight, gate_bias, activation)
         out, kept = call.forward(True)
-        ctx.save_for_backward(x, weight, gate_weight, kept)
+        ctx.save_for_backward(x, weight, bias, gate_weight, gate_bias, kept)
         ctx.activation = activation
         return out
 
     @staticmethod
     @once
     def backward(ctx, gout):
-        x, weight, gate_weight, kept = ctx.saved_tensors
-        call = _Call(x, weight, None, gate_weight, None, ctx.activation)
+        *inputs, kept = ctx.saved_tensors
+        call = _Call(*inputs, ctx.activation)
         return (*call.backward(kept, gout.contiguous(), ctx.needs_input_grad), None)
 
 

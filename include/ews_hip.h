@@ -766,7 +766,8 @@ typedef struct ews_gated_desc {
   int32_t activation;    /* EWS_GATED_* */
 } ews_gated_desc;
 
-/* What a forward keeps for its backward: two numbers for each of out's, of 24 bits (float32: 32). */
+/* What a forward keeps for its backward: two numbers for each of out's, of 24 bits (float32: 32); nothing (0: kept may
+ * be NULL) where H and F are 64 at most. */
 size_t ews_gated_kept_bytes(const ews_gated_desc* desc);
 
 /* Scratch of one call (EWS_GATED_FORWARD, _KEEP or _BACKWARD) with these addresses, of which nothing is read; 0: may be
@@ -777,7 +778,8 @@ size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, cons
 
 /* For tests and profiles: of product 0 (v and g of a call that keeps or of many rows), 1 (grad_x) or 2 (the weights'
  * gradients) tile[0] x tile[1] = the results of one workgroup, tile[2] = the splits of its sum, and tile[3] of the
- * tile[4] tiles are done by a workgroup each, the others shared by several. */
+ * tile[4] tiles are done by a workgroup each, the others shared by several. All 0 where H and F are 64 at most, which have
+ * kernels of their own. */
 int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile);
 
 /* out (N, F), contiguous, = (x weight^T + bias) act(x gate_weight^T + gate_bias); weight and gate_weight (F, H), either
@@ -787,9 +789,10 @@ int ews_gated_forward(const ews_gated_desc* desc, const void* x, const void* wei
                       ews_stream_t stream);
 
 /* The gradients (contiguous; each may be NULL) for out's (contiguous). */
-int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* weight, const void* gate_weight,
-                       const void* kept, const void* grad_out, void* grad_x, void* grad_weight, void* grad_bias,
-                       void* grad_gate_weight, void* grad_gate_bias, void* workspace, ews_stream_t stream);
+int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* weight, const void* bias,
+                       const void* gate_weight, const void* gate_bias, const void* kept, const void* grad_out,
+                       void* grad_x, void* grad_weight, void* grad_bias, void* grad_gate_weight, void* grad_gate_bias,
+                       void* workspace, ews_stream_t stream);
 
 /* Human-readable text of a return code. */
 const char* ews_error_string(int code);

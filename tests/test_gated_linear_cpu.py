@@ -42,11 +42,11 @@ def test_library_refuses(bad):
     d = _desc(**bad)
     assert lib.ews_gated_kept_bytes(d) == 0 and lib.ews_gated_workspace_bytes(d, one, one, one, 2) == 0
     assert lib.ews_gated_forward(d, one, one, None, one, None, one, None, one, None) in (-2, -4)
-    assert lib.ews_gated_backward(d, one, one, one, one, one, one, one, None, one, None, one, None) in (-2, -4)
+    assert lib.ews_gated_backward(d, one, one, None, one, None, one, one, one, one, None, one, None, one, None) in (-2, -4)
 
 
 def test_library_refuses_null():
-    lib, one, d = nat.load(), ctypes.c_void_p(16), _desc(rows=100)
+    lib, one, d = nat.load(), ctypes.c_void_p(16), _desc(rows=100, features=100)
     assert lib.ews_gated_forward(None, one, one, None, one, None, one, None, one, None) == -1
     for hole in range(5):
         p = [one] * 5
@@ -55,7 +55,8 @@ def test_library_refuses_null():
     for hole in range(6):
         p = [one] * 6
         p[hole] = None
-        assert lib.ews_gated_backward(d, p[0], p[1], p[2], p[3], p[4], one, one, None, one, None, p[5], None) == -1
+        assert lib.ews_gated_backward(d, p[0], p[1], None, p[2], None, p[3], p[4], one, one, None, one, None, p[5],
+                                      None) == -1
 
 
 @pytest.mark.parametrize("case", list(TILES))
@@ -79,3 +80,13 @@ def test_scratch_of_what_is_read_where_it_is():
     few = _desc(rows=64, width=130, features=512, x_stride=130, weight_stride=130, gate_stride=130)
     assert lib.ews_gated_workspace_bytes(few, 4098, 6, 10, nat.GATED_FORWARD) == 0
     assert lib.ews_gated_workspace_bytes(few, 4098, 6, 10, nat.GATED_KEEP) > 0
+
+
+def test_narrow_maps_keep_nothing():
+    lib = nat.load()
+    for H, F, narrow in ((64, 64, True), (1, 1, True), (65, 64, False), (64, 65, False)):
+        d = _desc(rows=1 << 20, width=H, features=F, x_stride=H, weight_stride=H, gate_stride=H)
+        assert (lib.ews_gated_kept_bytes(d) == 0) == narrow
+        if narrow:
+            assert lib.ews_gated_workspace_bytes(d, 4098, 6, 10, nat.GATED_KEEP) == 0
+            assert 0 < lib.ews_gated_workspace_bytes(d, 4098, 6, 10, nat.GATED_BACKWARD) <= 512 * 128 * 65 * 4

@@ -127,7 +127,8 @@ def _check(x, w, b, gw, gb, up, name):
 
 SHAPES = [
     (1, 1, 1), (1, 64, 64), (3, 5, 7), (2, 72, 130), (17, 64, 100), (33, 40, 24), (64, 128, 8), (65, 64, 65), (130, 200, 16),
-    (257, 72, 515), (700, 24, 33), (2111, 32, 32), (63, 1032, 40),
+    (257, 72, 515), (700, 24, 33), (2111, 32, 32), (63, 1032, 40), (1000, 33, 31), (999, 31, 64), (70, 64, 4), (5000, 60, 64),
+    (140000, 8, 12), (3, 65, 7), (130, 70, 2), (1, 65, 65), (129, 128, 200),
 ]
 
 
