@@ -75,8 +75,8 @@ struct Top {
   const int* token;       // (N, K) sorted; INT_MAX where there is none
   const float* p;         // (N, K) their probabilities
   const float* entropy;   // (N) sum_k p_k log p_k
-  const uint16_t* first;  // (N, buckets + 1) the first entry at or past every 128th token
-  int buckets;
+  const uint16_t* first;  // (N, stride) the first entry at or past every 128th token, buckets + 1 of them
+  int buckets, stride;
   float* z;               // (N, K) their logits
   float scale;            // log2(e) / T: of logits
   float temperature;
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_logits(LogitArgs a) 
     } else {
       const int row = j0 + j < live ? a.rows.map[a.c0 + j0 + j] : -1;
       tile_target[j] = row;
-      const uint16_t* first = a.top.first + (int64_t)row * (a.top.buckets + 1) + i0 / kBucket;
+      const uint16_t* first = a.top.first + (int64_t)row * a.top.stride + i0 / kBucket;
 #pragma unroll
       for (int k = 0; k <= kBuckets; ++k) tile_first[k * T::J + j] = row < 0 ? 0 : first[k];
     }
@@ -444,6 +444,12 @@ struct DzArgs {
   Top top;
 };
 
+// Memory that nothing writes while the kernel runs, at an index that a wavefront shares: by scalar loads.
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(4))) T* scalar(const T* p) {
+  return (const __attribute__((address_space(4))) T*)p;
+}
+
 // NP planes: 3 of float32 inputs, 1 or (few rows) 2 of bfloat16 ones. NARROW: a row fills half a wavefront at most, so
 // several rows share one (131072 rows by V=8: 94 -> 38 us). TOP: distillation.
 template <int NP, bool NARROW, bool TOP>
@@ -453,7 +459,6 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
     return;
   }
   __shared__ float part[4][64][9];
-  __shared__ int places[TOP ? 128 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lanes = NARROW ? a.lanes : 64, abreast = NARROW ? 64 / lanes : 1;
   const int v = NARROW ? (lane & (lanes - 1)) * 8 : (blockIdx.x * 64 + lane) * 8;
@@ -465,62 +470,78 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   float sums[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) sums[q] = 0.0f;
-  // TOP: the entries of a row's bucket are looked up a row ahead, and the rows' places before all of them: each would
-  // cost a row the memory's latency
-  int e0 = 0, e1 = 0;
-  auto look_up = [&](int j) {
-    e0 = e1 = 0;
-    if (j >= r1 || j >= live || !in) return;
-    const uint16_t* first = a.top.first + (int64_t)places[j - r0] * (a.top.buckets + 1) + v / kBucket;
-    e0 = first[0];
-    e1 = first[1];
+  // All of a row's loads go out before any is used (8192 rows by V=32000 209 -> 188 us). TOP: its entries too, where a
+  // wavefront has one row those of its 512 tokens, by scalar loads, which wait for nothing that is on its way to vector
+  // registers (K=32: 209 us; by vector loads 309, the range of the next row's looked up a row ahead 286; two rows on
+  // their way at a time 226).
+  constexpr bool kUniform = TOP && !NARROW;
+  const int b0 = blockIdx.x * (512 / kBucket);
+  auto first_of = [&](int place, int b) {
+    const int64_t i = (int64_t)place * a.top.stride + (b < a.top.buckets ? b : a.top.buckets);
+    return (int)(scalar((const uint32_t*)a.top.first)[i >> 1] >> (16 * (i & 1)) & 0xffffu);
   };
-  const int start = NARROW ? r0 + wave * abreast + lane / lanes : r0 + wave;
-  if (TOP) {
-    for (int t = threadIdx.x; t < r1 - r0; t += 256) places[t] = r0 + t < live ? a.rows.map[a.c0 + r0 + t] : 0;
-    __syncthreads();
-    look_up(start);
-  }
-  for (int j = start; j < r1; j += 4 * abreast) {
-    const int e = e0, end = e1;
-    if (TOP) look_up(j + 4 * abreast);
+  struct Row {
+    int t, e, end;
+    int64_t at;
+    float top, inv, g, m;
+    u32x4 w;
+    Pack<float, 4> lo, hi;
+  };
+  auto load = [&](Row& r, int j) {
+    if (j >= live || !in) return;
+    const int row = a.c0 + j;
+    if (TOP) {
+      const int place = kUniform ? scalar(a.rows.map)[row] : a.rows.map[row];
+      r.at = (int64_t)place * a.top.count;
+      if (kUniform) {
+        r.e = first_of(place, b0);
+        r.end = first_of(place, b0 + 512 / kBucket);
+      } else {
+        r.e = a.top.first[(int64_t)place * a.top.stride + v / kBucket];
+        r.end = a.top.first[(int64_t)place * a.top.stride + v / kBucket + 1];
+      }
+    }
+    r.t = a.rows.target[row];
+    r.top = a.st.top[row];
+    r.inv = a.st.inv[row];
+    r.g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
+    if (TOP) r.g *= a.top.temperature;
+    r.m = a.st.slab[(int64_t)slab * a.chunk + j].x;
+    if (NP != 3) {
+      r.w = *reinterpret_cast<const u32x4*>((const uint16_t*)a.prob + j * a.ld + v);
+    } else {
+      r.lo.load((const float*)a.prob + j * a.ld + v);
+      r.hi.load((const float*)a.prob + j * a.ld + v + 4);
+    }
+  };
+  auto finish_row = [&](const Row& r, int j) {
     float x[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) x[q] = 0.0f;
     if (j < live && in) {
-      const int row = a.c0 + j;
-      const int t = a.rows.target[row];
-      const float top = a.st.top[row], inv = a.st.inv[row];
-      float g = a.upstream ? a.upstream[a.rows.map[row]] : 1.0f;
-      if (TOP) g *= a.top.temperature;
-      const float m = a.st.slab[(int64_t)slab * a.chunk + j].x;
-      const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f(m - top) * inv * g;
+      const int row = a.c0 + j, t = r.t;
+      const float top = r.top, inv = r.inv, g = r.g;
+      const float f = t < 0 ? __builtin_nanf("") : __builtin_amdgcn_exp2f(r.m - top) * inv * g;
       if (NP != 3) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>((const uint16_t*)a.prob + j * a.ld + v);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const uint32_t y = (w[q >> 1] >> (16 * (q & 1))) & 0xffffu;
+          const uint32_t y = (r.w[q >> 1] >> (16 * (q & 1))) & 0xffffu;
           x[q] = y == 65535u ? 0.0f * f : __builtin_amdgcn_exp2f((float)y * (-kOctaves / 65535.0f)) * f;
         }
       } else {
-        Pack<float, 4> lo, hi;
-        lo.load((const float*)a.prob + j * a.ld + v);
-        hi.load((const float*)a.prob + j * a.ld + v + 4);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? lo.get(q) : hi.get(q - 4)) * f;
+        for (int q = 0; q < 8; ++q) x[q] = (q < 4 ? r.lo.get(q) : r.hi.get(q - 4)) * f;
       }
-      if (TOP && t >= 0 && e < end) {
-        const int64_t at = (int64_t)places[j - r0] * a.top.count;
+      if (TOP && t >= 0) {
         int before = -1;
-        for (int k = e; k < end; ++k) {
-          const int token = a.top.token[at + k];
-          const float p = a.top.p[at + k], z = a.top.z[at + k];
-          if (token >= v && token < v + 8) {
-            // the first entry of a token takes its probability's place, a further one adds to it
-            const float own = (__builtin_amdgcn_exp2f(z - top) * inv - p) * g;
+        for (int e = r.e; e < r.end; ++e) {
+          const int token = kUniform ? scalar(a.top.token)[r.at + e] : a.top.token[r.at + e];
+          const float p = kUniform ? scalar(a.top.p)[r.at + e] : a.top.p[r.at + e];
+          const float z = kUniform ? scalar(a.top.z)[r.at + e] : a.top.z[r.at + e];
+          // the first entry of a token takes its probability's place, a further one adds to it
+          const float own = (__builtin_amdgcn_exp2f(z - top) * inv - p) * g;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) x[q] = token == v + q ? (token == before ? x[q] - p * g : own) : x[q];
-          }
+          for (int q = 0; q < 8; ++q) x[q] = token == v + q ? (token == before ? x[q] - p * g : own) : x[q];
           before = token;
         }
       }
@@ -532,7 +553,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) sums[q] += x[q];
     }
-    if (!in) continue;
+    if (!in) return;
     if (NP != 3) {
       Pack<bf16, 8> p;
       p.set(x);
@@ -555,6 +576,11 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
         *reinterpret_cast<u32x4*>(a.dz + k * a.plane + j * a.ld + v) = w;
       }
     }
+  };
+  for (int j = NARROW ? r0 + wave * abreast + lane / lanes : r0 + wave; j < r1; j += 4 * abreast) {
+    Row r;
+    load(r, j);
+    finish_row(r, j);
   }
   if (!a.bias) return;
 #pragma unroll
@@ -602,7 +628,7 @@ struct TeacherArgs {
   const void* index;
   const void* logit;
   int64_t index_stride, logit_stride;
-  int n, count, vocab, buckets;
+  int n, count, vocab, buckets, stride;
   int ordered;             // count rounded up to a power of two
   int index_bytes, logit_bf16;
   float scale;             // log2(e) / T
@@ -623,6 +649,7 @@ __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
   const int row = blockIdx.x * 4 + wave;
   if (row >= a.n) return;  // a wavefront uses no other's part of LDS
   uint64_t* key = reinterpret_cast<uint64_t*>(lds) + wave * a.ordered;
+  float* value = reinterpret_cast<float*>(reinterpret_cast<uint64_t*>(lds) + 4 * a.ordered) + wave * a.ordered;
   auto logit = [&](int k) {
     const int64_t at = row * a.logit_stride + k;
     return a.logit_bf16 ? widen(((const bf16*)a.logit)[at]) : ((const float*)a.logit)[at];
@@ -635,6 +662,7 @@ __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
       const int64_t at = row * a.index_stride + k;
       const int64_t i = a.index_bytes == 8 ? ((const int64_t*)a.index)[at] : ((const int32_t*)a.index)[at];
       const float t = logit(k);
+      value[k] = t;
       if (i >= 0 && t != -__builtin_inff()) {
         any = true;
         bad |= i >= a.vocab;
@@ -669,7 +697,7 @@ __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
   float sum = 0.0f;
   for (int e = lane; e < a.count; e += 64) {
     const uint64_t k = key[e];
-    if ((uint32_t)(k >> 32) != 0x7fffffffu) sum += __builtin_amdgcn_exp2f((logit((uint32_t)k) - top) * a.scale);
+    if ((uint32_t)(k >> 32) != 0x7fffffffu) sum += __builtin_amdgcn_exp2f((value[(uint32_t)k] - top) * a.scale);
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -680,7 +708,7 @@ __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
     const int token = (int)(k >> 32);
     float p = 0.0f;
     if (token != 0x7fffffff) {
-      const float y = (logit((uint32_t)k) - top) * a.scale;
+      const float y = (value[(uint32_t)k] - top) * a.scale;
       p = __builtin_amdgcn_exp2f(y) / sum;
       if (p != 0.0f) entropy += p * (y - log_sum);
     }
@@ -699,7 +727,7 @@ __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
       else
         hi = mid;
     }
-    a.first[(int64_t)row * (a.buckets + 1) + b] = (uint16_t)lo;
+    a.first[(int64_t)row * a.stride + b] = (uint16_t)lo;
   }
   any = __any(any);
   bad = __any(bad);
@@ -911,6 +939,8 @@ struct LPlan {
   size_t total;
 };
 
+int bucket_stride(int buckets) { return (buckets + 2) / 2 * 2; }  // whole words
+
 // entries: the teacher's of a row; 0 where the targets are tokens.
 int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p, int entries = 0) {
   if (!s) return EWS_ERR_NULL;
@@ -977,7 +1007,7 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p, int ent
     p.token = take((size_t)p.N * entries * 4);
     p.share = take((size_t)p.N * entries * 4);
     p.entropy = take((size_t)p.N * 4);
-    p.first = take((size_t)p.N * (p.buckets + 1) * 2);
+    p.first = take((size_t)p.N * bucket_stride(p.buckets) * 2);
   }
   if (train) {
     p.prob = take((size_t)(p.chunk * p.Vp) * (p.np == 3 || p.twice ? 4 : 2));
@@ -1257,6 +1287,7 @@ Call make_call(const ews_loss_desc* s, const LPlan& p, void* workspace, ews_stre
     c.top.entropy = (const float*)(c.w + p.entropy);
     c.top.first = (const uint16_t*)(c.w + p.first);
     c.top.buckets = p.buckets;
+    c.top.stride = bucket_stride(p.buckets);
     c.top.z = c.stats.zt;
     c.top.temperature = temperature;
     c.top.scale = kLog2e / temperature;
@@ -1517,6 +1548,7 @@ struct Distill {
     t.count = p.entries;
     t.vocab = p.V;
     t.buckets = p.buckets;
+    t.stride = bucket_stride(p.buckets);
     t.ordered = 2;
     while (t.ordered < t.count) t.ordered *= 2;
     t.index_bytes = d->index_bytes;
@@ -1527,7 +1559,7 @@ struct Distill {
     t.p = (float*)(c.w + p.share);
     t.entropy = (float*)(c.w + p.entropy);
     t.first = (uint16_t*)(c.w + p.first);
-    hipLaunchKernelGGL(k_teacher, dim3(ceil_div(p.N, 4)), dim3(256), 4 * t.ordered * 8, c.st, t);
+    hipLaunchKernelGGL(k_teacher, dim3(ceil_div(p.N, 4)), dim3(256), 4 * t.ordered * 12, c.st, t);
     LOSS_CHECK();
     return ::begin(c, hidden, weight, bias, t.target, loss_rows, grad_hidden);
   }
