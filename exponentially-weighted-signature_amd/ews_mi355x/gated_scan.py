@@ -5,6 +5,7 @@ ews/conversion/reference/recurrences.py:48-113)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from .embed import DTYPES, check_tensor, launch, once, refuse_tangents
@@ -19,6 +20,22 @@ def _neighbours(t):
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+def _one(a, b):
+    """Whether two tensors of one shape are the same memory."""
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+
+
+def _span(t):
+    """The bytes from t's first number to behind its last."""
+    end = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (end * t.element_size() if t.numel() else 0)
+
+
+def _overlap(a, b):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _forward(x, gate, mask, state, last, form, train):
     """(out, last, the descriptor, the residual of a training call)."""
     B, L, D = x.shape
@@ -30,9 +47,9 @@ def _forward(x, gate, mask, state, last, form, train):
                              nat.GATED_SCAN_FORMS[form])
     lib = nat.load()
     residual = x.new_empty(lib.ews_gated_scan_residual_bytes(desc), dtype=torch.uint8) if train else None
+    ws = _workspace(lib, desc, x)
     nat.check(launch(x.device, lib.ews_gated_scan_forward, desc, x.data_ptr(), gate.data_ptr(), _ptr(mask), _ptr(state),
-                     out.data_ptr(), last.data_ptr(), _ptr(residual), _ptr(_workspace(lib, desc, x))),
-              "ews_gated_scan_forward")
+                     out.data_ptr(), last.data_ptr(), _ptr(residual), _ptr(ws)), "ews_gated_scan_forward")
     return out, last, desc, residual
 
 
@@ -62,9 +79,10 @@ class _GatedScan(torch.autograd.Function):
         gx, ggate = x.new_empty(x.shape), x.new_empty(x.shape)
         gstate = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         lib = nat.load()
+        ws = _workspace(lib, ctx.desc, x)
         nat.check(launch(x.device, lib.ews_gated_scan_backward, ctx.desc, x.data_ptr(), gate.data_ptr(), _ptr(mask),
                          residual.data_ptr(), _ptr(gout), _ptr(glast), gx.data_ptr(), ggate.data_ptr(), _ptr(gstate),
-                         _ptr(_workspace(lib, ctx.desc, x))), "ews_gated_scan_backward")
+                         _ptr(ws)), "ews_gated_scan_backward")
         return gx, ggate, gstate, None, None
 
 
@@ -108,7 +126,7 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
     for name, t in (("gate", gate), ("mask", mask), ("state", state), ("last", last)):
         if t is not None and t.device != x.device:
             raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    refuse_tangents((x, gate, state))
+    refuse_tangents((x, gate, state, last))
     train = torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
                                          (state is not None and state.requires_grad))
     if last is not None:
@@ -116,6 +134,9 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
             raise ValueError("last is written in place: call under torch.no_grad(), or take the state that is returned")
         if not last.is_contiguous():
             raise ValueError("last must be contiguous")
+        if any(t is not None and not same and _overlap(last, t) for t, same in (
+                (state, state is not None and _one(state, last)), (x, False), (gate, False))):
+            raise ValueError("last overlaps x, gate or a part of state: it may be state itself or apart from all of them")
     if B == 0 or L == 0:  # no step: the state stays
         end = x.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
         return x * gate, end if last is None else last.copy_(end)
@@ -128,5 +149,8 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
         state = state.contiguous()
     if train:
         return _GatedScan.apply(x, gate, state, mask, form)
+    given = last is not None
     out, last, _, _ = _forward(x, gate, mask, state, last, form, False)
+    if given:
+        increment_version(last)  # a graph that has saved it refuses its backward, as after torch's own writes
     return out, last
