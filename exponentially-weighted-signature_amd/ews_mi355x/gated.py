@@ -16,81 +16,96 @@ def _ptr(t):
 
 
 class _Call:
-    """One call's operands as the library takes them; ``gate_weight`` None: the second half of ``weight``'s rows."""
+    """One call's operands as the library takes them (copies only where rows are not contiguous); ``gate_weight`` None:
+    the second half of ``weight``'s rows. A backward is given the descriptor of its forward, and the operands that the
+    forward took: a small call costs its host time, and the backward's thread runs Python two to three times slower than
+    the caller's."""
 
-    def __init__(self, x, weight, bias, gate_weight, gate_bias, activation):
-        self.x, xs = row_major(x)
-        self.weight, ws = row_major(weight)
-        self.joint = gate_weight is None
-        features = weight.shape[0] // 2 if self.joint else weight.shape[0]
-        size = weight.element_size()
-        v = self.weight.data_ptr()
-        if self.joint:
-            g, gs = v + features * ws * size, ws
+    __slots__ = ("operands", "desc", "at")
+
+    def __init__(self, operands, desc=None, activation=None):
+        x, weight, bias, gate_weight, gate_bias = operands
+        joint = gate_weight is None
+        if desc is None:
+            x, xs = row_major(x)
+            weight, ws = row_major(weight)
+            gs = ws
+            if not joint:
+                gate_weight, gs = row_major(gate_weight)
+            if bias is not None:
+                bias = bias.contiguous()
+            if gate_bias is not None:
+                gate_bias = gate_bias.contiguous()
+            desc = nat.GatedDesc(xs, ws, gs, x.shape[0], x.shape[1], weight.shape[0] // 2 if joint else weight.shape[0],
+                                 DTYPES[x.dtype], nat.GATED_ACTIVATIONS[activation])
+            operands = x, weight, bias, gate_weight, gate_bias
+        self.operands, self.desc = operands, desc
+        v, b = weight.data_ptr(), _ptr(bias)
+        if joint:
+            size = 4 if desc.dtype == nat.DTYPE_F32 else 2
+            g = v + desc.features * desc.weight_stride * size
+            gb = None if b is None else b + desc.features * size
         else:
-            self.gate_weight, gs = row_major(gate_weight)
-            g = self.gate_weight.data_ptr()
-        self.bias = None if bias is None else bias.contiguous()
-        self.gate_bias = None if gate_bias is None else gate_bias.contiguous()
-        b, gb = _ptr(self.bias), _ptr(self.gate_bias)
-        if self.joint and b is not None:
-            gb = b + features * size
-        self.desc = nat.GatedDesc(xs, ws, gs, x.shape[0], x.shape[1], features, DTYPES[x.dtype],
-                                  nat.GATED_ACTIVATIONS[activation])
-        self.at = self.x.data_ptr(), v, g
-        self.biases = b, gb
+            g, gb = gate_weight.data_ptr(), _ptr(gate_bias)
+        self.at = x.data_ptr(), v, b, g, gb  # what the library is given of them
 
-    def workspace(self, call):
-        size = nat.load().ews_gated_workspace_bytes(self.desc, *self.at, call)
-        return self.x.new_empty(size, dtype=torch.uint8) if size else None
+    def scratch_bytes(self, call):
+        x, v, _, g, _ = self.at
+        return nat.load().ews_gated_workspace_bytes(self.desc, x, v, g, call)
 
     def forward(self, keep):
-        x, v, g = self.at
-        b, gb = self.biases
+        x = self.operands[0]
         lib = nat.load()
-        out = self.x.new_empty((self.desc.rows, self.desc.features))
+        out = x.new_empty((self.desc.rows, self.desc.features))
         size = lib.ews_gated_kept_bytes(self.desc) if keep else 0
-        kept = self.x.new_empty(size, dtype=torch.uint8) if size else None
-        ws = self.workspace(nat.GATED_KEEP if keep else nat.GATED_FORWARD)
-        nat.check(launch(self.x.device, lib.ews_gated_forward, self.desc, x, v, b, g, gb, out.data_ptr(), _ptr(kept),
-                         _ptr(ws)), "ews_gated_forward")
+        kept = x.new_empty(size, dtype=torch.uint8) if size else None
+        ws = _scratch(x, self.scratch_bytes(nat.GATED_KEEP if keep else nat.GATED_FORWARD))
+        nat.check(launch(x.device, lib.ews_gated_forward, self.desc, *self.at, out.data_ptr(), _ptr(kept), _ptr(ws)),
+                  "ews_gated_forward")
         return out, kept
 
-    def backward(self, kept, gout, needs):
+    def backward(self, kept, gout, needs, scratch_bytes):
         """The gradients of x, weight, bias, gate_weight and gate_bias that ``needs`` asks for."""
-        x, v, g = self.at
-        bias, gate_bias = self.biases
-        F, H, size = self.desc.features, self.desc.width, self.x.element_size()
-        new = self.x.new_empty
-        gx = new(self.x.shape) if needs[0] else None
-        rows = 2 * F if self.joint else F
-        gv, gb = new((rows, H)) if needs[1] else None, new((rows,)) if needs[2] else None
-        gg, ggb = new((F, H)) if needs[3] else None, new((F,)) if needs[4] else None
-        pv, pb, pg, pgb = _ptr(gv), _ptr(gb), _ptr(gg), _ptr(ggb)
-        if self.joint:
-            pg = None if gv is None else pv + F * H * size
-            pgb = None if gb is None else pb + F * size
-        ws = self.workspace(nat.GATED_BACKWARD)
-        nat.check(launch(gout.device, nat.load().ews_gated_backward, self.desc, x, v, bias, g, gate_bias, _ptr(kept),
-                         gout.data_ptr(), _ptr(gx), pv, pb, pg, pgb, ws.data_ptr()), "ews_gated_backward")
+        x, weight, _, gate_weight, _ = self.operands
+        F, H = self.desc.features, self.desc.width
+        new = x.new_empty
+        gx = new(x.shape) if needs[0] else None
+        gv = new(weight.shape) if needs[1] else None
+        gb = new((weight.shape[0],)) if needs[2] else None
+        gg = new(weight.shape) if needs[3] else None
+        ggb = new((F,)) if needs[4] else None
+        pv, pb = _ptr(gv), _ptr(gb)
+        if gate_weight is None:
+            size = 4 if self.desc.dtype == nat.DTYPE_F32 else 2
+            pg = None if pv is None else pv + F * H * size
+            pgb = None if pb is None else pb + F * size
+        else:
+            pg, pgb = _ptr(gg), _ptr(ggb)
+        ws = _scratch(x, scratch_bytes)
+        nat.check(launch(gout.device, nat.load().ews_gated_backward, self.desc, *self.at, _ptr(kept), gout.data_ptr(),
+                         _ptr(gx), pv, pb, pg, pgb, ws.data_ptr()), "ews_gated_backward")
         return gx, gv, gb, gg, ggb
+
+
+def _scratch(x, size):
+    return x.new_empty(size, dtype=torch.uint8) if size else None
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):
-        call = _Call(x, weight, bias, gate_weight, gate_bias, activation)
+        call = _Call((x, weight, bias, gate_weight, gate_bias), activation=activation)
         out, kept = call.forward(True)
-        ctx.save_for_backward(x, weight, bias, gate_weight, gate_bias, kept)
-        ctx.activation = activation
+        ctx.save_for_backward(*call.operands, kept)
+        ctx.args = call.desc, call.scratch_bytes(nat.GATED_BACKWARD)
         return out
 
     @staticmethod
     @once
     def backward(ctx, gout):
-        *inputs, kept = ctx.saved_tensors
-        call = _Call(*inputs, ctx.activation)
-        return (*call.backward(kept, gout.contiguous(), ctx.needs_input_grad), None)
+        *operands, kept = ctx.saved_tensors
+        desc, size = ctx.args
+        return (*_Call(operands, desc).backward(kept, gout.contiguous(), ctx.needs_input_grad, size), None)
 
 
 def takes(x, weight, bias):
@@ -151,5 +166,5 @@ def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activat
     if train:
         out = _GatedLinear.apply(x2, *others, activation)
     else:
-        out = _Call(x2, *others, activation).forward(False)[0]
+        out = _Call((x2, *others), activation=activation).forward(False)[0]
     return out if out.shape == shape else out.reshape(shape)

@@ -37,7 +37,7 @@ def _overlap(a, b):
 
 
 def _forward(x, gate, mask, state, last, form, train):
-    """(out, last, the descriptor, the residual of a training call)."""
+    """(out, last, the descriptor and the scratch's size, the residual of a training call)."""
     B, L, D = x.shape
     out = x.new_empty((B, L, D))
     if last is None:
@@ -47,21 +47,17 @@ def _forward(x, gate, mask, state, last, form, train):
                              nat.GATED_SCAN_FORMS[form])
     lib = nat.load()
     residual = x.new_empty(lib.ews_gated_scan_residual_bytes(desc), dtype=torch.uint8) if train else None
-    ws = _workspace(lib, desc, x)
+    size = lib.ews_gated_scan_workspace_bytes(desc)
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
     nat.check(launch(x.device, lib.ews_gated_scan_forward, desc, x.data_ptr(), gate.data_ptr(), _ptr(mask), _ptr(state),
                      out.data_ptr(), last.data_ptr(), _ptr(residual), _ptr(ws)), "ews_gated_scan_forward")
-    return out, last, desc, residual
-
-
-def _workspace(lib, desc, x):
-    size = lib.ews_gated_scan_workspace_bytes(desc)
-    return x.new_empty(size, dtype=torch.uint8) if size else None
+    return out, last, (desc, size), residual
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, state, mask, form):
-        out, last, ctx.desc, residual = _forward(x, gate, mask, state, None, form, True)
+        out, last, ctx.args, residual = _forward(x, gate, mask, state, None, form, True)
         ctx.save_for_backward(x, gate, mask, residual)
         ctx.set_materialize_grads(False)
         return out, last
@@ -79,8 +75,9 @@ class _GatedScan(torch.autograd.Function):
         gx, ggate = x.new_empty(x.shape), x.new_empty(x.shape)
         gstate = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         lib = nat.load()
-        ws = _workspace(lib, ctx.desc, x)
-        nat.check(launch(x.device, lib.ews_gated_scan_backward, ctx.desc, x.data_ptr(), gate.data_ptr(), _ptr(mask),
+        desc, size = ctx.args
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, x.data_ptr(), gate.data_ptr(), _ptr(mask),
                          residual.data_ptr(), _ptr(gout), _ptr(glast), gx.data_ptr(), ggate.data_ptr(), _ptr(gstate),
                          _ptr(ws)), "ews_gated_scan_backward")
         return gx, ggate, gstate, None, None
