@@ -9,11 +9,11 @@
 // Three pairs of products of 2 N H F operations each bound all but the smallest calls; they run on the matrix cores
 // (ews_tiles.h). v and g of the same output meet in a wavefront's registers: a tile's first operand is interleaved, half
 // of every wavefront's rows from V and half from G, which costs nothing, as the copies to LDS can start anywhere. So y is
-// formed where the sums end, and v and g are never in memory. A training call also writes act(g) and v act'(g), what the
-// backward multiplies dy with: float32 as it is, for bfloat16 x its upper 24 bits (dv and dg are rounded to bfloat16
-// afterwards, and a second rounding of that size before it makes the gradients 1.7 times as far off as their own rounding
-// alone, where one makes 1.4; 16 bits would save 3% of a call). k_dz forms dv | dg from them, one after the other along a
-// row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows.
+// formed where the sums end. A training call also writes v and g, for bfloat16 x the upper 24 bits of the sums: dv and dg
+// are rounded to bfloat16 afterwards, and a second rounding of that size before it makes the gradients 1.7 times as far
+// off as their own rounding alone, where one makes 1.4 (16 bits would save 3% of a call). k_dz forms dv | dg from them,
+// one after the other along a row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows. What act and
+// act' of g take is hidden there behind the memory; where the sums end it adds to the matrix cores' time.
 //
 // Narrow maps (both widths up to 64) have kernels of their own (ews_gated_narrow.h), and keep nothing.
 //
@@ -28,6 +28,7 @@
 #include "ews_pack.h"
 #include "ews_pick.h"
 #include "ews_tiles.h"
+#include "ews_tiles32.h"
 #include "ews_vec.h"
 
 namespace ews {
@@ -228,7 +229,7 @@ struct ForwardArgs {
   int act;
   int wide;                // rows of out start at multiples of 16 bytes and hold whole eights
   void* out;               // (N, F)
-  void* kept;              // (N, 2 ld): act(g) | v act'(g); or null (Kept)
+  void* kept;              // (N, 2 ld): v | g (Kept)
   int64_t ld;              // F up to a multiple of 64
 };
 
@@ -283,7 +284,8 @@ __device__ __forceinline__ float bias_at(const void* bias, int i) {
   return bias ? widen(((const B*)bias)[i]) : 0.0f;
 }
 
-template <class T, int PAIRS, typename O>
+// KEEP: for a backward.
+template <class T, int PAIRS, typename O, bool KEEP>
 __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_forward(ForwardArgs a) {
   extern __shared__ char lds[];
   int it, jt;
@@ -301,18 +303,17 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_forward(ForwardArgs 
   constexpr int kHalf = T::TI / 2;
 #pragma unroll
   for (int b = 0; b < T::TJ; ++b) {
-    f32x16 y[kHalf], p[kHalf], q[kHalf];
+    f32x16 y[kHalf], v[kHalf], g[kHalf];
 #pragma unroll
     for (int t = 0; t < kHalf; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int i = (wi * kHalf + t) * 32 + 8 * (r / 4) + 4 * half + r % 4;
-        const float v = acc[t][b][r] + bias[i];
+        v[t][r] = acc[t][b][r] + bias[i];
+        g[t][r] = acc[t + kHalf][b][r] + bias[T::I / 2 + i];
         float act, slope;
-        activate(a.act, acc[t + kHalf][b][r] + bias[T::I / 2 + i], act, slope);
-        y[t][r] = v * act;
-        p[t][r] = act;
-        q[t][r] = v * slope;
+        activate(a.act, g[t][r], act, slope);
+        y[t][r] = v[t][r] * act;
       }
     const int row0 = j0 + (wj * T::TJ + b) * 32, col0 = i0 + wi * kHalf * 32;
     auto out = [&](auto each) {
@@ -326,13 +327,13 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_forward(ForwardArgs 
       out(Eight{});
     else
       out(One{});
-    if (!a.kept) continue;
+    if (!KEEP) continue;
     // whole eights up to ld: what lies past F is not read
-    rows_of_half<T, Eight>(lds, p, [&](int row, int col, const Eight& e) {
+    rows_of_half<T, Eight>(lds, v, [&](int row, int col, const Eight& e) {
       if (row0 + row < a.N && col0 + col < a.ld)
         Kept<O>::store(a.kept, 2 * a.ld * a.N, (int64_t)(row0 + row) * 2 * a.ld + col0 + col, e);
     });
-    rows_of_half<T, Eight>(lds, q, [&](int row, int col, const Eight& e) {
+    rows_of_half<T, Eight>(lds, g, [&](int row, int col, const Eight& e) {
       if (row0 + row < a.N && col0 + col < a.ld)
         Kept<O>::store(a.kept, 2 * a.ld * a.N, (int64_t)(row0 + row) * 2 * a.ld + a.ld + col0 + col, e);
     });
@@ -354,67 +355,112 @@ struct FewArgs {
 
 constexpr int kFewWaves = 4;
 
-// 16 outputs of up to 16 COLS rows a workgroup; its wavefronts take every fourth 32 AHEAD of k and are joined in LDS.
-// v_mfma_f32_16x16x32_bf16: lane l holds row l % 16 of either operand at k = 8 (l / 16) + 0..7, and results
-// column l % 16, rows 4 (l / 16) + 0..3.
-template <typename T, int COLS, bool WIDE>
-__global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
-  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
-  __shared__ f32x4v part[kFewWaves][2][COLS][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r16 = lane & 15, k8 = (lane >> 4) * 8;
-  const int f0 = blockIdx.x * 16;
-  const int row = f0 + r16 < a.F ? f0 + r16 : a.F - 1;
-  const T* v = (const T*)a.v + row * a.ws;
-  const T* g = (const T*)a.g + row * a.gs;
-  f32x4v accv[COLS], accg[COLS];
+// A lane's eight numbers of 32 k of a row from column k on, zero past the row's end: bfloat16 k + 8 q .. 8 q + 7 for q its
+// fourth of the wavefront, float32 k + 4 q .. 4 q + 3 and 16 further on. Either way a load's lanes read 64 bytes of a row;
+// a product's k may be in any order that its operands share.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void few_eight(const T* row, int k, int H, T (&x)[8]) {
+  const int q = (threadIdx.x >> 4) & 3;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) accv[c] = accg[c] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int h = 0; h < 2; ++h) {
+      const int at = k + 16 * h + 4 * q;
+      if (WIDE) {  // H is a multiple of 8
+        *reinterpret_cast<u32x4*>(x + 4 * h) = at < H ? *reinterpret_cast<const u32x4*>(row + at) : u32x4{0, 0, 0, 0};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * h + e] = at + e < H ? row[at + e] : 0.0f;
+      }
+    }
+  } else {
+    eight_of<T>(row, k + 8 * q, H, WIDE, x);
+  }
+}
+
+template <typename T, bool CAREFUL>
+__device__ __forceinline__ void few_fragments(const T (&x)[8], bf16x8 (&f)[kPlanes<T>]) {
+  if constexpr (sizeof(T) == 4)
+    cut<CAREFUL>(x, f);
+  else
+    fragments<T>(x, f);
+}
+
+// One wavefront's part of the sums over k: of 16 of V's and G's rows and 16 COLS of x's.
+template <typename T, int COLS, bool WIDE, bool CAREFUL>
+__device__ __forceinline__ void few_sums(const FewArgs& a, f32x4v (&acc)[2][COLS]) {
+  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int f = blockIdx.x * 16 + (lane & 15), own = f < a.F ? f : a.F - 1;
+  const T* v = (const T*)a.v + own * a.ws;
+  const T* g = (const T*)a.g + own * a.gs;
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) acc[0][c] = acc[1][c] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
   for (int k0 = wave * 32 * kAhead; k0 < a.H; k0 += kFewWaves * 32 * kAhead) {
     T wv[kAhead][8], wg[kAhead][8];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
-      eight_of<T>(v, k0 + 32 * s + k8, a.H, WIDE, wv[s]);
-      eight_of<T>(g, k0 + 32 * s + k8, a.H, WIDE, wg[s]);
+      few_eight<T, WIDE>(v, k0 + 32 * s, a.H, wv[s]);
+      few_eight<T, WIDE>(g, k0 + 32 * s, a.H, wg[s]);
     }
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
       bf16x8 fv[kPlanes<T>], fg[kPlanes<T>];
-      fragments<T>(wv[s], fv);
-      fragments<T>(wg[s], fg);
+      few_fragments<T, CAREFUL>(wv[s], fv);
+      few_fragments<T, CAREFUL>(wg[s], fg);
 #pragma unroll
       for (int c = 0; c < COLS; ++c) {
-        const int n = c * 16 + r16 < a.N ? c * 16 + r16 : a.N - 1;
+        const int n = c * 16 + (lane & 15) < a.N ? c * 16 + (lane & 15) : a.N - 1;
         T x[8];
         bf16x8 fx[kPlanes<T>];
-        eight_of<T>((const T*)a.x + n * a.xs, k0 + 32 * s + k8, a.H, WIDE, x);
-        fragments<T>(x, fx);
-        mac(fv, fx, accv[c]);
-        mac(fg, fx, accg[c]);
+        few_eight<T, WIDE>((const T*)a.x + n * a.xs, k0 + 32 * s, a.H, x);
+        few_fragments<T, CAREFUL>(x, fx);
+        mac(fv, fx, acc[0][c]);
+        mac(fg, fx, acc[1][c]);
       }
     }
   }
+}
+
+// 16 outputs of up to 16 COLS rows a workgroup; its wavefronts take every fourth stretch of k and are joined in LDS.
+// v_mfma_f32_16x16x32_bf16: a lane gets results column l % 16 (x's row), rows 4 (l / 16) + 0..3 (outputs). One bfloat16
+// row through H=4096, F=11000 34 us (5.3 TB/s), float32 88 (4.1); 32 outputs a workgroup 46 and 106.
+template <typename T, int COLS, bool WIDE>
+__global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
+  __shared__ f32x4v part[kFewWaves][2 * COLS][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  f32x4v acc[2][COLS];
+  few_sums<T, COLS, WIDE, false>(a, acc);
+  if (sizeof(T) == 4) {
+    // infinities need care (ews_tiles32.h): looked for in the sums, not number by number, which took 124 us for 90
+    bool bad = false;
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    part[wave][0][c][lane] = accv[c];
-    part[wave][1][c][lane] = accg[c];
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bad |= __builtin_isnan(acc[side][c][r]);
+    if (__any(bad)) few_sums<T, COLS, WIDE, true>(a, acc);
   }
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) part[wave][side * COLS + c][lane] = acc[side][c];
   __syncthreads();
   for (int c = wave; c < COLS; c += kFewWaves) {
-    f32x4v sv = part[0][0][c][lane], sg = part[0][1][c][lane];
+    f32x4v sv = part[0][c][lane], sg = part[0][COLS + c][lane];
 #pragma unroll
     for (int w = 1; w < kFewWaves; ++w) {
-      sv += part[w][0][c][lane];
-      sg += part[w][1][c][lane];
+      sv += part[w][c][lane];
+      sg += part[w][COLS + c][lane];
     }
-    const int n = c * 16 + r16;
+    const int n = c * 16 + (lane & 15), f = blockIdx.x * 16 + (lane >> 4) * 4;
+    if (n >= a.N) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int f = f0 + (lane >> 4) * 4 + r;
-      if (n >= a.N || f >= a.F) continue;
+      if (f + r >= a.F) continue;
       float act, slope;
-      activate(a.act, sg[r] + bias_at<T>(a.gate_bias, f), act, slope);
-      ((T*)a.out)[(int64_t)n * a.F + f] = narrow<T>((sv[r] + bias_at<T>(a.bias, f)) * act);
+      activate(a.act, sg[r] + bias_at<T>(a.gate_bias, f + r), act, slope);
+      ((T*)a.out)[(int64_t)n * a.F + f + r] = narrow<T>((sv[r] + bias_at<T>(a.bias, f + r)) * act);
     }
   }
 }
@@ -422,7 +468,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
 // ------------------------------------------------------------------------------------------------------------ dv | dg
 struct DzArgs {
   const void* dy;          // (N, F)
-  const void* kept;        // (N, 2 ld)
+  const void* kept;        // (N, 2 ld): v | g
+  int act;
   int N, F, padded;        // rows; and zeros up to this one
   int64_t ld;
   int wide;                // rows of dy start at multiples of 16 bytes and hold whole eights
@@ -463,16 +510,25 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
       for (int q = 0; q < 8; ++q)
         if (q < live) u[q] = widen(dy[q]);
     }
+    float both[2][8];
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) both[side][q] = 0.0f;
+    if (live) {
+      Kept<T>::load(a.kept, 2 * a.ld * a.N, (int64_t)row * 2 * a.ld + f, both[0]);
+      Kept<T>::load(a.kept, 2 * a.ld * a.N, (int64_t)row * 2 * a.ld + a.ld + f, both[1]);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float act, slope;
+        activate(a.act, both[1][q], act, slope);
+        both[1][q] = q < live ? u[q] * (both[0][q] * slope) : 0.0f;
+        both[0][q] = q < live ? u[q] * act : 0.0f;
+      }
+    }
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      float z[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) z[q] = 0.0f;
-      if (live) {
-        Kept<T>::load(a.kept, 2 * a.ld * a.N, ((int64_t)row * 2 + side) * a.ld + f, z);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) z[q] = q < live ? u[q] * z[q] : 0.0f;
-      }
+      const float(&z)[8] = both[side];
       uint16_t p[8][NP];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
@@ -674,8 +730,9 @@ using tiles::Operand;
 using tiles::Product;
 using ews::vec::bf16;
 
-// Rows up to which a forward alone reads V and G straight into registers.
-constexpr int kFewRows = 64;
+// Rows up to which a forward alone reads V and G straight into registers: 32 of H=4096, F=11000 48 us in bfloat16 (by the
+// tiles 51), 33 rows 55 (48); float32, whose tiles need planes packed first, 64 rows 180 (420).
+constexpr int kFewRows = 32, kFewRows32 = 64;
 // Splits that one thread adds; more are added by eight groups of threads.
 constexpr int kFewSplits = 8;
 
@@ -743,7 +800,7 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
   // a launch has fewer than 2^32 threads, one for eight numbers; dv | dg's rows lie within the tiles' offsets
   if (p.Np * p.Hp > (int64_t)1 << 33 || p.F * p.Hp > (int64_t)1 << 33 || p.Np * p.ld > (int64_t)1 << 34)
     return EWS_ERR_SHAPE;
-  p.few = !back && !keep && p.N <= kFewRows;
+  p.few = !back && !keep && p.N <= (p.np == 3 ? kFewRows32 : kFewRows);
   p.narrow = p.H <= kNarrowWidth && p.F <= kNarrowWidth && !p.few;
   if (p.narrow) {
     // 32 rows a wavefront and turn; as many workgroups as are on the CUs at a time
@@ -845,22 +902,28 @@ int operands(GCall& c, const void* x, const void* v, const void* g, bool want_x,
   return EWS_OK;
 }
 
-template <class T, int PAIRS, typename O>
+template <class T, int PAIRS, typename O, bool KEEP>
 int launch_forward_as(const ForwardArgs& a, hipStream_t st) {
   const int lds = tiles::lds_bytes<T, PAIRS>(a.kblocks) + T::I * 4;
-  const int rc = tiles::allow_lds(k_forward<T, PAIRS, O>, lds);
+  const int rc = tiles::allow_lds(k_forward<T, PAIRS, O, KEEP>, lds);
   if (rc != EWS_OK) return rc;
-  hipLaunchKernelGGL((k_forward<T, PAIRS, O>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), lds, st, a);
+  hipLaunchKernelGGL((k_forward<T, PAIRS, O, KEEP>), dim3((uint32_t)(a.ti * a.tj)), dim3(T::kThreads), lds, st, a);
   GATED_CHECK();
   return EWS_OK;
 }
 
-template <typename O>
+template <typename O, bool KEEP>
 int launch_forward(Kind kind, const ForwardArgs& a, hipStream_t st) {
   constexpr int kP = sizeof(O) == 4 ? tiles::kPairs : 1;
-  if (kind == tiles::kLarge) return launch_forward_as<tiles::Large, kP, O>(a, st);
-  return kind == tiles::kMedium ? launch_forward_as<tiles::Medium, kP, O>(a, st)
-                                : launch_forward_as<tiles::Flat, kP, O>(a, st);
+  if (kind == tiles::kLarge) return launch_forward_as<tiles::Large, kP, O, KEEP>(a, st);
+  // without a backward few rows have a kernel of their own
+  if (!KEEP || kind == tiles::kMedium) return launch_forward_as<tiles::Medium, kP, O, KEEP>(a, st);
+  return launch_forward_as<tiles::Flat, kP, O, true>(a, st);
+}
+
+template <typename O>
+int launch_forward(Kind kind, const ForwardArgs& a, hipStream_t st) {
+  return a.kept ? launch_forward<O, true>(kind, a, st) : launch_forward<O, false>(kind, a, st);
 }
 
 template <typename T, bool WIDE>
@@ -870,7 +933,7 @@ int launch_few(const FewArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_few<T, 1, WIDE>), grid, block, 0, st, a);
   else if (a.N <= 32)
     hipLaunchKernelGGL((k_few<T, 2, WIDE>), grid, block, 0, st, a);
-  else
+  else if constexpr (sizeof(T) == 4)
     hipLaunchKernelGGL((k_few<T, 4, WIDE>), grid, block, 0, st, a);
   GATED_CHECK();
   return EWS_OK;
@@ -1098,6 +1161,7 @@ int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* we
   DzArgs z{};
   z.dy = grad_out;
   z.kept = kept;
+  z.act = desc->activation;
   z.N = p.N;
   z.F = p.F;
   z.padded = (int)p.Np;

@@ -124,9 +124,9 @@ def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activat
     ``gate_bias`` (F,) G and c. Biases may be None. All of x's type. ``activation``: "sigmoid", "silu", "gelu" (its tanh
     form) or "relu". The result (..., F) is rounded to x's type once.
 
-    Differentiable in everything (reverse mode). A call that records gradients keeps act(g) and v act'(g), of 24 bits
-    each (float32: 32), beside the result. Up to 64 rows without gradients (a decoding step) the weights are read once, at the
-    memory's rate."""
+    Differentiable in everything (reverse mode). A call that records gradients keeps both products' sums, of 24
+    bits each (float32: 32), beside the result, unless H and F are 64 at most. A few rows without gradients (a decoding
+    step: 32, of float32 64) read the weights once, at the memory's rate."""
     if activation not in nat.GATED_ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(nat.GATED_ACTIVATIONS)}, got {activation!r}")
     joint = gate_weight is None

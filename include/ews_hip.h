@@ -766,8 +766,8 @@ typedef struct ews_gated_desc {
   int32_t activation;    /* EWS_GATED_* */
 } ews_gated_desc;
 
-/* What a forward keeps for its backward: two numbers for each of out's, of 24 bits (float32: 32); nothing (0: kept may
- * be NULL) where H and F are 64 at most. */
+/* What a forward keeps for its backward: two sums for each of out's numbers, of 24 bits (float32: 32); nothing (0: kept
+ * may be NULL) where H and F are 64 at most. */
 size_t ews_gated_kept_bytes(const ews_gated_desc* desc);
 
 /* Scratch of one call (EWS_GATED_FORWARD, _KEEP or _BACKWARD) with these addresses, of which nothing is read; 0: may be
