@@ -20,20 +20,13 @@ def _neighbours(t):
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def _one(a, b):
-    """Whether two tensors of one shape are the same memory."""
-    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
-
-
-def _span(t):
-    """The bytes from t's first number to behind its last."""
-    end = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (end * t.element_size() if t.numel() else 0)
-
-
-def _overlap(a, b):
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+def _touches(t, start, end):
+    """Whether t lies in the bytes from start to end, in part."""
+    first = t.data_ptr()
+    if first >= end or t.numel() == 0:
+        return False
+    span = t.numel() if t.is_contiguous() else 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return first + span * t.element_size() > start
 
 
 def _forward(x, gate, mask, state, last, form, train):
@@ -131,8 +124,10 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
             raise ValueError("last is written in place: call under torch.no_grad(), or take the state that is returned")
         if not last.is_contiguous():
             raise ValueError("last must be contiguous")
-        if any(t is not None and not same and _overlap(last, t) for t, same in (
-                (state, state is not None and _one(state, last)), (x, False), (gate, False))):
+        start = last.data_ptr()
+        end = start + last.numel() * 4
+        own = state is None or state is last or (state.data_ptr() == start and state.is_contiguous())
+        if _touches(x, start, end) or _touches(gate, start, end) or not own and _touches(state, start, end):
             raise ValueError("last overlaps x, gate or a part of state: it may be state itself or apart from all of them")
     if B == 0 or L == 0:  # no step: the state stays
         end = x.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
