@@ -7,13 +7,18 @@
 // act: the logistic function s, g s(g), g s(2 sqrt(2/pi) (g + 0.044715 g^3)) (the tanh form of GELU), or max(g, 0).
 //
 // Three pairs of products of 2 N H F operations each bound all but the smallest calls; they run on the matrix cores
-// (ews_tiles.h). v and g of the same output meet in a wavefront's registers: a tile's first operand is interleaved, half
-// of every wavefront's rows from V and half from G, which costs nothing, as the copies to LDS can start anywhere. So y is
-// formed where the sums end. A training call also writes v and g, for bfloat16 x the upper 24 bits of the sums: dv and dg
-// are rounded to bfloat16 afterwards, and a second rounding of that size before it makes the gradients 1.7 times as far
-// off as their own rounding alone, where one makes 1.4 (16 bits would save 3% of a call). k_dz forms dv | dg from them,
-// one after the other along a row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows. What act and
-// act' of g take is hidden there behind the memory; where the sums end it adds to the matrix cores' time.
+// (ews_tiles.h). v and g of the same output meet in a wavefront's registers: a tile's first operand is interleaved,
+// half of every wavefront's rows from V and half from G, which costs nothing, as the copies to LDS can start anywhere.
+// So y is formed where the sums end. A training call also writes v and g, for bfloat16 x the upper 24 bits of the sums:
+// dv and dg are rounded to bfloat16 afterwards, and a second rounding of that size before it makes the gradients 1.7
+// times as far off as their own rounding alone, where one makes 1.4 (16 bits would save 3% of a call). k_dz forms dv |
+// dg from them, one after the other along a row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows.
+// What act and act' of g take is hidden there behind the memory; where the sums end it adds to the matrix cores' time.
+//
+// Measured (N=8192, H=2048, F=5504, bfloat16, 1.11e12 operations, 1.09 ms): v and g 0.44 (0.84 PFLOP/s: 1376 tiles are
+// 5.4 rounds of the CUs, and 270 MB kept are written), k_dz 0.105 (5.1 TB/s), dx 0.32 (1.16 PFLOP/s), dV and dG 0.36
+// (1.03). Float32 (N=4095, H=512, F=1365) 0.29: 93, 78 and 82 us the three (122 to 147 TFLOP/s). One row of H=4096,
+// F=11000, bfloat16: 34 us, 5.3 TB/s.
 //
 // Narrow maps (both widths up to 64) have kernels of their own (ews_gated_narrow.h), and keep nothing.
 //
@@ -106,7 +111,9 @@ struct CopierPair {
                   16 * place(row, idx & 7);
     }
   }
-  __device__ __forceinline__ const uint16_t* at(int piece, int kb) const { return base + piece * plane + (int64_t)kb * 64; }
+  __device__ __forceinline__ const uint16_t* at(int piece, int kb) const {
+    return base + piece * plane + (int64_t)kb * 64;
+  }
   __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const {
     copy_piece(gate(c) ? from + to_g : from, offset[c], to + c * T::kThreads * 16);
   }
@@ -247,7 +254,8 @@ __device__ __forceinline__ void store(O* to, const One& e) {
   *to = narrow<O>(e.x);
 }
 
-// A wavefront's 32 rows of 16 TI results each, z[a] its blocks, through its own part of LDS: f(row of the 32, column, W).
+// A wavefront's 32 rows of 16 TI results each, z[a] its blocks, through its own part of LDS: f(row of the 32, column,
+// W).
 template <class T, typename W, class F>
 __device__ __forceinline__ void rows_of_half(char* lds, const f32x16 (&z)[T::TI / 2], F f) {
   constexpr int kCols = 16 * T::TI, kRow = kCols + 4, kEach = sizeof(W) / 4;
@@ -355,9 +363,9 @@ struct FewArgs {
 
 constexpr int kFewWaves = 4;
 
-// A lane's eight numbers of 32 k of a row from column k on, zero past the row's end: bfloat16 k + 8 q .. 8 q + 7 for q its
-// fourth of the wavefront, float32 k + 4 q .. 4 q + 3 and 16 further on. Either way a load's lanes read 64 bytes of a row;
-// a product's k may be in any order that its operands share.
+// A lane's eight numbers of 32 k of a row from column k on, zero past the row's end: bfloat16 k + 8 q .. 8 q + 7 for q
+// its fourth of the wavefront, float32 k + 4 q .. 4 q + 3 and 16 further on. Either way a load's lanes read 64 bytes of
+// a row; a product's k may be in any order that its operands share.
 template <typename T, bool WIDE>
 __device__ __forceinline__ void few_eight(const T* row, int k, int H, T (&x)[8]) {
   const int q = (threadIdx.x >> 4) & 3;
@@ -479,8 +487,8 @@ struct DzArgs {
   int each;                // rows of a workgroup
 };
 
-// A thread eight columns of every fourth of its workgroup's rows. SUMS: for the biases (the registers of which cost waves:
-// 8192 rows by F=5504 in bfloat16 127 us with them, 105 without).
+// A thread eight columns of every fourth of its workgroup's rows. SUMS: for the biases (the registers of which cost
+// waves: 8192 rows by F=5504 in bfloat16 127 us with them, 105 without).
 template <typename T, bool SUMS>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   constexpr int NP = kPlanes<T>;
@@ -672,8 +680,8 @@ __global__ __launch_bounds__(1024 / (sizeof(W) / 4)) void k_shared(GradArgs a) {
   store<O>(to + i, w);
 }
 
-// The splits' results added in order, by GROUPS groups of a workgroup's threads a contiguous part of them each; a thread
-// takes one result (W: One) or eight.
+// The splits' results added in order, by GROUPS groups of a workgroup's threads a contiguous part of them each; a
+// thread takes one result (W: One) or eight.
 template <bool ROWS, typename O, typename W, int GROUPS>
 __global__ __launch_bounds__(256) void k_join(GradArgs a) {
   constexpr int kEach = sizeof(W) / 4, kThreads = 256 / GROUPS;
@@ -731,8 +739,8 @@ using tiles::Operand;
 using tiles::Product;
 using ews::vec::bf16;
 
-// Rows up to which a forward alone reads V and G straight into registers: 32 of H=4096, F=11000 48 us in bfloat16 (by the
-// tiles 51), 33 rows 55 (48); float32, whose tiles need planes packed first, 64 rows 180 (420).
+// Rows up to which a forward alone reads V and G straight into registers: 32 of H=4096, F=11000 48 us in bfloat16 (by
+// the tiles 51), 33 rows 55 (48); float32, whose tiles need planes packed first, 64 rows 180 (420).
 constexpr int kFewRows = 32, kFewRows32 = 64;
 // Splits that one thread adds; more are added by eight groups of threads.
 constexpr int kFewSplits = 8;
@@ -1149,7 +1157,8 @@ int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* we
     n.wide_f = fours(grad_out, n.F, f32);
     n.wide_h = fours(grad_x, n.H, f32);
     n.part = weights || biases ? (float*)workspace : nullptr;
-    rc = f32 ? launch_narrow<float>(n, p.narrow_groups, true, c.st) : launch_narrow<bf16>(n, p.narrow_groups, true, c.st);
+    rc = f32 ? launch_narrow<float>(n, p.narrow_groups, true, c.st)
+             : launch_narrow<bf16>(n, p.narrow_groups, true, c.st);
     if (rc != EWS_OK || !n.part) return rc;
     const int FP = narrow_pad(n.F), HP = narrow_pad(n.H);
     const dim3 grid(ceil_div(2 * FP * (HP + 1), 64));

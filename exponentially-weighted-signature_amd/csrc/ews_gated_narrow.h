@@ -1,18 +1,19 @@
-// The gated linear map of ews_gated.hip for widths up to 64: many rows through small V and G, bound by x, y, dy and dx's
-// bytes. (131072 rows of 32 by 32, float32, by the tiles, forward and backward: x packed into planes, 50 MB, and dv |
-// dg, 100 MB, are most of what moves, and the call takes 282 us; here the forward's kernel takes 19, the backward's 45.)
+// The gated linear map of ews_gated.hip for widths up to 64: many rows through small V and G, bound by x, y, dy and
+// dx's bytes. (131072 rows of 32 by 32, float32, by the tiles, forward and backward: x packed into planes, 50 MB, and
+// dv | dg, 100 MB, are most of what moves, and the call takes 282 us; here the forward's kernel takes 19, the
+// backward's 45.)
 //
 // Nothing is kept and nothing but results is written: a wavefront holds 32 rows, and the backward forms v and g anew. V
 // and G lie in LDS as the matrix instructions' fragments, cut into planes once by every workgroup, which then walks
-// through rows. v_mfma_f32_16x16x32_bf16: lane l holds row (of the second operand column) l % 16 at k = 8 (l / 16) + 0..7,
-// and results column l % 16, rows 4 (l / 16) + 0..3.
+// through rows. v_mfma_f32_16x16x32_bf16: lane l holds row (of the second operand column) l % 16 at k = 8 (l / 16) +
+// 0..7, and results column l % 16, rows 4 (l / 16) + 0..3.
 //
 //   v, g   [f, n] = sum over h of V[f, h] x[n, h]: a lane gets four neighbouring f of one row.
-//   dx     [h, n] = sum over f of V[f, h] dv[n, f] + G[f, h] dg[n, f]: dv and dg are in that layout already. A product's k
-//          may be in any order that its operands share: of 32 f lane l's are 4 (l / 16) + 0..3 and 16 more, which are two
-//          of its results, so only V's and G's fragments are laid out for it.
-//   dV, dG [f, h] = sum over n of dv[n, f] x[n, h]: n has to run along a lane's eight, so both are turned through LDS, 32
-//          rows at a time. The sums stay in registers; the workgroups' are joined by k_join_narrow in order.
+//   dx     [h, n] = sum over f of V[f, h] dv[n, f] + G[f, h] dg[n, f]: dv and dg are in that layout already. A
+//          product's k may be in any order that its operands share: of 32 f lane l's are 4 (l / 16) + 0..3 and 16 more,
+//          which are two of its results, so only V's and G's fragments are laid out for it.
+//   dV, dG [f, h] = sum over n of dv[n, f] x[n, h]: n has to run along a lane's eight, so both are turned through LDS,
+//          32 rows at a time. The sums stay in registers; the workgroups' are joined by k_join_narrow in order.
 //
 // Float32 is multiplied as six products of bfloat16 planes; dv and dg of bfloat16 calls have two planes, which costs
 // nothing here and rounds the gradients once.
@@ -110,7 +111,8 @@ template <typename T>
 __device__ __forceinline__ void eight_of(const T* row, int k, int H, bool wide, T (&x)[8]) {
   if (wide && k < H) {  // H is a multiple of 8
 #pragma unroll
-    for (int q = 0; q < 8; q += kWide<T>) *reinterpret_cast<u32x4*>(x + q) = *reinterpret_cast<const u32x4*>(row + k + q);
+    for (int q = 0; q < 8; q += kWide<T>)
+      *reinterpret_cast<u32x4*>(x + q) = *reinterpret_cast<const u32x4*>(row + k + q);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q) x[q] = k + q < H ? row[k + q] : narrow<T>(0.0f);
@@ -227,7 +229,8 @@ __device__ __forceinline__ void front_of(const NarrowArgs& a, const bf16x8* frag
     for (int f16 = 0; f16 < 2 * FB; ++f16) z[side][f16] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int hb = 0; hb < HB; ++hb)
-    eight_of<T>((const T*)a.x + (n < a.N ? n : 0) * a.xs, hb * 32 + (lane >> 4) * 8, n < a.N ? a.H : 0, a.wide_x, x[hb]);
+    eight_of<T>((const T*)a.x + (n < a.N ? n : 0) * a.xs, hb * 32 + (lane >> 4) * 8, n < a.N ? a.H : 0, a.wide_x,
+                x[hb]);
 #pragma unroll
   for (int hb = 0; hb < HB; ++hb) {
     bf16x8 p[S::NP];

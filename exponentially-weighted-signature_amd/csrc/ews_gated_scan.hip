@@ -3,8 +3,8 @@
 //   convex   a_t = sigmoid(g_t), h_t = a_t h_{t-1} + (1 - a_t) x_t
 //   linear   a_t = g_t,          h_t = a_t h_{t-1} + x_t
 //
-// for every channel by itself, h_0 given or zero. A step off the mask has a = 1 and no input (h stays), and nothing that
-// its x and g hold is used. With l_t the gradient of h_t and m_t = a_t l_t that of h_{t-1}:
+// for every channel by itself, h_0 given or zero. A step off the mask has a = 1 and no input (h stays), and nothing
+// that its x and g hold is used. With l_t the gradient of h_t and m_t = a_t l_t that of h_{t-1}:
 //
 //   l_t = dh_t + m_{t+1} (m after the last step: the last state's own gradient)
 //   convex   dx_t = l_t (1 - a_t),   dg_t = l_t (h_{t-1} - x_t) a_t (1 - a_t)
@@ -12,16 +12,20 @@
 //
 // 1 - a is formed as e a with e = exp(-g), so neither side of the gate loses digits. States are float32.
 //
-// A few operations a number: memory bounds it. The forward reads x and g and writes h; the backward reads x, g and dh and
-// writes dx and dg. It forms the states anew from those at the starts of tiles, which the forward leaves in float32 (one
-// state in 64 steps or more): h in bfloat16 would be as large as x, and dg would lose what h - x cancels.
+// A few operations a number: memory bounds it. The forward reads x and g and writes h; the backward reads x, g and dh
+// and writes dx and dg. It forms the states anew from those at the starts of tiles, which the forward leaves in float32
+// (one state in 64 steps or more): h in bfloat16 would be as large as x, and dg would lose what h - x cancels.
 //
 // A step is the map h -> a h + b, and maps compose: (a2, b2) after (a1, b1) is (a2 a1, a2 b1 + b2). A workgroup owns a
 // strip of channels of one sequence and walks it in tiles of steps, a thread kSteps steps of its channels: it composes
 // its own steps, its wavefront's by shuffles, the workgroup's through LDS, and then applies them to the state before.
-// Loads of the next tile are on their way meanwhile. Where there are channels enough to fill the chip, a thread walks its
-// channels alone and nothing is exchanged. Where there are few, sequences are cut into segments: a first launch
+// Loads of the next tile are on their way meanwhile. Where there are channels enough to fill the chip, a thread walks
+// its channels alone and nothing is exchanged. Where there are few, sequences are cut into segments: a first launch
 // composes each segment's steps (k_ends), and each workgroup of the second applies those before its own.
+//
+// Measured, bfloat16: 8 x 4095 x 2048 (strips) forward 104 us (3.9 TB/s with the tiles' states), backward 153 (4.4),
+// one workgroup a CU and the VALU busy for half of it; 1 x 131071 x 1024 (segments, which read x and g, backward g and
+// dh, twice) 148 + 176 and 139 + 314; a step of 8 x 1 x 2048 3.6.
 #include <hip/hip_runtime.h>
 
 #include "ews_hip.h"

@@ -25,7 +25,7 @@
 //             split over k and joined in order by k_reduce.
 //
 // 8192 rows (a tenth of them ignored), H=2048, V=32000, bfloat16, in a trace of ten calls: k_logits 0.94 ms (1.0
-// PFLOP/s), k_dz 0.20 (4.6 TB/s), dh and dW 0.83 each (1.16), all else 0.035; calls in a row, untraced, take 2.69 ms in
+// PFLOP/s), k_dz 0.17 (5.4 TB/s), dh and dW 0.83 each (1.16), all else 0.035; calls in a row, untraced, take 2.68 ms in
 // all. One row by V=100003, H=4096: k_logits 0.15 ms, 5.6 TB/s of W.
 //
 // The probabilities are kept for kChunkBytes of rows at a time; dW is summed over the chunks in float32. Nothing is
@@ -65,10 +65,10 @@ struct Rows {
 //   q[n, v] = softmax_v (z[n, v] / T)        l[n] = T^2 sum_k p_k (log p_k - log q[n, v_k])
 //   dz[n, v] = T g_n (q[n, v] - sum of the p_k with v_k = v)
 //
-// Everything above stays as it is but for what the targets need. k_teacher sorts a row's entries by token and says where
-// those of every 128 tokens begin, so that a tile finds its own at once (16384 rows of 64 entries each: one entry in four
-// tiles' rows). k_logits puts its block of z through LDS where one of its rows has an entry there, and hands out the
-// entries' own float32 logits; k_dz takes them in place of the kept probabilities, as it does a target's.
+// Everything above stays as it is but for what the targets need. k_teacher sorts a row's entries by token and says
+// where those of every 128 tokens begin, so that a tile finds its own at once (16384 rows of 64 entries each: one entry
+// in four tiles' rows). k_logits puts its block of z through LDS where one of its rows has an entry there, and hands
+// out the entries' own float32 logits; k_dz takes them in place of the kept probabilities, as it does a target's.
 constexpr int kBucket = 128;
 struct Top {
   int count;              // K
@@ -641,8 +641,8 @@ struct TeacherArgs {
 constexpr int64_t kNone = -100;
 constexpr int kMostTop = 1024;
 
-// A wavefront a row: its entries that count (a token that is not negative, a logit that is not -inf) sorted by token, by
-// a bitonic network in LDS, ties in the order given, with the teacher's softmax over them.
+// A wavefront a row: its entries that count (a token that is not negative, a logit that is not -inf) sorted by token,
+// by a bitonic network in LDS, ties in the order given, with the teacher's softmax over them.
 __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
   extern __shared__ char lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1225,7 +1225,8 @@ int launch_join(const Call& c, int c0, float* loss_rows) {
     hipLaunchKernelGGL((k_join<4, TOP>), dim3(ceil_div(p.chunk, 4)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, c0,
                        chunk, loss_rows);
   else
-    hipLaunchKernelGGL((k_join<64, TOP>), dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs, c0,
+    hipLaunchKernelGGL((k_join<64, TOP>), dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs,
+                       c0,
                        chunk, loss_rows);
   LOSS_CHECK();
   if (TOP) {

@@ -1,5 +1,5 @@
-// Operands of the products of ews_tiles.h laid out for them: rows of whole k blocks with zeros behind their columns, float32
-// numbers as three bfloat16 planes.
+// Operands of the products of ews_tiles.h laid out for them: rows of whole k blocks with zeros behind their columns,
+// float32 numbers as three bfloat16 planes.
 #pragma once
 
 #include <hip/hip_runtime.h>

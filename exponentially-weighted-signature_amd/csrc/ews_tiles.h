@@ -1,5 +1,5 @@
 // Matrix products of bfloat16 operands on the matrix cores of MI355X (gfx950), as tiles for kernels with epilogues of
-// their own (ews_loss.hip).
+// their own (ews_loss.hip, ews_gated.hip).
 //
 //   D[j, i] = sum_k Q[j, k] P[i, k]      float32 sums; each operand with k contiguous, or stored turned, k its rows
 //

@@ -1,5 +1,6 @@
 // Rows of float32 or bfloat16 numbers read and written sixteen bytes a lane, for the kernels around a token model's
-// blocks (ews_embed.hip, ews_clip.hip, ews_loss.hip). Arithmetic is float32; a store rounds once, to nearest even.
+// blocks (ews_embed.hip, ews_clip.hip, ews_loss.hip, ews_gated*.hip). Arithmetic is float32; a store rounds once, to
+// nearest even.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -7,7 +7,7 @@ import torch
 
 import ews_mi355x as E
 from ews_mi355x import _native as nat
-from gated_shapes import TILES
+from gated_shapes import SHARED, TILES
 
 
 @pytest.mark.parametrize("change,error,says", [
@@ -68,6 +68,17 @@ def test_tiles(case):
     for product, want in enumerate(TILES[case]):
         assert nat.load().ews_gated_tile(d, product, tile) == 0
         assert tuple(tile[:2]) == want, product
+
+
+@pytest.mark.parametrize("dtype", [nat.DTYPE_F32, nat.DTYPE_BF16])
+@pytest.mark.parametrize("size", list(SHARED))
+def test_shared_tiles(size, dtype):
+    N, H, F = size
+    d = _desc(rows=N, width=H, features=F, x_stride=H, weight_stride=H, gate_stride=H, dtype=dtype)
+    tile = (ctypes.c_int32 * 5)()
+    product, alone, tiles = SHARED[size]
+    assert nat.load().ews_gated_tile(d, product, tile) == 0
+    assert tuple(tile) == (256, 256, 1, alone, tiles)
 
 
 def test_scratch_of_what_is_read_where_it_is():

@@ -14,7 +14,7 @@ import pytest
 import torch
 
 import ews_mi355x as E
-from gated_shapes import TILES
+from gated_shapes import SHARED, TILES
 
 pytestmark = pytest.mark.gpu
 
@@ -148,6 +148,13 @@ def test_every_tile(name, N, H, F, joint):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,F", list(SHARED))
+def test_shared_tiles(N, H, F, dtype):
+    print(f"{N} {H} {F} {dtype}", flush=True)
+    _check(*_inputs(N, H, F, dtype), "gelu")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 31, 33, 48, 64])
 @pytest.mark.parametrize("H,F", [(8, 16), (31, 50), (512, 100), (1030, 37), (1096, 130)])
 def test_few_rows(N, H, F, dtype):
@@ -224,6 +231,27 @@ def test_far_gates(name):
         hit = torch.zeros(80, dtype=torch.bool, device=DEV)
         hit[[3, 70]] = True
         assert bool(y[hit[rows]].isnan().all()) and torch.equal(y[~hit[rows]], fine[~hit[rows]])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,F", [(7, 200, 40), (60, 200, 40), (90, 200, 40), (7, 31, 40), (90, 31, 40)])
+def test_infinities(N, H, F, dtype):
+    """Infinite x, and weights, where the formula gives infinities, not NaN: rows straight into registers, tiles, narrow."""
+    x, w, b, gw, gb, up = _inputs(N, H, F, dtype, joint=False)
+    inf = float("inf")
+    for tensor, at, value in ((x, (3, 5), inf), (x, (N - 1, H - 1), -inf), (w, (4, H - 1), inf), (w, (F - 1, 0), -inf)):
+        bad, badw = x.clone(), w.clone()
+        (bad if tensor is x else badw)[at] = value
+        v, g = bad.double() @ badw.double().t() + b.double(), bad.double() @ gw.double().t() + gb.double()
+        want = v * torch.sigmoid(g)
+        with torch.no_grad():
+            y = E.gated_linear(bad, badw, b, gw, gb)
+            fine = E.gated_linear(x, w, b, gw, gb)
+        hit = ~v.isfinite() | ~g.isfinite()
+        assert bool(hit.any()) and torch.equal(y[~hit], fine[~hit])
+        assert torch.equal(y[hit].isnan(), want[hit].isnan())
+        there = hit & ~want.isnan()
+        assert torch.equal(y[there].double(), want[there])
 
 
 def test_gradient_against_differences():
