@@ -1226,8 +1226,7 @@ int launch_join(const Call& c, int c0, float* loss_rows) {
                        chunk, loss_rows);
   else
     hipLaunchKernelGGL((k_join<64, TOP>), dim3(ceil_div(p.chunk, 64)), dim3(1024), 0, c.st, c.stats, c.rows, p.slabs,
-                       c0,
-                       chunk, loss_rows);
+                       c0, chunk, loss_rows);
   LOSS_CHECK();
   if (TOP) {
     hipLaunchKernelGGL(k_top_loss, dim3(ceil_div(p.chunk, 4)), dim3(256), 0, c.st, c.stats, c.rows, c.top, c0, chunk,

@@ -11,12 +11,12 @@ Per block (norm_placement "pre", ews/block.py:376-424):
 
 The norms, the gate and the channel stages without a gate (plain linear maps and pointwise functions around the scan)
 are torch operations; gated channel stages run as ``gated_linear`` (csrc/ews_gated.hip). Field names follow the
-reference (``norm1``, ``ewms``, ``graded``, ``c_down``, ``gate``, ``norm2``, ``ff1``, ``ff2``, ``clock``, ``append_clock``, ``b_layer``), so a checkpoint converted key by key loads into the
-same places. Two differences from the reference's constructor: the generator is passed as a module (``a_param``,
-any parametrisation of ``ews_mi355x.params``; default the reference's definite_plus_skew with entries N(0, 0.005))
-instead of an ``a_config`` dict, and ``key`` is an int seed or a ``torch.Generator`` (initial values are drawn from
-the same distributions as the reference's, not the same numbers). Dropout draws from torch's generator.
-"""
+reference (``norm1``, ``ewms``, ``graded``, ``c_down``, ``gate``, ``norm2``, ``ff1``, ``ff2``, ``clock``,
+``append_clock``, ``b_layer``), so a checkpoint converted key by key loads into the same places. Two differences from
+the reference's constructor: the generator is passed as a module (``a_param``, any parametrisation of
+``ews_mi355x.params``; default the reference's definite_plus_skew with entries N(0, 0.005)) instead of an ``a_config``
+dict, and ``key`` is an int seed or a ``torch.Generator`` (initial values are drawn from the same distributions as the
+reference's, not the same numbers). Dropout draws from torch's generator."""
 
 from __future__ import annotations
 

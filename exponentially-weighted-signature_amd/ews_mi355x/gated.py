@@ -8,7 +8,14 @@ import torch
 from . import _native as nat
 from .embed import DTYPES, check_tensor, launch, once, refuse_tangents, row_major
 
-_MOST_WIDTH, _MOST_FEATURES = 1 << 16, 1 << 20
+_MOST_ROWS, _MOST_WIDTH, _MOST_FEATURES = 1 << 24, 1 << 16, 1 << 20
+
+
+def _fits(N, H, F):
+    """Whether the library takes these sizes."""
+    Np, Hp, ld = (-(-n // 64) * 64 for n in (N, H, F))
+    return (N <= _MOST_ROWS and H <= _MOST_WIDTH and F <= _MOST_FEATURES
+            and max(Np, F) * Hp <= 1 << 33 and Np * ld <= 1 << 34)
 
 
 def _ptr(t):
@@ -112,8 +119,8 @@ def takes(x, weight, bias):
     """Whether ``gated_linear`` does what a linear map of x and torch's operations after it would, types included."""
     return (x.is_cuda and x.dtype in DTYPES and weight.dtype is x.dtype and weight.device == x.device
             and (bias is None or (bias.dtype is x.dtype and bias.device == x.device))
-            and x.shape[-1] == weight.shape[1] and weight.shape[1] <= _MOST_WIDTH
-            and weight.shape[0] <= _MOST_FEATURES and not torch.is_autocast_enabled())
+            and x.shape[-1] == weight.shape[1] and _fits(x.numel() // x.shape[-1], weight.shape[1], weight.shape[0])
+            and not torch.is_autocast_enabled())
 
 
 def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activation="sigmoid"):
@@ -145,8 +152,10 @@ def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activat
         raise ValueError(f"bias must be {(rows,)}, got {tuple(bias.shape)}")
     if gate_bias is not None and gate_bias.shape != (F,):
         raise ValueError(f"gate_bias must be {(F,)}, got {tuple(gate_bias.shape)}")
-    if H > _MOST_WIDTH or F > _MOST_FEATURES:
-        raise ValueError(f"H must be up to {_MOST_WIDTH} and F up to {_MOST_FEATURES}, got {H} and {F}")
+    N = x.numel() // H
+    if not _fits(N, H, F):
+        raise ValueError(f"up to {_MOST_ROWS} rows, H up to {_MOST_WIDTH} and F up to {_MOST_FEATURES}, and, padded to "
+                         f"whole 64s, rows * H and F * H up to 2^33 and rows * F up to 2^34, got {N}, {H} and {F}")
     check_tensor("x", x)
     others = weight, bias, gate_weight, gate_bias
     for name, t in zip(("weight", "bias", "gate_weight", "gate_bias"), others):
@@ -160,7 +169,7 @@ def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activat
     shape = (*x.shape[:-1], F)
     x2 = x if x.dim() == 2 else x.reshape(-1, H)
     train = torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in others))
-    if x2.shape[0] == 0:
+    if N == 0:
         none = x.new_zeros(shape)
         return none + sum(t[:0].sum() for t in (x2, *others) if t is not None) if train else none
     if train:

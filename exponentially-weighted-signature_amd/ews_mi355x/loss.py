@@ -284,15 +284,15 @@ def linear_distillation(hidden, weight, indices, logits, bias=None, temperature=
         p = softmax(logits / T) over a row's entries     q = softmax((hidden @ weight.T + bias) / T)
         loss = T^2 sum_k p_k (log p_k - log q[indices_k])
 
-    hidden (..., H), weight (V, H) and bias (V,) or None as ``linear_cross_entropy``'s; indices (..., K) int64 or int32
-    and logits (..., K) float32 or bfloat16, K up to 1024: the teacher's tokens of every position and their logits, in
-    any order, the teacher's distribution being that over them alone. T is ``temperature`` (1e-6 to 1e6); its square
-    keeps the gradients' size. ``reduction``: "mean" over the rows that have an entry (0 where none has), "sum", or "none"
-    for every row's own loss, (...), float32. Differentiable in hidden, weight and bias (reverse mode); the teacher's
-    logits have no gradient, and one that requires it is refused: detach them.
+    hidden (..., H), weight (V, H) and bias (V,) or None as ``linear_cross_entropy``'s; indices (..., K) int64 or
+    int32 and logits (..., K) float32 or bfloat16, K up to 1024: the teacher's tokens of every position and their
+    logits, in any order, the teacher's distribution being that over them alone. T is ``temperature`` (1e-6 to 1e6);
+    its square keeps the gradients' size. ``reduction``: "mean" over the rows that have an entry (0 where none has),
+    "sum", or "none" for every row's own loss, (...), float32. Differentiable in hidden, weight and bias (reverse
+    mode); the teacher's logits have no gradient, and one that requires it is refused: detach them.
 
-    An entry with a negative index or a logit of -inf is none: rows may have fewer than K. A row without any has loss and
-    gradient zero, whatever it holds, and costs nothing. A token that is named twice is two entries of its
+    An entry with a negative index or a logit of -inf is none: rows may have fewer than K. A row without any has loss
+    and gradient zero, whatever it holds, and costs nothing. A token that is named twice is two entries of its
     probabilities. An index of V or more gives NaN. A token that the student's bias has taken out (-inf) and that the
     teacher gives any probability has an infinite loss, and the row's gradients may be NaN. When and how gradients are
     formed is as in ``linear_cross_entropy``."""

@@ -82,14 +82,16 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
         convex   h_t = a_t h_{t-1} + (1 - a_t) x_t    a_t = sigmoid(gate_t)
         linear   h_t = gate_t h_{t-1} + x_t
 
-    x and gate (B, L, D), both float32 or both bfloat16 on the HIP device; any strides, read where they are if a step's
-    channels are neighbours (the halves of a joint projection). ``h`` is of their type; states are summed in float32 and
-    the last one is handed back in float32, unrounded. ``state`` (B, D) float32 is the state before the first step
-    (default zero). ``mask`` (B, L) or (L,) bool: a step off it leaves the state as it is, whatever x and gate hold there
-    (NaN too). Differentiable in x, gate and state (reverse mode).
+    x and gate (B, L, D), both float32 or both bfloat16 on the HIP device; any strides, read where they are if a
+    step's channels are neighbours (the halves of a joint projection). ``h`` is of their type; states are summed in
+    float32 and the last one is handed back in float32, unrounded. ``state`` (B, D) float32 is the state before the
+    first step (default zero). ``mask`` (B, L) or (L,) bool: a step off it leaves the state as it is, whatever x and
+    gate hold there (NaN too). Differentiable in x, gate and state (reverse mode). Steps are composed over stretches
+    of a sequence: where a stretch's product of linear gates leaves float32's range, its states are infinite or NaN,
+    also where they would have been zero.
 
-    One token at a time is L = 1. ``last`` (B, D) float32, contiguous, takes the last state, and may be ``state`` itself:
-    a decoding loop that updates its state in place, also in a captured graph. It is for calls that record no
+    One token at a time is L = 1. ``last`` (B, D) float32, contiguous, takes the last state, and may be ``state``
+    itself: a decoding loop that updates its state in place, also in a captured graph. It is for calls that record no
     gradients."""
     if form not in nat.GATED_SCAN_FORMS:
         raise ValueError(f"form must be one of {tuple(nat.GATED_SCAN_FORMS)}, got {form!r}")
@@ -128,7 +130,7 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
         end = start + last.numel() * 4
         own = state is None or state is last or (state.data_ptr() == start and state.is_contiguous())
         if _touches(x, start, end) or _touches(gate, start, end) or not own and _touches(state, start, end):
-            raise ValueError("last overlaps x, gate or a part of state: it may be state itself or apart from all of them")
+            raise ValueError("last overlaps x, gate or a part of state: it may be state itself or apart from them all")
     if B == 0 or L == 0:  # no step: the state stays
         end = x.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
         return x * gate, end if last is None else last.copy_(end)

@@ -735,7 +735,8 @@ size_t ews_gated_scan_workspace_bytes(const ews_gated_scan_desc* desc);
 
 /* out (B, L, D) contiguous and last (B, D) float32, the state after the last step. state (B, D) float32 may be NULL
  * (zero) or last itself; mask (B, L), one byte a step, may be NULL: a step whose byte is 0 leaves the state as it is.
- * residual may be NULL where no backward follows. */
+ * residual may be NULL where no backward follows. Where a stretch's product of linear gates leaves float32's range, its
+ * states are infinite or NaN. */
 int ews_gated_scan_forward(const ews_gated_scan_desc* desc, const void* x, const void* gate, const uint8_t* mask,
                            const float* state, void* out, float* last, void* residual, void* workspace,
                            ews_stream_t stream);

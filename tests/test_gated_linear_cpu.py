@@ -95,6 +95,25 @@ def test_scratch_of_what_is_read_where_it_is():
     assert lib.ews_gated_workspace_bytes(some, 4098, 6, 10, nat.GATED_FORWARD) > 0
 
 
+@pytest.mark.parametrize("N,H,F", [
+    (1 << 24, 4, 4), ((1 << 24) + 1, 4, 4), (6, 1 << 16, 100), (6, (1 << 16) + 1, 100), (6, 100, 1 << 20),
+    (6, 100, (1 << 20) + 1), (1 << 24, 512, 4), (1 << 24, 513, 4), (6, 1 << 13, 1 << 20), (6, (1 << 13) + 1, 1 << 20),
+    (1 << 24, 4, 1024), (1 << 24, 4, 1025), ((1 << 23) - 1, 1024, 65), ((1 << 23) + 1, 1024, 65), (1, 1, 1),
+])
+def test_sizes_that_fit_are_the_librarys(N, H, F):
+    from ews_mi355x.gated import _fits
+
+    tile = (ctypes.c_int32 * 5)()
+    d = _desc(rows=N, width=H, features=F, x_stride=H, weight_stride=H, gate_stride=H)
+    assert (nat.load().ews_gated_tile(d, 0, tile) == 0) == _fits(N, H, F)
+
+
+def test_sizes_that_do_not_fit_are_refused():
+    x = torch.zeros(1, 4).expand((1 << 24) + 1, 4)
+    with pytest.raises(ValueError, match="rows"):
+        E.gated_linear(x, torch.zeros(8, 4))
+
+
 def test_narrow_maps_keep_nothing():
     lib = nat.load()
     for H, F, narrow in ((64, 64, True), (1, 1, True), (65, 64, False), (64, 65, False)):
