@@ -22,12 +22,14 @@
 //
 // Narrow maps (both widths up to 64) have kernels of their own (ews_gated_narrow.h), and keep nothing.
 //
-// Few rows (decoding) are bound by V and G's bytes: k_few reads them straight into the matrix instructions' registers,
+// Few rows are bound by V and G's bytes: the forward's k_few reads them straight into the matrix instructions' registers,
 // many loads on their way at once, without LDS.
 //
 // Float32 numbers are multiplied as three bfloat16 planes and six products (ews_tiles.h), float32's accuracy. Sums are
 // float32, nothing is added with atomics: the same inputs give the same bits.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "ews_hip.h"
 #include "ews_pack.h"
@@ -189,6 +191,9 @@ struct Kept {
     __builtin_nontemporal_store(f32x4{e.x[0], e.x[1], e.x[2], e.x[3]}, reinterpret_cast<f32x4*>(to));
     __builtin_nontemporal_store(f32x4{e.x[4], e.x[5], e.x[6], e.x[7]}, reinterpret_cast<f32x4*>(to + 4));
   }
+  static __device__ __forceinline__ void store_four(void* kept, int64_t, int64_t at, const float (&x)[4]) {
+    *reinterpret_cast<f32x4*>((float*)kept + at) = f32x4{x[0], x[1], x[2], x[3]};
+  }
   static __device__ __forceinline__ void load(const void* kept, int64_t, int64_t at, float (&x)[8]) {
     const float* from = (const float*)kept + at;
 #pragma unroll
@@ -213,6 +218,15 @@ struct Kept<bf16> {
     }
     __builtin_nontemporal_store(hi, reinterpret_cast<u32x4*>((uint16_t*)kept + at));
     __builtin_nontemporal_store(lo, reinterpret_cast<u32x2*>((uint8_t*)kept + 2 * count + at));
+  }
+  static __device__ __forceinline__ void store_four(void* kept, int64_t count, int64_t at, const float (&x)[4]) {
+    uint32_t n[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) n[q] = __float_as_uint(x[q]) + 0x80u;
+    *reinterpret_cast<u32x2*>((uint16_t*)kept + at) =
+        u32x2{(n[0] >> 16) | (n[1] & 0xffff0000u), (n[2] >> 16) | (n[3] & 0xffff0000u)};
+    *reinterpret_cast<uint32_t*>((uint8_t*)kept + 2 * count + at) =
+        ((n[0] >> 8) & 0xffu) | (n[1] & 0xff00u) | ((n[2] >> 8) & 0xffu) << 16 | (n[3] & 0xff00u) << 16;
   }
   static __device__ __forceinline__ void load(const void* kept, int64_t count, int64_t at, float (&x)[8]) {
     const u32x4 hi = *reinterpret_cast<const u32x4*>((const uint16_t*)kept + at);
@@ -359,6 +373,8 @@ struct FewArgs {
   const void* gate_bias;
   int act;
   void* out;
+  void* kept;              // as ForwardArgs'; or null
+  int64_t ld;
 };
 
 constexpr int kFewWaves = 4;
@@ -366,22 +382,25 @@ constexpr int kFewWaves = 4;
 // A lane's eight numbers of 32 k of a row from column k on, zero past the row's end: bfloat16 k + 8 q .. 8 q + 7 for q
 // its fourth of the wavefront, float32 k + 4 q .. 4 q + 3 and 16 further on. Either way a load's lanes read 64 bytes of
 // a row; a product's k may be in any order that its operands share.
-template <typename T, bool WIDE>
+// kAligned: rows of whole eights at multiples of 16 bytes. kInside: all 32 k lie in the row, at any address (19 rows by
+// H=3761, F=6047, bfloat16: 64 us, number by number 126). kAny: neither is known.
+enum Rows16 { kAny, kAligned, kInside };
+template <typename T, Rows16 ROWS>
 __device__ __forceinline__ void few_eight(const T* row, int k, int H, T (&x)[8]) {
+  constexpr int kLoads = sizeof(T) == 4 ? 2 : 1, kEach = 8 / kLoads;
   const int q = (threadIdx.x >> 4) & 3;
-  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = k + 16 * h + 4 * q;
-      if (WIDE) {  // H is a multiple of 8
-        *reinterpret_cast<u32x4*>(x + 4 * h) = at < H ? *reinterpret_cast<const u32x4*>(row + at) : u32x4{0, 0, 0, 0};
-      } else {
+  for (int h = 0; h < kLoads; ++h) {
+    const int at = k + 16 * h + kEach * q;
+    if (ROWS == kAligned) {
+      *reinterpret_cast<u32x4*>(x + kEach * h) =
+          at < H ? *reinterpret_cast<const u32x4*>(row + at) : u32x4{0, 0, 0, 0};
+    } else if (ROWS == kInside || k + 32 <= H) {
+      __builtin_memcpy(x + kEach * h, row + at, 16);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * h + e] = at + e < H ? row[at + e] : 0.0f;
-      }
+      for (int e = 0; e < kEach; ++e) x[kEach * h + e] = at + e < H ? row[at + e] : narrow<T>(0.0f);
     }
-  } else {
-    eight_of<T>(row, k + 8 * q, H, WIDE, x);
   }
 }
 
@@ -403,12 +422,13 @@ __device__ __forceinline__ void few_sums(const FewArgs& a, f32x4v (&acc)[2][COLS
   const T* g = (const T*)a.g + own * a.gs;
 #pragma unroll
   for (int c = 0; c < COLS; ++c) acc[0][c] = acc[1][c] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k0 = wave * 32 * kAhead; k0 < a.H; k0 += kFewWaves * 32 * kAhead) {
+  auto stretch = [&](auto rows, int k0) {
+    constexpr Rows16 kRows = decltype(rows)::value;
     T wv[kAhead][8], wg[kAhead][8];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
-      few_eight<T, WIDE>(v, k0 + 32 * s, a.H, wv[s]);
-      few_eight<T, WIDE>(g, k0 + 32 * s, a.H, wg[s]);
+      few_eight<T, kRows>(v, k0 + 32 * s, a.H, wv[s]);
+      few_eight<T, kRows>(g, k0 + 32 * s, a.H, wg[s]);
     }
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
@@ -420,12 +440,20 @@ __device__ __forceinline__ void few_sums(const FewArgs& a, f32x4v (&acc)[2][COLS
         const int n = c * 16 + (lane & 15) < a.N ? c * 16 + (lane & 15) : a.N - 1;
         T x[8];
         bf16x8 fx[kPlanes<T>];
-        few_eight<T, WIDE>((const T*)a.x + n * a.xs, k0 + 32 * s, a.H, x);
+        few_eight<T, kRows>((const T*)a.x + n * a.xs, k0 + 32 * s, a.H, x);
         few_fragments<T, CAREFUL>(x, fx);
         mac(fv, fx, acc[0][c]);
         mac(fg, fx, acc[1][c]);
       }
     }
+  };
+  for (int k0 = wave * 32 * kAhead; k0 < a.H; k0 += kFewWaves * 32 * kAhead) {
+    if constexpr (WIDE)
+      stretch(std::integral_constant<Rows16, kAligned>{}, k0);
+    else if (k0 + 32 * kAhead <= a.H)
+      stretch(std::integral_constant<Rows16, kInside>{}, k0);
+    else
+      stretch(std::integral_constant<Rows16, kAny>{}, k0);
   }
 }
 
@@ -463,12 +491,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
     }
     const int n = c * 16 + (lane & 15), f = blockIdx.x * 16 + (lane >> 4) * 4;
     if (n >= a.N) continue;
+    float v[4], g[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      if (f + r >= a.F) continue;
+      const int in = f + r < a.F ? f + r : a.F - 1;
+      v[r] = sv[r] + bias_at<T>(a.bias, in);
+      g[r] = sg[r] + bias_at<T>(a.gate_bias, in);
       float act, slope;
-      activate(a.act, sg[r] + bias_at<T>(a.gate_bias, f + r), act, slope);
-      ((T*)a.out)[(int64_t)n * a.F + f + r] = narrow<T>((sv[r] + bias_at<T>(a.bias, f + r)) * act);
+      activate(a.act, g[r], act, slope);
+      if (f + r < a.F) ((T*)a.out)[(int64_t)n * a.F + f + r] = narrow<T>(v[r] * act);
+    }
+    if (a.kept && f < a.F) {
+      Kept<T>::store_four(a.kept, 2 * a.ld * a.N, (int64_t)n * 2 * a.ld + f, v);
+      Kept<T>::store_four(a.kept, 2 * a.ld * a.N, (int64_t)n * 2 * a.ld + a.ld + f, g);
     }
   }
 }
@@ -739,7 +774,7 @@ using tiles::Operand;
 using tiles::Product;
 using ews::vec::bf16;
 
-// Rows up to which a forward alone reads V and G straight into registers: 32 of H=4096, F=11000 48 us in bfloat16 (by
+// Rows up to which a forward reads V and G straight into registers: 32 of H=4096, F=11000 48 us in bfloat16 (by
 // the tiles 51), 33 rows 55 (48); float32, whose tiles need planes packed first, 64 rows 180 (420).
 constexpr int kFewRows = 32, kFewRows32 = 64;
 // Splits that one thread adds; more are added by eight groups of threads.
@@ -809,8 +844,8 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
   // a launch has fewer than 2^32 threads, one for eight numbers; dv | dg's rows lie within the tiles' offsets
   if (p.Np * p.Hp > (int64_t)1 << 33 || p.F * p.Hp > (int64_t)1 << 33 || p.Np * p.ld > (int64_t)1 << 34)
     return EWS_ERR_SHAPE;
-  p.few = !back && !keep && p.N <= (p.np == 3 ? kFewRows32 : kFewRows);
-  p.narrow = p.H <= kNarrowWidth && p.F <= kNarrowWidth && !p.few;
+  p.few = p.N <= (p.np == 3 ? kFewRows32 : kFewRows);
+  p.narrow = p.H <= kNarrowWidth && p.F <= kNarrowWidth && (back || keep || !p.few);  // and keeps nothing
   if (p.narrow) {
     // 32 rows a wavefront and turn; as many workgroups as are on the CUs at a time
     const int groups = ceil_div(p.N, 32 * 4);
@@ -832,7 +867,7 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
     off += tiles::al256x(bytes);
     return at;
   };
-  if (!p.few) {
+  if (back || !p.few) {
     p.xp = take(p.pack_x ? (size_t)(p.N * p.Hp * p.np * 2) : 0);
     p.wp = take(p.pack_w ? (size_t)(2 * p.F * p.Hp * p.np * 2) : 0);
   }
@@ -925,9 +960,7 @@ template <typename O, bool KEEP>
 int launch_forward(Kind kind, const ForwardArgs& a, hipStream_t st) {
   constexpr int kP = sizeof(O) == 4 ? tiles::kPairs : 1;
   if (kind == tiles::kLarge) return launch_forward_as<tiles::Large, kP, O, KEEP>(a, st);
-  // without a backward few rows have a kernel of their own
-  if (!KEEP || kind == tiles::kMedium) return launch_forward_as<tiles::Medium, kP, O, KEEP>(a, st);
-  return launch_forward_as<tiles::Flat, kP, O, true>(a, st);
+  return launch_forward_as<tiles::Medium, kP, O, KEEP>(a, st);  // few rows have a kernel of their own
 }
 
 template <typename O>
@@ -1076,7 +1109,7 @@ int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile) {
   if (rc != EWS_OK) return rc;
   if (!tile) return EWS_ERR_NULL;
   if (product < 0 || product > 2) return EWS_ERR_OPTION;
-  if (p.narrow) {
+  if (p.narrow || (product == 0 && p.few)) {
     for (int k = 0; k < 5; ++k) tile[k] = 0;
     return EWS_OK;
   }
@@ -1100,10 +1133,10 @@ int ews_gated_forward(const ews_gated_desc* desc, const void* x, const void* wei
   c.s = desc;
   c.w = (char*)workspace;
   c.st = (hipStream_t)stream;
-  if (c.p.few) {
+  if (c.p.few && !c.p.narrow) {
     const FewArgs a{x,       weight,  gate_weight, desc->x_stride, desc->weight_stride, desc->gate_stride,
                     c.p.N,   c.p.H,   c.p.F,       bias,           gate_bias,           desc->activation,
-                    out};
+                    out,     kept,    c.p.ld};
     const bool wide = c.p.H % 8 == 0 && tiles::rows_wide(x, desc->x_stride, f32) &&
                       tiles::rows_wide(weight, desc->weight_stride, f32) &&
                       tiles::rows_wide(gate_weight, desc->gate_stride, f32);

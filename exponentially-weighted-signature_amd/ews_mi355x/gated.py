@@ -132,8 +132,8 @@ def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activat
     form) or "relu". The result (..., F) is rounded to x's type once.
 
     Differentiable in everything (reverse mode). A call that records gradients keeps both products' sums, of 24
-    bits each (float32: 32), beside the result, unless H and F are 64 at most. A few rows without gradients (a decoding
-    step: 32, of float32 64) read the weights once, at the memory's rate."""
+    bits each (float32: 32), beside the result, unless H and F are 64 at most. A few rows (a decoding step:
+    32, of float32 64) read the weights once, at the memory's rate."""
     if activation not in nat.GATED_ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(nat.GATED_ACTIVATIONS)}, got {activation!r}")
     joint = gate_weight is None
