@@ -22,8 +22,8 @@
 //
 // Narrow maps (both widths up to 64) have kernels of their own (ews_gated_narrow.h), and keep nothing.
 //
-// Few rows are bound by V and G's bytes: the forward's k_few reads them straight into the matrix instructions' registers,
-// many loads on their way at once, without LDS.
+// Few rows are bound by V and G's bytes: the forward's k_few reads them straight into the matrix instructions'
+// registers, many loads on their way at once, without LDS.
 //
 // Float32 numbers are multiplied as three bfloat16 planes and six products (ews_tiles.h), float32's accuracy. Sums are
 // float32, nothing is added with atomics: the same inputs give the same bits.
@@ -508,6 +508,129 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
   }
 }
 
+// x's gradient of few float32 rows: V and G are read as they are, a lane four columns of eight rows, the eight k of
+// four operands. One row by H=1066, F=14344 40 us, by the tiles 49 and 67 to pack the weights for them; 48 rows by
+// H=1024, F=4096 26 (22 and 12). bfloat16, with eight columns a lane, turns too much in registers: 32 rows by H=4096,
+// F=11000 78 (by the tiles 33, nothing to pack).
+struct FewDxArgs {
+  const uint16_t* dz;      // as DzArgs'
+  int64_t plane, ld;
+  const float* v;
+  const float* g;
+  int64_t ws, gs;
+  int N, H, F;
+  int blocks, per;         // of 32 rows of V and then of G; of a workgroup
+  float* part;             // (workgroups along y, N, H)
+};
+
+constexpr int kDxCols = 4;
+
+// One wavefront's part of the sums over f, of 16 ROWS rows and 64 columns.
+template <int ROWS, bool CAREFUL>
+__device__ __forceinline__ void few_dx_sums(const FewDxArgs& a, int b0, int b1, f32x4v (&acc)[ROWS][kDxCols]) {
+  constexpr int NP = kPlanes<float>, kAhead = 2;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+  const int h = ((int)blockIdx.x * 16 + r16) * kDxCols, sides = a.blocks / 2;
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j)
+#pragma unroll
+    for (int c = 0; c < kDxCols; ++c) acc[j][c] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+  float w[kAhead][8][kDxCols];
+  auto load = [&](int s, int b) {
+    const bool gate = b >= sides;
+    const float* from = gate ? a.g : a.v;
+    const int64_t stride = gate ? a.gs : a.ws;
+    const int f = (gate ? b - sides : b) * 32 + 8 * q;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float* row = from + (f + i < a.F ? f + i : a.F - 1) * stride;  // those past F meet zeros
+      if (h + kDxCols <= a.H) {
+        __builtin_memcpy(w[s][i], row + h, 16);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kDxCols; ++c) w[s][i][c] = h + c < a.H ? row[h + c] : 0.0f;
+      }
+    }
+  };
+  for (int b = b0; b < b1; b += kAhead) {
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+      if (b + s < b1) load(s, b + s);
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      if (b + s >= b1) break;
+      const bool gate = b + s >= sides;
+      const int64_t at = (gate ? a.ld : 0) + (gate ? b + s - sides : b + s) * 32 + 8 * q;
+      bf16x8 z[ROWS][NP];
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j)
+#pragma unroll
+        for (int k = 0; k < NP; ++k)
+          z[j][k] = *reinterpret_cast<const bf16x8*>(a.dz + k * a.plane + (int64_t)(j * 16 + r16) * 2 * a.ld + at);
+#pragma unroll
+      for (int c = 0; c < kDxCols; ++c) {
+        float x[8];
+        bf16x8 fw[NP];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = w[s][i][c];
+        cut<CAREFUL>(x, fw);
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) mac(z[j], fw, acc[j][c]);
+      }
+    }
+  }
+}
+
+template <int ROWS>
+__global__ __launch_bounds__(64 * kFewWaves) void k_few_dx(FewDxArgs a) {
+  __shared__ f32x4v part[kFewWaves - 1][ROWS * kDxCols][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int first = blockIdx.y * a.per, last = first + a.per < a.blocks ? first + a.per : a.blocks;
+  const int each = (a.per + kFewWaves - 1) / kFewWaves;
+  const int b0 = first + wave * each < last ? first + wave * each : last, b1 = b0 + each < last ? b0 + each : last;
+  f32x4v acc[ROWS][kDxCols];
+  few_dx_sums<ROWS, false>(a, b0, b1, acc);
+  bool bad = false;  // as in k_few
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j)
+#pragma unroll
+    for (int c = 0; c < kDxCols; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bad |= __builtin_isnan(acc[j][c][r]);
+  if (__any(bad)) few_dx_sums<ROWS, true>(a, b0, b1, acc);
+  if (wave)
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j)
+#pragma unroll
+      for (int c = 0; c < kDxCols; ++c) part[wave - 1][j * kDxCols + c][lane] = acc[j][c];
+  __syncthreads();
+  if (wave) return;
+  const int h = ((int)blockIdx.x * 16 + (lane & 15)) * kDxCols;
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+#pragma unroll
+    for (int c = 0; c < kDxCols; ++c)
+#pragma unroll
+      for (int w = 0; w < kFewWaves - 1; ++w) acc[j][c] += part[w][j * kDxCols + c][lane];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = j * 16 + (lane >> 4) * 4 + r;
+      if (n >= a.N) continue;
+      float* to = a.part + ((int64_t)blockIdx.y * a.N + n) * a.H + h;
+      float x[kDxCols];
+#pragma unroll
+      for (int c = 0; c < kDxCols; ++c) x[c] = acc[j][c][r];
+      if (h + kDxCols <= a.H) {
+        __builtin_memcpy(to, x, sizeof(x));
+      } else {
+#pragma unroll
+        for (int c = 0; c < kDxCols; ++c)
+          if (h + c < a.H) to[c] = x[c];
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------ dv | dg
 struct DzArgs {
   const void* dy;          // (N, F)
@@ -774,8 +897,8 @@ using tiles::Operand;
 using tiles::Product;
 using ews::vec::bf16;
 
-// Rows up to which a forward reads V and G straight into registers: 32 of H=4096, F=11000 48 us in bfloat16 (by
-// the tiles 51), 33 rows 55 (48); float32, whose tiles need planes packed first, 64 rows 180 (420).
+// Rows up to which V and G go straight into registers (the measured: of a forward): 32 of H=4096, F=11000 48 us in
+// bfloat16 (by the tiles 51), 33 rows 55 (48); float32, whose tiles need planes packed first, 64 rows 180 (420).
 constexpr int kFewRows = 32, kFewRows32 = 64;
 // Splits that one thread adds; more are added by eight groups of threads.
 constexpr int kFewSplits = 8;
@@ -813,10 +936,11 @@ GProduct share(const Product& of) {
 struct GPlan {
   int N, H, F, np;
   int64_t Hp, ld, Np;
-  bool pack_x, pack_w, few, narrow;
+  bool pack_x, pack_w, few, few_dx, narrow;
   Product forward;
   GProduct dx, dw;
   int dz_rows, dz_parts, narrow_groups;
+  int dx_blocks, dx_per, dx_parts;  // of few_dx
   size_t xp, wp, dz, sums, part, total;
 };
 
@@ -855,8 +979,9 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
     return EWS_OK;
   }
   p.pack_x = p.np == 3 || !direct(x, s->x_stride, p.H);
-  p.pack_w = p.np == 3 || !direct(v, s->weight_stride, p.H) || !direct(g, s->gate_stride, p.H) ||
-             s->weight_stride != s->gate_stride || ((uintptr_t)g - (uintptr_t)v) % 2;
+  p.few_dx = back && p.few && p.np == 3;
+  p.pack_w = !p.few_dx && (p.np == 3 || !direct(v, s->weight_stride, p.H) || !direct(g, s->gate_stride, p.H) ||
+             s->weight_stride != s->gate_stride || ((uintptr_t)g - (uintptr_t)v) % 2);
   const int pairs = p.np == 3 ? tiles::kPairs : 1;
   p.forward = tiles::pick(2 * p.ld, p.N, (int)(p.Hp / 64), pairs, false, false);
   p.dx = share(tiles::pick(p.H, p.N, (int)(2 * p.ld / 64), pairs, true, false));
@@ -879,7 +1004,15 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
     while (ceil_div(p.Np, p.dz_rows) > 65535) p.dz_rows *= 2;  // a grid's second side
     p.dz_parts = ceil_div(p.Np, p.dz_rows);
     p.sums = take((size_t)p.dz_parts * 2 * p.ld * 4);
-    const size_t dx = p.dx.part_bytes(p.H, p.N), dw = p.dw.part_bytes(p.H, 2 * p.ld);
+    // four workgroups a CU, of eight blocks at least
+    const int wide = ceil_div(p.H, 16 * kDxCols);
+    p.dx_blocks = 2 * ceil_div(p.F, 32);
+    p.dx_parts = ceil_div(1024, wide);
+    if (p.dx_parts > ceil_div(p.dx_blocks, 8)) p.dx_parts = ceil_div(p.dx_blocks, 8);
+    p.dx_per = ceil_div(p.dx_blocks, p.dx_parts);
+    p.dx_parts = ceil_div(p.dx_blocks, p.dx_per);
+    const size_t dx = p.few_dx ? (size_t)p.dx_parts * p.N * p.H * 4 : p.dx.part_bytes(p.H, p.N);
+    const size_t dw = p.dw.part_bytes(p.H, 2 * p.ld);
     p.part = take(dx > dw ? dx : dw);
   }
   p.total = off;
@@ -981,6 +1114,18 @@ int launch_few(const FewArgs& a, hipStream_t st) {
   return EWS_OK;
 }
 
+int launch_few_dx(const FewDxArgs& a, int parts, hipStream_t st) {
+  const dim3 grid(ceil_div(a.H, 16 * kDxCols), parts), block(64 * kFewWaves);
+  if (a.N <= 16)
+    hipLaunchKernelGGL(k_few_dx<1>, grid, block, 0, st, a);
+  else if (a.N <= 32)
+    hipLaunchKernelGGL(k_few_dx<2>, grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL(k_few_dx<4>, grid, block, 0, st, a);
+  GATED_CHECK();
+  return EWS_OK;
+}
+
 template <class T, int PAIRS, bool ROWS, typename O>
 int launch_grad_as(const GradArgs& a, hipStream_t st) {
   const int lds = tiles::lds_bytes<T, PAIRS>(a.per);
@@ -1003,6 +1148,19 @@ int launch_grad_as(const GradArgs& a, hipStream_t st) {
 }
 
 template <bool ROWS, typename O>
+int launch_join(const GradArgs& a, hipStream_t st) {
+  const int64_t n = (int64_t)a.J * a.I;
+  if (a.splits > kFewSplits)
+    hipLaunchKernelGGL((k_join<ROWS, O, One, 8>), dim3((uint32_t)((n + 31) / 32)), dim3(256), 0, st, a);
+  else if (a.wide)
+    hipLaunchKernelGGL((k_join<ROWS, O, Eight, 1>), dim3((uint32_t)((n / 8 + 255) / 256)), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((k_join<ROWS, O, One, 1>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
+  GATED_CHECK();
+  return EWS_OK;
+}
+
+template <bool ROWS, typename O>
 int launch_grad(const GProduct& p, GradArgs a, hipStream_t st) {
   constexpr int kP = sizeof(O) == 4 ? tiles::kPairs : 1;
   a.ti = p.ti;
@@ -1015,20 +1173,11 @@ int launch_grad(const GProduct& p, GradArgs a, hipStream_t st) {
   int rc;
   if (p.kind == tiles::kLarge)
     rc = launch_grad_as<tiles::Large, kP, ROWS, O>(a, st);
-  else if (ROWS || p.kind == tiles::kMedium)  // the weights' gradients are 128 rows at least
+  else if (ROWS || sizeof(O) == 4 || p.kind == tiles::kMedium)
     rc = launch_grad_as<tiles::Medium, kP, ROWS, O>(a, st);
-  else
-    rc = launch_grad_as<tiles::Flat, kP, false, O>(a, st);
-  if (rc != EWS_OK || a.splits == 1) return rc;
-  const int64_t n = (int64_t)a.J * a.I;
-  if (a.splits > kFewSplits)
-    hipLaunchKernelGGL((k_join<ROWS, O, One, 8>), dim3((uint32_t)((n + 31) / 32)), dim3(256), 0, st, a);
-  else if (a.wide)
-    hipLaunchKernelGGL((k_join<ROWS, O, Eight, 1>), dim3((uint32_t)((n / 8 + 255) / 256)), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((k_join<ROWS, O, One, 1>), dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, a);
-  GATED_CHECK();
-  return EWS_OK;
+  else  // the weights' gradients are 128 rows at least, and few float32 rows of x's have a kernel of their own
+    rc = launch_grad_as<tiles::Flat, 1, false, bf16>(a, st);
+  return rc != EWS_OK || a.splits == 1 ? rc : launch_join<ROWS, O>(a, st);
 }
 
 template <typename T, bool SUMS>
@@ -1109,7 +1258,7 @@ int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile) {
   if (rc != EWS_OK) return rc;
   if (!tile) return EWS_ERR_NULL;
   if (product < 0 || product > 2) return EWS_ERR_OPTION;
-  if (p.narrow || (product == 0 && p.few)) {
+  if (p.narrow || (product == 0 && p.few) || (product == 1 && p.few_dx)) {
     for (int k = 0; k < 5; ++k) tile[k] = 0;
     return EWS_OK;
   }
@@ -1204,7 +1353,7 @@ int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* we
     GATED_CHECK();
     return EWS_OK;
   }
-  rc = operands(c, x, weight, gate_weight, weights, grad_x != nullptr);
+  rc = operands(c, x, weight, gate_weight, weights, grad_x && !p.few_dx);
   if (rc != EWS_OK) return rc;
   DzArgs z{};
   z.dy = grad_out;
@@ -1240,7 +1389,18 @@ int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* we
   a.F = p.F;
   a.ld = (int)p.ld;
   a.part = (float*)(c.w + p.part);
-  if (grad_x) {
+  if (grad_x && p.few_dx) {
+    const FewDxArgs d{z.dz, z.plane, p.ld, (const float*)weight, (const float*)gate_weight, desc->weight_stride,
+                      desc->gate_stride, p.N, p.H, p.F, p.dx_blocks, p.dx_per, a.part};
+    rc = launch_few_dx(d, p.dx_parts, c.st);
+    if (rc != EWS_OK) return rc;
+    a.splits = p.dx_parts;
+    a.J = p.N;
+    a.out = grad_x;
+    a.wide = results_wide(grad_x, p.H);
+    rc = launch_join<false, float>(a, c.st);
+    if (rc != EWS_OK) return rc;
+  } else if (grad_x) {
     a.W = Chain{c.v, c.to_g, (int)(p.ld / 64)};
     a.Z = Operand{z.dz, 2 * p.ld, z.plane, (int)p.Np, 0};
     a.J = p.N;

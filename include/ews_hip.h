@@ -780,7 +780,7 @@ size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, cons
 /* For tests and profiles: of product 0 (v and g), 1 (grad_x) or 2 (the weights'
  * gradients) tile[0] x tile[1] = the results of one workgroup, tile[2] = the splits of its sum, and tile[3] of the
  * tile[4] tiles are done by a workgroup each, the others shared by several. All 0 where H and F are 64 at most, and
- * of product 0 where rows are few (32; float32 64): those have kernels of their own. */
+ * of product 0 (float32: and 1) where rows are few (32; float32 64): those have kernels of their own. */
 int ews_gated_tile(const ews_gated_desc* desc, int product, int32_t* tile);
 
 /* out (N, F), contiguous, = (x weight^T + bias) act(x gate_weight^T + gate_bias); weight and gate_weight (F, H), either

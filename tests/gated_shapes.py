@@ -11,7 +11,7 @@ TILES = {
     ("bfloat16", 1100, 520, 3330): (LARGE, MEDIUM, MEDIUM),
     ("float32", 300, 136, 700): (MEDIUM, MEDIUM, MEDIUM),
     ("bfloat16", 300, 136, 700): (MEDIUM, MEDIUM, MEDIUM),
-    ("float32", 30, 520, 600): (OWN, FLAT, MEDIUM),
+    ("float32", 30, 520, 600): (OWN, OWN, MEDIUM),
     ("bfloat16", 30, 520, 600): (OWN, FLAT, MEDIUM),
 }
 

@@ -254,6 +254,22 @@ def test_infinities(N, H, F, dtype):
         assert torch.equal(y[there].double(), want[there])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [7, 30, 60, 90])
+def test_gradients_of_infinite_weights(N, dtype):
+    """An infinite weight makes x's gradient infinite or NaN where the formula's is."""
+    x, w, b, gw, gb, up = _inputs(N, 200, 40, dtype, joint=False)
+    w[4, 9] = float("inf")
+    xd, V, G = x.double(), w.double(), gw.double()
+    v, s = xd @ V.t() + b.double(), torch.sigmoid(xd @ G.t() + gb.double())
+    want = (up.double() * s) @ V + (up.double() * v * s * (1 - s)) @ G
+    leaf = x.clone().requires_grad_()
+    got, = torch.autograd.grad(E.gated_linear(leaf, w, b, gw, gb), leaf, up)
+    assert not bool(want.isfinite().any()) and torch.equal(got.isnan(), want.isnan())
+    there = ~want.isnan()
+    assert torch.equal(got[there].double(), want[there])
+
+
 def test_gradient_against_differences():
     for name in ("sigmoid", "silu", "gelu"):
         x, w, b, _, _, up = _inputs(90, 32, 24, torch.float32)
