@@ -528,8 +528,9 @@ int scan_plan(const ews_gated_scan_desc* s, SPlan& p) {
     return EWS_ERR_SHAPE;
   if (s->x_step < 0 || s->gate_step < 0 || s->x_batch < 0 || s->gate_batch < 0 || s->mask_batch < 0)
     return EWS_ERR_SHAPE;
-  p.pairs = s->dtype == EWS_DTYPE_BF16 && s->dim % 2 == 0 && s->x_step % 2 == 0 && s->gate_step % 2 == 0 &&
-            s->x_batch % 2 == 0 && s->gate_batch % 2 == 0;
+  // The plan asks for sizes and types alone, so that a backward finds the forward's tiles in the residual whatever x's
+  // and gate's strides have become; rows of pairs that do not start at whole words are read number by number.
+  p.pairs = s->dtype == EWS_DTYPE_BF16 && s->dim % 2 == 0;
   const int cells = p.pairs ? s->dim / 2 : s->dim;  // threads that the channels need
   // threads that walk alone: where sixteen wavefronts a CU can (bfloat16 64 x 512 x 4096 both ways: 437 us, by strips
   // 455; half as many wavefronts: 510, by strips 456), or a sequence is but one or two of their tiles
@@ -625,6 +626,12 @@ int scan_launch(const ews_gated_scan_desc* s, const Args& a, const SPlan& p, boo
 
 bool words(const void* p) { return (uintptr_t)p % 4 == 0; }
 
+// Whether x's and gate's steps start at whole words.
+bool word_steps(const ews_gated_scan_desc* s, const void* x, const void* gate) {
+  return s->x_step % 2 == 0 && s->gate_step % 2 == 0 && s->x_batch % 2 == 0 && s->gate_batch % 2 == 0 && words(x) &&
+         words(gate);
+}
+
 }  // namespace
 
 extern "C" {
@@ -648,7 +655,7 @@ int ews_gated_scan_forward(const ews_gated_scan_desc* desc, const void* x, const
   const int rc = scan_plan(desc, p);
   if (rc != EWS_OK) return rc;
   if (!x || !gate || !out || !last || (p.segs > 1 && !workspace)) return EWS_ERR_NULL;
-  const bool pairs = p.pairs && words(x) && words(gate) && words(out);
+  const bool pairs = p.pairs && word_steps(desc, x, gate) && words(out);
   Args a = scan_args(desc, p, pairs, x, gate, mask, workspace);
   a.state = state;
   a.h = out;
@@ -664,7 +671,8 @@ int ews_gated_scan_backward(const ews_gated_scan_desc* desc, const void* x, cons
   const int rc = scan_plan(desc, p);
   if (rc != EWS_OK) return rc;
   if (!x || !gate || !residual || !grad_x || !grad_gate || (p.segs > 1 && !workspace)) return EWS_ERR_NULL;
-  const bool pairs = p.pairs && words(x) && words(gate) && words(grad_out) && words(grad_x) && words(grad_gate);
+  const bool pairs =
+      p.pairs && word_steps(desc, x, gate) && words(grad_out) && words(grad_x) && words(grad_gate);
   Args a = scan_args(desc, p, pairs, x, gate, mask, workspace);
   a.starts = (float*)residual;
   a.dh = grad_out;

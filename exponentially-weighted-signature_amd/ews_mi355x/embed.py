@@ -32,6 +32,30 @@ def once(backward):
     return run
 
 
+def stamps(tensors):
+    """Where tensors (or None) lie and how: what a call's descriptor and scratch are made for."""
+    return [t if t is None else (t.data_ptr(), t.dtype, t.shape, t.stride()) for t in tensors]
+
+
+def unmoved(tensors, made_for, dev):
+    """Whether saved tensors came back as the forward left them (``made_for``, their ``stamps``). Hooks on saved tensors
+    may bring them back at other addresses, with other strides; of another type, shape or device they are refused."""
+    now = stamps(tensors)
+    if now == made_for:
+        return True
+    for t, n, m in zip(tensors, now, made_for):
+        if n is not None and (n[1:3] != m[1:3] or t.device != dev):
+            raise RuntimeError(f"a saved tensor came back as {n[1]} {tuple(n[2])} on {t.device}: it was {m[1]} "
+                               f"{tuple(m[2])} on {dev}")
+    return False
+
+
+def aligned(t):
+    """A saved buffer of the library's own, contiguous, at a multiple of 16 bytes (a copy only where it is not)."""
+    return t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(
+        memory_format=torch.contiguous_format)
+
+
 def refuse_tangents(tensors):
     """Forward-mode derivatives are not formed: a tensor (or None) that carries one is refused, as an autograd function
     without a jvp refuses it, not answered without a tangent, which would read as a derivative of zero."""

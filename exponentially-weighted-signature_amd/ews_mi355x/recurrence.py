@@ -8,7 +8,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _native as nat
-from .embed import DTYPES, check_tensor, launch, once, refuse_tangents
+from .embed import DTYPES, aligned, check_tensor, launch, once, refuse_tangents, stamps, unmoved
 
 
 def _ptr(t):
@@ -29,15 +29,26 @@ def _touches(t, start, end):
     return first + span * t.element_size() > start
 
 
+def _readable(x, gate, mask):
+    """x, gate and mask (B, L) or None as the library can read them."""
+    if mask is not None and mask.stride(1) != 1 and mask.shape[1] > 1:
+        mask = mask.contiguous()
+    return _neighbours(x), _neighbours(gate), mask
+
+
+def _describe(x, gate, mask, form):
+    return nat.GatedScanDesc(x.stride(0), x.stride(1), gate.stride(0), gate.stride(1),
+                             0 if mask is None else mask.stride(0), *x.shape, DTYPES[x.dtype],
+                             nat.GATED_SCAN_FORMS[form])
+
+
 def _forward(x, gate, mask, state, last, form, train):
     """(out, last, the descriptor and the scratch's size, the residual of a training call)."""
     B, L, D = x.shape
     out = x.new_empty((B, L, D))
     if last is None:
         last = x.new_empty((B, D), dtype=torch.float32)
-    desc = nat.GatedScanDesc(x.stride(0), x.stride(1), gate.stride(0), gate.stride(1),
-                             0 if mask is None else mask.stride(0), B, L, D, DTYPES[x.dtype],
-                             nat.GATED_SCAN_FORMS[form])
+    desc = _describe(x, gate, mask, form)
     lib = nat.load()
     residual = x.new_empty(lib.ews_gated_scan_residual_bytes(desc), dtype=torch.uint8) if train else None
     size = lib.ews_gated_scan_workspace_bytes(desc)
@@ -50,8 +61,10 @@ def _forward(x, gate, mask, state, last, form, train):
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, state, mask, form):
-        out, last, ctx.args, residual = _forward(x, gate, mask, state, None, form, True)
-        ctx.save_for_backward(x, gate, mask, residual)
+        out, last, (desc, size), residual = _forward(x, gate, mask, state, None, form, True)
+        saved = x, gate, mask, residual
+        ctx.save_for_backward(*saved)
+        ctx.args = desc, size, form, stamps(saved)
         ctx.set_materialize_grads(False)
         return out, last
 
@@ -60,7 +73,11 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, gout, glast):
         if gout is None and glast is None:
             return None, None, None, None, None
-        x, gate, mask, residual = ctx.saved_tensors
+        x, gate, mask, residual = saved = ctx.saved_tensors
+        desc, size, form, made_for = ctx.args
+        if not unmoved(saved, made_for, (glast if gout is None else gout).device):
+            x, gate, mask = _readable(x, gate, mask)
+            desc, residual = _describe(x, gate, mask, form), aligned(residual)  # the scratch's size asks for no strides
         if gout is not None:
             gout = gout.contiguous()
         if glast is not None:
@@ -68,7 +85,6 @@ class _GatedScan(torch.autograd.Function):
         gx, ggate = x.new_empty(x.shape), x.new_empty(x.shape)
         gstate = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         lib = nat.load()
-        desc, size = ctx.args
         ws = x.new_empty(size, dtype=torch.uint8) if size else None
         nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, x.data_ptr(), gate.data_ptr(), _ptr(mask),
                          residual.data_ptr(), _ptr(gout), _ptr(glast), gx.data_ptr(), ggate.data_ptr(), _ptr(gstate),
@@ -134,11 +150,7 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
     if B == 0 or L == 0:  # no step: the state stays
         end = x.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
         return x * gate, end if last is None else last.copy_(end)
-    x, gate = _neighbours(x), _neighbours(gate)
-    if mask is not None:
-        mask = mask.expand(B, L)
-        if mask.stride(1) != 1 and L > 1:
-            mask = mask.contiguous()
+    x, gate, mask = _readable(x, gate, None if mask is None else mask.expand(B, L))
     if state is not None:
         state = state.contiguous()
     if train:

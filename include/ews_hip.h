@@ -729,7 +729,8 @@ typedef struct ews_gated_scan_desc {
   int32_t form;                  /* EWS_GATED_SCAN_* */
 } ews_gated_scan_desc;
 
-/* The residual that a forward leaves for its backward, and the scratch of either (0: may be NULL). */
+/* The residual that a forward leaves for its backward, and the scratch of either (0: may be NULL). Both depend on batch,
+ * length, dim, dtype and form alone: a backward may be given x and gate with other strides than its forward. */
 size_t ews_gated_scan_residual_bytes(const ews_gated_scan_desc* desc);
 size_t ews_gated_scan_workspace_bytes(const ews_gated_scan_desc* desc);
 

@@ -1,0 +1,100 @@
+"""What the backward calls of ``gated_scan`` hand to the library where hooks on saved tensors bring them back with other
+strides or at other addresses: descriptors and scratch of the tensors that came back. The launches are recorded, not run."""
+
+import ctypes
+
+import pytest
+import torch
+
+from ews_mi355x import _native as nat
+from ews_mi355x import recurrence
+
+
+def _value(a):
+    return a.value if isinstance(a, ctypes.c_void_p) else a
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+
+    def record(dev, fn, *args):
+        made.append((fn.__name__, [_value(a) for a in args]))
+        return 0
+
+    monkeypatch.setattr(recurrence, "launch", record)
+    return made
+
+
+class _Elsewhere:
+    """Hooks that bring saved tensors back contiguous, ``off`` bytes behind a multiple of 64."""
+
+    def __init__(self, off=0):
+        self.off, self.came = off, {}
+
+    def unpack(self, t):
+        size = t.element_size()
+        flat = torch.empty(t.numel() * size + 192, dtype=torch.uint8)
+        flat = flat[-flat.data_ptr() % 64 + self.off:][:t.numel() * size].view(t.dtype).view(t.shape)
+        flat.copy_(t)
+        self.came[flat.data_ptr()] = flat
+        return flat
+
+    def __enter__(self):
+        self.hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t, self.unpack)
+        self.hooks.__enter__()
+        return self
+
+    def __exit__(self, *args):
+        self.hooks.__exit__(*args)
+
+
+def _halves(B, L, D, dtype):
+    joint = torch.randn(B, L, 2 * D).to(dtype).requires_grad_()
+    return joint, joint.chunk(2, -1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("masked", [False, True])
+def test_scan_backward_describes_what_came_back(calls, dtype, masked):
+    _, (x, gate) = _halves(2, 30, 24, dtype)
+    mask = (torch.arange(30) % 3 != 0).expand(2, 30) if masked else None
+    with _Elsewhere() as there:
+        h, last = recurrence._GatedScan.apply(x, gate, None, mask, "convex")
+    (h.float().sum() + last.sum()).backward()
+    (_, forward), (name, (desc, px, pg, pm, *_)) = calls
+    assert name == "ews_gated_scan_backward" and (forward[0].x_batch, forward[0].x_step) == (30 * 48, 48)
+    for p, stride in ((px, (desc.x_batch, desc.x_step)), (pg, (desc.gate_batch, desc.gate_step))):
+        assert there.came[p].stride() == (*stride, 1)
+    if masked:
+        assert there.came[pm].stride(0) == desc.mask_batch
+
+
+def test_scan_backward_without_hooks_reads_where_the_forward_did(calls):
+    _, (x, gate) = _halves(2, 30, 24, torch.float32)
+    h, _ = recurrence._GatedScan.apply(x, gate, None, None, "convex")
+    h.sum().backward()
+    (_, f), (_, b) = calls
+    assert b[0] is f[0] and b[1:3] == f[1:3]
+
+
+def test_scan_refuses_a_saved_tensor_of_another_type_or_shape(calls):
+    for change, says in ((lambda t: t.double() if t.is_floating_point() else t, "came back as torch.float64"),
+                         (lambda t: t[..., :3].contiguous() if t.dim() == 3 else t, r"\(2, 30, 3\)")):
+        _, (x, gate) = _halves(2, 30, 24, torch.float32)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            h, _ = recurrence._GatedScan.apply(x, gate, None, None, "convex")
+        with pytest.raises(RuntimeError, match=says):
+            h.sum().backward()
+    assert all(name != "ews_gated_scan_backward" for name, _ in calls)
+
+
+@pytest.mark.parametrize("B,L,D", [(1, 17, 2), (2, 200, 24), (8, 4095, 2048), (1, 131071, 1024), (600, 17, 450)])
+def test_the_residual_does_not_depend_on_strides(B, L, D):
+    """The tiles whose first states a forward leaves are those that its backward looks for."""
+    lib = nat.load()
+    sizes = set()
+    for step in (D, 2 * D, 2 * D + 1):
+        d = nat.GatedScanDesc(L * step, step, L * D, D, L, B, L, D, nat.DTYPE_BF16, 0)
+        sizes.add((lib.ews_gated_scan_residual_bytes(d), lib.ews_gated_scan_workspace_bytes(d)))
+    assert len(sizes) == 1

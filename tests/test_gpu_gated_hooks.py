@@ -1,0 +1,46 @@
+"""Gradients where hooks on saved tensors bring them back contiguous, or off their 16-byte addresses: those without."""
+
+import contextlib
+
+import pytest
+import torch
+
+import ews_mi355x as E
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def _off(t, by=1):
+    """t's numbers contiguous, ``by`` elements behind a 16-byte address."""
+    size = t.element_size()
+    flat = torch.empty(t.numel() * size + 64, dtype=torch.uint8, device=t.device)[by * size:][:t.numel() * size]
+    return flat.view(t.dtype).view(t.shape).copy_(t)
+
+
+def _hooks(kind):
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    return {"none": contextlib.nullcontext, "cpu": torch.autograd.graph.save_on_cpu,
+            "contiguous": lambda: hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t),
+            "off": lambda: hooks(_off, lambda t: t)}[kind]()
+
+
+@pytest.mark.parametrize("kind", ["cpu", "contiguous", "off"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,L,D", [(2, 300, 24), (2, 9, 25), (1, 2100, 24), (600, 20, 450)])
+def test_scan_of_halves(B, L, D, dtype, kind):
+    """The halves of a joint projection, a mask for all sequences: strips, threads alone, segments."""
+    print(f"{B} {L} {D} {dtype} {kind}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(B + L + D)
+    joint = torch.randn(B, L, 2 * D, generator=g, device="cuda").to(dtype).requires_grad_()
+    state = torch.randn(B, D, generator=g, device="cuda", requires_grad=True)
+    up = torch.randn(B, L, D, generator=g, device="cuda").to(dtype)
+    mask = torch.arange(L, device="cuda") % 5 != 0
+    grads = []
+    for k in ("none", kind):
+        with _hooks(k):
+            h, last = E.gated_scan(*joint.chunk(2, -1), state=state, mask=mask)
+        grads.append(torch.autograd.grad((h, last), (joint, state), (up, torch.ones_like(last))))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
