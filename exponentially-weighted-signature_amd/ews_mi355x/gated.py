@@ -6,7 +6,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
-from .embed import DTYPES, check_tensor, launch, once, refuse_tangents, row_major
+from .embed import DTYPES, aligned, check_tensor, launch, once, refuse_tangents, row_major, stamps, unmoved
 
 _MOST_ROWS, _MOST_WIDTH, _MOST_FEATURES = 1 << 24, 1 << 16, 1 << 20
 
@@ -24,8 +24,8 @@ def _ptr(t):
 
 class _Call:
     """One call's operands as the library takes them (copies only where rows are not contiguous); ``gate_weight`` None:
-    the second half of ``weight``'s rows. A backward is given the descriptor of its forward, and the operands that the
-    forward took: a small call costs its host time, and the backward's thread runs Python two to three times slower than
+    the second half of ``weight``'s rows. A backward whose operands lie where its forward's did is given the forward's
+    descriptor: a small call costs its host time, and the backward's thread runs Python two to three times slower than
     the caller's."""
 
     __slots__ = ("operands", "desc", "at")
@@ -103,16 +103,22 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):
         call = _Call((x, weight, bias, gate_weight, gate_bias), activation=activation)
         out, kept = call.forward(True)
-        ctx.save_for_backward(*call.operands, kept)
-        ctx.args = call.desc, call.scratch_bytes(nat.GATED_BACKWARD)
+        saved = *call.operands, kept
+        ctx.save_for_backward(*saved)
+        ctx.args = call.desc, call.scratch_bytes(nat.GATED_BACKWARD), activation, stamps(saved)
         return out
 
     @staticmethod
     @once
     def backward(ctx, gout):
-        *operands, kept = ctx.saved_tensors
-        desc, size = ctx.args
-        return (*_Call(operands, desc).backward(kept, gout.contiguous(), ctx.needs_input_grad, size), None)
+        *operands, kept = saved = ctx.saved_tensors
+        desc, size, activation, made_for = ctx.args
+        if unmoved(saved, made_for, gout.device):
+            call = _Call(operands, desc)
+        else:
+            call, kept = _Call(operands, activation=activation), aligned(kept)
+            size = call.scratch_bytes(nat.GATED_BACKWARD)
+        return (*call.backward(kept, gout.contiguous(), ctx.needs_input_grad, size), None)
 
 
 def takes(x, weight, bias):

@@ -1,4 +1,4 @@
-"""What the backward calls of ``gated_scan`` hand to the library where hooks on saved tensors bring them back with other
+"""What the backward calls of ``gated_scan`` and ``gated_linear`` hand to the library where hooks on saved tensors bring them back with other
 strides or at other addresses: descriptors and scratch of the tensors that came back. The launches are recorded, not run."""
 
 import ctypes
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from ews_mi355x import _native as nat
-from ews_mi355x import recurrence
+from ews_mi355x import gated, recurrence
 
 
 def _value(a):
@@ -23,6 +23,7 @@ def calls(monkeypatch):
         return 0
 
     monkeypatch.setattr(recurrence, "launch", record)
+    monkeypatch.setattr(gated, "launch", record)
     return made
 
 
@@ -98,3 +99,45 @@ def test_the_residual_does_not_depend_on_strides(B, L, D):
         d = nat.GatedScanDesc(L * step, step, L * D, D, L, B, L, D, nat.DTYPE_BF16, 0)
         sizes.add((lib.ews_gated_scan_residual_bytes(d), lib.ews_gated_scan_workspace_bytes(d)))
     assert len(sizes) == 1
+
+
+def _apart(rows, cols, stride, dtype):
+    return torch.randn(rows, stride).to(dtype)[:, :cols].requires_grad_()
+
+
+@pytest.mark.parametrize("off", [0, 2, 4])
+@pytest.mark.parametrize("joint", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gated_backward_describes_what_came_back(calls, monkeypatch, dtype, joint, off):
+    """Strides, V's and G's addresses, and scratch as large as the plan of these addresses asks for."""
+    if dtype is torch.float32 and off == 2:
+        pytest.skip("no address of float32 numbers")
+    N, H, F, sizes = 100, 128, 96, []
+    scratch = gated._scratch
+
+    def seen(x, size):
+        sizes.append(size)
+        return scratch(x, size)
+
+    monkeypatch.setattr(gated, "_scratch", seen)
+    x, w = _apart(N, H, 136, dtype), _apart(2 * F if joint else F, H, 144, dtype)
+    g = None if joint else _apart(F, H, 144, dtype)
+    with _Elsewhere(off) as there:
+        y = gated._GatedLinear.apply(x, w, None, g, None, "silu")
+    y.float().sum().backward()
+    (_, forward), (name, (desc, px, pv, _, pg, _, kept, *_)) = calls
+    assert name == "ews_gated_backward" and forward[0].x_stride == 136 and forward[0].weight_stride == 144
+    came = there.came
+    assert (desc.x_stride, desc.weight_stride, desc.gate_stride) == (H, H, H)
+    assert came[px].shape == (N, H) and came[pv].shape == w.shape
+    assert pg == pv + F * H * w.element_size() if joint else came[pg].shape == (F, H)
+    assert kept % 16 == 0
+    assert sizes[-1] >= nat.load().ews_gated_workspace_bytes(desc, px, pv, pg, nat.GATED_BACKWARD) > 0
+
+
+def test_gated_backward_without_hooks_reads_where_the_forward_did(calls):
+    y = gated._GatedLinear.apply(_apart(100, 128, 136, torch.float32), _apart(192, 128, 128, torch.float32), None, None,
+                                 None, "silu")
+    y.sum().backward()
+    (_, f), (_, b) = calls
+    assert b[0] is f[0] and b[1:6] == f[1:6]

@@ -44,3 +44,28 @@ def test_scan_of_halves(B, L, D, dtype, kind):
         grads.append(torch.autograd.grad((h, last), (joint, state), (up, torch.ones_like(last))))
     for a, b in zip(*grads):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["cpu", "contiguous", "off"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,F", [(7, 128, 96), (200, 128, 96), (200, 64, 40), (300, 136, 130), (9, 1030, 70)])
+def test_linear_of_rows_apart(N, H, F, dtype, kind):
+    """Rows of x and of the weights apart: few rows, tiles, narrow maps, widths that have to be packed. Sums are of the
+    same numbers in the same order, whether the rows are packed or read as they are."""
+    print(f"{N} {H} {F} {dtype} {kind}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(N + H + F)
+
+    def apart(rows, cols, by):
+        wide = torch.randn(rows, cols + by, generator=g, device="cuda").to(dtype).requires_grad_()
+        return wide, wide[:, :cols]
+
+    for joint in (True, False):
+        leaves, views = zip(apart(N, H, 8), apart(2 * F if joint else F, H, 16), *([] if joint else [apart(F, H, 16)]))
+        up = torch.randn(N, F, generator=g, device="cuda").to(dtype)
+        grads = []
+        for k in ("none", kind):
+            with _hooks(k):
+                y = E.gated_linear(views[0], views[1], None, *views[2:], activation="silu")
+            grads.append(torch.autograd.grad(y, leaves, up))
+        for a, b in zip(*grads):
+            assert torch.equal(a, b)
