@@ -69,12 +69,18 @@ struct Rows {
 // where those of every 128 tokens begin, so that a tile finds its own at once (16384 rows of 64 entries each: one entry
 // in four tiles' rows). k_logits puts its block of z through LDS where one of its rows has an entry there, and hands
 // out the entries' own float32 logits; k_dz takes them in place of the kept probabilities, as it does a target's.
+//
+// sum_k p_k log (p_k / q_k) cancels where p and q are alike, as they are at a high temperature, and T^2 brings out what is
+// left: float32 has no digit of it where K = V and T = 1000. So l is formed of terms that are not negative,
+//   l = T^2 (sum_k q_k f(p_k / q_k - 1) + 1 - sum_k q_k)     f(x) = (1 + x) log (1 + x) - x,
+// f by its series where x is small. What no entry names, 1 - sum_k q_k, is 0 where the entries name all tokens once.
+// With r the relative rounding of p / q (2^-21 or so) such a row is off by T r and (T r)^2, not by T^2 r.
 constexpr int kBucket = 128;
 struct Top {
   int count;              // K
   const int* token;       // (N, K) sorted; INT_MAX where there is none
   const float* p;         // (N, K) their probabilities
-  const float* entropy;   // (N) sum_k p_k log p_k
+  const float* rest;      // (N) 0 where the entries name every token once, else 1
   const uint16_t* first;  // (N, stride) the first entry at or past every 128th token, buckets + 1 of them
   int buckets, stride;
   float* z;               // (N, K) their logits
@@ -385,27 +391,47 @@ __global__ __launch_bounds__(1024) void k_join(Stats st, Rows rows, int slabs, i
   if (loss_rows) loss_rows[rows.map[row]] = l;
 }
 
-// A wavefront a row: l = T^2 (sum_k p_k log p_k + sum_k p_k (log sum exp (z - M) + M - z_k)). Entries of probability 0
-// count nothing, also where z_k is -inf.
+// q f(p / q - 1), p's part of a row's loss and what it is short of q's. log_q: log q, of any size.
+__device__ __forceinline__ float divergence(float p, float q, float log_q) {
+  const float x = (p - q) / q;
+  if (fabsf(x) < 0.25f) {
+    // x^2 (1/2 - x/6 + x^2/12 - ... +- x^n / ((n + 1) (n + 2))), the next term 2^-23 of the first at most
+    constexpr int kTerms = 10;
+    float s = 0.0f;
+#pragma unroll
+    for (int n = kTerms; n >= 0; --n) s = fmaf(s, -x, 1.0f / (float)((n + 1) * (n + 2)));
+    return q * x * x * s;
+  }
+  constexpr float kSmall = 1e-30f;
+  const float d = p > kSmall && q > kSmall ? logf(p / q) : logf(p) - log_q;
+  return (p != 0.0f ? p * d : 0.0f) + (q - p);
+}
+
+// A wavefront a row. Entries of probability 0 count nothing, also where z_k is -inf.
 __global__ __launch_bounds__(256) void k_top_loss(Stats st, Rows rows, Top top, int c0, int chunk, float* loss_rows) {
   const int live = rows.kept[0] - c0 < chunk ? rows.kept[0] - c0 : chunk;
   const int j = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (j >= live) return;
-  const int row = c0 + j;
-  const int64_t from = (int64_t)rows.map[row] * top.count;
-  const float m = st.top[row], lse = st.loss[row];
-  float s = 0.0f;
-  for (int e = threadIdx.x & 63; e < top.count; e += 64) {
-    const float p = top.p[from + e];
-    if (p != 0.0f) s += p * (lse + (m - top.z[from + e]) * kLn2);
+  const int row = c0 + j, place = rows.map[row];
+  const int64_t from = (int64_t)place * top.count;
+  const int entries = top.first[(int64_t)place * top.stride + top.buckets];
+  const float m = st.top[row], inv = st.inv[row], lse = st.loss[row];
+  float s = 0.0f, named = 0.0f;
+  for (int e = threadIdx.x & 63; e < entries; e += 64) {
+    const float z = top.z[from + e] - m, q = __builtin_amdgcn_exp2f(z) * inv;
+    s += divergence(top.p[from + e], q, z * kLn2 - lse);
+    named += q;
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  for (int d = 32; d; d >>= 1) {
+    s += __shfl_xor(s, d);
+    named += __shfl_xor(named, d);
+  }
   if (threadIdx.x & 63) return;
   const float t2 = top.temperature * top.temperature;
-  const float l = rows.target[row] < 0 ? __builtin_nanf("") : t2 * (top.entropy[rows.map[row]] + s);
+  const float l = rows.target[row] < 0 ? __builtin_nanf("") : t2 * (s + top.rest[place] * (1.0f - named));
   st.loss[row] = l;
-  if (loss_rows) loss_rows[rows.map[row]] = l;
+  if (loss_rows) loss_rows[place] = l;
 }
 
 // The sum or mean of the kept rows' losses, by one workgroup of up to 1024 threads.
@@ -635,7 +661,7 @@ struct TeacherArgs {
   int64_t* target;         // (n) 0; -1 where a token is outside the vocabulary, kNone where there is no entry
   int* token;
   float* p;
-  float* entropy;
+  float* rest;
   uint16_t* first;
 };
 constexpr int64_t kNone = -100;
@@ -701,22 +727,20 @@ __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-  const float log_sum = __builtin_amdgcn_logf(sum);  // base 2
-  float entropy = 0.0f;
+  int named = 0;  // tokens of the vocabulary, each once
   for (int e = lane; e < a.count; e += 64) {
     const uint64_t k = key[e];
     const int token = (int)(k >> 32);
-    float p = 0.0f;
-    if (token != 0x7fffffff) {
-      const float y = (value[(uint32_t)k] - top) * a.scale;
-      p = __builtin_amdgcn_exp2f(y) / sum;
-      if (p != 0.0f) entropy += p * (y - log_sum);
-    }
+    const float p = token == 0x7fffffff ? 0.0f : __builtin_amdgcn_exp2f((value[(uint32_t)k] - top) * a.scale) / sum;
     a.token[(int64_t)row * a.count + e] = token;
     a.p[(int64_t)row * a.count + e] = p;
+    if (a.count >= a.vocab && token < a.vocab) {  // else there are too few
+      ++named;
+      if (e > 0 && (int)(key[e - 1] >> 32) == token) named = -2 * kMostTop;  // one twice: that is less than none
+    }
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) entropy += __shfl_xor(entropy, d);
+  for (int d = 32; d; d >>= 1) named += __shfl_xor(named, d);
   for (int b = lane; b <= a.buckets; b += 64) {
     const uint64_t want = (uint64_t)b * kBucket << 32;
     int lo = 0, hi = a.count;  // the first entry at or past it
@@ -732,7 +756,7 @@ __global__ __launch_bounds__(256) void k_teacher(TeacherArgs a) {
   any = __any(any);
   bad = __any(bad);
   if (lane) return;
-  a.entropy[row] = entropy * kLn2;
+  a.rest[row] = named == a.vocab ? 0.0f : 1.0f;
   a.target[row] = !any ? kNone : bad ? -1 : 0;
 }
 
@@ -935,7 +959,7 @@ struct LPlan {
   Product logits, dh, dw;
   size_t map, target, meta, zt, top, inv, loss, xp, wp, bias, slab, prob, dz, dbias, dbsum, part, acc;
   int entries, buckets;    // distillation: K; the vocabulary's buckets
-  size_t flags, token, share, entropy, first;
+  size_t flags, token, share, rest, first;
   size_t total;
 };
 
@@ -1006,7 +1030,7 @@ int loss_plan(const ews_loss_desc* s, bool train, bool direct, LPlan& p, int ent
     p.flags = take((size_t)p.N * 8);
     p.token = take((size_t)p.N * entries * 4);
     p.share = take((size_t)p.N * entries * 4);
-    p.entropy = take((size_t)p.N * 4);
+    p.rest = take((size_t)p.N * 4);
     p.first = take((size_t)p.N * bucket_stride(p.buckets) * 2);
   }
   if (train) {
@@ -1284,7 +1308,7 @@ Call make_call(const ews_loss_desc* s, const LPlan& p, void* workspace, ews_stre
     c.top.count = p.entries;
     c.top.token = (const int*)(c.w + p.token);
     c.top.p = (const float*)(c.w + p.share);
-    c.top.entropy = (const float*)(c.w + p.entropy);
+    c.top.rest = (const float*)(c.w + p.rest);
     c.top.first = (const uint16_t*)(c.w + p.first);
     c.top.buckets = p.buckets;
     c.top.stride = bucket_stride(p.buckets);
@@ -1513,7 +1537,7 @@ int distill_plan(const ews_distill_desc* d, bool train, bool direct, LPlan& p) {
   if (!d) return EWS_ERR_NULL;
   if (d->index_bytes != 4 && d->index_bytes != 8) return EWS_ERR_OPTION;
   if (d->logit_dtype != EWS_DTYPE_F32 && d->logit_dtype != EWS_DTYPE_BF16) return EWS_ERR_OPTION;
-  if (!(d->temperature >= 1e-6f) || d->temperature > 1e6f) return EWS_ERR_OPTION;
+  if (!(d->temperature >= 1e-6f) || d->temperature > 1e4f) return EWS_ERR_OPTION;
   if (d->entries < 1 || d->entries > kMostTop || d->index_stride < 0 || d->logit_stride < 0) return EWS_ERR_SHAPE;
   return loss_plan(&d->head, train, direct, p, d->entries);
 }
@@ -1557,7 +1581,7 @@ struct Distill {
     t.target = (int64_t*)(c.w + p.flags);
     t.token = (int*)(c.w + p.token);
     t.p = (float*)(c.w + p.share);
-    t.entropy = (float*)(c.w + p.entropy);
+    t.rest = (float*)(c.w + p.rest);
     t.first = (uint16_t*)(c.w + p.first);
     hipLaunchKernelGGL(k_teacher, dim3(ceil_div(p.N, 4)), dim3(256), 4 * t.ordered * 12, c.st, t);
     LOSS_CHECK();

@@ -222,14 +222,15 @@ def logits_distillation(student, indices, logits, temperature, reduction):
     kept = has.any(-1)
     known = ~(has & (indices >= student.shape[-1])).any(-1)
     at = torch.where(has & (indices < student.shape[-1]), indices, 0).long()
-    teacher = torch.where(has, logits.detach().float() / temperature, -float("inf"))
+    # in float64: the logarithms cancel at a high temperature, whose square brings out what is left
+    teacher = torch.where(has, logits.detach().double() / temperature, -float("inf"))
     logp = torch.log_softmax(torch.where(kept[..., None], teacher, 0.0), -1)
     p = torch.where(has, logp.exp(), 0.0)
-    z = torch.where(kept[..., None], student.float(), 0.0)
+    z = torch.where(kept[..., None], student.double(), 0.0)
     logq = torch.log_softmax(z / temperature, -1).gather(-1, at)
     rows = temperature**2 * torch.where(p != 0, p * (logp - logq), 0.0).sum(-1)
     rows = torch.where(kept, rows * torch.where(known, 1.0, float("nan")), 0.0)
-    return _reduced(rows, kept, reduction)
+    return _reduced(rows, kept, reduction).float()
 
 
 def _check_teacher(shape, indices, logits, temperature):
@@ -239,8 +240,8 @@ def _check_teacher(shape, indices, logits, temperature):
         raise ValueError(f"indices must have 1 to {nat.DISTILL_MOST_ENTRIES} entries a row, got {indices.shape[-1]}")
     if logits.shape != indices.shape:
         raise ValueError(f"logits must be {tuple(indices.shape)}, got {tuple(logits.shape)}")
-    if not 1e-6 <= temperature <= 1e6:
-        raise ValueError(f"temperature must be from 1e-6 to 1e6, got {temperature}")
+    if not 1e-6 <= temperature <= 1e4:
+        raise ValueError(f"temperature must be from 1e-6 to 1e4, got {temperature}")
     if indices.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"indices must be int64 or int32, got {indices.dtype}")
     if torch.is_grad_enabled() and logits.requires_grad:
@@ -286,8 +287,9 @@ def linear_distillation(hidden, weight, indices, logits, bias=None, temperature=
 
     hidden (..., H), weight (V, H) and bias (V,) or None as ``linear_cross_entropy``'s; indices (..., K) int64 or
     int32 and logits (..., K) float32 or bfloat16, K up to 1024: the teacher's tokens of every position and their
-    logits, in any order, the teacher's distribution being that over them alone. T is ``temperature`` (1e-6 to 1e6);
-    its square keeps the gradients' size. ``reduction``: "mean" over the rows that have an entry (0 where none has),
+    logits, in any order, the teacher's distribution being that over them alone. T is ``temperature`` (1e-6 to 1e4);
+    its square keeps the gradients' size. At a high one p and q differ by little: float32's rounding of them, 2^-20 of
+    q at most, is T 2^-20 of q in a gradient (1% of a token's at T = 1e4 and logits a unit apart). ``reduction``: "mean" over the rows that have an entry (0 where none has),
     "sum", or "none" for every row's own loss, (...), float32. Differentiable in hidden, weight and bias (reverse
     mode); the teacher's logits have no gradient, and one that requires it is refused: detach them.
 

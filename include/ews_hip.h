@@ -687,7 +687,7 @@ typedef struct ews_distill_desc {
   int32_t entries;       /* K: 1..1024 */
   int32_t index_bytes;   /* 8 (int64) or 4 (int32) */
   int32_t logit_dtype;   /* EWS_DTYPE_* of teacher */
-  float temperature;     /* T: 1e-6..1e6 */
+  float temperature;     /* T: 1e-6..1e4 */
 } ews_distill_desc;
 
 /* As their namesakes of ews_loss; ews_loss_scale serves them too. */

@@ -112,3 +112,25 @@ def test_of_logits(reduction):
     index[3, 0] = V
     t[3, 0] = 0.0
     assert bool(logits_distillation(z, index, t, T, "none")[3].isnan())
+
+
+@pytest.mark.parametrize("T", [32.0, 1000.0, 1e4])
+def test_of_logits_at_high_temperatures(T):
+    """T^2 brings out what is left of logarithms that cancel: some digits of float32, not a few of T^2 of them."""
+    g = torch.Generator().manual_seed(5)
+    z, t = 2 * torch.randn(12, 300, generator=g), 2 * torch.randn(12, 300, generator=g)
+    index = torch.stack([torch.randperm(300, generator=g) for _ in range(12)])
+    logp, logq = torch.log_softmax(t.double() / T, 1), torch.log_softmax(z.double() / T, 1).gather(1, index)
+    want = T * T * (logp.exp() * (logp - logq)).sum(1)
+    got = logits_distillation(z, index, t, T, "none")
+    # the result's rounding, and float64's own of 300 terms of 6: T^2 2^-44
+    assert bool(((got.double() - want).abs() <= 2.0**-23 * want + T * T * 2.0**-44).all())
+
+
+def test_temperatures_without_digits_are_refused():
+    with pytest.raises(ValueError, match="temperature must be from 1e-6 to 1e4"):
+        E.linear_distillation(**{**BASE, "temperature": 2e4})
+    lib, one = nat.load(), ctypes.c_void_p(16)
+    d = _desc(temperature=2e4)
+    assert lib.ews_distill_workspace_bytes_for(d, one, 1) == 0
+    assert lib.ews_distill_forward(d, one, one, None, one, one, one, one, None) == -4
