@@ -56,14 +56,18 @@ def aligned(t):
         memory_format=torch.contiguous_format)
 
 
+def has_tangent(tensors):
+    """Whether a tensor (or None) of them carries a forward-mode derivative."""
+    if forward_ad._current_level < 0:  # no forward-mode differentiation is going on
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def refuse_tangents(tensors):
     """Forward-mode derivatives are not formed: a tensor (or None) that carries one is refused, as an autograd function
     without a jvp refuses it, not answered without a tangent, which would read as a derivative of zero."""
-    if forward_ad._current_level < 0:  # no forward-mode differentiation is going on
-        return
-    for t in tensors:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError("ews_mi355x has no forward-mode derivatives (jvp) of this operator")
+    if has_tangent(tensors):
+        raise NotImplementedError("ews_mi355x has no forward-mode derivatives (jvp) of this operator")
 
 
 def check_tensor(name, t):

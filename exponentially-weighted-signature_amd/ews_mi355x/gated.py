@@ -6,7 +6,8 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
-from .embed import DTYPES, aligned, check_tensor, launch, once, refuse_tangents, row_major, stamps, unmoved
+from .embed import (DTYPES, aligned, check_tensor, has_tangent, launch, once, refuse_tangents, row_major, stamps,
+                    unmoved)
 
 _MOST_ROWS, _MOST_WIDTH, _MOST_FEATURES = 1 << 24, 1 << 16, 1 << 20
 
@@ -126,7 +127,7 @@ def takes(x, weight, bias):
     return (x.is_cuda and x.dtype in DTYPES and weight.dtype is x.dtype and weight.device == x.device
             and (bias is None or (bias.dtype is x.dtype and bias.device == x.device))
             and x.shape[-1] == weight.shape[1] and _fits(x.numel() // x.shape[-1], weight.shape[1], weight.shape[0])
-            and not torch.is_autocast_enabled())
+            and not torch.is_autocast_enabled() and not has_tangent((x, weight, bias)))
 
 
 def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activation="sigmoid"):
