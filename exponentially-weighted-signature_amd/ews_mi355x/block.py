@@ -30,7 +30,7 @@ from torch.nn.modules import module as nn_module
 
 from .embed import embedding_lookup
 from .front import B, BlockFront, ClockSpec, make_clock
-from .gated import gated_linear, takes
+from .gated import gated_stage, takes
 from .layer import EWS
 from .loss import linear_cross_entropy, linear_distillation, logits_cross_entropy, logits_distillation
 from .mixer import MixerEpilogue
@@ -209,12 +209,12 @@ class EWSBlock(nn.Module):
             return torch.tanh(self.ff1(xhat))
         if self.channel_stage == "glu":
             if self._fuses(xhat, self.ff1):
-                return gated_linear(xhat, self.ff1.weight, self.ff1.bias)
+                return gated_stage(xhat, self.ff1.weight, self.ff1.bias)
             a, b = self.ff1(xhat).chunk(2, dim=-1)
             return a * torch.sigmoid(b)
         h = F.gelu(xhat, approximate="tanh")
         if self._fuses(h, self.ff1, self.ff2):
-            return gated_linear(h, self.ff1.weight, self.ff1.bias, self.ff2.weight, self.ff2.bias)
+            return gated_stage(h, self.ff1.weight, self.ff1.bias, self.ff2.weight, self.ff2.bias)
         return self.ff1(h) * torch.sigmoid(self.ff2(h))
 
     def _fuses(self, x, *maps):

@@ -4,6 +4,7 @@ kernel (the "glu" and "gelu_glu" stages of ews/block.py:361-374, and their like)
 from __future__ import annotations
 
 import torch
+from torch.nn.functional import linear
 
 from . import _native as nat
 from .embed import (DTYPES, aligned, check_tensor, has_tangent, launch, once, refuse_tangents, row_major, stamps,
@@ -104,9 +105,8 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):
         call = _Call((x, weight, bias, gate_weight, gate_bias), activation=activation)
         out, kept = call.forward(True)
-        saved = *call.operands, kept
-        ctx.save_for_backward(*saved)
-        ctx.args = call.desc, call.scratch_bytes(nat.GATED_BACKWARD), activation, stamps(saved)
+        ctx.save_for_backward(*call.operands, kept)
+        ctx.args = call.desc, call.scratch_bytes(nat.GATED_BACKWARD), activation, stamps((*call.operands, kept))
         return out
 
     @staticmethod
@@ -122,12 +122,44 @@ class _GatedLinear(torch.autograd.Function):
         return (*call.backward(kept, gout.contiguous(), ctx.needs_input_grad, size), None)
 
 
+class _GatedStage(_GatedLinear):
+    """``_GatedLinear`` with the activation "sigmoid" and a graph of its backward, in torch's operations."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):
+        out = _GatedLinear.forward(ctx, x, weight, bias, gate_weight, gate_bias, activation)
+        # what came in: a copy that the library took has no graph (the backward then makes it once more)
+        ctx.save_for_backward(x, weight, bias, gate_weight, gate_bias, ctx.to_save[-1])
+        return out
+
+    @staticmethod
+    def backward(ctx, gout):
+        if not torch.is_grad_enabled():
+            return _GatedLinear.backward(ctx, gout)
+        needs = ctx.needs_input_grad[:5]
+        x, weight, bias, gate_weight, gate_bias = leaves = [t if t is None else t.view_as(t)
+                                                            for t in ctx.saved_tensors[:5]]
+        if gate_weight is None:
+            v, g = linear(x, weight, bias).chunk(2, -1)
+        else:
+            v, g = linear(x, weight, bias), linear(x, gate_weight, gate_bias)
+        grads = iter(torch.autograd.grad(v * torch.sigmoid(g), [t for t, n in zip(leaves, needs) if n], gout,
+                                         create_graph=True))
+        return (*(next(grads) if n else None for n in needs), None)
+
+
 def takes(x, weight, bias):
     """Whether ``gated_linear`` does what a linear map of x and torch's operations after it would, types included."""
     return (x.is_cuda and x.dtype in DTYPES and weight.dtype is x.dtype and weight.device == x.device
             and (bias is None or (bias.dtype is x.dtype and bias.device == x.device))
             and x.shape[-1] == weight.shape[1] and _fits(x.numel() // x.shape[-1], weight.shape[1], weight.shape[0])
             and not torch.is_autocast_enabled() and not has_tangent((x, weight, bias)))
+
+
+def gated_stage(x, weight, bias=None, gate_weight=None, gate_bias=None):
+    """``gated_linear`` for a block's gated channel stage, whose maps have second derivatives: a graph of the backward is
+    that of the maps' own."""
+    return _gated(_GatedStage, x, weight, bias, gate_weight, gate_bias, "sigmoid")
 
 
 def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activation="sigmoid"):
@@ -141,6 +173,10 @@ def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activat
     Differentiable in everything (reverse mode). A call that records gradients keeps both products' sums, of 24
     bits each (float32: 32), beside the result, unless H and F are 64 at most. A few rows (a decoding step:
     32, of float32 64) read the weights once, at the memory's rate."""
+    return _gated(_GatedLinear, x, weight, bias, gate_weight, gate_bias, activation)
+
+
+def _gated(function, x, weight, bias, gate_weight, gate_bias, activation):
     if activation not in nat.GATED_ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(nat.GATED_ACTIVATIONS)}, got {activation!r}")
     joint = gate_weight is None
@@ -180,7 +216,7 @@ def gated_linear(x, weight, bias=None, gate_weight=None, gate_bias=None, activat
         none = x.new_zeros(shape)
         return none + sum(t[:0].sum() for t in (x2, *others) if t is not None) if train else none
     if train:
-        out = _GatedLinear.apply(x2, *others, activation)
+        out = function.apply(x2, *others, activation)
     else:
         out = _Call((x2, *others), activation=activation).forward(False)[0]
     return out if out.shape == shape else out.reshape(shape)

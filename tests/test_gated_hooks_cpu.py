@@ -141,3 +141,34 @@ def test_gated_backward_without_hooks_reads_where_the_forward_did(calls):
     y.sum().backward()
     (_, f), (_, b) = calls
     assert b[0] is f[0] and b[1:6] == f[1:6]
+
+
+@pytest.mark.parametrize("joint", [False, True])
+@pytest.mark.parametrize("turned", [False, True])
+def test_a_stages_graph_of_its_backward(calls, joint, turned):
+    """Its gradients and theirs are those of the maps; turned weights, which the library takes a copy of, keep theirs."""
+    N, H, F = 9, 6, 5
+    g = torch.Generator().manual_seed(1)
+
+    def leaf(*shape):
+        return torch.randn(*shape, generator=g, dtype=torch.float32).requires_grad_()
+
+    x, up = leaf(N, H), leaf(N, F)
+    w, b = leaf(*((H, 2 * F if joint else F) if turned else (2 * F if joint else F, H))), leaf(2 * F if joint else F)
+    gw, gb = (None, None) if joint else (leaf(F, H), leaf(F))
+    leaves = [t for t in (x, w, b, gw, gb) if t is not None]
+    first = []
+    for fused in (True, False):
+        weight = w.t() if turned else w
+        if fused:
+            y = gated._GatedStage.apply(x, weight, b, gw, gb, "sigmoid")
+        else:
+            z = torch.nn.functional.linear(x, weight, b)
+            v, s = z.chunk(2, -1) if joint else (z, torch.nn.functional.linear(x, gw, gb))
+            y = v * torch.sigmoid(s)
+        grads = torch.autograd.grad(y, leaves, up, create_graph=True)
+        first.append((grads, torch.autograd.grad(sum(t.square().sum() for t in grads), [*leaves, up])))
+    for (a, a2), (r, r2) in [first]:
+        for s, t in zip((*a, *a2), (*r, *r2)):
+            assert torch.equal(s, t)
+    assert [name for name, _ in calls] == ["ews_gated_forward"]
