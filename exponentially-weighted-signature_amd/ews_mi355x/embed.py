@@ -32,22 +32,18 @@ def once(backward):
     return run
 
 
-def stamps(tensors):
-    """Where tensors (or None) lie and how: what a call's descriptor and scratch are made for."""
-    return [t if t is None else (t.data_ptr(), t.dtype, t.shape, t.stride()) for t in tensors]
+def layouts(tensors):
+    """Strides and types of tensors (or None): with their addresses, what a call's descriptor and scratch are made for.
+    Hooks on saved tensors may bring them back at other addresses, with other strides."""
+    return [None if t is None else (t.stride(), t.dtype) for t in tensors]
 
 
-def unmoved(tensors, made_for, dev):
-    """Whether saved tensors came back as the forward left them (``made_for``, their ``stamps``). Hooks on saved tensors
-    may bring them back at other addresses, with other strides; of another type, shape or device they are refused."""
-    now = stamps(tensors)
-    if now == made_for:
-        return True
-    for t, n, m in zip(tensors, now, made_for):
-        if n is not None and (n[1:3] != m[1:3] or t.device != dev):
-            raise RuntimeError(f"a saved tensor came back as {n[1]} {tuple(n[2])} on {t.device}: it was {m[1]} "
-                               f"{tuple(m[2])} on {dev}")
-    return False
+def returned(t, dtype, shape, dev):
+    """A saved tensor (or None) as it came back, refused where it is of another type, shape or device than it was."""
+    if t is not None and (t.dtype is not dtype or t.shape != shape or t.device != dev):
+        raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}: it was {dtype} "
+                           f"{tuple(shape)} on {dev}")
+    return t
 
 
 def aligned(t):

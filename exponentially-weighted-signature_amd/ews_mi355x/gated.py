@@ -7,8 +7,8 @@ import torch
 from torch.nn.functional import linear
 
 from . import _native as nat
-from .embed import (DTYPES, aligned, check_tensor, has_tangent, launch, once, refuse_tangents, row_major, stamps,
-                    unmoved)
+from .embed import (DTYPES, aligned, check_tensor, has_tangent, launch, layouts, once, refuse_tangents, returned,
+                    row_major)
 
 _MOST_ROWS, _MOST_WIDTH, _MOST_FEATURES = 1 << 24, 1 << 16, 1 << 20
 
@@ -100,24 +100,36 @@ def _scratch(x, size):
     return x.new_empty(size, dtype=torch.uint8) if size else None
 
 
+def _come_back(operands, kept, desc, dtype, dev):
+    """Saved tensors that are not where the forward left them."""
+    N, H, F = desc.rows, desc.width, desc.features
+    rows = 2 * F if operands[3] is None else F
+    shapes = (N, H), (rows, H), (rows,), (F, H), (F,)
+    size = nat.load().ews_gated_kept_bytes(desc)
+    return [returned(t, dtype, s, dev) for t, s in zip(operands, shapes)], aligned(returned(kept, torch.uint8, (size,), dev))
+
+
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):
         call = _Call((x, weight, bias, gate_weight, gate_bias), activation=activation)
         out, kept = call.forward(True)
         ctx.save_for_backward(*call.operands, kept)
-        ctx.args = call.desc, call.scratch_bytes(nat.GATED_BACKWARD), activation, stamps((*call.operands, kept))
+        x, weight, _, gate_weight, _ = call.operands
+        ctx.args = (call.desc, call.scratch_bytes(nat.GATED_BACKWARD), activation, (*call.at, _ptr(kept)),
+                    layouts((x, weight, gate_weight)))
         return out
 
     @staticmethod
     @once
     def backward(ctx, gout):
-        *operands, kept = saved = ctx.saved_tensors
-        desc, size, activation, made_for = ctx.args
-        if unmoved(saved, made_for, gout.device):
-            call = _Call(operands, desc)
-        else:
-            call, kept = _Call(operands, activation=activation), aligned(kept)
+        *operands, kept = ctx.saved_tensors
+        desc, size, activation, forward_at, laid_out = ctx.args
+        x, weight, _, gate_weight, _ = operands
+        call = _Call(operands, desc)
+        if (*call.at, _ptr(kept)) != forward_at or layouts((x, weight, gate_weight)) != laid_out:
+            operands, kept = _come_back(operands, kept, desc, laid_out[0][1], gout.device)
+            call = _Call(operands, activation=activation)
             size = call.scratch_bytes(nat.GATED_BACKWARD)
         return (*call.backward(kept, gout.contiguous(), ctx.needs_input_grad, size), None)
 

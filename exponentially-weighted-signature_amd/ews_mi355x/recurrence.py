@@ -8,7 +8,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _native as nat
-from .embed import DTYPES, aligned, check_tensor, launch, once, refuse_tangents, stamps, unmoved
+from .embed import DTYPES, aligned, check_tensor, launch, layouts, once, refuse_tangents, returned
 
 
 def _ptr(t):
@@ -43,7 +43,7 @@ def _describe(x, gate, mask, form):
 
 
 def _forward(x, gate, mask, state, last, form, train):
-    """(out, last, the descriptor and the scratch's size, the residual of a training call)."""
+    """(out, last, the residual of a training call, the descriptor, the scratch's size and the addresses that it read)."""
     B, L, D = x.shape
     out = x.new_empty((B, L, D))
     if last is None:
@@ -53,18 +53,27 @@ def _forward(x, gate, mask, state, last, form, train):
     residual = x.new_empty(lib.ews_gated_scan_residual_bytes(desc), dtype=torch.uint8) if train else None
     size = lib.ews_gated_scan_workspace_bytes(desc)
     ws = x.new_empty(size, dtype=torch.uint8) if size else None
-    nat.check(launch(x.device, lib.ews_gated_scan_forward, desc, x.data_ptr(), gate.data_ptr(), _ptr(mask), _ptr(state),
-                     out.data_ptr(), last.data_ptr(), _ptr(residual), _ptr(ws)), "ews_gated_scan_forward")
-    return out, last, (desc, size), residual
+    at = x.data_ptr(), gate.data_ptr(), _ptr(mask)
+    nat.check(launch(x.device, lib.ews_gated_scan_forward, desc, *at, _ptr(state), out.data_ptr(), last.data_ptr(),
+                     _ptr(residual), _ptr(ws)), "ews_gated_scan_forward")
+    return out, last, residual, desc, size, at
+
+
+def _come_back(x, gate, mask, residual, desc, dtype, dev):
+    """Saved tensors that are not where the forward left them, as the library can read them."""
+    shape = desc.batch, desc.length, desc.dim
+    size = nat.load().ews_gated_scan_residual_bytes(desc)
+    x, gate, mask = _readable(returned(x, dtype, shape, dev), returned(gate, dtype, shape, dev),
+                              returned(mask, torch.bool, shape[:2], dev))
+    return x, gate, mask, aligned(returned(residual, torch.uint8, (size,), dev))
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, state, mask, form):
-        out, last, (desc, size), residual = _forward(x, gate, mask, state, None, form, True)
-        saved = x, gate, mask, residual
-        ctx.save_for_backward(*saved)
-        ctx.args = desc, size, form, stamps(saved)
+        out, last, residual, desc, size, at = _forward(x, gate, mask, state, None, form, True)
+        ctx.save_for_backward(x, gate, mask, residual)
+        ctx.args = desc, size, form, (*at, residual.data_ptr()), layouts((x, gate))
         ctx.set_materialize_grads(False)
         return out, last
 
@@ -73,11 +82,14 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, gout, glast):
         if gout is None and glast is None:
             return None, None, None, None, None
-        x, gate, mask, residual = saved = ctx.saved_tensors
-        desc, size, form, made_for = ctx.args
-        if not unmoved(saved, made_for, (glast if gout is None else gout).device):
-            x, gate, mask = _readable(x, gate, mask)
-            desc, residual = _describe(x, gate, mask, form), aligned(residual)  # the scratch's size asks for no strides
+        x, gate, mask, residual = ctx.saved_tensors
+        desc, size, form, forward_at, laid_out = ctx.args
+        at = x.data_ptr(), gate.data_ptr(), _ptr(mask), residual.data_ptr()
+        if at != forward_at or layouts((x, gate)) != laid_out:
+            x, gate, mask, residual = _come_back(x, gate, mask, residual, desc, laid_out[0][1],
+                                                 (glast if gout is None else gout).device)
+            desc = _describe(x, gate, mask, form)  # the residual's and the scratch's sizes ask for no strides
+            at = x.data_ptr(), gate.data_ptr(), _ptr(mask), residual.data_ptr()
         if gout is not None:
             gout = gout.contiguous()
         if glast is not None:
@@ -86,9 +98,8 @@ class _GatedScan(torch.autograd.Function):
         gstate = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         lib = nat.load()
         ws = x.new_empty(size, dtype=torch.uint8) if size else None
-        nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, x.data_ptr(), gate.data_ptr(), _ptr(mask),
-                         residual.data_ptr(), _ptr(gout), _ptr(glast), gx.data_ptr(), ggate.data_ptr(), _ptr(gstate),
-                         _ptr(ws)), "ews_gated_scan_backward")
+        nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, *at, _ptr(gout), _ptr(glast), gx.data_ptr(),
+                         ggate.data_ptr(), _ptr(gstate), _ptr(ws)), "ews_gated_scan_backward")
         return gx, ggate, gstate, None, None
 
 
@@ -156,7 +167,7 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
     if train:
         return _GatedScan.apply(x, gate, state, mask, form)
     given = last is not None
-    out, last, _, _ = _forward(x, gate, mask, state, last, form, False)
+    out, last, *_ = _forward(x, gate, mask, state, last, form, False)
     if given:
         increment_version(last)  # a graph that has saved it refuses its backward, as after torch's own writes
     return out, last
