@@ -32,14 +32,9 @@ def once(backward):
     return run
 
 
-def layouts(tensors):
-    """Strides and types of tensors (or None): with their addresses, what a call's descriptor and scratch are made for.
-    Hooks on saved tensors may bring them back at other addresses, with other strides."""
-    return [None if t is None else (t.stride(), t.dtype) for t in tensors]
-
-
 def returned(t, dtype, shape, dev):
-    """A saved tensor (or None) as it came back, refused where it is of another type, shape or device than it was."""
+    """A saved tensor (or None) as it came back: hooks on saved tensors may bring it back at another address, with other
+    strides; of another type, shape or device it is refused."""
     if t is not None and (t.dtype is not dtype or t.shape != shape or t.device != dev):
         raise RuntimeError(f"a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}: it was {dtype} "
                            f"{tuple(shape)} on {dev}")

@@ -7,7 +7,7 @@ import torch
 from torch.nn.functional import linear
 
 from . import _native as nat
-from .embed import (DTYPES, aligned, check_tensor, has_tangent, launch, layouts, once, refuse_tangents, returned,
+from .embed import (DTYPES, aligned, check_tensor, has_tangent, launch, once, refuse_tangents, returned,
                     row_major)
 
 _MOST_ROWS, _MOST_WIDTH, _MOST_FEATURES = 1 << 24, 1 << 16, 1 << 20
@@ -116,19 +116,21 @@ class _GatedLinear(torch.autograd.Function):
         out, kept = call.forward(True)
         ctx.save_for_backward(*call.operands, kept)
         x, weight, _, gate_weight, _ = call.operands
-        ctx.args = (call.desc, call.scratch_bytes(nat.GATED_BACKWARD), activation, (*call.at, _ptr(kept)),
-                    layouts((x, weight, gate_weight)))
+        ctx.args = (call.desc, call.scratch_bytes(nat.GATED_BACKWARD), activation, call.at, _ptr(kept), x.stride(),
+                    weight.stride(), gate_weight is not None and gate_weight.stride(), x.dtype)
         return out
 
     @staticmethod
     @once
     def backward(ctx, gout):
         *operands, kept = ctx.saved_tensors
-        desc, size, activation, forward_at, laid_out = ctx.args
+        desc, size, activation, at, left, x_strides, strides, gate_strides, dtype = ctx.args
         x, weight, _, gate_weight, _ = operands
         call = _Call(operands, desc)
-        if (*call.at, _ptr(kept)) != forward_at or layouts((x, weight, gate_weight)) != laid_out:
-            operands, kept = _come_back(operands, kept, desc, laid_out[0][1], gout.device)
+        if (call.at != at or (left and kept.data_ptr() != left) or x.stride() != x_strides or weight.stride() != strides
+                or (gate_strides and gate_weight.stride() != gate_strides) or x.dtype is not dtype
+                or weight.dtype is not dtype):
+            operands, kept = _come_back(operands, kept, desc, dtype, gout.device)
             call = _Call(operands, activation=activation)
             size = call.scratch_bytes(nat.GATED_BACKWARD)
         return (*call.backward(kept, gout.contiguous(), ctx.needs_input_grad, size), None)

@@ -8,7 +8,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _native as nat
-from .embed import DTYPES, aligned, check_tensor, launch, layouts, once, refuse_tangents, returned
+from .embed import DTYPES, aligned, check_tensor, launch, once, refuse_tangents, returned
 
 
 def _ptr(t):
@@ -29,16 +29,9 @@ def _touches(t, start, end):
     return first + span * t.element_size() > start
 
 
-def _readable(x, gate, mask):
-    """x, gate and mask (B, L) or None as the library can read them."""
-    if mask is not None and mask.stride(1) != 1 and mask.shape[1] > 1:
-        mask = mask.contiguous()
-    return _neighbours(x), _neighbours(gate), mask
-
-
-def _describe(x, gate, mask, form):
-    return nat.GatedScanDesc(x.stride(0), x.stride(1), gate.stride(0), gate.stride(1),
-                             0 if mask is None else mask.stride(0), *x.shape, DTYPES[x.dtype],
+def _describe(x, gate, mask, B, L, D, form):
+    (xb, xs, _), (gb, gs, _) = x.stride(), gate.stride()
+    return nat.GatedScanDesc(xb, xs, gb, gs, 0 if mask is None else mask.stride(0), B, L, D, DTYPES[x.dtype],
                              nat.GATED_SCAN_FORMS[form])
 
 
@@ -48,7 +41,7 @@ def _forward(x, gate, mask, state, last, form, train):
     out = x.new_empty((B, L, D))
     if last is None:
         last = x.new_empty((B, D), dtype=torch.float32)
-    desc = _describe(x, gate, mask, form)
+    desc = _describe(x, gate, mask, B, L, D, form)
     lib = nat.load()
     residual = x.new_empty(lib.ews_gated_scan_residual_bytes(desc), dtype=torch.uint8) if train else None
     size = lib.ews_gated_scan_workspace_bytes(desc)
@@ -63,8 +56,9 @@ def _come_back(x, gate, mask, residual, desc, dtype, dev):
     """Saved tensors that are not where the forward left them, as the library can read them."""
     shape = desc.batch, desc.length, desc.dim
     size = nat.load().ews_gated_scan_residual_bytes(desc)
-    x, gate, mask = _readable(returned(x, dtype, shape, dev), returned(gate, dtype, shape, dev),
-                              returned(mask, torch.bool, shape[:2], dev))
+    if returned(mask, torch.bool, shape[:2], dev) is not None:
+        mask = mask.contiguous()
+    x, gate = _neighbours(returned(x, dtype, shape, dev)), _neighbours(returned(gate, dtype, shape, dev))
     return x, gate, mask, aligned(returned(residual, torch.uint8, (size,), dev))
 
 
@@ -73,7 +67,8 @@ class _GatedScan(torch.autograd.Function):
     def forward(ctx, x, gate, state, mask, form):
         out, last, residual, desc, size, at = _forward(x, gate, mask, state, None, form, True)
         ctx.save_for_backward(x, gate, mask, residual)
-        ctx.args = desc, size, form, (*at, residual.data_ptr()), layouts((x, gate))
+        ctx.args = desc, size, form, at, (residual.data_ptr(), x.stride(), gate.stride(),
+                                            mask is not None and mask.stride(), x.dtype)
         ctx.set_materialize_grads(False)
         return out, last
 
@@ -83,13 +78,14 @@ class _GatedScan(torch.autograd.Function):
         if gout is None and glast is None:
             return None, None, None, None, None
         x, gate, mask, residual = ctx.saved_tensors
-        desc, size, form, forward_at, laid_out = ctx.args
-        at = x.data_ptr(), gate.data_ptr(), _ptr(mask), residual.data_ptr()
-        if at != forward_at or layouts((x, gate)) != laid_out:
-            x, gate, mask, residual = _come_back(x, gate, mask, residual, desc, laid_out[0][1],
+        desc, size, form, forward_at, (left, x_strides, gate_strides, mask_strides, dtype) = ctx.args
+        at, starts = (x.data_ptr(), gate.data_ptr(), _ptr(mask)), residual.data_ptr()
+        if (at != forward_at or starts != left or x.stride() != x_strides or gate.stride() != gate_strides
+                or (mask_strides and mask.stride() != mask_strides) or x.dtype is not dtype or gate.dtype is not dtype):
+            x, gate, mask, residual = _come_back(x, gate, mask, residual, desc, dtype,
                                                  (glast if gout is None else gout).device)
-            desc = _describe(x, gate, mask, form)  # the residual's and the scratch's sizes ask for no strides
-            at = x.data_ptr(), gate.data_ptr(), _ptr(mask), residual.data_ptr()
+            desc = _describe(x, gate, mask, *x.shape, form)  # the residual's and the scratch's sizes ask for no strides
+            at, starts = (x.data_ptr(), gate.data_ptr(), _ptr(mask)), residual.data_ptr()
         if gout is not None:
             gout = gout.contiguous()
         if glast is not None:
@@ -98,7 +94,7 @@ class _GatedScan(torch.autograd.Function):
         gstate = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         lib = nat.load()
         ws = x.new_empty(size, dtype=torch.uint8) if size else None
-        nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, *at, _ptr(gout), _ptr(glast), gx.data_ptr(),
+        nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, *at, starts, _ptr(gout), _ptr(glast), gx.data_ptr(),
                          ggate.data_ptr(), _ptr(gstate), _ptr(ws)), "ews_gated_scan_backward")
         return gx, ggate, gstate, None, None
 
@@ -161,7 +157,11 @@ def gated_scan(x, gate, state=None, mask=None, form="convex", last=None):
     if B == 0 or L == 0:  # no step: the state stays
         end = x.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
         return x * gate, end if last is None else last.copy_(end)
-    x, gate, mask = _readable(x, gate, None if mask is None else mask.expand(B, L))
+    x, gate = _neighbours(x), _neighbours(gate)
+    if mask is not None:
+        mask = mask.expand(B, L)
+        if mask.stride(1) != 1 and L > 1:
+            mask = mask.contiguous()
     if state is not None:
         state = state.contiguous()
     if train:
