@@ -121,26 +121,37 @@ struct CopierPair {
   }
 };
 
-// V and G one after the other along k: k blocks of V's rows (the last one's missing rows read its last row, which meets
-// zeros), then as many of G's.
+// V and G one after the other along k, turned: k blocks of V's rows, then as many of G's (or one operand's alone). Rows
+// that a last block lacks meet zeros, and have to be zero for it: an infinity in their place would make NaN. Packed
+// copies have such rows; of an operand that is read as it is that block lies in a copy, V's and behind it G's.
 struct Chain {
   Operand v;
   int64_t to_g;
-  int blocks;  // of either
+  int blocks, whole;      // of either; of those, blocks that have all rows
+  const uint16_t* tail;   // the block after them; or null
+  int64_t tail_ld;
 };
 
 template <class T>
 struct CopierChain {
   static constexpr int kCopies = T::kCopiesP;
+  const Chain& o;
   Copier<true, T::I, T::kThreads> rows;
-  int64_t to_g;
-  int blocks;
-  __device__ __forceinline__ CopierChain(const Chain& o, int tile) : rows(o.v, tile), to_g(o.to_g), blocks(o.blocks) {}
+  __device__ __forceinline__ CopierChain(const Chain& c, int tile) : o(c), rows(c.v, tile) {}
+  __device__ __forceinline__ void aim(int64_t ld) {
+    rows.stride = (uint32_t)ld * 2;
+    rows.aim_turned(63);
+  }
+  // Blocks are asked for in order.
   __device__ __forceinline__ const uint16_t* at(int piece, int kb) {
-    const bool second = kb >= blocks;
-    const int own = second ? kb - blocks : kb;
-    if (second && own == 0) rows.aim_turned(63);  // V's last block may have had fewer
-    return rows.at(piece, own) + (second ? to_g : 0);
+    const bool second = kb >= o.blocks;
+    const int own = second ? kb - o.blocks : kb;
+    if (own == o.whole) {
+      aim(o.tail_ld);
+      return o.tail + (second ? 64 * o.tail_ld : 0);
+    }
+    if (second && own == 0 && o.tail) aim(o.v.ld);  // V's last block lay elsewhere
+    return o.v.p + piece * o.v.plane + own * 64 * o.v.ld + (second ? o.to_g : 0);
   }
   __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const { rows.copy(c, from, to); }
 };
@@ -169,7 +180,7 @@ struct Packs {
   void add(const PackArgs& a) {
     from[count] = blocks;
     each[count++] = a;
-    blocks += (uint32_t)((a.rows * (a.ld / 8) + 255) / 256);
+    blocks += (uint32_t)((a.dst_rows * (a.ld / 8) + 255) / 256);
   }
 };
 
@@ -550,6 +561,9 @@ __device__ __forceinline__ void few_dx_sums(const FewDxArgs& a, int b0, int b1, 
 #pragma unroll
         for (int c = 0; c < kDxCols; ++c) w[s][i][c] = h + c < a.H ? row[h + c] : 0.0f;
       }
+      if (CAREFUL && f + i >= a.F)  // zero times an infinity is not
+#pragma unroll
+        for (int c = 0; c < kDxCols; ++c) w[s][i][c] = 0.0f;
     }
   };
   for (int b = b0; b < b1; b += kAhead) {
@@ -750,7 +764,7 @@ __global__ __launch_bounds__(1024) void k_dbias(const float* sums, int parts, in
 // ------------------------------------------------------------------------------------------------------ the gradients
 struct GradArgs {
   Chain W;                 // dx: k along 2 F
-  Operand X;               // dV | dG: k along the rows
+  Chain X;                 // dV | dG: k along the rows
   Operand Z;               // dv | dg
   int ti, tj, splits, kblocks, per;
   int whole, pieces;       // tiles done by a workgroup each; workgroups that share each of the others
@@ -941,6 +955,7 @@ struct GPlan {
   GProduct dx, dw;
   int dz_rows, dz_parts, narrow_groups;
   int dx_blocks, dx_per, dx_parts;  // of few_dx
+  bool tail_x, tail_w;     // of a backward
   size_t xp, wp, dz, sums, part, total;
 };
 
@@ -993,8 +1008,11 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
     return at;
   };
   if (back || !p.few) {
-    p.xp = take(p.pack_x ? (size_t)(p.N * p.Hp * p.np * 2) : 0);
-    p.wp = take(p.pack_w ? (size_t)(2 * p.F * p.Hp * p.np * 2) : 0);
+    // whole blocks of rows, zeros past the last; or of operands that a backward reads as they are the last block alone
+    p.tail_x = back && !p.pack_x && p.N % 64;
+    p.tail_w = back && !p.pack_w && !p.few_dx && p.F % 64;
+    p.xp = take(p.pack_x ? (size_t)(p.Np * p.Hp * p.np * 2) : p.tail_x ? (size_t)(64 * p.Hp * 2) : 0);
+    p.wp = take(p.pack_w ? (size_t)(2 * p.ld * p.Hp * p.np * 2) : p.tail_w ? (size_t)(128 * p.Hp * 2) : 0);
   }
   if (back) {
     p.dz = take((size_t)(p.Np * 2 * p.ld * p.np * 2));
@@ -1029,23 +1047,50 @@ struct GCall {
   GPlan p;
   char* w;
   hipStream_t st;
-  Operand x;
-  Operand v;
-  int64_t to_g;
+  Chain x;
+  Chain weights;
 };
 
-tiles::PackArgs pack_args(const GPlan& p, const void* src, int64_t stride, int rows, uint16_t* dst, int64_t plane) {
+// Rows of an operand from `first` on, as far as they go, laid out as dst_rows with zeros behind them.
+tiles::PackArgs pack_args(const GPlan& p, const void* src, int64_t stride, int first, int rows, int dst_rows,
+                          uint16_t* dst, int64_t plane) {
   tiles::PackArgs a{};
-  a.src = src;
+  a.src = (const char*)src + first * stride * (p.np == 3 ? 4 : 2);
   a.stride = stride;
-  a.rows = rows;
+  a.rows = rows - first;
   a.cols = p.H;
   a.dst = dst;
   a.ld = p.Hp;
   a.plane = plane;
-  a.dst_rows = rows;
+  a.dst_rows = dst_rows;
   a.wide = tiles::rows_wide(src, stride, p.np == 3);
   return a;
+}
+
+// An operand, or V and G (g; else null), as the tiles read them. packed: copies of all rows, else tail: of the last,
+// incomplete block. to: where those go; want: whether the call reads them.
+Chain lay_out(Packs& a, const GPlan& p, const void* v, int64_t v_stride, const void* g, int64_t g_stride, int rows,
+              bool packed, bool tail, char* to, bool want) {
+  const int padded = ceil_div(rows, 64) * 64, sides = g ? 2 : 1;
+  Chain c{};
+  c.blocks = padded / 64;
+  c.whole = c.blocks;
+  if (packed) {
+    c.v = Operand{(const uint16_t*)to, p.Hp, sides * padded * p.Hp, padded, (int)p.Hp};
+    c.to_g = padded * p.Hp;
+  } else {
+    c.v = Operand{(const uint16_t*)v, v_stride, 0, rows, (int)p.Hp};
+    c.to_g = g ? ((intptr_t)g - (intptr_t)v) / 2 : 0;
+    if (!tail) return c;
+    c.whole = rows / 64;
+    c.tail = (const uint16_t*)to;
+    c.tail_ld = p.Hp;
+  }
+  if (!want) return c;
+  const int first = packed ? 0 : c.whole * 64, each = packed ? padded : 64;
+  a.add(pack_args(p, v, v_stride, first, rows, each, (uint16_t*)to, c.v.plane));
+  if (g) a.add(pack_args(p, g, g_stride, first, rows, each, (uint16_t*)to + each * p.Hp, c.v.plane));
+  return c;
 }
 
 // The operands, packed where they cannot be read as they are. want_x, want_w: those that the call reads.
@@ -1053,23 +1098,8 @@ int operands(GCall& c, const void* x, const void* v, const void* g, bool want_x,
   const GPlan& p = c.p;
   const ews_gated_desc* s = c.s;
   Packs a{};
-  c.x = Operand{(const uint16_t*)x, s->x_stride, 0, p.N, (int)p.Hp};
-  if (p.pack_x) {
-    uint16_t* to = (uint16_t*)(c.w + p.xp);
-    c.x = Operand{to, p.Hp, p.N * p.Hp, p.N, (int)p.Hp};
-    if (want_x) a.add(pack_args(p, x, s->x_stride, p.N, to, c.x.plane));
-  }
-  c.v = Operand{(const uint16_t*)v, s->weight_stride, 0, p.F, (int)p.Hp};
-  c.to_g = ((intptr_t)g - (intptr_t)v) / 2;
-  if (p.pack_w) {
-    uint16_t* to = (uint16_t*)(c.w + p.wp);
-    c.v = Operand{to, p.Hp, 2 * p.F * p.Hp, p.F, (int)p.Hp};
-    c.to_g = p.F * p.Hp;
-    if (want_w) {
-      a.add(pack_args(p, v, s->weight_stride, p.F, to, c.v.plane));
-      a.add(pack_args(p, g, s->gate_stride, p.F, to + c.to_g, c.v.plane));
-    }
-  }
+  c.x = lay_out(a, p, x, s->x_stride, nullptr, 0, p.N, p.pack_x, p.tail_x, c.w + p.xp, want_x);
+  c.weights = lay_out(a, p, v, s->weight_stride, g, s->gate_stride, p.F, p.pack_w, p.tail_w, c.w + p.wp, want_w);
   if (!a.blocks) return EWS_OK;
   if (p.np == 3)
     hipLaunchKernelGGL((k_packs<float>), dim3(a.blocks), dim3(256), 0, c.st, a);
@@ -1301,8 +1331,8 @@ int ews_gated_forward(const ews_gated_desc* desc, const void* x, const void* wei
   rc = operands(c, x, weight, gate_weight, true, true);
   if (rc != EWS_OK) return rc;
   ForwardArgs a{};
-  a.W = Pair{c.v, c.to_g};
-  a.X = c.x;
+  a.W = Pair{c.weights.v, c.weights.to_g};
+  a.X = c.x.v;
   a.ti = c.p.forward.ti;
   a.tj = c.p.forward.tj;
   a.kblocks = c.p.forward.kblocks;
@@ -1401,7 +1431,7 @@ int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* we
     rc = launch_join<false, float>(a, c.st);
     if (rc != EWS_OK) return rc;
   } else if (grad_x) {
-    a.W = Chain{c.v, c.to_g, (int)(p.ld / 64)};
+    a.W = c.weights;
     a.Z = Operand{z.dz, 2 * p.ld, z.plane, (int)p.Np, 0};
     a.J = p.N;
     a.out = grad_x;
