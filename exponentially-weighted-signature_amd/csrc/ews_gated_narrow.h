@@ -16,10 +16,13 @@
 //          32 rows at a time. The sums stay in registers; the workgroups' are joined by k_join_narrow in order.
 //
 // Float32 is multiplied as six products of bfloat16 planes; dv and dg of bfloat16 calls have two planes, which costs
-// nothing here and rounds the gradients once.
+// nothing here and rounds the gradients once. The second plane, of either sign or 0, must not meet an infinity: where V
+// or G hold one, or the rows of x, which makes their v infinite or NaN, the products are formed with care.
 #pragma once
 
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "ews_hip.h"
 #include "ews_pack.h"
@@ -104,6 +107,20 @@ __device__ __forceinline__ void mac(const bf16x8 (&p)[NA], const bf16x8 (&q)[NB]
     for (int n = (NA > NB ? NA : NB) - 1; n >= 0; --n)
       acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p[NA > 1 ? n : 0], q[NB > 1 ? n : 0], acc, 0, 0, 0);
   }
+}
+
+// The same of one plane w, which may hold infinities, and two planes z: W_FIRST, w is the first operand.
+template <bool W_FIRST, int NZ>
+__device__ __forceinline__ void mac_infinite(const bf16x8& w, const bf16x8 (&z)[NZ], f32x4v& acc) {
+  u32x4 u = __builtin_bit_cast(u32x4, w);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if ((u[q] & 0x7f80u) == 0x7f80u) u[q] &= 0xffff0000u;
+    if ((u[q] & 0x7f800000u) == 0x7f800000u) u[q] &= 0xffffu;
+  }
+  const bf16x8 finite = __builtin_bit_cast(bf16x8, u);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(W_FIRST ? finite : z[1], W_FIRST ? z[1] : finite, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(W_FIRST ? w : z[0], W_FIRST ? z[0] : w, acc, 0, 0, 0);
 }
 
 // Eight neighbouring numbers of a row from column k on, zero past the row's end.
@@ -296,14 +313,26 @@ __global__ __launch_bounds__((64 * Narrow<T, HB, FB>::kWaves)) void k_narrow_bac
 #pragma unroll
       for (int h = 0; h < 2 * HB; ++h) dw[i][h][r] = 0.0f;
     }
+  bool infinite_weights = false;
+  if (NZ == 2) {
+    for (int n = 0; n < S::kFront; ++n) {
+      const u32x4 u = __builtin_bit_cast(u32x4, frag[n * 64 + lane]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        infinite_weights |= (u[q] & 0x7f80u) == 0x7f80u || (u[q] & 0x7f800000u) == 0x7f800000u;
+    }
+    infinite_weights = __any(infinite_weights);
+  }
   const int step = gridDim.x * S::kWaves * 32;
   for (int n0 = (blockIdx.x * S::kWaves + wave) * 32; n0 < a.N; n0 += step) {
+    bool infinite = infinite_weights;  // an operand of these rows may be
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int n = n0 + c * 16 + r16;
       T x[HB][8];
       f32x4v z[2][2 * FB];
       front_of<T, HB, FB>(a, frag, n0 + c * 16, x, z);
+      if (NZ == 2) infinite |= __any(!__builtin_isfinite(z[0][0][0]));  // as with any infinity in the row of x
       // z becomes dv and dg
 #pragma unroll
       for (int f16 = 0; f16 < 2 * FB; ++f16) {
@@ -335,7 +364,7 @@ __global__ __launch_bounds__((64 * Narrow<T, HB, FB>::kWaves)) void k_narrow_bac
           for (int e = 0; e < 8; ++e)
             turn[(2 * S::FP + hb * 32 + k8 + e) * kTurnRow + c * 16 + r16] = widen(x[hb][e]);
       }
-      if (a.dx) {
+      auto form_dx = [&](auto careful) {
         f32x4v d[2 * HB];
 #pragma unroll
         for (int h = 0; h < 2 * HB; ++h) d[h] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -353,7 +382,10 @@ __global__ __launch_bounds__((64 * Narrow<T, HB, FB>::kWaves)) void k_narrow_bac
               bf16x8 w[NP];
 #pragma unroll
               for (int q = 0; q < NP; ++q) w[q] = frag[S::turned(q, side, fb, h) * 64 + lane];
-              mac(w, p, d[h]);
+              if constexpr (decltype(careful)::value)
+                mac_infinite<true>(w[0], p, d[h]);
+              else
+                mac(w, p, d[h]);
             }
           }
         if (n < a.N) {
@@ -363,6 +395,12 @@ __global__ __launch_bounds__((64 * Narrow<T, HB, FB>::kWaves)) void k_narrow_bac
             store_four<T>((T*)a.dx + (int64_t)n * a.H, h * 16 + q4, a.H, a.wide_h, y);
           }
         }
+      };
+      if (a.dx) {
+        if (NZ == 2 && infinite)
+          form_dx(std::bool_constant<NZ == 2>{});
+        else
+          form_dx(std::false_type{});
       }
     }
     if (!a.part) continue;
@@ -381,21 +419,32 @@ __global__ __launch_bounds__((64 * Narrow<T, HB, FB>::kWaves)) void k_narrow_bac
       }
       fragments<T>(y, px[h]);
     }
+    auto add_dw = [&](auto careful) {
 #pragma unroll
-    for (int i = 0; i < 4 * FB; ++i) {
-      const float* from = turn + (i * 16 + r16) * kTurnRow + k8;
-      float y[8];
+      for (int i = 0; i < 4 * FB; ++i) {
+        const float* from = turn + (i * 16 + r16) * kTurnRow + k8;
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const f32x4 w = *reinterpret_cast<const f32x4*>(from + e);
+        for (int e = 0; e < 8; e += 4) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(from + e);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[e + k] = w[k];
+          for (int k = 0; k < 4; ++k) y[e + k] = w[k];
+        }
+        bf16x8 pz[NZ];
+        z_fragments<NZ>(y, pz);
+#pragma unroll
+        for (int h = 0; h < 2 * HB; ++h) {
+          if constexpr (decltype(careful)::value)
+            mac_infinite<false>(px[h][0], pz, dw[i][h]);
+          else
+            mac(pz, px[h], dw[i][h]);
+        }
       }
-      bf16x8 pz[NZ];
-      z_fragments<NZ>(y, pz);
-#pragma unroll
-      for (int h = 0; h < 2 * HB; ++h) mac(pz, px[h], dw[i][h]);
-    }
+    };
+    if (NZ == 2 && infinite)
+      add_dw(std::bool_constant<NZ == 2>{});
+    else
+      add_dw(std::false_type{});
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
   }
