@@ -164,6 +164,15 @@ __device__ __forceinline__ uint32_t steps_on(const Args& a, uint64_t mask, int t
 }
 static_assert(kSteps == 8, "two bits a step in one word, a byte of the mask each in another");
 
+// A product of convex gates is 0 by underflow alone, but zero times an infinite state, which the steps one by one would
+// keep, is NaN. So such products are held at float32's least number: of a finite state that is 2^-149 of it in place of
+// less, which is nothing beside float32's roundings unless it was beyond 2^100 (looking for NaN and composing again with
+// care took 3 to 5% of strips).
+template <bool CONVEX>
+__device__ __forceinline__ float above_zero(float a) {
+  return CONVEX ? fmaxf(a, 1.40129846e-45f) : a;
+}
+
 // (a, b) = (a2, b2) after (a, b).
 __device__ __forceinline__ void then(float& a, float& b, float a2, float b2) {
   b = fmaf(a2, b, b2);
@@ -227,13 +236,15 @@ __global__ __launch_bounds__(64 * WAVES) void k_forward(Args a) {
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = carry[v];
     } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) A[v] = above_zero<CONVEX>(A[v]);
       for (int d = row; d < 64; d <<= 1)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float a0 = __shfl_up(A[v], d), h0 = __shfl_up(H[v], d);
           if (lane >= d) {
             then(a0, h0, A[v], H[v]);
-            A[v] = a0;
+            A[v] = above_zero<CONVEX>(a0);
             H[v] = h0;
           }
         }
@@ -348,7 +359,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_backward(Args a) {
         for (int i = 0; i < kSteps; ++i) then(A[v], H[v], ka[i][v], take[i][v] * x[i][v]);
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) M[v] = ka[i][v] * (u[i][v] + M[v]);
-        B[v] = A[v];
+        B[v] = A[v] = above_zero<CONVEX>(A[v]);
       }
       for (int d = row; d < 64; d <<= 1)
 #pragma unroll
@@ -356,13 +367,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_backward(Args a) {
           float a0 = __shfl_up(A[v], d), h0 = __shfl_up(H[v], d);
           if (lane >= d) {
             then(a0, h0, A[v], H[v]);
-            A[v] = a0;
+            A[v] = above_zero<CONVEX>(a0);
             H[v] = h0;
           }
           float b0 = __shfl_down(B[v], d), m0 = __shfl_down(M[v], d);
           if (lane + d < 64) {
             then(b0, m0, B[v], M[v]);
-            B[v] = b0;
+            B[v] = above_zero<CONVEX>(b0);
             M[v] = m0;
           }
         }
@@ -482,7 +493,7 @@ __global__ __launch_bounds__(512) void k_ends(Args a) {
           H[v] = f * (x[v] + H[v]);
         else
           H[v] = fmaf(f, H[v], take * x[v]);
-        A[v] *= f;
+        A[v] = above_zero<CONVEX>(A[v] * f);
       }
     }
   }
@@ -496,6 +507,7 @@ __global__ __launch_bounds__(512) void k_ends(Args a) {
     for (int n = 0; n < slots; ++n) {
       const float2 e = parts[((BACK ? slots - 1 - n : n) << a.shift) + threadIdx.x][v];
       then(A[v], H[v], e.x, e.y);
+      A[v] = above_zero<CONVEX>(A[v]);
     }
     const int64_t to = ((int64_t)at.seg * a.B + at.b) * a.D + at.c + v;
     if (!BACK && a.state && at.seg == 0) a.first[to] = a.state[to];
