@@ -66,8 +66,7 @@ class _Call:
         x = self.operands[0]
         lib = nat.load()
         out = x.new_empty((self.desc.rows, self.desc.features))
-        size = lib.ews_gated_kept_bytes(self.desc) if keep else 0
-        kept = x.new_empty(size, dtype=torch.uint8) if size else None
+        kept = _scratch(x, lib.ews_gated_kept_bytes(self.desc)) if keep else None
         ws = _scratch(x, self.scratch_bytes(nat.GATED_KEEP if keep else nat.GATED_FORWARD))
         nat.check(launch(x.device, lib.ews_gated_forward, self.desc, *self.at, out.data_ptr(), _ptr(kept), _ptr(ws)),
                   "ews_gated_forward")

@@ -9,6 +9,7 @@ from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from .embed import DTYPES, aligned, check_tensor, launch, once, refuse_tangents, returned
+from .gated import _scratch
 
 
 def _ptr(t):
@@ -43,9 +44,9 @@ def _forward(x, gate, mask, state, last, form, train):
         last = x.new_empty((B, D), dtype=torch.float32)
     desc = _describe(x, gate, mask, B, L, D, form)
     lib = nat.load()
-    residual = x.new_empty(lib.ews_gated_scan_residual_bytes(desc), dtype=torch.uint8) if train else None
+    residual = _scratch(x, lib.ews_gated_scan_residual_bytes(desc)) if train else None
     size = lib.ews_gated_scan_workspace_bytes(desc)
-    ws = x.new_empty(size, dtype=torch.uint8) if size else None
+    ws = _scratch(x, size)
     at = x.data_ptr(), gate.data_ptr(), _ptr(mask)
     nat.check(launch(x.device, lib.ews_gated_scan_forward, desc, *at, _ptr(state), out.data_ptr(), last.data_ptr(),
                      _ptr(residual), _ptr(ws)), "ews_gated_scan_forward")
@@ -93,7 +94,7 @@ class _GatedScan(torch.autograd.Function):
         gx, ggate = x.new_empty(x.shape), x.new_empty(x.shape)
         gstate = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         lib = nat.load()
-        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        ws = _scratch(x, size)
         nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, *at, starts, _ptr(gout), _ptr(glast), gx.data_ptr(),
                          ggate.data_ptr(), _ptr(gstate), _ptr(ws)), "ews_gated_scan_backward")
         return gx, ggate, gstate, None, None
