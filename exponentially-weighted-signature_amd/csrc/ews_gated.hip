@@ -46,31 +46,40 @@ using namespace ews::vec;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// s(g) and s(-g), either without the other's rounding.
+// s(g) and s(-g), either without the other's rounding. FINE: nor that of g log2(e), |g| 2^-24 of exp(-g), which bfloat16
+// results do not show.
+template <bool FINE>
 __device__ __forceinline__ void logistic(float g, float& p, float& q) {
   const float y = g * -kLog2e;
-  const float e = __builtin_amdgcn_exp2f(y);
+  float e = __builtin_amdgcn_exp2f(y);
+  if (FINE) {
+    constexpr float kLog2eRest = 1.925963033500e-8f, kLn2 = 0.693147180559945309f;
+    const float rest = fmaf(g, -kLog2eRest, fmaf(g, -kLog2e, -y));
+    e = fabsf(y) < 126.0f ? fmaf(e, rest * kLn2, e) : e;
+  }
   p = __builtin_amdgcn_rcpf(1.0f + e);
   q = y > 126.0f ? 1.0f : e * p;  // e may be infinite
 }
 
-// act(g) and act'(g).
+// act(g) and act'(g) for a call of type T.
+template <typename T>
 __device__ __forceinline__ void activate(int kind, float g, float& act, float& slope) {
   if (kind == EWS_GATED_RELU) {
     act = g <= 0.0f ? 0.0f : g;  // a NaN stays one
     slope = g > 0.0f ? 1.0f : 0.0f;
     return;
   }
+  constexpr bool kFine = sizeof(T) == 4;
   float p, q;
   if (kind == EWS_GATED_GELU) {
     const float c = g > 30.0f ? 30.0f : g < -30.0f ? -30.0f : g;  // s is 0 or 1 long before; g^3 stays finite
     const float c2 = c * c;
-    logistic(1.5957691216057308f * c * fmaf(0.044715f, c2, 1.0f), p, q);
+    logistic<kFine>(1.5957691216057308f * c * fmaf(0.044715f, c2, 1.0f), p, q);
     act = g * p;
     slope = fmaf(c * p * q, 1.5957691216057308f * fmaf(0.134145f, c2, 1.0f), p);
     return;
   }
-  logistic(g, p, q);
+  logistic<kFine>(g, p, q);
   act = kind == EWS_GATED_SILU ? g * p : p;
   slope = kind == EWS_GATED_SILU ? fmaf(g * p, q, p) : p * q;
 }
@@ -345,7 +354,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWaves) void k_forward(ForwardArgs 
         v[t][r] = acc[t][b][r] + bias[i];
         g[t][r] = acc[t + kHalf][b][r] + bias[T::I / 2 + i];
         float act, slope;
-        activate(a.act, g[t][r], act, slope);
+        activate<O>(a.act, g[t][r], act, slope);
         y[t][r] = v[t][r] * act;
       }
     const int row0 = j0 + (wj * T::TJ + b) * 32, col0 = i0 + wi * kHalf * 32;
@@ -509,7 +518,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(FewArgs a) {
       v[r] = sv[r] + bias_at<T>(a.bias, in);
       g[r] = sg[r] + bias_at<T>(a.gate_bias, in);
       float act, slope;
-      activate(a.act, g[r], act, slope);
+      activate<T>(a.act, g[r], act, slope);
       if (f + r < a.F) ((T*)a.out)[(int64_t)n * a.F + f + r] = narrow<T>(v[r] * act);
     }
     if (a.kept && f < a.F) {
@@ -701,7 +710,7 @@ __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         float act, slope;
-        activate(a.act, both[1][q], act, slope);
+        activate<T>(a.act, both[1][q], act, slope);
         both[1][q] = q < live ? u[q] * (both[0][q] * slope) : 0.0f;
         both[0][q] = q < live ? u[q] * act : 0.0f;
       }

@@ -284,7 +284,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void k_narrow_forward(NarrowArgs
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float act, slope;
-        activate(a.act, z[1][f16][r] + bias[S::FP + f + r], act, slope);
+        activate<T>(a.act, z[1][f16][r] + bias[S::FP + f + r], act, slope);
         y[r] = (z[0][f16][r] + bias[f + r]) * act;
       }
       if (n < a.N) store_four<T>((T*)a.out + (int64_t)n * a.F, f, a.F, a.wide_f, y);
@@ -343,7 +343,7 @@ __global__ __launch_bounds__((64 * Narrow<T, HB, FB>::kWaves)) void k_narrow_bac
           const int f = f16 * 16 + q4 + r;
           float act, slope;
           const float v = z[0][f16][r] + bias[f];
-          activate(a.act, z[1][f16][r] + bias[S::FP + f], act, slope);
+          activate<T>(a.act, z[1][f16][r] + bias[S::FP + f], act, slope);
           z[0][f16][r] = n < a.N ? u[r] * act : 0.0f;
           z[1][f16][r] = n < a.N ? u[r] * (v * slope) : 0.0f;
         }
