@@ -996,7 +996,7 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
   p.narrow = p.H <= kNarrowWidth && p.F <= kNarrowWidth && (back || keep || !p.few);  // and keeps nothing
   if (p.narrow) {
     // 32 rows a wavefront and turn; as many workgroups as are on the CUs at a time
-    const int groups = ceil_div(p.N, 32 * 4);
+    const int groups = ceil_div(p.N, 32 * (p.np == 3 ? narrow_waves<float>(p.H, p.F) : narrow_waves<bf16>(p.H, p.F)));
     p.narrow_groups = groups < 512 ? groups : 512;
     p.part = 0;
     p.total = back ? (size_t)p.narrow_groups * 2 * narrow_pad(p.F) * (narrow_pad(p.H) + 1) * 4 : 0;
@@ -1235,7 +1235,8 @@ int launch_narrow_as(const NarrowArgs& a, int groups, bool back, hipStream_t st)
     const int n = ceil_div(a.N, 16 * kNarrowWaves);
     hipLaunchKernelGGL((k_narrow_forward<T, HB, FB>), dim3(n < 2048 ? n : 2048), dim3(64 * kNarrowWaves), 0, st, a);
   } else {
-    static_assert(S::kLdsBytes <= 160 << 10 && 2 * S::FP * (S::HP + 1) * 4 <= S::kLdsBytes, "the sums fit too");
+    static_assert(S::kLdsBytes <= 160 << 10 && S::kWaves * 2 * S::FP * (S::HP + 1) * 4 <= S::kLdsBytes,
+                  "the sums fit too");
     const int rc = tiles::allow_lds(k_narrow_backward<T, HB, FB>, S::kLdsBytes);
     if (rc != EWS_OK) return rc;
     hipLaunchKernelGGL((k_narrow_backward<T, HB, FB>), dim3(groups), dim3(64 * S::kWaves), S::kLdsBytes, st, a);

@@ -192,6 +192,13 @@ struct Narrow {
   static __device__ __forceinline__ int f_of(int lane, int e) { return (e >> 2) * 16 + (lane >> 4) * 4 + (e & 3); }
 };
 
+// Wavefronts of a workgroup of the backward.
+template <typename T>
+int narrow_waves(int H, int F) {
+  if (H <= 32) return F <= 32 ? Narrow<T, 1, 1>::kWaves : Narrow<T, 1, 2>::kWaves;
+  return F <= 32 ? Narrow<T, 2, 1>::kWaves : Narrow<T, 2, 2>::kWaves;
+}
+
 // V's and G's fragments and the biases ([side][FP]) into LDS.
 template <typename T, int HB, int FB, int WAVES, bool BACK>
 __device__ __forceinline__ void lay_out(const NarrowArgs& a, bf16x8* frag, float* bias) {
@@ -449,28 +456,32 @@ __global__ __launch_bounds__((64 * Narrow<T, HB, FB>::kWaves)) void k_narrow_bac
     __builtin_amdgcn_wave_barrier();
   }
   if (!a.part) return;
-  // the wavefronts' sums one after the other into LDS, then out
-  constexpr int kRow = S::HP + 1;
+  // the wavefronts' sums side by side into LDS, then added in order and out
+  constexpr int kRow = S::HP + 1, kSums = 2 * S::FP * kRow;
   float* sum = reinterpret_cast<float*>(lds);
-  for (int w = 0; w < S::kWaves; ++w) {
-    __syncthreads();
-    if (w != wave) continue;
 #pragma unroll
-    for (int i = 0; i < 4 * FB; ++i)
+  for (int i = 0; i < 4 * FB; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float* to = sum + (i * 16 + q4 + r) * kRow;
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int h = 0; h < 2 * HB; ++h) to[h * 16 + r16] = (w ? to[h * 16 + r16] : 0.0f) + dw[i][h][r];
-        float s = db[i][r];
-#pragma unroll
-        for (int d = 8; d; d >>= 1) s += __shfl_xor(s, d);
-        if (r16 == 0) to[S::HP] = (w ? to[S::HP] : 0.0f) + s;
-      }
-  }
+      for (int d = 8; d; d >>= 1) db[i][r] += __shfl_xor(db[i][r], d);
   __syncthreads();
-  for (int t = threadIdx.x; t < 2 * S::FP * kRow; t += 64 * S::kWaves)
-    a.part[(int64_t)blockIdx.x * 2 * S::FP * kRow + t] = sum[t];
+#pragma unroll
+  for (int i = 0; i < 4 * FB; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float* to = sum + wave * kSums + (i * 16 + q4 + r) * kRow;
+#pragma unroll
+      for (int h = 0; h < 2 * HB; ++h) to[h * 16 + r16] = dw[i][h][r];
+      if (r16 == 0) to[S::HP] = db[i][r];
+    }
+  __syncthreads();
+  for (int t = threadIdx.x; t < kSums; t += 64 * S::kWaves) {
+    float s = sum[t];
+#pragma unroll
+    for (int w = 1; w < S::kWaves; ++w) s += sum[w * kSums + t];
+    a.part[(int64_t)blockIdx.x * kSums + t] = s;
+  }
 }
 
 // The workgroups' sums added in order: 64 of them at a time by a workgroup, its sixteen wavefronts a contiguous part of
