@@ -15,9 +15,10 @@
 // dg from them, one after the other along a row, so that dx is one product over 2 F, and dV and dG are one of 2 F rows.
 // What act and act' of g take is hidden there behind the memory; where the sums end it adds to the matrix cores' time.
 //
-// Measured (N=8192, H=2048, F=5504, bfloat16, 1.11e12 operations, 1.09 ms): v and g 0.44 (0.84 PFLOP/s: 1376 tiles are
-// 5.4 rounds of the CUs, and 270 MB kept are written), k_dz 0.105 (5.1 TB/s), dx 0.32 (1.16 PFLOP/s), dV and dG 0.36
-// (1.03). Float32 (N=4095, H=512, F=1365) 0.29: 93, 78 and 82 us the three (122 to 147 TFLOP/s). One row of H=4096,
+// Measured (N=8192, H=2048, F=5504, bfloat16, 1.11e12 operations, 1.08 to 1.12 ms over cards, calls in a row): the
+// medians of a trace, which runs slower (1.25 ms of kernels), are v and g 0.44 (0.85 PFLOP/s: 1376 tiles are 5.4 rounds
+// of the CUs, and 270 MB kept are written), k_dz 0.106 (5.1 TB/s), dx 0.325 (1.14 PFLOP/s), dV and dG 0.37 (0.99).
+// Float32 (N=4095, H=512, F=1365) 0.29 to 0.32 ms: 92, 78 and 84 us the three (122 to 147 TFLOP/s). One row of H=4096,
 // F=11000, bfloat16: 34 us, 5.3 TB/s.
 //
 // Narrow maps (both widths up to 64) have kernels of their own (ews_gated_narrow.h), and keep nothing.
@@ -46,8 +47,8 @@ using namespace ews::vec;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// s(g) and s(-g), either without the other's rounding. FINE: nor that of g log2(e), |g| 2^-24 of exp(-g), which bfloat16
-// results do not show.
+// s(g) and s(-g), either without the other's rounding. FINE: nor that of g log2(e), |g| 2^-24 of exp(-g), which
+// bfloat16 results do not show.
 template <bool FINE>
 __device__ __forceinline__ void logistic(float g, float& p, float& q) {
   const float y = g * -kLog2e;

@@ -14,7 +14,8 @@
 //
 // A few operations a number: memory bounds it. The forward reads x and g and writes h; the backward reads x, g and dh
 // and writes dx and dg. It forms the states anew from those at the starts of tiles, which the forward leaves in float32
-// (one state in 64 steps or more): h in bfloat16 would be as large as x, and dg would lose what h - x cancels.
+// (one state in the 8 steps of a thread that walks alone, 8% more bytes of a bfloat16 forward and 5% of its backward;
+// in 64 to 512 of a strip's tile): h in bfloat16 would be as large as x, and dg would lose what h - x cancels.
 //
 // A step is the map h -> a h + b, and maps compose: (a2, b2) after (a1, b1) is (a2 a1, a2 b1 + b2). A workgroup owns a
 // strip of channels of one sequence and walks it in tiles of steps, a thread kSteps steps of its channels: it composes
@@ -23,9 +24,10 @@
 // its channels alone and nothing is exchanged. Where there are few, sequences are cut into segments: a first launch
 // composes each segment's steps (k_ends), and each workgroup of the second applies those before its own.
 //
-// Measured, bfloat16: 8 x 4095 x 2048 (strips) forward 104 us (3.9 TB/s with the tiles' states), backward 153 (4.4),
-// one workgroup a CU and the VALU busy for half of it; 1 x 131071 x 1024 (segments, which read x and g, backward g and
-// dh, twice) 148 + 176 and 139 + 314; a step of 8 x 1 x 2048 3.6.
+// Medians of a trace of ten calls, bfloat16: 8 x 4095 x 2048 (strips) forward 106 us (3.8 TB/s with the tiles' states),
+// backward 155 (4.4), one workgroup a CU and the VALU busy for half of it; 1 x 131071 x 1024 (segments, which read x
+// and g, backward g and dh, twice) 143 + 164 and 139 + 299; a step of 8 x 1 x 2048 3.6. (Calls in a row, untraced, take
+// a twentieth less.)
 #include <hip/hip_runtime.h>
 
 #include "ews_hip.h"
@@ -166,8 +168,8 @@ static_assert(kSteps == 8, "two bits a step in one word, a byte of the mask each
 
 // A product of convex gates is 0 by underflow alone, but zero times an infinite state, which the steps one by one would
 // keep, is NaN. So such products are held at float32's least number: of a finite state that is 2^-149 of it in place of
-// less, which is nothing beside float32's roundings unless it was beyond 2^100 (looking for NaN and composing again with
-// care took 3 to 5% of strips).
+// less, which is nothing beside float32's roundings unless it was beyond 2^100 (looking for NaN and composing again
+// with care took 3 to 5% of strips).
 template <bool CONVEX>
 __device__ __forceinline__ float above_zero(float a) {
   return CONVEX ? fmaxf(a, 1.40129846e-45f) : a;

@@ -16,7 +16,11 @@ reference (``norm1``, ``ewms``, ``graded``, ``c_down``, ``gate``, ``norm2``, ``f
 the reference's constructor: the generator is passed as a module (``a_param``, any parametrisation of
 ``ews_mi355x.params``; default the reference's definite_plus_skew with entries N(0, 0.005)) instead of an ``a_config``
 dict, and ``key`` is an int seed or a ``torch.Generator`` (initial values are drawn from the same distributions as the
-reference's, not the same numbers). Dropout draws from torch's generator."""
+reference's, not the same numbers). Dropout draws from torch's generator.
+
+A gated channel stage calls its maps, as it did before it had a kernel, where one is more than a map (hooks, a
+parametrization), under autocast, and where one or what goes in carries a forward-mode tangent; a backward that is asked
+for a graph of itself is formed by the maps' operations. ``fused_channel = False`` calls them always."""
 
 from __future__ import annotations
 

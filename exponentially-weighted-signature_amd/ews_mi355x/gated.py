@@ -105,7 +105,8 @@ def _come_back(operands, kept, desc, dtype, dev):
     rows = 2 * F if operands[3] is None else F
     shapes = (N, H), (rows, H), (rows,), (F, H), (F,)
     size = nat.load().ews_gated_kept_bytes(desc)
-    return [returned(t, dtype, s, dev) for t, s in zip(operands, shapes)], aligned(returned(kept, torch.uint8, (size,), dev))
+    operands = [returned(t, dtype, s, dev) for t, s in zip(operands, shapes)]
+    return operands, aligned(returned(kept, torch.uint8, (size,), dev))
 
 
 class _GatedLinear(torch.autograd.Function):
@@ -170,8 +171,8 @@ def takes(x, weight, bias):
 
 
 def gated_stage(x, weight, bias=None, gate_weight=None, gate_bias=None):
-    """``gated_linear`` for a block's gated channel stage, whose maps have second derivatives: a graph of the backward is
-    that of the maps' own."""
+    """``gated_linear`` for a block's gated channel stage, whose maps have second derivatives: a graph of the backward
+    is that of the maps' own."""
     return _gated(_GatedStage, x, weight, bias, gate_weight, gate_bias, "sigmoid")
 
 

@@ -289,9 +289,10 @@ def linear_distillation(hidden, weight, indices, logits, bias=None, temperature=
     int32 and logits (..., K) float32 or bfloat16, K up to 1024: the teacher's tokens of every position and their
     logits, in any order, the teacher's distribution being that over them alone. T is ``temperature`` (1e-6 to 1e4);
     its square keeps the gradients' size. At a high one p and q differ by little: float32's rounding of them, 2^-20 of
-    q at most, is T 2^-20 of q in a gradient (1% of a token's at T = 1e4 and logits a unit apart). ``reduction``: "mean" over the rows that have an entry (0 where none has),
-    "sum", or "none" for every row's own loss, (...), float32. Differentiable in hidden, weight and bias (reverse
-    mode); the teacher's logits have no gradient, and one that requires it is refused: detach them.
+    q at most, is T 2^-20 of q in a gradient (1% of a token's at T = 1e4 and logits a unit apart). ``reduction``: "mean"
+    over the rows that have an entry (0 where none has), "sum", or "none" for every row's own loss, (...), float32.
+    Differentiable in hidden, weight and bias (reverse mode); the teacher's logits have no gradient, and one that
+    requires it is refused: detach them.
 
     An entry with a negative index or a logit of -inf is none: rows may have fewer than K. A row without any has loss
     and gradient zero, whatever it holds, and costs nothing. A token that is named twice is two entries of its

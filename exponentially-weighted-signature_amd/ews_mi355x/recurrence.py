@@ -37,7 +37,7 @@ def _describe(x, gate, mask, B, L, D, form):
 
 
 def _forward(x, gate, mask, state, last, form, train):
-    """(out, last, the residual of a training call, the descriptor, the scratch's size and the addresses that it read)."""
+    """(out, last, the residual of a training call, the descriptor, the scratch's size, the addresses that it read)."""
     B, L, D = x.shape
     out = x.new_empty((B, L, D))
     if last is None:
@@ -95,8 +95,8 @@ class _GatedScan(torch.autograd.Function):
         gstate = x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32) if ctx.needs_input_grad[2] else None
         lib = nat.load()
         ws = _scratch(x, size)
-        nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, *at, starts, _ptr(gout), _ptr(glast), gx.data_ptr(),
-                         ggate.data_ptr(), _ptr(gstate), _ptr(ws)), "ews_gated_scan_backward")
+        nat.check(launch(x.device, lib.ews_gated_scan_backward, desc, *at, starts, _ptr(gout), _ptr(glast),
+                         gx.data_ptr(), ggate.data_ptr(), _ptr(gstate), _ptr(ws)), "ews_gated_scan_backward")
         return gx, ggate, gstate, None, None
 
 

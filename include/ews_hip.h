@@ -729,8 +729,8 @@ typedef struct ews_gated_scan_desc {
   int32_t form;                  /* EWS_GATED_SCAN_* */
 } ews_gated_scan_desc;
 
-/* The residual that a forward leaves for its backward, and the scratch of either (0: may be NULL). Both depend on batch,
- * length, dim, dtype and form alone: a backward may be given x and gate with other strides than its forward. */
+/* The residual that a forward leaves for its backward, and the scratch of either (0: may be NULL). Both depend on
+ * batch, length, dim, dtype and form alone: a backward may be given x and gate with other strides than its forward. */
 size_t ews_gated_scan_residual_bytes(const ews_gated_scan_desc* desc);
 size_t ews_gated_scan_workspace_bytes(const ews_gated_scan_desc* desc);
 
@@ -774,7 +774,9 @@ size_t ews_gated_kept_bytes(const ews_gated_desc* desc);
 
 /* Scratch of one call (EWS_GATED_FORWARD, _KEEP or _BACKWARD) with these addresses, of which nothing is read; 0: may be
  * NULL. Packed copies of x and the weights where they cannot be read as they are (float32; bfloat16 rows that do not
- * start at multiples of 16 bytes or whose width is no multiple of 64), and for a backward 2 N F gradients. */
+ * start at multiples of 16 bytes or whose width is no multiple of 64); for a backward 2 N F gradients, and of operands
+ * that are read as they are the last rows that make no whole 64. A backward may be given operands at other strides and
+ * addresses than its forward: its descriptor and scratch are those of what it is given. */
 size_t ews_gated_workspace_bytes(const ews_gated_desc* desc, const void* x, const void* weight,
                                  const void* gate_weight, int call);
 

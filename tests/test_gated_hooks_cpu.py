@@ -1,5 +1,6 @@
-"""What the backward calls of ``gated_scan`` and ``gated_linear`` hand to the library where hooks on saved tensors bring them back with other
-strides or at other addresses: descriptors and scratch of the tensors that came back. The launches are recorded, not run."""
+"""What the backward calls of ``gated_scan`` and ``gated_linear`` hand to the library where hooks on saved tensors bring
+them back with other strides or at other addresses: descriptors and scratch of the tensors that came back. The launches
+are recorded, not run."""
 
 import ctypes
 
@@ -146,7 +147,7 @@ def test_gated_backward_without_hooks_reads_where_the_forward_did(calls):
 @pytest.mark.parametrize("joint", [False, True])
 @pytest.mark.parametrize("turned", [False, True])
 def test_a_stages_graph_of_its_backward(calls, joint, turned):
-    """Its gradients and theirs are those of the maps; turned weights, which the library takes a copy of, keep theirs."""
+    """Its gradients and theirs are those of the maps; turned weights, which the library copies, keep theirs."""
     N, H, F = 9, 6, 5
     g = torch.Generator().manual_seed(1)
 

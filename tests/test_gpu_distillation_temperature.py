@@ -1,9 +1,9 @@
 """``linear_distillation`` at high temperatures and where student and teacher are alike, against float64.
 
-With r the relative error of p / q, ep + e of ``test_gpu_linear_distillation`` (of a logit's error over T, and some twenty
-roundings), a row whose entries name all tokens is T^2 sum_k q_k f(x_k) with x = p / q - 1, f'(x) = log (1 + x) = d and
-f'' = 1 / (1 + x): off by T^2 sum_k q_k (|d_k| r + r^2) and (K + 32) u of itself. Other rows have 1 - sum_k q_k too, off by
-e + (K + 8) u at most, times T^2."""
+With r the relative error of p / q, ep + e of ``test_gpu_linear_distillation`` (of a logit's error over T, and some
+twenty roundings), a row whose entries name all tokens is T^2 sum_k q_k f(x_k) with x = p / q - 1, f'(x) = log (1 + x) =
+d and f'' = 1 / (1 + x): off by T^2 sum_k q_k (|d_k| r + r^2) and (K + 32) u of itself. Other rows have 1 - sum_k q_k
+too, off by e + (K + 8) u at most, times T^2."""
 
 import math
 

@@ -1,7 +1,7 @@
 """The logistic function of float32 gates alone: x = 1 and V = 1 make y = act(g), for every kernel that forms it.
 
-An exponential and a reciprocal of one unit (2 half units of 2^-24) each, its argument's second part (rounded twice, of a
-part that is 2^-24 |g|: nothing), their sum and products, and y's own rounding: 8 half units, at any |g| up to 80."""
+An exponential and a reciprocal of one unit (2 half units of 2^-24) each, its argument's second part (rounded twice, of
+a part that is 2^-24 |g|: nothing), their sum and products, and y's own rounding: 8 half units, at any |g| up to 80."""
 
 import pytest
 import torch

@@ -1,5 +1,5 @@
-"""Gradients of ``gated_linear`` where an infinity stands in the last row of an operand: zeros behind it, which fill up the
-last stage of a product, must not meet it (zero times an infinity is NaN)."""
+"""Gradients of ``gated_linear`` where an infinity stands in the last row of an operand: zeros behind it, which fill up
+the last stage of a product, must not meet it (zero times an infinity is NaN)."""
 
 import pytest
 import torch
@@ -33,8 +33,8 @@ def _same(got, want, off):
 
 @pytest.mark.parametrize("joint", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("N,H,F", [(7, 200, 40), (30, 192, 40), (60, 200, 41), (90, 200, 40), (90, 192, 40), (300, 520, 700),
-                                   (300, 512, 700), (1030, 832, 4616)])
+@pytest.mark.parametrize("N,H,F", [(7, 200, 40), (30, 192, 40), (60, 200, 41), (90, 200, 40), (90, 192, 40),
+                                   (300, 520, 700), (300, 512, 700), (1030, 832, 4616)])
 def test_the_last_row(N, H, F, dtype, joint):
     print(f"{N} {H} {F} {dtype} {joint}", flush=True)
     _check(N, H, F, dtype, joint, ((1, (F - 1, 9)), (3, (F - 1, 9)), (0, (N - 1, 5))))
@@ -44,7 +44,7 @@ def test_the_last_row(N, H, F, dtype, joint):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("N,H,F", [(90, 31, 40), (300, 16, 64), (70, 64, 4), (200, 64, 64), (2111, 32, 32)])
 def test_narrow(N, H, F, dtype, joint):
-    """Widths with kernels of their own, whose dv and dg have two planes for bfloat16: the second is none of an infinity."""
+    """Widths with kernels of their own; bfloat16's dv and dg have two planes there, the second none of an infinity."""
     print(f"{N} {H} {F} {dtype} {joint}", flush=True)
     _check(N, H, F, dtype, joint, ((1, (F - 1, 9)), (3, (1, 2)), (0, (N - 1, 5)), (0, (3, H - 1))))
 

@@ -1,6 +1,6 @@
-"""Gradients of ``gated_linear`` where its operands are views: rows apart, off their 16-byte addresses, turned, V and G at
-different strides. The leaves are what the views are taken of, so the layouts reach the backward; values and bounds are
-those of ``test_gpu_gated_linear``."""
+"""Gradients of ``gated_linear`` where its operands are views: rows apart, off their 16-byte addresses, turned, V and G
+at different strides. The leaves are what the views are taken of, so the layouts reach the backward; values and bounds
+are those of ``test_gpu_gated_linear``."""
 
 import pytest
 import torch
@@ -43,9 +43,9 @@ def _of_view(make, grad, shape):
     return grad.t() if make is _turned else grad[:, :shape[1]]
 
 
-LAYOUTS = [(_apart(8), _apart(16), _apart(16)), (_plain, _apart(16), _plain), (_plain, _apart(3), _plain), (_off, _plain, _plain),
-           (_plain, _off, _plain), (_plain, _plain, _off), (_apart(1), _off, _off), (_turned, _turned, _plain),
-           (_apart(8), _plain, _plain)]
+LAYOUTS = [(_apart(8), _apart(16), _apart(16)), (_plain, _apart(16), _plain), (_plain, _apart(3), _plain),
+           (_off, _plain, _plain), (_plain, _off, _plain), (_plain, _plain, _off), (_apart(1), _off, _off),
+           (_turned, _turned, _plain), (_apart(8), _plain, _plain)]
 
 
 @pytest.mark.parametrize("layout", range(len(LAYOUTS)))

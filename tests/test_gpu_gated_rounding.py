@@ -1,9 +1,9 @@
 """How often bfloat16 gradients of ``gated_linear`` are rounded, by their errors' lengths.
 
-Rounding numbers of all mantissas m to bfloat16 leaves an error of 2^-8 / sqrt(3) sqrt(E[1 / m^2]) of their length, E[1 / m^2]
-being 1/2 of uniform mantissas and 0.54 of logarithmic ones: r <= 1.75e-3 with 0.6. dv | dg are rounded once and a product
-of them once more, at random: sqrt(2) r. (Sums kept in 16 bits would add 1 or 2 of v's and g's own, sqrt(3) r at least.) Narrow
-maps have them in two planes: r. What is kept in 24 bits adds 2^-17, float32 sums (H + F) 2^-24.
+Rounding numbers of all mantissas m to bfloat16 leaves an error of 2^-8 / sqrt(3) sqrt(E[1 / m^2]) of their length, E[1
+/ m^2] being 1/2 of uniform mantissas and 0.54 of logarithmic ones: r <= 1.75e-3 with 0.6. dv | dg are rounded once and
+a product of them once more, at random: sqrt(2) r. (Sums kept in 16 bits would add 1 or 2 of v's and g's own, sqrt(3) r
+at least.) Narrow maps have them in two planes: r. What is kept in 24 bits adds 2^-17, float32 sums (H + F) 2^-24.
 
 The biases' gradients are sums of dv and dg before that, rounded once. They are F numbers, some 64, whose errors' length
 the few largest decide, by where in their unit they lie: so each is held to half a unit of itself, 2^-8, and to 2^-15 of
@@ -23,7 +23,8 @@ R = 2.0**-8 / math.sqrt(3) * math.sqrt(0.6)
 
 
 @pytest.mark.parametrize("act", ["sigmoid", "silu"])
-@pytest.mark.parametrize("N,H,F,roundings", [(300, 512, 700, 2), (30, 520, 1200, 2), (1030, 776, 4610, 2), (5000, 60, 64, 1)])
+@pytest.mark.parametrize("N,H,F,roundings", [(300, 512, 700, 2), (30, 520, 1200, 2), (1030, 776, 4610, 2),
+                                             (5000, 60, 64, 1)])
 def test_roundings(N, H, F, roundings, act):
     print(f"{N} {H} {F} {act}", flush=True)
     x, w, b, gw, gb, up = _inputs(N, H, F, torch.bfloat16, joint=False)

@@ -1,5 +1,5 @@
-"""``gated_scan`` of the convex form with infinite inputs, states and upstream gradients: a gate that is not shut keeps an
-infinity, however many steps' product of gates has left float32's range, and an infinity of the other sign makes NaN."""
+"""``gated_scan`` of the convex form with infinite inputs, states and upstream gradients: a gate that is not shut keeps
+an infinity, however many steps' product of gates has left float32's range; one of the other sign makes NaN."""
 
 import pytest
 import torch
@@ -9,8 +9,8 @@ import ews_mi355x as E
 pytestmark = pytest.mark.gpu
 
 INF = float("inf")
-SIZES = [(3, 2, 5), (2, 127, 33), (3, 200, 9), (2, 257, 16), (128, 40, 516), (12, 260, 516), (24, 260, 516), (1, 2100, 3),
-         (2, 4099, 40), (600, 17, 450)]
+SIZES = [(3, 2, 5), (2, 127, 33), (3, 200, 9), (2, 257, 16), (128, 40, 516), (12, 260, 516), (24, 260, 516),
+         (1, 2100, 3), (2, 4099, 40), (600, 17, 450)]
 
 
 def _steps(x, gate, state, dh):
