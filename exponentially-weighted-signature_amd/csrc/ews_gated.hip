@@ -145,23 +145,28 @@ struct Chain {
 template <class T>
 struct CopierChain {
   static constexpr int kCopies = T::kCopiesP;
-  const Chain& o;
   Copier<true, T::I, T::kThreads> rows;
-  __device__ __forceinline__ CopierChain(const Chain& c, int tile) : o(c), rows(c.v, tile) {}
-  __device__ __forceinline__ void aim(int64_t ld) {
-    rows.stride = (uint32_t)ld * 2;
+  const uint16_t* tail;
+  int64_t to_g;
+  int blocks, whole;
+  uint32_t ld, tail_ld;
+  __device__ __forceinline__ CopierChain(const Chain& o, int tile)
+      : rows(o.v, tile), tail(o.tail), to_g(o.to_g), blocks(o.blocks), whole(o.whole), ld((uint32_t)o.v.ld),
+        tail_ld((uint32_t)o.tail_ld) {}
+  __device__ __forceinline__ void aim(uint32_t to) {
+    rows.stride = to * 2;
     rows.aim_turned(63);
   }
   // Blocks are asked for in order.
   __device__ __forceinline__ const uint16_t* at(int piece, int kb) {
-    const bool second = kb >= o.blocks;
-    const int own = second ? kb - o.blocks : kb;
-    if (own == o.whole) {
-      aim(o.tail_ld);
-      return o.tail + (second ? 64 * o.tail_ld : 0);
+    const bool second = kb >= blocks;
+    const int own = second ? kb - blocks : kb;
+    if (own == whole) {
+      aim(tail_ld);
+      return tail + (second ? 64 * tail_ld : 0);
     }
-    if (second && own == 0 && o.tail) aim(o.v.ld);  // V's last block lay elsewhere
-    return o.v.p + piece * o.v.plane + own * 64 * o.v.ld + (second ? o.to_g : 0);
+    if (second && own == 0 && tail) aim(ld);  // V's last block lay elsewhere
+    return rows.base + piece * rows.plane + (int64_t)own * 64 * ld + (second ? to_g : 0);
   }
   __device__ __forceinline__ void copy(int c, const uint16_t* from, char* to) const { rows.copy(c, from, to); }
 };
@@ -666,7 +671,8 @@ struct DzArgs {
   uint16_t* dz;            // planes (padded, 2 ld), zero past F
   int64_t plane;
   float* sums;             // (workgroups along y, 2 ld) over the rows; or null
-  int each;                // rows of a workgroup
+  int each, parts;         // rows of a workgroup; workgroups along y, but for those that lay out
+  Packs tails;             // the last blocks of operands that are read as they are (bfloat16)
 };
 
 // A thread eight columns of every fourth of its workgroup's rows. SUMS: for the biases (the registers of which cost
@@ -674,6 +680,14 @@ struct DzArgs {
 template <typename T, bool SUMS>
 __global__ __launch_bounds__(256) void k_dz(DzArgs a) {
   constexpr int NP = kPlanes<T>;
+  if (NP == 1 && blockIdx.y >= a.parts) {
+    const uint32_t block = (blockIdx.y - a.parts) * gridDim.x + blockIdx.x;
+#pragma unroll
+    for (int k = 2; k >= 0; --k)
+      if (k < a.tails.count && block >= a.tails.from[k])
+        return pack_eight<T>(a.tails.each[k], (int64_t)(block - a.tails.from[k]) * 256 + threadIdx.x);
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int f = (blockIdx.x * 64 + lane) * 8;
   const int n = f >= a.F ? 0 : a.F - f < 8 ? a.F - f : 8;
@@ -1029,7 +1043,8 @@ int gated_plan(const ews_gated_desc* s, const void* x, const void* v, const void
     // 64 rows a workgroup (the biases' partial sums stay small), fewer where that leaves CUs without one
     p.dz_rows = 64;
     while (p.dz_rows > 4 && (int64_t)ceil_div(p.Np, p.dz_rows) * ceil_div(p.ld, 512) < 1024) p.dz_rows /= 2;
-    while (ceil_div(p.Np, p.dz_rows) > 65535) p.dz_rows *= 2;  // a grid's second side
+    // a grid's second side, on which up to 6144 workgroups lay out tails
+    while (ceil_div(p.Np, p.dz_rows) > 59000) p.dz_rows *= 2;
     p.dz_parts = ceil_div(p.Np, p.dz_rows);
     p.sums = take((size_t)p.dz_parts * 2 * p.ld * 4);
     // four workgroups a CU, of eight blocks at least
@@ -1059,6 +1074,7 @@ struct GCall {
   hipStream_t st;
   Chain x;
   Chain weights;
+  Packs tails;
 };
 
 // Rows of an operand from `first` on, as far as they go, laid out as dst_rows with zeros behind them.
@@ -1077,9 +1093,9 @@ tiles::PackArgs pack_args(const GPlan& p, const void* src, int64_t stride, int f
   return a;
 }
 
-// An operand, or V and G (g; else null), as the tiles read them. packed: copies of all rows, else tail: of the last,
-// incomplete block. to: where those go; want: whether the call reads them.
-Chain lay_out(Packs& a, const GPlan& p, const void* v, int64_t v_stride, const void* g, int64_t g_stride, int rows,
+// An operand, or V and G (g; else null), as the tiles read them. packed: copies of all rows (a), else tail: of the last,
+// incomplete block (tails). to: where those go; want: whether the call reads them.
+Chain lay_out(Packs& a, Packs& tails, const GPlan& p, const void* v, int64_t v_stride, const void* g, int64_t g_stride, int rows,
               bool packed, bool tail, char* to, bool want) {
   const int padded = ceil_div(rows, 64) * 64, sides = g ? 2 : 1;
   Chain c{};
@@ -1098,18 +1114,21 @@ Chain lay_out(Packs& a, const GPlan& p, const void* v, int64_t v_stride, const v
   }
   if (!want) return c;
   const int first = packed ? 0 : c.whole * 64, each = packed ? padded : 64;
-  a.add(pack_args(p, v, v_stride, first, rows, each, (uint16_t*)to, c.v.plane));
-  if (g) a.add(pack_args(p, g, g_stride, first, rows, each, (uint16_t*)to + each * p.Hp, c.v.plane));
+  Packs& list = packed ? a : tails;
+  list.add(pack_args(p, v, v_stride, first, rows, each, (uint16_t*)to, c.v.plane));
+  if (g) list.add(pack_args(p, g, g_stride, first, rows, each, (uint16_t*)to + each * p.Hp, c.v.plane));
   return c;
 }
 
-// The operands, packed where they cannot be read as they are. want_x, want_w: those that the call reads.
+// The operands, packed where they cannot be read as they are; tails are left to k_dz. want_x, want_w: those that the call
+// reads.
 int operands(GCall& c, const void* x, const void* v, const void* g, bool want_x, bool want_w) {
   const GPlan& p = c.p;
   const ews_gated_desc* s = c.s;
   Packs a{};
-  c.x = lay_out(a, p, x, s->x_stride, nullptr, 0, p.N, p.pack_x, p.tail_x, c.w + p.xp, want_x);
-  c.weights = lay_out(a, p, v, s->weight_stride, g, s->gate_stride, p.F, p.pack_w, p.tail_w, c.w + p.wp, want_w);
+  c.x = lay_out(a, c.tails, p, x, s->x_stride, nullptr, 0, p.N, p.pack_x, p.tail_x, c.w + p.xp, want_x);
+  c.weights = lay_out(a, c.tails, p, v, s->weight_stride, g, s->gate_stride, p.F, p.pack_w, p.tail_w, c.w + p.wp,
+                      want_w);
   if (!a.blocks) return EWS_OK;
   if (p.np == 3)
     hipLaunchKernelGGL((k_packs<float>), dim3(a.blocks), dim3(256), 0, c.st, a);
@@ -1409,7 +1428,10 @@ int ews_gated_backward(const ews_gated_desc* desc, const void* x, const void* we
   z.plane = p.Np * 2 * p.ld;
   z.sums = biases ? (float*)(c.w + p.sums) : nullptr;
   z.each = p.dz_rows;
-  const dim3 grid(ceil_div(p.ld, 512), p.dz_parts);
+  z.parts = p.dz_parts;
+  z.tails = c.tails;
+  const int wide = ceil_div(p.ld, 512);
+  const dim3 grid(wide, p.dz_parts + ceil_div(c.tails.blocks, wide));
   if (f32)
     z.sums ? launch_dz<float, true>(z, grid, c.st) : launch_dz<float, false>(z, grid, c.st);
   else

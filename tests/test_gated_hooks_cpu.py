@@ -106,13 +106,11 @@ def _apart(rows, cols, stride, dtype):
     return torch.randn(rows, stride).to(dtype)[:, :cols].requires_grad_()
 
 
-@pytest.mark.parametrize("off", [0, 2, 4])
 @pytest.mark.parametrize("joint", [False, True])
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_gated_backward_describes_what_came_back(calls, monkeypatch, dtype, joint, off):
+@pytest.mark.parametrize("dtype,off", [(torch.float32, 0), (torch.float32, 4), (torch.bfloat16, 0), (torch.bfloat16, 2),
+                                       (torch.bfloat16, 4)])
+def test_gated_backward_describes_what_came_back(calls, monkeypatch, dtype, off, joint):
     """Strides, V's and G's addresses, and scratch as large as the plan of these addresses asks for."""
-    if dtype is torch.float32 and off == 2:
-        pytest.skip("no address of float32 numbers")
     N, H, F, sizes = 100, 128, 96, []
     scratch = gated._scratch
 
