@@ -4,6 +4,7 @@ kernel (the "glu" and "gelu_glu" stages of ews/block.py:361-374, and their like)
 from __future__ import annotations
 
 import torch
+from torch._C._functorch import is_batchedtensor, is_legacy_batchedtensor
 from torch.nn.functional import linear
 
 from . import _native as nat
@@ -137,7 +138,8 @@ class _GatedLinear(torch.autograd.Function):
 
 
 class _GatedStage(_GatedLinear):
-    """``_GatedLinear`` with the activation "sigmoid" and a graph of its backward, in torch's operations."""
+    """``_GatedLinear`` with the activation "sigmoid" and, in torch's operations, a graph of its backward and a backward of
+    many upstream gradients at a time (``is_grads_batched``)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):
@@ -148,17 +150,19 @@ class _GatedStage(_GatedLinear):
 
     @staticmethod
     def backward(ctx, gout):
-        if not torch.is_grad_enabled():
+        graph = torch.is_grad_enabled()
+        if not (graph or is_legacy_batchedtensor(gout) or is_batchedtensor(gout)):
             return _GatedLinear.backward(ctx, gout)
         needs = ctx.needs_input_grad[:5]
-        x, weight, bias, gate_weight, gate_bias = leaves = [t if t is None else t.view_as(t)
-                                                            for t in ctx.saved_tensors[:5]]
-        if gate_weight is None:
-            v, g = linear(x, weight, bias).chunk(2, -1)
-        else:
-            v, g = linear(x, weight, bias), linear(x, gate_weight, gate_bias)
-        grads = iter(torch.autograd.grad(v * torch.sigmoid(g), [t for t, n in zip(leaves, needs) if n], gout,
-                                         create_graph=True))
+        with torch.enable_grad():
+            x, weight, bias, gate_weight, gate_bias = leaves = [t if t is None else t.view_as(t)
+                                                                for t in ctx.saved_tensors[:5]]
+            if gate_weight is None:
+                v, g = linear(x, weight, bias).chunk(2, -1)
+            else:
+                v, g = linear(x, weight, bias), linear(x, gate_weight, gate_bias)
+            y = v * torch.sigmoid(g)
+        grads = iter(torch.autograd.grad(y, [t for t, n in zip(leaves, needs) if n], gout, create_graph=graph))
         return (*(next(grads) if n else None for n in needs), None)
 
 

@@ -171,3 +171,17 @@ def test_a_stages_graph_of_its_backward(calls, joint, turned):
         for s, t in zip((*a, *a2), (*r, *r2)):
             assert torch.equal(s, t)
     assert [name for name, _ in calls] == ["ews_gated_forward"]
+
+
+def test_a_stages_backward_of_many_gradients_at_a_time(calls):
+    g = torch.Generator().manual_seed(2)
+    x, w, b = (torch.randn(*s, generator=g).requires_grad_() for s in ((9, 6), (10, 6), (10,)))
+    ups = torch.randn(4, 9, 5, generator=g)
+    y = gated._GatedStage.apply(x, w, b, None, None, "sigmoid")
+    v, s = torch.nn.functional.linear(x, w, b).chunk(2, -1)
+    z = v * torch.sigmoid(s)
+    for many in (lambda out: torch.autograd.grad(out, (x, w, b), ups, is_grads_batched=True, retain_graph=True),
+                 lambda out: torch.func.vmap(lambda u: torch.autograd.grad(out, (x, w, b), u, retain_graph=True))(ups)):
+        for a, r in zip(many(y), many(z)):
+            assert torch.equal(a, r) and not a.requires_grad
+    assert [name for name, _ in calls] == ["ews_gated_forward"]

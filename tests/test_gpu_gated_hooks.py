@@ -4,6 +4,7 @@ import contextlib
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import ews_mi355x as E
 
@@ -42,6 +43,30 @@ def test_scan_of_halves(B, L, D, dtype, kind):
         with _hooks(k):
             h, last = E.gated_scan(*joint.chunk(2, -1), state=state, mask=mask)
         grads.append(torch.autograd.grad((h, last), (joint, state), (up, torch.ones_like(last))))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_checkpoints(dtype, reentrant):
+    """Both operators formed again in the backward, between operations whose results are formed again too."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(2, 300, 72, generator=g, device="cuda").to(dtype).requires_grad_()
+    w, o = ((0.2 * torch.randn(n, 72, generator=g, device="cuda")).to(dtype).requires_grad_() for n in (144, 200))
+
+    def block(t):
+        h, last = E.gated_scan(*torch.nn.functional.linear(t, w).chunk(2, -1))
+        return E.gated_linear(h, o, activation="silu"), last
+
+    up = torch.randn(2, 300, 100, generator=g, device="cuda").to(dtype)
+    grads = []
+    for call in (block, lambda t: torch.utils.checkpoint.checkpoint(block, t, use_reentrant=reentrant)):
+        for p in (x, w, o):
+            p.grad = None
+        y, last = call(x)
+        torch.autograd.backward((y, last), (up, torch.ones_like(last)))
+        grads.append([p.grad for p in (x, w, o)])
     for a, b in zip(*grads):
         assert torch.equal(a, b)
 
