@@ -1093,10 +1093,10 @@ tiles::PackArgs pack_args(const GPlan& p, const void* src, int64_t stride, int f
   return a;
 }
 
-// An operand, or V and G (g; else null), as the tiles read them. packed: copies of all rows (a), else tail: of the last,
-// incomplete block (tails). to: where those go; want: whether the call reads them.
-Chain lay_out(Packs& a, Packs& tails, const GPlan& p, const void* v, int64_t v_stride, const void* g, int64_t g_stride, int rows,
-              bool packed, bool tail, char* to, bool want) {
+// An operand, or V and G (g; else null), as the tiles read them. packed: copies of all rows (a), else tail: of the
+// last, incomplete block (tails). to: where those go; want: whether the call reads them.
+Chain lay_out(Packs& a, Packs& tails, const GPlan& p, const void* v, int64_t v_stride, const void* g, int64_t g_stride,
+              int rows, bool packed, bool tail, char* to, bool want) {
   const int padded = ceil_div(rows, 64) * 64, sides = g ? 2 : 1;
   Chain c{};
   c.blocks = padded / 64;
@@ -1120,8 +1120,8 @@ Chain lay_out(Packs& a, Packs& tails, const GPlan& p, const void* v, int64_t v_s
   return c;
 }
 
-// The operands, packed where they cannot be read as they are; tails are left to k_dz. want_x, want_w: those that the call
-// reads.
+// The operands, packed where they cannot be read as they are; tails are left to k_dz. want_x, want_w: those that the
+// call reads.
 int operands(GCall& c, const void* x, const void* v, const void* g, bool want_x, bool want_w) {
   const GPlan& p = c.p;
   const ews_gated_desc* s = c.s;

@@ -138,8 +138,8 @@ class _GatedLinear(torch.autograd.Function):
 
 
 class _GatedStage(_GatedLinear):
-    """``_GatedLinear`` with the activation "sigmoid" and, in torch's operations, a graph of its backward and a backward of
-    many upstream gradients at a time (``is_grads_batched``)."""
+    """``_GatedLinear`` with the activation "sigmoid" and, in torch's operations, a graph of its backward and a backward
+    of many upstream gradients at a time (``is_grads_batched``)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, activation):

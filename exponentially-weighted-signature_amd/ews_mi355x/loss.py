@@ -17,10 +17,10 @@ def _ptr(t):
 class _Call:
     """One call's operands as the library takes them; ``targets``: the rows' tokens."""
 
-    ABI = "ews_loss"
+    ABI = "ews_loss_"
 
     def __init__(self, hidden, weight, bias, reduction, targets, ignore_index):
-        self.targets = (targets,)
+        self.targets, self.at = targets, (targets.data_ptr(),)
         self.desc = self.head = self._head(hidden, weight, bias, reduction, ignore_index)
 
     def _head(self, hidden, weight, bias, reduction, ignore_index):
@@ -32,19 +32,19 @@ class _Call:
         return nat.LossDesc(hs, wst, ignore_index, hidden.shape[0], H, V, DTYPES[weight.dtype],
                             nat.DTYPE_F32 if bias is None else DTYPES[bias.dtype], nat.LOSS_REDUCTIONS[reduction])
 
-    def fn(self, name):
-        return getattr(nat.load(), f"{self.ABI}_{name}")
-
     def call(self, name, *args):
-        nat.check(launch(self.dev, self.fn(name), *args), f"{self.ABI}_{name}")
+        name = self.ABI + name
+        nat.check(launch(self.dev, getattr(nat.load(), name), *args), name)
+
+    def keeps(self):
+        return getattr(nat.load(), self.ABI + "keeps")(self.desc)
 
     def workspace(self, train):
-        size = self.fn("workspace_bytes_for")(self.desc, self.weight.data_ptr(), train)
+        size = getattr(nat.load(), self.ABI + "workspace_bytes_for")(self.desc, self.weight.data_ptr(), train)
         return self.hidden.new_empty(size, dtype=torch.uint8)
 
     def inputs(self):
-        return (self.desc, self.hidden.data_ptr(), self.weight.data_ptr(), _ptr(self.bias),
-                *[t.data_ptr() for t in self.targets])
+        return self.desc, self.hidden.data_ptr(), self.weight.data_ptr(), _ptr(self.bias), *self.at
 
     def loss(self):
         return self.hidden.new_empty((self.head.rows,) if self.head.reduction == 0 else (), dtype=torch.float32)
@@ -81,12 +81,12 @@ class _Call:
 class _DistillCall(_Call):
     """``targets``: a teacher's tokens and logits of every row, and the temperature."""
 
-    ABI = "ews_distill"
+    ABI = "ews_distill_"
 
     def __init__(self, hidden, weight, bias, reduction, indices, logits, temperature):
         indices, index_stride = row_major(indices)
         logits, logit_stride = row_major(logits)
-        self.targets = indices, logits
+        self.targets, self.at = (indices, logits), (indices.data_ptr(), logits.data_ptr())
         self.head = self._head(hidden, weight, bias, reduction, 0)
         self.desc = nat.DistillDesc(self.head, index_stride, logit_stride, indices.shape[1], indices.element_size(),
                                     DTYPES[logits.dtype], temperature)
@@ -111,7 +111,7 @@ class _HeadLoss(torch.autograd.Function):
         if reduction != "none":
             loss, grads = call.train(needs[:3])
             first = call.head, grads
-        elif call.fn("keeps")(call.desc):
+        elif call.keeps():
             loss, *state = call.keep(needs[0])
             first = call, state
         else:
@@ -168,10 +168,10 @@ def _check_operands(hidden, weight, bias):
         check_tensor("bias", bias)
 
 
-def _check_places(weight, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != weight.device:
-            raise ValueError(f"{name} is on {t.device}, weight on {weight.device}")
+def _check_places(dev, names, tensors):
+    for name, t in zip(names, tensors):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, weight on {dev}")
 
 
 def _head_loss(kind, hidden, weight, bias, reduction, args, *targets):
@@ -270,7 +270,7 @@ def linear_cross_entropy(hidden, weight, targets, bias=None, ignore_index=-100, 
     _check_operands(hidden, weight, bias)
     if targets.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"targets must be int64 or int32, got {targets.dtype}")
-    _check_places(weight, hidden=hidden, targets=targets, bias=bias)
+    _check_places(weight.device, ("hidden", "targets", "bias"), (hidden, targets, bias))
     refuse_tangents((hidden, weight, bias))
     t = targets if targets.dim() == 1 else targets.reshape(-1)
     if t.dtype is not torch.int64 or not t.is_contiguous():
@@ -304,7 +304,7 @@ def linear_distillation(hidden, weight, indices, logits, bias=None, temperature=
     _check_teacher(shape, indices, logits, temperature)
     _check_operands(hidden, weight, bias)
     check_tensor("logits", logits)
-    _check_places(weight, hidden=hidden, indices=indices, logits=logits, bias=bias)
+    _check_places(weight.device, ("hidden", "indices", "logits", "bias"), (hidden, indices, logits, bias))
     refuse_tangents((hidden, weight, bias, logits))
     K = indices.shape[-1]
     return _head_loss(_DistillCall, hidden, weight, bias, reduction, (temperature,), indices.reshape(-1, K),
